@@ -512,6 +512,57 @@ race_status race_causal_bwd_profiled(const void* probsQ, const void* probsK, con
                                      void* workspace, size_t workspace_bytes, hipStream_t stream,
                                      hipEvent_t* events, int32_t max_events, int32_t* n_events);
 
+/* ---- Gated linear recurrence -------------------------------------------
+ * Per stream and channel, for t = 0 .. T-1 from a carried state h_{-1}:
+ *     h_t = a_t h_{t-1} + u_t,   out_t = h_t,
+ *     a = sigmoid(gate) or exp(gate),   u = x or (1 - a) x.
+ * The recurrent layer beside the per-bucket op in a mixed stack, with the same
+ * contract: streams of tokens, a state handed on (prefill, then a step per
+ * token), and a backward.  No counterpart in the reference. */
+typedef enum race_gate {
+    RACE_GATE_SIGMOID = 0, /* gate holds logits: a = 1 / (1 + exp(-gate)) */
+    RACE_GATE_LOG = 1      /* gate holds log a: a = exp(gate); -inf starts anew */
+} race_gate;
+
+/* x and gate are [num_streams][seq_len][channels] with the strides given (in
+ * elements; the channels of a token next to each other), 16-byte aligned; out,
+ * dout, dx and dgate are contiguous in that order; states are
+ * [num_streams][channels] fp32.  Rows of whole 4-channel pieces (channels and
+ * all strides multiples of 4) run vectorized.  Limits: 1 <= channels <= 65536,
+ * num_streams <= 65535. */
+typedef struct race_scan_shape {
+    int64_t num_streams, seq_len, channels;
+    int64_t x_stream_stride, x_token_stride;
+    int64_t gate_stream_stride, gate_token_stride;
+    int32_t dtype;      /* race_dtype of x, gate, out and their gradients */
+    int32_t gate_form;  /* race_gate */
+    int32_t complement; /* nonzero: u = (1 - a) x; zero: u = x */
+    int32_t lengths_group; /* streams that share one entry of `lengths`, >= 1 */
+} race_scan_shape;
+
+/* Workspace of race_gated_scan_fwd (and, with `backward`, of
+ * race_gated_scan_bwd) in bytes, and the floats of `records` (nullable). */
+race_status race_gated_scan_workspace_bytes(const race_scan_shape* shape, int32_t backward, size_t* bytes,
+                                            int64_t* record_floats);
+
+/* out, and with final_state (nullable) the state after the last token.
+ * state (nullable: zero) is the carried state; final_state may be the same
+ * array.  lengths (nullable): int32, one per lengths_group streams; tokens from
+ * lengths on are not read, their rows of out are zero and the state passes
+ * them unchanged (a value outside 0 .. seq_len counts as the nearer end).
+ * records (nullable): what race_gated_scan_bwd needs. */
+race_status race_gated_scan_fwd(const void* x, const void* gate, const float* state, const int32_t* lengths,
+                                void* out, float* final_state, float* records, const race_scan_shape* shape,
+                                void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Gradients for the upstream gradients dout and dfinal (nullable: zero) of out
+ * and final_state, from the forward's x, gate, lengths and records.  dx, dgate
+ * (zero in the rows from lengths on) and dstate may each be NULL to skip it. */
+race_status race_gated_scan_bwd(const void* x, const void* gate, const int32_t* lengths, const void* dout,
+                                const float* dfinal, const float* records, void* dx, void* dgate, float* dstate,
+                                const race_scan_shape* shape, void* workspace, size_t workspace_bytes,
+                                hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

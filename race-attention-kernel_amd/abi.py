@@ -26,6 +26,8 @@ RACE_KERNEL_SINGLE = 5
 RACE_KERNEL_MFMA_PRECISE = 6
 RACE_DECODE_TOKENS = 16
 RACE_SUB_CHUNK_TOKENS = 64
+RACE_GATE_SIGMOID = 0
+RACE_GATE_LOG = 1
 RACE_ALG1_FP32 = 0
 RACE_ALG1_BF16 = 1
 RACE_ALG1_SUB_CHUNK_TOKENS = 64
@@ -66,6 +68,9 @@ EXPORTED_SYMBOLS = (
     "race_alg1_fwd",
     "race_alg1_fwd_carry",
     "race_alg1_fwd_profiled",
+    "race_gated_scan_workspace_bytes",
+    "race_gated_scan_fwd",
+    "race_gated_scan_bwd",
 )
 
 
@@ -92,6 +97,22 @@ class RaceShape(ctypes.Structure):
 
 class RaceOptions(ctypes.Structure):
     _fields_ = [("tile_tokens", ctypes.c_int32), ("kernel", ctypes.c_int32)]
+
+
+class RaceScanShape(ctypes.Structure):
+    _fields_ = [
+        ("num_streams", ctypes.c_int64),
+        ("seq_len", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("x_stream_stride", ctypes.c_int64),
+        ("x_token_stride", ctypes.c_int64),
+        ("gate_stream_stride", ctypes.c_int64),
+        ("gate_token_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("gate_form", ctypes.c_int32),
+        ("complement", ctypes.c_int32),
+        ("lengths_group", ctypes.c_int32),
+    ]
 
 
 _configured = False
@@ -149,6 +170,10 @@ def lib() -> ctypes.CDLL:
         L.race_alg1_fwd_carry.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, a1, i32, i32, vp, sz, vp]
         L.race_alg1_fwd_profiled.argtypes = [vp, vp, vp, vp, vp, vp, vp, a1, i32, i32, vp, sz, vp,
                                              ctypes.POINTER(vp), i32, ctypes.POINTER(i32)]
+        sc = ctypes.POINTER(RaceScanShape)
+        L.race_gated_scan_workspace_bytes.argtypes = [sc, i32, ctypes.POINTER(sz), ctypes.POINTER(i64)]
+        L.race_gated_scan_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
+        L.race_gated_scan_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
         for name in EXPORTED_SYMBOLS[2:]:
             getattr(L, name).restype = i32
         _configured = True
@@ -407,3 +432,32 @@ def alg1_fwd_profiled(q, k, v, W, beta, out, final_state, sh: RaceAlg1Shape, til
                                       variant, workspace, workspace_bytes, stream, events, len(events),
                                       ctypes.byref(n))
     return st, n.value
+
+
+def scan_shape(N: int, T: int, D: int, dtype: int = RACE_F32, gate_form: int = RACE_GATE_SIGMOID,
+               complement: bool = True, lengths_group: int = 1) -> RaceScanShape:
+    """The shape of contiguous x and gates [N][T][D]."""
+    return RaceScanShape(N, T, D, T * D, D, T * D, D, dtype, gate_form, int(complement), lengths_group)
+
+
+def gated_scan_workspace_bytes(sh: RaceScanShape, backward: bool = False):
+    """(status, bytes, record_floats)."""
+    b, r = ctypes.c_size_t(0), ctypes.c_int64(0)
+    st = lib().race_gated_scan_workspace_bytes(ctypes.byref(sh), int(backward), ctypes.byref(b), ctypes.byref(r))
+    return st, b.value, r.value
+
+
+def gated_scan_fwd(x: int, gate: int, state: int | None, lengths: int | None, out: int, final_state: int | None,
+                   records: int | None, sh: RaceScanShape, workspace: int | None, workspace_bytes: int,
+                   stream: int) -> int:
+    """race_gated_scan_fwd on raw device addresses; returns the status."""
+    return lib().race_gated_scan_fwd(x, gate, state, lengths, out, final_state, records, ctypes.byref(sh), workspace,
+                                     workspace_bytes, stream)
+
+
+def gated_scan_bwd(x: int, gate: int, lengths: int | None, dout: int, dfinal: int | None, records: int,
+                   dx: int | None, dgate: int | None, dstate: int | None, sh: RaceScanShape, workspace: int | None,
+                   workspace_bytes: int, stream: int) -> int:
+    """race_gated_scan_bwd on raw device addresses; returns the status."""
+    return lib().race_gated_scan_bwd(x, gate, lengths, dout, dfinal, records, dx, dgate, dstate, ctypes.byref(sh),
+                                     workspace, workspace_bytes, stream)

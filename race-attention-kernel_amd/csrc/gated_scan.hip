@@ -1,0 +1,672 @@
+// gated_scan.hip -- the gated linear recurrence and its gradients:
+//
+//     h_t = a_t h_{t-1} + u_t        per stream and channel, t = 0 .. T-1
+//     a_t = sigmoid(g_t) or exp(g_t),  u_t = x_t or (1 - a_t) x_t
+//
+// from a carried state h_{-1} to the state after the last token, and with
+// lambda_t = dh_t + mu_{t+1}, mu_t = a_t lambda_t (mu_T the gradient of the
+// final state):
+//
+//     dx_t = lambda_t (or (1 - a_t) lambda_t),  dh_{-1} = mu_0,
+//     dlog a_t = mu_t (h_{t-1} - (0 or x_t)),   dg_t = dlog a_t (1 - a_t or 1).
+//
+// mu runs backward through the same recurrence as h runs forward (mu_t = a_t
+// mu_{t+1} + a_t dh_t), so both directions are one scan over pairs (P, H): a
+// run of tokens takes a state s to P s + H.
+//
+// Bound by memory: x, g in and h out once, about 20 vector instructions an
+// element.  A workgroup takes a block of channels (128 bytes of a row) of one
+// stream through all its tokens, a tile of kTile tokens at a time: a thread
+// has kRun consecutive tokens of V channels in registers (the next tile's rows
+// loaded meanwhile), the threads' pairs are scanned over a wave by lane
+// shuffles and over the waves through LDS, and every element is read once.  The
+// state a tile starts from stays in 32 bits; with a gradient to come it is kept
+// (one value per tile and channel), and the backward recomputes h from it
+// exactly instead of from the rounded output.
+// Few channels and many tokens are split over the tokens: one launch gives
+// every segment's pair, the next starts each segment from the pairs before it.
+// Sums have a fixed order: results are bitwise reproducible.
+#include <algorithm>
+
+#include "mfma_common.h"
+
+namespace race {
+namespace {
+
+// V consecutive channels of a row.
+template <typename TIn, int V>
+struct Piece {
+    using Raw = std::conditional_t<V == 1, TIn, std::conditional_t<sizeof(TIn) == 4, mfma::u32x4, mfma::u32x2>>;
+    Raw v;
+    __device__ __forceinline__ void load(const TIn* p) { v = *reinterpret_cast<const Raw*>(p); }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (V == 1)
+            return to_f32(v);
+        else if constexpr (sizeof(TIn) == 4)
+            return __uint_as_float(v[j]);
+        else
+            return (j & 1) ? mfma::hi_half(v[j >> 1]) : mfma::lo_half(v[j >> 1]);
+    }
+    __device__ __forceinline__ static void store(TIn* p, const float (&x)[V]) {
+        if constexpr (V == 1)
+            store_val(p, x[0]);
+        else if constexpr (sizeof(TIn) == 4)
+            *reinterpret_cast<Raw*>(p) = Raw{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                                             __float_as_uint(x[3])};
+        else
+            *reinterpret_cast<Raw*>(p) = Raw{mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3])};
+    }
+};
+
+template <int V>
+__device__ __forceinline__ void load_floats(float (&x)[V], const float* p) {
+    if constexpr (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(p);
+        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = p[j];
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_floats(float* p, const float (&x)[V]) {
+    if constexpr (V == 4)
+        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+#pragma unroll
+        for (int j = 0; j < V; ++j) p[j] = x[j];
+}
+
+// a and b = 1 - a of a gate value, each to its own last bits (b would lose
+// them as a difference where a is near 1).  With t = exp(-|g|), sigmoid(|g|) =
+// 1 / (1 + t) and sigmoid(-|g|) = t / (1 + t); t as 2^p with the rounding of
+// p = -|g| log2(e) put back to first order.
+template <int kForm>
+__device__ __forceinline__ void open_gate(float g, float& a, float& b) {
+    if constexpr (kForm == RACE_GATE_SIGMOID) {
+        constexpr float kLog2e = 1.44269504f, kLog2eLo = 1.92596299e-8f, kLn2 = 0.693147181f;
+        float x = -fabsf(g);
+        x = x < -150.f ? -150.f : x;  // 0 from here on; NaN stays NaN
+        const float p = x * kLog2e;
+        const float e = fmaf(x, kLog2eLo, fmaf(x, kLog2e, -p));
+        float t = __builtin_amdgcn_exp2f(p);
+        t = fmaf(t, e * kLn2, t);
+        const float r = __builtin_amdgcn_rcpf(1.f + t), tr = t * r;
+        a = g >= 0.f ? r : tr;
+        b = g >= 0.f ? tr : r;
+    } else {
+        a = expf(g);
+        b = -expm1f(g);  // only where it is used
+    }
+}
+
+struct ScanGeo {
+    int64_t T, D;
+    int64_t xn, xt, gn, gt;  // strides of x and the gates, in elements
+    const int32_t* lengths;  // nullable: live tokens of streams group n .. group n + group - 1
+    int64_t group;
+    int64_t seg_len;  // tokens per segment, whole tiles
+    int segs;
+    int64_t tiles;
+    __device__ __forceinline__ int64_t live(int64_t n) const {
+        if (!lengths) return T;
+        const int64_t len = lengths[n / group];
+        return len < 0 ? 0 : len < T ? len : T;
+    }
+};
+
+struct ScanFwdArgs {
+    const void *x, *gate;
+    const float* state_in;  // nullable: zero
+    void* out;
+    float* state_out;  // nullable
+    float* records;    // nullable: [N][tiles][D], the state each tile starts from
+    float* pairs;      // [N][segs][2][D] with more than one segment
+};
+
+struct ScanBwdArgs {
+    const void *x, *gate, *dout;
+    const float* records;
+    const float* dfinal;  // nullable: zero
+    void *dx, *dgate;     // nullable
+    float* dstate;        // nullable
+    float* pairs;
+};
+
+// One workgroup's shape: CL lanes across channels, the others across tokens.
+template <int NT, int CL, int R, int V>
+struct ScanTile {
+    static constexpr int kWaves = NT / 64, kTokenLanes = NT / CL, kTile = kTokenLanes * R, kChannels = CL * V;
+    static constexpr int kLdsFloats = 2 * 2 * kWaves * kChannels;  // two buffers of the waves' pairs
+    // The threads' pairs (P, H), in token order for kUp and against it
+    // otherwise, applied to `carry`: start = the state this thread's tokens begin
+    // with, carry = the state after all of them; with kProduct, `product` takes
+    // the product of every P too.  `lds` is one of the two buffers, in turn.
+    template <bool kUp, bool kProduct>
+    __device__ __forceinline__ static void join(float (&P)[V], float (&H)[V], float (&carry)[V], float (&start)[V],
+                                                float (&product)[V], float* lds) {
+        const int lane = threadIdx.x & 63, cl = lane % CL;
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int off = CL; off < 64; off *= 2) {
+            const bool has = kUp ? lane >= off : lane + off < 64;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float p = kUp ? __shfl_up(P[j], off) : __shfl_down(P[j], off);
+                const float h = kUp ? __shfl_up(H[j], off) : __shfl_down(H[j], off);
+                if (has) {
+                    H[j] = fmaf(P[j], h, H[j]);
+                    P[j] *= p;
+                }
+            }
+        }
+        float* lp = lds;                        // [waves][channels]
+        float* lh = lds + kWaves * kChannels;
+        if (kUp ? lane >= 64 - CL : lane < CL) {
+            store_floats<V>(lp + w * kChannels + cl * V, P);
+            store_floats<V>(lh + w * kChannels + cl * V, H);
+        }
+        // Of the lanes before this one alone.
+        float p0[V], h0[V];
+        const bool first = kUp ? lane < CL : lane >= 64 - CL;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float p = kUp ? __shfl_up(P[j], CL & 63) : __shfl_down(P[j], CL & 63);
+            const float h = kUp ? __shfl_up(H[j], CL & 63) : __shfl_down(H[j], CL & 63);
+            p0[j] = first ? 1.f : p;
+            h0[j] = first ? 0.f : h;
+        }
+        __syncthreads();
+        float mine[V];
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const int o = kUp ? i : kWaves - 1 - i;
+            float p[V], h[V];
+            load_floats<V>(p, lp + o * kChannels + cl * V);
+            load_floats<V>(h, lh + o * kChannels + cl * V);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (o == w) mine[j] = carry[j];
+                carry[j] = fmaf(p[j], carry[j], h[j]);
+                if constexpr (kProduct) product[j] *= p[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) start[j] = fmaf(p0[j], mine[j], h0[j]);
+    }
+};
+
+// The state a segment starts from: `carry` taken through the pairs of the
+// segments before it (kUp: 0 .. seg - 1; else segs - 1 .. seg + 1), each token
+// lane joining a run of them.
+template <typename S, int V, bool kUp>
+__device__ __forceinline__ void through_segments(float (&carry)[V], const float* pairs, int64_t n, int64_t D, int64_t c,
+                                                 int seg, int segs, int tl, float* lds) {
+    const int count = kUp ? seg : segs - 1 - seg, first = kUp ? 0 : seg + 1;
+    const int per = (count + S::kTokenLanes - 1) / S::kTokenLanes;
+    float P[V], H[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) P[j] = 1.f, H[j] = 0.f;
+    for (int i = 0; i < per; ++i) {
+        const int at = tl * per + (kUp ? i : per - 1 - i);
+        if (at >= count) continue;
+        const float* r = pairs + ((n * segs + first + at) * 2) * D + c;
+        float p[V], h[V];
+        load_floats<V>(p, r);
+        load_floats<V>(h, r + D);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            H[j] = fmaf(p[j], H[j], h[j]);
+            P[j] *= p[j];
+        }
+    }
+    float start[V], none[V];
+    S::template join<kUp, false>(P, H, carry, start, none, lds);
+}
+
+// One workgroup per (block of channels, stream, segment).  kPairs: only the
+// segment's pair, into a.pairs.
+template <typename TIn, int V, int CL, int NT, int R, int kForm, bool kComplement, bool kPairs>
+__global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const ScanFwdArgs a) {
+    using S = ScanTile<NT, CL, R, V>;
+    using X = Piece<TIn, V>;
+    __shared__ __align__(16) float lds[S::kLdsFloats];
+    const int cl = threadIdx.x % CL, tl = threadIdx.x / CL;
+    const int64_t n = blockIdx.y, D = g.D;
+    const int seg = blockIdx.z;
+    int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
+    const bool mine = c < D;
+    if (!mine) c = D - V;  // reads a column that is there, writes nothing
+    const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live(n));
+    const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn + c;
+    const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn + c;
+    TIn* op = static_cast<TIn*>(a.out) + n * g.T * D + c;
+    X xn[R], gn[R];
+    auto load = [&](int64_t r0) {
+        const int64_t t = r0 + tl * R;
+        if (r0 + S::kTile <= end) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                xn[r].load(xp + (t + r) * g.xt);
+                gn[r].load(gp + (t + r) * g.gt);
+            }
+        } else {  // the last row again past the end
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t u = min(t + r, end - 1);
+                xn[r].load(xp + u * g.xt);
+                gn[r].load(gp + u * g.gt);
+            }
+        }
+    };
+    if (t0 < end) load(t0);
+    float carry[V], product[V], start[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) carry[j] = 0.f, product[j] = 1.f;
+    int parity = 0;
+    if constexpr (!kPairs) {
+        if (a.state_in) load_floats<V>(carry, a.state_in + n * D + c);
+        if (seg > 0) {
+            through_segments<S, V, true>(carry, a.pairs, n, D, c, seg, g.segs, tl, lds);
+            parity = 1;
+        }
+    }
+    for (int64_t r0 = t0; r0 < t1; r0 += S::kTile) {
+        const int64_t t = r0 + tl * R;
+        if constexpr (!kPairs) {
+            if (a.records && mine && tl == 0) store_floats<V>(a.records + (n * g.tiles + r0 / S::kTile) * D + c, carry);
+        }
+        if (r0 >= end) {  // nothing live from here on
+            if constexpr (kPairs) break;
+            const float zero[V] = {};
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (mine && t + r < t1) X::store(op + (t + r) * D, zero);
+            continue;
+        }
+        float av[R][V], uv[R][V], P[V], H[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) P[j] = 1.f, H[j] = 0.f;
+        const bool whole = r0 + S::kTile <= end;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float b;
+                open_gate<kForm>(gn[r].get(j), av[r][j], b);
+                uv[r][j] = kComplement ? b * xn[r].get(j) : xn[r].get(j);
+            }
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    av[r][j] = t + r < end ? av[r][j] : 1.f;
+                    uv[r][j] = t + r < end ? uv[r][j] : 0.f;
+                }
+        }
+        if (r0 + S::kTile < end) load(r0 + S::kTile);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                H[j] = fmaf(av[r][j], H[j], uv[r][j]);
+                P[j] *= av[r][j];
+            }
+        S::template join<true, kPairs>(P, H, carry, start, product, lds + parity * (S::kLdsFloats / 2));
+        parity ^= 1;
+        if constexpr (!kPairs) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) start[j] = fmaf(av[r][j], start[j], uv[r][j]);
+                if (whole) {
+                    if (mine) X::store(op + (t + r) * D, start);
+                } else if (mine && t + r < t1) {
+                    float y[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) y[j] = t + r < end ? start[j] : 0.f;
+                    X::store(op + (t + r) * D, y);
+                }
+            }
+        }
+    }
+    if (!mine || tl != 0) return;
+    if constexpr (kPairs) {
+        float* r = a.pairs + ((n * g.segs + seg) * 2) * D + c;
+        store_floats<V>(r, product);
+        store_floats<V>(r + D, carry);
+    } else {
+        if (a.state_out && seg == g.segs - 1) store_floats<V>(a.state_out + n * D + c, carry);
+    }
+}
+
+// The gradients, tiles and segments from the last to the first.
+template <typename TIn, int V, int CL, int NT, int R, int kForm, bool kComplement, bool kPairs>
+__global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, const ScanBwdArgs a) {
+    using S = ScanTile<NT, CL, R, V>;
+    using X = Piece<TIn, V>;
+    __shared__ __align__(16) float lds[S::kLdsFloats];
+    const int cl = threadIdx.x % CL, tl = threadIdx.x / CL;
+    const int64_t n = blockIdx.y, D = g.D;
+    const int seg = blockIdx.z;
+    int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
+    const bool mine = c < D;
+    if (!mine) c = D - V;
+    const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live(n));
+    const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn + c;
+    const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn + c;
+    const TIn* yp = static_cast<const TIn*>(a.dout) + n * g.T * D + c;
+    const float* hp = kPairs ? nullptr : a.records + n * g.tiles * D + c;
+    TIn* dxp = a.dx ? static_cast<TIn*>(a.dx) + n * g.T * D + c : nullptr;
+    TIn* dgp = a.dgate ? static_cast<TIn*>(a.dgate) + n * g.T * D + c : nullptr;
+    X xn[R], gn[R], yn[R];
+    float hn[V];
+    auto load = [&](int64_t r0) {
+        const int64_t t = r0 + tl * R;
+        if constexpr (!kPairs) load_floats<V>(hn, hp + r0 / S::kTile * D);
+        if (r0 + S::kTile <= end) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if constexpr (!kPairs) xn[r].load(xp + (t + r) * g.xt);
+                gn[r].load(gp + (t + r) * g.gt);
+                yn[r].load(yp + (t + r) * D);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t u = min(t + r, end - 1);
+                if constexpr (!kPairs) xn[r].load(xp + u * g.xt);
+                gn[r].load(gp + u * g.gt);
+                yn[r].load(yp + u * D);
+            }
+        }
+    };
+    const int64_t last_tile = t0 + (t1 - 1 - t0) / S::kTile * S::kTile;       // of the segment
+    const int64_t last_live = t0 + (end - 1 - t0) / S::kTile * S::kTile;      // where end > t0
+    if (t0 < end) load(last_live);
+    float carry[V], product[V], start[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) carry[j] = 0.f, product[j] = 1.f;
+    int parity = 0;
+    if constexpr (!kPairs) {
+        if (a.dfinal) load_floats<V>(carry, a.dfinal + n * D + c);
+        if (seg < g.segs - 1) {
+            through_segments<S, V, false>(carry, a.pairs, n, D, c, seg, g.segs, tl, lds);
+            parity = 1;
+        }
+    }
+    for (int64_t r0 = last_tile; r0 >= t0; r0 -= S::kTile) {
+        const int64_t t = r0 + tl * R;
+        if (r0 >= end) {
+            if constexpr (kPairs) continue;
+            const float zero[V] = {};
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (mine && t + r < t1) {
+                    if (dxp) X::store(dxp + (t + r) * D, zero);
+                    if (dgp) X::store(dgp + (t + r) * D, zero);
+                }
+            continue;
+        }
+        const bool whole = r0 + S::kTile <= end;
+        float av[R][V], bv[R][V], ev[R][V], yv[R][V], P[V], H[V];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                open_gate<kForm>(gn[r].get(j), av[r][j], bv[r][j]);
+                yv[r][j] = yn[r].get(j);
+                if constexpr (!kPairs) ev[r][j] = xn[r].get(j);
+            }
+        if (!whole) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const bool live = t + r < end;
+                    av[r][j] = live ? av[r][j] : 1.f;
+                    bv[r][j] = live ? bv[r][j] : 0.f;
+                    yv[r][j] = live ? yv[r][j] : 0.f;
+                    if constexpr (!kPairs) ev[r][j] = live ? ev[r][j] : 0.f;
+                }
+        }
+        float h[V];
+        if constexpr (!kPairs) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) h[j] = hn[j];
+        }
+        if (r0 > t0) load(r0 - S::kTile);
+        if constexpr (!kPairs) {
+            // h before each token, from the tile's record; then ev = what lambda_t
+            // is multiplied with in the gate's gradient.
+#pragma unroll
+            for (int j = 0; j < V; ++j) P[j] = 1.f, H[j] = 0.f;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float u = kComplement ? bv[r][j] * ev[r][j] : ev[r][j];
+                    H[j] = fmaf(av[r][j], H[j], u);
+                    P[j] *= av[r][j];
+                }
+            float none[V];
+            S::template join<true, false>(P, H, h, start, none, lds + parity * (S::kLdsFloats / 2));
+            parity ^= 1;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float x = ev[r][j], before = start[j];
+                    start[j] = fmaf(av[r][j], before, kComplement ? bv[r][j] * x : x);
+                    const float dlog = av[r][j] * (kComplement ? before - x : before);
+                    ev[r][j] = kForm == RACE_GATE_SIGMOID ? bv[r][j] * dlog : dlog;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) P[j] = 1.f, H[j] = 0.f;
+#pragma unroll
+        for (int r = R - 1; r >= 0; --r)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                H[j] = av[r][j] * (H[j] + yv[r][j]);
+                P[j] *= av[r][j];
+            }
+        S::template join<false, kPairs>(P, H, carry, start, product, lds + parity * (S::kLdsFloats / 2));
+        parity ^= 1;
+        if constexpr (!kPairs) {
+#pragma unroll
+            for (int r = R - 1; r >= 0; --r) {
+                float dx[V], dg[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float lam = start[j] + yv[r][j];
+                    start[j] = av[r][j] * lam;
+                    dx[j] = kComplement ? bv[r][j] * lam : lam;
+                    dg[j] = ev[r][j] * lam;
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        dx[j] = t + r < end ? dx[j] : 0.f;
+                        dg[j] = t + r < end ? dg[j] : 0.f;
+                    }
+                }
+                if (mine && (whole || t + r < t1)) {
+                    if (dxp) X::store(dxp + (t + r) * D, dx);
+                    if (dgp) X::store(dgp + (t + r) * D, dg);
+                }
+            }
+        }
+    }
+    if (!mine || tl != 0) return;
+    if constexpr (kPairs) {
+        float* r = a.pairs + ((n * g.segs + seg) * 2) * D + c;
+        store_floats<V>(r, product);
+        store_floats<V>(r + D, carry);
+    } else {
+        if (a.dstate && seg == 0) store_floats<V>(a.dstate + n * D + c, carry);
+    }
+}
+
+// A few tokens (decode): V channels of a stream per thread, token by token.
+// state_out may be state_in.
+template <typename TIn, int V, int kForm, bool kComplement>
+__global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanGeo g, const ScanFwdArgs a, int64_t N) {
+    using X = Piece<TIn, V>;
+    const int64_t per = g.D / V, i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+    if (i >= N * per) return;
+    const int64_t n = i / per, c = (i - n * per) * V;
+    const int64_t end = g.live(n);
+    const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn + c;
+    const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn + c;
+    TIn* op = static_cast<TIn*>(a.out) + n * g.T * g.D + c;
+    float h[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) h[j] = 0.f;
+    if (a.state_in) load_floats<V>(h, a.state_in + n * g.D + c);
+    for (int64_t t = 0; t < end; ++t) {
+        X x, gate;
+        x.load(xp + t * g.xt);
+        gate.load(gp + t * g.gt);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float av, b;
+            open_gate<kForm>(gate.get(j), av, b);
+            h[j] = fmaf(av, h[j], kComplement ? b * x.get(j) : x.get(j));
+        }
+        X::store(op + t * g.D, h);
+    }
+    const float zero[V] = {};
+    for (int64_t t = end; t < g.T; ++t) X::store(op + t * g.D, zero);
+    if (a.state_out) store_floats<V>(a.state_out + n * g.D + c, h);
+}
+
+// Workgroup shapes: rows of whole four-value pieces, and any others.
+constexpr int kScanThreads = 512, kScanRun = 8, kScanLanes = 16, kScanLanes1 = 64;
+
+int scan_piece(const GatedScan& s) {
+    return s.D % 4 == 0 && s.xn % 4 == 0 && s.xt % 4 == 0 && s.gn % 4 == 0 && s.gt % 4 == 0 ? 4 : 1;
+}
+
+ScanGeo geometry(const GatedScan& s) {
+    ScanGeo g;
+    g.T = s.T;
+    g.D = s.D;
+    g.xn = s.xn, g.xt = s.xt, g.gn = s.gn, g.gt = s.gt;
+    g.lengths = s.lengths;
+    g.group = s.group;
+    g.tiles = scan_tiles(s);
+    const int64_t tile = scan_tile_tokens(s);
+    g.segs = int(scan_segments(s));
+    g.seg_len = (g.tiles + g.segs - 1) / g.segs * tile;
+    return g;
+}
+
+// f(form, complement) as compile-time values.
+template <typename F>
+hipError_t by_gate(const GatedScan& s, F f) {
+    using Sig = std::integral_constant<int, RACE_GATE_SIGMOID>;
+    using Log = std::integral_constant<int, RACE_GATE_LOG>;
+    if (s.form == RACE_GATE_SIGMOID) return s.complement ? f(Sig{}, std::true_type{}) : f(Sig{}, std::false_type{});
+    return s.complement ? f(Log{}, std::true_type{}) : f(Log{}, std::false_type{});
+}
+
+template <typename TIn, int V, int CL>
+hipError_t launch_forward_v(const GatedScan& s, const ScanFwdArgs& a, hipStream_t stream) {
+    using S = ScanTile<kScanThreads, CL, kScanRun, V>;
+    const ScanGeo g = geometry(s);
+    const dim3 grid(unsigned((s.D + S::kChannels - 1) / S::kChannels), unsigned(s.N), unsigned(g.segs));
+    return by_gate(s, [&](auto form, auto comp) {
+        if (g.segs > 1) {
+            scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, true>
+                <<<grid, kScanThreads, 0, stream>>>(g, a);
+            const hipError_t err = hipGetLastError();
+            if (err != hipSuccess) return err;
+        }
+        scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, false>
+            <<<grid, kScanThreads, 0, stream>>>(g, a);
+        return hipGetLastError();
+    });
+}
+
+template <typename TIn, int V, int CL>
+hipError_t launch_backward_v(const GatedScan& s, const ScanBwdArgs& a, hipStream_t stream) {
+    using S = ScanTile<kScanThreads, CL, kScanRun, V>;
+    const ScanGeo g = geometry(s);
+    const dim3 grid(unsigned((s.D + S::kChannels - 1) / S::kChannels), unsigned(s.N), unsigned(g.segs));
+    return by_gate(s, [&](auto form, auto comp) {
+        if (g.segs > 1) {
+            scan_backward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, true>
+                <<<grid, kScanThreads, 0, stream>>>(g, a);
+            const hipError_t err = hipGetLastError();
+            if (err != hipSuccess) return err;
+        }
+        scan_backward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, false>
+            <<<grid, kScanThreads, 0, stream>>>(g, a);
+        return hipGetLastError();
+    });
+}
+
+template <typename TIn, int V>
+hipError_t launch_step_v(const GatedScan& s, const ScanFwdArgs& a, hipStream_t stream) {
+    const ScanGeo g = geometry(s);
+    const int64_t threads = s.N * (s.D / V);
+    return by_gate(s, [&](auto form, auto comp) {
+        scan_step_kernel<TIn, V, form.value, comp.value>
+            <<<unsigned((threads + kThreads - 1) / kThreads), kThreads, 0, stream>>>(g, a, s.N);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace
+
+int64_t scan_tile_tokens(const GatedScan& s) {
+    return scan_piece(s) == 4 ? ScanTile<kScanThreads, kScanLanes, kScanRun, 4>::kTile
+                              : ScanTile<kScanThreads, kScanLanes1, kScanRun, 1>::kTile;
+}
+
+int64_t scan_tiles(const GatedScan& s) {
+    const int64_t tile = scan_tile_tokens(s);
+    return (s.T + tile - 1) / tile;
+}
+
+// Enough workgroups for two on every CU; whole tiles each.
+int64_t scan_segments(const GatedScan& s) {
+    constexpr int64_t kWorkgroups = 512, kEnough = 200;
+    const int64_t channels = scan_piece(s) == 4 ? kScanLanes * 4 : kScanLanes1;
+    const int64_t base = s.N * ((s.D + channels - 1) / channels), tiles = scan_tiles(s);
+    if (base >= kEnough || tiles <= 1) return 1;
+    const int64_t per = (tiles + kWorkgroups / base - 1) / (kWorkgroups / base);  // tiles of a segment
+    return (tiles + per - 1) / per;
+}
+
+hipError_t launch_gated_scan(const GatedScan& s, const void* x, const void* gate, const float* state_in, void* out,
+                             float* state_out, float* records, float* pairs, hipStream_t stream) {
+    const ScanFwdArgs a{x, gate, state_in, out, state_out, records, pairs};
+    const bool four = scan_piece(s) == 4;
+    if (!records && s.T <= kScanStepTokens) {
+        if (s.dtype == RACE_BF16)
+            return four ? launch_step_v<bf16_t, 4>(s, a, stream) : launch_step_v<bf16_t, 1>(s, a, stream);
+        return four ? launch_step_v<float, 4>(s, a, stream) : launch_step_v<float, 1>(s, a, stream);
+    }
+    if (s.dtype == RACE_BF16)
+        return four ? launch_forward_v<bf16_t, 4, kScanLanes>(s, a, stream)
+                    : launch_forward_v<bf16_t, 1, kScanLanes1>(s, a, stream);
+    return four ? launch_forward_v<float, 4, kScanLanes>(s, a, stream)
+                : launch_forward_v<float, 1, kScanLanes1>(s, a, stream);
+}
+
+hipError_t launch_gated_scan_bwd(const GatedScan& s, const void* x, const void* gate, const void* dout,
+                                 const float* records, const float* dfinal, void* dx, void* dgate, float* dstate,
+                                 float* pairs, hipStream_t stream) {
+    const ScanBwdArgs a{x, gate, dout, records, dfinal, dx, dgate, dstate, pairs};
+    const bool four = scan_piece(s) == 4;
+    if (s.dtype == RACE_BF16)
+        return four ? launch_backward_v<bf16_t, 4, kScanLanes>(s, a, stream)
+                    : launch_backward_v<bf16_t, 1, kScanLanes1>(s, a, stream);
+    return four ? launch_backward_v<float, 4, kScanLanes>(s, a, stream)
+                : launch_backward_v<float, 1, kScanLanes1>(s, a, stream);
+}
+
+}  // namespace race

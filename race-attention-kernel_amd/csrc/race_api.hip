@@ -1662,3 +1662,98 @@ race_status race_alg1_fwd_profiled(const void* q, const void* k, const void* v, 
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Gated linear recurrence (gated_scan.hip).
+
+namespace race {
+namespace {
+
+bool scan_shape(const race_scan_shape* sh, const int32_t* lengths, GatedScan* s) {
+    if (!sh || sh->num_streams < 0 || sh->num_streams > kMaxStreams) return false;
+    if (sh->seq_len < 0 || sh->seq_len > int64_t(INT_MAX) - kMaxAutoTile) return false;
+    if (sh->channels < 1 || sh->channels > 65536) return false;
+    if (sh->dtype != RACE_F32 && sh->dtype != RACE_BF16) return false;
+    if (sh->gate_form != RACE_GATE_SIGMOID && sh->gate_form != RACE_GATE_LOG) return false;
+    if (sh->lengths_group < 1) return false;
+    for (int64_t stride : {sh->x_stream_stride, sh->x_token_stride, sh->gate_stream_stride, sh->gate_token_stride})
+        if (stride < 0 || stride > (int64_t(1) << 46)) return false;
+    *s = GatedScan{sh->num_streams,        sh->seq_len,           sh->channels,
+                   sh->x_stream_stride,    sh->x_token_stride,    sh->gate_stream_stride,
+                   sh->gate_token_stride,  sh->dtype,             sh->gate_form,
+                   sh->complement != 0,    lengths,               sh->lengths_group};
+    return true;
+}
+
+int64_t scan_pair_floats(const GatedScan& s) {
+    const int64_t segs = scan_segments(s);
+    return segs > 1 ? round64(s.N * segs * 2 * s.D) : 0;
+}
+
+}  // namespace
+}  // namespace race
+
+extern "C" {
+
+race_status race_gated_scan_workspace_bytes(const race_scan_shape* shape, int32_t backward, size_t* bytes,
+                                            int64_t* record_floats_out) {
+    GatedScan s;
+    if (!scan_shape(shape, nullptr, &s) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    const bool empty = s.N == 0 || s.T == 0;
+    // The forward also has room for the state it started from, which later
+    // segments still read when the call is in place.
+    const int64_t pairs = empty ? 0 : scan_pair_floats(s);
+    *bytes = size_t(pairs + (pairs && !backward ? s.N * s.D : 0)) * sizeof(float);
+    if (record_floats_out) *record_floats_out = empty ? 0 : s.N * scan_tiles(s) * s.D;
+    return RACE_SUCCESS;
+}
+
+race_status race_gated_scan_fwd(const void* x, const void* gate, const float* state, const int32_t* lengths, void* out,
+                                float* final_state, float* records, const race_scan_shape* shape, void* workspace,
+                                size_t workspace_bytes, hipStream_t stream) {
+    GatedScan s;
+    if (!scan_shape(shape, lengths, &s)) return RACE_ERROR_INVALID_VALUE;
+    if (!aligned16(state) || !aligned16(final_state) || !aligned16(records)) return RACE_ERROR_INVALID_VALUE;
+    if (s.N == 0) return RACE_SUCCESS;
+    if (s.T == 0) {
+        if (!final_state || state == final_state) return RACE_SUCCESS;
+        if (!state) return zero_fill(final_state, s.N * s.D, stream);
+        return copy_floats(state, final_state, s.N * s.D, stream);
+    }
+    if (!x || !gate || !out || !aligned16(x) || !aligned16(gate) || !aligned16(out)) return RACE_ERROR_INVALID_VALUE;
+    size_t need = 0;
+    race_gated_scan_workspace_bytes(shape, 0, &need, nullptr);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return RACE_ERROR_INVALID_VALUE;
+    float* pairs = static_cast<float*>(workspace);
+    const bool step = !records && s.T <= kScanStepTokens;
+    if (state && state == final_state && !step && scan_segments(s) > 1) {
+        float* from = pairs + scan_pair_floats(s);
+        RACE_TRY(copy_floats(state, from, s.N * s.D, stream));
+        state = from;
+    }
+    return launch_gated_scan(s, x, gate, state, out, final_state, records, pairs, stream);
+}
+
+race_status race_gated_scan_bwd(const void* x, const void* gate, const int32_t* lengths, const void* dout,
+                                const float* dfinal, const float* records, void* dx, void* dgate, float* dstate,
+                                const race_scan_shape* shape, void* workspace, size_t workspace_bytes,
+                                hipStream_t stream) {
+    GatedScan s;
+    if (!scan_shape(shape, lengths, &s)) return RACE_ERROR_INVALID_VALUE;
+    if (!aligned16(dfinal) || !aligned16(dx) || !aligned16(dgate) || !aligned16(dstate)) return RACE_ERROR_INVALID_VALUE;
+    if (s.N == 0 || (!dx && !dgate && !dstate)) return RACE_SUCCESS;
+    if (s.T == 0) {
+        if (!dstate || dstate == dfinal) return RACE_SUCCESS;
+        if (!dfinal) return zero_fill(dstate, s.N * s.D, stream);
+        return copy_floats(dfinal, dstate, s.N * s.D, stream);
+    }
+    if (!x || !gate || !dout || !records || !aligned16(x) || !aligned16(gate) || !aligned16(dout) || !aligned16(records))
+        return RACE_ERROR_INVALID_VALUE;
+    size_t need = 0;
+    race_gated_scan_workspace_bytes(shape, 1, &need, nullptr);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return RACE_ERROR_INVALID_VALUE;
+    return launch_gated_scan_bwd(s, x, gate, dout, records, dfinal, dx, dgate, dstate, static_cast<float*>(workspace),
+                                 stream);
+}
+
+}  // extern "C"

@@ -406,6 +406,35 @@ hipError_t launch_hash_rows(const void* x, const float* planes_T, const void* dp
 hipError_t launch_pack_heads(const void* const* src, void* const* dst, int count, int64_t batch, int64_t T, int H,
                              int row_bytes, hipStream_t stream);
 
+// ---- gated linear recurrence (gated_scan.hip) ----
+// x and the gates [N][T][D] by strides (channels next to each other), out, dout,
+// dx and dgate contiguous, states [N][D] fp32.
+struct GatedScan {
+    int64_t N, T, D;
+    int64_t xn, xt, gn, gt;  // strides in elements
+    int dtype;               // race_dtype of x, gate, out and their gradients
+    int form;                // race_gate
+    bool complement;
+    const int32_t* lengths;  // nullable: live tokens, one per `group` streams
+    int64_t group;
+};
+// Calls without records of at most this many tokens run one thread per piece of
+// a row, token by token.
+constexpr int64_t kScanStepTokens = 16;
+int64_t scan_tile_tokens(const GatedScan& s);
+int64_t scan_tiles(const GatedScan& s);
+// Segments of whole tiles the tokens are split into; more than one take
+// `pairs`, [N][segments][2][D] floats.
+int64_t scan_segments(const GatedScan& s);
+// records (nullable): [N][tiles][D] floats, the state each tile starts from.
+// state_out may be state_in with one segment.
+hipError_t launch_gated_scan(const GatedScan& s, const void* x, const void* gate, const float* state_in, void* out,
+                             float* state_out, float* records, float* pairs, hipStream_t stream);
+// dfinal, dx, dgate and dstate may be null.
+hipError_t launch_gated_scan_bwd(const GatedScan& s, const void* x, const void* gate, const void* dout,
+                                 const float* records, const float* dfinal, void* dx, void* dgate, float* dstate,
+                                 float* pairs, hipStream_t stream);
+
 // ---- Algorithm 1 with the hashing inside (alg1.hip): bf16 q, k, v, out ----
 struct Alg1Args {
     const void* q;

@@ -852,6 +852,8 @@ bool alg1_fits_on_device(int64_t head_dim, int64_t num_planes, int64_t num_table
 
 }  // namespace
 
+#include "torch_operators.h"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
     m.doc() = "Per-bucket RACE attention on MI355X (gfx950): PyTorch binding of librace_mi355x";
@@ -930,5 +932,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("alg1_fits_on_device", &alg1_fits_on_device,
           "True when an Algorithm-1 output-pass workgroup fits this GPU's LDS", py::arg("head_dim"), py::arg("num_planes"),
           py::arg("num_tables"), py::arg("tensor_cores") = false);
+    bind_operators(m);
     m.def("abi_version", &race_abi_version, "ABI version of the loaded librace_mi355x");
 }

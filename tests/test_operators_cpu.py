@@ -1,0 +1,53 @@
+"""CPU tests of the operators beside the per-bucket op: what they refuse, before
+any device is touched, and the sizes they report."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+def test_scan_shapes_and_workspaces(race):
+    from race_attention_kernel_amd import abi
+
+    ok = abi.scan_shape(8, 4096, 2048)
+    st, nbytes, floats = abi.gated_scan_workspace_bytes(ok)
+    assert st == abi.RACE_SUCCESS and nbytes == 0 and floats == 8 * 16 * 2048  # 256-token tiles
+    # Few channels: the tokens are split, and the pairs of the segments need room.
+    st, nbytes, _ = abi.gated_scan_workspace_bytes(abi.scan_shape(8, 65536, 64))
+    assert st == abi.RACE_SUCCESS and nbytes > 0
+    st, back, _ = abi.gated_scan_workspace_bytes(abi.scan_shape(8, 65536, 64), backward=True)
+    assert st == abi.RACE_SUCCESS and 0 < back <= nbytes
+    st, nbytes, floats = abi.gated_scan_workspace_bytes(abi.scan_shape(0, 5, 64))
+    assert (st, nbytes, floats) == (abi.RACE_SUCCESS, 0, 0)
+    for bad in (abi.scan_shape(65536, 1, 4), abi.scan_shape(-1, 1, 4), abi.scan_shape(1, -1, 4),
+                abi.scan_shape(1, 2 ** 31 - 1, 4), abi.scan_shape(1, 1, 0), abi.scan_shape(1, 1, 65537),
+                abi.scan_shape(1, 1, 4, dtype=2), abi.scan_shape(1, 1, 4, gate_form=2),
+                abi.scan_shape(1, 1, 4, lengths_group=0)):
+        assert abi.gated_scan_workspace_bytes(bad)[0] == abi.RACE_ERROR_INVALID_VALUE
+
+
+def test_scan_refuses_bad_pointers_on_the_host(race):
+    from race_attention_kernel_amd import abi
+
+    sh = abi.scan_shape(2, 300, 64)
+    bad = abi.RACE_ERROR_INVALID_VALUE
+    assert abi.gated_scan_fwd(0, 16, None, None, 16, None, None, sh, None, 0, 0) == bad
+    assert abi.gated_scan_fwd(8, 16, None, None, 16, None, None, sh, None, 0, 0) == bad
+    assert abi.gated_scan_fwd(16, 16, 4, None, 16, None, None, sh, None, 0, 0) == bad
+    assert abi.gated_scan_bwd(16, 16, None, 16, None, None, 16, None, None, sh, None, 0, 0) == bad
+    assert abi.gated_scan_bwd(16, 16, None, 8, None, 16, 16, None, None, sh, None, 0, 0) == bad
+    split = abi.scan_shape(8, 65536, 64)  # needs a workspace
+    assert abi.gated_scan_fwd(16, 16, None, None, 16, None, None, split, None, 0, 0) == bad
+    # Nothing to do touches no device.
+    assert abi.gated_scan_fwd(0, 0, None, None, 0, None, None, abi.scan_shape(0, 5, 64), None, 0, 0) == 0
+    assert abi.gated_scan_bwd(0, 0, None, 0, None, 0, None, None, None, sh, None, 0, 0) == 0
+
+
+def test_scan_binding_validates_inputs_on_the_host(race):
+    x = torch.randn(2, 5, 8)
+    with pytest.raises(RuntimeError, match="race_gated_scan: x lives on the CPU"):
+        race.race_gated_scan(x, x)
+    with pytest.raises(RuntimeError, match="x lives on the CPU"):
+        race.race_gated_scan_carry(x, x, torch.zeros(2, 8))
+    with pytest.raises(ValueError, match="gate_form"):
+        race.race_gated_scan(x, x, gate_form="tanh")
