@@ -529,7 +529,8 @@ typedef enum race_gate {
  * dout, dx and dgate are contiguous in that order; states are
  * [num_streams][channels] fp32.  Rows of whole 4-channel pieces (channels and
  * all strides multiples of 4) run vectorized.  Limits: 1 <= channels <= 65536,
- * num_streams <= 65535. */
+ * num_streams <= 65535, token strides up to RACE_SCAN_MAX_TOKEN_STRIDE. */
+#define RACE_SCAN_MAX_TOKEN_STRIDE (1 << 20)
 typedef struct race_scan_shape {
     int64_t num_streams, seq_len, channels;
     int64_t x_stream_stride, x_token_stride;

@@ -33,12 +33,22 @@
 namespace race {
 namespace {
 
-// V consecutive channels of a row.
+// V consecutive channels of a row, at a byte offset of a buffer.
 template <typename TIn, int V>
 struct Piece {
+    static constexpr int kBytes = V * int(sizeof(TIn));
     using Raw = std::conditional_t<V == 1, TIn, std::conditional_t<sizeof(TIn) == 4, mfma::u32x4, mfma::u32x2>>;
     Raw v;
-    __device__ __forceinline__ void load(const TIn* p) { v = *reinterpret_cast<const Raw*>(p); }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int off) {
+        if constexpr (kBytes == 16)
+            v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, mfma::kPolicyDefault);
+        else if constexpr (kBytes == 8)
+            v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, mfma::kPolicyDefault);
+        else if constexpr (kBytes == 4)
+            v = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, mfma::kPolicyDefault));
+        else
+            v = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, mfma::kPolicyDefault);
+    }
     __device__ __forceinline__ float get(int j) const {
         if constexpr (V == 1)
             return to_f32(v);
@@ -47,16 +57,37 @@ struct Piece {
         else
             return (j & 1) ? mfma::hi_half(v[j >> 1]) : mfma::lo_half(v[j >> 1]);
     }
-    __device__ __forceinline__ static void store(TIn* p, const float (&x)[V]) {
+    __device__ __forceinline__ static void store(__amdgpu_buffer_rsrc_t r, int off, const float (&x)[V]) {
+        if constexpr (kBytes == 16)
+            __builtin_amdgcn_raw_buffer_store_b128(mfma::u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]),
+                                                               __float_as_uint(x[2]), __float_as_uint(x[3])},
+                                                   r, off, 0, mfma::kPolicyDefault);
+        else if constexpr (kBytes == 8)
+            __builtin_amdgcn_raw_buffer_store_b64(mfma::u32x2{mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3])}, r, off,
+                                                  0, mfma::kPolicyDefault);
+        else if constexpr (kBytes == 4)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[0]), r, off, 0, mfma::kPolicyDefault);
+        else
+            __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x[0]), r, off, 0, mfma::kPolicyDefault);
+    }
+    __device__ __forceinline__ static void put(TIn* p, const float (&x)[V]) {
         if constexpr (V == 1)
             store_val(p, x[0]);
         else if constexpr (sizeof(TIn) == 4)
-            *reinterpret_cast<Raw*>(p) = Raw{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
-                                             __float_as_uint(x[3])};
+            *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
         else
-            *reinterpret_cast<Raw*>(p) = Raw{mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3])};
+            *reinterpret_cast<uint2*>(p) = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
     }
 };
+
+// The rows from `r0` on (at most kTile of them, before `end`) of an array with
+// rows of D values `stride` apart: loads past them give zero, stores past them
+// are dropped.
+template <int kTile, typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_view(T* base, int64_t r0, int64_t end, int64_t stride, int64_t D) {
+    const int64_t rows = min<int64_t>(end - r0, kTile);
+    return mfma::make_rsrc(base + r0 * stride, rows > 0 ? ((rows - 1) * stride + D) * int64_t(sizeof(T)) : 0);
+}
 
 template <int V>
 __device__ __forceinline__ void load_floats(float (&x)[V], const float* p) {
@@ -107,7 +138,7 @@ struct ScanGeo {
     int64_t group;
     int64_t seg_len;  // tokens per segment, whole tiles
     int segs;
-    int64_t tiles;
+    int64_t tiles;    // records of a stream
     __device__ __forceinline__ int64_t live(int64_t n) const {
         if (!lengths) return T;
         const int64_t len = lengths[n / group];
@@ -120,7 +151,7 @@ struct ScanFwdArgs {
     const float* state_in;  // nullable: zero
     void* out;
     float* state_out;  // nullable
-    float* records;    // nullable: [N][tiles][D], the state each tile starts from
+    float* records;    // nullable: [N][tiles][D], the state each backward tile starts from
     float* pairs;      // [N][segs][2][D] with more than one segment
 };
 
@@ -178,7 +209,8 @@ struct ScanTile {
         }
         __syncthreads();
         float mine[V];
-#pragma unroll
+        // Two waves' pairs in flight (all eight took 64 registers).
+#pragma unroll 2
         for (int i = 0; i < kWaves; ++i) {
             const int o = kUp ? i : kWaves - 1 - i;
             float p[V], h[V];
@@ -209,7 +241,7 @@ __device__ __forceinline__ void through_segments(float (&carry)[V], const float*
     for (int j = 0; j < V; ++j) P[j] = 1.f, H[j] = 0.f;
     for (int i = 0; i < per; ++i) {
         const int at = tl * per + (kUp ? i : per - 1 - i);
-        if (at >= count) continue;
+        if (at >= count || c >= D) continue;
         const float* r = pairs + ((n * segs + first + at) * 2) * D + c;
         float p[V], h[V];
         load_floats<V>(p, r);
@@ -226,7 +258,7 @@ __device__ __forceinline__ void through_segments(float (&carry)[V], const float*
 
 // One workgroup per (block of channels, stream, segment).  kPairs: only the
 // segment's pair, into a.pairs.
-template <typename TIn, int V, int CL, int NT, int R, int kForm, bool kComplement, bool kPairs>
+template <typename TIn, int V, int CL, int NT, int R, int RB, int kForm, bool kComplement, bool kPairs>
 __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const ScanFwdArgs a) {
     using S = ScanTile<NT, CL, R, V>;
     using X = Piece<TIn, V>;
@@ -234,29 +266,27 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
     const int cl = threadIdx.x % CL, tl = threadIdx.x / CL;
     const int64_t n = blockIdx.y, D = g.D;
     const int seg = blockIdx.z;
-    int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
+    const int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
     const bool mine = c < D;
-    if (!mine) c = D - V;  // reads a column that is there, writes nothing
     const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live(n));
-    const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn + c;
-    const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn + c;
-    TIn* op = static_cast<TIn*>(a.out) + n * g.T * D + c;
+    const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn;
+    const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn;
+    TIn* op = static_cast<TIn*>(a.out) + n * g.T * D;
+    // Byte offsets of this thread's first row in a tile; a thread past the
+    // channels reads zeros and writes nothing.
+    constexpr int es = int(sizeof(TIn));
+    const int xs = int(g.xt) * es, gs = int(g.gt) * es, os = int(D) * es;
+    const int xo = mine ? tl * R * xs + int(c) * es : mfma::kOutside;
+    const int go = mine ? tl * R * gs + int(c) * es : mfma::kOutside;
+    const int oo = mine ? tl * R * os + int(c) * es : mfma::kOutside;
     X xn[R], gn[R];
     auto load = [&](int64_t r0) {
-        const int64_t t = r0 + tl * R;
-        if (r0 + S::kTile <= end) {
+        const auto xr = rows_view<S::kTile>(xp, r0, end, g.xt, D);
+        const auto gr = rows_view<S::kTile>(gp, r0, end, g.gt, D);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                xn[r].load(xp + (t + r) * g.xt);
-                gn[r].load(gp + (t + r) * g.gt);
-            }
-        } else {  // the last row again past the end
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t u = min(t + r, end - 1);
-                xn[r].load(xp + u * g.xt);
-                gn[r].load(gp + u * g.gt);
-            }
+        for (int r = 0; r < R; ++r) {
+            xn[r].load(xr, xo + r * xs);
+            gn[r].load(gr, go + r * gs);
         }
     };
     if (t0 < end) load(t0);
@@ -265,7 +295,7 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
     for (int j = 0; j < V; ++j) carry[j] = 0.f, product[j] = 1.f;
     int parity = 0;
     if constexpr (!kPairs) {
-        if (a.state_in) load_floats<V>(carry, a.state_in + n * D + c);
+        if (a.state_in && mine) load_floats<V>(carry, a.state_in + n * D + c);
         if (seg > 0) {
             through_segments<S, V, true>(carry, a.pairs, n, D, c, seg, g.segs, tl, lds);
             parity = 1;
@@ -273,15 +303,12 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
     }
     for (int64_t r0 = t0; r0 < t1; r0 += S::kTile) {
         const int64_t t = r0 + tl * R;
-        if constexpr (!kPairs) {
-            if (a.records && mine && tl == 0) store_floats<V>(a.records + (n * g.tiles + r0 / S::kTile) * D + c, carry);
-        }
         if (r0 >= end) {  // nothing live from here on
             if constexpr (kPairs) break;
             const float zero[V] = {};
+            const auto orr = rows_view<S::kTile>(op, r0, t1, D, D);
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (mine && t + r < t1) X::store(op + (t + r) * D, zero);
+            for (int r = 0; r < R; ++r) X::store(orr, oo + r * os, zero);
             continue;
         }
         float av[R][V], uv[R][V], P[V], H[V];
@@ -316,18 +343,20 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
         S::template join<true, kPairs>(P, H, carry, start, product, lds + parity * (S::kLdsFloats / 2));
         parity ^= 1;
         if constexpr (!kPairs) {
+            constexpr int kRecord = ScanTile<NT, CL, RB, V>::kTile;
+            static_assert(kRecord % R == 0 && S::kTile % kRecord == 0, "a thread's tokens start a record or do not");
+            if (a.records && mine && tl * R % kRecord == 0 && t < end)
+                store_floats<V>(a.records + (n * g.tiles + t / kRecord) * D + c, start);
+            const auto orr = rows_view<S::kTile>(op, r0, t1, D, D);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
+                float y[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) start[j] = fmaf(av[r][j], start[j], uv[r][j]);
-                if (whole) {
-                    if (mine) X::store(op + (t + r) * D, start);
-                } else if (mine && t + r < t1) {
-                    float y[V];
-#pragma unroll
-                    for (int j = 0; j < V; ++j) y[j] = t + r < end ? start[j] : 0.f;
-                    X::store(op + (t + r) * D, y);
+                for (int j = 0; j < V; ++j) {
+                    start[j] = fmaf(av[r][j], start[j], uv[r][j]);
+                    y[j] = whole || t + r < end ? start[j] : 0.f;
                 }
+                X::store(orr, oo + r * os, y);
             }
         }
     }
@@ -350,38 +379,38 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
     const int cl = threadIdx.x % CL, tl = threadIdx.x / CL;
     const int64_t n = blockIdx.y, D = g.D;
     const int seg = blockIdx.z;
-    int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
+    const int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
     const bool mine = c < D;
-    if (!mine) c = D - V;
     const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live(n));
-    const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn + c;
-    const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn + c;
-    const TIn* yp = static_cast<const TIn*>(a.dout) + n * g.T * D + c;
+    const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn;
+    const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn;
+    const TIn* yp = static_cast<const TIn*>(a.dout) + n * g.T * D;
     const float* hp = kPairs ? nullptr : a.records + n * g.tiles * D + c;
-    TIn* dxp = a.dx ? static_cast<TIn*>(a.dx) + n * g.T * D + c : nullptr;
-    TIn* dgp = a.dgate ? static_cast<TIn*>(a.dgate) + n * g.T * D + c : nullptr;
+    TIn* dxp = a.dx ? static_cast<TIn*>(a.dx) + n * g.T * D : nullptr;
+    TIn* dgp = a.dgate ? static_cast<TIn*>(a.dgate) + n * g.T * D : nullptr;
+    constexpr int es = int(sizeof(TIn));
+    const int xs = int(g.xt) * es, gs = int(g.gt) * es, os = int(D) * es;
+    const int xo = mine ? tl * R * xs + int(c) * es : mfma::kOutside;
+    const int go = mine ? tl * R * gs + int(c) * es : mfma::kOutside;
+    const int oo = mine ? tl * R * os + int(c) * es : mfma::kOutside;
     X xn[R], gn[R], yn[R];
-    float hn[V];
+    float hn[V] = {};
     auto load = [&](int64_t r0) {
-        const int64_t t = r0 + tl * R;
-        if constexpr (!kPairs) load_floats<V>(hn, hp + r0 / S::kTile * D);
-        if (r0 + S::kTile <= end) {
+        if constexpr (!kPairs) {
+            if (mine) load_floats<V>(hn, hp + r0 / S::kTile * D);
+        }
+        const auto xr = rows_view<S::kTile>(xp, r0, end, g.xt, D);
+        const auto gr = rows_view<S::kTile>(gp, r0, end, g.gt, D);
+        const auto yr = rows_view<S::kTile>(yp, r0, end, D, D);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if constexpr (!kPairs) xn[r].load(xp + (t + r) * g.xt);
-                gn[r].load(gp + (t + r) * g.gt);
-                yn[r].load(yp + (t + r) * D);
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t u = min(t + r, end - 1);
-                if constexpr (!kPairs) xn[r].load(xp + u * g.xt);
-                gn[r].load(gp + u * g.gt);
-                yn[r].load(yp + u * D);
-            }
+        for (int r = 0; r < R; ++r) {
+            if constexpr (!kPairs) xn[r].load(xr, xo + r * xs);
+            gn[r].load(gr, go + r * gs);
+            yn[r].load(yr, oo + r * os);
         }
     };
+    // A gradient that is not asked for: a view of no rows.
+    auto out_view = [&](TIn* p, int64_t r0) { return rows_view<S::kTile>(p, p ? r0 : 0, p ? t1 : 0, D, D); };
     const int64_t last_tile = t0 + (t1 - 1 - t0) / S::kTile * S::kTile;       // of the segment
     const int64_t last_live = t0 + (end - 1 - t0) / S::kTile * S::kTile;      // where end > t0
     if (t0 < end) load(last_live);
@@ -390,7 +419,7 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
     for (int j = 0; j < V; ++j) carry[j] = 0.f, product[j] = 1.f;
     int parity = 0;
     if constexpr (!kPairs) {
-        if (a.dfinal) load_floats<V>(carry, a.dfinal + n * D + c);
+        if (a.dfinal && mine) load_floats<V>(carry, a.dfinal + n * D + c);
         if (seg < g.segs - 1) {
             through_segments<S, V, false>(carry, a.pairs, n, D, c, seg, g.segs, tl, lds);
             parity = 1;
@@ -401,12 +430,12 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
         if (r0 >= end) {
             if constexpr (kPairs) continue;
             const float zero[V] = {};
+            const auto dxr = out_view(dxp, r0), dgr = out_view(dgp, r0);
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (mine && t + r < t1) {
-                    if (dxp) X::store(dxp + (t + r) * D, zero);
-                    if (dgp) X::store(dgp + (t + r) * D, zero);
-                }
+            for (int r = 0; r < R; ++r) {
+                X::store(dxr, oo + r * os, zero);
+                X::store(dgr, oo + r * os, zero);
+            }
             continue;
         }
         const bool whole = r0 + S::kTile <= end;
@@ -475,6 +504,7 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
         S::template join<false, kPairs>(P, H, carry, start, product, lds + parity * (S::kLdsFloats / 2));
         parity ^= 1;
         if constexpr (!kPairs) {
+            const auto dxr = out_view(dxp, r0), dgr = out_view(dgp, r0);
 #pragma unroll
             for (int r = R - 1; r >= 0; --r) {
                 float dx[V], dg[V];
@@ -492,10 +522,8 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
                         dg[j] = t + r < end ? dg[j] : 0.f;
                     }
                 }
-                if (mine && (whole || t + r < t1)) {
-                    if (dxp) X::store(dxp + (t + r) * D, dx);
-                    if (dgp) X::store(dgp + (t + r) * D, dg);
-                }
+                X::store(dxr, oo + r * os, dx);
+                X::store(dgr, oo + r * os, dg);
             }
         }
     }
@@ -527,27 +555,37 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanGeo g, co
     if (a.state_in) load_floats<V>(h, a.state_in + n * g.D + c);
     for (int64_t t = 0; t < end; ++t) {
         X x, gate;
-        x.load(xp + t * g.xt);
-        gate.load(gp + t * g.gt);
+        x.v = *reinterpret_cast<const typename X::Raw*>(xp + t * g.xt);
+        gate.v = *reinterpret_cast<const typename X::Raw*>(gp + t * g.gt);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float av, b;
             open_gate<kForm>(gate.get(j), av, b);
             h[j] = fmaf(av, h[j], kComplement ? b * x.get(j) : x.get(j));
         }
-        X::store(op + t * g.D, h);
+        X::put(op + t * g.D, h);
     }
     const float zero[V] = {};
-    for (int64_t t = end; t < g.T; ++t) X::store(op + t * g.D, zero);
+    for (int64_t t = end; t < g.T; ++t) X::put(op + t * g.D, zero);
     if (a.state_out) store_floats<V>(a.state_out + n * g.D + c, h);
 }
 
 // Workgroup shapes: rows of whole four-value pieces, and any others.
-constexpr int kScanThreads = 512, kScanRun = 8, kScanLanes = 16, kScanLanes1 = 64;
+constexpr int kScanThreads = 512, kScanLanes = 16, kScanLanes1 = 64;
+// Tokens per thread, forward and backward.  The backward holds four values an
+// element: with 8 tokens of 4 channels it spilled 640 bytes a lane (8 x 4096
+// tokens of 2048 bf16 channels: 746 us).
+constexpr int kScanRun = 8, kScanRunBwd = 4, kScanRunBwd1 = 8;
+template <int V>
+using FwdTile = ScanTile<kScanThreads, V == 4 ? kScanLanes : kScanLanes1, kScanRun, V>;
+template <int V>
+using BwdTile = ScanTile<kScanThreads, V == 4 ? kScanLanes : kScanLanes1, V == 4 ? kScanRunBwd : kScanRunBwd1, V>;
 
 int scan_piece(const GatedScan& s) {
     return s.D % 4 == 0 && s.xn % 4 == 0 && s.xt % 4 == 0 && s.gn % 4 == 0 && s.gt % 4 == 0 ? 4 : 1;
 }
+
+int64_t forward_tile(const GatedScan& s) { return scan_piece(s) == 4 ? FwdTile<4>::kTile : FwdTile<1>::kTile; }
 
 ScanGeo geometry(const GatedScan& s) {
     ScanGeo g;
@@ -557,9 +595,9 @@ ScanGeo geometry(const GatedScan& s) {
     g.lengths = s.lengths;
     g.group = s.group;
     g.tiles = scan_tiles(s);
-    const int64_t tile = scan_tile_tokens(s);
     g.segs = int(scan_segments(s));
-    g.seg_len = (g.tiles + g.segs - 1) / g.segs * tile;
+    const int64_t tile = forward_tile(s);
+    g.seg_len = ((s.T + tile - 1) / tile + g.segs - 1) / g.segs * tile;
     return g;
 }
 
@@ -572,37 +610,39 @@ hipError_t by_gate(const GatedScan& s, F f) {
     return s.complement ? f(Log{}, std::true_type{}) : f(Log{}, std::false_type{});
 }
 
-template <typename TIn, int V, int CL>
+template <typename TIn, int V>
 hipError_t launch_forward_v(const GatedScan& s, const ScanFwdArgs& a, hipStream_t stream) {
-    using S = ScanTile<kScanThreads, CL, kScanRun, V>;
+    using S = FwdTile<V>;
+    constexpr int CL = S::kChannels / V, RB = BwdTile<V>::kTile / BwdTile<V>::kTokenLanes;
     const ScanGeo g = geometry(s);
     const dim3 grid(unsigned((s.D + S::kChannels - 1) / S::kChannels), unsigned(s.N), unsigned(g.segs));
     return by_gate(s, [&](auto form, auto comp) {
         if (g.segs > 1) {
-            scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, true>
+            scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, RB, form.value, comp.value, true>
                 <<<grid, kScanThreads, 0, stream>>>(g, a);
             const hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
         }
-        scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, false>
+        scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, RB, form.value, comp.value, false>
             <<<grid, kScanThreads, 0, stream>>>(g, a);
         return hipGetLastError();
     });
 }
 
-template <typename TIn, int V, int CL>
+template <typename TIn, int V>
 hipError_t launch_backward_v(const GatedScan& s, const ScanBwdArgs& a, hipStream_t stream) {
-    using S = ScanTile<kScanThreads, CL, kScanRun, V>;
+    using S = BwdTile<V>;
+    constexpr int CL = S::kChannels / V, RB = S::kTile / S::kTokenLanes;
     const ScanGeo g = geometry(s);
     const dim3 grid(unsigned((s.D + S::kChannels - 1) / S::kChannels), unsigned(s.N), unsigned(g.segs));
     return by_gate(s, [&](auto form, auto comp) {
         if (g.segs > 1) {
-            scan_backward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, true>
+            scan_backward_kernel<TIn, V, CL, kScanThreads, RB, form.value, comp.value, true>
                 <<<grid, kScanThreads, 0, stream>>>(g, a);
             const hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
         }
-        scan_backward_kernel<TIn, V, CL, kScanThreads, kScanRun, form.value, comp.value, false>
+        scan_backward_kernel<TIn, V, CL, kScanThreads, RB, form.value, comp.value, false>
             <<<grid, kScanThreads, 0, stream>>>(g, a);
         return hipGetLastError();
     });
@@ -622,8 +662,7 @@ hipError_t launch_step_v(const GatedScan& s, const ScanFwdArgs& a, hipStream_t s
 }  // namespace
 
 int64_t scan_tile_tokens(const GatedScan& s) {
-    return scan_piece(s) == 4 ? ScanTile<kScanThreads, kScanLanes, kScanRun, 4>::kTile
-                              : ScanTile<kScanThreads, kScanLanes1, kScanRun, 1>::kTile;
+    return scan_piece(s) == 4 ? BwdTile<4>::kTile : BwdTile<1>::kTile;
 }
 
 int64_t scan_tiles(const GatedScan& s) {
@@ -635,7 +674,8 @@ int64_t scan_tiles(const GatedScan& s) {
 int64_t scan_segments(const GatedScan& s) {
     constexpr int64_t kWorkgroups = 512, kEnough = 200;
     const int64_t channels = scan_piece(s) == 4 ? kScanLanes * 4 : kScanLanes1;
-    const int64_t base = s.N * ((s.D + channels - 1) / channels), tiles = scan_tiles(s);
+    const int64_t base = s.N * ((s.D + channels - 1) / channels), tile = forward_tile(s);
+    const int64_t tiles = (s.T + tile - 1) / tile;
     if (base >= kEnough || tiles <= 1) return 1;
     const int64_t per = (tiles + kWorkgroups / base - 1) / (kWorkgroups / base);  // tiles of a segment
     return (tiles + per - 1) / per;
@@ -651,10 +691,8 @@ hipError_t launch_gated_scan(const GatedScan& s, const void* x, const void* gate
         return four ? launch_step_v<float, 4>(s, a, stream) : launch_step_v<float, 1>(s, a, stream);
     }
     if (s.dtype == RACE_BF16)
-        return four ? launch_forward_v<bf16_t, 4, kScanLanes>(s, a, stream)
-                    : launch_forward_v<bf16_t, 1, kScanLanes1>(s, a, stream);
-    return four ? launch_forward_v<float, 4, kScanLanes>(s, a, stream)
-                : launch_forward_v<float, 1, kScanLanes1>(s, a, stream);
+        return four ? launch_forward_v<bf16_t, 4>(s, a, stream) : launch_forward_v<bf16_t, 1>(s, a, stream);
+    return four ? launch_forward_v<float, 4>(s, a, stream) : launch_forward_v<float, 1>(s, a, stream);
 }
 
 hipError_t launch_gated_scan_bwd(const GatedScan& s, const void* x, const void* gate, const void* dout,
@@ -663,10 +701,8 @@ hipError_t launch_gated_scan_bwd(const GatedScan& s, const void* x, const void* 
     const ScanBwdArgs a{x, gate, dout, records, dfinal, dx, dgate, dstate, pairs};
     const bool four = scan_piece(s) == 4;
     if (s.dtype == RACE_BF16)
-        return four ? launch_backward_v<bf16_t, 4, kScanLanes>(s, a, stream)
-                    : launch_backward_v<bf16_t, 1, kScanLanes1>(s, a, stream);
-    return four ? launch_backward_v<float, 4, kScanLanes>(s, a, stream)
-                : launch_backward_v<float, 1, kScanLanes1>(s, a, stream);
+        return four ? launch_backward_v<bf16_t, 4>(s, a, stream) : launch_backward_v<bf16_t, 1>(s, a, stream);
+    return four ? launch_backward_v<float, 4>(s, a, stream) : launch_backward_v<float, 1>(s, a, stream);
 }
 
 }  // namespace race

@@ -1676,8 +1676,11 @@ bool scan_shape(const race_scan_shape* sh, const int32_t* lengths, GatedScan* s)
     if (sh->dtype != RACE_F32 && sh->dtype != RACE_BF16) return false;
     if (sh->gate_form != RACE_GATE_SIGMOID && sh->gate_form != RACE_GATE_LOG) return false;
     if (sh->lengths_group < 1) return false;
-    for (int64_t stride : {sh->x_stream_stride, sh->x_token_stride, sh->gate_stream_stride, sh->gate_token_stride})
-        if (stride < 0 || stride > (int64_t(1) << 46)) return false;
+    for (int64_t stride : {sh->x_stream_stride, sh->gate_stream_stride})
+        if (stride < 0 || stride > (int64_t(1) << 40)) return false;
+    // A tile's rows are addressed through one buffer resource.
+    for (int64_t stride : {sh->x_token_stride, sh->gate_token_stride})
+        if (stride < 0 || stride > RACE_SCAN_MAX_TOKEN_STRIDE) return false;
     *s = GatedScan{sh->num_streams,        sh->seq_len,           sh->channels,
                    sh->x_stream_stride,    sh->x_token_stride,    sh->gate_stream_stride,
                    sh->gate_token_stride,  sh->dtype,             sh->gate_form,

@@ -421,12 +421,13 @@ struct GatedScan {
 // Calls without records of at most this many tokens run one thread per piece of
 // a row, token by token.
 constexpr int64_t kScanStepTokens = 16;
+// Tokens of a backward tile, and the tiles (and records) of a stream.
 int64_t scan_tile_tokens(const GatedScan& s);
 int64_t scan_tiles(const GatedScan& s);
 // Segments of whole tiles the tokens are split into; more than one take
 // `pairs`, [N][segments][2][D] floats.
 int64_t scan_segments(const GatedScan& s);
-// records (nullable): [N][tiles][D] floats, the state each tile starts from.
+// records (nullable): [N][tiles][D] floats, the state each backward tile starts from.
 // state_out may be state_in with one segment.
 hipError_t launch_gated_scan(const GatedScan& s, const void* x, const void* gate, const float* state_in, void* out,
                              float* state_out, float* records, float* pairs, hipStream_t stream);

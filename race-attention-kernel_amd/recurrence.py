@@ -25,10 +25,14 @@ def _form_id(gate_form: str) -> int:
         raise ValueError(f"gate_form must be one of {sorted(GATE_FORMS)}, got {gate_form!r}") from None
 
 
+MAX_TOKEN_STRIDE = 1 << 20  # elements; RACE_SCAN_MAX_TOKEN_STRIDE
+
+
 def _channel_rows(t: torch.Tensor) -> torch.Tensor:
     """t as the kernels read it, by strides: a copy only where the channels of a
-    token are apart or the first is not 16-byte aligned."""
-    if t.dim() == 3 and t.numel() and ((t.size(2) > 1 and t.stride(2) != 1) or t.data_ptr() % 16):
+    token are apart, the first is not 16-byte aligned, or tokens lie very far apart."""
+    if t.dim() == 3 and t.numel() and ((t.size(2) > 1 and t.stride(2) != 1) or t.data_ptr() % 16 or
+                                       (t.size(1) > 1 and t.stride(1) > MAX_TOKEN_STRIDE)):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 

@@ -175,9 +175,11 @@ def test_strided_inputs_equal_dense_ones(race, cuda, dtype):
     turned = both.permute(1, 0, 2, 3).contiguous().permute(1, 0, 2, 3)  # tokens outermost in memory
     shifted = torch.empty(N * T * 2 * D + 1, dtype=dtype, device=cuda)[1:].view(N, T, 2, D).copy_(both)
     apart = torch.empty(N, T, 2, D, 2, dtype=dtype, device=cuda)[..., 0].copy_(both)
+    far = torch.empty(T, (1 << 20) + 16, dtype=dtype, device=cuda)[:, :N * 2 * D].view(T, N, 2, D).copy_(
+        both.permute(1, 0, 2, 3)).permute(1, 0, 2, 3)          # tokens megabytes apart
     odd = torch.empty(N, T, 2, D + 1, dtype=dtype, device=cuda)[..., :D].copy_(both)
     want = race.race_gated_scan(x, gate, state)
-    for src in (both, turned, shifted, apart, odd):
+    for src in (both, turned, shifted, apart, far, odd):
         xs, gs = src[:, :, 0], src[:, :, 1]
         got = race.race_gated_scan(xs, gs, state)
         exact = src is not odd  # an odd stride takes the narrow kernel, another order of sums

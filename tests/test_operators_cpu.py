@@ -11,7 +11,7 @@ def test_scan_shapes_and_workspaces(race):
 
     ok = abi.scan_shape(8, 4096, 2048)
     st, nbytes, floats = abi.gated_scan_workspace_bytes(ok)
-    assert st == abi.RACE_SUCCESS and nbytes == 0 and floats == 8 * 16 * 2048  # 256-token tiles
+    assert st == abi.RACE_SUCCESS and nbytes == 0 and floats == 8 * 32 * 2048  # 128-token tiles
     # Few channels: the tokens are split, and the pairs of the segments need room.
     st, nbytes, _ = abi.gated_scan_workspace_bytes(abi.scan_shape(8, 65536, 64))
     assert st == abi.RACE_SUCCESS and nbytes > 0
@@ -22,7 +22,9 @@ def test_scan_shapes_and_workspaces(race):
     for bad in (abi.scan_shape(65536, 1, 4), abi.scan_shape(-1, 1, 4), abi.scan_shape(1, -1, 4),
                 abi.scan_shape(1, 2 ** 31 - 1, 4), abi.scan_shape(1, 1, 0), abi.scan_shape(1, 1, 65537),
                 abi.scan_shape(1, 1, 4, dtype=2), abi.scan_shape(1, 1, 4, gate_form=2),
-                abi.scan_shape(1, 1, 4, lengths_group=0)):
+                abi.scan_shape(1, 1, 4, lengths_group=0),
+                abi.RaceScanShape(1, 9, 4, 0, (1 << 20) + 1, 0, 4, 0, 0, 1, 1),
+                abi.RaceScanShape(1, 9, 4, -4, 4, 0, 4, 0, 0, 1, 1)):
         assert abi.gated_scan_workspace_bytes(bad)[0] == abi.RACE_ERROR_INVALID_VALUE
 
 
