@@ -39,15 +39,16 @@ struct Piece {
     static constexpr int kBytes = V * int(sizeof(TIn));
     using Raw = std::conditional_t<V == 1, TIn, std::conditional_t<sizeof(TIn) == 4, mfma::u32x4, mfma::u32x2>>;
     Raw v;
+    template <int P>
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int off) {
         if constexpr (kBytes == 16)
-            v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, mfma::kPolicyDefault);
+            v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, P);
         else if constexpr (kBytes == 8)
-            v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, mfma::kPolicyDefault);
+            v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, P);
         else if constexpr (kBytes == 4)
-            v = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, mfma::kPolicyDefault));
+            v = __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, P));
         else
-            v = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, mfma::kPolicyDefault);
+            v = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, P);
     }
     __device__ __forceinline__ float get(int j) const {
         if constexpr (V == 1)
@@ -57,18 +58,19 @@ struct Piece {
         else
             return (j & 1) ? mfma::hi_half(v[j >> 1]) : mfma::lo_half(v[j >> 1]);
     }
+    template <int P>
     __device__ __forceinline__ static void store(__amdgpu_buffer_rsrc_t r, int off, const float (&x)[V]) {
         if constexpr (kBytes == 16)
             __builtin_amdgcn_raw_buffer_store_b128(mfma::u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]),
                                                                __float_as_uint(x[2]), __float_as_uint(x[3])},
-                                                   r, off, 0, mfma::kPolicyDefault);
+                                                   r, off, 0, P);
         else if constexpr (kBytes == 8)
             __builtin_amdgcn_raw_buffer_store_b64(mfma::u32x2{mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3])}, r, off,
-                                                  0, mfma::kPolicyDefault);
+                                                  0, P);
         else if constexpr (kBytes == 4)
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[0]), r, off, 0, mfma::kPolicyDefault);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x[0]), r, off, 0, P);
         else
-            __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x[0]), r, off, 0, mfma::kPolicyDefault);
+            __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(x[0]), r, off, 0, P);
     }
     __device__ __forceinline__ static void put(TIn* p, const float (&x)[V]) {
         if constexpr (V == 1)
@@ -258,7 +260,7 @@ __device__ __forceinline__ void through_segments(float (&carry)[V], const float*
 
 // One workgroup per (block of channels, stream, segment).  kPairs: only the
 // segment's pair, into a.pairs.
-template <typename TIn, int V, int CL, int NT, int R, int RB, int kForm, bool kComplement, bool kPairs>
+template <typename TIn, int V, int CL, int NT, int R, int RB, int kForm, bool kComplement, bool kPairs, int kPolicy>
 __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const ScanFwdArgs a) {
     using S = ScanTile<NT, CL, R, V>;
     using X = Piece<TIn, V>;
@@ -285,8 +287,8 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
         const auto gr = rows_view<S::kTile>(gp, r0, end, g.gt, D);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            xn[r].load(xr, xo + r * xs);
-            gn[r].load(gr, go + r * gs);
+            xn[r].template load<kPolicy>(xr, xo + r * xs);
+            gn[r].template load<kPolicy>(gr, go + r * gs);
         }
     };
     if (t0 < end) load(t0);
@@ -308,7 +310,7 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
             const float zero[V] = {};
             const auto orr = rows_view<S::kTile>(op, r0, t1, D, D);
 #pragma unroll
-            for (int r = 0; r < R; ++r) X::store(orr, oo + r * os, zero);
+            for (int r = 0; r < R; ++r) X::template store<kPolicy>(orr, oo + r * os, zero);
             continue;
         }
         float av[R][V], uv[R][V], P[V], H[V];
@@ -343,7 +345,7 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
         S::template join<true, kPairs>(P, H, carry, start, product, lds + parity * (S::kLdsFloats / 2));
         parity ^= 1;
         if constexpr (!kPairs) {
-            constexpr int kRecord = ScanTile<NT, CL, RB, V>::kTile;
+            constexpr int kRecord = S::kTokenLanes * RB;  // tokens of a backward tile
             static_assert(kRecord % R == 0 && S::kTile % kRecord == 0, "a thread's tokens start a record or do not");
             if (a.records && mine && tl * R % kRecord == 0 && t < end)
                 store_floats<V>(a.records + (n * g.tiles + t / kRecord) * D + c, start);
@@ -356,7 +358,7 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
                     start[j] = fmaf(av[r][j], start[j], uv[r][j]);
                     y[j] = whole || t + r < end ? start[j] : 0.f;
                 }
-                X::store(orr, oo + r * os, y);
+                X::template store<kPolicy>(orr, oo + r * os, y);
             }
         }
     }
@@ -371,7 +373,7 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
 }
 
 // The gradients, tiles and segments from the last to the first.
-template <typename TIn, int V, int CL, int NT, int R, int kForm, bool kComplement, bool kPairs>
+template <typename TIn, int V, int CL, int NT, int R, int kForm, bool kComplement, bool kPairs, int kPolicy>
 __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, const ScanBwdArgs a) {
     using S = ScanTile<NT, CL, R, V>;
     using X = Piece<TIn, V>;
@@ -404,9 +406,9 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
         const auto yr = rows_view<S::kTile>(yp, r0, end, D, D);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if constexpr (!kPairs) xn[r].load(xr, xo + r * xs);
-            gn[r].load(gr, go + r * gs);
-            yn[r].load(yr, oo + r * os);
+            if constexpr (!kPairs) xn[r].template load<kPolicy>(xr, xo + r * xs);
+            gn[r].template load<kPolicy>(gr, go + r * gs);
+            yn[r].template load<kPolicy>(yr, oo + r * os);
         }
     };
     // A gradient that is not asked for: a view of no rows.
@@ -433,8 +435,8 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
             const auto dxr = out_view(dxp, r0), dgr = out_view(dgp, r0);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                X::store(dxr, oo + r * os, zero);
-                X::store(dgr, oo + r * os, zero);
+                X::template store<kPolicy>(dxr, oo + r * os, zero);
+                X::template store<kPolicy>(dgr, oo + r * os, zero);
             }
             continue;
         }
@@ -522,8 +524,8 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
                         dg[j] = t + r < end ? dg[j] : 0.f;
                     }
                 }
-                X::store(dxr, oo + r * os, dx);
-                X::store(dgr, oo + r * os, dg);
+                X::template store<kPolicy>(dxr, oo + r * os, dx);
+                X::template store<kPolicy>(dgr, oo + r * os, dg);
             }
         }
     }
@@ -570,22 +572,53 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanGeo g, co
     if (a.state_out) store_floats<V>(a.state_out + n * g.D + c, h);
 }
 
-// Workgroup shapes: rows of whole four-value pieces, and any others.
-constexpr int kScanThreads = 512, kScanLanes = 16, kScanLanes1 = 64;
-// Tokens per thread, forward and backward.  The backward holds four values an
-// element: with 8 tokens of 4 channels it spilled 640 bytes a lane (8 x 4096
-// tokens of 2048 bf16 channels: 746 us).
-constexpr int kScanRun = 8, kScanRunBwd = 4, kScanRunBwd1 = 8;
-template <int V>
-using FwdTile = ScanTile<kScanThreads, V == 4 ? kScanLanes : kScanLanes1, kScanRun, V>;
-template <int V>
-using BwdTile = ScanTile<kScanThreads, V == 4 ? kScanLanes : kScanLanes1, V == 4 ? kScanRunBwd : kScanRunBwd1, V>;
+// Workgroup shapes: CL lanes across the channels, NF and NB threads forward
+// and backward.  Measured in us, forward / backward:
+//   32 x 2048 tokens of 2048 bf16 channels, row pieces of 256 bytes (CL 32)
+//     155 / 284 with 512 threads, 166 / 267 with 256; of 128 bytes (CL 16)
+//     171 / 323 with 512;
+//   8 x 4096 x 2048, 256 workgroups of CL 16 or 128 of CL 32: 98 / 170 (512
+//     threads), 113 / 203 (256) and 168 / 207;
+//   8 x 65536 x 64 (segments): 84 / 120 with 512 threads, 79 / 110 with 256;
+//   2 x 4096 x 2048 (segments): CL 32 46 / 60 and 41 / 53, CL 16 49 / 65.
+// Per thread 8 tokens forward and 4 backward, which holds four values an
+// element: with 8 it spilled 640 bytes a lane (8 x 4096 x 2048: 746 us).
+template <int V_, int CL, int NF, int NB, int RF = 8, int RB = 4>
+struct ScanShape {
+    static constexpr int V = V_, kLanes = CL, kFwdThreads = NF, kBwdThreads = NB, kFwdRun = RF, kBwdRun = RB;
+    using Fwd = ScanTile<NF, CL, RF, V>;
+    using Bwd = ScanTile<NB, CL, RB, V>;
+    static constexpr int kChannels = CL * V;
+};
+using Wide = ScanShape<4, 32, 512, 256>;
+using WideSplit = ScanShape<4, 32, 256, 256>;
+using Narrow = ScanShape<4, 16, 512, 512>;
+using NarrowSplit = ScanShape<4, 16, 256, 256>;
+using Single = ScanShape<1, 64, 512, 512, 8, 8>;  // any strides and widths
 
-int scan_piece(const GatedScan& s) {
-    return s.D % 4 == 0 && s.xn % 4 == 0 && s.xt % 4 == 0 && s.gn % 4 == 0 && s.gt % 4 == 0 ? 4 : 1;
+// Workgroups that fill the device without a split of the tokens, and that a
+// split aims for.
+constexpr int64_t kScanEnough = 200, kScanSplit = 512;
+
+int64_t blocks_of(const GatedScan& s, int64_t channels) { return s.N * ((s.D + channels - 1) / channels); }
+
+bool scan_vectors(const GatedScan& s) {
+    return s.D % 4 == 0 && s.xn % 4 == 0 && s.xt % 4 == 0 && s.gn % 4 == 0 && s.gt % 4 == 0;
 }
 
-int64_t forward_tile(const GatedScan& s) { return scan_piece(s) == 4 ? FwdTile<4>::kTile : FwdTile<1>::kTile; }
+// f(shape) for the shape of these arguments.
+template <typename F>
+auto by_shape(const GatedScan& s, F f) {
+    if (!scan_vectors(s)) return f(Single{});
+    if (blocks_of(s, Wide::kChannels) >= kScanEnough) return f(Wide{});
+    if (blocks_of(s, Narrow::kChannels) >= kScanEnough) return f(Narrow{});
+    return s.D > 96 ? f(WideSplit{}) : f(NarrowSplit{});
+}
+
+// Tokens a segment is made of.
+int64_t forward_tile(const GatedScan& s) {
+    return by_shape(s, [](auto shape) { return int64_t(decltype(shape)::Fwd::kTile); });
+}
 
 ScanGeo geometry(const GatedScan& s) {
     ScanGeo g;
@@ -610,40 +643,58 @@ hipError_t by_gate(const GatedScan& s, F f) {
     return s.complement ? f(Log{}, std::true_type{}) : f(Log{}, std::false_type{});
 }
 
-template <typename TIn, int V>
-hipError_t launch_forward_v(const GatedScan& s, const ScanFwdArgs& a, hipStream_t stream) {
-    using S = FwdTile<V>;
-    constexpr int CL = S::kChannels / V, RB = BwdTile<V>::kTile / BwdTile<V>::kTokenLanes;
+// Calls whose `arrays` row arrays are larger than the memory-side cache holds
+// go past the caches, if their rows are whole cache lines: 8 x 4096 x 2048 bf16,
+// forward / backward, 105 / 181 us through them and 98 / 170 past them; 1 x
+// 32768 x 1024 fp32 139 / 182 and 122 / 158; but 24 x 1531 x 520 fp32, whose
+// workgroups share lines, 55 / 99 and 68 / 119.
+bool past_scan_caches(const GatedScan& s, int arrays) {
+    constexpr int64_t kCacheBytes = int64_t(256) << 20, kLine = 128;
+    const int64_t row = s.D * (s.dtype == RACE_BF16 ? 2 : 4);
+    return row % kLine == 0 && s.N * s.T * row * arrays > kCacheBytes;
+}
+
+template <typename TIn, typename Sh>
+hipError_t launch_forward(const GatedScan& s, const ScanFwdArgs& a, hipStream_t stream) {
+    constexpr int V = Sh::V, CL = Sh::kLanes, NT = Sh::kFwdThreads, R = Sh::kFwdRun, RB = Sh::Bwd::kTile * CL / NT;
     const ScanGeo g = geometry(s);
-    const dim3 grid(unsigned((s.D + S::kChannels - 1) / S::kChannels), unsigned(s.N), unsigned(g.segs));
+    const dim3 grid(unsigned((s.D + Sh::kChannels - 1) / Sh::kChannels), unsigned(s.N), unsigned(g.segs));
     return by_gate(s, [&](auto form, auto comp) {
+        // The pairs' reads stay in the caches for the pass that reads the rows again.
         if (g.segs > 1) {
-            scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, RB, form.value, comp.value, true>
-                <<<grid, kScanThreads, 0, stream>>>(g, a);
+            scan_forward_kernel<TIn, V, CL, NT, R, RB, form.value, comp.value, true, mfma::kPolicyDefault>
+                <<<grid, NT, 0, stream>>>(g, a);
             const hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
         }
-        scan_forward_kernel<TIn, V, CL, kScanThreads, kScanRun, RB, form.value, comp.value, false>
-            <<<grid, kScanThreads, 0, stream>>>(g, a);
+        if (past_scan_caches(s, 3))
+            scan_forward_kernel<TIn, V, CL, NT, R, RB, form.value, comp.value, false, mfma::kPolicyStream>
+                <<<grid, NT, 0, stream>>>(g, a);
+        else
+            scan_forward_kernel<TIn, V, CL, NT, R, RB, form.value, comp.value, false, mfma::kPolicyDefault>
+                <<<grid, NT, 0, stream>>>(g, a);
         return hipGetLastError();
     });
 }
 
-template <typename TIn, int V>
-hipError_t launch_backward_v(const GatedScan& s, const ScanBwdArgs& a, hipStream_t stream) {
-    using S = BwdTile<V>;
-    constexpr int CL = S::kChannels / V, RB = S::kTile / S::kTokenLanes;
+template <typename TIn, typename Sh>
+hipError_t launch_backward(const GatedScan& s, const ScanBwdArgs& a, hipStream_t stream) {
+    constexpr int V = Sh::V, CL = Sh::kLanes, NT = Sh::kBwdThreads, R = Sh::kBwdRun;
     const ScanGeo g = geometry(s);
-    const dim3 grid(unsigned((s.D + S::kChannels - 1) / S::kChannels), unsigned(s.N), unsigned(g.segs));
+    const dim3 grid(unsigned((s.D + Sh::kChannels - 1) / Sh::kChannels), unsigned(s.N), unsigned(g.segs));
     return by_gate(s, [&](auto form, auto comp) {
         if (g.segs > 1) {
-            scan_backward_kernel<TIn, V, CL, kScanThreads, RB, form.value, comp.value, true>
-                <<<grid, kScanThreads, 0, stream>>>(g, a);
+            scan_backward_kernel<TIn, V, CL, NT, R, form.value, comp.value, true, mfma::kPolicyDefault>
+                <<<grid, NT, 0, stream>>>(g, a);
             const hipError_t err = hipGetLastError();
             if (err != hipSuccess) return err;
         }
-        scan_backward_kernel<TIn, V, CL, kScanThreads, RB, form.value, comp.value, false>
-            <<<grid, kScanThreads, 0, stream>>>(g, a);
+        if (past_scan_caches(s, 5))
+            scan_backward_kernel<TIn, V, CL, NT, R, form.value, comp.value, false, mfma::kPolicyStream>
+                <<<grid, NT, 0, stream>>>(g, a);
+        else
+            scan_backward_kernel<TIn, V, CL, NT, R, form.value, comp.value, false, mfma::kPolicyDefault>
+                <<<grid, NT, 0, stream>>>(g, a);
         return hipGetLastError();
     });
 }
@@ -662,7 +713,7 @@ hipError_t launch_step_v(const GatedScan& s, const ScanFwdArgs& a, hipStream_t s
 }  // namespace
 
 int64_t scan_tile_tokens(const GatedScan& s) {
-    return scan_piece(s) == 4 ? BwdTile<4>::kTile : BwdTile<1>::kTile;
+    return by_shape(s, [](auto shape) { return int64_t(decltype(shape)::Bwd::kTile); });
 }
 
 int64_t scan_tiles(const GatedScan& s) {
@@ -670,39 +721,37 @@ int64_t scan_tiles(const GatedScan& s) {
     return (s.T + tile - 1) / tile;
 }
 
-// Enough workgroups for two on every CU; whole tiles each.
 int64_t scan_segments(const GatedScan& s) {
-    constexpr int64_t kWorkgroups = 512, kEnough = 200;
-    const int64_t channels = scan_piece(s) == 4 ? kScanLanes * 4 : kScanLanes1;
-    const int64_t base = s.N * ((s.D + channels - 1) / channels), tile = forward_tile(s);
-    const int64_t tiles = (s.T + tile - 1) / tile;
-    if (base >= kEnough || tiles <= 1) return 1;
-    const int64_t per = (tiles + kWorkgroups / base - 1) / (kWorkgroups / base);  // tiles of a segment
+    const int64_t tile = forward_tile(s), tiles = (s.T + tile - 1) / tile;
+    const int64_t base = by_shape(s, [&](auto shape) { return blocks_of(s, decltype(shape)::kChannels); });
+    if (base >= kScanEnough || tiles <= 1) return 1;
+    const int64_t per = (tiles + kScanSplit / base - 1) / (kScanSplit / base);  // tiles of a segment
     return (tiles + per - 1) / per;
 }
 
 hipError_t launch_gated_scan(const GatedScan& s, const void* x, const void* gate, const float* state_in, void* out,
                              float* state_out, float* records, float* pairs, hipStream_t stream) {
     const ScanFwdArgs a{x, gate, state_in, out, state_out, records, pairs};
-    const bool four = scan_piece(s) == 4;
     if (!records && s.T <= kScanStepTokens) {
+        const bool four = scan_vectors(s);
         if (s.dtype == RACE_BF16)
             return four ? launch_step_v<bf16_t, 4>(s, a, stream) : launch_step_v<bf16_t, 1>(s, a, stream);
         return four ? launch_step_v<float, 4>(s, a, stream) : launch_step_v<float, 1>(s, a, stream);
     }
-    if (s.dtype == RACE_BF16)
-        return four ? launch_forward_v<bf16_t, 4>(s, a, stream) : launch_forward_v<bf16_t, 1>(s, a, stream);
-    return four ? launch_forward_v<float, 4>(s, a, stream) : launch_forward_v<float, 1>(s, a, stream);
+    return by_shape(s, [&](auto shape) {
+        return s.dtype == RACE_BF16 ? launch_forward<bf16_t, decltype(shape)>(s, a, stream)
+                                    : launch_forward<float, decltype(shape)>(s, a, stream);
+    });
 }
 
 hipError_t launch_gated_scan_bwd(const GatedScan& s, const void* x, const void* gate, const void* dout,
                                  const float* records, const float* dfinal, void* dx, void* dgate, float* dstate,
                                  float* pairs, hipStream_t stream) {
     const ScanBwdArgs a{x, gate, dout, records, dfinal, dx, dgate, dstate, pairs};
-    const bool four = scan_piece(s) == 4;
-    if (s.dtype == RACE_BF16)
-        return four ? launch_backward_v<bf16_t, 4>(s, a, stream) : launch_backward_v<bf16_t, 1>(s, a, stream);
-    return four ? launch_backward_v<float, 4>(s, a, stream) : launch_backward_v<float, 1>(s, a, stream);
+    return by_shape(s, [&](auto shape) {
+        return s.dtype == RACE_BF16 ? launch_backward<bf16_t, decltype(shape)>(s, a, stream)
+                                    : launch_backward<float, decltype(shape)>(s, a, stream);
+    });
 }
 
 }  // namespace race

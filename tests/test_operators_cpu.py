@@ -12,6 +12,7 @@ def test_scan_shapes_and_workspaces(race):
     ok = abi.scan_shape(8, 4096, 2048)
     st, nbytes, floats = abi.gated_scan_workspace_bytes(ok)
     assert st == abi.RACE_SUCCESS and nbytes == 0 and floats == 8 * 32 * 2048  # 128-token tiles
+    assert abi.gated_scan_workspace_bytes(abi.scan_shape(32, 4096, 2048))[2] == 32 * 128 * 2048  # 32-token tiles
     # Few channels: the tokens are split, and the pairs of the segments need room.
     st, nbytes, _ = abi.gated_scan_workspace_bytes(abi.scan_shape(8, 65536, 64))
     assert st == abi.RACE_SUCCESS and nbytes > 0
