@@ -512,6 +512,52 @@ race_status race_causal_bwd_profiled(const void* probsQ, const void* probsK, con
                                      void* workspace, size_t workspace_bytes, hipStream_t stream,
                                      hipEvent_t* events, int32_t max_events, int32_t* n_events);
 
+/* ---- Norm and rotation of query and key heads ----------------------------
+ * In front of the hashing: every row of the query and key heads divided by its
+ * root mean square, times a weight per column, and its first 2 * pairs values
+ * turned as pairs by position * inv_freq[pair], from [batch][seq_len][heads]
+ * rows to the op's streams [batch * heads][seq_len] in one launch.  The
+ * permutes are src/race_baseline.py:35-40's; the norm and the rotation have no
+ * counterpart in the reference. */
+typedef struct race_norm_rope_shape {
+    int64_t batch, seq_len;     /* batch * seq_len < 2^31 */
+    int32_t q_heads, k_heads;   /* k_heads 0: no keys; each at most 65535 */
+    int32_t head_dim;           /* 1 .. 256 */
+    int32_t pairs;              /* 0 .. head_dim / 2; 0: no rotation */
+    /* Strides of the rows in elements (the values of a row next to each other). */
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    /* Strides of the positions; an axis takes sections[axis] pairs, in order. */
+    int64_t pos_axis_stride, pos_batch_stride, pos_token_stride;
+    int32_t axes;               /* 1 .. 4 */
+    int32_t sections[4];        /* sum to pairs */
+    int32_t pos_bits;           /* 32 or 64: int32_t or int64_t positions */
+    int32_t interleaved;        /* pairs (2p, 2p + 1); else (p, p + pairs) */
+    int32_t norm;               /* 0: rotation only */
+    float eps;
+    int32_t dtype;              /* race_dtype of the rows */
+    int32_t weight_dtype;       /* race_dtype of the weights */
+} race_norm_rope_shape;
+
+/* q_out [batch * q_heads][seq_len][head_dim] and k_out alike, contiguous.
+ * inv_freq: [pairs] fp32.  Weights: [head_dim], nullable (ones).  Rows, outputs
+ * and weights start 16-byte aligned.  Angles are formed in 64 bits. */
+race_status race_norm_rope_fwd(const void* q, const void* k, const void* positions, const float* inv_freq,
+                               const void* q_weight, const void* k_weight, void* q_out, void* k_out,
+                               const race_norm_rope_shape* shape, hipStream_t stream);
+
+/* Workspace of race_norm_rope_bwd in bytes (needed only for weight gradients). */
+race_status race_norm_rope_bwd_workspace_bytes(const race_norm_rope_shape* shape, size_t* bytes);
+
+/* Gradients for the upstream gradients dq_out and dk_out (a null one leaves
+ * that tensor out): dq and dk [batch][seq_len][heads][head_dim], contiguous,
+ * and the weights' in weight_dtype, each nullable. */
+race_status race_norm_rope_bwd(const void* q, const void* k, const void* positions, const float* inv_freq,
+                               const void* q_weight, const void* k_weight, const void* dq_out, const void* dk_out,
+                               void* dq, void* dk, void* dq_weight, void* dk_weight,
+                               const race_norm_rope_shape* shape, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+
 /* ---- Gated linear recurrence -------------------------------------------
  * Per stream and channel, for t = 0 .. T-1 from a carried state h_{-1}:
  *     h_t = a_t h_{t-1} + u_t,   out_t = h_t,

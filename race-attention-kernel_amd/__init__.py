@@ -12,11 +12,13 @@ from .ops import (HashedRaceFunction, HashProbsFunction, RaceFusedFunction, hash
                   race_fused_fwd_with_state, race_hash_probs, race_noncausal_backward,
                   select_tile_tokens)
 from .recurrence import GatedScanFunction, race_gated_scan, race_gated_scan_carry
+from .rope import NormRopeFunction, race_norm_rope
 
 __all__ = [
     "BatchedACE", "CONFIGS", "Config", "RaceFusedFunction", "config_inputs", "make_inputs",
     "race_fused_fwd", "race_fused_fwd_carry", "race_fused_fwd_with_state", "race_noncausal_backward",
     "race_causal_backward", "race_fused_fwd_hashed", "hashed_supported", "HashedRaceFunction",
     "HashProbsFunction", "race_hash_probs", "select_tile_tokens", "causal_v2",
+    "NormRopeFunction", "race_norm_rope",
     "GatedScanFunction", "race_gated_scan", "race_gated_scan_carry",
 ]

@@ -68,6 +68,9 @@ EXPORTED_SYMBOLS = (
     "race_alg1_fwd",
     "race_alg1_fwd_carry",
     "race_alg1_fwd_profiled",
+    "race_norm_rope_fwd",
+    "race_norm_rope_bwd_workspace_bytes",
+    "race_norm_rope_bwd",
     "race_gated_scan_workspace_bytes",
     "race_gated_scan_fwd",
     "race_gated_scan_bwd",
@@ -97,6 +100,28 @@ class RaceShape(ctypes.Structure):
 
 class RaceOptions(ctypes.Structure):
     _fields_ = [("tile_tokens", ctypes.c_int32), ("kernel", ctypes.c_int32)]
+
+
+class RaceNormRopeShape(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("seq_len", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("pairs", ctypes.c_int32),
+        ("q_strides", ctypes.c_int64 * 3),    # batch, token, head
+        ("k_strides", ctypes.c_int64 * 3),
+        ("pos_strides", ctypes.c_int64 * 3),  # axis, batch, token
+        ("axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("pos_bits", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+    ]
 
 
 class RaceScanShape(ctypes.Structure):
@@ -170,6 +195,10 @@ def lib() -> ctypes.CDLL:
         L.race_alg1_fwd_carry.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, a1, i32, i32, vp, sz, vp]
         L.race_alg1_fwd_profiled.argtypes = [vp, vp, vp, vp, vp, vp, vp, a1, i32, i32, vp, sz, vp,
                                              ctypes.POINTER(vp), i32, ctypes.POINTER(i32)]
+        nr = ctypes.POINTER(RaceNormRopeShape)
+        L.race_norm_rope_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, nr, vp]
+        L.race_norm_rope_bwd_workspace_bytes.argtypes = [nr, ctypes.POINTER(sz)]
+        L.race_norm_rope_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, nr, vp, sz, vp]
         sc = ctypes.POINTER(RaceScanShape)
         L.race_gated_scan_workspace_bytes.argtypes = [sc, i32, ctypes.POINTER(sz), ctypes.POINTER(i64)]
         L.race_gated_scan_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
@@ -461,3 +490,37 @@ def gated_scan_bwd(x: int, gate: int, lengths: int | None, dout: int, dfinal: in
     """race_gated_scan_bwd on raw device addresses; returns the status."""
     return lib().race_gated_scan_bwd(x, gate, lengths, dout, dfinal, records, dx, dgate, dstate, ctypes.byref(sh),
                                      workspace, workspace_bytes, stream)
+
+
+def norm_rope_shape(B: int, T: int, Hq: int, Hk: int, d: int, pairs: int, *, sections=None, interleaved: bool = False,
+                    norm: bool = True, eps: float = 1e-6, pos_bits: int = 64, dtype: int = RACE_F32,
+                    weight_dtype: int = RACE_F32) -> RaceNormRopeShape:
+    """The shape of contiguous rows [B][T][H][d] and positions [axes][B][T]."""
+    s3, s4 = ctypes.c_int64 * 3, ctypes.c_int32 * 4
+    parts = list(sections) if sections else [pairs]
+    return RaceNormRopeShape(B, T, Hq, Hk, d, pairs, s3(T * Hq * d, Hq * d, d), s3(T * Hk * d, Hk * d, d),
+                             s3(B * T, T, 1), len(parts), s4(*(parts + [0] * (4 - len(parts)))), pos_bits,
+                             int(interleaved), int(norm), eps, dtype, weight_dtype)
+
+
+def norm_rope_fwd(q: int, k: int | None, positions: int | None, inv_freq: int | None, q_weight: int | None,
+                  k_weight: int | None, q_out: int, k_out: int | None, sh: RaceNormRopeShape, stream: int) -> int:
+    """race_norm_rope_fwd on raw device addresses; returns the status."""
+    return lib().race_norm_rope_fwd(q, k, positions, inv_freq, q_weight, k_weight, q_out, k_out, ctypes.byref(sh),
+                                    stream)
+
+
+def norm_rope_bwd_workspace_bytes(sh: RaceNormRopeShape):
+    """(status, bytes)."""
+    b = ctypes.c_size_t(0)
+    st = lib().race_norm_rope_bwd_workspace_bytes(ctypes.byref(sh), ctypes.byref(b))
+    return st, b.value
+
+
+def norm_rope_bwd(q: int, k: int | None, positions: int | None, inv_freq: int | None, q_weight: int | None,
+                  k_weight: int | None, dq_out: int | None, dk_out: int | None, dq: int | None, dk: int | None,
+                  dq_weight: int | None, dk_weight: int | None, sh: RaceNormRopeShape, workspace: int | None,
+                  workspace_bytes: int, stream: int) -> int:
+    """race_norm_rope_bwd on raw device addresses; returns the status."""
+    return lib().race_norm_rope_bwd(q, k, positions, inv_freq, q_weight, k_weight, dq_out, dk_out, dq, dk, dq_weight,
+                                    dk_weight, ctypes.byref(sh), workspace, workspace_bytes, stream)

@@ -355,6 +355,18 @@ hipError_t zero_fill(float* p, int64_t n, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// bytes of zeros at p, a multiple of 2.
+__global__ void fill_zero16_kernel(uint16_t* __restrict__ p, int64_t n) {
+    const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+hipError_t zero_bytes(void* p, size_t bytes, hipStream_t stream) {
+    const int64_t n = int64_t(bytes / 2);
+    if (n <= 0) return hipSuccess;
+    fill_zero16_kernel<<<unsigned((n + kThreads - 1) / kThreads), kThreads, 0, stream>>>(static_cast<uint16_t*>(p), n);
+    return hipGetLastError();
+}
+
 // The reverse scan of suffix records kept as pr.N record streams (several
 // arrays of N streams each, back to back), in launches of at most
 // kMaxStreams streams (the scan's grid.y).
@@ -1757,6 +1769,106 @@ race_status race_gated_scan_bwd(const void* x, const void* gate, const int32_t* 
     if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return RACE_ERROR_INVALID_VALUE;
     return launch_gated_scan_bwd(s, x, gate, dout, records, dfinal, dx, dgate, dstate, static_cast<float*>(workspace),
                                  stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Norm and rotation of query and key heads (norm_rope.hip).
+
+namespace race {
+namespace {
+
+bool norm_rope_shape(const race_norm_rope_shape* sh, NormRope* r) {
+    if (!sh || sh->batch < 0 || sh->seq_len < 0) return false;
+    if (sh->seq_len > 0 && sh->batch > int64_t(INT_MAX) / sh->seq_len) return false;
+    if (sh->q_heads < 1 || sh->q_heads > 65535 || sh->k_heads < 0 || sh->k_heads > 65535) return false;
+    if (sh->head_dim < 1 || sh->head_dim > kRopeMaxDim || sh->pairs < 0 || sh->pairs > sh->head_dim / 2) return false;
+    if (sh->dtype != RACE_F32 && sh->dtype != RACE_BF16) return false;
+    if (sh->weight_dtype != RACE_F32 && sh->weight_dtype != RACE_BF16) return false;
+    if (sh->pos_bits != 32 && sh->pos_bits != 64) return false;
+    if (sh->axes < 1 || sh->axes > 4) return false;
+    if (sh->norm && !(sh->eps >= 0.f)) return false;
+    int64_t sum = 0;
+    for (int i = 0; i < sh->axes; ++i) {
+        if (sh->sections[i] < 0) return false;
+        sum += sh->sections[i];
+    }
+    if (sum != sh->pairs) return false;
+    for (int64_t s : {sh->q_batch_stride, sh->q_token_stride, sh->q_head_stride, sh->k_batch_stride, sh->k_token_stride,
+                      sh->k_head_stride, sh->pos_axis_stride, sh->pos_batch_stride, sh->pos_token_stride})
+        if (s < 0 || s > (int64_t(1) << 40)) return false;
+    *r = NormRope{};
+    r->B = sh->batch, r->T = sh->seq_len;
+    r->heads[0] = sh->q_heads, r->heads[1] = sh->k_heads;
+    r->d = sh->head_dim, r->pairs = sh->pairs;
+    r->xb[0] = sh->q_batch_stride, r->xt[0] = sh->q_token_stride, r->xh[0] = sh->q_head_stride;
+    r->xb[1] = sh->k_batch_stride, r->xt[1] = sh->k_token_stride, r->xh[1] = sh->k_head_stride;
+    r->pa = sh->pos_axis_stride, r->pb = sh->pos_batch_stride, r->pt = sh->pos_token_stride;
+    r->pos64 = sh->pos_bits == 64;
+    r->axes = sh->axes;
+    for (int i = 0; i < 4; ++i) r->sections[i] = sh->sections[i];
+    r->interleaved = sh->interleaved != 0, r->norm = sh->norm != 0, r->eps = sh->eps;
+    r->dtype = sh->dtype, r->weight_dtype = sh->weight_dtype;
+    return true;
+}
+
+}  // namespace
+}  // namespace race
+
+extern "C" {
+
+race_status race_norm_rope_fwd(const void* q, const void* k, const void* positions, const float* inv_freq,
+                               const void* q_weight, const void* k_weight, void* q_out, void* k_out,
+                               const race_norm_rope_shape* shape, hipStream_t stream) {
+    NormRope r;
+    if (!norm_rope_shape(shape, &r)) return RACE_ERROR_INVALID_VALUE;
+    if (r.B == 0 || r.T == 0) return RACE_SUCCESS;
+    if (!q || !q_out || (r.heads[1] && (!k || !k_out))) return RACE_ERROR_INVALID_VALUE;
+    if (r.pairs && (!positions || !inv_freq)) return RACE_ERROR_INVALID_VALUE;
+    for (const void* p : {q, k, q_weight, k_weight, static_cast<const void*>(q_out), static_cast<const void*>(k_out)})
+        if (!aligned16(p)) return RACE_ERROR_INVALID_VALUE;
+    r.positions = positions, r.inv_freq = inv_freq;
+    return launch_norm_rope(r, {q, r.heads[1] ? k : nullptr}, {q_weight, k_weight}, {q_out, k_out}, stream);
+}
+
+race_status race_norm_rope_bwd_workspace_bytes(const race_norm_rope_shape* shape, size_t* bytes) {
+    NormRope r;
+    if (!norm_rope_shape(shape, &r) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    *bytes = size_t(norm_rope_partial_floats(r)) * sizeof(float);
+    return RACE_SUCCESS;
+}
+
+race_status race_norm_rope_bwd(const void* q, const void* k, const void* positions, const float* inv_freq,
+                               const void* q_weight, const void* k_weight, const void* dq_out, const void* dk_out,
+                               void* dq, void* dk, void* dq_weight, void* dk_weight,
+                               const race_norm_rope_shape* shape, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream) {
+    NormRope r;
+    if (!norm_rope_shape(shape, &r)) return RACE_ERROR_INVALID_VALUE;
+    // A tensor without an upstream gradient, or with nothing to write, is left out.
+    const bool use_q = dq_out && (dq || dq_weight), use_k = r.heads[1] && dk_out && (dk || dk_weight);
+    if (!use_q && !use_k) return RACE_SUCCESS;
+    const bool sums = (use_q && dq_weight) || (use_k && dk_weight);
+    if (sums && !r.norm) return RACE_ERROR_INVALID_VALUE;
+    if (sums && (!workspace || !aligned16(workspace) ||
+                 workspace_bytes < size_t(norm_rope_partial_floats(r)) * sizeof(float)))
+        return RACE_ERROR_INVALID_VALUE;
+    const size_t wsize = size_t(r.d) * (r.weight_dtype == RACE_BF16 ? 2 : 4);
+    if (r.B == 0 || r.T == 0) {
+        for (void* w : {use_q ? dq_weight : nullptr, use_k ? dk_weight : nullptr})
+            if (w) RACE_TRY(zero_bytes(w, wsize, stream));
+        return RACE_SUCCESS;
+    }
+    if ((use_q && !q) || (use_k && !k) || (r.pairs && (!positions || !inv_freq))) return RACE_ERROR_INVALID_VALUE;
+    for (const void* p : {q, k, q_weight, k_weight, dq_out, dk_out, static_cast<const void*>(dq),
+                          static_cast<const void*>(dk), static_cast<const void*>(dq_weight),
+                          static_cast<const void*>(dk_weight)})
+        if (!aligned16(p)) return RACE_ERROR_INVALID_VALUE;
+    r.positions = positions, r.inv_freq = inv_freq;
+    return launch_norm_rope_bwd(r, {use_q ? q : nullptr, use_k ? k : nullptr}, {q_weight, k_weight}, {dq_out, dk_out},
+                                {dq, dk}, {use_q ? dq_weight : nullptr, use_k ? dk_weight : nullptr},
+                                static_cast<float*>(workspace), stream);
 }
 
 }  // extern "C"

@@ -406,6 +406,32 @@ hipError_t launch_hash_rows(const void* x, const float* planes_T, const void* dp
 hipError_t launch_pack_heads(const void* const* src, void* const* dst, int count, int64_t batch, int64_t T, int H,
                              int row_bytes, hipStream_t stream);
 
+// ---- norm and rotation of query and key heads (norm_rope.hip) ----
+// Rows [B][T][heads][d] by strides (queries 0, keys 1; no keys: heads[1] = 0)
+// to streams [B * heads][T][d].
+struct NormRope {
+    int64_t B, T;
+    int heads[2], d, pairs;
+    int64_t xb[2], xt[2], xh[2];  // strides in elements
+    const void* positions;        // by axis, batch and token strides
+    int64_t pa, pb, pt;
+    int pos64;
+    const float* inv_freq;
+    int axes, sections[4];
+    int interleaved, norm;
+    float eps;
+    int dtype, weight_dtype;
+};
+constexpr int kRopeMaxDim = 256;
+int64_t norm_rope_partial_floats(const NormRope& r);
+hipError_t launch_norm_rope(const NormRope& r, const void* const (&x)[2], const void* const (&w)[2], void* const (&out)[2],
+                            hipStream_t stream);
+// x[z] null leaves tensor z out; dx[z] and dw[z] may be null.  dx is contiguous
+// [B][T][heads][d].
+hipError_t launch_norm_rope_bwd(const NormRope& r, const void* const (&x)[2], const void* const (&w)[2],
+                                const void* const (&up)[2], void* const (&dx)[2], void* const (&dw)[2], float* partial,
+                                hipStream_t stream);
+
 // ---- gated linear recurrence (gated_scan.hip) ----
 // x and the gates [N][T][D] by strides (channels next to each other), out, dout,
 // dx and dgate contiguous, states [N][D] fp32.

@@ -43,6 +43,7 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
 #include <cstdint>

@@ -40,6 +40,29 @@ int64_t check_lengths(ArgCheck& c, const c10::optional<at::Tensor>& lengths, con
     return l.dim() == 1 && l.numel() > 0 && streams >= l.numel() ? streams / l.numel() : 1;
 }
 
+// Refuses a differentiable call on a stream under capture whose leaf inputs are
+// still held by a graph from the default stream: the backward would wait for
+// that stream inside the capture, which ends the process.  Deleting the eager
+// outputs (or detaching them) frees the leaves.
+void check_capture(const char* entry, const std::vector<c10::optional<at::Tensor>>& inputs) {
+    bool capturing = false, asked = false;
+    for (const auto& t : inputs) {
+        if (!t || !t->defined() || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
+        if (!asked) {
+            hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+            TORCH_CHECK(hipStreamIsCapturing(current_stream(), &status) == hipSuccess, entry, ": hipStreamIsCapturing failed");
+            capturing = status == hipStreamCaptureStatusActive;
+            asked = true;
+        }
+        if (!capturing) return;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = node ? node->stream() : c10::nullopt;
+        TORCH_CHECK(!stream || stream->id() != 0, entry,
+                    ": an input that requires a gradient belongs to a graph built on the default stream that is still "
+                    "alive, so its backward cannot be captured; delete or detach that graph's outputs first");
+    }
+}
+
 // ---- gated linear recurrence ----
 
 race_scan_shape scan_shape(const char* entry, const at::Tensor& x, const at::Tensor& gate,
@@ -129,8 +152,175 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
     return {dx, dgate, dstate};
 }
 
+// ---- norm and rotation of query and key heads ----
+
+struct RopeCall {
+    race_norm_rope_shape sh{};
+    int64_t B = 0, T = 0, d = 0;
+};
+
+RopeCall rope_call(const char* entry, const at::Tensor& q, const c10::optional<at::Tensor>& k,
+                   const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& inv_freq,
+                   const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight, double eps,
+                   bool norm, const std::vector<int64_t>& sections, bool interleaved) {
+    ArgCheck c(entry);
+    check_rows(c, "q", q, 4, "[B, T, H, d]");
+    c.raise();
+    RopeCall r;
+    r.B = q.size(0), r.T = q.size(1), r.d = q.size(3);
+    c.require(q.size(2) >= 1 && q.size(2) <= 65535 && r.d >= 1 && r.d <= 256, "q",
+              "has shape " + dims(q) + "; rows of 1 .. 256 values in 1 .. 65535 heads are taken")
+        .require(r.T == 0 || r.B <= INT32_MAX / r.T, "q", "has 2^31 tokens or more");
+    if (k) {
+        check_rows(c, "k", *k, 4, "[B, T, H, d]");
+        c.matches("k", *k, "q", q)
+            .require(k->dim() == 4 && k->size(0) == r.B && k->size(1) == r.T && k->size(3) == r.d && k->size(2) >= 1 &&
+                         k->size(2) <= 65535,
+                     "k", "has shape " + dims(*k) + ", not q's batch, tokens and head width");
+    }
+    int64_t pairs = 0;
+    const bool many = inv_freq && sections.size() > 1;  // without a rotation there are no axes
+    if (inv_freq) {
+        c.on_gpu("inv_freq", *inv_freq)
+            .require(inv_freq->scalar_type() == at::kFloat && inv_freq->device() == q.device() && inv_freq->dim() == 1,
+                     "inv_freq", "must be a float32 vector on q's device")
+            .require(2 * inv_freq->numel() <= r.d, "inv_freq",
+                     "has " + std::to_string(inv_freq->numel()) + " pairs, more than half of d = " + std::to_string(r.d));
+        pairs = inv_freq->numel();
+        c.require(positions.has_value(), "positions", "are needed for a rotation");
+        if (positions) {
+            const at::Tensor& p = *positions;
+            c.require(p.device() == q.device() && (p.scalar_type() == at::kInt || p.scalar_type() == at::kLong),
+                      "positions", "must be int32 or int64 on q's device")
+                .require(p.dim() >= 1 && p.dim() <= 3 && p.size(p.dim() - 1) == r.T &&
+                             (p.dim() < 2 || p.size(p.dim() - 2) == r.B),
+                         "positions", "have shape " + dims(p) + ", not [T], [B, T] or [axes, B, T]")
+                .require(sections.size() <= 4 && (p.dim() == 3 ? p.size(0) == int64_t(many ? sections.size() : 1) : !many),
+                         "positions", "have shape " + dims(p) + " for " +
+                                          std::to_string(sections.empty() ? 1 : sections.size()) +
+                                          " sections; one axis each (at most 4)");
+        }
+        int64_t sum = 0;
+        for (int64_t s : sections) {
+            c.require(s >= 0 && s <= 256, "sections", "hold a count that is not 0 .. 256");
+            sum += s;
+        }
+        c.require(sections.empty() || sum == pairs, "sections",
+                  "sum to " + std::to_string(sum) + ", not the " + std::to_string(pairs) + " pairs of inv_freq");
+    }
+    at::ScalarType wt = q.scalar_type();
+    bool first = true;
+    for (const auto& [name, w] : {std::make_pair("q_weight", &q_weight), std::make_pair("k_weight", &k_weight)}) {
+        if (!*w) continue;
+        const at::Tensor& t = **w;
+        c.on_gpu(name, t).dtype_is(name, t, true)
+            .require(t.device() == q.device() && t.dim() == 1 && t.numel() == r.d, name,
+                     "must hold d = " + std::to_string(r.d) + " values on q's device")
+            .require(first || t.scalar_type() == wt, name, "has another dtype than q_weight")
+            .require(norm, name, "is given without a norm (eps is None)");
+        wt = t.scalar_type(), first = false;
+    }
+    c.require(!norm || (eps >= 0 && eps < 1e30), "eps", "must be a number of at least 0").raise();
+    race_norm_rope_shape& sh = r.sh;
+    sh.batch = r.B, sh.seq_len = r.T;
+    sh.q_heads = static_cast<int32_t>(q.size(2)), sh.k_heads = k ? static_cast<int32_t>(k->size(2)) : 0;
+    sh.head_dim = static_cast<int32_t>(r.d), sh.pairs = static_cast<int32_t>(pairs);
+    auto stride = [](const at::Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; };
+    sh.q_batch_stride = stride(q, 0), sh.q_token_stride = stride(q, 1), sh.q_head_stride = stride(q, 2);
+    if (k) sh.k_batch_stride = stride(*k, 0), sh.k_token_stride = stride(*k, 1), sh.k_head_stride = stride(*k, 2);
+    sh.axes = many ? static_cast<int32_t>(sections.size()) : 1;
+    for (int i = 0; i < sh.axes; ++i) sh.sections[i] = static_cast<int32_t>(many ? sections[i] : pairs);
+    sh.pos_bits = 64;
+    if (pairs > 0) {
+        const at::Tensor& p = *positions;
+        const int64_t n = p.dim();
+        sh.pos_bits = p.scalar_type() == at::kLong ? 64 : 32;
+        sh.pos_token_stride = stride(p, n - 1);
+        sh.pos_batch_stride = n > 1 ? stride(p, n - 2) : 0;
+        sh.pos_axis_stride = n > 2 ? stride(p, 0) : 0;
+    }
+    sh.interleaved = interleaved, sh.norm = norm, sh.eps = static_cast<float>(eps);
+    sh.dtype = dtype_of(q), sh.weight_dtype = wt == at::kFloat ? RACE_F32 : RACE_BF16;
+    return r;
+}
+
+const void* data_of(const c10::optional<at::Tensor>& t) { return t ? t->data_ptr() : nullptr; }
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> norm_rope_forward(
+    const at::Tensor& q, const c10::optional<at::Tensor>& k, const c10::optional<at::Tensor>& positions,
+    const c10::optional<at::Tensor>& inv_freq, const c10::optional<at::Tensor>& q_weight,
+    const c10::optional<at::Tensor>& k_weight, double eps, bool norm, const std::vector<int64_t>& sections,
+    bool interleaved) {
+    const RopeCall r = rope_call("race_norm_rope", q, k, positions, inv_freq, q_weight, k_weight, eps, norm, sections,
+                                 interleaved);
+    const c10::DeviceGuard guard(q.device());
+    const at::Tensor q_out = at::empty({r.B * q.size(2), r.T, r.d}, q.options());
+    c10::optional<at::Tensor> k_out;
+    if (k) k_out = at::empty({r.B * k->size(2), r.T, r.d}, q.options());
+    check_status(race_norm_rope_fwd(q.data_ptr(), data_of(k), data_of(positions),
+                                    static_cast<const float*>(data_of(inv_freq)), data_of(q_weight), data_of(k_weight),
+                                    q_out.data_ptr(), ptr_of(k_out), &r.sh, current_stream()),
+                 "race_norm_rope_fwd");
+    return {q_out, k_out};
+}
+
+// Gradients of q, k and the weights, for those asked for; dq_out or dk_out
+// missing leaves that tensor's out.
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+norm_rope_backward(const at::Tensor& q, const c10::optional<at::Tensor>& k, const c10::optional<at::Tensor>& positions,
+                   const c10::optional<at::Tensor>& inv_freq, const c10::optional<at::Tensor>& q_weight,
+                   const c10::optional<at::Tensor>& k_weight, const c10::optional<at::Tensor>& dq_out,
+                   const c10::optional<at::Tensor>& dk_out, double eps, bool norm, const std::vector<int64_t>& sections,
+                   bool interleaved, bool need_q, bool need_k, bool need_qw, bool need_kw) {
+    const char* entry = "race_norm_rope backward";
+    const RopeCall r = rope_call(entry, q, k, positions, inv_freq, q_weight, k_weight, eps, norm, sections, interleaved);
+    ArgCheck c(entry);
+    if (dq_out)
+        c.on_gpu("dq_out", *dq_out).matches("dq_out", *dq_out, "q", q)
+            .require(dq_out->sizes() == at::IntArrayRef({r.B * q.size(2), r.T, r.d}), "dq_out", "has shape " + dims(*dq_out));
+    if (dk_out)
+        c.require(k.has_value(), "dk_out", "is given without k")
+            .on_gpu("dk_out", *dk_out).matches("dk_out", *dk_out, "q", q)
+            .require(k && dk_out->sizes() == at::IntArrayRef({r.B * k->size(2), r.T, r.d}), "dk_out",
+                     "has shape " + dims(*dk_out));
+    c.raise();
+    const c10::DeviceGuard guard(q.device());
+    c10::optional<at::Tensor> dq, dk, dqw, dkw;
+    if (need_q && dq_out) dq = at::empty(q.sizes(), q.options());
+    if (need_k && dk_out) dk = at::empty(k->sizes(), k->options());
+    if (need_qw && dq_out && q_weight) dqw = at::empty_like(*q_weight);
+    if (need_kw && dk_out && k_weight) dkw = at::empty_like(*k_weight);
+    if (r.B == 0 || r.T == 0) {  // empty tensors have no address to hand on
+        if (dqw) dqw->zero_();
+        if (dkw) dkw->zero_();
+        return {dq, dk, dqw, dkw};
+    }
+    size_t bytes = 0;
+    at::Tensor ws;
+    if (dqw || dkw) {
+        check_status(race_norm_rope_bwd_workspace_bytes(&r.sh, &bytes), "race_norm_rope_bwd_workspace_bytes");
+        ws = workspace_of(bytes, q);
+    }
+    check_status(race_norm_rope_bwd(q.data_ptr(), data_of(k), data_of(positions),
+                                    static_cast<const float*>(data_of(inv_freq)), data_of(q_weight), data_of(k_weight),
+                                    data_of(dq_out), data_of(dk_out), ptr_of(dq), ptr_of(dk), ptr_of(dqw), ptr_of(dkw),
+                                    &r.sh, bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
+                 "race_norm_rope_bwd");
+    return {dq, dk, dqw, dkw};
+}
+
 void bind_operators(pybind11::module& m) {
     namespace py = pybind11;
+    m.def("check_capture", &check_capture, "Refuses a capture whose backward would wait for the default stream",
+          py::arg("entry"), py::arg("inputs"));
+    m.def("norm_rope_forward", &norm_rope_forward, "Heads normed and rotated, to streams -> (q, k or None)",
+          py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"), py::arg("q_weight"),
+          py::arg("k_weight"), py::arg("eps"), py::arg("norm"), py::arg("sections"), py::arg("interleaved"));
+    m.def("norm_rope_backward", &norm_rope_backward,
+          "Gradients of norm_rope_forward -> (dq, dk, dq_weight, dk_weight)", py::arg("q"), py::arg("k"),
+          py::arg("positions"), py::arg("inv_freq"), py::arg("q_weight"), py::arg("k_weight"), py::arg("dq_out"),
+          py::arg("dk_out"), py::arg("eps"), py::arg("norm"), py::arg("sections"), py::arg("interleaved"),
+          py::arg("need_q"), py::arg("need_k"), py::arg("need_qw"), py::arg("need_kw"));
     m.def("gated_scan_forward", &gated_scan_forward,
           "h_t = a_t h_{t-1} + u_t -> (out, final state, records or None)", py::arg("x"), py::arg("gate"),
           py::arg("state"), py::arg("lengths"), py::arg("form"), py::arg("complement"), py::arg("want_records"),

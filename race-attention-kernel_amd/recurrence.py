@@ -51,6 +51,8 @@ class GatedScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, state, lengths, form, complement):
         needs = any(ctx.needs_input_grad[:3])
+        if needs:
+            _lib.ext().check_capture("race_gated_scan", [x, gate, state])
         out, final, records = _lib.ext().gated_scan_forward(x, gate, state, lengths, form, complement, needs, False)
         ctx.set_materialize_grads(False)
         if needs:
@@ -64,6 +66,7 @@ class GatedScanFunction(torch.autograd.Function):
         if dout is None and dfinal is None:
             return None, None, None, None, None, None
         x, gate, lengths, records = ctx.saved_tensors
+        _lib.ext().check_capture("race_gated_scan backward", [x, gate])
         dout = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dout is None else _dense(dout.to(x.dtype))
         if dfinal is not None:
             dfinal = _dense(dfinal.float())

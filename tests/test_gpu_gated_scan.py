@@ -331,7 +331,7 @@ def test_other_streams_and_captured_steps(race, cuda):
 
     def step():
         out, final = race.race_gated_scan(xs, gs, ss)
-        return (out, final, *torch.autograd.grad((out, final), (xs, gs, ss), (dout, dfinal)))
+        return (out.detach(), final.detach(), *torch.autograd.grad((out, final), (xs, gs, ss), (dout, dfinal)))
 
     with torch.cuda.stream(side):
         step(), race.race_gated_scan_carry(xd, gd, carried, inplace=True)
@@ -353,6 +353,18 @@ def test_other_streams_and_captured_steps(race, cuda):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(outs, eager)), i
         assert torch.equal(decoded, wd) and torch.equal(carried, ws), i
+
+
+def test_a_live_eager_graph_refuses_the_capture(race, cuda):
+    # The backward would wait for the default stream inside the capture.
+    x, gate, _, _, _ = make(1, 40, 64, torch.float32, "sigmoid", 17, cuda)
+    x.requires_grad_(True)
+    eager, _ = race.race_gated_scan(x, gate)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            gate.mul(2)  # something to record
+            race.race_gated_scan(x, gate)
+    del eager
 
 
 def test_offsets_past_32_bits(race, cuda):

@@ -1,0 +1,424 @@
+"""Norm and rotation of query and key heads against the formulas in 64 bits.
+
+Tolerances come from the arithmetic, with u = 2^-24.  A row's sum of squares has
+no cancellation: at most 22 roundings deep, so its root's reciprocal is within 15
+u, a normed value within 17 u.  An angle less its whole turns is rounded once (at
+most pi u) and its cosine is good to 4 u: 8 u absolute.  With A = |a| + |b| of a
+pair a rotated value is within 27 u A (10 u A without the norm).  Backward, with G
+= |g_a| + |g_b|, S = sum |w| G |x|: dx within r |w| G 28 u + |x| r^3 / d S 80 u; a
+weight's gradient within (250 + rows / 64) u of the sum of its terms' magnitudes
+(a few hundred sums one after another at most).  Half a step of the output's type
+on top.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from gpu_util import say
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: U, torch.bfloat16: 2.0 ** -8}
+
+
+def freqs(pairs, device, theta=10000.0):
+    return (theta ** (-torch.arange(pairs, dtype=torch.float64) / max(pairs, 1))).float().to(device)
+
+
+def turn(y, c, s, pairs, interleaved):
+    """(rotated, |a| + |b| of each value's pair)"""
+    out, size = y.clone(), y.abs()
+    if interleaved:
+        i, j = slice(0, 2 * pairs, 2), slice(1, 2 * pairs, 2)
+    else:
+        i, j = slice(0, pairs), slice(pairs, 2 * pairs)
+    a, b = y[..., i], y[..., j]
+    out[..., i], out[..., j] = a * c - b * s, a * s + b * c
+    size[..., i] = size[..., j] = a.abs() + b.abs()
+    return out, size
+
+
+def angles(positions, inv_freq, sections, B, T):
+    pos = positions.double()
+    if pos.dim() == 1:
+        pos = pos.expand(1, B, T)
+    elif pos.dim() == 2:
+        pos = pos[None]
+    counts = sections or [inv_freq.numel()]
+    per = torch.cat([pos[i][..., None].expand(B, T, n) for i, n in enumerate(counts)], -1)
+    f = per * inv_freq.double()
+    return torch.cos(f)[:, None], torch.sin(f)[:, None]  # [B, 1, T, pairs]
+
+
+def reference(x, w, positions, inv_freq, sections, interleaved, eps, up=None, wdtype=None):
+    """name -> (value, bound); x [B, T, H, d]."""
+    B, T, H, d = x.shape
+    half = HALF[x.dtype]
+    rows = x.double().transpose(1, 2)
+    wd = torch.ones(d, dtype=torch.float64, device=x.device) if w is None else w.double()
+    if eps is None:
+        r, y, k = torch.ones_like(rows[..., :1]), rows, 10
+    else:
+        r = ((rows * rows).mean(-1, keepdim=True) + eps).rsqrt()
+        y, k = rows * r * wd, 27
+    pairs = 0 if inv_freq is None else inv_freq.numel()
+    c = s = None
+    size = y.abs()
+    out = y
+    if pairs:
+        c, s = angles(positions, inv_freq, sections, B, T)
+        out, size = turn(y, c, s, pairs, interleaved)
+    res = {"out": (out.reshape(B * H, T, d), (k * U * size + half * out.abs()).reshape(B * H, T, d))}
+    if up is None:
+        return res
+    g = up.double().view(B, H, T, d)
+    G = g.abs()
+    if pairs:
+        g, G = turn(g, c, -s, pairs, interleaved)
+    if eps is None:
+        dx, bound = g, 10 * U * G
+    else:
+        S = (wd.abs() * G * rows.abs()).sum(-1, keepdim=True)
+        dx = r * (g * wd - rows * r * r * (g * wd * rows).mean(-1, keepdim=True))
+        bound = r * wd.abs() * G * 28 * U + rows.abs() * r ** 3 / d * S * 80 * U
+        terms, mags = (g * rows * r).sum((0, 1, 2)), (G * rows.abs() * r).sum((0, 1, 2))
+        res["dw"] = (terms, (250 + B * T * H / 64) * U * mags + HALF[wdtype or x.dtype] * terms.abs())
+    res["dx"] = (dx.transpose(1, 2), (bound + half * dx.abs()).transpose(1, 2))
+    return res
+
+
+def check(got, want, label):
+    value, bound = want
+    assert got.shape == value.shape, label
+    err = (got.double() - value).abs()
+    worst = float((err / (bound + 1e-300)).max()) if err.numel() else 0.0
+    say(label, f"{worst:.3f} of the bound")
+    assert bool((err <= bound + 1e-37).all()), (label, worst)
+
+
+def make(B, T, Hq, Hk, d, dtype, seed, device, wdtype=None):
+    g = torch.Generator(device=device).manual_seed(seed)
+    n = lambda *s: torch.randn(s, generator=g, device=device)
+    rows = n(B, T, Hq + 2 * Hk, d).to(dtype)
+    return (rows[:, :, :Hq], rows[:, :, Hq:Hq + Hk], (1 + 0.2 * n(d)).to(wdtype or dtype),
+            (1 + 0.2 * n(d)).to(wdtype or dtype), n(B * Hq, T, d).to(dtype), n(B * Hk, T, d).to(dtype))
+
+
+# (B, T, Hq, Hk, d, pairs, sections, interleaved)
+CASES = [(2, 65, 4, 2, 64, 32, None, False), (2, 65, 4, 2, 64, 32, None, True), (1, 1, 1, 1, 128, 64, None, False),
+         (64, 1, 32, 8, 128, 64, None, False), (3, 7, 5, 5, 96, 24, None, True), (2, 33, 12, 12, 64, 32, [8, 12, 12], False),
+         (2, 40, 3, 1, 80, 40, [10, 0, 14, 16], True), (1, 300, 2, 1, 256, 128, None, False), (2, 19, 3, 2, 33, 16, None, False),
+         (2, 19, 3, 2, 33, 8, None, True), (1, 5, 1, 1, 1, 0, None, False), (1, 9, 2, 1, 2, 1, None, True),
+         (2, 50, 3, 3, 40, 20, None, False), (2, 50, 3, 3, 72, 36, None, True), (1, 77, 2, 2, 250, 100, None, False),
+         (1, 50, 4, 4, 48, 8, None, False), (1, 50, 4, 4, 48, 5, None, True), (1, 60, 2, 2, 64, 0, None, False),
+         (3, 1000, 24, 8, 32, 16, None, False), (1, 2100, 8, 8, 64, 16, [4, 4, 8], False), (1, 8, 130, 1, 16, 8, None, False)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B, T, Hq, Hk, d, pairs, sections, interleaved", CASES)
+def test_forward_and_gradients(race, cuda, B, T, Hq, Hk, d, pairs, sections, interleaved, dtype):
+    q, k, qw, kw, dq, dk = make(B, T, Hq, Hk, d, dtype, 100 * d + T, cuda)
+    freq = freqs(pairs, cuda) if pairs else None
+    pos = torch.randint(0, 100000, (len(sections) if sections else 1, B, T), device=cuda)
+    pos = pos if sections else pos[0]
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+    outs = race.race_norm_rope(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[3], eps=1e-6,
+                               sections=sections, interleaved=interleaved)
+    grads = torch.autograd.grad(outs, leaves, (dq, dk))
+    for name, x, w, up, out, dx, dw in (("q", q, qw, dq, outs[0], grads[0], grads[2]),
+                                        ("k", k, kw, dk, outs[1], grads[1], grads[3])):
+        assert out.dtype == dtype and dw.dtype == dtype
+        ref = reference(x, w, pos, freq, sections, interleaved, 1e-6, up)
+        label = f"{name} {dtype} {B}x{T}x{Hq}/{Hk}x{d} p{pairs}"
+        check(out, ref["out"], label + " out")
+        check(dx, ref["dx"], label + " dx")
+        check(dw, ref["dw"], label + " dw")
+    # The rotation alone, and the rows as they are.
+    for f in (freq, None):
+        out, none = race.race_norm_rope(leaves[0], None, pos, f, eps=None, sections=sections, interleaved=interleaved)
+        assert none is None
+        (dx,) = torch.autograd.grad(out, leaves[0], dq)
+        ref = reference(q, None, pos, f, sections, interleaved, None, dq)
+        check(out, ref["out"], label + " no norm out")
+        check(dx, ref["dx"], label + " no norm dx")
+        if f is None:
+            assert torch.equal(out, q.transpose(1, 2).reshape(B * Hq, T, d)) and torch.equal(
+                dx, dq.view(B, Hq, T, d).transpose(1, 2))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_rows_per_workgroup(race, cuda, interleaved):
+    # More token tiles than the backward's workgroups: each takes several.
+    B, T, H, d = 3, 90001, 4, 32
+    q, k, qw, kw, dq, dk = make(B, T, H, 1, d, torch.float32, 3, cuda, torch.float32)
+    freq, pos = freqs(16, cuda), torch.arange(T, dtype=torch.int32, device=cuda)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+    outs = race.race_norm_rope(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[3],
+                               interleaved=interleaved)
+    grads = torch.autograd.grad(outs, leaves, (dq, dk))
+    for i, (x, w, up) in enumerate(((q, qw, dq), (k, kw, dk))):
+        ref = reference(x, w, pos, freq, None, interleaved, 1e-6, up)
+        check(outs[i], ref["out"], "many rows out")
+        check(grads[i], ref["dx"], "many rows dx")
+        check(grads[2 + i], ref["dw"], "many rows dw")
+
+
+@pytest.mark.parametrize("start", [1 << 20, (1 << 31) - 100, -(1 << 30), 1 << 40])
+def test_far_positions_keep_their_angles(race, cuda, start):
+    q, k, qw, kw, _, _ = make(1, 64, 2, 2, 64, torch.float32, 4, cuda)
+    freq = freqs(32, cuda, 500000.0)
+    pos = start + torch.arange(64, device=cuda)
+    out, _ = race.race_norm_rope(q, k, pos, freq, q_weight=qw, k_weight=kw)
+    value, bound = reference(q, qw, pos, freq, None, False, 1e-6)["out"]
+    # The product itself has 53 bits: |position| 2^-52 turns at most, beside the bound's.
+    slack = abs(start) * 2.0 ** -52 * 6.3
+    assert bool(((out.double() - value).abs() <= bound + 8 * slack).all())
+    if abs(start) < 1 << 31:
+        low, _ = race.race_norm_rope(q, k, pos.int(), freq, q_weight=qw, k_weight=kw)
+        assert torch.equal(low, out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layouts_give_the_same_rows(race, cuda, dtype):
+    B, T, H, d = 3, 21, 4, 64
+    q, k, qw, kw, dq, _ = make(B, T, H, H, d, dtype, 5, cuda)
+    q, freq, pos = q.contiguous(), freqs(32, cuda), torch.arange(T, device=cuda)
+    want, _ = race.race_norm_rope(q, None, pos, freq, q_weight=qw)
+    heads_first = q.transpose(1, 2).contiguous().transpose(1, 2)
+    tokens_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    shifted = torch.empty(q.numel() + 1, dtype=dtype, device=cuda)[1:].view(q.shape).copy_(q)
+    apart = torch.empty(B, T, H, d, 3, dtype=dtype, device=cuda)[..., 1].copy_(q)
+    odd = torch.empty(B, T, H, d + 1, dtype=dtype, device=cuda)[..., :d].copy_(q)
+    for src in (heads_first, tokens_first, shifted, apart):
+        got, _ = race.race_norm_rope(src, None, pos, freq, q_weight=qw)
+        assert torch.equal(got, want)
+    got, _ = race.race_norm_rope(odd, None, pos, freq, q_weight=qw)  # one value at a time, sums in another order
+    check(got, reference(q, qw, pos, freq, None, False, 1e-6)["out"], "odd strides")
+    # Positions by strides: one axis of interleaved triples, and one batch's for all.
+    triples = torch.randint(0, 999, (B, T, 3), device=cuda)
+    a, _ = race.race_norm_rope(q, None, triples.permute(2, 0, 1), freq, q_weight=qw, sections=[10, 11, 11])
+    b, _ = race.race_norm_rope(q, None, triples.permute(2, 0, 1).contiguous(), freq, q_weight=qw, sections=[10, 11, 11])
+    c, _ = race.race_norm_rope(q, None, pos[None].expand(B, T), freq, q_weight=qw)
+    assert torch.equal(a, b) and torch.equal(c, want)
+    # One row for the whole batch: its gradient is the sum over the batch.
+    one = q[:1].detach().requires_grad_(True)
+    out, _ = race.race_norm_rope(one.expand(B, T, H, d), None, pos, freq, q_weight=qw)
+    (g,) = torch.autograd.grad(out, one, dq)
+    value, bound = reference(q[:1].expand(B, T, H, d), qw, pos, freq, None, False, 1e-6, dq)["dx"]
+    size = value.abs().sum(0, keepdim=True)
+    assert bool(((g.double() - value.sum(0, keepdim=True)).abs() <= bound.sum(0, keepdim=True) + 4 * HALF[dtype] * size).all())
+
+
+def test_gradients_against_differences(race, cuda):
+    q, k, qw, kw, dq, dk = make(2, 13, 3, 2, 48, torch.float32, 6, cuda)
+    freq, pos = freqs(12, cuda), torch.arange(13, device=cuda) + 50
+    leaves = [t.contiguous().requires_grad_(True) for t in (q, k, qw, kw)]
+    run = lambda a, b, c, d: race.race_norm_rope(a, b, pos, freq, q_weight=c, k_weight=d, interleaved=True)
+    outs = run(*leaves)
+    grads = torch.autograd.grad(outs, leaves, (dq, dk))
+    step = 2.0 ** -9
+    for i, grad in enumerate(grads):
+        way = torch.randn(grad.shape, generator=torch.Generator().manual_seed(i)).to(cuda)
+        loss = []
+        for sign in (1, -1):
+            moved = [t.detach() + sign * step * way if j == i else t.detach() for j, t in enumerate(leaves)]
+            a, b = run(*moved)
+            loss.append(float((a.double() * dq).sum() + (b.double() * dk).sum()))
+        along = float((grad.double() * way).sum())
+        size = sum(float((o.detach().double().abs() * g.abs()).sum()) for o, g in zip(outs, (dq, dk)))
+        assert abs((loss[0] - loss[1]) / (2 * step) - along) <= 1e-3 * float(
+            (grad.double().abs() * way.abs()).sum()) + 30 * U * size / step, i
+
+
+def test_parts_left_out(race, cuda):
+    q, k, qw, kw, dq, dk = make(2, 30, 4, 2, 64, torch.bfloat16, 7, cuda, torch.float32)
+    freq, pos = freqs(32, cuda), torch.arange(30, device=cuda)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+    outs = race.race_norm_rope(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[3])
+    full = torch.autograd.grad(outs, leaves, (dq, dk), retain_graph=True)
+    assert full[2].dtype == torch.float32
+    only_q = torch.autograd.grad(outs[0], leaves, dq, retain_graph=True, allow_unused=True)
+    assert only_q[1] is None and only_q[3] is None
+    assert torch.equal(only_q[0], full[0])
+    check(only_q[2], reference(q, qw, pos, freq, None, False, 1e-6, dq, torch.float32)["dw"], "q alone dw")
+    only_w = torch.autograd.grad(outs[1], leaves[3], dk, retain_graph=True)[0]
+    check(only_w, reference(k, kw, pos, freq, None, False, 1e-6, dk, torch.float32)["dw"], "k weight alone")
+    frozen, _ = race.race_norm_rope(leaves[0], k, pos, freq, q_weight=qw, k_weight=kw)
+    assert torch.equal(torch.autograd.grad(frozen, leaves[0], dq)[0], full[0])
+    plain, _ = race.race_norm_rope(q, None, pos, freq)
+    check(plain, reference(q, None, pos, freq, None, False, 1e-6)["out"], "no weight")
+
+
+def test_rows_of_zeros_and_rows_with_nan(race, cuda):
+    q, _, qw, _, dq, _ = make(2, 40, 4, 1, 64, torch.float32, 8, cuda)
+    q, freq, pos = q.contiguous(), freqs(32, cuda), torch.arange(40, device=cuda)
+    q[0, 3, 1] = 0
+    want, _ = race.race_norm_rope(q, None, pos, freq, q_weight=qw)
+    assert (want.view(2, 4, 40, 64)[0, 1, 3] == 0).all() and torch.isfinite(want).all()
+    q[1, 5, 2, 7] = float("nan")
+    leaf = q.clone().requires_grad_(True)
+    out, _ = race.race_norm_rope(leaf, None, pos, freq, q_weight=qw)
+    bad = torch.isnan(out).view(2, 4, 40, 64)
+    assert bad[1, 2, 5].all() and int(bad.sum()) == 64
+    (g,) = torch.autograd.grad(out, leaf, dq)
+    assert torch.isnan(g[1, 5, 2]).all() and int(torch.isnan(g).sum()) == 64
+
+
+def test_repeatable_empty_and_refused(race, cuda):
+    q, k, qw, kw, dq, dk = make(4, 700, 8, 8, 64, torch.bfloat16, 9, cuda)
+    freq, pos = freqs(32, cuda), torch.arange(700, device=cuda)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+
+    def once():
+        outs = race.race_norm_rope(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[3])
+        return (*outs, *torch.autograd.grad(outs, leaves, (dq, dk)))
+
+    assert all(torch.equal(a, b) for a, b in zip(once(), once()))
+    for B, T in ((0, 5), (3, 0)):
+        e = torch.empty(B, T, 4, 64, device=cuda, requires_grad=True)
+        w = torch.ones(64, device=cuda, requires_grad=True)
+        out, _ = race.race_norm_rope(e, e, torch.zeros(T, dtype=torch.long, device=cuda), freqs(32, cuda), q_weight=w,
+                                     k_weight=w)
+        assert out.shape == (B * 4, T, 64)
+        assert (torch.autograd.grad(out, w, torch.ones_like(out))[0] == 0).all()
+    x, w = torch.zeros(2, 5, 4, 64, device=cuda), torch.ones(64, device=cuda)
+    f, p = freqs(32, cuda), torch.arange(5, device=cuda)
+    refused = [
+        (dict(q=x[0]), "q has shape"), (dict(q=x.half()), "neither float32 nor bfloat16"),
+        (dict(q=torch.zeros(2, 5, 4, 257, device=cuda)), "1 .. 256"), (dict(k=x[:, :4]), "k has shape"),
+        (dict(k=x.bfloat16()), "another dtype"), (dict(positions=None), "positions are needed"),
+        (dict(positions=p.float()), "int32 or int64"), (dict(positions=p[:4]), "positions have shape"),
+        (dict(inv_freq=freqs(33, cuda)), "more than half"), (dict(inv_freq=f.double()), "float32 vector"),
+        (dict(sections=[8, 8]), "one axis each"), (dict(sections=[31]), "sum to 31"),
+        (dict(positions=p.expand(3, 2, 5), sections=[8, 8, 8]), "sum to 24"),
+        (dict(positions=p.expand(5, 2, 5), sections=[8, 8, 8, 4, 4]), "at most 4"),
+        (dict(q_weight=w[:63]), "q_weight must hold"), (dict(q_weight=w, k_weight=w.bfloat16()), "another dtype than q_weight"),
+        (dict(q_weight=w, eps=None), "without a norm"), (dict(eps=-1.0), "eps"), (dict(q_weight=w.cpu()), "CPU"),
+    ]
+    for change, message in refused:
+        args = dict(q=x, k=x, positions=p, inv_freq=f) | change
+        with pytest.raises(RuntimeError, match=message):
+            race.race_norm_rope(**args)
+
+
+def test_other_stream_and_captured_steps(race, cuda):
+    q, k, qw, kw, dq, dk = make(2, 300, 4, 2, 64, torch.bfloat16, 10, cuda)
+    freq, pos = freqs(32, cuda), torch.arange(300, device=cuda)
+    leaves = [t.contiguous().requires_grad_(True) for t in (q, k, qw, kw)]
+
+    def step():
+        outs = race.race_norm_rope(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[3])
+        return (*(o.detach() for o in outs), *torch.autograd.grad(outs, leaves, (dq, dk)))
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(3):
+        new = make(2, 300, 4, 2, 64, torch.bfloat16, 20 + i, cuda)
+        with torch.no_grad():
+            for leaf, t in zip(leaves, new):
+                leaf.copy_(t)
+        pos.add_(1000)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager)), i
+
+
+def test_a_live_eager_graph_refuses_the_capture(race, cuda):
+    # The backward would wait for the default stream inside the capture.
+    q, _, _, _, dq, _ = make(1, 40, 2, 1, 64, torch.float32, 11, cuda)
+    leaf = q.contiguous().requires_grad_(True)
+    freq, pos = freqs(32, cuda), torch.arange(40, device=cuda)
+    run = lambda: race.race_norm_rope(leaf, None, pos, freq)[0]
+    eager = run()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            dq.mul(2)  # something to record
+            run()
+    want = torch.autograd.grad(eager, leaf, dq)[0]
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (got,) = torch.autograd.grad(run(), leaf, dq)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.skip(reason="torch's autograd engine runs the backward of an eagerly built graph on the stream of its "
+                  "forward and ties that stream to the capture before any node runs: the process ends at the end of "
+                  "the capture, whatever the op does.  A forward and its backward are captured together.")
+def test_the_backward_of_an_eager_graph_in_a_capture(race, cuda):
+    q, _, _, _, dq, _ = make(1, 40, 2, 1, 64, torch.float32, 11, cuda)
+    leaf = q.contiguous().requires_grad_(True)
+    eager, _ = race.race_norm_rope(leaf, None, torch.arange(40, device=cuda), freqs(32, cuda))
+    with pytest.raises(RuntimeError):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(eager, leaf, dq)
+
+
+def test_offsets_past_32_bits(race, cuda):
+    # 5.2 GB of rows: the last tokens against those tokens alone.
+    T, H, d = 40000, 128, 256
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    x = torch.randn(1, T, H, d, generator=gen, device=cuda)
+    freq, pos = freqs(128, cuda), torch.arange(T, device=cuda)
+    out, _ = race.race_norm_rope(x, None, pos, freq)
+    tail, _ = race.race_norm_rope(x[:, -64:], None, pos[-64:], freq)
+    assert torch.equal(out[:, -64:], tail)
+    del out
+    up = torch.randn(H, T, d, generator=gen, device=cuda)
+    leaf = x.requires_grad_(True)
+    out, _ = race.race_norm_rope(leaf, None, pos, freq)
+    (g,) = torch.autograd.grad(out, leaf, up)
+    del out
+    part = x.detach()[:, -64:].clone().requires_grad_(True)
+    out, _ = race.race_norm_rope(part, None, pos[-64:], freq)
+    assert torch.equal(g[:, -64:], torch.autograd.grad(out, part, up[:, -64:].contiguous())[0])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("options", [dict(qk_norm=True), dict(rope_pairs=32), dict(qk_norm=True, rope_pairs=16,
+                                                                                  rope_sections=[4, 6, 6])])
+def test_module_with_norm_and_rotation(race, cuda, causal, options):
+    # The module's own parts one after another: the same kernels, the same bits.
+    torch.manual_seed(0)
+    M, B, T, H, d, K, L = 1, 2, 200, 3, 64, 4, 4
+    module = race.BatchedACE(d, K, L, M, device=cuda, causal=causal, **options)
+    rows = [torch.randn(M, B, T, H, d, device=cuda, requires_grad=True) for _ in range(3)]
+    sections = options.get("rope_sections")
+    pos = torch.randint(0, 500, (len(sections), M * B, T) if sections else (M * B, T), device=cuda)
+    out = module(*rows, positions=pos)
+    assert out.shape == (M, B, T, H, d)
+    up = torch.randn_like(out)
+    weights = [p for p in module.parameters()]
+    assert len(weights) == (2 if options.get("qk_norm") else 0)
+    grads = torch.autograd.grad(out, rows + weights, up)
+    q2, k2 = race.race_norm_rope(rows[2][0], rows[0][0], pos, module.inv_freq(cuda), q_weight=module.q_norm,
+                                 k_weight=module.k_norm, eps=1e-6 if options.get("qk_norm") else None,
+                                 sections=sections)
+    v2 = rows[1][0].transpose(1, 2).reshape(B * H, T, d)
+    if causal:
+        want = race.race_fused_fwd_hashed(k2, q2, v2, module.planes_T.t().contiguous(), L)
+    else:
+        want = race.race_fused_fwd(race.race_hash_probs(q2, module.planes_T, L, K),
+                                   race.race_hash_probs(k2, module.planes_T, L, K), v2, False)
+    want = want.view(1, B, H, T, d).transpose(2, 3)
+    assert torch.equal(out, want)
+    for g, w in zip(grads, torch.autograd.grad(want, rows + weights, up)):
+        assert torch.equal(g, w)
+    assert sorted(module.state_dict()) == sorted(["planes_T", "protos_T"] + ["q_norm", "k_norm"] * bool(weights))

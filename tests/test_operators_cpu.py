@@ -54,3 +54,28 @@ def test_scan_binding_validates_inputs_on_the_host(race):
         race.race_gated_scan_carry(x, x, torch.zeros(2, 8))
     with pytest.raises(ValueError, match="gate_form"):
         race.race_gated_scan(x, x, gate_form="tanh")
+
+
+def test_norm_rope_refuses_on_the_host(race):
+    from race_attention_kernel_amd import abi
+
+    bad = abi.RACE_ERROR_INVALID_VALUE
+    ok = abi.norm_rope_shape(2, 300, 12, 4, 64, 32)
+    st, nbytes = abi.norm_rope_bwd_workspace_bytes(ok)
+    assert st == abi.RACE_SUCCESS and nbytes == 2048 * 64 * 4
+    for kw in (dict(B=-1), dict(T=-1), dict(B=1 << 16, T=1 << 15), dict(Hq=0), dict(Hk=-1), dict(d=0, pairs=0),
+               dict(d=257), dict(pairs=33), dict(pairs=-1), dict(sections=[16, 15]), dict(sections=[33, -1]),
+               dict(pos_bits=16), dict(eps=-1.0), dict(eps=float("nan")), dict(dtype=2), dict(weight_dtype=3)):
+        args = dict(B=2, T=300, Hq=12, Hk=4, d=64, pairs=32) | kw
+        assert abi.norm_rope_bwd_workspace_bytes(abi.norm_rope_shape(**args))[0] == bad, kw
+    assert abi.norm_rope_fwd(0, 16, 16, 16, None, None, 16, 16, ok, 0) == bad
+    assert abi.norm_rope_fwd(16, 16, None, 16, None, None, 16, 16, ok, 0) == bad
+    assert abi.norm_rope_fwd(16, 16, 16, 16, 4, None, 16, 16, ok, 0) == bad
+    assert abi.norm_rope_fwd(16, None, 16, 16, None, None, 16, None, ok, 0) == bad
+    assert abi.norm_rope_bwd(16, 16, 16, 16, None, None, 16, 16, 16, 16, 16, None, ok, None, 0, 0) == bad
+    # Nothing to do touches no device.
+    assert abi.norm_rope_fwd(0, None, None, None, None, None, 0, None, abi.norm_rope_shape(0, 5, 1, 0, 64, 32), 0) == 0
+    assert abi.norm_rope_bwd(16, 16, 16, 16, None, None, None, None, 16, 16, None, None, ok, None, 0, 0) == 0
+    x = torch.zeros(1, 2, 3, 64)
+    with pytest.raises(RuntimeError, match="race_norm_rope: q lives on the CPU"):
+        race.race_norm_rope(x, x)
