@@ -90,9 +90,27 @@ struct RopeArgs {
     float eps;
 };
 
-__device__ __forceinline__ float weight_at(const RopeTensor& t, int w_f32, int c) {
-    if (!t.w) return 1.f;
-    return w_f32 ? static_cast<const float*>(t.w)[c] : to_f32(static_cast<const bf16_t*>(t.w)[c]);
+// Weights c .. c + V - 1 (ones without any), zeros where `in` is false.
+template <int V>
+__device__ __forceinline__ void load_weights(float (&x)[V], const RopeTensor& t, int w_f32, int c, bool in) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = in ? 1.f : 0.f;
+    if (!t.w || !in) return;
+    if (w_f32) {
+        constexpr int kPer = V >= 4 ? 4 : 1;
+#pragma unroll
+        for (int i = 0; i < V; i += kPer) {
+            Run<float, kPer> r;
+            r.load(static_cast<const float*>(t.w) + c + i);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) x[i + j] = r.get(j);
+        }
+    } else {
+        Run<bf16_t, V> r;
+        r.load(static_cast<const bf16_t*>(t.w) + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = r.get(i);
+    }
 }
 
 // Floats of one token's cosines and sines; the four more spread the tokens'
@@ -227,11 +245,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const RopeArgs a) {
     float w1[NS][V], w2[NS][V];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            w1[j][i] = ln.one[j] ? weight_at(t, a.w_f32, ln.o1[j] + i) : 0.f;
-            w2[j][i] = ln.two[j] ? weight_at(t, a.w_f32, ln.o2[j] + i) : 0.f;
-        }
+        load_weights<V>(w1[j], t, a.w_f32, ln.o1[j], ln.one[j]);
+        load_weights<V>(w2[j], t, a.w_f32, ln.o2[j], ln.two[j]);
     }
     for (int ti = blockIdx.x; ti < tiles; ti += gridDim.x) {
         const int first = ti << t.tile_shift;
@@ -303,12 +318,10 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(const RopeArgs 
     float w1[NS][V], w2[NS][V], dw1[NS][V], dw2[NS][V];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
+        load_weights<V>(w1[j], t, a.w_f32, ln.o1[j], ln.one[j]);
+        load_weights<V>(w2[j], t, a.w_f32, ln.o2[j], ln.two[j]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            w1[j][i] = ln.one[j] ? weight_at(t, a.w_f32, ln.o1[j] + i) : 0.f;
-            w2[j][i] = ln.two[j] ? weight_at(t, a.w_f32, ln.o2[j] + i) : 0.f;
-            dw1[j][i] = dw2[j][i] = 0.f;
-        }
+        for (int i = 0; i < V; ++i) dw1[j][i] = dw2[j][i] = 0.f;
     }
     for (int ti = blockIdx.x; ti < tiles; ti += gridDim.x) {
         const int first = ti << t.tile_shift;
@@ -463,9 +476,14 @@ struct RopePlan {
     int rows_each;  // NR
 };
 
-// A lane group takes four rows where that leaves kRopeEnough workgroups; the
-// backward runs at most kRopeBwdWorkgroups.
-constexpr int kRopeEnough = 512, kRopeBwdWorkgroups = 2048;
+// A lane group takes two rows where that leaves kRopeEnough workgroups (of 1 x
+// 16384 tokens of 32 + 8 heads of 128 in bf16, forward: 69 us; one row 123, four
+// rows 77, whose registers leave fewer waves).  The workgroups stay for several
+// tiles: 3072 forward (69 us; one tile each 75), and backward two rounds of what
+// is resident (bf16 two rounds of three per CU: 8 x 8192 tokens of 16 + 16 heads
+// of 64 165 us, 1280 workgroups 179, 2048 178; fp32 one of four: 32 x 1024 tokens
+// of 12 + 12 heads of 64 119 us, 1536 workgroups 138).
+constexpr int kRopeEnough = 512, kRopeFwdWorkgroups = 3072, kRopeBwdWorkgroups = 1536, kRopeBwdWorkgroupsF32 = 1024;
 constexpr int kRopeTableBytes = 64 * 1024;
 
 RopePlan rope_plan(const NormRope& r, const void* const (&x)[2], const void* const (&w)[2], bool backward) {
@@ -480,7 +498,7 @@ RopePlan rope_plan(const NormRope& r, const void* const (&x)[2], const void* con
     a.lane_shift = v == 1 ? 5 : log2_up((slots + v - 1) / v);
     const int lane_groups = kThreads >> a.lane_shift;
     const int64_t rows = int64_t(a.tokens) * (r.heads[0] + r.heads[1]);
-    p.rows_each = v > 1 && rows >= int64_t(4) * lane_groups * kRopeEnough ? 4 : 1;
+    p.rows_each = v > 1 && rows >= int64_t(2) * lane_groups * kRopeEnough ? 2 : 1;
     const int wg_rows = lane_groups * p.rows_each;
     int64_t most_tiles = 0;
     int groups = 0, tile_tokens = 0;
@@ -502,10 +520,9 @@ RopePlan rope_plan(const NormRope& r, const void* const (&x)[2], const void* con
         tile_tokens = std::max(tile_tokens, 1 << t.tile_shift);
         most_tiles = std::max<int64_t>(most_tiles, (a.tokens + (1 << t.tile_shift) - 1) >> t.tile_shift);
     }
-    // The forward's workgroups take a tile each; the backward's a share of the
-    // tiles, with one partial row of the weights' gradients.
-    const int64_t most_wgs = backward ? std::max(1, kRopeBwdWorkgroups / std::max(groups, 1)) : int64_t(1) << 20;
-    p.grid = dim3(unsigned(std::min(most_tiles, most_wgs)), unsigned(groups));
+    // The backward's workgroups leave one partial row each of the weights' gradients.
+    const int wgs = !backward ? kRopeFwdWorkgroups : r.dtype == RACE_BF16 ? kRopeBwdWorkgroups : kRopeBwdWorkgroupsF32;
+    p.grid = dim3(unsigned(std::min<int64_t>(most_tiles, std::max(1, wgs / std::max(groups, 1)))), unsigned(groups));
     p.lds = sizeof(float) * std::max<int64_t>(int64_t(tile_tokens) * table_pitch(r.pairs),
                                               backward ? int64_t(lane_groups) * r.d : 4);
     return p;
@@ -522,9 +539,9 @@ void launch_rope(const RopePlan& p, bool backward, hipStream_t stream) {
 template <typename TIn, int V, int NS>
 void launch_rope_v(const NormRope& r, const RopePlan& p, bool backward, hipStream_t stream) {
     if constexpr (V > 1) {
-        if (p.rows_each == 4) {
-            if (r.interleaved) return launch_rope<TIn, V, NS, 4, true>(p, backward, stream);
-            return launch_rope<TIn, V, NS, 4, false>(p, backward, stream);
+        if (p.rows_each == 2) {
+            if (r.interleaved) return launch_rope<TIn, V, NS, 2, true>(p, backward, stream);
+            return launch_rope<TIn, V, NS, 2, false>(p, backward, stream);
         }
     }
     if (r.interleaved) return launch_rope<TIn, V, NS, 1, true>(p, backward, stream);

@@ -50,14 +50,11 @@ class GatedScanFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gate, state, lengths, form, complement):
-        needs = any(ctx.needs_input_grad[:3])
-        if needs:
-            _lib.ext().check_capture("race_gated_scan", [x, gate, state])
-        out, final, records = _lib.ext().gated_scan_forward(x, gate, state, lengths, form, complement, needs, False)
+        _lib.ext().check_capture("race_gated_scan", [x, gate, state])
+        out, final, records = _lib.ext().gated_scan_forward(x, gate, state, lengths, form, complement, True, False)
         ctx.set_materialize_grads(False)
-        if needs:
-            ctx.save_for_backward(x, gate, lengths, records)
-            ctx.args = (form, complement)
+        ctx.save_for_backward(x, gate, lengths, records)
+        ctx.args = (form, complement)
         return out, final
 
     @staticmethod
@@ -92,8 +89,10 @@ def race_gated_scan(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | N
     Returns out [N, T, D] in x's dtype and the float32 state [N, D] after the
     last token.  Sums are in float32.  Differentiable w.r.t. x, gate and state,
     through out and final."""
-    return GatedScanFunction.apply(_channel_rows(x), _channel_rows(gate), state, _lengths(lengths),
-                                   _form_id(gate_form), bool(complement))
+    x, gate, lengths, form = _channel_rows(x), _channel_rows(gate), _lengths(lengths), _form_id(gate_form)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (state is not None and state.requires_grad)):
+        return GatedScanFunction.apply(x, gate, state, lengths, form, bool(complement))
+    return _lib.ext().gated_scan_forward(x, gate, state, lengths, form, bool(complement), False, False)[:2]
 
 
 def race_gated_scan_carry(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, gate_form: str = "sigmoid",

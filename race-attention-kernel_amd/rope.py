@@ -30,14 +30,12 @@ class NormRopeFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, inv_freq, eps, norm, sections, interleaved):
-        if any(ctx.needs_input_grad[:4]):
-            _lib.ext().check_capture("race_norm_rope", [q, k, q_weight, k_weight])
+        _lib.ext().check_capture("race_norm_rope", [q, k, q_weight, k_weight])
         out_q, out_k = _lib.ext().norm_rope_forward(q, k, positions, inv_freq, q_weight, k_weight, eps, norm, sections,
                                                     interleaved)
         ctx.set_materialize_grads(False)
-        if any(ctx.needs_input_grad[:4]):
-            ctx.save_for_backward(q, k, q_weight, k_weight, positions, inv_freq)
-            ctx.args = (eps, norm, sections, interleaved)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, inv_freq)
+        ctx.args = (eps, norm, sections, interleaved)
         return out_q, out_k
 
     @staticmethod
@@ -75,6 +73,9 @@ def race_norm_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Ten
 
     Returns streams [B * Hq, T, d] and [B * Hk, T, d] (or None) in q's dtype.
     Differentiable w.r.t. q, k and the weights."""
-    return NormRopeFunction.apply(_rows(q), None if k is None else _rows(k), q_weight, k_weight, positions, inv_freq,
-                                  0.0 if eps is None else float(eps), eps is not None,
-                                  [int(s) for s in sections] if sections is not None else [], bool(interleaved))
+    q, k = _rows(q), None if k is None else _rows(k)
+    options = (0.0 if eps is None else float(eps), eps is not None, list(sections) if sections is not None else [],
+               bool(interleaved))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return NormRopeFunction.apply(q, k, q_weight, k_weight, positions, inv_freq, *options)
+    return _lib.ext().norm_rope_forward(q, k, positions, inv_freq, q_weight, k_weight, *options)

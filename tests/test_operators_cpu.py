@@ -62,7 +62,7 @@ def test_norm_rope_refuses_on_the_host(race):
     bad = abi.RACE_ERROR_INVALID_VALUE
     ok = abi.norm_rope_shape(2, 300, 12, 4, 64, 32)
     st, nbytes = abi.norm_rope_bwd_workspace_bytes(ok)
-    assert st == abi.RACE_SUCCESS and nbytes == 2048 * 64 * 4
+    assert st == abi.RACE_SUCCESS and nbytes == 1536 * 64 * 4
     for kw in (dict(B=-1), dict(T=-1), dict(B=1 << 16, T=1 << 15), dict(Hq=0), dict(Hk=-1), dict(d=0, pairs=0),
                dict(d=257), dict(pairs=33), dict(pairs=-1), dict(sections=[16, 15]), dict(sections=[33, -1]),
                dict(pos_bits=16), dict(eps=-1.0), dict(eps=float("nan")), dict(dtype=2), dict(weight_dtype=3)):
