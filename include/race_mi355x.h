@@ -512,6 +512,52 @@ race_status race_causal_bwd_profiled(const void* probsQ, const void* probsK, con
                                      void* workspace, size_t workspace_bytes, hipStream_t stream,
                                      hipEvent_t* events, int32_t max_events, int32_t* n_events);
 
+/* ---- The non-causal op between two sequences (cross attention) -----------
+ * The queries of one sequence over the keys and values of another (an
+ * encoder's), of its own length:
+ *     out[t] = sum_s probsQ[t,s] * B[s,:] / (A[s] + 1e-6),
+ * A, B summed over the first lengths[n] of the kv_len keys; a sequence without
+ * keys gives zeros.  The sums are the whole of what the queries need: kept as a
+ * state they serve every later query (race_cross_query).  Query heads that share
+ * a key head are its consecutive streams, read as one run of q_len tokens.  The
+ * reference's non-causal op (analysis/hot-path.md:157-162) has one length. */
+typedef struct race_cross_shape {
+    int64_t kv_streams;  /* streams of keys, <= 65535 */
+    int64_t q_len;       /* query tokens per key stream, all sharing heads together */
+    int64_t kv_len;
+    int32_t num_tables, num_buckets, head_dim;
+    int32_t dtype;         /* race_dtype of every token tensor */
+    int32_t lengths_group; /* key streams that share one entry of `lengths`, >= 1 */
+} race_cross_shape;
+
+/* Calls of at most this many query tokens per key stream read the state
+ * straight (race_cross_query's small launch). */
+#define RACE_CROSS_QUERY_TOKENS 16
+
+race_status race_cross_fwd_workspace_bytes(const race_cross_shape* shape, size_t* bytes);
+
+/* probsQ [kv_streams][q_len][S], probsK [kv_streams][kv_len][S], V, out alike
+ * with d columns.  lengths (nullable): int32, one per lengths_group key streams;
+ * keys from lengths on are not read (a value outside 0 .. kv_len counts as the
+ * nearer end).  out NULL: the state alone.  state (nullable): [kv_streams]
+ * [S*d + S] fp32, as race_fwd's. */
+race_status race_cross_fwd(const void* probsQ, const void* probsK, const void* V, const int32_t* lengths, void* out,
+                           float* state, const race_cross_shape* shape, void* workspace, size_t workspace_bytes,
+                           hipStream_t stream);
+
+/* out for queries against a kept state (kv_len is not used). */
+race_status race_cross_query(const void* probsQ, const float* state, void* out, const race_cross_shape* shape,
+                             hipStream_t stream);
+
+race_status race_cross_bwd_workspace_bytes(const race_cross_shape* shape, size_t* bytes);
+
+/* Gradients for the upstream gradient dOut, from the forward's inputs and
+ * state; dK and dV are zero in the rows from lengths on.  Any of dQ, dK, dV may
+ * be NULL to skip it. */
+race_status race_cross_bwd(const void* probsQ, const void* probsK, const void* V, const int32_t* lengths,
+                           const void* dOut, const float* state, void* dQ, void* dK, void* dV,
+                           const race_cross_shape* shape, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* ---- Norm and rotation of query and key heads ----------------------------
  * In front of the hashing: every row of the query and key heads divided by its
  * root mean square, times a weight per column, and its first 2 * pairs values

@@ -6,6 +6,7 @@ through the _race_torch binding.  There is no CPU fallback.
 """
 from . import causal_v2
 from .batched_ace import BatchedACE
+from .cross import CrossACE, CrossFunction, race_cross_fwd, race_cross_query, race_cross_state
 from .inputs import CONFIGS, Config, config_inputs, make_inputs
 from .ops import (HashedRaceFunction, HashProbsFunction, RaceFusedFunction, hashed_supported,
                   race_causal_backward, race_fused_fwd, race_fused_fwd_carry, race_fused_fwd_hashed,
@@ -19,6 +20,7 @@ __all__ = [
     "race_fused_fwd", "race_fused_fwd_carry", "race_fused_fwd_with_state", "race_noncausal_backward",
     "race_causal_backward", "race_fused_fwd_hashed", "hashed_supported", "HashedRaceFunction",
     "HashProbsFunction", "race_hash_probs", "select_tile_tokens", "causal_v2",
+    "CrossACE", "CrossFunction", "race_cross_fwd", "race_cross_query", "race_cross_state",
     "NormRopeFunction", "race_norm_rope",
     "GatedScanFunction", "race_gated_scan", "race_gated_scan_carry",
 ]

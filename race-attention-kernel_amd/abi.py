@@ -26,6 +26,7 @@ RACE_KERNEL_SINGLE = 5
 RACE_KERNEL_MFMA_PRECISE = 6
 RACE_DECODE_TOKENS = 16
 RACE_SUB_CHUNK_TOKENS = 64
+RACE_CROSS_QUERY_TOKENS = 16
 RACE_GATE_SIGMOID = 0
 RACE_GATE_LOG = 1
 RACE_ALG1_FP32 = 0
@@ -68,6 +69,11 @@ EXPORTED_SYMBOLS = (
     "race_alg1_fwd",
     "race_alg1_fwd_carry",
     "race_alg1_fwd_profiled",
+    "race_cross_fwd_workspace_bytes",
+    "race_cross_fwd",
+    "race_cross_query",
+    "race_cross_bwd_workspace_bytes",
+    "race_cross_bwd",
     "race_norm_rope_fwd",
     "race_norm_rope_bwd_workspace_bytes",
     "race_norm_rope_bwd",
@@ -100,6 +106,19 @@ class RaceShape(ctypes.Structure):
 
 class RaceOptions(ctypes.Structure):
     _fields_ = [("tile_tokens", ctypes.c_int32), ("kernel", ctypes.c_int32)]
+
+
+class RaceCrossShape(ctypes.Structure):
+    _fields_ = [
+        ("kv_streams", ctypes.c_int64),
+        ("q_len", ctypes.c_int64),
+        ("kv_len", ctypes.c_int64),
+        ("num_tables", ctypes.c_int32),
+        ("num_buckets", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("lengths_group", ctypes.c_int32),
+    ]
 
 
 class RaceNormRopeShape(ctypes.Structure):
@@ -195,6 +214,12 @@ def lib() -> ctypes.CDLL:
         L.race_alg1_fwd_carry.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, a1, i32, i32, vp, sz, vp]
         L.race_alg1_fwd_profiled.argtypes = [vp, vp, vp, vp, vp, vp, vp, a1, i32, i32, vp, sz, vp,
                                              ctypes.POINTER(vp), i32, ctypes.POINTER(i32)]
+        cs = ctypes.POINTER(RaceCrossShape)
+        L.race_cross_fwd_workspace_bytes.argtypes = [cs, ctypes.POINTER(sz)]
+        L.race_cross_fwd.argtypes = [vp, vp, vp, vp, vp, vp, cs, vp, sz, vp]
+        L.race_cross_query.argtypes = [vp, vp, vp, cs, vp]
+        L.race_cross_bwd_workspace_bytes.argtypes = [cs, ctypes.POINTER(sz)]
+        L.race_cross_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, cs, vp, sz, vp]
         nr = ctypes.POINTER(RaceNormRopeShape)
         L.race_norm_rope_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, nr, vp]
         L.race_norm_rope_bwd_workspace_bytes.argtypes = [nr, ctypes.POINTER(sz)]
@@ -524,3 +549,33 @@ def norm_rope_bwd(q: int, k: int | None, positions: int | None, inv_freq: int | 
     """race_norm_rope_bwd on raw device addresses; returns the status."""
     return lib().race_norm_rope_bwd(q, k, positions, inv_freq, q_weight, k_weight, dq_out, dk_out, dq, dk, dq_weight,
                                     dk_weight, ctypes.byref(sh), workspace, workspace_bytes, stream)
+
+
+def cross_shape(kv_streams: int, q_len: int, kv_len: int, L: int, R: int, d: int, dtype: int = RACE_F32,
+                lengths_group: int = 1) -> RaceCrossShape:
+    return RaceCrossShape(kv_streams, q_len, kv_len, L, R, d, dtype, lengths_group)
+
+
+def cross_workspace_bytes(sh: RaceCrossShape, backward: bool = False):
+    """(status, bytes) of race_cross_fwd, or race_cross_bwd."""
+    b = ctypes.c_size_t(0)
+    f = lib().race_cross_bwd_workspace_bytes if backward else lib().race_cross_fwd_workspace_bytes
+    return f(ctypes.byref(sh), ctypes.byref(b)), b.value
+
+
+def cross_fwd(q: int | None, k: int, v: int, lengths: int | None, out: int | None, state: int | None,
+              sh: RaceCrossShape, workspace: int | None, workspace_bytes: int, stream: int) -> int:
+    """race_cross_fwd on raw device addresses; returns the status."""
+    return lib().race_cross_fwd(q, k, v, lengths, out, state, ctypes.byref(sh), workspace, workspace_bytes, stream)
+
+
+def cross_query(q: int, state: int, out: int, sh: RaceCrossShape, stream: int) -> int:
+    """race_cross_query on raw device addresses; returns the status."""
+    return lib().race_cross_query(q, state, out, ctypes.byref(sh), stream)
+
+
+def cross_bwd(q: int, k: int, v: int, lengths: int | None, g: int, state: int, dq: int | None, dk: int | None,
+              dv: int | None, sh: RaceCrossShape, workspace: int | None, workspace_bytes: int, stream: int) -> int:
+    """race_cross_bwd on raw device addresses; returns the status."""
+    return lib().race_cross_bwd(q, k, v, lengths, g, state, dq, dk, dv, ctypes.byref(sh), workspace, workspace_bytes,
+                                stream)

@@ -136,16 +136,10 @@ __device__ __forceinline__ void open_gate(float g, float& a, float& b) {
 struct ScanGeo {
     int64_t T, D;
     int64_t xn, xt, gn, gt;  // strides of x and the gates, in elements
-    const int32_t* lengths;  // nullable: live tokens of streams group n .. group n + group - 1
-    int64_t group;
+    Live live;
     int64_t seg_len;  // tokens per segment, whole tiles
     int segs;
     int64_t tiles;    // records of a stream
-    __device__ __forceinline__ int64_t live(int64_t n) const {
-        if (!lengths) return T;
-        const int64_t len = lengths[n / group];
-        return len < 0 ? 0 : len < T ? len : T;
-    }
 };
 
 struct ScanFwdArgs {
@@ -270,7 +264,7 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
     const int seg = blockIdx.z;
     const int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
     const bool mine = c < D;
-    const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live(n));
+    const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live.of(n, g.T));
     const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn;
     const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn;
     TIn* op = static_cast<TIn*>(a.out) + n * g.T * D;
@@ -383,7 +377,7 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
     const int seg = blockIdx.z;
     const int64_t c = (int64_t(blockIdx.x) * CL + cl) * V;
     const bool mine = c < D;
-    const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live(n));
+    const int64_t t0 = seg * g.seg_len, t1 = min(g.T, t0 + g.seg_len), end = min(t1, g.live.of(n, g.T));
     const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn;
     const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn;
     const TIn* yp = static_cast<const TIn*>(a.dout) + n * g.T * D;
@@ -547,7 +541,7 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(const ScanGeo g, co
     const int64_t per = g.D / V, i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
     if (i >= N * per) return;
     const int64_t n = i / per, c = (i - n * per) * V;
-    const int64_t end = g.live(n);
+    const int64_t end = g.live.of(n, g.T);
     const TIn* xp = static_cast<const TIn*>(a.x) + n * g.xn + c;
     const TIn* gp = static_cast<const TIn*>(a.gate) + n * g.gn + c;
     TIn* op = static_cast<TIn*>(a.out) + n * g.T * g.D + c;
@@ -625,8 +619,7 @@ ScanGeo geometry(const GatedScan& s) {
     g.T = s.T;
     g.D = s.D;
     g.xn = s.xn, g.xt = s.xt, g.gn = s.gn, g.gt = s.gt;
-    g.lengths = s.lengths;
-    g.group = s.group;
+    g.live = s.live;
     g.tiles = scan_tiles(s);
     g.segs = int(scan_segments(s));
     const int64_t tile = forward_tile(s);

@@ -229,7 +229,7 @@ struct Outer {
 template <typename TIn, int EA, int EB, bool kEndFirst>
 __global__ __launch_bounds__(kThreads, 3) void nc_sums_kernel(
     const TIn* __restrict__ x, const TIn* __restrict__ y, float* __restrict__ records, int64_t T, int chunk,
-    int64_t chunks, int64_t rec, int Wa, int Wb, int bblocks, int kept) {
+    int64_t chunks, int64_t rec, int Wa, int Wb, int bblocks, int kept, const Live live) {
     extern __shared__ __align__(16) float smem[];
     constexpr int es = int(sizeof(TIn)), kTok = kStep<TIn>, kLoads = kTok / 4;
     const int lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kThreads, 3) void nc_sums_kernel(
     const int64_t n = blockIdx.y, ci = blockIdx.x;
     const int a0 = 16 * EA * int(blockIdx.z / bblocks), b0 = 16 * EB * int(blockIdx.z % bblocks);
     const int64_t t0 = ci * chunk;
-    const int rows = int(min(T, t0 + chunk) - t0);
+    const int rows = int(max(int64_t(0), min(live.of(n, T), t0 + chunk) - t0));
     const auto xr = mfma::make_rsrc(x + (n * T + t0) * Wa, int64_t(rows) * Wa * es);
     const auto yr = mfma::make_rsrc(y + (n * T + t0) * Wb, int64_t(rows) * Wb * es);
     const int ca = a0 + EA * lr, cb = b0 + EB * lr;
@@ -594,7 +594,7 @@ __device__ __forceinline__ void stream_block(int64_t id, int64_t N, int per, int
 template <typename TIn, int NJ, int NCB, bool kB16, int NW>
 __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__ x, TIn* __restrict__ out,
                                                           const MapOperand op, int64_t N, int64_t T, int Wa,
-                                                          int Wb, int wg_tokens, int per) {
+                                                          int Wb, int wg_tokens, int per, const Live live) {
     extern __shared__ __align__(16) float smem[];
     using X = MapRows<TIn, NJ, kB16>;
     using O = OutRows<TIn, NCB>;
@@ -609,8 +609,9 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
     stream_block(blockIdx.x, N, per, n, blk);
     const int64_t t0 = int64_t(blk) * wg_tokens;
     const int rows = int(min<int64_t>(T - t0, wg_tokens));
+    const int alive = int(max(int64_t(0), min<int64_t>(live.of(n, T) - t0, rows)));
     const int c0 = 16 * NCB * int(blockIdx.y), ncols = min(16 * NCB, Wb - c0);
-    const auto xr = mfma::make_rsrc(x + (n * T + t0) * Wa, int64_t(rows) * Wa * es);
+    const auto xr = mfma::make_rsrc(x + (n * T + t0) * Wa, int64_t(alive) * Wa * es);
     const auto orr = mfma::make_rsrc(out + (n * T + t0) * Wb, int64_t(rows) * Wb * es);
     auto load = [&](X& v, int row0) {
         if constexpr (kTurn) {
@@ -648,6 +649,10 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
         for (int cb = 0; cb < NCB; ++cb) acc[cb] = bias[cb];
         const uint64_t bad = cur.nonfinite();
         cur.template times<NCB>(smem, lane, acc);
+        if (r0 + lr >= alive) {  // a lane's sums are one token's
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb) acc[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
         typename O::Raw* to = reinterpret_cast<typename O::Raw*>(mine);
         O::store(to, acc, orr, r0, Wb, c0, ncols, lane, g, lr, [&] {
             if constexpr (kB16) {
@@ -767,7 +772,7 @@ __global__ __launch_bounds__(64 * NW) void nc_key64_kernel(
     const TIn* __restrict__ k, const TIn* __restrict__ v, TIn* __restrict__ dk, TIn* __restrict__ dv,
     const float* __restrict__ dE_records, int parts, int64_t rec, const float* __restrict__ state,
     const float* __restrict__ dB_ready, const float* __restrict__ dA_ready, int64_t N, int64_t T, int wg_tokens,
-    int per) {
+    int per, const Live live) {
     constexpr int W = 64, es = int(sizeof(TIn));
     constexpr bool kB16 = sizeof(TIn) == 2;
     using X = MapRows<TIn, 4, kB16>;
@@ -786,9 +791,11 @@ __global__ __launch_bounds__(64 * NW) void nc_key64_kernel(
     const int64_t t0 = int64_t(blk) * wg_tokens;
     const int rows = int(min<int64_t>(T - t0, wg_tokens));
     // A gradient that is not asked for: its rows are neither read nor written.
+    const int alive = int(max(int64_t(0), min<int64_t>(live.of(n, T) - t0, rows)));
     const int64_t kb = dv ? int64_t(rows) * W * es : 0, vb = dk ? int64_t(rows) * W * es : 0;
-    const auto kr = mfma::make_rsrc(dv ? k + (n * T + t0) * W : nullptr, kb);
-    const auto vr = mfma::make_rsrc(dk ? v + (n * T + t0) * W : nullptr, vb);
+    const int64_t ab = int64_t(alive) * W * es;
+    const auto kr = mfma::make_rsrc(dv ? k + (n * T + t0) * W : nullptr, dv ? ab : 0);
+    const auto vr = mfma::make_rsrc(dk ? v + (n * T + t0) * W : nullptr, dk ? ab : 0);
     const auto dkr = mfma::make_rsrc(dk ? dk + (n * T + t0) * W : nullptr, vb);
     const auto dvr = mfma::make_rsrc(dv ? dv + (n * T + t0) * W : nullptr, kb);
     X kn, vn;
@@ -872,6 +879,10 @@ __global__ __launch_bounds__(64 * NW) void nc_key64_kernel(
             for (int cb = 0; cb < 4; ++cb) acc[cb] = bias[cb];
             const uint64_t bad = vc.nonfinite();
             vc.template times<4>(Mk, lane, acc);
+            if (r0 + lr >= alive) {
+#pragma unroll
+                for (int cb = 0; cb < 4; ++cb) acc[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
             O::store(to, acc, dkr, r0, W, 0, W, lane, g, lr, [&] {
                 if constexpr (kB16) {
                     if (bad)
@@ -890,6 +901,10 @@ __global__ __launch_bounds__(64 * NW) void nc_key64_kernel(
             for (int cb = 0; cb < 4; ++cb) acc[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
             const uint64_t bad = kc.nonfinite();
             kc.template times<4>(Mv, lane, acc);
+            if (r0 + lr >= alive) {
+#pragma unroll
+                for (int cb = 0; cb < 4; ++cb) acc[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
             O::store(to, acc, dvr, r0, W, 0, W, lane, g, lr, [&] {
                 if constexpr (kB16) {
                     if (bad)
@@ -920,7 +935,7 @@ hipError_t launch_sums_e(const void* x, const void* y, float* records, const Pro
     const dim3 grid(unsigned(p.tiles), unsigned(p.N), unsigned(ab * bb));
     nc_sums_kernel<TIn, EA, EB, kEndFirst><<<grid, kThreads, Outer<EA, EB>::kLdsFloats * sizeof(float), stream>>>(
         static_cast<const TIn*>(x), static_cast<const TIn*>(y), records, p.T, p.tile, p.tiles, p.rec, Wa, Wb, bb,
-        kEndFirst ? cache_kept_rows(p) : 0);
+        kEndFirst ? cache_kept_rows(p) : 0, p.live);
     return hipGetLastError();
 }
 
@@ -946,7 +961,7 @@ hipError_t launch_map_b(const void* x, void* out, const MapOperand& op, const Pr
     constexpr size_t kTurn = NJ <= 8 ? MapRows<TIn, NJ, kB16>::kBytes : 0, kOut = OutRows<TIn, NCB>::kBytes;
     const size_t lds = kMatrixFloats<NJ, NCB, kB16> * sizeof(float) + NW * (kTurn > kOut ? kTurn : kOut);
     nc_map_kernel<TIn, NJ, NCB, kB16, NW><<<grid, 64 * NW, lds, stream>>>(static_cast<const TIn*>(x), static_cast<TIn*>(out),
-                                                                 op, p.N, p.T, Wa, Wb, wt, per);
+                                                                 op, p.N, p.T, Wa, Wb, wt, per, p.live);
     return hipGetLastError();
 }
 
@@ -1064,11 +1079,13 @@ hipError_t launch_nc_key64(const void* k, const void* v, void* dk, void* dv, con
     if (p.dtype == RACE_BF16)
         nc_key64_kernel<bf16_t, kMapWaves><<<grid, 64 * kMapWaves, lds, stream>>>(
             static_cast<const bf16_t*>(k), static_cast<const bf16_t*>(v), static_cast<bf16_t*>(dk),
-            static_cast<bf16_t*>(dv), dE_records, parts, p.rec, state, dB_ready, dA_ready, p.N, p.T, wt, per);
+            static_cast<bf16_t*>(dv), dE_records, parts, p.rec, state, dB_ready, dA_ready, p.N, p.T, wt, per,
+            p.live);
     else
         nc_key64_kernel<float, kMapWaves><<<grid, 64 * kMapWaves, lds, stream>>>(
             static_cast<const float*>(k), static_cast<const float*>(v), static_cast<float*>(dk),
-            static_cast<float*>(dv), dE_records, parts, p.rec, state, dB_ready, dA_ready, p.N, p.T, wt, per);
+            static_cast<float*>(dv), dE_records, parts, p.rec, state, dB_ready, dA_ready, p.N, p.T, wt, per,
+            p.live);
     return hipGetLastError();
 }
 

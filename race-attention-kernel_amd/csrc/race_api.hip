@@ -1696,7 +1696,7 @@ bool scan_shape(const race_scan_shape* sh, const int32_t* lengths, GatedScan* s)
     *s = GatedScan{sh->num_streams,        sh->seq_len,           sh->channels,
                    sh->x_stream_stride,    sh->x_token_stride,    sh->gate_stream_stride,
                    sh->gate_token_stride,  sh->dtype,             sh->gate_form,
-                   sh->complement != 0,    lengths,               sh->lengths_group};
+                   sh->complement != 0,    {lengths, sh->lengths_group}};
     return true;
 }
 
@@ -1869,6 +1869,210 @@ race_status race_norm_rope_bwd(const void* q, const void* k, const void* positio
     return launch_norm_rope_bwd(r, {use_q ? q : nullptr, use_k ? k : nullptr}, {q_weight, k_weight}, {dq_out, dk_out},
                                 {dq, dk}, {use_q ? dq_weight : nullptr, use_k ? dk_weight : nullptr},
                                 static_cast<float*>(workspace), stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// The non-causal op between two sequences (cross attention).
+
+namespace race {
+namespace {
+
+// Both sides of a call: `q` for the query tokens (those of the heads that share
+// a key stream one after another), `k` for the keys.  The token chunks of the
+// reductions depend on the shape alone.
+struct CrossProblem {
+    Problem q, k;
+};
+
+Problem cross_side(const race_cross_shape* sh, int64_t T) {
+    Problem p;
+    p.N = sh->kv_streams, p.T = T;
+    p.S = sh->num_tables * sh->num_buckets, p.d = sh->head_dim;
+    p.dtype = sh->dtype, p.kernel = RACE_KERNEL_AUTO;
+    p.rec = record_floats(p.S, p.d);
+    p.tile = RACE_SUB_CHUNK_TOKENS, p.tiles = 0;
+    if (p.N > 0 && T > 0) {
+        const int64_t per = nc_blocks_per_stream(p.N, T, p.dtype, kMaxAutoTileOther);
+        p.tile = int(((T + per - 1) / per + 15) / 16 * 16);
+        p.tiles = (T + p.tile - 1) / p.tile;
+    }
+    return p;
+}
+
+bool cross_problem(const race_cross_shape* sh, const int32_t* lengths, CrossProblem* c) {
+    if (!sh || sh->lengths_group < 1) return false;
+    for (int64_t T : {sh->q_len, sh->kv_len}) {
+        const race_shape one{sh->kv_streams, T, sh->num_tables, sh->num_buckets, sh->head_dim, sh->dtype};
+        if (!shape_ok(&one)) return false;
+    }
+    c->q = cross_side(sh, sh->q_len);
+    c->k = cross_side(sh, sh->kv_len);
+    c->k.live = Live{lengths, sh->lengths_group};
+    return true;
+}
+
+// Few queries read the state as it is; more go through a map, which stages it
+// once for many tokens.
+bool cross_few(const Problem& q) { return q.T <= RACE_CROSS_QUERY_TOKENS; }
+
+struct CrossFwdLayout {
+    int64_t records = 0, E = 0, state = 0;
+    int64_t total() const { return records + E + state; }
+};
+CrossFwdLayout cross_fwd_layout(const CrossProblem& c) {
+    CrossFwdLayout l;
+    l.records = c.k.N * c.k.tiles * c.k.rec;
+    l.E = round64(c.k.N * c.k.S * c.k.d);
+    l.state = round64(c.k.N * state_floats(c.k.S, c.k.d));
+    return l;
+}
+
+// The key side's problem with the query side's dE records.
+Problem with_records_of(const Problem& k, const Problem& q) {
+    Problem p = k;
+    p.tiles = q.tiles, p.rec = q.rec;
+    return p;
+}
+
+hipError_t zero_rows(void* p, int64_t elements, int dtype, hipStream_t stream) {
+    return p ? zero_bytes(p, size_t(elements) * (dtype == RACE_BF16 ? 2 : 4), stream) : hipSuccess;
+}
+
+// Queries against a state: the map with E = B / (A + eps) read straight from it.
+hipError_t cross_map(const void* probsQ, const float* state, void* out, const Problem& q, hipStream_t stream) {
+    if (cross_few(q)) return launch_cross_query(probsQ, state, out, q, stream);
+    const int64_t Sd = int64_t(q.S) * q.d;
+    MapOperand op = map_operand(state, Sd + q.S, q.d, 1);
+    op.div = state + Sd;
+    op.div_stream = Sd + q.S;
+    return token_map(probsQ, out, op, q, q.S, q.d, stream);
+}
+
+}  // namespace
+}  // namespace race
+
+extern "C" {
+
+race_status race_cross_fwd_workspace_bytes(const race_cross_shape* shape, size_t* bytes) {
+    CrossProblem c;
+    if (!cross_problem(shape, nullptr, &c) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    *bytes = c.k.N == 0 ? 0 : size_t(cross_fwd_layout(c).total()) * sizeof(float);
+    return RACE_SUCCESS;
+}
+
+race_status race_cross_fwd(const void* probsQ, const void* probsK, const void* V, const int32_t* lengths, void* out,
+                           float* state, const race_cross_shape* shape, void* workspace, size_t workspace_bytes,
+                           hipStream_t stream) {
+    CrossProblem c;
+    if (!cross_problem(shape, lengths, &c) || !aligned16(state)) return RACE_ERROR_INVALID_VALUE;
+    const Problem &q = c.q, &k = c.k;
+    const int64_t Sd = int64_t(q.S) * q.d;
+    if (q.N == 0) return RACE_SUCCESS;
+    const bool want_out = out && q.T > 0;
+    if (want_out && (!probsQ || !aligned16(probsQ) || !aligned16(out))) return RACE_ERROR_INVALID_VALUE;
+    if (k.T == 0) {  // no keys: every sum is zero
+        RACE_TRY(zero_fill(state, q.N * (Sd + q.S), stream));
+        return want_out ? zero_rows(out, q.N * q.T * q.d, q.dtype, stream) : hipSuccess;
+    }
+    if (!want_out && !state) return RACE_SUCCESS;
+    if (!probsK || !V || !aligned16(probsK) || !aligned16(V)) return RACE_ERROR_INVALID_VALUE;
+    const CrossFwdLayout l = cross_fwd_layout(c);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < size_t(l.total()) * sizeof(float))
+        return RACE_ERROR_INVALID_VALUE;
+    float* records = static_cast<float*>(workspace);
+    RACE_TRY(outer_sums(probsK, V, records, k, k.S, k.d, stream));
+    if (!want_out) return launch_tile_reduce(records, state, nullptr, k, stream);
+    if (cross_few(q)) {
+        float* sums = state ? state : records + l.records + l.E;
+        RACE_TRY(launch_tile_reduce(records, sums, nullptr, k, stream));
+        return launch_cross_query(probsQ, sums, out, q, stream);
+    }
+    if (k.tiles > kNcFoldParts) {
+        float* E = records + l.records;
+        RACE_TRY(launch_tile_reduce(records, state, E, k, stream));
+        return token_map(probsQ, out, map_operand(E, Sd, q.d, 1), q, q.S, q.d, stream);
+    }
+    // The map adds the records as it stages them and leaves the state.
+    MapOperand op = map_operand(records, k.tiles * k.rec, q.d, 1);
+    op.parts = int(k.tiles);
+    op.part_stride = k.rec;
+    op.div = records + Sd;
+    op.div_stream = k.tiles * k.rec;
+    op.save = state;
+    op.save_stream = Sd + q.S;
+    op.save_div_off = Sd;
+    return token_map(probsQ, out, op, q, q.S, q.d, stream);
+}
+
+race_status race_cross_query(const void* probsQ, const float* state, void* out, const race_cross_shape* shape,
+                             hipStream_t stream) {
+    CrossProblem c;
+    if (!cross_problem(shape, nullptr, &c)) return RACE_ERROR_INVALID_VALUE;
+    if (c.q.N == 0 || c.q.T == 0) return RACE_SUCCESS;
+    if (!probsQ || !state || !out || !aligned16(probsQ) || !aligned16(state) || !aligned16(out))
+        return RACE_ERROR_INVALID_VALUE;
+    return cross_map(probsQ, state, out, c.q, stream);
+}
+
+race_status race_cross_bwd_workspace_bytes(const race_cross_shape* shape, size_t* bytes) {
+    CrossProblem c;
+    if (!cross_problem(shape, nullptr, &c) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    *bytes = c.q.N == 0 ? 0 : size_t(bwd_layout(c.q).total()) * sizeof(float);
+    return RACE_SUCCESS;
+}
+
+race_status race_cross_bwd(const void* probsQ, const void* probsK, const void* V, const int32_t* lengths,
+                           const void* dOut, const float* state, void* dQ, void* dK, void* dV,
+                           const race_cross_shape* shape, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    CrossProblem c;
+    if (!cross_problem(shape, lengths, &c)) return RACE_ERROR_INVALID_VALUE;
+    const Problem &q = c.q, &k = c.k;
+    if (q.T == 0) dQ = nullptr;
+    if (k.T == 0) dK = dV = nullptr;
+    if (q.N == 0 || (!dQ && !dK && !dV)) return RACE_SUCCESS;
+    for (const void* p : {probsQ, probsK, V, dOut, static_cast<const void*>(state), static_cast<const void*>(dQ),
+                          static_cast<const void*>(dK), static_cast<const void*>(dV)})
+        if (!aligned16(p)) return RACE_ERROR_INVALID_VALUE;
+    if (q.T == 0) {  // no queries: nothing reaches the keys
+        RACE_TRY(zero_rows(dK, k.N * k.T * k.S, k.dtype, stream));
+        return zero_rows(dV, k.N * k.T * k.d, k.dtype, stream);
+    }
+    if (!state || !dOut || ((dK || dV) && !probsQ) || (dK && !V) || (dV && !probsK)) return RACE_ERROR_INVALID_VALUE;
+    const BwdLayout l = bwd_layout(q);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < size_t(l.total()) * sizeof(float))
+        return RACE_ERROR_INVALID_VALUE;
+    float* records = static_cast<float*>(workspace);
+    float* dB = records + l.records;
+    float* dA = dB + l.dB;
+    const int64_t Sd = int64_t(q.S) * q.d;
+    // dQ = dOut E^T, E from the state.
+    MapOperand et = map_operand(state, Sd + q.S, 1, q.d);
+    et.div = state + Sd;
+    et.div_stream = Sd + q.S;
+    et.div_by_col = true;
+    const bool w64 = q.S == 64 && q.d == 64;
+    if (w64 && dQ && (dK || dV)) {
+        RACE_TRY(launch_nc_query64(probsQ, dOut, dQ, state, records, q, stream));
+    } else {
+        if (dQ) RACE_TRY(token_map(dOut, dQ, et, q, q.d, q.S, stream));
+        if (!dK && !dV) return RACE_SUCCESS;
+        RACE_TRY(outer_sums(probsQ, dOut, records, q, q.S, q.d, stream));
+    }
+    if (!dK && !dV) return RACE_SUCCESS;
+    if (w64 && q.tiles <= kNcFoldParts)
+        return launch_nc_key64(probsK, V, dK, dV, records, state, nullptr, nullptr, with_records_of(k, q), stream);
+    RACE_TRY(launch_bwd_finalize(records, state, dB, dA, q, stream));
+    if (w64) return launch_nc_key64(probsK, V, dK, dV, nullptr, nullptr, dB, dA, k, stream);
+    if (dK) {
+        MapOperand op = map_operand(dB, Sd, 1, q.d);
+        op.bias = dA;
+        op.bias_stream = q.S;
+        RACE_TRY(token_map(V, dK, op, k, k.d, k.S, stream));
+    }
+    if (dV) RACE_TRY(token_map(probsK, dV, map_operand(dB, Sd, q.d, 1), k, k.S, k.d, stream));
+    return RACE_SUCCESS;
 }
 
 }  // extern "C"

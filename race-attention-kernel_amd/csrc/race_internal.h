@@ -42,6 +42,18 @@ inline int64_t record_floats(int64_t S, int64_t d) { return ((S * d + S + 63) / 
 constexpr int kGfx950LdsBytes = 160 * 1024;
 inline int64_t state_floats(int64_t S, int64_t d) { return S * d + S; }
 
+// Live tokens of a stream: lengths[n / group] of its T (padded batches), or all
+// of them without lengths.
+struct Live {
+    const int32_t* lengths = nullptr;
+    int64_t group = 1;
+    __device__ __forceinline__ int64_t of(int64_t n, int64_t T) const {
+        if (!lengths) return T;
+        const int64_t len = lengths[n / group];
+        return len < 0 ? 0 : len < T ? len : T;
+    }
+};
+
 // Problem description handed from the API layer to the launchers (all sizes
 // validated by the API layer before any launch).
 struct Problem {
@@ -56,6 +68,9 @@ struct Problem {
     // Causal forward continued from a carried state ([N][S*d+S], B then A):
     // the scan starts every stream from it instead of zero.  Null otherwise.
     const float* init = nullptr;
+    // Non-causal passes over keys: tokens past a stream's live ones are not
+    // read, add nothing and get zero gradients.
+    Live live;
 };
 
 // Optional hipEventRecord after each launch (race_fwd_profiled).
@@ -406,6 +421,11 @@ hipError_t launch_hash_rows(const void* x, const float* planes_T, const void* dp
 hipError_t launch_pack_heads(const void* const* src, void* const* dst, int count, int64_t batch, int64_t T, int H,
                              int row_bytes, hipStream_t stream);
 
+// ---- few queries against a kept state (cross_query.hip) ----
+// out[n][t][c] = sum_s q[n][t][s] B[n][s][c] / (A[n][s] + eps) for the states
+// [N][S*d + S] (B then A).
+hipError_t launch_cross_query(const void* q, const float* state, void* out, const Problem& p, hipStream_t stream);
+
 // ---- norm and rotation of query and key heads (norm_rope.hip) ----
 // Rows [B][T][heads][d] by strides (queries 0, keys 1; no keys: heads[1] = 0)
 // to streams [B * heads][T][d].
@@ -441,8 +461,7 @@ struct GatedScan {
     int dtype;               // race_dtype of x, gate, out and their gradients
     int form;                // race_gate
     bool complement;
-    const int32_t* lengths;  // nullable: live tokens, one per `group` streams
-    int64_t group;
+    Live live;
 };
 // Calls without records of at most this many tokens run one thread per piece of
 // a row, token by token.

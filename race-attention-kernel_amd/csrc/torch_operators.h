@@ -309,8 +309,131 @@ norm_rope_backward(const at::Tensor& q, const c10::optional<at::Tensor>& k, cons
     return {dq, dk, dqw, dkw};
 }
 
+// ---- the non-causal op between two sequences ----
+
+struct CrossCall {
+    race_cross_shape sh{};
+    int64_t S = 0, d = 0, Nq = 0, Tq = 0;
+};
+
+int64_t buckets_of(const at::Tensor& t) { return t.dim() == 4 ? t.size(2) * t.size(3) : t.size(2); }
+
+// q (nullable): [Nq, Tq, L, R] or [Nq, Tq, S]; k likewise and V [Nk, Tk, d], or
+// in their place a state [Nk, S*d + S].
+CrossCall cross_call(const char* entry, const at::Tensor* q, const at::Tensor* k, const at::Tensor* v,
+                     const at::Tensor* state, const c10::optional<at::Tensor>& lengths) {
+    ArgCheck c(entry);
+    CrossCall r;
+    const at::Tensor& ref = q ? *q : *k;
+    auto probs = [&](const char* name, const at::Tensor& t) {
+        c.on_gpu(name, t).dtype_is(name, t, true)
+            .require(t.dim() == 3 || t.dim() == 4, name, "has shape " + dims(t) + ", not [N, T, L, R] or [N, T, S]");
+    };
+    if (q) probs("probsQ", *q);
+    if (k) probs("probsK", *k);
+    c.raise();
+    r.S = buckets_of(ref);
+    int64_t Nk = 0;
+    if (k) {
+        Nk = k->size(0);
+        c.matches("probsK", *k, "probsQ", ref)
+            .require(buckets_of(*k) == r.S, "probsK", "has shape " + dims(*k) + ", another number of buckets than probsQ")
+            .on_gpu("V", *v).matches("V", *v, "probsK", *k)
+            .require(v->dim() == 3 && v->size(0) == Nk && v->size(1) == k->size(1), "V",
+                     "has shape " + dims(*v) + ", not [N, T, d] with probsK's N and T");
+        if (v->dim() == 3) r.d = v->size(2);
+        r.sh.kv_len = k->size(1);
+    } else {
+        c.on_gpu("state", *state)
+            .require(state->scalar_type() == at::kFloat && state->device() == ref.device(), "state",
+                     "must be float32 on probsQ's device")
+            .require(state->dim() == 2 && r.S > 0 && state->size(1) % r.S == 0 && state->size(1) / r.S >= 2, "state",
+                     "has shape " + dims(*state) + ", not [N, S*d + S] with probsQ's S");
+        c.raise();
+        Nk = state->size(0);
+        r.d = state->size(1) / r.S - 1;
+    }
+    r.Nq = q ? q->size(0) : Nk, r.Tq = q ? q->size(1) : 0;
+    c.require(Nk > 0 ? r.Nq % Nk == 0 : r.Nq == 0, "probsQ",
+              "has " + std::to_string(r.Nq) + " streams, no multiple of the " + std::to_string(Nk) + " key streams");
+    const int64_t group = check_lengths(c, lengths, ref, Nk);
+    const int64_t heads = Nk > 0 ? std::max<int64_t>(r.Nq / Nk, 1) : 1;
+    constexpr int64_t kMost = int64_t(1) << 30;
+    c.require(Nk <= 65535 && r.S >= 1 && r.S <= 256 && r.d >= 1 && r.d <= 128 && heads <= kMost && r.Tq <= kMost / heads &&
+                  r.sh.kv_len <= kMost,
+              "probsQ", "has no kernel: up to 65535 key streams, S <= 256 buckets, d <= 128 columns and 2^30 tokens a "
+                        "key stream are taken")
+        .raise();
+    r.sh.kv_streams = Nk, r.sh.q_len = r.Tq * heads;
+    r.sh.num_tables = 1, r.sh.num_buckets = static_cast<int32_t>(r.S), r.sh.head_dim = static_cast<int32_t>(r.d);
+    r.sh.dtype = dtype_of(ref), r.sh.lengths_group = static_cast<int32_t>(group);
+    return r;
+}
+
+const int32_t* lengths_of(const c10::optional<at::Tensor>& t) { return t ? t->data_ptr<int32_t>() : nullptr; }
+
+// (out or None, state or None).
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>> cross_forward(
+    const c10::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v,
+    const c10::optional<at::Tensor>& lengths, bool want_state) {
+    const CrossCall r = cross_call(q ? "race_cross_fwd" : "race_cross_state", q ? &*q : nullptr, &k, &v, nullptr, lengths);
+    const c10::DeviceGuard guard(k.device());
+    c10::optional<at::Tensor> out, state;
+    if (q) out = at::empty({r.Nq, r.Tq, r.d}, v.options());
+    if (want_state) state = at::empty({r.sh.kv_streams, r.S * r.d + r.S}, v.options().dtype(at::kFloat));
+    size_t bytes = 0;
+    check_status(race_cross_fwd_workspace_bytes(&r.sh, &bytes), "race_cross_fwd_workspace_bytes");
+    const at::Tensor ws = workspace_of(bytes, k);
+    check_status(race_cross_fwd(q ? q->data_ptr() : nullptr, k.data_ptr(), v.data_ptr(), lengths_of(lengths), ptr_of(out),
+                                floats_of(state), &r.sh, ws.data_ptr(), bytes, current_stream()),
+                 "race_cross_fwd");
+    return {out, state};
+}
+
+at::Tensor cross_query(const at::Tensor& q, const at::Tensor& state) {
+    const CrossCall r = cross_call("race_cross_query", &q, nullptr, nullptr, &state, c10::nullopt);
+    const c10::DeviceGuard guard(q.device());
+    const at::Tensor out = at::empty({r.Nq, r.Tq, r.d}, q.options());
+    check_status(race_cross_query(q.data_ptr(), state.data_ptr<float>(), out.data_ptr(), &r.sh, current_stream()),
+                 "race_cross_query");
+    return out;
+}
+
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<at::Tensor>> cross_backward(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths,
+    const at::Tensor& dout, const at::Tensor& state, bool need_q, bool need_k, bool need_v) {
+    const char* entry = "race_cross_fwd backward";
+    const CrossCall r = cross_call(entry, &q, &k, &v, nullptr, lengths);
+    ArgCheck(entry).on_gpu("dout", dout).matches("dout", dout, "V", v)
+        .require(dout.sizes() == at::IntArrayRef({r.Nq, r.Tq, r.d}), "dout", "has shape " + dims(dout))
+        .on_gpu("state", state)
+        .require(state.scalar_type() == at::kFloat && state.device() == q.device() &&
+                     state.sizes() == at::IntArrayRef({r.sh.kv_streams, r.S * r.d + r.S}),
+                 "state", "is not the forward's float32 [N, S*d + S] state")
+        .raise();
+    const c10::DeviceGuard guard(q.device());
+    c10::optional<at::Tensor> dq, dk, dv;
+    if (need_q) dq = at::empty_like(q);
+    if (need_k) dk = at::empty_like(k);
+    if (need_v) dv = at::empty_like(v);
+    size_t bytes = 0;
+    check_status(race_cross_bwd_workspace_bytes(&r.sh, &bytes), "race_cross_bwd_workspace_bytes");
+    const at::Tensor ws = workspace_of(bytes, q);
+    check_status(race_cross_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), lengths_of(lengths), dout.data_ptr(),
+                                state.data_ptr<float>(), ptr_of(dq), ptr_of(dk), ptr_of(dv), &r.sh, ws.data_ptr(), bytes,
+                                current_stream()),
+                 "race_cross_bwd");
+    return {dq, dk, dv};
+}
+
 void bind_operators(pybind11::module& m) {
     namespace py = pybind11;
+    m.def("cross_forward", &cross_forward, "The non-causal op over another sequence's keys -> (out, state)",
+          py::arg("probsQ"), py::arg("probsK"), py::arg("V"), py::arg("lengths"), py::arg("want_state"));
+    m.def("cross_query", &cross_query, "Queries against a kept state -> out", py::arg("probsQ"), py::arg("state"));
+    m.def("cross_backward", &cross_backward, "Gradients of cross_forward -> (dQ, dK, dV)", py::arg("probsQ"),
+          py::arg("probsK"), py::arg("V"), py::arg("lengths"), py::arg("dout"), py::arg("state"), py::arg("need_q"),
+          py::arg("need_k"), py::arg("need_v"));
     m.def("check_capture", &check_capture, "Refuses a capture whose backward would wait for the default stream",
           py::arg("entry"), py::arg("inputs"));
     m.def("norm_rope_forward", &norm_rope_forward, "Heads normed and rotated, to streams -> (q, k or None)",

@@ -79,3 +79,32 @@ def test_norm_rope_refuses_on_the_host(race):
     x = torch.zeros(1, 2, 3, 64)
     with pytest.raises(RuntimeError, match="race_norm_rope: q lives on the CPU"):
         race.race_norm_rope(x, x)
+
+
+def test_cross_refuses_on_the_host(race):
+    from race_attention_kernel_amd import abi
+
+    bad = abi.RACE_ERROR_INVALID_VALUE
+    ok = abi.cross_shape(8, 40, 300, 4, 16, 64)
+    for backward in (False, True):
+        st, nbytes = abi.cross_workspace_bytes(ok, backward)
+        assert st == abi.RACE_SUCCESS and nbytes >= 8 * 64 * 65 * 4
+        assert abi.cross_workspace_bytes(abi.cross_shape(0, 40, 300, 4, 16, 64), backward) == (abi.RACE_SUCCESS, 0)
+        for args in ((65536, 1, 1, 4, 16, 64), (1, -1, 1, 4, 16, 64), (1, 1, -1, 4, 16, 64), (1, 2 ** 31 - 1, 1, 4, 16, 64),
+                     (1, 1, 1, 0, 16, 64), (1, 1, 1, 4, 65, 64), (1, 1, 1, 4, 16, 129), (1, 1, 1, 4, 16, 64, 2),
+                     (1, 1, 1, 4, 16, 64, 0, 0)):
+            assert abi.cross_workspace_bytes(abi.cross_shape(*args), backward)[0] == bad, args
+    assert abi.cross_fwd(None, 16, 16, None, 16, None, ok, 16, 1 << 30, 0) == bad
+    assert abi.cross_fwd(16, 16, 16, None, 16, None, ok, 16, 64, 0) == bad
+    assert abi.cross_fwd(16, 16, 8, None, 16, None, ok, 16, 1 << 30, 0) == bad
+    assert abi.cross_query(16, 4, 16, ok, 0) == bad
+    assert abi.cross_bwd(16, 16, 16, None, 16, None, 16, 16, 16, ok, 16, 1 << 30, 0) == bad
+    assert abi.cross_bwd(16, 16, 16, None, 16, 16, 16, 16, 16, ok, None, 0, 0) == bad
+    # Nothing to do touches no device.
+    assert abi.cross_fwd(None, 16, 16, None, None, None, ok, None, 0, 0) == 0
+    assert abi.cross_bwd(16, 16, 16, None, 16, 16, None, None, None, ok, None, 0, 0) == 0
+    x = torch.zeros(2, 3, 16)
+    with pytest.raises(RuntimeError, match="race_cross_fwd: probsQ lives on the CPU"):
+        race.race_cross_fwd(x, x, x)
+    with pytest.raises(RuntimeError, match="race_cross_state: probsK lives on the CPU"):
+        race.race_cross_state(x, x)
