@@ -96,6 +96,13 @@ class ArgCheck {
         if (!ok) fail(name, what);
         return *this;
     }
+    // The same with the text formed only when it fails (shapes take a
+    // microsecond each to print).
+    template <typename F, typename = decltype(std::declval<F>()())>
+    ArgCheck& require(bool ok, const char* name, F&& what) {
+        if (!ok) fail(name, what());
+        return *this;
+    }
     void raise() const {
         TORCH_CHECK(reason_.empty(), entry_, ": ", reason_);
     }

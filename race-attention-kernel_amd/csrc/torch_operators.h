@@ -21,7 +21,7 @@ bool starts_aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.
 void check_rows(ArgCheck& c, const char* name, const at::Tensor& t, int64_t dim, const char* layout) {
     c.require(t.is_cuda(), name, "lives on the CPU; the library reads it on the GPU")
         .dtype_is(name, t, true)
-        .require(t.dim() == dim, name, "has shape " + dims(t) + ", not " + layout)
+        .require(t.dim() == dim, name, [&] { return "has shape " + dims(t) + ", not " + layout; })
         .require(t.dim() != dim || t.numel() == 0 || t.size(dim - 1) == 1 || t.stride(dim - 1) == 1, name,
                  "has a strided last dimension; its elements must be next to each other")
         .require(t.numel() == 0 || starts_aligned(t), name,
@@ -35,8 +35,8 @@ int64_t check_lengths(ArgCheck& c, const c10::optional<at::Tensor>& lengths, con
     c.require(l.scalar_type() == at::kInt && l.device() == rows.device() && l.is_contiguous() && l.dim() == 1, "lengths",
               "must be a contiguous int32 vector on the rows' device")
         .require(l.numel() > 0 ? streams % l.numel() == 0 : streams == 0, "lengths",
-                 "has " + std::to_string(l.numel()) + " entries, which do not divide the " + std::to_string(streams) +
-                     " streams");
+                 [&] { return "has " + std::to_string(l.numel()) + " entries, which do not divide the " + std::to_string(streams) +
+                     " streams"; });
     return l.dim() == 1 && l.numel() > 0 && streams >= l.numel() ? streams / l.numel() : 1;
 }
 
@@ -72,17 +72,17 @@ race_scan_shape scan_shape(const char* entry, const at::Tensor& x, const at::Ten
     check_rows(c, "x", x, 3, "[N, T, D]");
     check_rows(c, "gate", gate, 3, "[N, T, D]");
     c.matches("gate", gate, "x", x)
-        .require(gate.sizes() == x.sizes(), "gate", "has shape " + dims(gate) + ", x " + dims(x));
+        .require(gate.sizes() == x.sizes(), "gate", [&] { return "has shape " + dims(gate) + ", x " + dims(x); });
     c.raise();
     const int64_t N = x.size(0), D = x.size(2);
     if (state)
         c.on_gpu("state", *state)
             .require(state->scalar_type() == at::kFloat && state->device() == x.device(), "state",
                      "must be float32 on x's device")
-            .require(state->sizes() == at::IntArrayRef({N, D}), "state", "has shape " + dims(*state) + ", not [N, D]");
+            .require(state->sizes() == at::IntArrayRef({N, D}), "state", [&] { return "has shape " + dims(*state) + ", not [N, D]"; });
     const int64_t group = check_lengths(c, lengths, x, N);
     c.require(N <= 65535 && D >= 1 && D <= 65536, "x",
-              "has shape " + dims(x) + "; the scan takes up to 65535 streams of 1 .. 65536 channels")
+              [&] { return "has shape " + dims(x) + "; the scan takes up to 65535 streams of 1 .. 65536 channels"; })
         .raise();
     race_scan_shape sh{};
     sh.num_streams = N;
@@ -133,7 +133,7 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
     int64_t floats = 0;
     check_status(race_gated_scan_workspace_bytes(&sh, 1, &bytes, &floats), "race_gated_scan_workspace_bytes");
     ArgCheck(entry).on_gpu("dout", dout).matches("dout", dout, "x", x)
-        .require(dout.sizes() == x.sizes(), "dout", "has shape " + dims(dout) + ", x " + dims(x))
+        .require(dout.sizes() == x.sizes(), "dout", [&] { return "has shape " + dims(dout) + ", x " + dims(x); })
         .on_gpu("records", records)
         .require(records.scalar_type() == at::kFloat && records.device() == x.device() && records.numel() == floats,
                  "records", "are not those of the forward of these inputs")
@@ -169,14 +169,14 @@ RopeCall rope_call(const char* entry, const at::Tensor& q, const c10::optional<a
     RopeCall r;
     r.B = q.size(0), r.T = q.size(1), r.d = q.size(3);
     c.require(q.size(2) >= 1 && q.size(2) <= 65535 && r.d >= 1 && r.d <= 256, "q",
-              "has shape " + dims(q) + "; rows of 1 .. 256 values in 1 .. 65535 heads are taken")
+              [&] { return "has shape " + dims(q) + "; rows of 1 .. 256 values in 1 .. 65535 heads are taken"; })
         .require(r.T == 0 || r.B <= INT32_MAX / r.T, "q", "has 2^31 tokens or more");
     if (k) {
         check_rows(c, "k", *k, 4, "[B, T, H, d]");
         c.matches("k", *k, "q", q)
             .require(k->dim() == 4 && k->size(0) == r.B && k->size(1) == r.T && k->size(3) == r.d && k->size(2) >= 1 &&
                          k->size(2) <= 65535,
-                     "k", "has shape " + dims(*k) + ", not q's batch, tokens and head width");
+                     "k", [&] { return "has shape " + dims(*k) + ", not q's batch, tokens and head width"; });
     }
     int64_t pairs = 0;
     const bool many = inv_freq && sections.size() > 1;  // without a rotation there are no axes
@@ -185,7 +185,7 @@ RopeCall rope_call(const char* entry, const at::Tensor& q, const c10::optional<a
             .require(inv_freq->scalar_type() == at::kFloat && inv_freq->device() == q.device() && inv_freq->dim() == 1,
                      "inv_freq", "must be a float32 vector on q's device")
             .require(2 * inv_freq->numel() <= r.d, "inv_freq",
-                     "has " + std::to_string(inv_freq->numel()) + " pairs, more than half of d = " + std::to_string(r.d));
+                     [&] { return "has " + std::to_string(inv_freq->numel()) + " pairs, more than half of d = " + std::to_string(r.d); });
         pairs = inv_freq->numel();
         c.require(positions.has_value(), "positions", "are needed for a rotation");
         if (positions) {
@@ -194,11 +194,11 @@ RopeCall rope_call(const char* entry, const at::Tensor& q, const c10::optional<a
                       "positions", "must be int32 or int64 on q's device")
                 .require(p.dim() >= 1 && p.dim() <= 3 && p.size(p.dim() - 1) == r.T &&
                              (p.dim() < 2 || p.size(p.dim() - 2) == r.B),
-                         "positions", "have shape " + dims(p) + ", not [T], [B, T] or [axes, B, T]")
+                         "positions", [&] { return "have shape " + dims(p) + ", not [T], [B, T] or [axes, B, T]"; })
                 .require(sections.size() <= 4 && (p.dim() == 3 ? p.size(0) == int64_t(many ? sections.size() : 1) : !many),
-                         "positions", "have shape " + dims(p) + " for " +
+                         "positions", [&] { return "have shape " + dims(p) + " for " +
                                           std::to_string(sections.empty() ? 1 : sections.size()) +
-                                          " sections; one axis each (at most 4)");
+                                          " sections; one axis each (at most 4)"; });
         }
         int64_t sum = 0;
         for (int64_t s : sections) {
@@ -206,7 +206,7 @@ RopeCall rope_call(const char* entry, const at::Tensor& q, const c10::optional<a
             sum += s;
         }
         c.require(sections.empty() || sum == pairs, "sections",
-                  "sum to " + std::to_string(sum) + ", not the " + std::to_string(pairs) + " pairs of inv_freq");
+                  [&] { return "sum to " + std::to_string(sum) + ", not the " + std::to_string(pairs) + " pairs of inv_freq"; });
     }
     at::ScalarType wt = q.scalar_type();
     bool first = true;
@@ -215,7 +215,7 @@ RopeCall rope_call(const char* entry, const at::Tensor& q, const c10::optional<a
         const at::Tensor& t = **w;
         c.on_gpu(name, t).dtype_is(name, t, true)
             .require(t.device() == q.device() && t.dim() == 1 && t.numel() == r.d, name,
-                     "must hold d = " + std::to_string(r.d) + " values on q's device")
+                     [&] { return "must hold d = " + std::to_string(r.d) + " values on q's device"; })
             .require(first || t.scalar_type() == wt, name, "has another dtype than q_weight")
             .require(norm, name, "is given without a norm (eps is None)");
         wt = t.scalar_type(), first = false;
@@ -277,12 +277,12 @@ norm_rope_backward(const at::Tensor& q, const c10::optional<at::Tensor>& k, cons
     ArgCheck c(entry);
     if (dq_out)
         c.on_gpu("dq_out", *dq_out).matches("dq_out", *dq_out, "q", q)
-            .require(dq_out->sizes() == at::IntArrayRef({r.B * q.size(2), r.T, r.d}), "dq_out", "has shape " + dims(*dq_out));
+            .require(dq_out->sizes() == at::IntArrayRef({r.B * q.size(2), r.T, r.d}), "dq_out", [&] { return "has shape " + dims(*dq_out); });
     if (dk_out)
         c.require(k.has_value(), "dk_out", "is given without k")
             .on_gpu("dk_out", *dk_out).matches("dk_out", *dk_out, "q", q)
             .require(k && dk_out->sizes() == at::IntArrayRef({r.B * k->size(2), r.T, r.d}), "dk_out",
-                     "has shape " + dims(*dk_out));
+                     [&] { return "has shape " + dims(*dk_out); });
     c.raise();
     const c10::DeviceGuard guard(q.device());
     c10::optional<at::Tensor> dq, dk, dqw, dkw;
@@ -327,7 +327,7 @@ CrossCall cross_call(const char* entry, const at::Tensor* q, const at::Tensor* k
     const at::Tensor& ref = q ? *q : *k;
     auto probs = [&](const char* name, const at::Tensor& t) {
         c.on_gpu(name, t).dtype_is(name, t, true)
-            .require(t.dim() == 3 || t.dim() == 4, name, "has shape " + dims(t) + ", not [N, T, L, R] or [N, T, S]");
+            .require(t.dim() == 3 || t.dim() == 4, name, [&] { return "has shape " + dims(t) + ", not [N, T, L, R] or [N, T, S]"; });
     };
     if (q) probs("probsQ", *q);
     if (k) probs("probsK", *k);
@@ -337,10 +337,10 @@ CrossCall cross_call(const char* entry, const at::Tensor* q, const at::Tensor* k
     if (k) {
         Nk = k->size(0);
         c.matches("probsK", *k, "probsQ", ref)
-            .require(buckets_of(*k) == r.S, "probsK", "has shape " + dims(*k) + ", another number of buckets than probsQ")
+            .require(buckets_of(*k) == r.S, "probsK", [&] { return "has shape " + dims(*k) + ", another number of buckets than probsQ"; })
             .on_gpu("V", *v).matches("V", *v, "probsK", *k)
             .require(v->dim() == 3 && v->size(0) == Nk && v->size(1) == k->size(1), "V",
-                     "has shape " + dims(*v) + ", not [N, T, d] with probsK's N and T");
+                     [&] { return "has shape " + dims(*v) + ", not [N, T, d] with probsK's N and T"; });
         if (v->dim() == 3) r.d = v->size(2);
         r.sh.kv_len = k->size(1);
     } else {
@@ -348,14 +348,14 @@ CrossCall cross_call(const char* entry, const at::Tensor* q, const at::Tensor* k
             .require(state->scalar_type() == at::kFloat && state->device() == ref.device(), "state",
                      "must be float32 on probsQ's device")
             .require(state->dim() == 2 && r.S > 0 && state->size(1) % r.S == 0 && state->size(1) / r.S >= 2, "state",
-                     "has shape " + dims(*state) + ", not [N, S*d + S] with probsQ's S");
+                     [&] { return "has shape " + dims(*state) + ", not [N, S*d + S] with probsQ's S"; });
         c.raise();
         Nk = state->size(0);
         r.d = state->size(1) / r.S - 1;
     }
     r.Nq = q ? q->size(0) : Nk, r.Tq = q ? q->size(1) : 0;
     c.require(Nk > 0 ? r.Nq % Nk == 0 : r.Nq == 0, "probsQ",
-              "has " + std::to_string(r.Nq) + " streams, no multiple of the " + std::to_string(Nk) + " key streams");
+              [&] { return "has " + std::to_string(r.Nq) + " streams, no multiple of the " + std::to_string(Nk) + " key streams"; });
     const int64_t group = check_lengths(c, lengths, ref, Nk);
     const int64_t heads = Nk > 0 ? std::max<int64_t>(r.Nq / Nk, 1) : 1;
     constexpr int64_t kMost = int64_t(1) << 30;
@@ -405,7 +405,7 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
     const char* entry = "race_cross_fwd backward";
     const CrossCall r = cross_call(entry, &q, &k, &v, nullptr, lengths);
     ArgCheck(entry).on_gpu("dout", dout).matches("dout", dout, "V", v)
-        .require(dout.sizes() == at::IntArrayRef({r.Nq, r.Tq, r.d}), "dout", "has shape " + dims(dout))
+        .require(dout.sizes() == at::IntArrayRef({r.Nq, r.Tq, r.d}), "dout", [&] { return "has shape " + dims(dout); })
         .on_gpu("state", state)
         .require(state.scalar_type() == at::kFloat && state.device() == q.device() &&
                      state.sizes() == at::IntArrayRef({r.sh.kv_streams, r.S * r.d + r.S}),
