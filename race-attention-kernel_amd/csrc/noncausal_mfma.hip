@@ -220,7 +220,20 @@ struct Outer {
     static constexpr int kLdsFloats = 2 * kBlockFloats + 16 * 16 * EA;
 };
 
-// One workgroup per (chunk of tokens, stream, block of R).  Wave w takes the
+// Stream and block of a workgroup: gfx950 hands consecutive workgroups to its 8
+// XCDs in turn, so the `per` blocks of one stream are 8 apart in launch order
+// and share an XCD's L2 (the matrix records a stream's workgroups all read).
+__device__ __forceinline__ void stream_block(int64_t id, int64_t N, int per, int64_t& n, int& blk) {
+    const int64_t group = id / (8 * per);
+    const int in = int(id - group * 8 * per);
+    const int streams = int(min<int64_t>(8, N - 8 * group));
+    n = 8 * group + in % streams;
+    blk = in / streams;
+}
+
+// One workgroup per (chunk of tokens, stream, block of R); with several blocks
+// (flat > 0 of them) those of one chunk run on one XCD, one after another, and
+// read the tokens from its L2.  Wave w takes the
 // steps w, w + 4, .. of the chunk.  The operand vectors of the next step are
 // loaded before the current step's products.
 // kEndFirst (the causal tile sums, whose tiles the output pass then walks from
@@ -229,13 +242,20 @@ struct Outer {
 template <typename TIn, int EA, int EB, bool kEndFirst>
 __global__ __launch_bounds__(kThreads, 3) void nc_sums_kernel(
     const TIn* __restrict__ x, const TIn* __restrict__ y, float* __restrict__ records, int64_t T, int chunk,
-    int64_t chunks, int64_t rec, int Wa, int Wb, int bblocks, int kept, const Live live) {
+    int64_t chunks, int64_t rec, int Wa, int Wb, int bblocks, int kept, const Live live, int64_t N, int flat) {
     extern __shared__ __align__(16) float smem[];
     constexpr int es = int(sizeof(TIn)), kTok = kStep<TIn>, kLoads = kTok / 4;
     const int lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t n = blockIdx.y, ci = blockIdx.x;
-    const int a0 = 16 * EA * int(blockIdx.z / bblocks), b0 = 16 * EB * int(blockIdx.z % bblocks);
+    int64_t n = blockIdx.y, ci = blockIdx.x;
+    int z = blockIdx.z;
+    if (flat) {
+        int64_t pair;
+        stream_block(blockIdx.x, N * chunks, flat, pair, z);
+        n = pair / chunks;
+        ci = pair - n * chunks;
+    }
+    const int a0 = 16 * EA * (z / bblocks), b0 = 16 * EB * (z % bblocks);
     const int64_t t0 = ci * chunk;
     const int rows = int(max(int64_t(0), min(live.of(n, T), t0 + chunk) - t0));
     const auto xr = mfma::make_rsrc(x + (n * T + t0) * Wa, int64_t(rows) * Wa * es);
@@ -576,17 +596,6 @@ __device__ __forceinline__ void stage_operand(float* __restrict__ dst, const Map
     }
 }
 
-// Stream and block of a workgroup: gfx950 hands consecutive workgroups to its 8
-// XCDs in turn, so the `per` blocks of one stream are 8 apart in launch order
-// and share an XCD's L2 (the matrix records a stream's workgroups all read).
-__device__ __forceinline__ void stream_block(int64_t id, int64_t N, int per, int64_t& n, int& blk) {
-    const int64_t group = id / (8 * per);
-    const int in = int(id - group * 8 * per);
-    const int streams = int(min<int64_t>(8, N - 8 * group));
-    n = 8 * group + in % streams;
-    blk = in / streams;
-}
-
 // One workgroup per (block of `wg_tokens` tokens, stream, slice of 16 NCB
 // output columns); wave w takes the 16-token tiles w, w + NW, ..  Rows of up to
 // 128 values are loaded as whole rows a tile ahead; longer ones straight in
@@ -594,7 +603,7 @@ __device__ __forceinline__ void stream_block(int64_t id, int64_t N, int per, int
 template <typename TIn, int NJ, int NCB, bool kB16, int NW>
 __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__ x, TIn* __restrict__ out,
                                                           const MapOperand op, int64_t N, int64_t T, int Wa,
-                                                          int Wb, int wg_tokens, int per, const Live live) {
+                                                          int Wb, int wg_tokens, int per, const Live live, int slices) {
     extern __shared__ __align__(16) float smem[];
     using X = MapRows<TIn, NJ, kB16>;
     using O = OutRows<TIn, NCB>;
@@ -605,12 +614,16 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned char* mine = reinterpret_cast<unsigned char*>(smem + kMatrixFloats<NJ, NCB, kB16>) + w * kWaveBytes;
     int64_t n;
-    int blk;
-    stream_block(blockIdx.x, N, per, n, blk);
+    int blk, slice = blockIdx.y;
+    stream_block(blockIdx.x, N, per * slices, n, blk);
+    if (slices > 1) {  // a block's slices one after another, its tokens from the XCD's L2
+        slice = blk % slices;
+        blk /= slices;
+    }
     const int64_t t0 = int64_t(blk) * wg_tokens;
     const int rows = int(min<int64_t>(T - t0, wg_tokens));
     const int alive = int(max(int64_t(0), min<int64_t>(live.of(n, T) - t0, rows)));
-    const int c0 = 16 * NCB * int(blockIdx.y), ncols = min(16 * NCB, Wb - c0);
+    const int c0 = 16 * NCB * slice, ncols = min(16 * NCB, Wb - c0);
     const auto xr = mfma::make_rsrc(x + (n * T + t0) * Wa, int64_t(alive) * Wa * es);
     const auto orr = mfma::make_rsrc(out + (n * T + t0) * Wb, int64_t(rows) * Wb * es);
     auto load = [&](X& v, int row0) {
@@ -626,7 +639,7 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
     };
     X next;
     load(next, 16 * w);
-    stage_operand<64 * NW, NJ, NCB, kB16>(smem, op, n, Wa, c0, ncols, blk == 0, blockIdx.y == 0);
+    stage_operand<64 * NW, NJ, NCB, kB16>(smem, op, n, Wa, c0, ncols, blk == 0, slice == 0);
     auto bias_of = [&](int cb, int g) {
         f32x4 b;
 #pragma unroll
@@ -659,6 +672,245 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
                 if (bad) whole_products<TIn, NJ, NCB>(to, bad, xr, r0, Wa, smem, lane, bias_of);
             }
         });
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Map of bf16 tokens of 72 .. 256 values to more than 64 columns.
+// nc_map_kernel reads the tokens once per slice of 64 columns and its matrix from
+// LDS once per 16 tokens, 1 KB an instruction; at 256 x 128 both cost more than
+// the tokens themselves.  Here a workgroup takes every column: wave w holds the
+// matrix's columns of the 16-column blocks w, w + 8, .. in registers, all its
+// terms (96 of them), read straight from memory, and the waves share tiles of 32
+// tokens staged in LDS, two tiles' loads under way.  One barrier a tile: the
+// results of tile i leave through LDS as whole rows while tile i + 1 is
+// multiplied.  The same products in the same order: the same bits.  32 x 4096
+// tokens, 256 to 128 columns (100 MB): 36 us, 45 with nc_map_kernel; 32 x 8192 74
+// and 93.  Bound by its three-term products (26 GFLOP) and the tokens together,
+// 21 us each at the rates of a large product and a large copy.  At 64 values
+// nc_map_kernel is the faster (15 us for 32 x 4096 x 64 to 128, 23 here).
+constexpr int kWideTile = 32;
+
+template <int NJ, int NCW>
+struct MapWide {
+    static constexpr int kOps = (NJ + 1) / 2, kUnits = 4 * kOps;   // 16-byte units of a staged row
+    static constexpr int kThreads = 64 * kMapWaves;
+    static constexpr int kPer = kWideTile * kUnits / kThreads;
+    static_assert(kPer * kThreads == kWideTile * kUnits, "whole loads");
+    static constexpr int kOutUnits = 4 * kMapWaves * NCW;          // 8-byte units of a result row
+    static constexpr int kRowUnits = kWideTile * kUnits, kOutSize = kWideTile * kOutUnits;
+    static constexpr int kLds = 2 * (kRowUnits * 16 + kOutSize * 8);
+    __device__ __forceinline__ static int at(int row, int u) { return row * kUnits + (u ^ (row & (kUnits - 1))); }
+    __device__ __forceinline__ static int out_at(int row, int u) { return row * kOutUnits + (u ^ (row & 15)); }
+};
+
+// The three terms of M[32 j + 8 g .. + 7][c] for j < kOps, zero past Wa rows and
+// Wb columns: a lane's operands of column c.  The operand as stage_operand reads
+// it, its divisors summed in `den` (LDS); the workgroups with `save` write the
+// undivided values.  A part's loads are all in flight together.
+template <int kOps>
+__device__ __forceinline__ void load_operand(bf16x8 (&m)[kOps][3], const MapOperand& op, const float* __restrict__ den,
+                                             int64_t n, int Wa, int Wb, int c, int g, bool save) {
+    const bool plain = op.col == 1;
+    const int ld = int(plain ? op.row : op.col), k0 = 8 * g;
+    const bool there = c < Wb;
+    // Byte offsets; past the end (kOutside and what is added to it) reads zeros.
+    const int bytes = (plain ? (Wa - 1) * ld + Wb : (Wb - 1) * ld + Wa) * 4;
+    const int at = there ? (plain ? k0 * ld + c : c * ld + k0) * 4 : kOutside;
+    const float* mn = op.m + n * op.stream;
+    float v[kOps][8];
+    for (int p = 0; p < op.parts; ++p) {
+        const auto mr = mfma::make_rsrc(mn + p * op.part_stride, bytes);
+        float x[kOps][8];
+#pragma unroll
+        for (int j = 0; j < kOps; ++j) {
+            const int off = 32 * j + k0 < Wa ? at : kOutside;  // rows come in whole eights
+            if (plain) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[j][e] = __uint_as_float(
+                        __builtin_amdgcn_raw_buffer_load_b32(mr, int(unsigned(off) + (32 * j + e) * ld * 4u), 0, 0));
+            } else {
+                const uint4 x0 = mfma::buf_load16<mfma::kPolicyDefault>(mr, int(unsigned(off) + 128 * j));
+                const uint4 x1 = mfma::buf_load16<mfma::kPolicyDefault>(mr, int(unsigned(off) + 128 * j + 16));
+                const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][e] = __uint_as_float(w[e]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kOps; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = p ? v[j][e] + x[j][e] : x[j][e];
+    }
+    if (op.save && save) {
+        const auto sr = mfma::make_rsrc(op.save + n * op.save_stream, bytes);
+#pragma unroll
+        for (int j = 0; j < kOps; ++j) {
+            const int off = 32 * j + k0 < Wa ? at : kOutside;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[j][e]), sr,
+                                                      int(unsigned(off) + (32 * j + e) * 4u * (plain ? ld : 1)), 0, 0);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kOps; ++j) {
+        u32x4 t[3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int k = 32 * j + k0 + e;
+            float x = v[j][e];
+            if (op.div && there && k < Wa) x /= den[plain ? k : c] + kEps;
+            uint16_t s[3];
+            split3(x, s);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) t[i][e >> 1] = (e & 1) ? t[i][e >> 1] | uint32_t(s[i]) << 16 : uint32_t(s[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) m[j][i] = __builtin_bit_cast(bf16x8, t[i]);
+    }
+}
+
+template <int NJ, int NCW>
+__global__ __launch_bounds__(64 * kMapWaves) void nc_map_wide_kernel(const bf16_t* __restrict__ x,
+                                                                     bf16_t* __restrict__ out, const MapOperand op,
+                                                                     int64_t N, int64_t T, int Wa, int Wb,
+                                                                     int wg_tokens, int per, const Live live) {
+    extern __shared__ __align__(16) float smem[];
+    using M = MapWide<NJ, NCW>;
+    constexpr int es = 2, kHalves = kWideTile / 16;
+    const int lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t n;
+    int blk;
+    stream_block(blockIdx.x, N, per, n, blk);
+    const int64_t t0 = int64_t(blk) * wg_tokens;
+    const int rows = int(min<int64_t>(T - t0, wg_tokens));
+    const int alive = int(max(int64_t(0), min<int64_t>(live.of(n, T) - t0, rows)));
+    const auto xr = mfma::make_rsrc(x + (n * T + t0) * Wa, int64_t(alive) * Wa * es);
+    const auto orr = mfma::make_rsrc(out + (n * T + t0) * Wb, int64_t(rows) * Wb * es);
+    using Held = uint4[M::kPer];
+    auto load = [&](Held& h, int row0) {
+#pragma unroll
+        for (int i = 0; i < M::kPer; ++i) {
+            const int u = i * M::kThreads + int(threadIdx.x), row = u / M::kUnits, c = 8 * (u % M::kUnits);
+            h[i] = mfma::buf_load16<mfma::kPolicyDefault>(xr, c < Wa ? ((row0 + row) * Wa + c) * es : kOutside);
+        }
+    };
+    Held a, b;
+    load(a, 0);
+    load(b, kWideTile);  // past the block: zeros
+    if (op.div) {
+        const int dens = op.col == 1 ? Wa : Wb;
+        if (int(threadIdx.x) < dens) {
+            const float* dv = op.div + n * op.div_stream + threadIdx.x;
+            float q = dv[0];
+            for (int p = 1; p < op.parts; ++p) q += dv[p * op.part_stride];
+            smem[threadIdx.x] = q;
+            if (op.save && blk == 0) op.save[n * op.save_stream + op.save_div_off + threadIdx.x] = q;
+        }
+        __syncthreads();
+    }
+    bf16x8 m[NCW][M::kOps][3];
+    f32x4 bias[NCW];
+#pragma unroll
+    for (int i = 0; i < NCW; ++i) {
+        const int c0 = 16 * (w + kMapWaves * i);
+        load_operand(m[i], op, smem, n, Wa, Wb, c0 + lr, g, blk == 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int c = c0 + 4 * g + r;
+            bias[i][r] = op.bias && c < Wb ? op.bias[n * op.bias_stream + c] : 0.f;
+        }
+    }
+    uint4* const rows_lds = reinterpret_cast<uint4*>(smem);                        // [2][kRowUnits]
+    u32x2* const out_lds = reinterpret_cast<u32x2*>(rows_lds + 2 * M::kRowUnits);  // [2][kOutSize]
+    auto put = [&](const Held& h, int buf) {
+#pragma unroll
+        for (int i = 0; i < M::kPer; ++i) {
+            const int u = i * M::kThreads + int(threadIdx.x);
+            rows_lds[buf * M::kRowUnits + M::at(u / M::kUnits, u % M::kUnits)] = h[i];
+        }
+    };
+    __syncthreads();  // the divisors have been read
+    put(a, 0);
+    __syncthreads();
+    // Tile r0 from buffer `buf`: the loads of the tile after next into `fresh`,
+    // the next tile (in `ready`) to the other buffer.
+    auto step = [&](Held& fresh, const Held& ready, int r0, int buf) {
+        load(fresh, r0 + 2 * kWideTile);
+        const bf16x8* xb = reinterpret_cast<const bf16x8*>(rows_lds + buf * M::kRowUnits);
+        u32x2* const ob = out_lds + buf * M::kOutSize;
+        f32x4 acc[kHalves][NCW];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+            for (int i = 0; i < NCW; ++i) acc[h][i] = bias[i];
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 top[kHalves] = {};
+#pragma unroll
+        for (int j = 0; j < M::kOps; ++j) {
+            bf16x8 xv[kHalves];
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                xv[h] = xb[M::at(16 * h + lr, 4 * j + g)];
+                const u32x4 xw = __builtin_bit_cast(u32x4, xv[h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    top[h] = __builtin_elementwise_max(top[h], __builtin_bit_cast(u16x2, xw[e] & 0x7fff7fffu));
+            }
+            // Smallest terms first.
+#pragma unroll
+            for (int t = 2; t >= 0; --t)
+#pragma unroll
+                for (int i = 0; i < NCW; ++i)
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) acc[h][i] = mfma16(m[i][j][t], xv[h], acc[h][i]);
+        }
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            const uint64_t bad = __ballot(top[h][0] >= 0x7f80 || top[h][1] >= 0x7f80);
+            if (bad) {  // tokens with an infinity or NaN: fp32 products, as whole_products
+                const bool mine = ((bad | bad >> 16 | bad >> 32 | bad >> 48) >> lr) & 1;
+                auto half = [](uint32_t v, int e) { return (e & 1) ? mfma::hi_half(v) : mfma::lo_half(v); };
+#pragma unroll
+                for (int i = 0; i < NCW; ++i) {
+                    f32x4 full = bias[i];
+#pragma unroll
+                    for (int j = 0; j < M::kOps; ++j) {
+                        const u32x4 xw = __builtin_bit_cast(u32x4, xb[M::at(16 * h + lr, 4 * j + g)]);
+                        u32x4 m0 = __builtin_bit_cast(u32x4, m[i][j][0]);
+                        u32x4 m1 = __builtin_bit_cast(u32x4, m[i][j][1]);
+                        u32x4 m2 = __builtin_bit_cast(u32x4, m[i][j][2]);
+                        asm volatile("" : "+v"(m0), "+v"(m1), "+v"(m2));  // not widened ahead, for every tile
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            full = mfma4(half(m0[e >> 1], e) + (half(m1[e >> 1], e) + half(m2[e >> 1], e)),
+                                         half(xw[e >> 1], e), full);
+                    }
+                    if (mine) acc[h][i] = full;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NCW; ++i) {
+                if (r0 + 16 * h + lr >= alive) acc[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                ob[M::out_at(16 * h + lr, 4 * (w + kMapWaves * i) + g)] =
+                    u32x2{mfma::pack2(acc[h][i][0], acc[h][i][1]), mfma::pack2(acc[h][i][2], acc[h][i][3])};
+            }
+        }
+        put(ready, buf ^ 1);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < M::kOutSize / M::kThreads; ++i) {
+            const int u = i * M::kThreads + int(threadIdx.x), row = u / M::kOutUnits, c = 4 * (u % M::kOutUnits);
+            __builtin_amdgcn_raw_buffer_store_b64(ob[M::out_at(row, u % M::kOutUnits)], orr,
+                                                  c < Wb ? ((r0 + row) * Wb + c) * es : kOutside, 0, kNcStorePolicy);
+        }
+    };
+    for (int r0 = 0; r0 < rows; r0 += 2 * kWideTile) {
+        step(a, b, r0, 0);
+        if (r0 + kWideTile < rows) step(b, a, r0 + kWideTile, 1);
     }
 }
 
@@ -932,10 +1184,12 @@ template <typename TIn, int EA, int EB, bool kEndFirst = false>
 hipError_t launch_sums_e(const void* x, const void* y, float* records, const Problem& p, int Wa, int Wb,
                          hipStream_t stream) {
     const int ab = (Wa + 16 * EA - 1) / (16 * EA), bb = (Wb + 16 * EB - 1) / (16 * EB);
-    const dim3 grid(unsigned(p.tiles), unsigned(p.N), unsigned(ab * bb));
+    const int64_t all = p.tiles * p.N * ab * bb;
+    const bool flat = ab * bb > 1 && all * kThreads < (int64_t(1) << 32);
+    const dim3 grid = flat ? dim3(unsigned(all)) : dim3(unsigned(p.tiles), unsigned(p.N), unsigned(ab * bb));
     nc_sums_kernel<TIn, EA, EB, kEndFirst><<<grid, kThreads, Outer<EA, EB>::kLdsFloats * sizeof(float), stream>>>(
         static_cast<const TIn*>(x), static_cast<const TIn*>(y), records, p.T, p.tile, p.tiles, p.rec, Wa, Wb, bb,
-        kEndFirst ? cache_kept_rows(p) : 0, p.live);
+        kEndFirst ? cache_kept_rows(p) : 0, p.live, p.N, flat ? ab * bb : 0);
     return hipGetLastError();
 }
 
@@ -956,12 +1210,14 @@ hipError_t launch_map_b(const void* x, void* out, const MapOperand& op, const Pr
     const int slices = (Wb + 16 * NCB - 1) / (16 * NCB);
     const int wt = map_wg_tokens(p, slices);
     const int per = int((p.T + wt - 1) / wt);
-    const dim3 grid(unsigned(per * p.N), unsigned(slices));
     constexpr int NW = kMapWaves;
+    const bool flat = per * p.N * slices * 64 * NW < (int64_t(1) << 32);
+    const dim3 grid = flat ? dim3(unsigned(per * p.N * slices)) : dim3(unsigned(per * p.N), unsigned(slices));
     constexpr size_t kTurn = NJ <= 8 ? MapRows<TIn, NJ, kB16>::kBytes : 0, kOut = OutRows<TIn, NCB>::kBytes;
     const size_t lds = kMatrixFloats<NJ, NCB, kB16> * sizeof(float) + NW * (kTurn > kOut ? kTurn : kOut);
     nc_map_kernel<TIn, NJ, NCB, kB16, NW><<<grid, 64 * NW, lds, stream>>>(static_cast<const TIn*>(x), static_cast<TIn*>(out),
-                                                                 op, p.N, p.T, Wa, Wb, wt, per, p.live);
+                                                                 op, p.N, p.T, Wa, Wb, wt, per, p.live,
+                                                                 flat ? slices : 1);
     return hipGetLastError();
 }
 
@@ -984,9 +1240,26 @@ hipError_t launch_map_j(const void* x, void* out, const MapOperand& op, const Pr
     return launch_map_e<TIn, NJ, 4>(x, out, op, p, Wa, Wb, stream);
 }
 
+template <int NJ, int NCW>
+hipError_t launch_map_wide(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
+                           hipStream_t stream) {
+    const int wt = map_wg_tokens(p, 1);
+    const int per = int((p.T + wt - 1) / wt);
+    nc_map_wide_kernel<NJ, NCW><<<unsigned(per * p.N), 64 * kMapWaves, MapWide<NJ, NCW>::kLds, stream>>>(
+        static_cast<const bf16_t*>(x), static_cast<bf16_t*>(out), op, p.N, p.T, Wa, Wb, wt, per, p.live);
+    return hipGetLastError();
+}
+
 template <typename TIn>
 hipError_t launch_map_t(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
                         hipStream_t stream) {
+    if constexpr (sizeof(TIn) == 2) {
+        if (Wb > 64 && Wa > 64 && Wa % 8 == 0) {
+            if (Wa > 128) return launch_map_wide<16, 1>(x, out, op, p, Wa, Wb, stream);
+            return Wb > 128 ? launch_map_wide<8, 2>(x, out, op, p, Wa, Wb, stream)
+                            : launch_map_wide<8, 1>(x, out, op, p, Wa, Wb, stream);
+        }
+    }
     if (Wa <= 16) return launch_map_j<TIn, 1>(x, out, op, p, Wa, Wb, stream);
     if (Wa <= 32) return launch_map_j<TIn, 2>(x, out, op, p, Wa, Wb, stream);
     if (Wa <= 64) return launch_map_j<TIn, 4>(x, out, op, p, Wa, Wb, stream);

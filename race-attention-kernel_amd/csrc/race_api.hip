@@ -5,6 +5,7 @@
 // (src/causal_v2/kernels/race_causal_fwd.h:40-49): caller-owned outputs and
 // workspace, one stream, no allocation, no host synchronization, first error
 // returned, hipErrorInvalidValue for anything the kernels do not support.
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <mutex>
@@ -1894,7 +1895,12 @@ Problem cross_side(const race_cross_shape* sh, int64_t T) {
     p.rec = record_floats(p.S, p.d);
     p.tile = RACE_SUB_CHUNK_TOKENS, p.tiles = 0;
     if (p.N > 0 && T > 0) {
-        const int64_t per = nc_blocks_per_stream(p.N, T, p.dtype, kMaxAutoTileOther);
+        // A chunk has a workgroup for every 64 x 64 block of its sums.  Counted up
+        // to four: 32 key streams of 4096 bf16 tokens at S = 256, d = 128 (8
+        // blocks), forward + backward, 222 us with none counted, 208 with four,
+        // 217 with eight.
+        const int64_t blocks = std::min(4, ((p.S + 63) / 64) * ((p.d + 63) / 64));
+        const int64_t per = nc_blocks_per_stream(p.N * blocks, T, p.dtype, kMaxAutoTileOther);
         p.tile = int(((T + per - 1) / per + 15) / 16 * 16);
         p.tiles = (T + p.tile - 1) / p.tile;
     }
@@ -1916,6 +1922,14 @@ bool cross_problem(const race_cross_shape* sh, const int32_t* lengths, CrossProb
 // Few queries read the state as it is; more go through a map, which stages it
 // once for many tokens.
 bool cross_few(const Problem& q) { return q.T <= RACE_CROSS_QUERY_TOKENS; }
+
+// Records a map's workgroups add as they stage their matrix, each on its own:
+// up to eight of 64 x 64; of larger ones fewer, whose reading would cost more
+// than a launch that adds them once (S = 256, d = 128, 8 records: 57 us the map,
+// 36 + 6 with them added first).
+int64_t cross_fold(const Problem& k) {
+    return std::max<int64_t>(1, std::min<int64_t>(kNcFoldParts, kNcFoldParts * 64 * 64 / (int64_t(k.S) * k.d)));
+}
 
 struct CrossFwdLayout {
     int64_t records = 0, E = 0, state = 0;
@@ -1989,7 +2003,7 @@ race_status race_cross_fwd(const void* probsQ, const void* probsK, const void* V
         RACE_TRY(launch_tile_reduce(records, sums, nullptr, k, stream));
         return launch_cross_query(probsQ, sums, out, q, stream);
     }
-    if (k.tiles > kNcFoldParts) {
+    if (k.tiles > cross_fold(k)) {
         float* E = records + l.records;
         RACE_TRY(launch_tile_reduce(records, state, E, k, stream));
         return token_map(probsQ, out, map_operand(E, Sd, q.d, 1), q, q.S, q.d, stream);
