@@ -6,21 +6,21 @@ through the _race_torch binding.  There is no CPU fallback.
 """
 from . import causal_v2
 from .batched_ace import BatchedACE
-from .cross import CrossACE, CrossFunction, race_cross_fwd, race_cross_query, race_cross_state
+from .cross import CrossACE, race_cross_fwd, race_cross_query, race_cross_state
 from .inputs import CONFIGS, Config, config_inputs, make_inputs
 from .ops import (HashedRaceFunction, HashProbsFunction, RaceFusedFunction, hashed_supported,
                   race_causal_backward, race_fused_fwd, race_fused_fwd_carry, race_fused_fwd_hashed,
                   race_fused_fwd_with_state, race_hash_probs, race_noncausal_backward,
                   select_tile_tokens)
-from .recurrence import GatedScanFunction, race_gated_scan, race_gated_scan_carry
-from .rope import NormRopeFunction, race_norm_rope
+from .recurrence import race_gated_scan, race_gated_scan_carry
+from .rope import race_norm_rope
 
 __all__ = [
     "BatchedACE", "CONFIGS", "Config", "RaceFusedFunction", "config_inputs", "make_inputs",
     "race_fused_fwd", "race_fused_fwd_carry", "race_fused_fwd_with_state", "race_noncausal_backward",
     "race_causal_backward", "race_fused_fwd_hashed", "hashed_supported", "HashedRaceFunction",
     "HashProbsFunction", "race_hash_probs", "select_tile_tokens", "causal_v2",
-    "CrossACE", "CrossFunction", "race_cross_fwd", "race_cross_query", "race_cross_state",
-    "NormRopeFunction", "race_norm_rope",
-    "GatedScanFunction", "race_gated_scan", "race_gated_scan_carry",
+    "CrossACE", "race_cross_fwd", "race_cross_query", "race_cross_state",
+    "race_norm_rope",
+    "race_gated_scan", "race_gated_scan_carry",
 ]

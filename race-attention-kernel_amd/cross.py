@@ -12,33 +12,10 @@ reference's non-causal op (analysis/hot-path.md:157-162) has one length.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .batched_ace import BatchedACE
-from .ops import _dense
-from .recurrence import _lengths
 from .rope import race_norm_rope
-
-
-class CrossFunction(torch.autograd.Function):
-    """out = race_cross_fwd(probsQ, probsK, V, lengths); saves the inputs and the
-    sums of the keys."""
-
-    @staticmethod
-    def forward(ctx, probsQ, probsK, V, lengths):
-        _lib.ext().check_capture("race_cross_fwd", [probsQ, probsK, V])
-        out, state = _lib.ext().cross_forward(probsQ, probsK, V, lengths, True)
-        ctx.save_for_backward(probsQ, probsK, V, lengths, state)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, lengths, state = ctx.saved_tensors
-        _lib.ext().check_capture("race_cross_fwd backward", [q, k, v])
-        return (*_lib.ext().cross_backward(q, k, v, lengths, _dense(dout.to(v.dtype)), state,
-                                           *ctx.needs_input_grad[:3]), None)
 
 
 def race_cross_fwd(probsQ: torch.Tensor, probsK: torch.Tensor, V: torch.Tensor,
@@ -51,21 +28,20 @@ def race_cross_fwd(probsQ: torch.Tensor, probsK: torch.Tensor, V: torch.Tensor,
         probsK: [Nk, Tk, L, R] (or [Nk, Tk, S]), V: [Nk, Tk, d], same dtype and
             device.  Nq = g Nk: query streams g n .. g n + g - 1 share key
             stream n (query heads that share a key head).
-        lengths: int32 [Nk] or [Nk / h] (entry i for key streams h i .. h i + h -
+        lengths: int32 (or int64) [Nk] or [Nk / h] (entry i for key streams h i .. h i + h -
             1: one per batch entry): keys from lengths on are not read and get
             zero gradients.  A stream without keys gives zeros.
 
-    Returns [Nq, Tq, d] in V's dtype.  Differentiable w.r.t. probsQ, probsK, V."""
-    lengths = _lengths(lengths)
-    if torch.is_grad_enabled() and (probsQ.requires_grad or probsK.requires_grad or V.requires_grad):
-        return CrossFunction.apply(probsQ, probsK, V, lengths)
-    return _lib.ext().cross_forward(probsQ, probsK, V, lengths, False)[0]
+    Returns [Nq, Tq, d] in V's dtype.  Differentiable once, w.r.t. probsQ, probsK
+    and V.  A backward is captured into a graph together with its forward, and not
+    while an eager graph of the same leaves is alive."""
+    return _lib.ext().cross(probsQ, probsK, V, lengths)
 
 
 def race_cross_state(probsK: torch.Tensor, V: torch.Tensor, lengths: torch.Tensor | None = None) -> torch.Tensor:
     """The sums [Nk, S*d + S] (float32, B then A) that race_cross_query reads; no
     autograd."""
-    return _lib.ext().cross_forward(None, probsK, V, _lengths(lengths), True)[1]
+    return _lib.ext().cross_state(probsK, V, lengths)
 
 
 def race_cross_query(probsQ: torch.Tensor, state: torch.Tensor) -> torch.Tensor:

@@ -426,16 +426,250 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
     return {dq, dk, dv};
 }
 
+// ---- the operators with their gradients ----
+// Autograd nodes in C++: a training step of small tensors is bound by the host,
+// and nodes in Python cost it about 50 us more (forward and backward of a
+// few rows through race_norm_rope: 93 us with one).
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Inputs the kernels read by strides; a copy where the last dimension is apart,
+// the first value is not 16-byte aligned, or dimension 1 strides too far.
+at::Tensor as_rows(const at::Tensor& t, int64_t far = int64_t(1) << 40) {
+    const int64_t n = t.dim();
+    if (t.numel() == 0 || n < 2) return t;
+    const bool apart = t.size(n - 1) > 1 && t.stride(n - 1) != 1;
+    if (!apart && starts_aligned(t) && !(t.size(1) > 1 && t.stride(1) > far)) return t;
+    return t.clone(at::MemoryFormat::Contiguous);
+}
+
+c10::optional<at::Tensor> as_lengths(const c10::optional<at::Tensor>& lengths) {
+    if (lengths && lengths->scalar_type() == at::kLong) return lengths->to(at::kInt);
+    return lengths;
+}
+
+bool wants_grad(std::initializer_list<c10::optional<at::Tensor>> inputs) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const auto& t : inputs)
+        if (t && t->requires_grad()) return true;
+    return false;
+}
+
+// An upstream gradient as the kernels read it.
+c10::optional<at::Tensor> dense_grad(const at::Tensor& g, at::ScalarType type) {
+    if (!g.defined()) return c10::nullopt;
+    at::Tensor t = g.detach().to(type).contiguous();
+    return t.numel() > 0 && !starts_aligned(t) ? t.clone() : t;
+}
+
+c10::optional<at::Tensor> if_defined(const at::Tensor& t) {
+    if (t.defined()) return t;
+    return c10::nullopt;
+}
+at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return t ? *t : at::Tensor(); }
+
+// Gradients of a node whose backward has none of its own: differentiating them
+// raises, as once_differentiable does.
+variable_list differentiated_once(const char* entry, const variable_list& upstream, variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    bool again = false;
+    for (const at::Tensor& g : upstream) again = again || (g.defined() && g.requires_grad());
+    if (!again) return grads;
+    for (at::Tensor& g : grads)
+        if (g.defined()) g = g.detach().requires_grad_(true);
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string("trying to differentiate ") + entry + " twice, whose backward has no gradient",
+        static_cast<int64_t>(grads.size()));
+    return (*error)(std::move(grads));
+}
+
+// Which of the node's inputs need a gradient now (those that were given, in
+// order, have the edges).
+std::vector<bool> needed(AutogradContext* ctx, std::initializer_list<bool> given) {
+    std::vector<bool> need;
+    size_t edge = 0;
+    for (bool there : given) need.push_back(there && ctx->needs_input_grad(edge++));
+    return need;
+}
+
+// What a node keeps beside its saved tensors, and its tensors without gradients.
+struct RopeHeld : torch::CustomClassHolder {
+    c10::optional<at::Tensor> positions, inv_freq;  // for the forward
+    double eps;
+    bool norm, interleaved;
+    std::vector<int64_t> sections;
+};
+struct ScanHeld : torch::CustomClassHolder {
+    c10::optional<at::Tensor> lengths;
+    int64_t form;
+    bool complement;
+};
+struct CrossHeld : torch::CustomClassHolder {
+    c10::optional<at::Tensor> lengths;
+};
+
+template <typename T>
+const T& held(AutogradContext* ctx) {
+    return static_cast<const T&>(*ctx->saved_data["held"].toCapsule());
+}
+
+struct NormRopeNode : torch::autograd::Function<NormRopeNode> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const c10::optional<at::Tensor>& k,
+                                 const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
+                                 const c10::intrusive_ptr<RopeHeld>& h) {
+        check_capture("race_norm_rope", {q, k, q_weight, k_weight});
+        const auto [q_out, k_out] = norm_rope_forward(q, k, h->positions, h->inv_freq, q_weight, k_weight, h->eps, h->norm,
+                                                      h->sections, h->interleaved);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, or_undefined(k), or_undefined(q_weight), or_undefined(k_weight),
+                                or_undefined(h->positions), or_undefined(h->inv_freq)});
+        h->positions = h->inv_freq = c10::nullopt;
+        ctx->saved_data["held"] = c10::IValue::make_capsule(h);
+        if (k_out) return {q_out, *k_out};
+        return {q_out};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list up) {
+        variable_list grads(5);
+        const variable_list saved = ctx->get_saved_variables();
+        const RopeHeld& h = held<RopeHeld>(ctx);
+        const at::Tensor& q = saved[0];
+        const auto k = if_defined(saved[1]), qw = if_defined(saved[2]), kw = if_defined(saved[3]);
+        check_capture("race_norm_rope backward", {q, k, qw, kw});
+        const auto dq = dense_grad(up[0], q.scalar_type());
+        const auto dk = up.size() > 1 ? dense_grad(up[1], q.scalar_type()) : c10::nullopt;
+        if (dq || dk) {
+            const auto need = needed(ctx, {true, k.has_value(), qw.has_value(), kw.has_value()});
+            const auto [a, b, c, d] = norm_rope_backward(q, k, if_defined(saved[4]), if_defined(saved[5]), qw, kw, dq, dk,
+                                                         h.eps, h.norm, h.sections, h.interleaved, need[0], need[1],
+                                                         need[2], need[3]);
+            grads = {or_undefined(a), or_undefined(b), or_undefined(c), or_undefined(d), at::Tensor()};
+        }
+        return differentiated_once("race_norm_rope", up, std::move(grads));
+    }
+};
+
+struct GatedScanNode : torch::autograd::Function<GatedScanNode> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate,
+                                 const c10::optional<at::Tensor>& state, const c10::intrusive_ptr<ScanHeld>& h) {
+        check_capture("race_gated_scan", {x, gate, state});
+        const auto [out, fin, records] = gated_scan_forward(x, gate, state, h->lengths, h->form, h->complement, true, false);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({x, gate, or_undefined(h->lengths), *records});
+        h->lengths = c10::nullopt;
+        ctx->saved_data["held"] = c10::IValue::make_capsule(h);
+        ctx->saved_data["state"] = state.has_value();
+        return {out, fin};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list up) {
+        variable_list grads(4);
+        const variable_list saved = ctx->get_saved_variables();
+        const ScanHeld& h = held<ScanHeld>(ctx);
+        const at::Tensor &x = saved[0], &gate = saved[1];
+        check_capture("race_gated_scan backward", {x, gate});
+        if (up[0].defined() || up[1].defined()) {
+            const auto need = needed(ctx, {true, true, ctx->saved_data["state"].toBool()});
+            const auto dout = dense_grad(up[0].defined() ? up[0] : at::zeros(x.sizes(), x.options()), x.scalar_type());
+            const auto [a, b, c] = gated_scan_backward(x, gate, if_defined(saved[2]), *dout, dense_grad(up[1], at::kFloat),
+                                                       saved[3], h.form, h.complement, need[0], need[1], need[2]);
+            grads = {or_undefined(a), or_undefined(b), or_undefined(c), at::Tensor()};
+        }
+        return differentiated_once("race_gated_scan", up, std::move(grads));
+    }
+};
+
+struct CrossNode : torch::autograd::Function<CrossNode> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                 const c10::intrusive_ptr<CrossHeld>& h) {
+        check_capture("race_cross_fwd", {q, k, v});
+        const auto [out, state] = cross_forward(q, k, v, h->lengths, true);
+        ctx->save_for_backward({q, k, v, or_undefined(h->lengths), *state});
+        return {*out};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list up) {
+        const variable_list saved = ctx->get_saved_variables();
+        check_capture("race_cross_fwd backward", {saved[0], saved[1], saved[2]});
+        const auto need = needed(ctx, {true, true, true});
+        const auto dout = dense_grad(up[0], saved[2].scalar_type());
+        const auto [a, b, c] = cross_backward(saved[0], saved[1], saved[2], if_defined(saved[3]), *dout, saved[4], need[0],
+                                              need[1], need[2]);
+        return differentiated_once("race_cross_fwd", up, {or_undefined(a), or_undefined(b), or_undefined(c), at::Tensor()});
+    }
+};
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> norm_rope(
+    const at::Tensor& q_in, const c10::optional<at::Tensor>& k_in, const c10::optional<at::Tensor>& positions,
+    const c10::optional<at::Tensor>& inv_freq, const c10::optional<at::Tensor>& q_weight,
+    const c10::optional<at::Tensor>& k_weight, c10::optional<double> eps, const std::vector<int64_t>& sections,
+    bool interleaved) {
+    const at::Tensor q = as_rows(q_in);
+    c10::optional<at::Tensor> k;
+    if (k_in) k = as_rows(*k_in);
+    if (!wants_grad({q, k, q_weight, k_weight}))
+        return norm_rope_forward(q, k, positions, inv_freq, q_weight, k_weight, eps.value_or(0.0), eps.has_value(),
+                                 sections, interleaved);
+    auto h = c10::make_intrusive<RopeHeld>();
+    h->positions = positions, h->inv_freq = inv_freq;
+    h->eps = eps.value_or(0.0), h->norm = eps.has_value();
+    h->sections = sections, h->interleaved = interleaved;
+    const variable_list outs = NormRopeNode::apply(q, k, q_weight, k_weight, h);
+    return {outs[0], outs.size() > 1 ? c10::optional<at::Tensor>(outs[1]) : c10::nullopt};
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x_in, const at::Tensor& gate_in,
+                                              const c10::optional<at::Tensor>& state,
+                                              const c10::optional<at::Tensor>& lengths_in, int64_t form, bool complement) {
+    const at::Tensor x = as_rows(x_in, RACE_SCAN_MAX_TOKEN_STRIDE), gate = as_rows(gate_in, RACE_SCAN_MAX_TOKEN_STRIDE);
+    const auto lengths = as_lengths(lengths_in);
+    if (!wants_grad({x, gate, state})) {
+        const auto r = gated_scan_forward(x, gate, state, lengths, form, complement, false, false);
+        return {std::get<0>(r), std::get<1>(r)};
+    }
+    auto h = c10::make_intrusive<ScanHeld>();
+    h->lengths = lengths, h->form = form, h->complement = complement;
+    const variable_list outs = GatedScanNode::apply(x, gate, state, h);
+    return {outs[0], outs[1]};
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_scan_carry(const at::Tensor& x, const at::Tensor& gate, const at::Tensor& state,
+                                                    const c10::optional<at::Tensor>& lengths, int64_t form,
+                                                    bool complement, bool inplace) {
+    const auto r = gated_scan_forward(as_rows(x, RACE_SCAN_MAX_TOKEN_STRIDE), as_rows(gate, RACE_SCAN_MAX_TOKEN_STRIDE),
+                                      state, as_lengths(lengths), form, complement, false, inplace);
+    return {std::get<0>(r), std::get<1>(r)};
+}
+
+at::Tensor cross(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths) {
+    if (!wants_grad({q, k, v})) return *std::get<0>(cross_forward(q, k, v, as_lengths(lengths), false));
+    auto h = c10::make_intrusive<CrossHeld>();
+    h->lengths = as_lengths(lengths);
+    return CrossNode::apply(q, k, v, h)[0];
+}
+
+at::Tensor cross_state(const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths) {
+    return *std::get<1>(cross_forward(c10::nullopt, k, v, as_lengths(lengths), true));
+}
+
 void bind_operators(pybind11::module& m) {
     namespace py = pybind11;
+    m.def("norm_rope", &norm_rope, "race_norm_rope with its gradients -> (q, k or None)", py::arg("q"), py::arg("k"),
+          py::arg("positions"), py::arg("inv_freq"), py::arg("q_weight"), py::arg("k_weight"), py::arg("eps"),
+          py::arg("sections"), py::arg("interleaved"));
+    m.def("gated_scan", &gated_scan, "race_gated_scan with its gradients -> (out, final state)", py::arg("x"),
+          py::arg("gate"), py::arg("state"), py::arg("lengths"), py::arg("form"), py::arg("complement"));
+    m.def("gated_scan_carry", &gated_scan_carry, "race_gated_scan from a carried state -> (out, state)", py::arg("x"),
+          py::arg("gate"), py::arg("state"), py::arg("lengths"), py::arg("form"), py::arg("complement"),
+          py::arg("inplace"));
+    m.def("cross", &cross, "race_cross_fwd with its gradients -> out", py::arg("probsQ"), py::arg("probsK"), py::arg("V"),
+          py::arg("lengths"));
+    m.def("cross_state", &cross_state, "The sums race_cross_query reads", py::arg("probsK"), py::arg("V"),
+          py::arg("lengths"));
     m.def("cross_forward", &cross_forward, "The non-causal op over another sequence's keys -> (out, state)",
           py::arg("probsQ"), py::arg("probsK"), py::arg("V"), py::arg("lengths"), py::arg("want_state"));
     m.def("cross_query", &cross_query, "Queries against a kept state -> out", py::arg("probsQ"), py::arg("state"));
     m.def("cross_backward", &cross_backward, "Gradients of cross_forward -> (dQ, dK, dV)", py::arg("probsQ"),
           py::arg("probsK"), py::arg("V"), py::arg("lengths"), py::arg("dout"), py::arg("state"), py::arg("need_q"),
           py::arg("need_k"), py::arg("need_v"));
-    m.def("check_capture", &check_capture, "Refuses a capture whose backward would wait for the default stream",
-          py::arg("entry"), py::arg("inputs"));
     m.def("norm_rope_forward", &norm_rope_forward, "Heads normed and rotated, to streams -> (q, k or None)",
           py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"), py::arg("q_weight"),
           py::arg("k_weight"), py::arg("eps"), py::arg("norm"), py::arg("sections"), py::arg("interleaved"));

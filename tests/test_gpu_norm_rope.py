@@ -336,6 +336,27 @@ def test_other_stream_and_captured_steps(race, cuda):
         assert all(torch.equal(a, b) for a, b in zip(outs, eager)), i
 
 
+def test_differentiating_twice_is_refused(race, cuda):
+    q, _, qw, _, dq, _ = make(1, 20, 2, 1, 64, torch.float32, 12, cuda)
+    leaf, up = q.contiguous().requires_grad_(True), dq.clone().requires_grad_(True)
+    out, _ = race.race_norm_rope(leaf, None, torch.arange(20, device=cuda), freqs(32, cuda), q_weight=qw)
+    (g,) = torch.autograd.grad(out, leaf, up, create_graph=True)
+    check(g, reference(q, qw, torch.arange(20, device=cuda), freqs(32, cuda), None, False, 1e-6, dq)["dx"], "first")
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+
+
+def test_inputs_changed_before_the_backward_are_refused(race, cuda):
+    q, _, _, _, dq, _ = make(1, 20, 2, 1, 64, torch.float32, 13, cuda)
+    leaf, pos = q.contiguous().requires_grad_(True), torch.arange(20, device=cuda)
+    for change in (lambda: pos.add_(1), lambda: mid.mul_(2)):
+        mid = leaf * 1.0
+        out, _ = race.race_norm_rope(mid, None, pos, freqs(32, cuda))
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, leaf, dq)
+
+
 def test_a_live_eager_graph_refuses_the_capture(race, cuda):
     # The backward would wait for the default stream inside the capture.
     q, _, _, _, dq, _ = make(1, 40, 2, 1, 64, torch.float32, 11, cuda)
