@@ -613,7 +613,7 @@ race_status race_norm_rope_bwd(const void* q, const void* k, const void* positio
  * token), and a backward.  No counterpart in the reference. */
 typedef enum race_gate {
     RACE_GATE_SIGMOID = 0, /* gate holds logits: a = 1 / (1 + exp(-gate)) */
-    RACE_GATE_LOG = 1      /* gate holds log a: a = exp(gate); -inf starts anew */
+    RACE_GATE_LOG = 1      /* gate holds log a <= 0: a = exp(gate); -inf starts anew */
 } race_gate;
 
 /* x and gate are [num_streams][seq_len][channels] with the strides given (in

@@ -591,8 +591,10 @@ using NarrowSplit = ScanShape<4, 16, 256, 256>;
 using Single = ScanShape<1, 64, 512, 512, 8, 8>;  // any strides and widths
 
 // Workgroups that fill the device without a split of the tokens, and that a
-// split aims for.
-constexpr int64_t kScanEnough = 200, kScanSplit = 512;
+// split aims for; a split costs a launch, two tiles cost less (10 x 160 x 24,
+// two tiles, 7.6 + 11.2 us whole and 9.9 + 13.3 split; 2 x 290 x 64, three, 10.2 +
+// 17.3 and 9.5 + 13.0).
+constexpr int64_t kScanEnough = 200, kScanSplit = 512, kScanWhole = 2;
 
 int64_t blocks_of(const GatedScan& s, int64_t channels) { return s.N * ((s.D + channels - 1) / channels); }
 
@@ -717,7 +719,7 @@ int64_t scan_tiles(const GatedScan& s) {
 int64_t scan_segments(const GatedScan& s) {
     const int64_t tile = forward_tile(s), tiles = (s.T + tile - 1) / tile;
     const int64_t base = by_shape(s, [&](auto shape) { return blocks_of(s, decltype(shape)::kChannels); });
-    if (base >= kScanEnough || tiles <= 1) return 1;
+    if (base >= kScanEnough || tiles <= kScanWhole) return 1;
     const int64_t per = (tiles + kScanSplit / base - 1) / (kScanSplit / base);  // tiles of a segment
     return (tiles + per - 1) / per;
 }

@@ -104,7 +104,9 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> gated_scan_forward
     const at::Tensor& x, const at::Tensor& gate, const c10::optional<at::Tensor>& state,
     const c10::optional<at::Tensor>& lengths, int64_t form, bool complement, bool want_records, bool inplace) {
     const race_scan_shape sh = scan_shape("race_gated_scan", x, gate, state, lengths, form, complement);
-    TORCH_CHECK(!inplace || state, "race_gated_scan: an in-place call needs a state");
+    TORCH_CHECK(!inplace || state, "race_gated_scan_carry: an in-place call needs a state");
+    TORCH_CHECK(!inplace || !(at::GradMode::is_enabled() && state->requires_grad()),
+                "race_gated_scan_carry: a state that requires a gradient cannot be advanced in place");
     const c10::DeviceGuard guard(x.device());
     const at::Tensor out = at::empty(x.sizes(), x.options());
     const auto fopt = x.options().dtype(at::kFloat);
@@ -120,6 +122,7 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> gated_scan_forward
                                      fin.data_ptr<float>(), floats_of(records), &sh, bytes > 0 ? ws.data_ptr() : nullptr,
                                      bytes, current_stream()),
                  "race_gated_scan_fwd");
+    if (inplace) state->unsafeGetTensorImpl()->bump_version();  // a graph that saved it must notice
     return {out, fin, records};
 }
 

@@ -30,8 +30,9 @@ def race_gated_scan(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor | N
     Args:
         x, gate: [N, T, D] float32 or bfloat16, of any stream and token strides.
         state: [N, D] float32, the state before the first token; None is zero.
-        gate_form: "sigmoid" (gate holds logits) or "log" (gate holds log a;
-            -inf forgets everything before the token).
+        gate_form: "sigmoid" (gate holds logits) or "log" (gate holds log a, 0 at
+            most: products of larger ones may overflow; -inf forgets everything
+            before the token).
         complement: u = (1 - a) x, else u = x.
         lengths: int32 (or int64) [N] or [N / g] (entry i for the streams g i .. g i + g - 1):
             tokens from lengths on are not read, their rows of out are zero and

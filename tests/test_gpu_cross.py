@@ -269,6 +269,32 @@ def test_other_stream_and_captured_steps(race, cuda):
     del held
 
 
+@pytest.mark.parametrize("S, d, Tq", [(64, 64, 200), (64, 64, 9), (256, 128, 70), (30, 50, 40)])
+def test_c_entry_with_used_memory(race, cuda, S, d, Tq):
+    from race_attention_kernel_amd import abi
+
+    N, Tk = 2, 5000
+    q, k, v, g = make(N, N, Tq, Tk, 1, S, d, torch.float32, 7, cuda)
+    n = torch.tensor([5000, 2100], dtype=torch.int32, device=cuda)
+    sh = abi.cross_shape(N, Tq, Tk, 1, S, d)
+    nan = lambda *s: torch.full(s, float("nan"), device=cuda)
+    (_, fwd), (_, bwd) = abi.cross_workspace_bytes(sh), abi.cross_workspace_bytes(sh, True)
+    ws, state = nan(max(fwd, bwd) // 4), nan(N, S * d + S)
+    out, dq, dk, dv = nan(N, Tq, d), nan(N, Tq, S), nan(N, Tk, S), nan(N, Tk, d)
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()
+    assert abi.cross_fwd(p(q), p(k), p(v), p(n), p(out), p(state), sh, p(ws), fwd, stream) == 0
+    ws.fill_(float("nan"))
+    assert abi.cross_bwd(p(q), p(k), p(v), p(n), p(g), p(state), p(dq), p(dk), p(dv), sh, p(ws), bwd, stream) == 0
+    again = nan(N, Tq, d)
+    assert abi.cross_query(p(q), p(state), p(again), sh, stream) == 0
+    torch.cuda.synchronize()
+    ref = reference(q, k, v, n, g)
+    for name, got in (("out", out), ("state", state), ("dq", dq), ("dk", dk), ("dv", dv), ("out", again)):
+        check(got, ref[name], f"c entry {name}")
+    assert abi.cross_fwd(p(q), p(k), p(v), p(n), p(out), p(state), sh, p(ws), fwd - 4, stream) == 1
+
+
 def test_offsets_past_32_bits(race, cuda):
     # 4.4 GB of key probabilities: the last stream against itself alone.
     N, Tk, S, d = 17, 65536, 256, 16

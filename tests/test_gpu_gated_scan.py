@@ -355,6 +355,58 @@ def test_other_streams_and_captured_steps(race, cuda):
         assert torch.equal(decoded, wd) and torch.equal(carried, ws), i
 
 
+def test_refusals(race, cuda):
+    x, gate, state, _, _ = make(2, 20, 64, torch.float32, "sigmoid", 18, cuda)
+    for args, kw, message in [
+        ((x[0], gate[0]), {}, "x has shape"), ((x, gate[:, :19]), {}, "gate has shape"), ((x, gate.bfloat16()), {}, "another dtype"),
+        ((x.half(), gate.half()), {}, "neither float32 nor bfloat16"), ((x, gate.cpu()), {}, "CPU"),
+        ((x, gate, state[:1]), {}, "state has shape"), ((x, gate, state.double()), {}, "state must be float32"),
+        ((x, gate, state.t().contiguous().t()), {}, "strided view"),
+        ((x, gate), dict(lengths=torch.zeros(3, dtype=torch.int32, device=cuda)), "do not divide"),
+        ((x, gate), dict(lengths=torch.zeros(2, device=cuda)), "int32"),
+        ((x, gate), dict(lengths=torch.zeros(2, dtype=torch.int32)), "rows' device"),
+        ((x[..., :0], gate[..., :0]), {}, "1 .. 65536 channels"),
+    ]:
+        with pytest.raises(RuntimeError, match=message):
+            race.race_gated_scan(*args, **kw)
+    state.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="in place"):
+        race.race_gated_scan_carry(x, gate, state, inplace=True)
+    # A graph that saved the state notices that it was advanced.
+    carried = state.detach().clone()
+    leaf = torch.ones_like(carried, requires_grad=True)
+    product = (leaf * carried).sum()
+    race.race_gated_scan_carry(x, gate, carried, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+
+
+def test_c_entry_with_used_memory(race, cuda):
+    # Outputs, records and workspace full of NaN before the calls; two streams of lengths.
+    from race_attention_kernel_amd import abi
+
+    N, T, D = 2, 3000, 64
+    x, gate, state, dout, dfinal = make(N, T, D, torch.float32, "sigmoid", 19, cuda)
+    sh = abi.scan_shape(N, T, D)
+    n = torch.tensor([3000, 1500], dtype=torch.int32, device=cuda)
+    st, nbytes, floats = abi.gated_scan_workspace_bytes(sh)
+    _, back, _ = abi.gated_scan_workspace_bytes(sh, True)
+    nan = lambda *s: torch.full(s, float("nan"), device=cuda)
+    ws, rec, out, final = nan(max(nbytes, back) // 4 + 4), nan(floats), nan(N, T, D), nan(N, D)
+    dx, dg, ds = nan(N, T, D), nan(N, T, D), nan(N, D)
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()
+    assert abi.gated_scan_fwd(p(x), p(gate), p(state), p(n), p(out), p(final), p(rec), sh, p(ws), nbytes, stream) == 0
+    ws.fill_(float("nan"))
+    assert abi.gated_scan_bwd(p(x), p(gate), p(n), p(dout), p(dfinal), p(rec), p(dx), p(dg), p(ds), sh, p(ws), back,
+                              stream) == 0
+    torch.cuda.synchronize()
+    ref = reference(x, gate, state, n, "sigmoid", True, dout, dfinal)
+    for name, got in (("out", out), ("final", final), ("dx", dx), ("dgate", dg), ("dstate", ds)):
+        check(got, ref[name], "c entry " + name)
+    assert abi.gated_scan_fwd(p(x), p(gate), p(state), p(n), p(out), p(final), p(rec), sh, p(ws), nbytes - 4, stream) == 1
+
+
 def test_a_live_eager_graph_refuses_the_capture(race, cuda):
     # The backward would wait for the default stream inside the capture.
     x, gate, _, _, _ = make(1, 40, 64, torch.float32, "sigmoid", 17, cuda)

@@ -357,6 +357,32 @@ def test_inputs_changed_before_the_backward_are_refused(race, cuda):
             torch.autograd.grad(out, leaf, dq)
 
 
+def test_c_entry_with_used_memory(race, cuda):
+    from race_attention_kernel_amd import abi
+
+    B, T, Hq, Hk, d = 2, 300, 6, 2, 64
+    q, k, qw, kw, dq, dk = make(B, T, Hq, Hk, d, torch.float32, 14, cuda)
+    q, k, freq = q.contiguous(), k.contiguous(), freqs(32, cuda)
+    pos = torch.randint(0, 5000, (B, T), device=cuda, dtype=torch.int32)
+    sh = abi.norm_rope_shape(B, T, Hq, Hk, d, 32, pos_bits=32)
+    st, nbytes = abi.norm_rope_bwd_workspace_bytes(sh)
+    nan = lambda *s: torch.full(s, float("nan"), device=cuda)
+    outs, grads, ws = [nan(B * Hq, T, d), nan(B * Hk, T, d)], [nan(*t.shape) for t in (q, k, qw, kw)], nan(nbytes // 4)
+    stream = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()
+    assert abi.norm_rope_fwd(p(q), p(k), p(pos), p(freq), p(qw), p(kw), p(outs[0]), p(outs[1]), sh, stream) == 0
+    assert abi.norm_rope_bwd(p(q), p(k), p(pos), p(freq), p(qw), p(kw), p(dq), p(dk), *map(p, grads), sh, p(ws), nbytes,
+                             stream) == 0
+    torch.cuda.synchronize()
+    for i, (x, w, up) in enumerate(((q, qw, dq), (k, kw, dk))):
+        ref = reference(x, w, pos, freq, None, False, 1e-6, up)
+        check(outs[i], ref["out"], "c entry out")
+        check(grads[i], ref["dx"], "c entry dx")
+        check(grads[2 + i], ref["dw"], "c entry dw")
+    assert abi.norm_rope_bwd(p(q), p(k), p(pos), p(freq), p(qw), p(kw), p(dq), p(dk), *map(p, grads), sh, p(ws),
+                             nbytes - 4, stream) == 1
+
+
 def test_a_live_eager_graph_refuses_the_capture(race, cuda):
     # The backward would wait for the default stream inside the capture.
     q, _, _, _, dq, _ = make(1, 40, 2, 1, 64, torch.float32, 11, cuda)
