@@ -1,6 +1,6 @@
 // noncausal_mfma.hip -- bucket reductions and token maps of the non-causal
-// forward and backward on the fp32 matrix cores, for widths that are multiples
-// of 4 (analysis/hot-path.md:157-162 and its VJP):
+// forward and backward on the matrix cores (analysis/hot-path.md:157-162 and its
+// VJP):
 //   reduction  R[a][b] = sum_t x[t][a] y[t][b],  colsum[a] = sum_t x[t][a]
 //              (B = K^T V and A in the forward, dE = Q^T dOut in the backward)
 //   map        out[t][c] = sum_a x[t][a] M[a][c] (+ bias[c])
@@ -42,6 +42,14 @@
 //     -> 9 / 11 / 13 / 15: launches of one workgroup per stream, bound by the
 //     latency of staging, the loop's few steps and the launch itself.
 // Other widths (S 12 .. 256, d 20 .. 128) ran 1.2x (100 x 36, fp32) to 9x.
+//
+// Widths that are no multiples of four (kParts; cross attention's) run the same
+// products, their rows loaded and stored value by value and maps in fp32.
+// Against the scalar kernels, forward / backward in us: fp32, 88 streams of 300
+// and 1000 tokens, S = 128, d = 17: 210 / 280 -> 37 / 84; bf16, 64 streams of
+// 1000 and 2000, S = 64, d = 50: 175 / 192 -> 35 / 87; bf16, 16 streams of 1000
+// and 2000, S = 256, d = 125: 520 / 658 -> 68 / 161.  Bound by the number of
+// loads, one a value.
 #include <algorithm>
 
 #include "mfma_common.h"
@@ -81,6 +89,28 @@ struct Vec {
             v = mfma::buf_load8<P>(r, off);
         else
             v = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, P);
+    }
+    // The first `left` of them one by one (rows that are no whole pieces), the
+    // others zero; or, not kParts, all or none.
+    template <bool kParts, int P = mfma::kPolicyDefault>
+    __device__ __forceinline__ void load_row(__amdgpu_buffer_rsrc_t r, int off, int left) {
+        if constexpr (kParts) {
+            uint32_t w[kBytes / 4];
+#pragma unroll
+            for (int i = 0; i < kBytes / 4; ++i) {
+                if constexpr (sizeof(TIn) == 4) {
+                    w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, i < left ? off + 4 * i : kOutside, 0, P);
+                } else {
+                    const uint32_t lo = __builtin_amdgcn_raw_buffer_load_b16(r, 2 * i < left ? off + 4 * i : kOutside, 0, P);
+                    const uint32_t hi =
+                        __builtin_amdgcn_raw_buffer_load_b16(r, 2 * i + 1 < left ? off + 4 * i + 2 : kOutside, 0, P);
+                    w[i] = (lo & 0xffffu) | hi << 16;
+                }
+            }
+            v = __builtin_bit_cast(Raw, w);
+        } else {
+            load<P>(r, left > 0 ? off : kOutside);
+        }
     }
     __device__ __forceinline__ uint32_t word(int i) const {
         if constexpr (kBytes == 16)
@@ -191,6 +221,7 @@ struct Outer {
     // two LDS buffers of kBlockFloats, and the column sums over lane groups
     // and waves in order; rows a0 .., columns b0 .. of the record `r`
     // ([Wa][Wb], then the column sums when `sums` asks for them).
+    template <bool kParts>
     __device__ __forceinline__ void combine(float* __restrict__ lds, float* __restrict__ r, int Wa, int Wb,
                                             int a0, int b0, bool sums, int w, int g, int lr) {
         float* cs = lds + 2 * kBlockFloats;  // [4 waves][4 groups][16 EA]
@@ -205,10 +236,17 @@ struct Outer {
         const int rows = min(16 * EA, Wa - a0), cols = min(16 * EB, Wb - b0);
         for (int e = threadIdx.x; e < 16 * EA * 4 * EB; e += kThreads) {
             const int a = e / (4 * EB), c = 4 * (e % (4 * EB));
-            if (a < rows && c < cols)
-                *reinterpret_cast<f32x4*>(r + int64_t(a0 + a) * Wb + b0 + c) =
-                    *reinterpret_cast<const f32x4*>(lds + a * 16 * EB + c) +
-                    *reinterpret_cast<const f32x4*>(lds + kBlockFloats + a * 16 * EB + c);
+            if (a >= rows || c >= cols) continue;
+            const f32x4 sum = *reinterpret_cast<const f32x4*>(lds + a * 16 * EB + c) +
+                              *reinterpret_cast<const f32x4*>(lds + kBlockFloats + a * 16 * EB + c);
+            float* at = r + int64_t(a0 + a) * Wb + b0 + c;
+            if constexpr (kParts) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c + i < cols) at[i] = sum[i];
+            } else {
+                *reinterpret_cast<f32x4*>(at) = sum;
+            }
         }
         if (sums && int(threadIdx.x) < rows) {
             float s = 0.f;
@@ -239,7 +277,7 @@ __device__ __forceinline__ void stream_block(int64_t id, int64_t N, int per, int
 // kEndFirst (the causal tile sums, whose tiles the output pass then walks from
 // their start): the steps go from the chunk's end to its start, past the
 // caches except for the first `kept` rows (cache_kept_rows), which come last.
-template <typename TIn, int EA, int EB, bool kEndFirst>
+template <typename TIn, int EA, int EB, bool kEndFirst, bool kParts>
 __global__ __launch_bounds__(kThreads, 3) void nc_sums_kernel(
     const TIn* __restrict__ x, const TIn* __restrict__ y, float* __restrict__ records, int64_t T, int chunk,
     int64_t chunks, int64_t rec, int Wa, int Wb, int bblocks, int kept, const Live live, int64_t N, int flat) {
@@ -268,8 +306,8 @@ __global__ __launch_bounds__(kThreads, 3) void nc_sums_kernel(
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int row = r0 + 4 * i + g;
-            xv[i].template load<P>(xr, ca < Wa ? (row * Wa + ca) * es : kOutside);
-            yv[i].template load<P>(yr, cb < Wb ? (row * Wb + cb) * es : kOutside);
+            xv[i].template load_row<kParts, P>(xr, (row * Wa + ca) * es, Wa - ca);
+            yv[i].template load_row<kParts, P>(yr, (row * Wb + cb) * es, Wb - cb);
         }
     };
     using Alloc = std::integral_constant<int, mfma::kPolicyDefault>;
@@ -300,7 +338,7 @@ __global__ __launch_bounds__(kThreads, 3) void nc_sums_kernel(
 #pragma unroll 2
         for (int r0 = kTok * w; r0 < rows; r0 += kAll) step(Alloc{}, r0 + kAll);
     }
-    o.combine(smem, records + (n * chunks + ci) * rec, Wa, Wb, a0, b0, b0 == 0, w, g, lr);
+    o.template combine<kParts>(smem, records + (n * chunks + ci) * rec, Wa, Wb, a0, b0, b0 == 0, w, g, lr);
 }
 
 // ---------------------------------------------------------------------------
@@ -325,11 +363,12 @@ struct MapRows {
     V x[kOps];
 
     // Unit i 64 + lane of the 16 rows (row-major): a load covers whole rows.
+    template <bool kParts = false>
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int row0, int W, int lane) {
 #pragma unroll
         for (int i = 0; i < kOps; ++i) {
             const int u = i * 64 + lane, row = u / kUnits, c = (u % kUnits) * kPer;
-            x[i].load(r, c < W ? ((row0 + row) * W + c) * int(sizeof(TIn)) : kOutside);
+            x[i].template load_row<kParts>(r, ((row0 + row) * W + c) * int(sizeof(TIn)), W - c);
         }
     }
     // From the loads' layout to the operands', through kBytes of LDS that only
@@ -463,7 +502,7 @@ struct OutRows {
     }
     // Rows row0 .. of the view `o`, row length W; columns c0 .. of it, ncols of
     // them.  `replace` runs with the results in `t`.
-    template <typename Replace>
+    template <bool kParts = false, typename Replace>
     __device__ __forceinline__ static void store(Raw* __restrict__ t, const f32x4 (&acc)[NCB], __amdgpu_buffer_rsrc_t o,
                                                  int row0, int W, int c0, int ncols, int lane, int g, int lr,
                                                  Replace replace) {
@@ -477,7 +516,17 @@ struct OutRows {
             const int u = i * 64 + lane, row = u / kUnits, c = 4 * (u % kUnits);
             const int off = c < ncols ? ((row0 + row) * W + c0 + c) * int(sizeof(TIn)) : kOutside;
             const Raw v = t[at(row, u % kUnits)];
-            if constexpr (sizeof(TIn) == 4)
+            if constexpr (kParts) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int to = c + i < ncols ? off + i * int(sizeof(TIn)) : kOutside;
+                    if constexpr (sizeof(TIn) == 4)
+                        __builtin_amdgcn_raw_buffer_store_b32(v[i], o, to, 0, mfma::kPolicyDefault);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b16(uint16_t(v[i >> 1] >> (16 * (i & 1))), o, to, 0,
+                                                              mfma::kPolicyDefault);
+                }
+            } else if constexpr (sizeof(TIn) == 4)
                 __builtin_amdgcn_raw_buffer_store_b128(v, o, off, 0, kNcStorePolicy);
             else
                 __builtin_amdgcn_raw_buffer_store_b64(v, o, off, 0, kNcStorePolicy);
@@ -526,11 +575,12 @@ __device__ __forceinline__ void whole_products(typename OutRows<TIn, NCB>::Raw* 
 // by s), taken plain (M[s][c]) or transposed (M[c][s]); a thread takes four
 // consecutive c of a row, the loads of four such groups and two parts in
 // flight together.
-template <int NT, int NJ, int NCB, bool kB16>
+// kParts: widths that are no multiples of four, value by value.
+template <int NT, int NJ, int NCB, bool kB16, bool kParts = false>
 __device__ __forceinline__ void stage_operand(float* __restrict__ dst, const MapOperand& op, int64_t n, int Wa,
                                               int c0, int ncols, bool first_block, bool first_slice) {
     constexpr int kCols = 16 * NCB, kRows = kB16 ? 32 * ((NJ + 1) / 2) : 16 * NJ, kQuads = kRows * kCols / 4;
-    const bool plain = op.col == 1;
+    const bool plain = op.div ? !op.div_by_col : op.col == 1;  // at one column both strides are one
     const int64_t ld = plain ? op.row : op.col;
     const float* mn = op.m + n * op.stream;
     const float* dv = op.div ? op.div + n * op.div_stream : nullptr;
@@ -560,8 +610,18 @@ __device__ __forceinline__ void stage_operand(float* __restrict__ dst, const Map
             float q0[kPer], q1[kPer];
 #pragma unroll
             for (int m = 0; m < kPer; ++m) {
-                v0[m] = *reinterpret_cast<const f32x4*>(mn + at[m] + o0);
-                v1[m] = *reinterpret_cast<const f32x4*>(mn + at[m] + o1);
+                if constexpr (kParts) {
+                    // Values past the row's end are not read (and not used).
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int in = i < (plain ? ncols - col[m] : Wa - row[m]) ? i : 0;
+                        v0[m][i] = mn[at[m] + o0 + in];
+                        v1[m][i] = mn[at[m] + o1 + in];
+                    }
+                } else {
+                    v0[m] = *reinterpret_cast<const f32x4*>(mn + at[m] + o0);
+                    v1[m] = *reinterpret_cast<const f32x4*>(mn + at[m] + o1);
+                }
                 q0[m] = dv ? dv[div[m] + o0] : 0.f;
                 q1[m] = dv ? dv[div[m] + o1] : 0.f;
             }
@@ -578,8 +638,15 @@ __device__ __forceinline__ void stage_operand(float* __restrict__ dst, const Map
 #pragma unroll
         for (int m = 0; m < kPer; ++m) {
             if (e0 + int(threadIdx.x) + m * NT >= kQuads) continue;
+            const int left = plain ? ncols - col[m] : Wa - row[m];  // values of the four that are there
             if (sv && ok[m]) {
-                *reinterpret_cast<f32x4*>(sv + at[m]) = v[m];
+                if constexpr (kParts) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < left) sv[at[m] + i] = v[m][i];
+                } else {
+                    *reinterpret_cast<f32x4*>(sv + at[m]) = v[m];
+                }
                 // Each divisor once: by the first values of its row of m.
                 if (dv && (plain ? col[m] == 0 && first_slice : row[m] == 0)) sv[op.save_div_off + div[m]] = q[m];
             }
@@ -587,6 +654,10 @@ __device__ __forceinline__ void stage_operand(float* __restrict__ dst, const Map
             if (dv && ok[m]) {
                 const float den = q[m] + kEps;
                 x = f32x4{x[0] / den, x[1] / den, x[2] / den, x[3] / den};
+            }
+            if constexpr (kParts) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = i < left ? x[i] : 0.f;
             }
             if (plain)
                 put_matrix<NCB, kB16, true>(dst, row[m], col[m], x);
@@ -600,7 +671,7 @@ __device__ __forceinline__ void stage_operand(float* __restrict__ dst, const Map
 // output columns); wave w takes the 16-token tiles w, w + NW, ..  Rows of up to
 // 128 values are loaded as whole rows a tile ahead; longer ones straight in
 // the operands' layout (their turn would take 64 KB of LDS).
-template <typename TIn, int NJ, int NCB, bool kB16, int NW>
+template <typename TIn, int NJ, int NCB, bool kB16, int NW, bool kParts>
 __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__ x, TIn* __restrict__ out,
                                                           const MapOperand op, int64_t N, int64_t T, int Wa,
                                                           int Wb, int wg_tokens, int per, const Live live, int slices) {
@@ -628,18 +699,18 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
     const auto orr = mfma::make_rsrc(out + (n * T + t0) * Wb, int64_t(rows) * Wb * es);
     auto load = [&](X& v, int row0) {
         if constexpr (kTurn) {
-            v.load(xr, row0, Wa, lane);
+            v.template load<kParts>(xr, row0, Wa, lane);
         } else {
 #pragma unroll
             for (int j = 0; j < X::kOps; ++j) {
                 const int c = X::kPer * (4 * j + g);
-                v.x[j].load(xr, c < Wa ? ((row0 + lr) * Wa + c) * es : kOutside);
+                v.x[j].template load_row<kParts>(xr, ((row0 + lr) * Wa + c) * es, Wa - c);
             }
         }
     };
     X next;
     load(next, 16 * w);
-    stage_operand<64 * NW, NJ, NCB, kB16>(smem, op, n, Wa, c0, ncols, blk == 0, slice == 0);
+    stage_operand<64 * NW, NJ, NCB, kB16, kParts>(smem, op, n, Wa, c0, ncols, blk == 0, slice == 0);
     auto bias_of = [&](int cb, int g) {
         f32x4 b;
 #pragma unroll
@@ -667,7 +738,7 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
             for (int cb = 0; cb < NCB; ++cb) acc[cb] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         typename O::Raw* to = reinterpret_cast<typename O::Raw*>(mine);
-        O::store(to, acc, orr, r0, Wb, c0, ncols, lane, g, lr, [&] {
+        O::template store<kParts>(to, acc, orr, r0, Wb, c0, ncols, lane, g, lr, [&] {
             if constexpr (kB16) {
                 if (bad) whole_products<TIn, NJ, NCB>(to, bad, xr, r0, Wa, smem, lane, bias_of);
             }
@@ -1013,7 +1084,7 @@ __global__ __launch_bounds__(kThreads, 2) void nc_query64_kernel(
             });
         }
     }
-    o.combine(smem, records + (n * chunks + ci) * rec, W, W, 0, 0, false, w, g, lr);
+    o.template combine<false>(smem, records + (n * chunks + ci) * rec, W, W, 0, 0, false, w, g, lr);
 }
 
 // Key side: one workgroup per (block of wg_tokens tokens, stream).  dB and dA
@@ -1180,31 +1251,31 @@ int map_wg_tokens(const Problem& p, int slices) {
     return int(((p.T + per - 1) / per + 15) / 16 * 16);
 }
 
-template <typename TIn, int EA, int EB, bool kEndFirst = false>
+template <typename TIn, int EA, int EB, bool kEndFirst = false, bool kParts = false>
 hipError_t launch_sums_e(const void* x, const void* y, float* records, const Problem& p, int Wa, int Wb,
                          hipStream_t stream) {
     const int ab = (Wa + 16 * EA - 1) / (16 * EA), bb = (Wb + 16 * EB - 1) / (16 * EB);
     const int64_t all = p.tiles * p.N * ab * bb;
     const bool flat = ab * bb > 1 && all * kThreads < (int64_t(1) << 32);
     const dim3 grid = flat ? dim3(unsigned(all)) : dim3(unsigned(p.tiles), unsigned(p.N), unsigned(ab * bb));
-    nc_sums_kernel<TIn, EA, EB, kEndFirst><<<grid, kThreads, Outer<EA, EB>::kLdsFloats * sizeof(float), stream>>>(
+    nc_sums_kernel<TIn, EA, EB, kEndFirst, kParts><<<grid, kThreads, Outer<EA, EB>::kLdsFloats * sizeof(float), stream>>>(
         static_cast<const TIn*>(x), static_cast<const TIn*>(y), records, p.T, p.tile, p.tiles, p.rec, Wa, Wb, bb,
         kEndFirst ? cache_kept_rows(p) : 0, p.live, p.N, flat ? ab * bb : 0);
     return hipGetLastError();
 }
 
-template <typename TIn>
+template <typename TIn, bool kParts>
 hipError_t launch_sums_t(const void* x, const void* y, float* records, const Problem& p, int Wa, int Wb,
                          hipStream_t stream) {
     // bf16 vectors are at least one word.
     const int ea = lane_values(Wa) < 2 ? 2 : lane_values(Wa), eb = lane_values(Wb) < 2 ? 2 : lane_values(Wb);
-    if (ea == 2 && eb == 2) return launch_sums_e<TIn, 2, 2>(x, y, records, p, Wa, Wb, stream);
-    if (ea == 2) return launch_sums_e<TIn, 2, 4>(x, y, records, p, Wa, Wb, stream);
-    if (eb == 2) return launch_sums_e<TIn, 4, 2>(x, y, records, p, Wa, Wb, stream);
-    return launch_sums_e<TIn, 4, 4>(x, y, records, p, Wa, Wb, stream);
+    if (ea == 2 && eb == 2) return launch_sums_e<TIn, 2, 2, false, kParts>(x, y, records, p, Wa, Wb, stream);
+    if (ea == 2) return launch_sums_e<TIn, 2, 4, false, kParts>(x, y, records, p, Wa, Wb, stream);
+    if (eb == 2) return launch_sums_e<TIn, 4, 2, false, kParts>(x, y, records, p, Wa, Wb, stream);
+    return launch_sums_e<TIn, 4, 4, false, kParts>(x, y, records, p, Wa, Wb, stream);
 }
 
-template <typename TIn, int NJ, int NCB, bool kB16>
+template <typename TIn, int NJ, int NCB, bool kB16, bool kParts = false>
 hipError_t launch_map_b(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
                         hipStream_t stream) {
     const int slices = (Wb + 16 * NCB - 1) / (16 * NCB);
@@ -1215,7 +1286,7 @@ hipError_t launch_map_b(const void* x, void* out, const MapOperand& op, const Pr
     const dim3 grid = flat ? dim3(unsigned(per * p.N * slices)) : dim3(unsigned(per * p.N), unsigned(slices));
     constexpr size_t kTurn = NJ <= 8 ? MapRows<TIn, NJ, kB16>::kBytes : 0, kOut = OutRows<TIn, NCB>::kBytes;
     const size_t lds = kMatrixFloats<NJ, NCB, kB16> * sizeof(float) + NW * (kTurn > kOut ? kTurn : kOut);
-    nc_map_kernel<TIn, NJ, NCB, kB16, NW><<<grid, 64 * NW, lds, stream>>>(static_cast<const TIn*>(x), static_cast<TIn*>(out),
+    nc_map_kernel<TIn, NJ, NCB, kB16, NW, kParts><<<grid, 64 * NW, lds, stream>>>(static_cast<const TIn*>(x), static_cast<TIn*>(out),
                                                                  op, p.N, p.T, Wa, Wb, wt, per, p.live,
                                                                  flat ? slices : 1);
     return hipGetLastError();
@@ -1223,21 +1294,21 @@ hipError_t launch_map_b(const void* x, void* out, const MapOperand& op, const Pr
 
 // bf16 rows of whole 8-value operands take the bf16 matrix instructions; rows
 // that end in half an operand are widened to fp32.
-template <typename TIn, int NJ, int NCB>
+template <typename TIn, int NJ, int NCB, bool kParts>
 hipError_t launch_map_e(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
                         hipStream_t stream) {
-    if constexpr (sizeof(TIn) == 2) {
+    if constexpr (sizeof(TIn) == 2 && !kParts) {
         if (Wa % 8 == 0) return launch_map_b<TIn, NJ, NCB, true>(x, out, op, p, Wa, Wb, stream);
     }
-    return launch_map_b<TIn, NJ, NCB, false>(x, out, op, p, Wa, Wb, stream);
+    return launch_map_b<TIn, NJ, NCB, false, kParts>(x, out, op, p, Wa, Wb, stream);
 }
 
-template <typename TIn, int NJ>
+template <typename TIn, int NJ, bool kParts>
 hipError_t launch_map_j(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
                         hipStream_t stream) {
-    if (Wb <= 16) return launch_map_e<TIn, NJ, 1>(x, out, op, p, Wa, Wb, stream);
-    if (Wb <= 32) return launch_map_e<TIn, NJ, 2>(x, out, op, p, Wa, Wb, stream);
-    return launch_map_e<TIn, NJ, 4>(x, out, op, p, Wa, Wb, stream);
+    if (Wb <= 16) return launch_map_e<TIn, NJ, 1, kParts>(x, out, op, p, Wa, Wb, stream);
+    if (Wb <= 32) return launch_map_e<TIn, NJ, 2, kParts>(x, out, op, p, Wa, Wb, stream);
+    return launch_map_e<TIn, NJ, 4, kParts>(x, out, op, p, Wa, Wb, stream);
 }
 
 template <int NJ, int NCW>
@@ -1250,21 +1321,21 @@ hipError_t launch_map_wide(const void* x, void* out, const MapOperand& op, const
     return hipGetLastError();
 }
 
-template <typename TIn>
+template <typename TIn, bool kParts>
 hipError_t launch_map_t(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
                         hipStream_t stream) {
-    if constexpr (sizeof(TIn) == 2) {
+    if constexpr (sizeof(TIn) == 2 && !kParts) {
         if (Wb > 64 && Wa > 64 && Wa % 8 == 0) {
             if (Wa > 128) return launch_map_wide<16, 1>(x, out, op, p, Wa, Wb, stream);
             return Wb > 128 ? launch_map_wide<8, 2>(x, out, op, p, Wa, Wb, stream)
                             : launch_map_wide<8, 1>(x, out, op, p, Wa, Wb, stream);
         }
     }
-    if (Wa <= 16) return launch_map_j<TIn, 1>(x, out, op, p, Wa, Wb, stream);
-    if (Wa <= 32) return launch_map_j<TIn, 2>(x, out, op, p, Wa, Wb, stream);
-    if (Wa <= 64) return launch_map_j<TIn, 4>(x, out, op, p, Wa, Wb, stream);
-    if (Wa <= 128) return launch_map_j<TIn, 8>(x, out, op, p, Wa, Wb, stream);
-    return launch_map_j<TIn, 16>(x, out, op, p, Wa, Wb, stream);
+    if (Wa <= 16) return launch_map_j<TIn, 1, kParts>(x, out, op, p, Wa, Wb, stream);
+    if (Wa <= 32) return launch_map_j<TIn, 2, kParts>(x, out, op, p, Wa, Wb, stream);
+    if (Wa <= 64) return launch_map_j<TIn, 4, kParts>(x, out, op, p, Wa, Wb, stream);
+    if (Wa <= 128) return launch_map_j<TIn, 8, kParts>(x, out, op, p, Wa, Wb, stream);
+    return launch_map_j<TIn, 16, kParts>(x, out, op, p, Wa, Wb, stream);
 }
 
 template <typename TIn>
@@ -1308,8 +1379,12 @@ int64_t nc_blocks_per_stream(int64_t streams, int64_t T, int dtype, int64_t max_
 
 hipError_t launch_nc_sums(const void* x, const void* y, float* records, const Problem& p, int Wa, int Wb,
                           hipStream_t stream) {
-    if (p.dtype == RACE_BF16) return launch_sums_t<bf16_t>(x, y, records, p, Wa, Wb, stream);
-    return launch_sums_t<float>(x, y, records, p, Wa, Wb, stream);
+    if (!v4_widths(Wa, Wb)) {
+        if (p.dtype == RACE_BF16) return launch_sums_t<bf16_t, true>(x, y, records, p, Wa, Wb, stream);
+        return launch_sums_t<float, true>(x, y, records, p, Wa, Wb, stream);
+    }
+    if (p.dtype == RACE_BF16) return launch_sums_t<bf16_t, false>(x, y, records, p, Wa, Wb, stream);
+    return launch_sums_t<float, false>(x, y, records, p, Wa, Wb, stream);
 }
 
 hipError_t launch_tile_sums_b16(const void* k, const void* v, float* records, const Problem& p, hipStream_t stream) {
@@ -1319,8 +1394,12 @@ hipError_t launch_tile_sums_b16(const void* k, const void* v, float* records, co
 
 hipError_t launch_nc_map(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
                          hipStream_t stream) {
-    if (p.dtype == RACE_BF16) return launch_map_t<bf16_t>(x, out, op, p, Wa, Wb, stream);
-    return launch_map_t<float>(x, out, op, p, Wa, Wb, stream);
+    if (!v4_widths(Wa, Wb)) {
+        if (p.dtype == RACE_BF16) return launch_map_t<bf16_t, true>(x, out, op, p, Wa, Wb, stream);
+        return launch_map_t<float, true>(x, out, op, p, Wa, Wb, stream);
+    }
+    if (p.dtype == RACE_BF16) return launch_map_t<bf16_t, false>(x, out, op, p, Wa, Wb, stream);
+    return launch_map_t<float, false>(x, out, op, p, Wa, Wb, stream);
 }
 
 hipError_t launch_nc_query64(const void* q, const void* g, void* dq, const float* state, float* records,

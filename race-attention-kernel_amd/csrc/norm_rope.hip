@@ -479,11 +479,11 @@ struct RopePlan {
 // A lane group takes two rows where that leaves kRopeEnough workgroups (of 1 x
 // 16384 tokens of 32 + 8 heads of 128 in bf16, forward: 69 us; one row 123, four
 // rows 77, whose registers leave fewer waves).  The workgroups stay for several
-// tiles: 3072 forward (69 us; one tile each 75), and backward two rounds of what
+// tiles: 2560 forward (69 us; one tile each 75), and backward two rounds of what
 // is resident (bf16 two rounds of three per CU: 8 x 8192 tokens of 16 + 16 heads
 // of 64 165 us, 1280 workgroups 179, 2048 178; fp32 one of four: 32 x 1024 tokens
 // of 12 + 12 heads of 64 119 us, 1536 workgroups 138).
-constexpr int kRopeEnough = 512, kRopeFwdWorkgroups = 3072, kRopeBwdWorkgroups = 1536, kRopeBwdWorkgroupsF32 = 1024;
+constexpr int kRopeEnough = 512, kRopeFwdWorkgroups = 2560, kRopeBwdWorkgroups = 1536, kRopeBwdWorkgroupsF32 = 1024;
 constexpr int kRopeTableBytes = 64 * 1024;
 
 RopePlan rope_plan(const NormRope& r, const void* const (&x)[2], const void* const (&w)[2], bool backward) {

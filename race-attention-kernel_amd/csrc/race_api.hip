@@ -1961,7 +1961,7 @@ hipError_t cross_map(const void* probsQ, const float* state, void* out, const Pr
     MapOperand op = map_operand(state, Sd + q.S, q.d, 1);
     op.div = state + Sd;
     op.div_stream = Sd + q.S;
-    return token_map(probsQ, out, op, q, q.S, q.d, stream);
+    return launch_nc_map(probsQ, out, op, q, q.S, q.d, stream);
 }
 
 }  // namespace
@@ -1996,7 +1996,7 @@ race_status race_cross_fwd(const void* probsQ, const void* probsK, const void* V
     if (!workspace || !aligned16(workspace) || workspace_bytes < size_t(l.total()) * sizeof(float))
         return RACE_ERROR_INVALID_VALUE;
     float* records = static_cast<float*>(workspace);
-    RACE_TRY(outer_sums(probsK, V, records, k, k.S, k.d, stream));
+    RACE_TRY(launch_nc_sums(probsK, V, records, k, k.S, k.d, stream));
     if (!want_out) return launch_tile_reduce(records, state, nullptr, k, stream);
     if (cross_few(q)) {
         float* sums = state ? state : records + l.records + l.E;
@@ -2006,7 +2006,7 @@ race_status race_cross_fwd(const void* probsQ, const void* probsK, const void* V
     if (k.tiles > cross_fold(k)) {
         float* E = records + l.records;
         RACE_TRY(launch_tile_reduce(records, state, E, k, stream));
-        return token_map(probsQ, out, map_operand(E, Sd, q.d, 1), q, q.S, q.d, stream);
+        return launch_nc_map(probsQ, out, map_operand(E, Sd, q.d, 1), q, q.S, q.d, stream);
     }
     // The map adds the records as it stages them and leaves the state.
     MapOperand op = map_operand(records, k.tiles * k.rec, q.d, 1);
@@ -2017,7 +2017,7 @@ race_status race_cross_fwd(const void* probsQ, const void* probsK, const void* V
     op.save = state;
     op.save_stream = Sd + q.S;
     op.save_div_off = Sd;
-    return token_map(probsQ, out, op, q, q.S, q.d, stream);
+    return launch_nc_map(probsQ, out, op, q, q.S, q.d, stream);
 }
 
 race_status race_cross_query(const void* probsQ, const float* state, void* out, const race_cross_shape* shape,
@@ -2070,9 +2070,9 @@ race_status race_cross_bwd(const void* probsQ, const void* probsK, const void* V
     if (w64 && dQ && (dK || dV)) {
         RACE_TRY(launch_nc_query64(probsQ, dOut, dQ, state, records, q, stream));
     } else {
-        if (dQ) RACE_TRY(token_map(dOut, dQ, et, q, q.d, q.S, stream));
+        if (dQ) RACE_TRY(launch_nc_map(dOut, dQ, et, q, q.d, q.S, stream));
         if (!dK && !dV) return RACE_SUCCESS;
-        RACE_TRY(outer_sums(probsQ, dOut, records, q, q.S, q.d, stream));
+        RACE_TRY(launch_nc_sums(probsQ, dOut, records, q, q.S, q.d, stream));
     }
     if (!dK && !dV) return RACE_SUCCESS;
     if (w64 && q.tiles <= kNcFoldParts)
@@ -2083,9 +2083,9 @@ race_status race_cross_bwd(const void* probsQ, const void* probsK, const void* V
         MapOperand op = map_operand(dB, Sd, 1, q.d);
         op.bias = dA;
         op.bias_stream = q.S;
-        RACE_TRY(token_map(V, dK, op, k, k.d, k.S, stream));
+        RACE_TRY(launch_nc_map(V, dK, op, k, k.d, k.S, stream));
     }
-    if (dV) RACE_TRY(token_map(probsK, dV, map_operand(dB, Sd, q.d, 1), k, k.S, k.d, stream));
+    if (dV) RACE_TRY(launch_nc_map(probsK, dV, map_operand(dB, Sd, q.d, 1), k, k.S, k.d, stream));
     return RACE_SUCCESS;
 }
 

@@ -208,8 +208,9 @@ hipError_t launch_key_grad64(const void* k, const void* v, void* dk, void* dv,
                              const float* dE_records, const float* state, const float* dB_ready,
                              const float* dA_ready, const Problem& p, hipStream_t stream);
 
-// ---- the same passes on the fp32 matrix cores (noncausal_mfma.hip), for the
-// same widths: fp32 products and sums, token operands straight from memory ----
+// ---- the same passes on the fp32 matrix cores (noncausal_mfma.hip): fp32
+// products and sums, token operands straight from memory.  Any widths in
+// launch_nc_sums and launch_nc_map, the others 64 ----
 
 // Tile records a map or a key side sums as it stages its matrix; longer
 // sequences reduce them first.

@@ -37,7 +37,7 @@ __device__ __forceinline__ float ld(const TIn* __restrict__ p, int64_t i) {
 template <typename TIn, int MI>
 __global__ __launch_bounds__(kThreads) void tile_outer_sums_kernel(
     const TIn* __restrict__ x, const TIn* __restrict__ y, float* __restrict__ records, int64_t T,
-    int tile, int64_t tiles, int64_t rec, int Wa, int Wb, const Live live) {
+    int tile, int64_t tiles, int64_t rec, int Wa, int Wb) {
     extern __shared__ float smem[];
     constexpr int kWaPad = MI * 16;
     float* xs = smem;                          // [kStageTokens][kWaPad]
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kThreads) void tile_outer_sums_kernel(
     const int c0 = blockIdx.z * kSliceCols;
     const int ncols = min(kSliceCols, Wb - c0);
     const int64_t t_begin = ti * tile;
-    const int64_t t_end = min(live.of(n, T), t_begin + tile);
+    const int64_t t_end = min(T, t_begin + tile);
     const TIn* xn = x + n * T * Wa;
     const TIn* yn = y + n * T * Wb;
 
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(kThreads) void causal_output_valu_kernel(
 template <typename TIn>
 __global__ __launch_bounds__(kThreads) void token_map_kernel(
     const TIn* __restrict__ x, TIn* __restrict__ out, const MapOperand op, int64_t T, int Wa,
-    int Wb, const Live live) {
+    int Wb) {
     extern __shared__ float smem[];
     float* Ms = smem;                    // [Wa][64]
     float* xs = Ms + Wa * kSliceCols;    // [kMapTokens][Wa]
@@ -438,12 +438,10 @@ __global__ __launch_bounds__(kThreads) void token_map_kernel(
         Ms[e] = v;
     }
     const TIn* xn = x + n * T * Wa;
-    const int alive = int(max(int64_t(0), min<int64_t>(live.of(n, T) - t0, cnt)));
-    for (int e = tid; e < alive * Wa; e += kThreads) xs[e] = ld(xn, t0 * Wa + e);
+    for (int e = tid; e < cnt * Wa; e += kThreads) xs[e] = ld(xn, t0 * Wa + e);
     __syncthreads();
     const int i = tid >> 3, tc = tid & 7;
     if (i >= cnt) return;
-    const bool dead = i >= alive;  // zero, whatever xs holds there
     float acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = 0.f;
@@ -459,7 +457,7 @@ __global__ __launch_bounds__(kThreads) void token_map_kernel(
         if (c < ncols) {
             float val = acc[j];
             if (op.bias) val += op.bias[n * op.bias_stream + c0 + c];
-            store_val(on + c0 + c, dead ? 0.f : val);
+            store_val(on + c0 + c, val);
         }
     }
 }
@@ -481,7 +479,7 @@ hipError_t launch_tile_outer_sums(const void* x, const void* y, float* records, 
 #define RACE_OUTER(TIN, MI)                                                                      \
     tile_outer_sums_kernel<TIN, MI><<<grid, kThreads, lds, stream>>>(                            \
         static_cast<const TIN*>(x), static_cast<const TIN*>(y), records, p.T, p.tile, p.tiles, \
-        p.rec, Wa, Wb, p.live)
+        p.rec, Wa, Wb)
 #define RACE_OUTER_MI(TIN)                     \
     switch (mi) {                              \
         case 1: RACE_OUTER(TIN, 1); break;     \
@@ -574,10 +572,10 @@ hipError_t launch_token_map(const void* x, void* out, const MapOperand& op, cons
     const size_t lds = token_map_lds_bytes(Wa);
     if (p.dtype == RACE_BF16) {
         token_map_kernel<bf16_t><<<grid, kThreads, lds, stream>>>(
-            static_cast<const bf16_t*>(x), static_cast<bf16_t*>(out), op, p.T, Wa, Wb, p.live);
+            static_cast<const bf16_t*>(x), static_cast<bf16_t*>(out), op, p.T, Wa, Wb);
     } else {
         token_map_kernel<float><<<grid, kThreads, lds, stream>>>(
-            static_cast<const float*>(x), static_cast<float*>(out), op, p.T, Wa, Wb, p.live);
+            static_cast<const float*>(x), static_cast<float*>(out), op, p.T, Wa, Wb);
     }
     return hipGetLastError();
 }

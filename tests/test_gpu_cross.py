@@ -88,7 +88,10 @@ CASES = [(3, 3, 1, 1, 4, 16, 64), (4, 2, 5, 70, 4, 16, 64), (2, 2, 16, 33, 4, 16
          (12, 3, 65, 129, 4, 16, 64), (8, 2, 40, 257, 8, 32, 128), (6, 6, 3, 50, 8, 32, 128), (3, 1, 30, 40, 1, 7, 17),
          (3, 1, 2, 40, 1, 7, 17), (4, 4, 100, 3, 3, 10, 50), (2, 2, 77, 190, 2, 8, 32), (2, 2, 64, 64, 3, 16, 96),
          (1, 1, 50, 40000, 4, 16, 64), (1, 1, 40000, 50, 4, 16, 64), (300, 300, 1, 20, 4, 16, 64),
-         (300, 300, 8, 20, 5, 6, 36), (2, 1, 7, 9, 1, 1, 1), (2, 2, 20, 30, 1, 1, 128), (5, 5, 12, 9, 7, 36, 128)]
+         (300, 300, 8, 20, 5, 6, 36), (2, 1, 7, 9, 1, 1, 1), (2, 2, 20, 30, 1, 1, 128), (5, 5, 12, 9, 7, 36, 128),
+         # Widths that are no multiples of four, over one block and several.
+         (4, 2, 90, 300, 8, 16, 17), (4, 4, 70, 200, 5, 7, 100), (2, 1, 200, 333, 3, 13, 121), (3, 3, 50, 70, 85, 3, 127),
+         (2, 2, 300, 2100, 8, 8, 66), (2, 2, 40, 40, 7, 31, 3), (6, 2, 33, 50, 1, 2, 1), (2, 2, 33, 50, 2, 3, 64)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -121,7 +124,8 @@ def test_forward_and_gradients(race, cuda, Nq, Nk, Tq, Tk, L, R, d, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("Tq, Tk, L, R, d, lengths", [(40, 130, 4, 16, 64, [0, 1, 130, 129]), (3, 700, 4, 16, 64, [700, 0]),
                                                       (50, 90, 8, 32, 128, [64, 0]), (20, 50, 3, 10, 50, [13, 50, 0, 1]),
-                                                      (30, 3000, 2, 8, 32, [1024, 1]), (19, 40, 4, 16, 64, [-3, 999])])
+                                                      (30, 3000, 2, 8, 32, [1024, 1]), (70, 301, 5, 7, 33, [301, 77, 0, 1]),
+                                                      (33, 200, 16, 8, 121, [150, 7]), (19, 40, 4, 16, 64, [-3, 999])])
 def test_padded_keys(race, cuda, Tq, Tk, L, R, d, lengths, dtype):
     Nk = 4
     q, k, v, dout = make(2 * Nk, Nk, Tq, Tk, L, R, d, dtype, Tk, cuda)
