@@ -566,7 +566,7 @@ race_status race_cross_bwd(const void* probsQ, const void* probsK, const void* V
  * permutes are src/race_baseline.py:35-40's; the norm and the rotation have no
  * counterpart in the reference. */
 typedef struct race_norm_rope_shape {
-    int64_t batch, seq_len;     /* batch * seq_len < 2^31 */
+    int64_t batch, seq_len;     /* batch * seq_len <= 2^30 */
     int32_t q_heads, k_heads;   /* k_heads 0: no keys; each at most 65535 */
     int32_t head_dim;           /* 1 .. 256 */
     int32_t pairs;              /* 0 .. head_dim / 2; 0: no rotation */

@@ -65,12 +65,15 @@ class BatchedACE(nn.Module):
             return None
         if self._inv_freq is None or self._inv_freq.device != device:
             p = torch.arange(self.rope_pairs, dtype=torch.float64, device=device)
-            self._inv_freq = (self.rope_theta ** (-p / self.rope_pairs)).float()
+            freq = (self.rope_theta ** (-p / self.rope_pairs)).float()
+            if freq.is_cuda and torch.cuda.is_current_stream_capturing():
+                return freq  # the graph's own: it holds values during its replays only
+            self._inv_freq = freq
         return self._inv_freq
 
     def _streams(self, Khf, Vhf, Qhf, positions):
         """K, Q (normed, rotated) and V rows as streams [M * B * H, T, d_k]."""
-        k, v, q = (x.reshape(-1, *x.shape[2:]) for x in (Khf, Vhf, Qhf))
+        k, v, q = (x.flatten(0, 1) for x in (Khf, Vhf, Qhf))
         freq = self.inv_freq(q.device)
         if freq is not None and positions is None:
             positions = torch.arange(q.shape[1], device=q.device)

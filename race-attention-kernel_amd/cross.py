@@ -60,7 +60,7 @@ class CrossACE(BatchedACE):
 
     def _side(self, x, weight, positions):
         """Rows [M, B, T, H, d_k] as bucket probabilities of streams."""
-        rows = x.reshape(-1, *x.shape[2:])
+        rows = x.flatten(0, 1)
         freq = self.inv_freq(rows.device)
         if freq is not None and positions is None:
             positions = torch.arange(rows.shape[1], device=rows.device)
@@ -69,7 +69,7 @@ class CrossACE(BatchedACE):
         return self.bucket_probs(streams)
 
     def _values(self, Vhf):
-        return race_norm_rope(Vhf.reshape(-1, *Vhf.shape[2:]), None, eps=None)[0]
+        return race_norm_rope(Vhf.flatten(0, 1), None, eps=None)[0]
 
     def _heads(self, out, Qhf):
         M, B, T, H, dk = Qhf.shape

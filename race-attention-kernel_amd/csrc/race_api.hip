@@ -356,15 +356,16 @@ hipError_t zero_fill(float* p, int64_t n, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// bytes of zeros at p, a multiple of 2.
+// bytes of zeros at p, a multiple of 2.  The grid stays under 2^32 threads, past
+// which a launch wraps around without an error.
 __global__ void fill_zero16_kernel(uint16_t* __restrict__ p, int64_t n) {
-    const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i < n) p[i] = 0;
+    for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < n; i += int64_t(gridDim.x) * kThreads) p[i] = 0;
 }
 hipError_t zero_bytes(void* p, size_t bytes, hipStream_t stream) {
     const int64_t n = int64_t(bytes / 2);
     if (n <= 0) return hipSuccess;
-    fill_zero16_kernel<<<unsigned((n + kThreads - 1) / kThreads), kThreads, 0, stream>>>(static_cast<uint16_t*>(p), n);
+    const int64_t blocks = std::min<int64_t>((n + kThreads - 1) / kThreads, 1 << 20);
+    fill_zero16_kernel<<<unsigned(blocks), kThreads, 0, stream>>>(static_cast<uint16_t*>(p), n);
     return hipGetLastError();
 }
 
@@ -1782,7 +1783,7 @@ namespace {
 
 bool norm_rope_shape(const race_norm_rope_shape* sh, NormRope* r) {
     if (!sh || sh->batch < 0 || sh->seq_len < 0) return false;
-    if (sh->seq_len > 0 && sh->batch > int64_t(INT_MAX) / sh->seq_len) return false;
+    if (sh->seq_len > 0 && sh->batch > (int64_t(1) << 30) / sh->seq_len) return false;
     if (sh->q_heads < 1 || sh->q_heads > 65535 || sh->k_heads < 0 || sh->k_heads > 65535) return false;
     if (sh->head_dim < 1 || sh->head_dim > kRopeMaxDim || sh->pairs < 0 || sh->pairs > sh->head_dim / 2) return false;
     if (sh->dtype != RACE_F32 && sh->dtype != RACE_BF16) return false;

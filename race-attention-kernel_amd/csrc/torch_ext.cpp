@@ -30,6 +30,8 @@
 //   alg1_sub_chunk_tokens / alg1_select_tile_tokens / alg1_output_lds_bytes /
 //   alg1_fits_on_device: the queries of the reference's causal v2 binding
 //       (src/causal_v2/kernels/torch_binding.cpp:1-25)
+//   norm_rope / gated_scan / gated_scan_carry / cross / cross_state / cross_query:
+//       the operators beside the per-bucket op (torch_operators.h)
 //
 // probsQ, probsK: [N, T, L, R] (or [N, T, S], read as L = 1, R = S) and V:
 // [N, T, d], all float32 or all bfloat16, on one HIP device, contiguous,

@@ -50,7 +50,8 @@ void check_capture(const char* entry, const std::vector<c10::optional<at::Tensor
         if (!t || !t->defined() || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
         if (!asked) {
             hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-            TORCH_CHECK(hipStreamIsCapturing(current_stream(), &status) == hipSuccess, entry, ": hipStreamIsCapturing failed");
+            const hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t->device().index()).stream();
+            TORCH_CHECK(hipStreamIsCapturing(stream, &status) == hipSuccess, entry, ": hipStreamIsCapturing failed");
             capturing = status == hipStreamCaptureStatusActive;
             asked = true;
         }
@@ -117,12 +118,12 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> gated_scan_forward
     c10::optional<at::Tensor> records;
     if (want_records) records = at::empty({floats}, fopt);
     const at::Tensor ws = bytes > 0 ? workspace_of(bytes, x) : at::Tensor();
+    if (inplace) state->unsafeGetTensorImpl()->bump_version();  // a graph that saved it must notice
     check_status(race_gated_scan_fwd(x.data_ptr(), gate.data_ptr(), floats_of(state),
                                      lengths ? lengths->data_ptr<int32_t>() : nullptr, out.data_ptr(),
                                      fin.data_ptr<float>(), floats_of(records), &sh, bytes > 0 ? ws.data_ptr() : nullptr,
                                      bytes, current_stream()),
                  "race_gated_scan_fwd");
-    if (inplace) state->unsafeGetTensorImpl()->bump_version();  // a graph that saved it must notice
     return {out, fin, records};
 }
 
@@ -173,7 +174,7 @@ RopeCall rope_call(const char* entry, const at::Tensor& q, const c10::optional<a
     r.B = q.size(0), r.T = q.size(1), r.d = q.size(3);
     c.require(q.size(2) >= 1 && q.size(2) <= 65535 && r.d >= 1 && r.d <= 256, "q",
               [&] { return "has shape " + dims(q) + "; rows of 1 .. 256 values in 1 .. 65535 heads are taken"; })
-        .require(r.T == 0 || r.B <= INT32_MAX / r.T, "q", "has 2^31 tokens or more");
+        .require(r.T == 0 || r.B <= (int64_t(1) << 30) / r.T, "q", "has more than 2^30 tokens");
     if (k) {
         check_rows(c, "k", *k, 4, "[B, T, H, d]");
         c.matches("k", *k, "q", q)
@@ -367,7 +368,7 @@ CrossCall cross_call(const char* entry, const at::Tensor* q, const at::Tensor* k
               "probsQ", "has no kernel: up to 65535 key streams, S <= 256 buckets, d <= 128 columns and 2^30 tokens a "
                         "key stream are taken")
         .raise();
-    r.sh.kv_streams = Nk, r.sh.q_len = r.Tq * heads;
+    r.sh.kv_streams = Nk, r.sh.q_len = r.Nq > 0 ? r.Tq * heads : 0;
     r.sh.num_tables = 1, r.sh.num_buckets = static_cast<int32_t>(r.S), r.sh.head_dim = static_cast<int32_t>(r.d);
     r.sh.dtype = dtype_of(ref), r.sh.lengths_group = static_cast<int32_t>(group);
     return r;
@@ -448,7 +449,8 @@ at::Tensor as_rows(const at::Tensor& t, int64_t far = int64_t(1) << 40) {
 }
 
 c10::optional<at::Tensor> as_lengths(const c10::optional<at::Tensor>& lengths) {
-    if (lengths && lengths->scalar_type() == at::kLong) return lengths->to(at::kInt);
+    if (lengths && lengths->scalar_type() == at::kLong)
+        return lengths->clamp(0, INT32_MAX).to(at::kInt).contiguous();
     return lengths;
 }
 
@@ -667,27 +669,7 @@ void bind_operators(pybind11::module& m) {
           py::arg("lengths"));
     m.def("cross_state", &cross_state, "The sums race_cross_query reads", py::arg("probsK"), py::arg("V"),
           py::arg("lengths"));
-    m.def("cross_forward", &cross_forward, "The non-causal op over another sequence's keys -> (out, state)",
-          py::arg("probsQ"), py::arg("probsK"), py::arg("V"), py::arg("lengths"), py::arg("want_state"));
     m.def("cross_query", &cross_query, "Queries against a kept state -> out", py::arg("probsQ"), py::arg("state"));
-    m.def("cross_backward", &cross_backward, "Gradients of cross_forward -> (dQ, dK, dV)", py::arg("probsQ"),
-          py::arg("probsK"), py::arg("V"), py::arg("lengths"), py::arg("dout"), py::arg("state"), py::arg("need_q"),
-          py::arg("need_k"), py::arg("need_v"));
-    m.def("norm_rope_forward", &norm_rope_forward, "Heads normed and rotated, to streams -> (q, k or None)",
-          py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("inv_freq"), py::arg("q_weight"),
-          py::arg("k_weight"), py::arg("eps"), py::arg("norm"), py::arg("sections"), py::arg("interleaved"));
-    m.def("norm_rope_backward", &norm_rope_backward,
-          "Gradients of norm_rope_forward -> (dq, dk, dq_weight, dk_weight)", py::arg("q"), py::arg("k"),
-          py::arg("positions"), py::arg("inv_freq"), py::arg("q_weight"), py::arg("k_weight"), py::arg("dq_out"),
-          py::arg("dk_out"), py::arg("eps"), py::arg("norm"), py::arg("sections"), py::arg("interleaved"),
-          py::arg("need_q"), py::arg("need_k"), py::arg("need_qw"), py::arg("need_kw"));
-    m.def("gated_scan_forward", &gated_scan_forward,
-          "h_t = a_t h_{t-1} + u_t -> (out, final state, records or None)", py::arg("x"), py::arg("gate"),
-          py::arg("state"), py::arg("lengths"), py::arg("form"), py::arg("complement"), py::arg("want_records"),
-          py::arg("inplace"));
-    m.def("gated_scan_backward", &gated_scan_backward, "Gradients of gated_scan_forward -> (dx, dgate, dstate)",
-          py::arg("x"), py::arg("gate"), py::arg("lengths"), py::arg("dout"), py::arg("dfinal"), py::arg("records"),
-          py::arg("form"), py::arg("complement"), py::arg("need_x"), py::arg("need_gate"), py::arg("need_state"));
 }
 
 }  // namespace

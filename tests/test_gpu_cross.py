@@ -210,6 +210,11 @@ def test_empty_sides_and_refusals(race, cuda):
     out = race.race_cross_fwd(*leaves)
     grads = torch.autograd.grad(out, leaves, torch.zeros_like(out))
     assert out.shape == (4, 0, 32) and all((g == 0).all() for g in grads)
+    # No query streams at all.
+    leaves = [t.detach().requires_grad_(True) for t in (q[:0], k, v)]
+    out = race.race_cross_fwd(*leaves)
+    assert out.shape == (0, 5, 32) and all((g == 0).all() for g in torch.autograd.grad(out, leaves, torch.zeros_like(out)))
+    assert race.race_cross_query(leaves[0].detach(), race.race_cross_state(k, v).detach()).shape == (0, 5, 32)
     e = torch.empty(0, 3, 16, device=cuda)
     assert race.race_cross_fwd(e, e, torch.empty(0, 3, 32, device=cuda)).shape == (0, 3, 32)
     q, k, v = (t.detach() for t in (q, k, v))
@@ -313,6 +318,25 @@ def test_offsets_past_32_bits(race, cuda):
     ref = reference(last[0], last[1], last[2], None, last[3])
     check(out[-1:], ref["out"], "last stream out")
     check(dk[-1:], ref["dk"], "last stream dk")
+
+
+def test_zeros_past_32_bits(race, cuda):
+    # No keys: 33 x 2^20 rows of 128 zeros, more than 2^32 values.
+    N, Tq, d = 33, 1 << 20, 128
+    used = torch.ones(N, Tq, d, dtype=torch.bfloat16, device=cuda)
+    del used
+    q = torch.ones(N, Tq, 2, dtype=torch.bfloat16, device=cuda)
+    out = race.race_cross_fwd(q, q[:, :0].contiguous(), torch.empty(N, 0, d, dtype=torch.bfloat16, device=cuda))
+    assert out.shape == (N, Tq, d) and not any(bool(rows.any()) for rows in out)
+
+
+def test_lengths_of_64_bits(race, cuda):
+    q, k, v, _ = make(3, 3, 20, 50, 2, 8, 32, torch.float32, 8, cuda)
+    far = torch.tensor([2 ** 40, 2 ** 31 + 5, -2 ** 40], device=cuda)
+    near = torch.tensor([50, 50, 0], dtype=torch.int32, device=cuda)
+    assert torch.equal(race.race_cross_fwd(q, k, v, far), race.race_cross_fwd(q, k, v, near))
+    pairs = torch.stack([near, near], 1).long()
+    assert torch.equal(race.race_cross_fwd(q, k, v, pairs[:, 0]), race.race_cross_fwd(q, k, v, near))
 
 
 @pytest.mark.parametrize("options", [dict(), dict(qk_norm=True, rope_pairs=32)])

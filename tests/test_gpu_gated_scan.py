@@ -167,6 +167,14 @@ def test_lengths_past_the_ends_count_as_the_ends(race, cuda):
     assert (out[0] == 0).all() and torch.equal(final[0], state[0])
 
 
+def test_lengths_of_64_bits(race, cuda):
+    x = torch.randn(2, 40, 24, device=cuda)
+    near = torch.tensor([40, 0], dtype=torch.int32, device=cuda)
+    far = torch.tensor([2 ** 32 + 7, -2 ** 33], device=cuda)
+    for a, b in zip(race.race_gated_scan(x, x, lengths=far), race.race_gated_scan(x, x, lengths=near)):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strided_inputs_equal_dense_ones(race, cuda, dtype):
     N, T, D = 3, 530, 96

@@ -469,3 +469,32 @@ def test_module_with_norm_and_rotation(race, cuda, causal, options):
     for g, w in zip(grads, torch.autograd.grad(want, rows + weights, up)):
         assert torch.equal(g, w)
     assert sorted(module.state_dict()) == sorted(["planes_T", "protos_T"] + ["q_norm", "k_norm"] * bool(weights))
+
+
+def test_a_module_whose_first_call_is_captured(race, cuda):
+    # The frequencies made inside a capture hold values during its replays only.
+    torch.manual_seed(0)
+    options = dict(device=cuda, causal=False, qk_norm=True, rope_pairs=32)
+    first, other = race.BatchedACE(64, 4, 4, 1, **options), race.BatchedACE(64, 4, 4, 1, **options)
+    rows = [torch.randn(1, 2, 30, 3, 64, device=cuda) for _ in range(3)]
+    with torch.no_grad():
+        other(*rows)  # loads what a capture must not
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = first(*rows)
+        eager = first(*rows)
+        other.load_state_dict(first.state_dict())
+        assert torch.equal(eager, other(*rows))
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
+            assert torch.equal(first(*rows), eager)
+
+
+def test_modules_without_tokens(race, cuda):
+    empty = torch.zeros(1, 2, 0, 3, 64, device=cuda)
+    assert race.BatchedACE(64, 4, 4, 1, device=cuda, rope_pairs=16)(empty, empty, empty).shape == empty.shape
+    module = race.CrossACE(64, 4, 4, 1, device=cuda, rope_pairs=16)
+    out = module(empty, empty, torch.randn(1, 2, 5, 3, 64, device=cuda))
+    assert out.shape == (1, 2, 5, 3, 64) and (out == 0).all()

@@ -63,6 +63,8 @@ def test_norm_rope_refuses_on_the_host(race):
     ok = abi.norm_rope_shape(2, 300, 12, 4, 64, 32)
     st, nbytes = abi.norm_rope_bwd_workspace_bytes(ok)
     assert st == abi.RACE_SUCCESS and nbytes == 1536 * 64 * 4
+    assert abi.norm_rope_bwd_workspace_bytes(abi.norm_rope_shape(1 << 15, 1 << 15, 1, 0, 64, 32))[0] == abi.RACE_SUCCESS
+    assert abi.norm_rope_bwd_workspace_bytes(abi.norm_rope_shape(1 << 15, (1 << 15) + 1, 1, 0, 64, 32))[0] == bad
     for kw in (dict(B=-1), dict(T=-1), dict(B=1 << 16, T=1 << 15), dict(Hq=0), dict(Hk=-1), dict(d=0, pairs=0),
                dict(d=257), dict(pairs=33), dict(pairs=-1), dict(sections=[16, 15]), dict(sections=[33, -1]),
                dict(pos_bits=16), dict(eps=-1.0), dict(eps=float("nan")), dict(dtype=2), dict(weight_dtype=3)):
