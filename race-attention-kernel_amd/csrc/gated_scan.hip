@@ -25,6 +25,10 @@
 // exactly instead of from the rounded output.
 // Few channels and many tokens are split over the tokens: one launch gives
 // every segment's pair, the next starts each segment from the pairs before it.
+// (A workgroup per tile that waits for the states of the tiles before it, which
+// reads the rows once, took longer: 8 x 65536 x 64 bf16 107 us forward and 187
+// backward against 82 and 120, 1 x 2^20 x 16 616 against 126: a state took 10 us
+// to reach the workgroups of the next 64 tiles.)
 // Sums have a fixed order: results are bitwise reproducible.
 #include <algorithm>
 
