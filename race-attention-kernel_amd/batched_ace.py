@@ -64,8 +64,9 @@ class BatchedACE(nn.Module):
         if self.rope_pairs == 0:
             return None
         if self._inv_freq is None or self._inv_freq.device != device:
-            p = torch.arange(self.rope_pairs, dtype=torch.float64, device=device)
-            freq = (self.rope_theta ** (-p / self.rope_pairs)).float()
+            with torch.inference_mode(False):  # kept for training calls too, whose node saves them
+                p = torch.arange(self.rope_pairs, dtype=torch.float64, device=device)
+                freq = (self.rope_theta ** (-p / self.rope_pairs)).float()
             if freq.is_cuda and torch.cuda.is_current_stream_capturing():
                 return freq  # the graph's own: it holds values during its replays only
             self._inv_freq = freq

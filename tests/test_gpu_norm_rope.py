@@ -498,3 +498,22 @@ def test_modules_without_tokens(race, cuda):
     module = race.CrossACE(64, 4, 4, 1, device=cuda, rope_pairs=16)
     out = module(empty, empty, torch.randn(1, 2, 5, 3, 64, device=cuda))
     assert out.shape == (1, 2, 5, 3, 64) and (out == 0).all()
+
+
+@pytest.mark.parametrize("cross", [False, True])
+def test_modules_first_called_under_inference_mode_train(race, cuda, cross):
+    # A validation pass before the first training step.
+    torch.manual_seed(0)
+    options = dict(device=cuda, qk_norm=True, rope_pairs=32)
+    make_module = lambda: race.CrossACE(64, 4, 4, 1, **options) if cross else race.BatchedACE(64, 4, 4, 1, **options)
+    module, fresh = make_module(), make_module()
+    fresh.load_state_dict(module.state_dict())
+    rows = [torch.randn(1, 2, 30, 3, 64, device=cuda, requires_grad=True) for _ in range(3)]
+    with torch.inference_mode():
+        before = module(*rows)
+    leaves = rows + list(module.parameters())
+    out = module(*rows)
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    other = fresh(*rows)
+    want = torch.autograd.grad(other, rows + list(fresh.parameters()), torch.ones_like(other))
+    assert torch.equal(before, out) and all(torch.equal(a, b) for a, b in zip((out, *grads), (other, *want)))

@@ -110,3 +110,14 @@ def test_cross_refuses_on_the_host(race):
         race.race_cross_fwd(x, x, x)
     with pytest.raises(RuntimeError, match="race_cross_state: probsK lives on the CPU"):
         race.race_cross_state(x, x)
+
+
+def test_frequencies_first_made_under_inference_mode_serve_training(race):
+    # An inference tensor could not be saved for a later backward.
+    module = race.BatchedACE(64, 4, 4, 1, rope_pairs=16)
+    with torch.inference_mode():
+        first = module.inv_freq(torch.device("cpu"))
+    assert not first.is_inference() and not module.inv_freq(torch.device("cpu")).is_inference()
+    leaf = torch.ones(16, requires_grad=True)
+    (leaf * module.inv_freq(torch.device("cpu"))).sum().backward()  # saves them
+    assert torch.equal(leaf.grad, race.BatchedACE(64, 4, 4, 1, rope_pairs=16).inv_freq(torch.device("cpu")))
