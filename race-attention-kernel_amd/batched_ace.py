@@ -57,20 +57,24 @@ class BatchedACE(nn.Module):
         self.k_norm = nn.Parameter(torch.ones(d_k, device=device)) if qk_norm else None
         self.rope_pairs, self.rope_theta = rope_pairs, rope_theta
         self.rope_sections, self.rope_interleaved = rope_sections, rope_interleaved
-        self._inv_freq = None  # float32 whatever the module is cast to, so no buffer
+        self._inv_freq = {}  # by device; float32 whatever the module is cast to, so no buffer
 
     def inv_freq(self, device) -> torch.Tensor | None:
         """The rotation's frequencies [rope_pairs], float32."""
         if self.rope_pairs == 0:
             return None
-        if self._inv_freq is None or self._inv_freq.device != device:
-            with torch.inference_mode(False):  # kept for training calls too, whose node saves them
-                p = torch.arange(self.rope_pairs, dtype=torch.float64, device=device)
-                freq = (self.rope_theta ** (-p / self.rope_pairs)).float()
-            if freq.is_cuda and torch.cuda.is_current_stream_capturing():
+        kept = self._inv_freq.get(device)
+        if kept is not None:
+            return kept
+        with torch.inference_mode(False):  # kept for training calls too, whose node saves them
+            p = torch.arange(self.rope_pairs, dtype=torch.float64, device=device)
+            freq = (self.rope_theta ** (-p / self.rope_pairs)).float()
+        if freq.is_cuda:
+            if torch.cuda.is_current_stream_capturing():
                 return freq  # the graph's own: it holds values during its replays only
-            self._inv_freq = freq
-        return self._inv_freq
+            torch.cuda.current_stream(freq.device).synchronize()  # once a device: later calls read it on any stream
+        self._inv_freq[device] = freq
+        return freq
 
     def _streams(self, Khf, Vhf, Qhf, positions):
         """K, Q (normed, rotated) and V rows as streams [M * B * H, T, d_k]."""

@@ -517,3 +517,21 @@ def test_modules_first_called_under_inference_mode_train(race, cuda, cross):
     other = fresh(*rows)
     want = torch.autograd.grad(other, rows + list(fresh.parameters()), torch.ones_like(other))
     assert torch.equal(before, out) and all(torch.equal(a, b) for a, b in zip((out, *grads), (other, *want)))
+
+
+def test_kept_frequencies_are_complete_for_every_stream(race, cuda):
+    # A later call on another stream waits for nothing, so what is kept must be there already.
+    module, busy = race.BatchedACE(64, 4, 4, 1, device=cuda, rope_pairs=32), torch.randn(8192, 8192, device=cuda)
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        for _ in range(20):
+            busy @ busy
+        freq = module.inv_freq(cuda)
+        assert first.query()
+    with torch.cuda.stream(second):
+        rows = [torch.randn(1, 2, 30, 3, 64, device=cuda) for _ in range(3)]
+        out = module(*rows)
+        assert module.inv_freq(cuda) is freq
+    torch.cuda.synchronize()
+    assert torch.equal(out, module(*rows))
