@@ -454,7 +454,11 @@ c10::optional<at::Tensor> as_lengths(const c10::optional<at::Tensor>& lengths) {
     return lengths;
 }
 
+// Whether a call takes its autograd node: for gradients, and for inputs with a
+// forward-mode tangent, which a node without that mode refuses.
 bool wants_grad(std::initializer_list<c10::optional<at::Tensor>> inputs) {
+    for (const auto& t : inputs)
+        if (t && t->_fw_grad(0).defined()) return true;
     if (!at::GradMode::is_enabled()) return false;
     for (const auto& t : inputs)
         if (t && t->requires_grad()) return true;

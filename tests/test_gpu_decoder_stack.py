@@ -115,3 +115,22 @@ def test_gradients_reach_every_parameter(race, cuda):
                 t.add_(w, alpha=-sign * step)
     size = sum(float((g.double().abs() * w.abs()).sum()) for g, w in zip(grads, way))
     assert abs((loss[0] - loss[1]) / (2 * step) - along) <= 5e-3 * size + FP32_TOL * np.sqrt(B * T * D) / step
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("which", ["norm_rope q", "norm_rope weight", "scan gate", "scan state", "cross V"])
+def test_forward_mode_derivatives_are_refused(race, cuda, which, grad):
+    # None of the operators has one: an output without a tangent would count as a zero derivative.
+    n = lambda *s: torch.randn(*s, device=cuda)
+    q, k, w, x, gate, state, probs, v = (n(2, 5, 3, 64), n(2, 5, 1, 64), n(64), n(2, 5, 64), n(2, 5, 64), n(2, 64),
+                                         torch.rand(2, 5, 16, device=cuda), n(2, 5, 64))
+    plain = {"norm_rope q": (q, lambda t: race.race_norm_rope(t, k)),
+             "norm_rope weight": (w, lambda t: race.race_norm_rope(q, k, q_weight=w, k_weight=t)),
+             "scan gate": (gate, lambda t: race.race_gated_scan(x, t)),
+             "scan state": (state, lambda t: race.race_gated_scan(x, gate, t)),
+             "cross V": (v, lambda t: race.race_cross_fwd(probs, probs, t))}
+    at, run = plain[which]
+    with torch.set_grad_enabled(grad), torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="jvp"):
+            run(torch.autograd.forward_ad.make_dual(at, torch.ones_like(at)))
+        run(at)
