@@ -43,7 +43,8 @@ int64_t check_lengths(ArgCheck& c, const c10::optional<at::Tensor>& lengths, con
 // Refuses a differentiable call on a stream under capture whose leaf inputs are
 // still held by a graph from the default stream: the backward would wait for
 // that stream inside the capture, which ends the process.  Deleting the eager
-// outputs (or detaching them) frees the leaves.
+// outputs (or detaching them) frees the leaves.  `inputs` are the caller's own:
+// a copy as_rows makes of a leaf is none.
 void check_capture(const char* entry, const std::vector<c10::optional<at::Tensor>>& inputs) {
     bool capturing = false, asked = false;
     for (const auto& t : inputs) {
@@ -527,7 +528,6 @@ struct NormRopeNode : torch::autograd::Function<NormRopeNode> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const c10::optional<at::Tensor>& k,
                                  const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
                                  const c10::intrusive_ptr<RopeHeld>& h) {
-        check_capture("race_norm_rope", {q, k, q_weight, k_weight});
         const auto [q_out, k_out] = norm_rope_forward(q, k, h->positions, h->inv_freq, q_weight, k_weight, h->eps, h->norm,
                                                       h->sections, h->interleaved);
         ctx->set_materialize_grads(false);
@@ -561,7 +561,6 @@ struct NormRopeNode : torch::autograd::Function<NormRopeNode> {
 struct GatedScanNode : torch::autograd::Function<GatedScanNode> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate,
                                  const c10::optional<at::Tensor>& state, const c10::intrusive_ptr<ScanHeld>& h) {
-        check_capture("race_gated_scan", {x, gate, state});
         const auto [out, fin, records] = gated_scan_forward(x, gate, state, h->lengths, h->form, h->complement, true, false);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, gate, or_undefined(h->lengths), *records});
@@ -590,7 +589,6 @@ struct GatedScanNode : torch::autograd::Function<GatedScanNode> {
 struct CrossNode : torch::autograd::Function<CrossNode> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                  const c10::intrusive_ptr<CrossHeld>& h) {
-        check_capture("race_cross_fwd", {q, k, v});
         const auto [out, state] = cross_forward(q, k, v, h->lengths, true);
         ctx->save_for_backward({q, k, v, or_undefined(h->lengths), *state});
         return {*out};
@@ -611,10 +609,12 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> norm_rope(
     const c10::optional<at::Tensor>& inv_freq, const c10::optional<at::Tensor>& q_weight,
     const c10::optional<at::Tensor>& k_weight, c10::optional<double> eps, const std::vector<int64_t>& sections,
     bool interleaved) {
+    const bool node = wants_grad({q_in, k_in, q_weight, k_weight});
+    if (node) check_capture("race_norm_rope", {q_in, k_in, q_weight, k_weight});
     const at::Tensor q = as_rows(q_in);
     c10::optional<at::Tensor> k;
     if (k_in) k = as_rows(*k_in);
-    if (!wants_grad({q, k, q_weight, k_weight}))
+    if (!node)
         return norm_rope_forward(q, k, positions, inv_freq, q_weight, k_weight, eps.value_or(0.0), eps.has_value(),
                                  sections, interleaved);
     auto h = c10::make_intrusive<RopeHeld>();
@@ -628,9 +628,11 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> norm_rope(
 std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x_in, const at::Tensor& gate_in,
                                               const c10::optional<at::Tensor>& state,
                                               const c10::optional<at::Tensor>& lengths_in, int64_t form, bool complement) {
+    const bool node = wants_grad({x_in, gate_in, state});
+    if (node) check_capture("race_gated_scan", {x_in, gate_in, state});
     const at::Tensor x = as_rows(x_in, RACE_SCAN_MAX_TOKEN_STRIDE), gate = as_rows(gate_in, RACE_SCAN_MAX_TOKEN_STRIDE);
     const auto lengths = as_lengths(lengths_in);
-    if (!wants_grad({x, gate, state})) {
+    if (!node) {
         const auto r = gated_scan_forward(x, gate, state, lengths, form, complement, false, false);
         return {std::get<0>(r), std::get<1>(r)};
     }
@@ -650,6 +652,7 @@ std::tuple<at::Tensor, at::Tensor> gated_scan_carry(const at::Tensor& x, const a
 
 at::Tensor cross(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& lengths) {
     if (!wants_grad({q, k, v})) return *std::get<0>(cross_forward(q, k, v, as_lengths(lengths), false));
+    check_capture("race_cross_fwd", {q, k, v});
     auto h = c10::make_intrusive<CrossHeld>();
     h->lengths = as_lengths(lengths);
     return CrossNode::apply(q, k, v, h)[0];

@@ -439,3 +439,23 @@ def test_offsets_past_32_bits(race, cuda):
     o, f = race.race_gated_scan(x[:, -tail:], gate[:, -tail:])
     assert torch.allclose(out[:, -50:], o[:, -50:], rtol=1e-5, atol=1e-5)
     assert torch.allclose(final, f, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("layout", ["shifted", "apart", "far"])
+def test_a_live_eager_graph_refuses_the_capture_of_copied_rows(race, cuda, layout):
+    # Rows that the op copies first are the caller's leaves all the same.
+    if layout == "shifted":  # not 16-byte aligned
+        x = torch.randn(1 * 40 * 64 + 1, device=cuda)[1:].view(1, 40, 64)
+    elif layout == "apart":  # the last dimension strided
+        x = torch.randn(1, 40, 64, 2, device=cuda)[..., 0]
+    else:  # tokens further apart than the kernels address
+        x = torch.randn(40, (1 << 20) + 16, device=cuda)[None, :, :64]
+    gate = torch.randn(1, 40, 64, device=cuda)
+    x.requires_grad_(True)
+    assert x.is_leaf
+    eager, _ = race.race_gated_scan(x, gate)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            gate.mul(2)  # something to record
+            race.race_gated_scan(x, gate)
+    del eager

@@ -535,3 +535,21 @@ def test_kept_frequencies_are_complete_for_every_stream(race, cuda):
         assert module.inv_freq(cuda) is freq
     torch.cuda.synchronize()
     assert torch.equal(out, module(*rows))
+
+
+@pytest.mark.parametrize("layout", ["shifted", "apart"])
+def test_a_live_eager_graph_refuses_the_capture_of_copied_rows(race, cuda, layout):
+    # Rows that the op copies first are the caller's leaves all the same.
+    if layout == "shifted":  # not 16-byte aligned
+        leaf = torch.randn(1 * 40 * 2 * 64 + 1, device=cuda)[1:].view(1, 40, 2, 64)
+    else:  # the last dimension strided
+        leaf = torch.randn(1, 40, 2, 64, 2, device=cuda)[..., 0]
+    leaf.requires_grad_(True)
+    assert leaf.is_leaf
+    freq, pos = freqs(32, cuda), torch.arange(40, device=cuda)
+    eager, _ = race.race_norm_rope(leaf, None, pos, freq)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            freq.mul(2)  # something to record
+            race.race_norm_rope(leaf, None, pos, freq)
+    del eager
