@@ -59,6 +59,13 @@ class BatchedACE(nn.Module):
         self.rope_sections, self.rope_interleaved = rope_sections, rope_interleaved
         self._inv_freq = {}  # by device; float32 whatever the module is cast to, so no buffer
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._inv_freq = {}  # a pickle's may come back on another device
+        if "rope_pairs" not in self.__dict__:  # pickled before there were these keywords
+            self.norm_eps = self.q_norm = self.k_norm = self.rope_sections = None
+            self.rope_pairs, self.rope_theta, self.rope_interleaved = 0, 10000.0, False
+
     def inv_freq(self, device) -> torch.Tensor | None:
         """The rotation's frequencies [rope_pairs], float32."""
         if self.rope_pairs == 0:

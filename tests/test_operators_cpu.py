@@ -121,3 +121,31 @@ def test_frequencies_first_made_under_inference_mode_serve_training(race):
     leaf = torch.ones(16, requires_grad=True)
     (leaf * module.inv_freq(torch.device("cpu"))).sum().backward()  # saves them
     assert torch.equal(leaf.grad, race.BatchedACE(64, 4, 4, 1, rope_pairs=16).inv_freq(torch.device("cpu")))
+
+
+def test_modules_pickled_before_the_norm_and_rotation_load(race):
+    import pickle
+
+    rows = torch.randn(1, 2, 5, 3, 64)
+    for causal in (True, False):
+        module = race.BatchedACE(64, 4, 4, 1, causal=causal)
+        for name in ("norm_eps", "q_norm", "k_norm", "rope_pairs", "rope_theta", "rope_sections", "rope_interleaved",
+                     "_inv_freq"):
+            del module.__dict__[name]
+        old = pickle.loads(pickle.dumps(module))
+        assert torch.equal(old.planes_T, module.planes_T) and old.inv_freq(rows.device) is None
+        with pytest.raises(RuntimeError, match="CPU"):  # as far as any module comes here
+            old(rows, rows, rows)
+
+
+def test_copies_and_pickles_make_their_own_frequencies(race):
+    import copy
+    import pickle
+
+    module = race.CrossACE(64, 4, 4, 1, qk_norm=True, rope_pairs=16, rope_sections=[8, 8], rope_interleaved=True)
+    freq = module.inv_freq(torch.device("cpu"))
+    for other in (copy.deepcopy(module), copy.copy(module), pickle.loads(pickle.dumps(module))):
+        assert not other._inv_freq and torch.equal(other.inv_freq(torch.device("cpu")), freq)
+        assert other.rope_sections == [8, 8] and other.rope_interleaved and other.norm_eps == module.norm_eps
+        assert sorted(n for n, _ in other.named_parameters()) == ["k_norm", "q_norm"]
+    assert module.inv_freq(torch.device("cpu")) is freq
