@@ -99,8 +99,8 @@ class BatchedACE(nn.Module):
         return race_hash_probs(x2, self.planes_T.float(), self.L, self.K)
 
     def forward(self, Khf, Vhf, Qhf, positions=None):
-        """positions (with rope_pairs): [T] or [M * B, T], or [axes, M * B, T]
-        with rope_sections; None: 0 .. T-1."""
+        """positions (read with rope_pairs only): [T] or [M * B, T], or [axes,
+        M * B, T] with rope_sections; None: 0 .. T-1."""
         M, B, T, H, dk = Khf.shape
         N = M * B * H
         hashed = self.causal and hashed_supported(self.L, self.K, dk)

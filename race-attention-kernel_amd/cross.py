@@ -76,7 +76,8 @@ class CrossACE(BatchedACE):
         return out.view(M, B, H, T, dk).permute(0, 1, 3, 2, 4)
 
     def forward(self, Khf, Vhf, Qhf, lengths=None, k_positions=None, q_positions=None):
-        """lengths: int32 [M * B], the live keys of every batch entry."""
+        """lengths: int32 [M * B], the live keys of every batch entry.
+        k_positions, q_positions (read with rope_pairs only): as BatchedACE's."""
         probsK = self._side(Khf, self.k_norm, k_positions)
         probsQ = self._side(Qhf, self.q_norm, q_positions)
         return self._heads(race_cross_fwd(probsQ, probsK, self._values(Vhf), lengths), Qhf)
@@ -88,5 +89,9 @@ class CrossACE(BatchedACE):
 
     @torch.no_grad()
     def query(self, Qhf, state, q_positions=None):
-        """forward's output for Qhf against encode()'s sums: a decode step."""
+        """forward's output for Qhf against encode()'s sums: a decode step.  With
+        rope_pairs the tokens' q_positions are needed."""
+        if self.rope_pairs > 0 and q_positions is None:
+            raise ValueError("CrossACE.query: q_positions are needed where rows are rotated (a step's tokens do not "
+                             "start at position 0)")
         return self._heads(race_cross_query(self._side(Qhf, self.q_norm, q_positions), state), Qhf)

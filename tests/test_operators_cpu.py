@@ -149,3 +149,13 @@ def test_copies_and_pickles_make_their_own_frequencies(race):
         assert other.rope_sections == [8, 8] and other.rope_interleaved and other.norm_eps == module.norm_eps
         assert sorted(n for n, _ in other.named_parameters()) == ["k_norm", "q_norm"]
     assert module.inv_freq(torch.device("cpu")) is freq
+
+
+def test_a_decode_step_of_a_rotating_module_needs_its_positions(race):
+    # Counted from 0 every step would be rotated as the first.
+    Q, state = torch.randn(1, 2, 1, 3, 64), torch.zeros(6, 64 * 64 + 64)
+    with pytest.raises(ValueError, match="q_positions are needed"):
+        race.CrossACE(64, 4, 4, 1, rope_pairs=16).query(Q, state)
+    for options, positions in ((dict(rope_pairs=16), torch.tensor([7])), (dict(), None), (dict(qk_norm=True), None)):
+        with pytest.raises(RuntimeError, match="lives on the CPU"):  # past that check
+            race.CrossACE(64, 4, 4, 1, **options).query(Q, state, positions)
