@@ -86,6 +86,10 @@ struct Piece {
     }
 };
 
+// Where a thread past the channels reads: behind every tile's view, and with the
+// steps over a thread's rows added still within 32 bits (ScanTile checks both).
+constexpr int kPastTile = 1 << 30;
+
 // The rows from `r0` on (at most kTile of them, before `end`) of an array with
 // rows of D values `stride` apart: loads past them give zero, stores past them
 // are dropped.
@@ -169,6 +173,9 @@ template <int NT, int CL, int R, int V>
 struct ScanTile {
     static constexpr int kWaves = NT / 64, kTokenLanes = NT / CL, kTile = kTokenLanes * R, kChannels = CL * V;
     static constexpr int kLdsFloats = 2 * 2 * kWaves * kChannels;  // two buffers of the waves' pairs
+    static constexpr int64_t kRowBytes = int64_t(RACE_SCAN_MAX_TOKEN_STRIDE) * 4;  // at most, from row to row
+    static_assert((kTile - 1) * kRowBytes + int64_t(kScanMaxChannels) * 4 <= kPastTile, "behind the longest tile");
+    static_assert(kPastTile + R * kRowBytes <= INT32_MAX, "offsets of 32 bits");
     // The threads' pairs (P, H), in token order for kUp and against it
     // otherwise, applied to `carry`: start = the state this thread's tokens begin
     // with, carry = the state after all of them; with kProduct, `product` takes
@@ -276,9 +283,9 @@ __global__ __launch_bounds__(NT) void scan_forward_kernel(const ScanGeo g, const
     // channels reads zeros and writes nothing.
     constexpr int es = int(sizeof(TIn));
     const int xs = int(g.xt) * es, gs = int(g.gt) * es, os = int(D) * es;
-    const int xo = mine ? tl * R * xs + int(c) * es : mfma::kOutside;
-    const int go = mine ? tl * R * gs + int(c) * es : mfma::kOutside;
-    const int oo = mine ? tl * R * os + int(c) * es : mfma::kOutside;
+    const int xo = mine ? tl * R * xs + int(c) * es : kPastTile;
+    const int go = mine ? tl * R * gs + int(c) * es : kPastTile;
+    const int oo = mine ? tl * R * os + int(c) * es : kPastTile;
     X xn[R], gn[R];
     auto load = [&](int64_t r0) {
         const auto xr = rows_view<S::kTile>(xp, r0, end, g.xt, D);
@@ -390,9 +397,9 @@ __global__ __launch_bounds__(NT) void scan_backward_kernel(const ScanGeo g, cons
     TIn* dgp = a.dgate ? static_cast<TIn*>(a.dgate) + n * g.T * D : nullptr;
     constexpr int es = int(sizeof(TIn));
     const int xs = int(g.xt) * es, gs = int(g.gt) * es, os = int(D) * es;
-    const int xo = mine ? tl * R * xs + int(c) * es : mfma::kOutside;
-    const int go = mine ? tl * R * gs + int(c) * es : mfma::kOutside;
-    const int oo = mine ? tl * R * os + int(c) * es : mfma::kOutside;
+    const int xo = mine ? tl * R * xs + int(c) * es : kPastTile;
+    const int go = mine ? tl * R * gs + int(c) * es : kPastTile;
+    const int oo = mine ? tl * R * os + int(c) * es : kPastTile;
     X xn[R], gn[R], yn[R];
     float hn[V] = {};
     auto load = [&](int64_t r0) {

@@ -1686,7 +1686,7 @@ namespace {
 bool scan_shape(const race_scan_shape* sh, const int32_t* lengths, GatedScan* s) {
     if (!sh || sh->num_streams < 0 || sh->num_streams > kMaxStreams) return false;
     if (sh->seq_len < 0 || sh->seq_len > int64_t(INT_MAX) - kMaxAutoTile) return false;
-    if (sh->channels < 1 || sh->channels > 65536) return false;
+    if (sh->channels < 1 || sh->channels > kScanMaxChannels) return false;
     if (sh->dtype != RACE_F32 && sh->dtype != RACE_BF16) return false;
     if (sh->gate_form != RACE_GATE_SIGMOID && sh->gate_form != RACE_GATE_LOG) return false;
     if (sh->lengths_group < 1) return false;

@@ -467,6 +467,7 @@ struct GatedScan {
 // Calls without records of at most this many tokens run one thread per piece of
 // a row, token by token.
 constexpr int64_t kScanStepTokens = 16;
+constexpr int kScanMaxChannels = 65536;
 // Tokens of a backward tile, and the tiles (and records) of a stream.
 int64_t scan_tile_tokens(const GatedScan& s);
 int64_t scan_tiles(const GatedScan& s);

@@ -459,3 +459,22 @@ def test_a_live_eager_graph_refuses_the_capture_of_copied_rows(race, cuda, layou
             gate.mul(2)  # something to record
             race.race_gated_scan(x, gate)
     del eager
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [4, 68, 5])
+def test_the_longest_token_stride(race, cuda, D, dtype):
+    # Lanes past the channels step over rows 2^20 values apart too; they read and write nothing.
+    T, stride = 300, 1 << 20
+    x, gate, state, dout, dfinal = make(1, T, D, dtype, "sigmoid", 21, cuda)
+    wide = torch.full((T, stride), float("nan"), dtype=dtype, device=cuda)
+    far = wide[None, :, :D]
+    assert far.stride(1) == stride
+    for i, rows in enumerate((x, gate)):  # each of the two in turn
+        far.copy_(rows)
+        leaves = [t.detach().requires_grad_(True) for t in ((far, gate) if i == 0 else (x, far))]
+        out, final = race.race_gated_scan(*leaves, state)
+        grads = torch.autograd.grad((out, final), leaves, (dout, dfinal))
+        ref = reference(x, gate, state, None, "sigmoid", True, dout, dfinal, dtype)
+        for name, got in (("out", out), ("final", final), ("dx", grads[0]), ("dgate", grads[1])):
+            check(got, ref[name], f"stride 2^20 D{D} {dtype} {name}")
