@@ -326,9 +326,8 @@ def _plain_scan(case, x):
     out, final = h if keep is None else torch.where(keep, h, 0.0), h[:, -1].contiguous()
     if not case["train"]:
         return out.to(dt), final
-    up = x["dout"].float()
-    if keep is not None:
-        up = torch.where(keep, up, 0.0)
+    # Not the input's own storage: the final state's gradient is added in place.
+    up = torch.where(keep, x["dout"].float(), 0.0) if keep is not None else x["dout"].to(torch.float32, copy=True)
     up[:, -1] += x["dfinal"]
     after = torch.cat([a[:, 1:], torch.zeros_like(a[:, :1])], dim=1)
     lam = _linear_scan(after.flip(1), up.flip(1)).flip(1)
