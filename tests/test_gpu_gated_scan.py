@@ -478,3 +478,36 @@ def test_the_longest_token_stride(race, cuda, D, dtype):
         ref = reference(x, gate, state, None, "sigmoid", True, dout, dfinal, dtype)
         for name, got in (("out", out), ("final", final), ("dx", grads[0]), ("dgate", grads[1])):
             check(got, ref[name], f"stride 2^20 D{D} {dtype} {name}")
+
+
+# Training steps as large calls launch them (tests/test_operators_cpu.py pins the shapes):
+# 64 channels a workgroup and 128-token backward tiles where those workgroups fill the
+# device, 128 channels where wider ones do, few workgroups split over the tokens, and
+# rows past the caches.  The bound above holds: whatever the tile, the joins of one are
+# fewer than 32, and the later tiles' are covered by the terms' ages.
+LARGE = [(105, 1700, 128, torch.float32, "sigmoid", True, None), (24, 600, 520, torch.float32, "log", False, None),
+         (24, 600, 520, torch.bfloat16, "sigmoid", True, [600, 599, 256, 257, 128, 1, 0, 384]),
+         (24, 600, 520, torch.float32, "log", False, [600, 0, 511, 513]),
+         (210, 1700, 128, torch.bfloat16, "sigmoid", True, None), (2, 1500, 260, torch.float32, "sigmoid", False, [1500, 700]),
+         (39, 640, 260, torch.bfloat16, "sigmoid", True, [640, 1, 321]), (2, 45000, 256, torch.float32, "sigmoid", True, [45000, 44000]),
+         (8, 65536, 64, torch.bfloat16, "sigmoid", True, None)]
+
+
+@pytest.mark.parametrize("N, T, D, dtype, form, complement, lengths", LARGE)
+def test_training_steps_of_large_calls(race, cuda, N, T, D, dtype, form, complement, lengths):
+    x, gate, state, dout, dfinal = make(N, T, D, dtype, form, 31 * T + D, cuda)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda) if lengths else None
+    for t in (x, gate, state):
+        t.requires_grad_(True)
+    out, final = race.race_gated_scan(x, gate, state, gate_form=form, complement=complement, lengths=n)
+    grads = torch.autograd.grad((out, final), (x, gate, state), (dout, dfinal))
+    got = dict(zip(("out", "final", "dx", "dgate", "dstate"), (out, final, *grads)))
+    assert all(bool(torch.isfinite(t).all()) for t in got.values())
+    # Streams are computed apart: some of every length against the definition, all their channels.
+    group = N // len(lengths) if lengths else N
+    few = sorted({*range(0, N, group), *range(0, N, 16), N - 1}) if T < 10000 else [N - 1]
+    part = lambda t: t.detach()[few]
+    ref = reference(part(x), part(gate), part(state), None if n is None else n.repeat_interleave(group)[few].contiguous(),
+                    form, complement, part(dout), part(dfinal), dtype)
+    for name, t in got.items():
+        check(part(t), ref[name], f"large {N}x{T}x{D} {dtype} {name}")

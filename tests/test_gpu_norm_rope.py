@@ -553,3 +553,48 @@ def test_a_live_eager_graph_refuses_the_capture_of_copied_rows(race, cuda, layou
             freq.mul(2)  # something to record
             race.race_norm_rope(leaf, None, pos, freq)
     del eager
+
+
+# Rows enough for two a lane group, whole pieces of 8 and of 4 values (B, T, Hq, Hk, d, pairs, interleaved).
+TWO_ROWS = [(2, 4100, 6, 2, 64, 32, False), (2, 4100, 6, 2, 64, 32, True), (2, 3001, 4, 2, 96, 24, True),
+            (3, 2801, 4, 2, 40, 20, False), (1, 6001, 2, 1, 256, 100, True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B, T, Hq, Hk, d, pairs, interleaved", TWO_ROWS)
+def test_two_rows_a_lane_group(race, cuda, B, T, Hq, Hk, d, pairs, interleaved, dtype):
+    q, k, qw, kw, dq, dk = make(B, T, Hq, Hk, d, dtype, d + T, cuda)
+    freq, pos = freqs(pairs, cuda), torch.randint(0, 100000, (B, T), device=cuda)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+    outs = race.race_norm_rope(leaves[0], leaves[1], pos, freq, q_weight=leaves[2], k_weight=leaves[3],
+                               interleaved=interleaved)
+    grads = torch.autograd.grad(outs, leaves, (dq, dk))
+    for i, (x, w, up) in enumerate(((q, qw, dq), (k, kw, dk))):
+        ref = reference(x, w, pos, freq, None, interleaved, 1e-6, up)
+        label = f"two rows {dtype} {B}x{T}x{Hq}/{Hk}x{d} {'qk'[i]}"
+        check(outs[i], ref["out"], label + " out")
+        check(grads[i], ref["dx"], label + " dx")
+        check(grads[2 + i], ref["dw"], label + " dw")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B, T, Hq, Hk, d, pairs", [(3, 90001, 4, 1, 32, 16), (2, 4100, 6, 2, 64, 32), (2, 4100, 6, 2, 64, 0),
+                                                    (5, 700, 3, 3, 33, 8), (1, 1, 1, 1, 128, 64)])
+def test_weight_gradients_count_every_row(race, cuda, B, T, Hq, Hk, d, pairs, dtype):
+    # Values of one and minus one, nothing turned (frequencies of zero) and the rows themselves as upstream
+    # gradient: every row's term is r x x = r, its root 1 up to two steps, so a column's gradient is the number
+    # of rows.  A sum of R positive terms, each below a few hundred others in its chains, is off by at most
+    # 252 2^-24 R: less than a tile's rows, and less than one where there are fewer than 60000.
+    g = torch.Generator(device=cuda).manual_seed(1)
+    ones = lambda H: (torch.randint(0, 2, (B, T, H, d), generator=g, device=cuda) * 2 - 1).to(dtype)
+    q, k = ones(Hq), ones(Hk)
+    weights = [torch.randn(d, generator=g, device=cuda).requires_grad_(True) for _ in range(2)]
+    outs = race.race_norm_rope(q, k, torch.arange(T, device=cuda), torch.zeros(pairs, device=cuda) if pairs else None,
+                               q_weight=weights[0], k_weight=weights[1], eps=0.0)
+    grads = torch.autograd.grad(outs, weights, [x.transpose(1, 2).reshape(-1, T, d) for x in (q, k)])
+    for dw, H in zip(grads, (Hq, Hk)):
+        rows = B * T * H
+        worst = float((dw.double() - rows).abs().max())
+        say(f"count {dtype} {rows} rows x {d}", f"off by {worst}")
+        assert worst <= 252 * U * rows
+        assert bool((dw == dw[0]).all())  # every column adds the same terms in the same order

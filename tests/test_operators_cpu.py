@@ -159,3 +159,21 @@ def test_a_decode_step_of_a_rotating_module_needs_its_positions(race):
     for options, positions in ((dict(rope_pairs=16), torch.tensor([7])), (dict(), None), (dict(qk_norm=True), None)):
         with pytest.raises(RuntimeError, match="lives on the CPU"):  # past that check
             race.CrossACE(64, 4, 4, 1, **options).query(Q, state, positions)
+
+
+# (N, T, D, dtype, tokens of a backward tile, segments): the launch shapes of training
+# steps, which tests/test_gpu_gated_scan.py runs at these sizes.
+SCAN_FORMS = [(105, 1700, 128, 0, 128, 1), (24, 600, 520, 0, 128, 1), (24, 600, 520, 1, 128, 1), (210, 1700, 128, 1, 32, 1),
+              (2, 1500, 260, 0, 32, 24), (39, 640, 260, 1, 32, 4), (2, 45000, 256, 0, 32, 118), (8, 65536, 64, 1, 64, 64),
+              (8, 4096, 2048, 1, 128, 1), (24, 1531, 520, 0, 128, 1), (32, 4096, 2048, 1, 32, 1)]
+
+
+@pytest.mark.parametrize("N, T, D, dtype, tile, segments", SCAN_FORMS)
+def test_scan_forms(race, N, T, D, dtype, tile, segments):
+    from race_attention_kernel_amd import abi
+
+    sh = abi.scan_shape(N, T, D, dtype=dtype)
+    st, back, records = abi.gated_scan_workspace_bytes(sh, backward=True)
+    assert st == abi.RACE_SUCCESS and records == N * -(-T // tile) * D
+    pairs = N * segments * 2 * D
+    assert back == (0 if segments == 1 else 4 * (-(-pairs // 64) * 64))
