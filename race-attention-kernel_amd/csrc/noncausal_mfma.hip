@@ -777,8 +777,8 @@ struct MapWide {
 
 // The three terms of M[32 j + 8 g .. + 7][c] for j < kOps, zero past Wa rows and
 // Wb columns: a lane's operands of column c.  The operand as stage_operand reads
-// it, its divisors summed in `den` (LDS); the workgroups with `save` write the
-// undivided values.  A part's loads are all in flight together.
+// it, of one record, its divisors in `den` (LDS); the workgroups with `save` write
+// the undivided values.  The loads are all in flight together.
 template <int kOps>
 __device__ __forceinline__ void load_operand(bf16x8 (&m)[kOps][3], const MapOperand& op, const float* __restrict__ den,
                                              int64_t n, int Wa, int Wb, int c, int g, bool save) {
@@ -788,31 +788,23 @@ __device__ __forceinline__ void load_operand(bf16x8 (&m)[kOps][3], const MapOper
     // Byte offsets; past the end (kOutside and what is added to it) reads zeros.
     const int bytes = (plain ? (Wa - 1) * ld + Wb : (Wb - 1) * ld + Wa) * 4;
     const int at = there ? (plain ? k0 * ld + c : c * ld + k0) * 4 : kOutside;
-    const float* mn = op.m + n * op.stream;
+    const auto mr = mfma::make_rsrc(op.m + n * op.stream, bytes);
     float v[kOps][8];
-    for (int p = 0; p < op.parts; ++p) {
-        const auto mr = mfma::make_rsrc(mn + p * op.part_stride, bytes);
-        float x[kOps][8];
 #pragma unroll
-        for (int j = 0; j < kOps; ++j) {
-            const int off = 32 * j + k0 < Wa ? at : kOutside;  // rows come in whole eights
-            if (plain) {
+    for (int j = 0; j < kOps; ++j) {
+        const int off = 32 * j + k0 < Wa ? at : kOutside;  // rows come in whole eights
+        if (plain) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[j][e] = __uint_as_float(
-                        __builtin_amdgcn_raw_buffer_load_b32(mr, int(unsigned(off) + (32 * j + e) * ld * 4u), 0, 0));
-            } else {
-                const uint4 x0 = mfma::buf_load16<mfma::kPolicyDefault>(mr, int(unsigned(off) + 128 * j));
-                const uint4 x1 = mfma::buf_load16<mfma::kPolicyDefault>(mr, int(unsigned(off) + 128 * j + 16));
-                const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            for (int e = 0; e < 8; ++e)
+                v[j][e] = __uint_as_float(
+                    __builtin_amdgcn_raw_buffer_load_b32(mr, int(unsigned(off) + (32 * j + e) * ld * 4u), 0, 0));
+        } else {
+            const uint4 x0 = mfma::buf_load16<mfma::kPolicyDefault>(mr, int(unsigned(off) + 128 * j));
+            const uint4 x1 = mfma::buf_load16<mfma::kPolicyDefault>(mr, int(unsigned(off) + 128 * j + 16));
+            const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][e] = __uint_as_float(w[e]);
-            }
+            for (int e = 0; e < 8; ++e) v[j][e] = __uint_as_float(w[e]);
         }
-#pragma unroll
-        for (int j = 0; j < kOps; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = p ? v[j][e] + x[j][e] : x[j][e];
     }
     if (op.save && save) {
         const auto sr = mfma::make_rsrc(op.save + n * op.save_stream, bytes);
@@ -875,9 +867,7 @@ __global__ __launch_bounds__(64 * kMapWaves) void nc_map_wide_kernel(const bf16_
     if (op.div) {
         const int dens = op.col == 1 ? Wa : Wb;
         if (int(threadIdx.x) < dens) {
-            const float* dv = op.div + n * op.div_stream + threadIdx.x;
-            float q = dv[0];
-            for (int p = 1; p < op.parts; ++p) q += dv[p * op.part_stride];
+            const float q = op.div[n * op.div_stream + threadIdx.x];
             smem[threadIdx.x] = q;
             if (op.save && blk == 0) op.save[n * op.save_stream + op.save_div_off + threadIdx.x] = q;
         }
@@ -1321,11 +1311,35 @@ hipError_t launch_map_wide(const void* x, void* out, const MapOperand& op, const
     return hipGetLastError();
 }
 
+// Which of the two kernels a bf16 map of 72 .. 256 values to 72 .. 256 columns takes.
+// nc_map_wide_kernel reads its matrix straight from memory, every workgroup the
+// whole of it, before its first product; that is paid back where the reading
+// is short or the tokens or the streams are many.  In us, N streams x T tokens, S =
+// 256, d = 128, wide / nc_map_kernel:
+//   several records to add: 8 x 512 28.6 / 18.3, 32 x 577 33.4 / 22.8, 64 x 1024
+//     33.6 / 30.2, 384 x 1024 151 / 147;
+//   read as rows, no divisors (256 to 128): faster everywhere: 1 x 64 10.3 / 13.6,
+//     8 x 1024 11.4 / 14.3, 32 x 2048 22.7 / 28.8, 384 x 1024 117 / 141;
+//   read as columns, no divisors (128 to 256): 1 x 64 11.4 / 7.4, 8 x 4096 15.4 /
+//     13.6, 64 x 512 15.6 / 13.7, 32 x 2048 21.4 / 21.7, 1 x 65536 22.0 / 23.2,
+//     128 x 256 15.7 / 17.8, 256 x 64 14.1 / 22.4, 8 x 32768 70 / 95;
+//   with divisors (which wait for those), 128 to 256: 1 x 64 15.3 / 7.4, 8 x 4096
+//     20.9 / 14.0, 64 x 1024 25.7 / 20.8, 1 x 65536 26.5 / 23.2, 128 x 256 20.6 /
+//     18.6, 384 x 256 49.8 / 50.5, 256 x 64 18.8 / 22.5, 8 x 32768 76 / 94; 256 to
+//     128, one record: 128 x 64 19.4 / 15.6, 256 x 64 23.4 / 28.9.
+bool map_in_registers(const MapOperand& op, const Problem& p, int Wa, int Wb) {
+    constexpr int64_t kMi = int64_t(1) << 20;
+    if (Wb <= 64 || Wa <= 64 || Wa % 8 != 0 || op.parts > 1) return false;
+    const int64_t results = p.N * p.T * Wb, matrices = p.N * Wa * Wb;
+    if (op.div) return results >= 24 * kMi || matrices >= 8 * kMi;
+    return op.col == 1 || results >= 16 * kMi || matrices >= 4 * kMi;
+}
+
 template <typename TIn, bool kParts>
 hipError_t launch_map_t(const void* x, void* out, const MapOperand& op, const Problem& p, int Wa, int Wb,
                         hipStream_t stream) {
     if constexpr (sizeof(TIn) == 2 && !kParts) {
-        if (Wb > 64 && Wa > 64 && Wa % 8 == 0) {
+        if (map_in_registers(op, p, Wa, Wb)) {
             if (Wa > 128) return launch_map_wide<16, 1>(x, out, op, p, Wa, Wb, stream);
             return Wb > 128 ? launch_map_wide<8, 2>(x, out, op, p, Wa, Wb, stream)
                             : launch_map_wide<8, 1>(x, out, op, p, Wa, Wb, stream);

@@ -362,3 +362,39 @@ def test_module_decoder_step_by_step(race, cuda, dtype, options):
     got, want = torch.cat(steps, 2).double(), out.detach().double()
     size = want.abs().amax(dim=-1, keepdim=True)
     assert bool(((got - want).abs() <= (64 * 4 * U + 2 * HALF[dtype]) * size + 1e-30).all())
+
+
+# Sizes where the bf16 maps' matrices stay in registers: many streams, many tokens, key
+# lengths of one record and of several (csrc/noncausal_mfma.hip, map_in_registers).
+LARGE = [(256, 256, 40, 70, 8, 32, 128, None), (512, 512, 20, 30, 8, 16, 128, [30, 0, 7, 17]), (1, 1, 66000, 40, 8, 32, 128, None),
+         (2, 1, 50000, 3000, 8, 32, 72, [2999]), (260, 260, 33, 300, 8, 32, 128, [300, 64])]
+
+
+@pytest.mark.parametrize("Nq, Nk, Tq, Tk, L, R, d, lengths", LARGE)
+def test_large_calls(race, cuda, Nq, Nk, Tq, Tk, L, R, d, lengths):
+    q, k, v, dout = make(Nq, Nk, Tq, Tk, L, R, d, torch.bfloat16, Tq + Tk, cuda)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda) if lengths else None
+    ref = reference(q, k, v, n, dout)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = race.race_cross_fwd(*leaves, n)
+    grads = torch.autograd.grad(out, leaves, dout)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+        check(got.detach(), ref[name], f"large {Nq}/{Nk} {Tq}x{Tk} S{L * R} d{d} {name}")
+
+
+@pytest.mark.parametrize("N, L, R, d", [(256, 8, 32, 128), (512, 8, 16, 128), (460, 8, 32, 72), (400, 9, 8, 128)])
+def test_streams_do_not_depend_on_their_number(race, cuda, N, L, R, d):
+    # Few streams and many take different kernels; a stream's bits are the same, tokens with infinities and NaN too.
+    q, k, v, dout = make(N, N, 40, 50, L, R, d, torch.bfloat16, 9, cuda)
+    q[1, 3, 5], v[2, 7, 11], dout[3, 17, 2] = float("inf"), float("nan"), float("-inf")
+    state = race.race_cross_state(k, v)
+
+    def run(few):
+        leaves = [t[:few].clone().requires_grad_(True) for t in (q, k, v)]
+        out = race.race_cross_fwd(*leaves)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout[:few].contiguous()),
+                race.race_cross_query(q[:few].contiguous(), state[:few].contiguous()))
+
+    for a, b in zip(run(N), run(6)):
+        a = a[:6]
+        assert bool(((a == b) | (a.isnan() & b.isnan())).all())
