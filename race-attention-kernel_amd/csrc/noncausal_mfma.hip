@@ -260,13 +260,13 @@ struct Outer {
 
 // Stream and block of a workgroup: gfx950 hands consecutive workgroups to its 8
 // XCDs in turn, so the `per` blocks of one stream are 8 apart in launch order
-// and share an XCD's L2 (the matrix records a stream's workgroups all read).
-__device__ __forceinline__ void stream_block(int64_t id, int64_t N, int per, int64_t& n, int& blk) {
-    const int64_t group = id / (8 * per);
-    const int in = int(id - group * 8 * per);
-    const int streams = int(min<int64_t>(8, N - 8 * group));
-    n = 8 * group + in % streams;
-    blk = in / streams;
+// and share an XCD's L2 (the matrix records a stream's workgroups all read).  In
+// 32 bits: every wave divides before its first load, and 64-bit divisions took
+// the reductions of short calls 1 us (64 x 128 tokens, S = 256, d = 128: 12.5 us).
+__device__ __forceinline__ void stream_block(unsigned id, unsigned N, unsigned per, int64_t& n, int& blk) {
+    const unsigned group = id / (8 * per), in = id - group * (8 * per), streams = min(8u, N - 8 * group);
+    blk = int(in / streams);
+    n = 8 * group + (in - unsigned(blk) * streams);
 }
 
 // One workgroup per (chunk of tokens, stream, block of R); with several blocks
@@ -289,8 +289,8 @@ __global__ __launch_bounds__(kThreads, 3) void nc_sums_kernel(
     int z = blockIdx.z;
     if (flat) {
         int64_t pair;
-        stream_block(blockIdx.x, N * chunks, flat, pair, z);
-        n = pair / chunks;
+        stream_block(blockIdx.x, unsigned(N * chunks), unsigned(flat), pair, z);
+        n = unsigned(pair) / unsigned(chunks);
         ci = pair - n * chunks;
     }
     const int a0 = 16 * EA * (z / bblocks), b0 = 16 * EB * (z % bblocks);
@@ -1246,7 +1246,13 @@ hipError_t launch_sums_e(const void* x, const void* y, float* records, const Pro
                          hipStream_t stream) {
     const int ab = (Wa + 16 * EA - 1) / (16 * EA), bb = (Wb + 16 * EB - 1) / (16 * EB);
     const int64_t all = p.tiles * p.N * ab * bb;
-    const bool flat = ab * bb > 1 && all * kThreads < (int64_t(1) << 32);
+    // Blocks of one chunk next to each other on an XCD pay where the rows are more than
+    // the eight L2s hold: S = 256, d = 128 in bf16, us so / apart: 384 x 1024 tokens 98
+    // / 136, 32 x 2048 (50 MB) 22.3 / 25.9, 32 x 1024 (25 MB) 18.2 / 18.0, 384 x 64 19.2
+    // / 18.4, 1000 x 16 46.8 / 41.0.
+    constexpr int64_t kL2Bytes = int64_t(32) << 20;
+    const bool flat = ab * bb > 1 && p.N * p.T * (Wa + Wb) * int64_t(sizeof(TIn)) >= kL2Bytes &&
+                      all * kThreads < (int64_t(1) << 32);
     const dim3 grid = flat ? dim3(unsigned(all)) : dim3(unsigned(p.tiles), unsigned(p.N), unsigned(ab * bb));
     nc_sums_kernel<TIn, EA, EB, kEndFirst, kParts><<<grid, kThreads, Outer<EA, EB>::kLdsFloats * sizeof(float), stream>>>(
         static_cast<const TIn*>(x), static_cast<const TIn*>(y), records, p.T, p.tile, p.tiles, p.rec, Wa, Wb, bb,
