@@ -601,11 +601,21 @@ using Narrow = ScanShape<4, 16, 512, 512>;
 using NarrowSplit = ScanShape<4, 16, 256, 256>;
 using Single = ScanShape<1, 64, 512, 512, 8, 8>;  // any strides and widths
 
-// Workgroups that fill the device without a split of the tokens, and that a
-// split aims for; a split costs a launch, two tiles cost less (10 x 160 x 24,
-// two tiles, 7.6 + 11.2 us whole and 9.9 + 13.3 split; 2 x 290 x 64, three, 10.2 +
-// 17.3 and 9.5 + 13.0).
-constexpr int64_t kScanEnough = 200, kScanSplit = 512, kScanWhole = 2;
+// Workgroups from which the tokens are not split, those of 128 channels that are
+// taken before those of 64, and those a split aims for; two tiles are never split.
+// Whole and split in us, forward and with the backward, by the workgroups of 64
+// channels (8 x 4096 tokens in bf16, then 8 x 4096 and 24 x 1531 in fp32):
+//   128    77 / 223 and 74 / 172     98 / 276 and 113 / 260
+//   144    75 / 222 and 88 / 205     96 / 273 and 126 / 300     39 / 106 and 51 / 118
+//   160    78 / 225 and 96 / 222    108 / 310 and 147 / 357
+//   168    75 / 222 and 105 / 257                               40 / 110 and 65 / 142
+//   192    80 / 238 and 102 / 260   121 / 328 and 164 / 407     48 / 123 and 75 / 159
+// from 168 on every call gains (at 160, 2 x 32768 tokens in bf16 trained in 1930
+// whole and 1750 split).  Of 128 channels 104 workgroups took 133 / 486 where 200 of
+// 64 took 75 / 225.  A split costs a launch, two tiles cost less (10 x 160 x 24, two
+// tiles, 7.6 + 11.2 whole and 9.9 + 13.3 split; 2 x 290 x 64, three, 10.2 + 17.3 and
+// 9.5 + 13.0).
+constexpr int64_t kScanEnough = 168, kScanWide = 200, kScanSplit = 512, kScanWhole = 2;
 
 int64_t blocks_of(const GatedScan& s, int64_t channels) { return s.N * ((s.D + channels - 1) / channels); }
 
@@ -617,7 +627,7 @@ bool scan_vectors(const GatedScan& s) {
 template <typename F>
 auto by_shape(const GatedScan& s, F f) {
     if (!scan_vectors(s)) return f(Single{});
-    if (blocks_of(s, Wide::kChannels) >= kScanEnough) return f(Wide{});
+    if (blocks_of(s, Wide::kChannels) >= kScanWide) return f(Wide{});
     if (blocks_of(s, Narrow::kChannels) >= kScanEnough) return f(Narrow{});
     return s.D > 96 ? f(WideSplit{}) : f(NarrowSplit{});
 }

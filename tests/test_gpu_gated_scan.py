@@ -489,7 +489,8 @@ LARGE = [(105, 1700, 128, torch.float32, "sigmoid", True, None), (24, 600, 520, 
          (24, 600, 520, torch.bfloat16, "sigmoid", True, [600, 599, 256, 257, 128, 1, 0, 384]),
          (24, 600, 520, torch.float32, "log", False, [600, 0, 511, 513]),
          (210, 1700, 128, torch.bfloat16, "sigmoid", True, None), (2, 1500, 260, torch.float32, "sigmoid", False, [1500, 700]),
-         (39, 640, 260, torch.bfloat16, "sigmoid", True, [640, 1, 321]), (2, 45000, 256, torch.float32, "sigmoid", True, [45000, 44000]),
+         (39, 640, 260, torch.bfloat16, "sigmoid", True, [640, 1, 321]), (32, 640, 260, torch.bfloat16, "log", True, [640, 1, 321, 0]),
+         (2, 45000, 256, torch.float32, "sigmoid", True, [45000, 44000]),
          (8, 65536, 64, torch.bfloat16, "sigmoid", True, None)]
 
 

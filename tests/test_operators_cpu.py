@@ -164,8 +164,9 @@ def test_a_decode_step_of_a_rotating_module_needs_its_positions(race):
 # (N, T, D, dtype, tokens of a backward tile, segments): the launch shapes of training
 # steps, which tests/test_gpu_gated_scan.py runs at these sizes.
 SCAN_FORMS = [(105, 1700, 128, 0, 128, 1), (24, 600, 520, 0, 128, 1), (24, 600, 520, 1, 128, 1), (210, 1700, 128, 1, 32, 1),
-              (2, 1500, 260, 0, 32, 24), (39, 640, 260, 1, 32, 4), (2, 45000, 256, 0, 32, 118), (8, 65536, 64, 1, 64, 64),
-              (8, 4096, 2048, 1, 128, 1), (24, 1531, 520, 0, 128, 1), (32, 4096, 2048, 1, 32, 1)]
+              (2, 1500, 260, 0, 32, 24), (39, 640, 260, 1, 128, 1), (32, 640, 260, 1, 32, 5), (2, 45000, 256, 0, 32, 118), (8, 65536, 64, 1, 64, 64),
+              (8, 4096, 2048, 1, 128, 1), (24, 1531, 520, 0, 128, 1), (32, 4096, 2048, 1, 32, 1), (8, 4096, 1536, 1, 128, 1),
+              (24, 1531, 448, 0, 128, 1), (8, 4096, 1280, 1, 32, 6)]
 
 
 @pytest.mark.parametrize("N, T, D, dtype, tile, segments", SCAN_FORMS)
