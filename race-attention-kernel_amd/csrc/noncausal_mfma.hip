@@ -757,9 +757,10 @@ __global__ __launch_bounds__(64 * NW) void nc_map_kernel(const TIn* __restrict__
 // results of tile i leave through LDS as whole rows while tile i + 1 is
 // multiplied.  The same products in the same order: the same bits.  32 x 4096
 // tokens, 256 to 128 columns (100 MB): 36 us, 45 with nc_map_kernel; 32 x 8192 74
-// and 93.  Bound by its three-term products (26 GFLOP) and the tokens together,
-// 21 us each at the rates of a large product and a large copy.  At 64 values
-// nc_map_kernel is the faster (15 us for 32 x 4096 x 64 to 128, 23 here).
+// and 93.  Bound by its three-term products (26 GFLOP, 21 us at the rate of a large
+// product) and the tokens (18 us at 5.7 TB/s) together, and by the matrix's reading
+// (7 us).  At 64 values nc_map_kernel is the faster (15 us for 32 x 4096 x 64 to 128,
+// 23 here), and on short calls (map_in_registers).
 constexpr int kWideTile = 32;
 
 template <int NJ, int NCW>
