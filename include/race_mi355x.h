@@ -656,6 +656,71 @@ race_status race_gated_scan_bwd(const void* x, const void* gate, const int32_t* 
                                 const race_scan_shape* shape, void* workspace, size_t workspace_bytes,
                                 hipStream_t stream);
 
+/* ---- Norms of whole rows around a recurrent layer -----------------------
+ * In front of a layer's projections: the residual's addition and the norm of
+ * the sum, s = x + residual, y = s / sqrt(mean(s^2) + eps) * weight, over rows
+ * of `width` values; with RACE_ROWS_E4M3 y in 8 bits for an 8-bit projection:
+ * scale = max |y| / 448 over a row or a group of its columns, and y / scale
+ * rounded to e4m3.  Behind a recurrence: its streams as rows, normed and gated,
+ * y = x / sqrt(mean(x^2) + eps) * weight * gate * sigmoid(gate).  No counterpart
+ * in the reference. */
+typedef enum race_rows {
+    RACE_ROWS_SAME = 0, /* y in the rows' dtype */
+    RACE_ROWS_E4M3 = 1  /* y as e4m3 bytes (4 exponent bits, no infinities) with fp32 scales */
+} race_rows;
+
+typedef struct race_add_norm_shape {
+    int64_t rows;
+    int32_t width;               /* 1 .. 16384 */
+    int32_t dtype, weight_dtype; /* race_dtype */
+    int32_t out;                 /* race_rows */
+    int32_t group;               /* columns of a scale: 0 (a row), 32, 64 or 128; widths and strides multiples of 8 */
+    float eps;
+    int64_t x_row_stride, residual_row_stride; /* in elements */
+} race_add_norm_shape;
+
+/* y [rows][width] and sum [rows][width] (the rows' dtype; with a residual only),
+ * scales [rows][ceil(width / group)] or [rows], contiguous.  residual and weight
+ * are nullable.  Everything starts 16-byte aligned. */
+race_status race_add_norm_fwd(const void* x, const void* residual, const void* weight, void* y, float* scales, void* sum,
+                              const race_add_norm_shape* shape, hipStream_t stream);
+
+/* Workspace of race_add_norm_bwd in bytes (needed only for the weight's gradient). */
+race_status race_add_norm_bwd_workspace_bytes(const race_add_norm_shape* shape, size_t* bytes);
+
+/* Gradients for the upstream gradients dy and dsum (each nullable: zero) of y and
+ * sum, from the normed rows s (sum, or x without a residual, by x_row_stride).
+ * dx [rows][width] is the gradient of x and of the residual alike; dx and dweight
+ * may be NULL to skip them.  Not for RACE_ROWS_E4M3. */
+race_status race_add_norm_bwd(const void* s, const void* weight, const void* dy, const void* dsum, void* dx,
+                              void* dweight, const race_add_norm_shape* shape, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream);
+
+typedef struct race_gate_norm_shape {
+    int64_t batch, seq_len;      /* batch * seq_len <= 2^30 */
+    int32_t heads;               /* 1 .. 65535 */
+    int32_t head_dim;            /* 1 .. 256 */
+    int32_t dtype, weight_dtype; /* race_dtype */
+    float eps;
+    /* Strides in elements, the values of a row next to each other. */
+    int64_t x_stream_stride, x_token_stride;
+    int64_t gate_batch_stride, gate_token_stride, gate_head_stride;
+} race_gate_norm_shape;
+
+/* x [batch * heads][seq_len] rows, gate [batch][seq_len][heads] rows, y
+ * [batch][seq_len][heads][head_dim], contiguous.  weight is nullable. */
+race_status race_gate_norm_fwd(const void* x, const void* gate, const void* weight, void* y,
+                               const race_gate_norm_shape* shape, hipStream_t stream);
+
+/* Workspace of race_gate_norm_bwd in bytes (needed only for the weight's gradient). */
+race_status race_gate_norm_bwd_workspace_bytes(const race_gate_norm_shape* shape, size_t* bytes);
+
+/* dx [batch * heads][seq_len][head_dim], dgate [batch][seq_len][heads][head_dim]
+ * and dweight, each nullable, for the upstream gradient dy. */
+race_status race_gate_norm_bwd(const void* x, const void* gate, const void* weight, const void* dy, void* dx,
+                               void* dgate, void* dweight, const race_gate_norm_shape* shape, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ from . import causal_v2
 from .batched_ace import BatchedACE
 from .cross import CrossACE, race_cross_fwd, race_cross_query, race_cross_state
 from .inputs import CONFIGS, Config, config_inputs, make_inputs
+from .norm import race_add_norm, race_add_norm_e4m3, race_gate_norm
 from .ops import (HashedRaceFunction, HashProbsFunction, RaceFusedFunction, hashed_supported,
                   race_causal_backward, race_fused_fwd, race_fused_fwd_carry, race_fused_fwd_hashed,
                   race_fused_fwd_with_state, race_hash_probs, race_noncausal_backward,
@@ -23,4 +24,5 @@ __all__ = [
     "CrossACE", "race_cross_fwd", "race_cross_query", "race_cross_state",
     "race_norm_rope",
     "race_gated_scan", "race_gated_scan_carry",
+    "race_add_norm", "race_add_norm_e4m3", "race_gate_norm",
 ]

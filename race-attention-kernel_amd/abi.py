@@ -80,6 +80,12 @@ EXPORTED_SYMBOLS = (
     "race_gated_scan_workspace_bytes",
     "race_gated_scan_fwd",
     "race_gated_scan_bwd",
+    "race_add_norm_fwd",
+    "race_add_norm_bwd_workspace_bytes",
+    "race_add_norm_bwd",
+    "race_gate_norm_fwd",
+    "race_gate_norm_bwd_workspace_bytes",
+    "race_gate_norm_bwd",
 )
 
 
@@ -118,6 +124,34 @@ class RaceCrossShape(ctypes.Structure):
         ("head_dim", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("lengths_group", ctypes.c_int32),
+    ]
+
+
+class RaceAddNormShape(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("width", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("out", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("x_row_stride", ctypes.c_int64),
+        ("residual_row_stride", ctypes.c_int64),
+    ]
+
+
+class RaceGateNormShape(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("seq_len", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("x_strides", ctypes.c_int64 * 2),  # stream, token
+        ("gate_strides", ctypes.c_int64 * 3),  # batch, token, head
     ]
 
 
@@ -228,6 +262,13 @@ def lib() -> ctypes.CDLL:
         L.race_gated_scan_workspace_bytes.argtypes = [sc, i32, ctypes.POINTER(sz), ctypes.POINTER(i64)]
         L.race_gated_scan_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
         L.race_gated_scan_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
+        an, gn = ctypes.POINTER(RaceAddNormShape), ctypes.POINTER(RaceGateNormShape)
+        L.race_add_norm_fwd.argtypes = [vp, vp, vp, vp, vp, vp, an, vp]
+        L.race_add_norm_bwd_workspace_bytes.argtypes = [an, ctypes.POINTER(sz)]
+        L.race_add_norm_bwd.argtypes = [vp, vp, vp, vp, vp, vp, an, vp, sz, vp]
+        L.race_gate_norm_fwd.argtypes = [vp, vp, vp, vp, gn, vp]
+        L.race_gate_norm_bwd_workspace_bytes.argtypes = [gn, ctypes.POINTER(sz)]
+        L.race_gate_norm_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, gn, vp, sz, vp]
         for name in EXPORTED_SYMBOLS[2:]:
             getattr(L, name).restype = i32
         _configured = True
@@ -579,3 +620,53 @@ def cross_bwd(q: int, k: int, v: int, lengths: int | None, g: int, state: int, d
     """race_cross_bwd on raw device addresses; returns the status."""
     return lib().race_cross_bwd(q, k, v, lengths, g, state, dq, dk, dv, ctypes.byref(sh), workspace, workspace_bytes,
                                 stream)
+
+
+def add_norm_shape(rows: int, D: int, *, dtype: int = RACE_F32, weight_dtype: int = RACE_F32, out: int = 0, group: int = 0,
+                   eps: float = 1e-6, x_stride: int | None = None, residual_stride: int | None = None) -> RaceAddNormShape:
+    """The shape of rows [rows][D], contiguous where no stride is given."""
+    return RaceAddNormShape(rows, D, dtype, weight_dtype, out, group, eps, D if x_stride is None else x_stride,
+                            D if residual_stride is None else residual_stride)
+
+
+def add_norm_fwd(x: int, residual: int | None, weight: int | None, y: int, scales: int | None, total: int | None,
+                 sh: RaceAddNormShape, stream: int) -> int:
+    """race_add_norm_fwd on raw device addresses; returns the status."""
+    return lib().race_add_norm_fwd(x, residual, weight, y, scales, total, ctypes.byref(sh), stream)
+
+
+def add_norm_bwd_workspace_bytes(sh: RaceAddNormShape):
+    """(status, bytes)."""
+    b = ctypes.c_size_t(0)
+    return lib().race_add_norm_bwd_workspace_bytes(ctypes.byref(sh), ctypes.byref(b)), b.value
+
+
+def add_norm_bwd(s: int, weight: int | None, dy: int | None, dsum: int | None, dx: int | None, dweight: int | None,
+                 sh: RaceAddNormShape, workspace: int | None, workspace_bytes: int, stream: int) -> int:
+    """race_add_norm_bwd on raw device addresses; returns the status."""
+    return lib().race_add_norm_bwd(s, weight, dy, dsum, dx, dweight, ctypes.byref(sh), workspace, workspace_bytes, stream)
+
+
+def gate_norm_shape(B: int, T: int, H: int, d: int, *, dtype: int = RACE_F32, weight_dtype: int = RACE_F32,
+                    eps: float = 1e-6) -> RaceGateNormShape:
+    """The shape of contiguous streams [B * H][T][d] and gates [B][T][H][d]."""
+    return RaceGateNormShape(B, T, H, d, dtype, weight_dtype, eps, (ctypes.c_int64 * 2)(T * d, d),
+                             (ctypes.c_int64 * 3)(T * H * d, H * d, d))
+
+
+def gate_norm_fwd(x: int, gate: int, weight: int | None, y: int, sh: RaceGateNormShape, stream: int) -> int:
+    """race_gate_norm_fwd on raw device addresses; returns the status."""
+    return lib().race_gate_norm_fwd(x, gate, weight, y, ctypes.byref(sh), stream)
+
+
+def gate_norm_bwd_workspace_bytes(sh: RaceGateNormShape):
+    """(status, bytes)."""
+    b = ctypes.c_size_t(0)
+    return lib().race_gate_norm_bwd_workspace_bytes(ctypes.byref(sh), ctypes.byref(b)), b.value
+
+
+def gate_norm_bwd(x: int, gate: int, weight: int | None, dy: int, dx: int | None, dgate: int | None, dweight: int | None,
+                  sh: RaceGateNormShape, workspace: int | None, workspace_bytes: int, stream: int) -> int:
+    """race_gate_norm_bwd on raw device addresses; returns the status."""
+    return lib().race_gate_norm_bwd(x, gate, weight, dy, dx, dgate, dweight, ctypes.byref(sh), workspace, workspace_bytes,
+                                    stream)

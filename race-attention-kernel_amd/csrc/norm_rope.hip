@@ -22,49 +22,10 @@
 // then over the workgroups by a second kernel, all in a fixed order.
 #include <algorithm>
 
-#include "mfma_common.h"
+#include "row_run.h"
 
 namespace race {
 namespace {
-
-// V consecutive values.
-template <typename TIn, int V>
-struct Run {
-    static constexpr int kWords = V * int(sizeof(TIn)) / 4 > 0 ? V * int(sizeof(TIn)) / 4 : 1;
-    uint32_t w[kWords];
-    __device__ __forceinline__ void load(const TIn* p) {
-        if constexpr (V * sizeof(TIn) == 16) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        } else if constexpr (V * sizeof(TIn) == 8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            w[0] = v.x, w[1] = v.y;
-        } else if constexpr (sizeof(TIn) == 4) {
-            w[0] = __float_as_uint(*p);
-        } else {
-            w[0] = *p;
-        }
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = 0;
-    }
-    __device__ __forceinline__ float get(int e) const {
-        if constexpr (sizeof(TIn) == 4) return __uint_as_float(w[e]);
-        return (e & 1) ? mfma::hi_half(w[e >> 1]) : mfma::lo_half(w[e >> 1]);
-    }
-    __device__ __forceinline__ static void store(TIn* p, const float (&x)[V]) {
-        if constexpr (V * sizeof(TIn) == 16 && sizeof(TIn) == 4)
-            *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        else if constexpr (V * sizeof(TIn) == 16)
-            *reinterpret_cast<uint4*>(p) = make_uint4(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]),
-                                                      mfma::pack2(x[4], x[5]), mfma::pack2(x[6], x[7]));
-        else if constexpr (V * sizeof(TIn) == 8)
-            *reinterpret_cast<uint2*>(p) = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
-        else
-            store_val(p, x[0]);
-    }
-};
 
 // Queries (0) and keys (1) of a launch.
 struct RopeTensor {

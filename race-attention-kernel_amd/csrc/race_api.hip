@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <initializer_list>
 #include <mutex>
 
 #include "race_internal.h"
@@ -2088,6 +2089,131 @@ race_status race_cross_bwd(const void* probsQ, const void* probsK, const void* V
     }
     if (dV) RACE_TRY(launch_nc_map(probsK, dV, map_operand(dB, Sd, q.d, 1), k, k.S, k.d, stream));
     return RACE_SUCCESS;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Norms of whole rows around a recurrent layer (row_norm.hip).
+
+namespace race {
+namespace {
+
+bool row_dtypes(int32_t rows, int32_t weights) {
+    return (rows == RACE_F32 || rows == RACE_BF16) && (weights == RACE_F32 || weights == RACE_BF16);
+}
+
+bool add_norm_shape(const race_add_norm_shape* sh, AddNorm* n) {
+    if (!sh || sh->rows < 0 || sh->width < 1 || sh->width > kAddNormMaxWidth) return false;
+    if (sh->rows > (int64_t(1) << 46) / sh->width) return false;
+    if (!row_dtypes(sh->dtype, sh->weight_dtype) || !(sh->eps >= 0.f)) return false;
+    for (int64_t s : {sh->x_row_stride, sh->residual_row_stride})
+        if (s < 0 || s > (int64_t(1) << 40)) return false;
+    if (sh->out != RACE_ROWS_SAME && sh->out != RACE_ROWS_E4M3) return false;
+    if (sh->group != 0) {
+        if (sh->out != RACE_ROWS_E4M3 || (sh->group != 32 && sh->group != 64 && sh->group != 128)) return false;
+        // A group is whole 16-byte pieces of a row.
+        if (sh->width % 8 != 0 || sh->x_row_stride % 8 != 0 || sh->residual_row_stride % 8 != 0) return false;
+    }
+    *n = AddNorm{sh->rows,  sh->x_row_stride, sh->residual_row_stride,   sh->width, sh->dtype, sh->weight_dtype,
+                 sh->out == RACE_ROWS_E4M3, sh->group, sh->eps};
+    return true;
+}
+
+bool gate_norm_shape(const race_gate_norm_shape* sh, GateNorm* n) {
+    if (!sh || sh->batch < 0 || sh->seq_len < 0 || sh->heads < 1 || sh->heads > 65535) return false;
+    if (sh->seq_len > 0 && sh->batch > (int64_t(1) << 30) / sh->seq_len) return false;
+    if (sh->head_dim < 1 || sh->head_dim > kGateNormMaxDim) return false;
+    if (!row_dtypes(sh->dtype, sh->weight_dtype) || !(sh->eps >= 0.f)) return false;
+    for (int64_t s : {sh->x_stream_stride, sh->x_token_stride, sh->gate_batch_stride, sh->gate_token_stride,
+                      sh->gate_head_stride})
+        if (s < 0 || s > (int64_t(1) << 40)) return false;
+    *n = GateNorm{sh->batch,           sh->seq_len,           sh->heads,
+                  sh->head_dim,        sh->x_stream_stride,   sh->x_token_stride,
+                  sh->gate_batch_stride, sh->gate_token_stride, sh->gate_head_stride,
+                  sh->dtype,           sh->weight_dtype,      sh->eps};
+    return true;
+}
+
+bool all_aligned16(std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if (!aligned16(p)) return false;
+    return true;
+}
+
+}  // namespace
+}  // namespace race
+
+extern "C" {
+
+race_status race_add_norm_fwd(const void* x, const void* residual, const void* weight, void* y, float* scales, void* sum,
+                              const race_add_norm_shape* shape, hipStream_t stream) {
+    AddNorm n;
+    if (!add_norm_shape(shape, &n)) return RACE_ERROR_INVALID_VALUE;
+    if (n.rows == 0) return RACE_SUCCESS;
+    if (!x || !y || (residual && !sum) || (n.e4m3 && !scales)) return RACE_ERROR_INVALID_VALUE;
+    if (!all_aligned16({x, residual, weight, y, scales, sum})) return RACE_ERROR_INVALID_VALUE;
+    return launch_add_norm(n, x, residual, weight, y, scales, sum, stream);
+}
+
+race_status race_add_norm_bwd_workspace_bytes(const race_add_norm_shape* shape, size_t* bytes) {
+    AddNorm n;
+    if (!add_norm_shape(shape, &n) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    *bytes = size_t(add_norm_partial_floats(n)) * sizeof(float);
+    return RACE_SUCCESS;
+}
+
+race_status race_add_norm_bwd(const void* s, const void* weight, const void* dy, const void* dsum, void* dx,
+                              void* dweight, const race_add_norm_shape* shape, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream) {
+    AddNorm n;
+    if (!add_norm_shape(shape, &n) || n.e4m3) return RACE_ERROR_INVALID_VALUE;
+    if (!all_aligned16({s, weight, dy, dsum, dx, dweight})) return RACE_ERROR_INVALID_VALUE;
+    if (!dx && !dweight) return RACE_SUCCESS;
+    if (n.rows == 0) {
+        if (!dweight) return RACE_SUCCESS;
+        return zero_bytes(dweight, size_t(n.D) * (n.weight_dtype == RACE_F32 ? 4 : 2), stream);
+    }
+    if (!s) return RACE_ERROR_INVALID_VALUE;
+    if (dweight && (!workspace || !aligned16(workspace) ||
+                    workspace_bytes < size_t(add_norm_partial_floats(n)) * sizeof(float)))
+        return RACE_ERROR_INVALID_VALUE;
+    n.rs = 0;
+    return launch_add_norm_bwd(n, s, weight, dy, dsum, dx, dweight, static_cast<float*>(workspace), stream);
+}
+
+race_status race_gate_norm_fwd(const void* x, const void* gate, const void* weight, void* y,
+                               const race_gate_norm_shape* shape, hipStream_t stream) {
+    GateNorm n;
+    if (!gate_norm_shape(shape, &n)) return RACE_ERROR_INVALID_VALUE;
+    if (n.B == 0 || n.T == 0) return RACE_SUCCESS;
+    if (!x || !gate || !y || !all_aligned16({x, gate, weight, y})) return RACE_ERROR_INVALID_VALUE;
+    return launch_gate_norm(n, x, gate, weight, y, stream);
+}
+
+race_status race_gate_norm_bwd_workspace_bytes(const race_gate_norm_shape* shape, size_t* bytes) {
+    GateNorm n;
+    if (!gate_norm_shape(shape, &n) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    *bytes = size_t(gate_norm_partial_floats(n)) * sizeof(float);
+    return RACE_SUCCESS;
+}
+
+race_status race_gate_norm_bwd(const void* x, const void* gate, const void* weight, const void* dy, void* dx,
+                               void* dgate, void* dweight, const race_gate_norm_shape* shape, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream) {
+    GateNorm n;
+    if (!gate_norm_shape(shape, &n)) return RACE_ERROR_INVALID_VALUE;
+    if (!all_aligned16({x, gate, weight, dy, dx, dgate, dweight})) return RACE_ERROR_INVALID_VALUE;
+    if (!dx && !dgate && !dweight) return RACE_SUCCESS;
+    if (n.B == 0 || n.T == 0) {
+        if (!dweight) return RACE_SUCCESS;
+        return zero_bytes(dweight, size_t(n.d) * (n.weight_dtype == RACE_F32 ? 4 : 2), stream);
+    }
+    if (!x || !gate || !dy) return RACE_ERROR_INVALID_VALUE;
+    if (dweight && (!workspace || !aligned16(workspace) ||
+                    workspace_bytes < size_t(gate_norm_partial_floats(n)) * sizeof(float)))
+        return RACE_ERROR_INVALID_VALUE;
+    return launch_gate_norm_bwd(n, x, gate, weight, dy, dx, dgate, dweight, static_cast<float*>(workspace), stream);
 }
 
 }  // extern "C"

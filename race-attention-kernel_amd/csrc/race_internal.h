@@ -483,6 +483,42 @@ hipError_t launch_gated_scan_bwd(const GatedScan& s, const void* x, const void* 
                                  const float* records, const float* dfinal, void* dx, void* dgate, float* dstate,
                                  float* pairs, hipStream_t stream);
 
+// ---- norms of whole rows around a recurrent layer (row_norm.hip) ----
+// Rows [rows][D] by row strides; the residual's addition, the norm and, with
+// e4m3, its rows in 8 bits with a scale per `group` columns (0: per row).
+struct AddNorm {
+    int64_t rows, xs, rs;  // row strides of x and the residual in elements
+    int D;
+    int dtype, weight_dtype;
+    bool e4m3;
+    int group;
+    float eps;
+};
+constexpr int kAddNormMaxWidth = 16384;
+int64_t add_norm_partial_floats(const AddNorm& n);
+// residual (with it sum) and w may be null; scales with e4m3 only.
+hipError_t launch_add_norm(const AddNorm& n, const void* x, const void* residual, const void* w, void* y, float* scales,
+                           void* sum, hipStream_t stream);
+// s: the rows that were normed, by n.xs; dy, dsum, dx and dw may be null.
+hipError_t launch_add_norm_bwd(const AddNorm& n, const void* s, const void* w, const void* dy, const void* dsum, void* dx,
+                               void* dw, float* partial, hipStream_t stream);
+
+// Streams x [B * H][T][d] and gates z [B][T][H][d] by strides, y and the
+// gradients contiguous in z's (dx: x's) order.
+struct GateNorm {
+    int64_t B, T;
+    int H, d;
+    int64_t xn, xt, zb, zt, zh;  // strides in elements
+    int dtype, weight_dtype;
+    float eps;
+};
+constexpr int kGateNormMaxDim = 256;
+int64_t gate_norm_partial_floats(const GateNorm& n);
+hipError_t launch_gate_norm(const GateNorm& n, const void* x, const void* z, const void* w, void* y, hipStream_t stream);
+// dx, dz and dw may be null.
+hipError_t launch_gate_norm_bwd(const GateNorm& n, const void* x, const void* z, const void* w, const void* dy, void* dx,
+                                void* dz, void* dw, float* partial, hipStream_t stream);
+
 // ---- Algorithm 1 with the hashing inside (alg1.hip): bf16 q, k, v, out ----
 struct Alg1Args {
     const void* q;

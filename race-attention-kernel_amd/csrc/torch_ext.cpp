@@ -32,6 +32,8 @@
 //       (src/causal_v2/kernels/torch_binding.cpp:1-25)
 //   norm_rope / gated_scan / gated_scan_carry / cross / cross_state / cross_query:
 //       the operators beside the per-bucket op (torch_operators.h)
+//   add_norm / add_norm_e4m3 / gate_norm: the layer of the gated delta rule
+//       (torch_recurrent_layer.h)
 //
 // probsQ, probsK: [N, T, L, R] (or [N, T, S], read as L = 1, R = S) and V:
 // [N, T, d], all float32 or all bfloat16, on one HIP device, contiguous,
@@ -866,6 +868,7 @@ bool alg1_fits_on_device(int64_t head_dim, int64_t num_planes, int64_t num_table
 }  // namespace
 
 #include "torch_operators.h"
+#include "torch_recurrent_layer.h"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     namespace py = pybind11;
@@ -946,5 +949,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "True when an Algorithm-1 output-pass workgroup fits this GPU's LDS", py::arg("head_dim"), py::arg("num_planes"),
           py::arg("num_tables"), py::arg("tensor_cores") = false);
     bind_operators(m);
+    bind_recurrent_layer(m);
     m.def("abi_version", &race_abi_version, "ABI version of the loaded librace_mi355x");
 }
