@@ -656,6 +656,59 @@ race_status race_gated_scan_bwd(const void* x, const void* gate, const int32_t* 
                                 const race_scan_shape* shape, void* workspace, size_t workspace_bytes,
                                 hipStream_t stream);
 
+/* ---- The gated delta rule ------------------------------------------------
+ * A recurrence whose state is a matrix S [key_dim][value_dim] per value stream:
+ *     S_t = a_t S_{t-1} + beta_t k_t (v_t - a_t S_{t-1}^T k_t)^T,
+ *     out_t = scale * S_t^T q_t,
+ * a = exp(gate) or sigmoid(gate), or 1 without gates.  Each token corrects what the
+ * state answers to its key.  Value streams g n .. g n + g - 1 share key stream n,
+ * g = value_streams / key_streams.  No counterpart in the reference. */
+typedef struct race_delta_shape {
+    int64_t value_streams;  /* <= 65535, a multiple of key_streams */
+    int64_t key_streams;
+    int64_t seq_len;        /* value_streams * ceil(seq_len / 64) < 2^24 */
+    int32_t key_dim;        /* 1 .. 128 */
+    int32_t value_dim;      /* 1 .. 256 */
+    int32_t dtype;          /* race_dtype of q, k, v, out and their gradients */
+    int32_t gate_dtype;     /* race_dtype of gate and beta and their gradients */
+    int32_t gate_form;      /* race_gate; log gates are at most 0, those below -200 count as -200 */
+    int32_t lengths_group;  /* value streams that share one entry of `lengths`, >= 1 */
+    float scale;
+    /* Strides in elements, the values of a row next to each other; token strides up to 2^30. */
+    int64_t q_stream_stride, q_token_stride, k_stream_stride, k_token_stride, v_stream_stride, v_token_stride;
+} race_delta_shape;
+
+/* Calls without records of at most this many tokens go token by token in one
+ * launch and need no workspace. */
+#define RACE_DELTA_STEP_TOKENS 16
+
+/* Workspace of race_delta_fwd in bytes (0 with records), and the bytes of the
+ * records (nullable) race_delta_bwd reads. */
+race_status race_delta_fwd_workspace_bytes(const race_delta_shape* shape, size_t* bytes, size_t* record_bytes);
+
+/* out [value_streams][seq_len][value_dim] and, with final_state (nullable), the
+ * state after the last token.  gate (nullable) and beta: [value_streams][seq_len].
+ * state (nullable: zero) and final_state: [value_streams][key_dim][value_dim] fp32;
+ * they may be the same array.  lengths (nullable): int32, one per lengths_group
+ * value streams; tokens from lengths on are not read, their rows of out are zero
+ * and the state passes them (a value outside 0 .. seq_len counts as the nearer
+ * end).  Everything starts 16-byte aligned. */
+race_status race_delta_fwd(const void* q, const void* k, const void* v, const void* gate, const void* beta,
+                           const float* state, const int32_t* lengths, void* out, float* final_state, void* records,
+                           const race_delta_shape* shape, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+race_status race_delta_bwd_workspace_bytes(const race_delta_shape* shape, size_t* bytes);
+
+/* Gradients for the upstream gradients dout and dfinal (nullable: zero) of out and
+ * final_state, from the forward's q, k, gate, beta, lengths and records.  dq, dk
+ * [key_streams][seq_len][key_dim], dv [value_streams][seq_len][value_dim], dgate and
+ * dbeta (gate_dtype; zero, as dv, in the rows from lengths on) and dstate may each be
+ * NULL to skip it.  The shape's strides of v are not used. */
+race_status race_delta_bwd(const void* q, const void* k, const void* gate, const void* beta, const int32_t* lengths,
+                           const void* dout, const float* dfinal, const void* records, void* dq, void* dk, void* dv,
+                           void* dgate, void* dbeta, float* dstate, const race_delta_shape* shape, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+
 /* ---- Norms of whole rows around a recurrent layer -----------------------
  * In front of a layer's projections: the residual's addition and the norm of
  * the sum, s = x + residual, y = s / sqrt(mean(s^2) + eps) * weight, over rows

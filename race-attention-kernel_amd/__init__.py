@@ -7,6 +7,7 @@ through the _race_torch binding.  There is no CPU fallback.
 from . import causal_v2
 from .batched_ace import BatchedACE
 from .cross import CrossACE, race_cross_fwd, race_cross_query, race_cross_state
+from .delta import race_delta_rule, race_delta_rule_carry
 from .inputs import CONFIGS, Config, config_inputs, make_inputs
 from .norm import race_add_norm, race_add_norm_e4m3, race_gate_norm
 from .ops import (HashedRaceFunction, HashProbsFunction, RaceFusedFunction, hashed_supported,
@@ -24,5 +25,6 @@ __all__ = [
     "CrossACE", "race_cross_fwd", "race_cross_query", "race_cross_state",
     "race_norm_rope",
     "race_gated_scan", "race_gated_scan_carry",
+    "race_delta_rule", "race_delta_rule_carry",
     "race_add_norm", "race_add_norm_e4m3", "race_gate_norm",
 ]

@@ -80,6 +80,10 @@ EXPORTED_SYMBOLS = (
     "race_gated_scan_workspace_bytes",
     "race_gated_scan_fwd",
     "race_gated_scan_bwd",
+    "race_delta_fwd_workspace_bytes",
+    "race_delta_fwd",
+    "race_delta_bwd_workspace_bytes",
+    "race_delta_bwd",
     "race_add_norm_fwd",
     "race_add_norm_bwd_workspace_bytes",
     "race_add_norm_bwd",
@@ -124,6 +128,22 @@ class RaceCrossShape(ctypes.Structure):
         ("head_dim", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("lengths_group", ctypes.c_int32),
+    ]
+
+
+class RaceDeltaShape(ctypes.Structure):
+    _fields_ = [
+        ("value_streams", ctypes.c_int64),
+        ("key_streams", ctypes.c_int64),
+        ("seq_len", ctypes.c_int64),
+        ("key_dim", ctypes.c_int32),
+        ("value_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("gate_dtype", ctypes.c_int32),
+        ("gate_form", ctypes.c_int32),
+        ("lengths_group", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("strides", ctypes.c_int64 * 6),  # stream and token strides of q, k, v
     ]
 
 
@@ -262,6 +282,11 @@ def lib() -> ctypes.CDLL:
         L.race_gated_scan_workspace_bytes.argtypes = [sc, i32, ctypes.POINTER(sz), ctypes.POINTER(i64)]
         L.race_gated_scan_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
         L.race_gated_scan_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
+        dl = ctypes.POINTER(RaceDeltaShape)
+        L.race_delta_fwd_workspace_bytes.argtypes = [dl, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        L.race_delta_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, dl, vp, sz, vp]
+        L.race_delta_bwd_workspace_bytes.argtypes = [dl, ctypes.POINTER(sz)]
+        L.race_delta_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, dl, vp, sz, vp]
         an, gn = ctypes.POINTER(RaceAddNormShape), ctypes.POINTER(RaceGateNormShape)
         L.race_add_norm_fwd.argtypes = [vp, vp, vp, vp, vp, vp, an, vp]
         L.race_add_norm_bwd_workspace_bytes.argtypes = [an, ctypes.POINTER(sz)]
@@ -620,6 +645,43 @@ def cross_bwd(q: int, k: int, v: int, lengths: int | None, g: int, state: int, d
     """race_cross_bwd on raw device addresses; returns the status."""
     return lib().race_cross_bwd(q, k, v, lengths, g, state, dq, dk, dv, ctypes.byref(sh), workspace, workspace_bytes,
                                 stream)
+
+
+def delta_shape(N: int, T: int, dk: int, dv: int, *, key_streams: int | None = None, dtype: int = RACE_F32,
+                gate_dtype: int = RACE_F32, gate_form: int = RACE_GATE_LOG, lengths_group: int = 1,
+                scale: float = 1.0, strides=None) -> RaceDeltaShape:
+    """The shape of contiguous q, k [key_streams][T][dk] and v [N][T][dv]."""
+    return RaceDeltaShape(N, N if key_streams is None else key_streams, T, dk, dv, dtype, gate_dtype, gate_form, lengths_group,
+                          scale, (ctypes.c_int64 * 6)(*(strides or (T * dk, dk, T * dk, dk, T * dv, dv))))
+
+
+def delta_workspace_bytes(sh: RaceDeltaShape):
+    """(status, bytes, record_bytes) of race_delta_fwd."""
+    b, r = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    st = lib().race_delta_fwd_workspace_bytes(ctypes.byref(sh), ctypes.byref(b), ctypes.byref(r))
+    return st, b.value, r.value
+
+
+def delta_bwd_workspace_bytes(sh: RaceDeltaShape):
+    """(status, bytes)."""
+    b = ctypes.c_size_t(0)
+    return lib().race_delta_bwd_workspace_bytes(ctypes.byref(sh), ctypes.byref(b)), b.value
+
+
+def delta_fwd(q: int, k: int, v: int, gate: int | None, beta: int, state: int | None, lengths: int | None, out: int,
+              final_state: int | None, records: int | None, sh: RaceDeltaShape, workspace: int | None, workspace_bytes: int,
+              stream: int) -> int:
+    """race_delta_fwd on raw device addresses; returns the status."""
+    return lib().race_delta_fwd(q, k, v, gate, beta, state, lengths, out, final_state, records, ctypes.byref(sh), workspace,
+                                workspace_bytes, stream)
+
+
+def delta_bwd(q: int, k: int, gate: int | None, beta: int, lengths: int | None, dout: int, dfinal: int | None, records: int,
+              dq: int | None, dk: int | None, dv: int | None, dgate: int | None, dbeta: int | None, dstate: int | None,
+              sh: RaceDeltaShape, workspace: int | None, workspace_bytes: int, stream: int) -> int:
+    """race_delta_bwd on raw device addresses; returns the status."""
+    return lib().race_delta_bwd(q, k, gate, beta, lengths, dout, dfinal, records, dq, dk, dv, dgate, dbeta, dstate,
+                                ctypes.byref(sh), workspace, workspace_bytes, stream)
 
 
 def add_norm_shape(rows: int, D: int, *, dtype: int = RACE_F32, weight_dtype: int = RACE_F32, out: int = 0, group: int = 0,

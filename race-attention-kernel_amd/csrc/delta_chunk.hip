@@ -1,0 +1,515 @@
+// delta_chunk.hip -- the gated delta rule, forward: per stream a state S [dk][dv],
+//
+//     S_t = a_t S_{t-1} + b_t k_t (v_t - a_t S_{t-1}^T k_t)^T,   o_t = scale S_t^T q_t.
+//
+// In chunks of 64 tokens, from the state S before the chunk: with G_i the sum of
+// log a up to token i, E_i = e^{G_i}, Z_i = e^{G_last - G_i}, Gam_ij = e^{G_i - G_j},
+//
+//     N_ij = Gam_ij (k_i . k_j) b_j  (j < i),   T = (I + N)^-1,
+//     D = V - E K S,   Y = T D                      (the error each token writes),
+//     O = scale (E Q S + (Gam o Q K^T) b Y)         (j <= i),
+//     S <- e^{G_last} S + K^T (Z b Y).
+//
+// Two launches.  delta_solve_kernel, a workgroup per chunk, forms T and the
+// masked Gam o Q K^T b; all chunks at once.  delta_chunk_kernel walks a stream's
+// chunks in order, 16 columns of the state in a wave's registers: the columns of
+// S, D, Y and O do not mix, so its waves share the K, Q and T tiles in LDS and
+// nothing else, and every product takes its right operand from the accumulators
+// before it (delta_tiles.h).
+// Precision.  Sums are fp32.  fp32 rows run in fp32 products.  With bf16 rows the
+// state's own path (T, D, Y, the state's update) takes what is computed as bf16
+// hi + lo pairs, 16 bits, and the output's path takes M, S and Y rounded to bf16
+// once, as the output is: relative errors of at most 8e-6 of a state and of two to
+// three roundings of an output.  Log decays are summed in 64 bits: differences of
+// long sums lose the digits the products keep.
+// A few tokens (decode) go token by token in 32 bits: delta_step_kernel.
+#include "delta_tiles.h"
+
+namespace race {
+namespace {
+
+using namespace delta;
+using mfma::mfma4;
+
+// ---- T and the masked scores of a chunk ----
+
+constexpr int kSolvePitch = 68;
+constexpr int kSolveMatrix = kChunk * kSolvePitch * 4;
+
+template <typename TIn, int DK>
+constexpr int solve_lds_bytes() {
+    constexpr int tiles = 2 * Tile<TIn, DK>::kBytes;
+    return (tiles > kSolveMatrix ? tiles : kSolveMatrix) + kSolveMatrix;
+}
+
+// acc += X[r0 ..][c0 ..] B for 16 x 16 fp32 blocks, B in accumulator order.
+__device__ __forceinline__ f32x4 block_times(const float* x, int r0, int c0, int g, int lr, const f32x4& b, f32x4 acc) {
+    const float4 a = *reinterpret_cast<const float4*>(x + (r0 + lr) * kSolvePitch + c0 + 4 * g);
+    acc = mfma4(a.x, b[0], acc);
+    acc = mfma4(a.y, b[1], acc);
+    acc = mfma4(a.z, b[2], acc);
+    return mfma4(a.w, b[3], acc);
+}
+__device__ __forceinline__ f32x4 block_of(const float* x, int r0, int c0, int g, int lr) {
+    f32x4 v;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) v[s] = x[(r0 + 4 * g + s) * kSolvePitch + c0 + lr];
+    return v;
+}
+
+template <typename TIn, int DK>
+__global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ double G[kChunk];
+    __shared__ float b[kChunk];
+    using Rows = Tile<TIn, DK>;
+    unsigned char *kt = lds, *qt = lds + Rows::kBytes;
+    float* T = reinterpret_cast<float*>(lds);  // over the tiles, once they are read
+    float* Nm = reinterpret_cast<float*>(lds + solve_lds_bytes<TIn, DK>() - kSolveMatrix);
+    const int64_t nc = blockIdx.x, n = nc / a.chunks;
+    const int t0 = int(nc - n * a.chunks) * kChunk;
+    const int64_t len = a.live.of(n, a.T);
+    if (t0 >= len) return;
+    const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
+    const int64_t nk = n / a.group;
+    {
+        Stage<TIn, DK, kThreads> k, q;
+        k.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, live, a.dk, a.vec_k);
+        q.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, live, a.dk, a.vec_k);
+        if (wave == 0) {
+            const int64_t at = n * a.T + t0 + lane;
+            double s = lane < live && a.gate ? double(log_decay(gate_value(a.gate, at, a.gate_f32), a.form)) * kLog2e : 0.0;
+            for (int d = 1; d < 64; d <<= 1) {
+                const double o = __shfl_up(s, d);
+                if (lane >= d) s += o;
+            }
+            G[lane] = s;
+            const float bv = lane < live ? gate_value(a.beta, at, a.gate_f32) : 0.f;
+            b[lane] = bv;
+            const double last = __shfl(s, 63);
+            float* vec = a.vec + nc * 128;
+            vec[lane] = __builtin_amdgcn_exp2f(float(s));
+            vec[64 + lane] = __builtin_amdgcn_exp2f(float(last - s)) * bv;
+        }
+        k.put(kt);
+        q.put(qt);
+    }
+    __syncthreads();
+    {
+        // K K^T: row block `wave`, to N.
+        const int i = wave;
+        for (int j = 0; j <= i; ++j) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < DK / 32; ++s)
+                acc = mac(Rows::one(kt, 16 * i + lr, 4 * s + g), Rows::one(kt, 16 * j + lr, 4 * s + g), acc);
+            const int col = 16 * j + lr;
+            const double gc = G[col];
+            const float bc = b[col];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * i + 4 * g + r;
+                const float e = __builtin_amdgcn_exp2f(float(G[row] - gc));
+                Nm[row * kSolvePitch + col] = row > col ? e * acc[r] * bc : 0.f;
+            }
+        }
+        // Q K^T: row block 3 - wave (five blocks a wave in all), a token's columns in a lane.
+        const int o = 3 - wave;
+        TIn* mm = static_cast<TIn*>(a.mm) + nc * (kChunk * kChunk);
+        for (int j = 0; j <= (o | 1); ++j) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            if (j <= o) {
+#pragma unroll
+                for (int s = 0; s < DK / 32; ++s)
+                    acc = mac(Rows::one(kt, 16 * j + lr, 4 * s + g), Rows::one(qt, 16 * o + lr, 4 * s + g), acc);
+            }
+            const int row = 16 * o + lr, col = 16 * j + 4 * g;
+            const double gr = G[row];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(float(gr - G[col + r]));
+                acc[r] = row >= col + r ? a.scale * e * acc[r] * b[col + r] : 0.f;
+            }
+            store4_of(mm + row * kChunk + col, acc);
+        }
+    }
+    __syncthreads();
+    // (I + N)^-1: the diagonal blocks by substitution, a column a lane, ...
+    {
+        const int r0 = 16 * wave;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s = i == lr ? 1.f : 0.f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) s = fmaf(-Nm[(r0 + i) * kSolvePitch + r0 + j], x[j], s);
+            x[i] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((i & 3) == g) T[(r0 + i) * kSolvePitch + r0 + lr] = x[i];
+    }
+    __syncthreads();
+    // ... then [A 0; C B]^-1 = [A' 0; -B' C A'  B'], of 16 and of 32 rows.
+    if (wave < 2) {
+        const int r0 = 32 * wave;
+        f32x4 w = {0.f, 0.f, 0.f, 0.f}, z = w;
+        w = block_times(Nm, r0 + 16, r0, g, lr, block_of(T, r0, r0, g, lr), w);
+        z = block_times(T, r0 + 16, r0 + 16, g, lr, w, z);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) T[(r0 + 16 + 4 * g + r) * kSolvePitch + r0 + lr] = -z[r];
+    }
+    __syncthreads();
+    {
+        const int i = wave >> 1, j = wave & 1;
+        f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        f32x4 from[2];
+#pragma unroll
+        for (int l = 0; l < 2; ++l)
+            if (l >= j) from[l] = block_of(T, 16 * l, 16 * j, g, lr);
+        for (int k = 0; k <= i; ++k) {
+            f32x4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int l = 0; l < 2; ++l)
+                if (l >= j) w = block_times(Nm, 32 + 16 * k, 16 * l, g, lr, from[l], w);
+            z = block_times(T, 32 + 16 * i, 32 + 16 * k, g, lr, w, z);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) T[(32 + 16 * i + 4 * g + r) * kSolvePitch + 16 * j + lr] = -z[r];
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 2, c0 = (threadIdx.x & 3) * 16;
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = c0 + e <= row ? T[row * kSolvePitch + c0 + e] : 0.f;
+    TIn* tm = static_cast<TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk) + row * kChunk + c0;
+    if constexpr (sizeof(TIn) == 4) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) store4_of(tm + e, f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; e += 8) {
+            uint2 hi[2], lo[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                mfma::split4<true>(x[e + 4 * p], x[e + 4 * p + 1], x[e + 4 * p + 2], x[e + 4 * p + 3], hi[p], lo[p]);
+            *reinterpret_cast<uint4*>(tm + e) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+            *reinterpret_cast<uint4*>(tm + kChunk * kChunk + e) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
+        }
+    }
+}
+
+// ---- the walk over a stream's chunks ----
+
+template <typename TIn, int DK>
+__global__ __launch_bounds__(kThreads, 1) void delta_chunk_kernel(const DeltaArgs a) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    using L = ChunkLds<TIn, DK>;
+    using Rows = Tile<TIn, DK>;
+    using Square = Tile<TIn, 64>;
+    using One = OneT<TIn>;
+    using Two = TwoT<TIn>;
+    constexpr int NS = DK / 32;
+    int64_t n;
+    int cb;
+    if (!stream_and_block(a.N, (a.dv + 63) / 64, n, cb)) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
+    const bool odd = g & 1;
+    const int c0 = cb * 64 + wave * 16, col = c0 + lr;
+    const bool active = c0 < a.dv;
+    const int64_t nk = n / a.group, len = a.live.of(n, a.T);
+    const int chunks = int((len + kChunk - 1) / kChunk);
+    const TIn* kp = static_cast<const TIn*>(a.k) + nk * a.kn;
+    const TIn* qp = static_cast<const TIn*>(a.q) + nk * a.qn;
+    const TIn* vp = static_cast<const TIn*>(a.v) + n * a.vn + cb * 64;
+    TIn* op = static_cast<TIn*>(a.out) + n * a.T * a.dv;
+
+    f32x4 S[DK / 16];
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = tok(i, 4 * g + r);
+            S[i][r] = a.state && active && row < a.dk && col < a.dv ? a.state[(n * a.dk + row) * a.dv + col] : 0.f;
+        }
+
+    Stage<TIn, DK, kThreads> sk, sq;
+    StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;
+    StageDense<TIn, 64, kChunk, kThreads> smm;
+    Stage<TIn, 64, kThreads> sv;
+    float svec;
+    auto fetch = [&](int c) {
+        const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
+        const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
+        sk.load(kp + t0 * a.kt, a.kt, live, a.dk, a.vec_k);
+        sq.load(qp + t0 * a.qt, a.qt, live, a.dk, a.vec_k);
+        stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
+        smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
+        sv.load(vp + t0 * a.vt, a.vt, live, a.dv - cb * 64, a.vec_v);
+        if (threadIdx.x < 128) svec = a.vec[nc * 128 + threadIdx.x];
+    };
+    if (chunks > 0) fetch(0);
+    for (int c = 0; c < chunks; ++c) {
+        unsigned char* buf = lds + (L::kBuffers == 2 ? (c & 1) * L::kBytes : 0);
+        if (L::kBuffers == 1 && c > 0) __syncthreads();  // the chunk before is done with the buffer
+        sk.put(buf + L::kK);
+        sq.put(buf + L::kQ);
+        stm.put(buf + L::kT);
+        smm.put(buf + L::kM);
+        sv.put(buf + L::kV);
+        if (threadIdx.x < 128) reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x] = svec;
+        if (c + 1 < chunks) fetch(c + 1);
+        __syncthreads();
+        if (!active) continue;
+        const float* E = reinterpret_cast<const float*>(buf + L::kVec);
+        const int64_t nc = n * a.chunks + c;
+        Two s[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) operand(S[2 * i], S[2 * i + 1], odd, s[i]);
+        if (a.st) {
+            TIn* st = static_cast<TIn*>(a.st) + (nc * a.dvp + col) * DK + 8 * g;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first(s[i]));
+        }
+        // D = V - E K S.
+        f32x4 x[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NS; ++i) acc = mac(Rows::one(buf + L::kK, tok(b, lr), 4 * i + g), s[i], acc);
+            const f32x4 e = *reinterpret_cast<const f32x4*>(E + tok(b, 4 * g));
+            const f32x4 v = Square::block(buf + L::kV, b, 16 * wave, g, lr);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[b][r] = fmaf(-e[r], acc[r], v[r]);
+        }
+        Two d[2];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, d[kk]);
+        // Y = T D; T is lower triangular.
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk <= (b >> 1); ++kk) acc = mac(Square::two(buf + L::kT, tok(b, lr), 4 * kk + g), d[kk], acc);
+            x[b] = acc;
+        }
+        One y[2];
+        Two z[2];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[2 * kk + h] *= *reinterpret_cast<const f32x4*>(E + 64 + tok(2 * kk + h, 4 * g));
+            operand(x[2 * kk], x[2 * kk + 1], odd, z[kk]);
+        }
+        if (a.yt) {
+            TIn* yt = static_cast<TIn*>(a.yt) + (nc * a.dvp + col) * kChunk + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, y[kk]);
+        }
+        // O^T = scale S^T Q^T E + Y^T M^T: a token's columns in a lane.
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            const int row = tok(b, lr);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) acc = mac(delta::first(s[i]), Rows::one(buf + L::kQ, row, 4 * i + g), acc);
+            acc *= E[row] * a.scale;
+#pragma unroll
+            for (int kk = 0; kk <= (b >> 1); ++kk) acc = mac(y[kk], Square::one(buf + L::kM, row, 4 * kk + g), acc);
+            const int64_t t = int64_t(c) * kChunk + row;
+            if (t < len) {
+                TIn* o = op + t * a.dv + c0 + 4 * g;
+                const int there = a.dv - (c0 + 4 * g);
+                if (a.vec_o && there >= 4) {
+                    store4_of(o, acc);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (r < there) store_val(o + r, acc[r]);
+                }
+            }
+        }
+        // S = e^{G_last} S + K^T (Z b Y).
+        const float decay = E[63];
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) {
+            f32x4 acc = S[i] * decay;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) acc = mac(Rows::transposed(buf + L::kK, 32 * kk, i, g, lr), z[kk], acc);
+            S[i] = acc;
+        }
+    }
+    if (!active || col >= a.dv) return;
+    for (int64_t t = len + g; t < a.T; t += 4) store_val(op + t * a.dv + col, 0.f);
+    if (a.final_state) {
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = tok(i, 4 * g + r);
+                if (row < a.dk) a.final_state[(n * a.dk + row) * a.dv + col] = S[i][r];
+            }
+    }
+}
+
+// ---- token by token ----
+
+// V columns a thread and R rows, every eighth: a workgroup holds 32 V columns of a
+// stream's state, all rows.  final_state may be state.
+template <typename TIn, int V, int R>
+__global__ __launch_bounds__(kThreads) void delta_step_kernel(const DeltaArgs a) {
+    constexpr int CQ = 32, RG = kThreads / CQ;
+    __shared__ float ks[R * RG], qs[R * RG], sums[4][CQ][2 * V + 1];
+    const int64_t n = blockIdx.y, nk = n / a.group, len = a.live.of(n, a.T);
+    const int cl = threadIdx.x % CQ, rg = threadIdx.x / CQ, wave = threadIdx.x >> 6;
+    const int c = (blockIdx.x * CQ + cl) * V;
+    const bool in = c < a.dv;
+    float S[R][V];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int row = i * RG + rg;
+#pragma unroll
+        for (int j = 0; j < V; ++j) S[i][j] = 0.f;
+        if (!a.state || !in || row >= a.dk) continue;
+        const float* p = a.state + (n * a.dk + row) * a.dv + c;
+        if constexpr (V == 4) {
+            const float4 s = *reinterpret_cast<const float4*>(p);
+            S[i][0] = s.x, S[i][1] = s.y, S[i][2] = s.z, S[i][3] = s.w;
+        } else {
+            S[i][0] = *p;
+        }
+    }
+    TIn* op = static_cast<TIn*>(a.out) + n * a.T * a.dv + c;
+#pragma unroll 1
+    for (int64_t t = 0; t < len; ++t) {
+        for (int i = threadIdx.x; i < 2 * R * RG; i += kThreads) {
+            const bool key = i < R * RG;
+            const int row = key ? i : i - R * RG;
+            const TIn* p = key ? static_cast<const TIn*>(a.k) + nk * a.kn + t * a.kt : static_cast<const TIn*>(a.q) + nk * a.qn + t * a.qt;
+            (key ? ks : qs)[row] = row < a.dk ? to_f32(p[row]) : 0.f;
+        }
+        float v[V];
+        const TIn* vp = static_cast<const TIn*>(a.v) + n * a.vn + t * a.vt + c;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = in ? to_f32(vp[j]) : 0.f;
+        const float decay = a.gate ? expf(log_decay(gate_value(a.gate, n * a.T + t, a.gate_f32), a.form)) : 1.f;
+        const float b = gate_value(a.beta, n * a.T + t, a.gate_f32);
+        __syncthreads();
+        float sum[2 * V + 1];
+#pragma unroll
+        for (int j = 0; j < 2 * V + 1; ++j) sum[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const float k = ks[i * RG + rg], q = qs[i * RG + rg];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                sum[j] = fmaf(k, S[i][j], sum[j]);
+                sum[V + j] = fmaf(q, S[i][j], sum[V + j]);
+            }
+            sum[2 * V] = fmaf(k, q, sum[2 * V]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * V + 1; ++j) sum[j] += __shfl_xor(sum[j], 32);
+        if ((threadIdx.x & 32) == 0) {
+#pragma unroll
+            for (int j = 0; j < 2 * V + 1; ++j) sums[wave][cl][j] = sum[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2 * V + 1; ++j)
+            sum[j] = (sums[0][cl][j] + sums[1][cl][j]) + (sums[2][cl][j] + sums[3][cl][j]);
+        float e[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            e[j] = b * fmaf(-decay, sum[j], v[j]);
+            const float o = a.scale * fmaf(decay, sum[V + j], sum[2 * V] * e[j]);
+            if (in && rg == 0) store_val(op + t * a.dv + j, o);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const float k = ks[i * RG + rg];
+#pragma unroll
+            for (int j = 0; j < V; ++j) S[i][j] = fmaf(k, e[j], decay * S[i][j]);
+        }
+        __syncthreads();  // ks, qs and sums are free again
+    }
+    if (!in) return;
+    for (int64_t t = len + rg; t < a.T; t += RG)
+#pragma unroll
+        for (int j = 0; j < V; ++j) store_val(op + t * a.dv + j, 0.f);
+    if (!a.final_state) return;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int row = i * RG + rg;
+        if (row >= a.dk) continue;
+        float* p = a.final_state + (n * a.dk + row) * a.dv + c;
+        if constexpr (V == 4)
+            *reinterpret_cast<float4*>(p) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
+        else
+            *p = S[i][0];
+    }
+}
+
+template <typename TIn, int DK>
+hipError_t launch_chunks(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
+    using L = ChunkLds<TIn, DK>;
+    constexpr int solve = solve_lds_bytes<TIn, DK>(), walk = L::kBuffers * L::kBytes;
+    static_assert(solve <= kGfx950LdsBytes && walk <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
+    delta_solve_kernel<TIn, DK><<<unsigned(r.N * a.chunks), kThreads, solve, stream>>>(a);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    const int64_t blocks = (r.dv + 63) / 64;
+    delta_chunk_kernel<TIn, DK><<<unsigned((r.N + 7) / 8 * 8 * blocks), kThreads, walk, stream>>>(a);
+    return hipGetLastError();
+}
+
+template <typename TIn, int V>
+void launch_step(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
+    const dim3 grid(unsigned((r.dv + 32 * V - 1) / (32 * V)), unsigned(r.N));
+    if (r.dk <= 64)
+        delta_step_kernel<TIn, V, 8><<<grid, kThreads, 0, stream>>>(a);
+    else
+        delta_step_kernel<TIn, V, 16><<<grid, kThreads, 0, stream>>>(a);
+}
+
+}  // namespace
+
+int64_t delta_chunks(const DeltaRule& r) { return (r.T + kChunk - 1) / kChunk; }
+
+DeltaLayout delta_layout(const DeltaRule& r) {
+    const int64_t nc = r.N * delta_chunks(r), es = r.dtype == RACE_BF16 ? 2 : 4, dvp = (r.dv + 15) / 16 * 16;
+    DeltaLayout l;
+    l.mm = round256(nc * kChunk * kChunk * 4);
+    l.vec = l.mm + round256(nc * kChunk * kChunk * es);
+    l.solve_bytes = l.vec + round256(nc * 512);
+    l.yt = l.solve_bytes + round256(nc * dvp * dk_padded(r) * es);
+    l.record_bytes = l.yt + round256(nc * dvp * kChunk * es);
+    return l;
+}
+
+hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* state, void* out, float* final_state,
+                        void* scratch, bool records, hipStream_t stream) {
+    DeltaArgs a = delta_args(r, in);
+    a.state = state, a.out = out, a.final_state = final_state;
+    if (!records && r.T <= kDeltaStepTokens) {
+        const bool four = r.dv % 4 == 0;
+        if (r.dtype == RACE_BF16)
+            four ? launch_step<bf16_t, 4>(r, a, stream) : launch_step<bf16_t, 1>(r, a, stream);
+        else
+            four ? launch_step<float, 4>(r, a, stream) : launch_step<float, 1>(r, a, stream);
+        return hipGetLastError();
+    }
+    const DeltaLayout l = delta_layout(r);
+    unsigned char* base = static_cast<unsigned char*>(scratch);
+    a.tm = base, a.mm = base + l.mm;
+    a.vec = reinterpret_cast<float*>(base + l.vec);
+    if (records) a.st = base + l.solve_bytes, a.yt = base + l.yt;
+    if (r.dtype == RACE_BF16)
+        return r.dk <= 64 ? launch_chunks<bf16_t, 64>(r, a, stream) : launch_chunks<bf16_t, 128>(r, a, stream);
+    return r.dk <= 64 ? launch_chunks<float, 64>(r, a, stream) : launch_chunks<float, 128>(r, a, stream);
+}
+
+}  // namespace race

@@ -7,6 +7,7 @@
 // returned, hipErrorInvalidValue for anything the kernels do not support.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <initializer_list>
 #include <mutex>
@@ -2214,6 +2215,101 @@ race_status race_gate_norm_bwd(const void* x, const void* gate, const void* weig
                     workspace_bytes < size_t(gate_norm_partial_floats(n)) * sizeof(float)))
         return RACE_ERROR_INVALID_VALUE;
     return launch_gate_norm_bwd(n, x, gate, weight, dy, dx, dgate, dweight, static_cast<float*>(workspace), stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// The gated delta rule (delta_chunk.hip, delta_bwd.hip).
+
+namespace race {
+namespace {
+
+bool delta_shape(const race_delta_shape* sh, const int32_t* lengths, DeltaRule* r) {
+    if (!sh || sh->value_streams < 0 || sh->value_streams > kMaxStreams || sh->key_streams < 0) return false;
+    if (sh->key_streams > sh->value_streams) return false;
+    if (sh->key_streams == 0 ? sh->value_streams != 0 : sh->value_streams % sh->key_streams != 0) return false;
+    // A launch has one workgroup of 256 threads a chunk, and less than 2^32 threads.
+    if (sh->seq_len < 0 || sh->seq_len > (int64_t(1) << 30)) return false;
+    if (sh->value_streams * ((sh->seq_len + 63) / 64) >= (int64_t(1) << 24)) return false;
+    if (sh->key_dim < 1 || sh->key_dim > kDeltaMaxKeyDim || sh->value_dim < 1 || sh->value_dim > kDeltaMaxValueDim) return false;
+    if (!row_dtypes(sh->dtype, sh->gate_dtype)) return false;
+    if (sh->gate_form != RACE_GATE_SIGMOID && sh->gate_form != RACE_GATE_LOG) return false;
+    if (sh->lengths_group < 1 || !(sh->scale >= -FLT_MAX && sh->scale <= FLT_MAX)) return false;
+    for (int64_t s : {sh->q_stream_stride, sh->k_stream_stride, sh->v_stream_stride})
+        if (s < 0 || s > (int64_t(1) << 40)) return false;
+    for (int64_t s : {sh->q_token_stride, sh->k_token_stride, sh->v_token_stride})
+        if (s < 0 || s > (int64_t(1) << 30)) return false;
+    *r = DeltaRule{sh->value_streams,   sh->key_streams,    sh->seq_len,         sh->key_dim,        sh->value_dim,
+                   sh->q_stream_stride, sh->q_token_stride, sh->k_stream_stride, sh->k_token_stride, sh->v_stream_stride,
+                   sh->v_token_stride,  sh->dtype,          sh->gate_dtype,      sh->gate_form,      sh->scale,
+                   {lengths, sh->lengths_group}};
+    return true;
+}
+
+bool delta_step(const DeltaRule& r, const void* records) { return !records && r.T <= kDeltaStepTokens; }
+
+}  // namespace
+}  // namespace race
+
+extern "C" {
+
+race_status race_delta_fwd_workspace_bytes(const race_delta_shape* shape, size_t* bytes, size_t* record_bytes) {
+    DeltaRule r;
+    if (!delta_shape(shape, nullptr, &r) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    const DeltaLayout l = delta_layout(r);
+    *bytes = delta_step(r, nullptr) ? 0 : size_t(l.solve_bytes);
+    if (record_bytes) *record_bytes = size_t(l.record_bytes);
+    return RACE_SUCCESS;
+}
+
+race_status race_delta_fwd(const void* q, const void* k, const void* v, const void* gate, const void* beta,
+                           const float* state, const int32_t* lengths, void* out, float* final_state, void* records,
+                           const race_delta_shape* shape, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    DeltaRule r;
+    if (!delta_shape(shape, lengths, &r)) return RACE_ERROR_INVALID_VALUE;
+    if (!all_aligned16({state, final_state, records})) return RACE_ERROR_INVALID_VALUE;
+    if (r.N == 0) return RACE_SUCCESS;
+    const int64_t floats = r.N * r.dk * r.dv;
+    if (r.T == 0) {
+        if (!final_state || state == final_state) return RACE_SUCCESS;
+        if (!state) return zero_fill(final_state, floats, stream);
+        return copy_floats(state, final_state, floats, stream);
+    }
+    if (!q || !k || !v || !beta || !out || !all_aligned16({q, k, v, gate, beta, out})) return RACE_ERROR_INVALID_VALUE;
+    if (!records && !delta_step(r, records) &&
+        (!workspace || !aligned16(workspace) || workspace_bytes < size_t(delta_layout(r).solve_bytes)))
+        return RACE_ERROR_INVALID_VALUE;
+    return launch_delta(r, {q, k, v, gate, beta}, state, out, final_state, records ? records : workspace, records != nullptr,
+                        stream);
+}
+
+race_status race_delta_bwd_workspace_bytes(const race_delta_shape* shape, size_t* bytes) {
+    DeltaRule r;
+    if (!delta_shape(shape, nullptr, &r) || !bytes) return RACE_ERROR_INVALID_VALUE;
+    *bytes = size_t(delta_bwd_bytes(r));
+    return RACE_SUCCESS;
+}
+
+race_status race_delta_bwd(const void* q, const void* k, const void* gate, const void* beta, const int32_t* lengths,
+                           const void* dout, const float* dfinal, const void* records, void* dq, void* dk, void* dv,
+                           void* dgate, void* dbeta, float* dstate, const race_delta_shape* shape, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream) {
+    DeltaRule r;
+    if (!delta_shape(shape, lengths, &r)) return RACE_ERROR_INVALID_VALUE;
+    if (!all_aligned16({dfinal, records, dq, dk, dv, dgate, dbeta, dstate})) return RACE_ERROR_INVALID_VALUE;
+    if (dgate && !gate) return RACE_ERROR_INVALID_VALUE;
+    if (r.N == 0 || (!dq && !dk && !dv && !dgate && !dbeta && !dstate)) return RACE_SUCCESS;
+    const int64_t floats = r.N * r.dk * r.dv;
+    if (r.T == 0) {
+        if (!dstate || dstate == dfinal) return RACE_SUCCESS;
+        if (!dfinal) return zero_fill(dstate, floats, stream);
+        return copy_floats(dfinal, dstate, floats, stream);
+    }
+    if (!q || !k || !beta || !dout || !records || !all_aligned16({q, k, gate, beta, dout})) return RACE_ERROR_INVALID_VALUE;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < size_t(delta_bwd_bytes(r))) return RACE_ERROR_INVALID_VALUE;
+    return launch_delta_bwd(r, {q, k, nullptr, gate, beta}, dout, dfinal, records, {dq, dk, dv, dgate, dbeta, dstate},
+                            workspace, stream);
 }
 
 }  // extern "C"

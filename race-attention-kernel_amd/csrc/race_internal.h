@@ -483,6 +483,49 @@ hipError_t launch_gated_scan_bwd(const GatedScan& s, const void* x, const void* 
                                  const float* records, const float* dfinal, void* dx, void* dgate, float* dstate,
                                  float* pairs, hipStream_t stream);
 
+// ---- the gated delta rule (delta_chunk.hip, delta_bwd.hip) ----
+// q, k [Nk][T][dk] and v [N][T][dv] by strides, N a multiple of Nk (value streams
+// that share a key stream are consecutive), gates and strengths [N][T], out
+// contiguous, states [N][dk][dv] fp32.
+struct DeltaRule {
+    int64_t N, Nk, T;
+    int dk, dv;
+    int64_t qn, qt, kn, kt, vn, vt;  // strides in elements
+    int dtype, gate_dtype;           // race_dtype
+    int form;                        // race_gate
+    float scale;
+    Live live;
+};
+struct DeltaInputs {
+    const void *q, *k, *v, *gate, *beta;  // gate nullable: no decay
+};
+constexpr int kDeltaMaxKeyDim = 128, kDeltaMaxValueDim = 256;
+// Calls without records of at most this many tokens go token by token.
+constexpr int64_t kDeltaStepTokens = 16;
+int64_t delta_chunks(const DeltaRule& r);
+// Bytes from the start of the chunks' arrays: T and M of every chunk and its
+// decays (solve_bytes in all), then, in records only, the state before every
+// chunk and the errors its tokens write.
+struct DeltaLayout {
+    int64_t mm, vec, solve_bytes, yt, record_bytes;
+};
+DeltaLayout delta_layout(const DeltaRule& r);
+// scratch: record_bytes with records, solve_bytes without.  state and final_state
+// may be null, and may be the same.
+hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* state, void* out, float* final_state,
+                        void* scratch, bool records, hipStream_t stream);
+
+// Gradients for dout and dfinal (nullable: zero) from the forward's inputs and
+// records; any of the outputs may be null.  dq, dk [Nk][T][dk], dv [N][T][dv],
+// contiguous; dgate, dbeta [N][T] in gate_dtype.  scratch: delta_bwd_bytes.
+struct DeltaGrads {
+    void *dq, *dk, *dv, *dgate, *dbeta;
+    float* dstate;
+};
+int64_t delta_bwd_bytes(const DeltaRule& r);
+hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const void* dout, const float* dfinal,
+                            const void* records, const DeltaGrads& g, void* scratch, hipStream_t stream);
+
 // ---- norms of whole rows around a recurrent layer (row_norm.hip) ----
 // Rows [rows][D] by row strides; the residual's addition, the norm and, with
 // e4m3, its rows in 8 bits with a scale per `group` columns (0: per row).

@@ -32,8 +32,8 @@
 //       (src/causal_v2/kernels/torch_binding.cpp:1-25)
 //   norm_rope / gated_scan / gated_scan_carry / cross / cross_state / cross_query:
 //       the operators beside the per-bucket op (torch_operators.h)
-//   add_norm / add_norm_e4m3 / gate_norm: the layer of the gated delta rule
-//       (torch_recurrent_layer.h)
+//   delta_rule / delta_rule_carry / add_norm / add_norm_e4m3 / gate_norm: the layer
+//       of the gated delta rule (torch_recurrent_layer.h)
 //
 // probsQ, probsK: [N, T, L, R] (or [N, T, S], read as L = 1, R = S) and V:
 // [N, T, d], all float32 or all bfloat16, on one HIP device, contiguous,

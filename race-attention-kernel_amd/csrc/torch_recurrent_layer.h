@@ -1,5 +1,5 @@
 // torch_recurrent_layer.h -- the part of the PyTorch binding for the layer of the
-// gated delta rule: the norms around it; included by torch_ext.cpp after
+// gated delta rule: the recurrence and the norms around it; included by torch_ext.cpp after
 // torch_operators.h, whose helpers it uses.
 #pragma once
 
@@ -154,7 +154,182 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
     return {dx, dz, dw};
 }
 
+// ---- the gated delta rule ----
+
+int64_t token_width(const at::Tensor& t) { return t.dim() == 4 ? t.size(2) * t.size(3) : t.size(2); }
+
+race_delta_shape delta_shape(const char* entry, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                             const c10::optional<at::Tensor>& gate, const at::Tensor& beta,
+                             const c10::optional<at::Tensor>& state, const c10::optional<at::Tensor>& lengths, int64_t form,
+                             double scale) {
+    ArgCheck c(entry);
+    check_rows(c, "q", q, 3, "[N, T, dk]");
+    check_rows(c, "k", k, 3, "[N, T, dk]");
+    check_rows(c, "v", v, 3, "[N, T, dv]");
+    c.matches("k", k, "q", q).matches("v", v, "q", q)
+        .require(k.sizes() == q.sizes(), "k", [&] { return "has shape " + dims(k) + ", q " + dims(q); })
+        .raise();
+    const int64_t N = v.size(0), Nk = q.size(0), T = q.size(1), dk = q.size(2), dv = v.size(2);
+    c.require(v.size(1) == T, "v", [&] { return "has shape " + dims(v) + ", not q's " + std::to_string(T) + " tokens"; })
+        .require(Nk > 0 ? N >= Nk && N % Nk == 0 : N == 0, "v",
+                 [&] { return "has " + std::to_string(N) + " streams, no multiple of the " + std::to_string(Nk) + " key streams"; })
+        .require(dk >= 1 && dk <= 128 && dv >= 1 && dv <= 256, "q",
+                 [&] { return "and v have rows of " + std::to_string(dk) + " and " + std::to_string(dv) +
+                           " values; keys of 1 .. 128 and values of 1 .. 256 are taken"; })
+        .require(N <= 65535 && T <= (int64_t(1) << 30) && (N == 0 || (T + 63) / 64 <= ((int64_t(1) << 24) - 1) / N), "v",
+                 [&] { return "has shape " + dims(v) + "; up to 65535 streams and 2^30 tokens in all are taken"; });
+    auto per_token = [&](const char* name, const at::Tensor& t) {
+        c.on_gpu(name, t).dtype_is(name, t, true)
+            .require(t.device() == q.device() && t.sizes() == at::IntArrayRef({N, T}), name,
+                     [&] { return "has shape " + dims(t) + ", not v's [N, T] on its device"; })
+            .require(t.scalar_type() == at::kFloat || t.scalar_type() == q.scalar_type(), name, "is neither float32 nor of q's dtype");
+    };
+    per_token("beta", beta);
+    if (gate) {
+        per_token("gate", *gate);
+        c.require(gate->scalar_type() == beta.scalar_type(), "gate", "has another dtype than beta");
+    }
+    if (state)
+        c.on_gpu("state", *state)
+            .require(state->scalar_type() == at::kFloat && state->device() == q.device(), "state", "must be float32 on q's device")
+            .require(state->sizes() == at::IntArrayRef({N, dk, dv}), "state",
+                     [&] { return "has shape " + dims(*state) + ", not [N, dk, dv] of v's streams"; });
+    const int64_t group = check_lengths(c, lengths, q, N);
+    c.require(scale > -1e30 && scale < 1e30, "scale", "must be a finite number").raise();
+    auto stride = [](const at::Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; };
+    race_delta_shape sh{};
+    sh.value_streams = N, sh.key_streams = Nk, sh.seq_len = T;
+    sh.key_dim = static_cast<int32_t>(dk), sh.value_dim = static_cast<int32_t>(dv);
+    sh.dtype = dtype_of(q), sh.gate_dtype = dtype_of(beta), sh.gate_form = static_cast<int32_t>(form);
+    sh.lengths_group = static_cast<int32_t>(group), sh.scale = static_cast<float>(scale);
+    sh.q_stream_stride = stride(q, 0), sh.q_token_stride = stride(q, 1);
+    sh.k_stream_stride = stride(k, 0), sh.k_token_stride = stride(k, 1);
+    sh.v_stream_stride = stride(v, 0), sh.v_token_stride = stride(v, 1);
+    return sh;
+}
+
+constexpr int64_t kDeltaFar = int64_t(1) << 30;  // the largest token stride
+
+// q or k as rows [N, T, dk]: bucket probabilities [N, T, L, R] are rows of L R.
+at::Tensor as_key_rows(const at::Tensor& t) { return as_rows(t.dim() == 4 ? t.flatten(2) : t, kDeltaFar); }
+
+// Gates and strengths [N, T] are small: a copy where they are not dense.
+at::Tensor as_per_token(const at::Tensor& t) {
+    const at::Tensor d = t.contiguous();
+    return d.numel() > 0 && !starts_aligned(d) ? d.clone() : d;
+}
+c10::optional<at::Tensor> as_per_token(const c10::optional<at::Tensor>& t) {
+    if (!t) return c10::nullopt;
+    return as_per_token(*t);
+}
+
+// (out, final state, records or None).
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> delta_forward(
+    const char* entry, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& gate,
+    const at::Tensor& beta, const c10::optional<at::Tensor>& state, const c10::optional<at::Tensor>& lengths, int64_t form,
+    double scale, bool want_records, bool inplace) {
+    const race_delta_shape sh = delta_shape(entry, q, k, v, gate, beta, state, lengths, form, scale);
+    TORCH_CHECK(!inplace || state, entry, ": an in-place call needs a state");
+    TORCH_CHECK(!inplace || !(at::GradMode::is_enabled() && state->requires_grad()), entry,
+                ": a state that requires a gradient cannot be advanced in place");
+    const c10::DeviceGuard guard(q.device());
+    const at::Tensor out = at::empty(v.sizes(), v.options());
+    const at::Tensor fin = inplace ? *state
+                                   : at::empty({sh.value_streams, sh.key_dim, sh.value_dim}, v.options().dtype(at::kFloat));
+    size_t bytes = 0, record_bytes = 0;
+    check_status(race_delta_fwd_workspace_bytes(&sh, &bytes, &record_bytes), "race_delta_fwd_workspace_bytes");
+    c10::optional<at::Tensor> records;
+    at::Tensor ws;
+    if (want_records)
+        records = workspace_of(record_bytes, q), bytes = 0;
+    else if (bytes > 0)
+        ws = workspace_of(bytes, q);
+    if (inplace) state->unsafeGetTensorImpl()->bump_version();  // a graph that saved it must notice
+    check_status(race_delta_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), data_of(gate), beta.data_ptr(), floats_of(state),
+                                lengths_of(lengths), out.data_ptr(), fin.data_ptr<float>(), ptr_of(records), &sh,
+                                bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream()),
+                 "race_delta_fwd");
+    return {out, fin, records};
+}
+
+struct DeltaBackward {
+    c10::optional<at::Tensor> dq, dk, dv, dgate, dbeta, dstate;
+};
+
+// Gradients for those asked for, in the order q, k, v, gate, beta, state.
+DeltaBackward delta_backward(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& gate,
+                             const at::Tensor& beta, const c10::optional<at::Tensor>& lengths, const at::Tensor& dout,
+                             const c10::optional<at::Tensor>& dfinal, const at::Tensor& records, int64_t form, double scale,
+                             const std::vector<bool>& need) {
+    const char* entry = "race_delta_rule backward";
+    const race_delta_shape sh = delta_shape(entry, q, k, dout, gate, beta, dfinal, lengths, form, scale);
+    size_t bytes = 0, record_bytes = 0;
+    check_status(race_delta_fwd_workspace_bytes(&sh, &bytes, &record_bytes), "race_delta_fwd_workspace_bytes");
+    check_status(race_delta_bwd_workspace_bytes(&sh, &bytes), "race_delta_bwd_workspace_bytes");
+    ArgCheck(entry).on_gpu("dout", dout).on_gpu("records", records)
+        .require(records.scalar_type() == at::kFloat && records.device() == q.device() &&
+                     records.numel() == static_cast<int64_t>((record_bytes + 3) / 4),
+                 "records", "are not those of the forward of these inputs")
+        .raise();
+    const c10::DeviceGuard guard(q.device());
+    DeltaBackward g;
+    if (need[0]) g.dq = at::empty(q.sizes(), q.options());
+    if (need[1]) g.dk = at::empty(k.sizes(), k.options());
+    if (need[2]) g.dv = at::empty(dout.sizes(), dout.options());
+    if (need[3]) g.dgate = at::empty(beta.sizes(), beta.options());
+    if (need[4]) g.dbeta = at::empty(beta.sizes(), beta.options());
+    if (need[5]) g.dstate = at::empty({sh.value_streams, sh.key_dim, sh.value_dim}, q.options().dtype(at::kFloat));
+    const at::Tensor ws = workspace_of(bytes, q);
+    check_status(race_delta_bwd(q.data_ptr(), k.data_ptr(), data_of(gate), beta.data_ptr(), lengths_of(lengths),
+                                dout.data_ptr(), floats_of(dfinal), records.data_ptr(), ptr_of(g.dq), ptr_of(g.dk),
+                                ptr_of(g.dv), ptr_of(g.dgate), ptr_of(g.dbeta), floats_of(g.dstate), &sh, ws.data_ptr(), bytes,
+                                current_stream()),
+                 "race_delta_bwd");
+    return g;
+}
+
 // ---- the operators with their gradients ----
+
+struct DeltaHeld : torch::CustomClassHolder {
+    c10::optional<at::Tensor> lengths;
+    int64_t form;
+    double scale;
+    bool state;
+    std::vector<int64_t> v_sizes;
+};
+
+struct DeltaNode : torch::autograd::Function<DeltaNode> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                 const c10::optional<at::Tensor>& gate, const at::Tensor& beta,
+                                 const c10::optional<at::Tensor>& state, const c10::intrusive_ptr<DeltaHeld>& h) {
+        const auto [out, fin, records] = delta_forward("race_delta_rule", q, k, v, gate, beta, state, h->lengths, h->form,
+                                                       h->scale, true, false);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, or_undefined(gate), beta, or_undefined(h->lengths), *records});
+        h->lengths = c10::nullopt;
+        h->state = state.has_value();
+        h->v_sizes.assign(v.sizes().begin(), v.sizes().end());
+        ctx->saved_data["held"] = c10::IValue::make_capsule(h);
+        return {out, fin};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list up) {
+        variable_list grads(7);
+        const variable_list saved = ctx->get_saved_variables();
+        const DeltaHeld& h = held<DeltaHeld>(ctx);
+        const at::Tensor &q = saved[0], &k = saved[1], &beta = saved[3];
+        const auto gate = if_defined(saved[2]);
+        check_capture("race_delta_rule backward", {q, k, gate, beta});
+        if (up[0].defined() || up[1].defined()) {
+            const auto need = needed(ctx, {true, true, true, gate.has_value(), true, h.state});
+            const auto dout = dense_grad(up[0].defined() ? up[0] : at::zeros(h.v_sizes, q.options()), q.scalar_type());
+            const DeltaBackward g = delta_backward(q, k, gate, beta, if_defined(saved[4]), *dout, dense_grad(up[1], at::kFloat),
+                                                   saved[5], h.form, h.scale, need);
+            grads = {or_undefined(g.dq),    or_undefined(g.dk),    or_undefined(g.dv), or_undefined(g.dgate),
+                     or_undefined(g.dbeta), or_undefined(g.dstate), at::Tensor()};
+        }
+        return differentiated_once("race_delta_rule", up, std::move(grads));
+    }
+};
 
 struct AddNormNode : torch::autograd::Function<AddNormNode> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& residual,
@@ -271,8 +446,43 @@ at::Tensor gate_norm(const at::Tensor& x_in, const at::Tensor& gate_in, const c1
     return GateNormNode::apply(x, gate, weight, eps)[0];
 }
 
+std::tuple<at::Tensor, at::Tensor> delta_rule(const at::Tensor& q_in, const at::Tensor& k_in, const at::Tensor& v_in,
+                                              const c10::optional<at::Tensor>& gate_in, const at::Tensor& beta_in,
+                                              const c10::optional<at::Tensor>& state,
+                                              const c10::optional<at::Tensor>& lengths_in, int64_t form, double scale) {
+    const char* entry = "race_delta_rule";
+    const bool node = wants_grad({q_in, k_in, v_in, gate_in, beta_in, state});
+    if (node) check_capture(entry, {q_in, k_in, v_in, gate_in, beta_in, state});
+    const at::Tensor q = as_key_rows(q_in), k = as_key_rows(k_in), v = as_rows(v_in, kDeltaFar), beta = as_per_token(beta_in);
+    const auto gate = as_per_token(gate_in);
+    const auto lengths = as_lengths(lengths_in);
+    if (!node) {
+        const auto r = delta_forward(entry, q, k, v, gate, beta, state, lengths, form, scale, false, false);
+        return {std::get<0>(r), std::get<1>(r)};
+    }
+    auto h = c10::make_intrusive<DeltaHeld>();
+    h->lengths = lengths, h->form = form, h->scale = scale;
+    const variable_list outs = DeltaNode::apply(q, k, v, gate, beta, state, h);
+    return {outs[0], outs[1]};
+}
+
+std::tuple<at::Tensor, at::Tensor> delta_rule_carry(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const c10::optional<at::Tensor>& gate, const at::Tensor& beta,
+                                                    const at::Tensor& state, const c10::optional<at::Tensor>& lengths,
+                                                    int64_t form, double scale, bool inplace) {
+    const auto r = delta_forward("race_delta_rule_carry", as_key_rows(q), as_key_rows(k), as_rows(v, kDeltaFar),
+                                 as_per_token(gate), as_per_token(beta), state, as_lengths(lengths), form, scale, false, inplace);
+    return {std::get<0>(r), std::get<1>(r)};
+}
+
 void bind_recurrent_layer(pybind11::module& m) {
     namespace py = pybind11;
+    m.def("delta_rule", &delta_rule, "race_delta_rule with its gradients -> (out, final state)", py::arg("q"), py::arg("k"),
+          py::arg("v"), py::arg("gate"), py::arg("beta"), py::arg("state"), py::arg("lengths"), py::arg("form"),
+          py::arg("scale"));
+    m.def("delta_rule_carry", &delta_rule_carry, "race_delta_rule from a carried state -> (out, state)", py::arg("q"),
+          py::arg("k"), py::arg("v"), py::arg("gate"), py::arg("beta"), py::arg("state"), py::arg("lengths"), py::arg("form"),
+          py::arg("scale"), py::arg("inplace"));
     m.def("add_norm", &add_norm, "race_add_norm with its gradients -> (y, sum or None)", py::arg("x"), py::arg("residual"),
           py::arg("weight"), py::arg("eps"));
     m.def("add_norm_e4m3", &add_norm_e4m3, "race_add_norm with y in 8 bits -> (y, scales, sum or None)", py::arg("x"),
