@@ -41,8 +41,8 @@ struct DeltaBwdArgs {
 
 // ---- the walk ----
 
-template <typename TIn, int DK>
-__global__ __launch_bounds__(kThreads, 1) void delta_bwd_walk_kernel(const DeltaBwdArgs w) {
+template <typename TIn, int DK, bool kVec>
+__global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwdArgs w) {
     extern __shared__ __align__(16) unsigned char lds[];
     const DeltaArgs& a = w.f;
     using L = ChunkLds<TIn, DK>;  // dO in the place of V
@@ -73,21 +73,27 @@ __global__ __launch_bounds__(kThreads, 1) void delta_bwd_walk_kernel(const Delta
             dS[i][r] = w.dfinal && active && row < a.dk && col < a.dv ? w.dfinal[(n * a.dk + row) * a.dv + col] : 0.f;
         }
 
-    Stage<TIn, DK, kThreads> sk, sq;
+    Stage<TIn, DK, kThreads, kVec> sk, sq;
     StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;
     StageDense<TIn, 64, kChunk, kThreads> smm;
-    Stage<TIn, 64, kThreads> so;
+    Stage<TIn, 64, kThreads, kVec> so;
     float svec;
+    sk.init(a.kt, a.dk);
+    sq.init(a.qt, a.dk);
+    so.init(a.dv, a.dv - cb * 64);
     auto fetch = [&](int c) {
         const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
-        sk.load(kp + t0 * a.kt, a.kt, live, a.dk, a.vec_k);
-        sq.load(qp + t0 * a.qt, a.qt, live, a.dk, a.vec_k);
+        sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
+        sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
         stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
         smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
-        so.load(op + t0 * a.dv, a.dv, live, a.dv - cb * 64, a.vec_o8);
-        if (threadIdx.x < 128) svec = a.vec[nc * 128 + threadIdx.x];
+        so.load(op + t0 * a.dv, a.dv, live, a.dv - cb * 64);
+        svec = a.vec[nc * 128 + (threadIdx.x & 127)];
     };
+    // What a lane adds to a tile's start.
+    const int k_row = Rows::row_base(lr, g), k_col = Rows::column_base(lr, g), s_col = Square::column_base(lr, g);
+    const int o_at = Square::block_base(16 * wave, lr, g);
     if (chunks > 0) fetch(chunks - 1);
     for (int c = chunks - 1; c >= 0; --c) {
         unsigned char* buf = lds + (L::kBuffers == 2 ? (c & 1) * L::kBytes : 0);
@@ -97,7 +103,7 @@ __global__ __launch_bounds__(kThreads, 1) void delta_bwd_walk_kernel(const Delta
         stm.put(buf + L::kT);
         smm.put(buf + L::kM);
         so.put(buf + L::kV);
-        if (threadIdx.x < 128) reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x] = svec;
+        reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
         if (c > 0) fetch(c - 1);
         __syncthreads();
         if (!active) continue;
@@ -116,7 +122,7 @@ __global__ __launch_bounds__(kThreads, 1) void delta_bwd_walk_kernel(const Delta
         for (int kk = 0; kk < 2; ++kk) {
             f32x4 x[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) x[h] = Square::block(buf + L::kV, 2 * kk + h, 16 * wave, g, lr);
+            for (int h = 0; h < 2; ++h) x[h] = Square::block(buf + L::kV, o_at, 2 * kk + h);
             operand(x[0], x[1], odd, o[kk]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) x[h] *= *reinterpret_cast<const f32x4*>(E + tok(2 * kk + h, 4 * g)) * a.scale;
@@ -125,26 +131,26 @@ __global__ __launch_bounds__(kThreads, 1) void delta_bwd_walk_kernel(const Delta
         // dY = M^T dO + Z b (K dS').
         f32x4 x[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < 4; ++b) x[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < NS; ++i) acc = mac(Rows::one(buf + L::kK, tok(b, lr), 4 * i + g), s[i], acc);
-            acc *= *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
+        for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int kk = b >> 1; kk < 2; ++kk) acc = mac(Square::transposed(buf + L::kM, 32 * kk, b, g, lr), o[kk], acc);
-            x[b] = acc;
-        }
+            for (int b = 0; b < 4; ++b) x[b] = mac(Rows::one(buf + L::kK, k_row, b, i), s[i], x[b]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] *= *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = mac(Square::transposed(buf + L::kM, s_col, 1, b), o[1], x[b]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) x[b] = mac(Square::transposed(buf + L::kM, s_col, 0, b), o[0], x[b]);
         Two y[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
         // dD = T^T dY.
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < 4; ++b)
+            x[b] = mac(Square::transposed_two(buf + L::kT, s_col, 1, b), y[1], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int kk = b >> 1; kk < 2; ++kk) acc = mac(Square::transposed_two(buf + L::kT, 32 * kk, b, g, lr), y[kk], acc);
-            x[b] = acc;
-        }
+        for (int b = 0; b < 2; ++b) x[b] = mac(Square::transposed_two(buf + L::kT, s_col, 0, b), y[0], x[b]);
         Two d[2];
         TIn* dd = static_cast<TIn*>(w.dd) + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
@@ -159,15 +165,14 @@ __global__ __launch_bounds__(kThreads, 1) void delta_bwd_walk_kernel(const Delta
         // dS = e^{G_last} dS' + scale Q^T (E dO) - K^T (E dD).
         const float decay = E[63];
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i) {
-            f32x4 acc = dS[i] * decay;
+        for (int i = 0; i < DK / 16; ++i) dS[i] *= decay;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                acc = mac(Rows::transposed(buf + L::kQ, 32 * kk, i, g, lr), eo[kk], acc);
-                acc = mac(Rows::transposed(buf + L::kK, 32 * kk, i, g, lr), d[kk], acc);
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) {
+                dS[i] = mac(Rows::transposed(buf + L::kQ, k_col, kk, i), eo[kk], dS[i]);
+                dS[i] = mac(Rows::transposed(buf + L::kK, k_col, kk, i), d[kk], dS[i]);
             }
-            dS[i] = acc;
-        }
     }
     if (!w.dstate || !active || col >= a.dv) return;
 #pragma unroll
@@ -228,8 +233,8 @@ __device__ __forceinline__ void store_gate(void* p, int64_t i, int f32, float x)
 
 // A chunk of a key stream: eight waves, wave (th, dq) of 32 tokens and a quarter of
 // the key columns; of the 64 x 64 matrices 32 rows and 16 columns.
-template <typename TIn, int DK>
-__global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const DeltaBwdArgs w) {
+template <typename TIn, int DK, bool kVec>
+__global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBwdArgs w) {
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ double G[kChunk];
     __shared__ float beta[kChunk];
@@ -252,12 +257,16 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
         most = max(most, int(l < kChunk ? l : kChunk));
     }
     if (most > 0) {
-        Stage<TIn, DK, kGradThreads> sk, sq;
-        sk.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, most, a.dk, a.vec_k);
-        sq.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, most, a.dk, a.vec_k);
+        Stage<TIn, DK, kGradThreads, kVec> sk, sq;
+        sk.init(a.kt, a.dk);
+        sq.init(a.qt, a.dk);
+        sk.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, most, a.dk);
+        sq.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, most, a.dk);
         sk.put(lds + L::kK);
         sq.put(lds + L::kQ);
     }
+    const int k_col = Rows::column_base(lr, g), s_col = Square::column_base(lr, g), o_row = Out::row_base(lr, g);
+    const int k_row = Rows::row_base(lr, g), s_row = Square::row_base(lr, g);
     f32x4 gq[2][NB], gk[2][NB];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -318,12 +327,19 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
             {
                 const TIn* p = static_cast<const TIn*>(w.dout) + (n * a.T + t0) * a.dv + v0;
                 constexpr int kEights = SL / 8, kVecs = Eight<TIn>::kVecs;
+                const auto view = mfma::make_rsrc(p, ((live - 1) * int64_t(a.dv) + a.dv - v0) * int(sizeof(TIn)));
 #pragma unroll
                 for (int i = 0; i < (kChunk * kEights + kGradThreads - 1) / kGradThreads; ++i) {
                     const int q = int(threadIdx.x) + i * kGradThreads, row = q / kEights, u = q % kEights;
                     if (kChunk * kEights < kGradThreads && q >= kChunk * kEights) break;
                     Eight<TIn> x;
-                    x.load(p + row * a.dv + 8 * u, row < live ? a.dv - v0 - 8 * u : 0, a.vec_o8);
+                    if constexpr (kVec) {
+#pragma unroll
+                        for (int j = 0; j < kVecs; ++j)
+                            x.v[j] = mfma::buf_load16<mfma::kPolicyDefault>(view, piece_at<TIn>(row, a.dv, 8 * u + 4 * j, a.dv - v0));
+                    } else {
+                        x.load(p + row * a.dv + 8 * u, row < live ? a.dv - v0 - 8 * u : 0);
+                    }
 #pragma unroll
                     for (int j = 0; j < kVecs; ++j)
                         *reinterpret_cast<uint4*>(lds + L::kO + Out::at(row, kVecs * u + j)) = x.v[j];
@@ -332,21 +348,21 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
             __syncthreads();
 #pragma unroll
             for (int kk = 0; kk < SL / 32; ++kk) {
-                const One yc = Square::transposed(lds + L::kYt, 32 * kk, dq, g, lr);
+                const One yc = Square::transposed(lds + L::kYt, s_col, kk, dq);
                 One ya[2], da[2], oa[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int b = 2 * th + i;
-                    ya[i] = Square::transposed(lds + L::kYt, 32 * kk, b, g, lr);
-                    da[i] = Square::transposed(lds + L::kDd, 32 * kk, b, g, lr);
-                    oa[i] = Out::one(lds + L::kO, tok(b, lr), 4 * kk + g);
+                    ya[i] = Square::transposed(lds + L::kYt, s_col, kk, b);
+                    da[i] = Square::transposed(lds + L::kDd, s_col, kk, b);
+                    oa[i] = Out::one(lds + L::kO, o_row, b, kk);
                     P[i] = mac(oa[i], yc, P[i]);
                     H[i] = mac(da[i], yc, H[i]);
                     // A token's dV: these waves hold the same rows, each writes every fourth run.
                     if (dv && ((v0 >> 5) + kk) % 4 == dq && tok(b, lr) < here) {
                         const int cv = v0 + 32 * kk + 8 * g;
                         TIn* o = dv + int64_t(tok(b, lr)) * a.dv + cv;
-                        if (a.vec_o8 && cv + 8 <= a.dv) {
+                        if (kVec && cv + 8 <= a.dv) {
                             store_run(o, da[i]);
                         } else {
                             const auto run = __builtin_bit_cast(Eight<TIn>, da[i]);
@@ -360,8 +376,8 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    const One st = Rows::transposed(lds + L::kSt, 32 * kk, dq * NB + b, g, lr);
-                    const One ds = Rows::transposed(lds + L::kDs, 32 * kk, dq * NB + b, g, lr);
+                    const One st = Rows::transposed(lds + L::kSt, k_col, kk, dq * NB + b);
+                    const One ds = Rows::transposed(lds + L::kDs, k_col, kk, dq * NB + b);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         qs[i][b] = mac(st, oa[i], qs[i][b]);
@@ -382,10 +398,9 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
             f32x4 qk = {0.f, 0.f, 0.f, 0.f}, kk = qk;
 #pragma unroll
             for (int s = 0; s < DK / 32; ++s) {
-                const int row = tok(2 * th + i, lr), u = 4 * s + g;
-                const One kj = Rows::one(lds + L::kK, jc, u);
-                qk = mac(Rows::one(lds + L::kQ, row, u), kj, qk);
-                kk = mac(Rows::one(lds + L::kK, row, u), kj, kk);
+                const One kj = Rows::one(lds + L::kK, k_row, dq, s);
+                qk = mac(Rows::one(lds + L::kQ, k_row, 2 * th + i, s), kj, qk);
+                kk = mac(Rows::one(lds + L::kK, k_row, 2 * th + i, s), kj, kk);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -425,7 +440,8 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int cd = tok(dq * NB + b, 4 * g);
-                const f32x4 q4 = Rows::four(lds + L::kQ, row, cd), k4 = Rows::four(lds + L::kK, row, cd);
+                const int at = Rows::four_at(row, cd);
+                const f32x4 q4 = Rows::four(lds + L::kQ, at), k4 = Rows::four(lds + L::kK, at);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float qv = qs[i][b][r] * (e * a.scale), fv = fs[i][b][r] * e, zv = zs[i][b][r] * z;
@@ -446,8 +462,9 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
         __syncthreads();  // the slices of S and dS' are read
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            Square::put4(lds + L::kL, jc, tok(2 * th + i, 4 * g), Lm[i]);
-            Square::put4(lds + L::kX, jc, tok(2 * th + i, 4 * g), Xm[i]);
+            const int at = Square::four_at(jc, tok(2 * th + i, 4 * g));
+            Square::put4(lds + L::kL, at, Lm[i]);
+            Square::put4(lds + L::kX, at, Xm[i]);
         }
         __syncthreads();
         if (wave == 0 && (w.dgate || w.dbeta)) {
@@ -489,23 +506,23 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
                 const int b = 2 * th + i;
                 One l, lt, x, xt;
                 if (kk <= th) {
-                    l = Square::transposed(lds + L::kL, 32 * kk, b, g, lr);
-                    x = Square::transposed(lds + L::kX, 32 * kk, b, g, lr);
+                    l = Square::transposed(lds + L::kL, s_col, kk, b);
+                    x = Square::transposed(lds + L::kX, s_col, kk, b);
                 }
                 if (kk >= th) {
-                    lt = Square::one(lds + L::kL, tok(b, lr), 4 * kk + g);
-                    xt = Square::one(lds + L::kX, tok(b, lr), 4 * kk + g);
+                    lt = Square::one(lds + L::kL, s_row, b, kk);
+                    xt = Square::one(lds + L::kX, s_row, b, kk);
                 }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    const One kf = Rows::transposed(lds + L::kK, 32 * kk, dq * NB + nb, g, lr);
+                    const One kf = Rows::transposed(lds + L::kK, k_col, kk, dq * NB + nb);
                     if (kk <= th) {
                         gq[i][nb] = mac(kf, l, gq[i][nb]);
                         gk[i][nb] = mac(kf, x, gk[i][nb]);
                     }
                     if (kk >= th) {
                         gk[i][nb] = mac(kf, xt, gk[i][nb]);
-                        gk[i][nb] = mac(Rows::transposed(lds + L::kQ, 32 * kk, dq * NB + nb, g, lr), lt, gk[i][nb]);
+                        gk[i][nb] = mac(Rows::transposed(lds + L::kQ, k_col, kk, dq * NB + nb), lt, gk[i][nb]);
                     }
                 }
             }
@@ -536,18 +553,23 @@ __global__ __launch_bounds__(kGradThreads, 1) void delta_grads_kernel(const Delt
     }
 }
 
-template <typename TIn, int DK>
+template <typename TIn, int DK, bool kVec>
 hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
     using L = ChunkLds<TIn, DK>;
     constexpr int walk = L::kBuffers * L::kBytes, grads = GradLds<TIn, DK>::kBytes;
     static_assert(walk <= kGfx950LdsBytes && grads + 8192 <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
     const int64_t blocks = (r.dv + 63) / 64;
-    delta_bwd_walk_kernel<TIn, DK><<<unsigned((r.N + 7) / 8 * 8 * blocks), kThreads, walk, stream>>>(w);
+    delta_bwd_walk_kernel<TIn, DK, kVec><<<unsigned((r.N + 7) / 8 * 8 * blocks), kThreads, walk, stream>>>(w);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (!w.dq && !w.dk && !w.dv && !w.dgate && !w.dbeta) return hipSuccess;
-    delta_grads_kernel<TIn, DK><<<unsigned(r.Nk * w.f.chunks), kGradThreads, grads, stream>>>(w);
+    delta_grads_kernel<TIn, DK, kVec><<<unsigned(r.Nk * w.f.chunks), kGradThreads, grads, stream>>>(w);
     return hipGetLastError();
+}
+
+template <typename TIn, bool kVec>
+hipError_t launch_by_width(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
+    return r.dk <= 64 ? launch_backward<TIn, 64, kVec>(r, w, stream) : launch_backward<TIn, 128, kVec>(r, w, stream);
 }
 
 }  // namespace
@@ -570,9 +592,10 @@ hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const voi
     w.ds = scratch;
     w.dd = static_cast<unsigned char*>(scratch) + round256(r.N * w.f.chunks * w.f.dvp * dk_padded(r) * es);
     w.dq = g.dq, w.dk = g.dk, w.dv = g.dv, w.dgate = g.dgate, w.dbeta = g.dbeta, w.dstate = g.dstate;
+    const bool vec = w.f.vec_k && w.f.vec_o;
     if (r.dtype == RACE_BF16)
-        return r.dk <= 64 ? launch_backward<bf16_t, 64>(r, w, stream) : launch_backward<bf16_t, 128>(r, w, stream);
-    return r.dk <= 64 ? launch_backward<float, 64>(r, w, stream) : launch_backward<float, 128>(r, w, stream);
+        return vec ? launch_by_width<bf16_t, true>(r, w, stream) : launch_by_width<bf16_t, false>(r, w, stream);
+    return vec ? launch_by_width<float, true>(r, w, stream) : launch_by_width<float, false>(r, w, stream);
 }
 
 }  // namespace race

@@ -57,7 +57,7 @@ __device__ __forceinline__ f32x4 block_of(const float* x, int r0, int c0, int g,
     return v;
 }
 
-template <typename TIn, int DK>
+template <typename TIn, int DK, bool kVec>
 __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a) {
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ double G[kChunk];
@@ -73,10 +73,13 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
     const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
     const int64_t nk = n / a.group;
+    auto row_of = [&](const unsigned char* t, int row, int s) { return Rows::load(t, Rows::run_at(row, 4 * s + g)); };
     {
-        Stage<TIn, DK, kThreads> k, q;
-        k.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, live, a.dk, a.vec_k);
-        q.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, live, a.dk, a.vec_k);
+        Stage<TIn, DK, kThreads, kVec> k, q;
+        k.init(a.kt, a.dk);
+        q.init(a.qt, a.dk);
+        k.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, live, a.dk);
+        q.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, live, a.dk);
         if (wave == 0) {
             const int64_t at = n * a.T + t0 + lane;
             double s = lane < live && a.gate ? double(log_decay(gate_value(a.gate, at, a.gate_f32), a.form)) * kLog2e : 0.0;
@@ -103,7 +106,7 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < DK / 32; ++s)
-                acc = mac(Rows::one(kt, 16 * i + lr, 4 * s + g), Rows::one(kt, 16 * j + lr, 4 * s + g), acc);
+                acc = mac(row_of(kt, 16 * i + lr, s), row_of(kt, 16 * j + lr, s), acc);
             const int col = 16 * j + lr;
             const double gc = G[col];
             const float bc = b[col];
@@ -122,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
             if (j <= o) {
 #pragma unroll
                 for (int s = 0; s < DK / 32; ++s)
-                    acc = mac(Rows::one(kt, 16 * j + lr, 4 * s + g), Rows::one(qt, 16 * o + lr, 4 * s + g), acc);
+                    acc = mac(row_of(kt, 16 * j + lr, s), row_of(qt, 16 * o + lr, s), acc);
             }
             const int row = 16 * o + lr, col = 16 * j + 4 * g;
             const double gr = G[row];
@@ -202,13 +205,12 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
 
 // ---- the walk over a stream's chunks ----
 
-template <typename TIn, int DK>
-__global__ __launch_bounds__(kThreads, 1) void delta_chunk_kernel(const DeltaArgs a) {
+template <typename TIn, int DK, bool kVec, bool kRecords>
+__global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a) {
     extern __shared__ __align__(16) unsigned char lds[];
     using L = ChunkLds<TIn, DK>;
     using Rows = Tile<TIn, DK>;
     using Square = Tile<TIn, 64>;
-    using One = OneT<TIn>;
     using Two = TwoT<TIn>;
     constexpr int NS = DK / 32;
     int64_t n;
@@ -234,21 +236,27 @@ __global__ __launch_bounds__(kThreads, 1) void delta_chunk_kernel(const DeltaArg
             S[i][r] = a.state && active && row < a.dk && col < a.dv ? a.state[(n * a.dk + row) * a.dv + col] : 0.f;
         }
 
-    Stage<TIn, DK, kThreads> sk, sq;
+    Stage<TIn, DK, kThreads, kVec> sk, sq;
     StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;
     StageDense<TIn, 64, kChunk, kThreads> smm;
-    Stage<TIn, 64, kThreads> sv;
+    Stage<TIn, 64, kThreads, kVec> sv;
     float svec;
+    sk.init(a.kt, a.dk);
+    sq.init(a.qt, a.dk);
+    sv.init(a.vt, a.dv - cb * 64);
     auto fetch = [&](int c) {
         const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
-        sk.load(kp + t0 * a.kt, a.kt, live, a.dk, a.vec_k);
-        sq.load(qp + t0 * a.qt, a.qt, live, a.dk, a.vec_k);
+        sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
+        sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
         stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
         smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
-        sv.load(vp + t0 * a.vt, a.vt, live, a.dv - cb * 64, a.vec_v);
-        if (threadIdx.x < 128) svec = a.vec[nc * 128 + threadIdx.x];
+        sv.load(vp + t0 * a.vt, a.vt, live, a.dv - cb * 64);
+        svec = a.vec[nc * 128 + (threadIdx.x & 127)];
     };
+    // What a lane adds to a tile's start.
+    const int k_row = Rows::row_base(lr, g), k_col = Rows::column_base(lr, g), s_row = Square::row_base(lr, g);
+    const int v_at = Square::block_base(16 * wave, lr, g);
     if (chunks > 0) fetch(0);
     for (int c = 0; c < chunks; ++c) {
         unsigned char* buf = lds + (L::kBuffers == 2 ? (c & 1) * L::kBytes : 0);
@@ -258,7 +266,7 @@ __global__ __launch_bounds__(kThreads, 1) void delta_chunk_kernel(const DeltaArg
         stm.put(buf + L::kT);
         smm.put(buf + L::kM);
         sv.put(buf + L::kV);
-        if (threadIdx.x < 128) reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x] = svec;
+        reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
         if (c + 1 < chunks) fetch(c + 1);
         __syncthreads();
         if (!active) continue;
@@ -267,7 +275,7 @@ __global__ __launch_bounds__(kThreads, 1) void delta_chunk_kernel(const DeltaArg
         Two s[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) operand(S[2 * i], S[2 * i + 1], odd, s[i]);
-        if (a.st) {
+        if constexpr (kRecords) {
             TIn* st = static_cast<TIn*>(a.st) + (nc * a.dvp + col) * DK + 8 * g;
 #pragma unroll
             for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first(s[i]));
@@ -275,28 +283,27 @@ __global__ __launch_bounds__(kThreads, 1) void delta_chunk_kernel(const DeltaArg
         // D = V - E K S.
         f32x4 x[4];
 #pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) x[b] = mac(Rows::one(buf + L::kK, k_row, b, i), s[i], x[b]);
+#pragma unroll
         for (int b = 0; b < 4; ++b) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < NS; ++i) acc = mac(Rows::one(buf + L::kK, tok(b, lr), 4 * i + g), s[i], acc);
             const f32x4 e = *reinterpret_cast<const f32x4*>(E + tok(b, 4 * g));
-            const f32x4 v = Square::block(buf + L::kV, b, 16 * wave, g, lr);
+            const f32x4 v = Square::block(buf + L::kV, v_at, b);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[b][r] = fmaf(-e[r], acc[r], v[r]);
+            for (int r = 0; r < 4; ++r) x[b][r] = fmaf(-e[r], x[b][r], v[r]);
         }
         Two d[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, d[kk]);
         // Y = T D; T is lower triangular.
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < 4; ++b) x[b] = mac(Square::two(buf + L::kT, s_row, b, 0), d[0], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int kk = 0; kk <= (b >> 1); ++kk) acc = mac(Square::two(buf + L::kT, tok(b, lr), 4 * kk + g), d[kk], acc);
-            x[b] = acc;
-        }
-        One y[2];
-        Two z[2];
+        for (int b = 2; b < 4; ++b) x[b] = mac(Square::two(buf + L::kT, s_row, b, 1), d[1], x[b]);
+        Two y[2], z[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
@@ -304,42 +311,52 @@ __global__ __launch_bounds__(kThreads, 1) void delta_chunk_kernel(const DeltaArg
             for (int h = 0; h < 2; ++h) x[2 * kk + h] *= *reinterpret_cast<const f32x4*>(E + 64 + tok(2 * kk + h, 4 * g));
             operand(x[2 * kk], x[2 * kk + 1], odd, z[kk]);
         }
-        if (a.yt) {
+        if constexpr (kRecords) {
             TIn* yt = static_cast<TIn*>(a.yt) + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, y[kk]);
+            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, delta::first(y[kk]));
         }
         // O^T = scale S^T Q^T E + Y^T M^T: a token's columns in a lane.
+        f32x4 o[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            const int row = tok(b, lr);
+        for (int b = 0; b < 4; ++b) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < NS; ++i) acc = mac(delta::first(s[i]), Rows::one(buf + L::kQ, row, 4 * i + g), acc);
-            acc *= E[row] * a.scale;
+        for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int kk = 0; kk <= (b >> 1); ++kk) acc = mac(y[kk], Square::one(buf + L::kM, row, 4 * kk + g), acc);
-            const int64_t t = int64_t(c) * kChunk + row;
-            if (t < len) {
-                TIn* o = op + t * a.dv + c0 + 4 * g;
-                const int there = a.dv - (c0 + 4 * g);
-                if (a.vec_o && there >= 4) {
-                    store4_of(o, acc);
-                } else {
+            for (int b = 0; b < 4; ++b) o[b] = mac(s[i], Rows::one(buf + L::kQ, k_row, b, i), o[b]);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (r < there) store_val(o + r, acc[r]);
-                }
-            }
-        }
+        for (int b = 0; b < 4; ++b) o[b] *= E[tok(b, lr)] * a.scale;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) o[b] = mac(y[0], Square::one(buf + L::kM, s_row, b, 0), o[b]);
+#pragma unroll
+        for (int b = 2; b < 4; ++b) o[b] = mac(y[1], Square::one(buf + L::kM, s_row, b, 1), o[b]);
         // S = e^{G_last} S + K^T (Z b Y).
         const float decay = E[63];
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i) {
-            f32x4 acc = S[i] * decay;
+        for (int i = 0; i < DK / 16; ++i) S[i] *= decay;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) acc = mac(Rows::transposed(buf + L::kK, 32 * kk, i, g, lr), z[kk], acc);
-            S[i] = acc;
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) S[i] = mac(Rows::transposed(buf + L::kK, k_col, kk, i), z[kk], S[i]);
+        const int64_t t0 = int64_t(c) * kChunk;
+        if constexpr (kVec) {
+            // Rows past the last live one lie outside the view.
+            const int rows = int(len - t0 < kChunk ? len - t0 : kChunk);
+            const auto out = mfma::make_rsrc(op + t0 * a.dv, int64_t(rows) * a.dv * int(sizeof(TIn)));
+            const bool there = c0 + 4 * g < a.dv;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                mfma::store4<TIn, mfma::kPolicyDefault>(
+                    out, there ? (tok(b, lr) * a.dv + c0 + 4 * g) * int(sizeof(TIn)) : mfma::kOutside, o[b]);
+        } else {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int64_t t = t0 + tok(b, lr);
+                if (t >= len) continue;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (c0 + 4 * g + r < a.dv) store_val(op + t * a.dv + c0 + 4 * g + r, o[b][r]);
+            }
         }
     }
     if (!active || col >= a.dv) return;
@@ -453,17 +470,25 @@ __global__ __launch_bounds__(kThreads) void delta_step_kernel(const DeltaArgs a)
     }
 }
 
-template <typename TIn, int DK>
+template <typename TIn, int DK, bool kVec>
 hipError_t launch_chunks(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
     using L = ChunkLds<TIn, DK>;
     constexpr int solve = solve_lds_bytes<TIn, DK>(), walk = L::kBuffers * L::kBytes;
     static_assert(solve <= kGfx950LdsBytes && walk <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
-    delta_solve_kernel<TIn, DK><<<unsigned(r.N * a.chunks), kThreads, solve, stream>>>(a);
+    delta_solve_kernel<TIn, DK, kVec><<<unsigned(r.N * a.chunks), kThreads, solve, stream>>>(a);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    const int64_t blocks = (r.dv + 63) / 64;
-    delta_chunk_kernel<TIn, DK><<<unsigned((r.N + 7) / 8 * 8 * blocks), kThreads, walk, stream>>>(a);
+    const unsigned grid = unsigned((r.N + 7) / 8 * 8 * ((r.dv + 63) / 64));
+    if (a.st)
+        delta_chunk_kernel<TIn, DK, kVec, true><<<grid, kThreads, walk, stream>>>(a);
+    else
+        delta_chunk_kernel<TIn, DK, kVec, false><<<grid, kThreads, walk, stream>>>(a);
     return hipGetLastError();
+}
+
+template <typename TIn, bool kVec>
+hipError_t launch_by_width(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
+    return r.dk <= 64 ? launch_chunks<TIn, 64, kVec>(r, a, stream) : launch_chunks<TIn, 128, kVec>(r, a, stream);
 }
 
 template <typename TIn, int V>
@@ -507,9 +532,10 @@ hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* 
     a.tm = base, a.mm = base + l.mm;
     a.vec = reinterpret_cast<float*>(base + l.vec);
     if (records) a.st = base + l.solve_bytes, a.yt = base + l.yt;
+    const bool vec = a.vec_k && a.vec_v && a.vec_o;
     if (r.dtype == RACE_BF16)
-        return r.dk <= 64 ? launch_chunks<bf16_t, 64>(r, a, stream) : launch_chunks<bf16_t, 128>(r, a, stream);
-    return r.dk <= 64 ? launch_chunks<float, 64>(r, a, stream) : launch_chunks<float, 128>(r, a, stream);
+        return vec ? launch_by_width<bf16_t, true>(r, a, stream) : launch_by_width<bf16_t, false>(r, a, stream);
+    return vec ? launch_by_width<float, true>(r, a, stream) : launch_by_width<float, false>(r, a, stream);
 }
 
 }  // namespace race

@@ -65,6 +65,9 @@ __device__ __forceinline__ f32x4 mac(const OneT<bf16_t>& x, const OneT<bf16_t>& 
 __device__ __forceinline__ f32x4 mac(const OneT<bf16_t>& x, const TwoT<bf16_t>& y, f32x4 acc) {
     return mfma::mfma16(x.h, y.h, mfma::mfma16(x.h, y.l, acc));
 }
+__device__ __forceinline__ f32x4 mac(const TwoT<bf16_t>& x, const OneT<bf16_t>& y, f32x4 acc) {
+    return mfma::mfma16(x.h, y.h, mfma::mfma16(x.l, y.h, acc));
+}
 __device__ __forceinline__ f32x4 mac(const TwoT<bf16_t>& x, const TwoT<bf16_t>& y, f32x4 acc) {
     return mfma::mfma16(x.h, y.h, mfma::mfma16(x.h, y.l, mfma::mfma16(x.l, y.h, acc)));
 }
@@ -110,11 +113,15 @@ __device__ __forceinline__ void store_run(float* p, const OneT<float>& x) {
 
 // ---- tiles ----
 
+// Offsets come in two parts: a lane's own (`..._base`, the same for every chunk)
+// and what a product adds to it, which does not depend on the lane: rows of a
+// block pair by addition, columns by exclusive or.
 template <typename E, int K>
 struct Tile {
     static constexpr int kRow = K * int(sizeof(E));  // bytes
     static constexpr int kChunks = kRow / 16;
     static constexpr int kBytes = kChunk * kRow;
+    static constexpr int kRun = 32 * int(sizeof(E));  // bytes of 32 values
     __device__ __forceinline__ static int at(int r, int u) {
         static_assert(kRow == 128 || kRow == 256 || kRow == 512, "");
         if constexpr (sizeof(E) == 4 && kRow > 128)
@@ -125,89 +132,107 @@ struct Tile {
             return r * kRow + 16 * (u ^ (((r >> 1) & 1) | ((r >> 3) & 2) | ((r >> 1) & 4)));
     }
     // Values 8 u .. 8 u + 7 of a row.
-    __device__ __forceinline__ static OneT<E> one(const unsigned char* t, int row, int u) {
+    __device__ __forceinline__ static int run_at(int row, int u) { return at(row, int(sizeof(E)) / 2 * u); }
+    __device__ __forceinline__ static OneT<E> load(const unsigned char* t, int off) {
         if constexpr (sizeof(E) == 4)
-            return {*reinterpret_cast<const f32x4*>(t + at(row, 2 * u)), *reinterpret_cast<const f32x4*>(t + at(row, 2 * u + 1))};
+            return {*reinterpret_cast<const f32x4*>(t + off), *reinterpret_cast<const f32x4*>(t + (off ^ 16))};
         else
-            return {*reinterpret_cast<const bf16x8*>(t + at(row, u))};
+            return {*reinterpret_cast<const bf16x8*>(t + off)};
+    }
+    // Row lr of block b (rows tok(b, .)), values 32 i + 8 g .., from row_base.
+    __device__ __forceinline__ static int row_base(int lr, int g) { return run_at(tok(0, lr), g); }
+    __device__ __forceinline__ static int row_off(int base, int b, int i) {
+        return (base ^ (4 * (b & 1) * kRow) ^ (kRun * i)) + (b >> 1) * 32 * kRow;
+    }
+    __device__ __forceinline__ static OneT<E> one(const unsigned char* t, int base, int b, int i) {
+        return load(t, row_off(base, b, i));
     }
     // The same of a tile in two planes (bf16), or of fp32 values.
-    __device__ __forceinline__ static TwoT<E> two(const unsigned char* t, int row, int u) {
+    __device__ __forceinline__ static TwoT<E> two(const unsigned char* t, int base, int b, int i) {
         TwoT<E> x;
-        if constexpr (sizeof(E) == 4) {
-            const OneT<E> o = one(t, row, u);
-            x.a = o.a, x.b = o.b;
-        } else {
-            x.h = one(t, row, u).h, x.l = one(t + kBytes, row, u).h;
-        }
-        return x;
-    }
-    // Four rows from `row` of one column: of the 16 lanes of a group, lane 4 r + q
-    // names the four columns from `col` in row r, and lane i gets column i of the 16.
-    __device__ __forceinline__ static uint2 read_tr(const unsigned char* t, int row, int col) {
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const unsigned char* p = t + at(row, col >> 3) + 8 * ((col >> 2) & 1);
-        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
-    }
-    __device__ __forceinline__ static float value(const unsigned char* t, int row, int col) {
-        return *reinterpret_cast<const float*>(t + at(row, col >> 2) + 4 * (col & 3));
-    }
-    // Values of rows row0 + 8 g + e, e = 0 .. 7, in column c(lr) of 16: c(4 q + j) = cols(q) + j.
-    template <typename F>
-    __device__ __forceinline__ static OneT<E> column(const unsigned char* t, int row0, int g, int lr, F cols) {
-        OneT<E> x;
-        if constexpr (sizeof(E) == 4) {
-            const int col = cols(lr >> 2) + (lr & 3);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x.a[e] = value(t, row0 + 8 * g + e, col);
-                x.b[e] = value(t, row0 + 8 * g + 4 + e, col);
-            }
-        } else {
-            const int row = row0 + 8 * g + (lr >> 2), col = cols(lr & 3);
-            const uint2 a = read_tr(t, row, col), b = read_tr(t, row + 4, col);
-            x.h = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, b.x, b.y));
-        }
-        return x;
-    }
-    // Of the columns tok(b, 0..15).
-    __device__ __forceinline__ static OneT<E> transposed(const unsigned char* t, int row0, int b, int g, int lr) {
-        return column(t, row0, g, lr, [&](int q) { return tok(b, 4 * q); });
-    }
-    // The same of a tile in two planes.
-    __device__ __forceinline__ static TwoT<E> transposed_two(const unsigned char* t, int row0, int b, int g, int lr) {
-        TwoT<E> x;
-        const OneT<E> o = transposed(t, row0, b, g, lr);
+        const OneT<E> o = one(t, base, b, i);
         if constexpr (sizeof(E) == 4)
             x.a = o.a, x.b = o.b;
         else
-            x.h = o.h, x.l = transposed(t + kBytes, row0, b, g, lr).h;
+            x.h = o.h, x.l = one(t + kBytes, base, b, i).h;
+        return x;
+    }
+    // Four rows of one column: of the 16 lanes of a group, lane 4 r + q names four
+    // columns of row r, and lane i gets column i of the 16.
+    __device__ __forceinline__ static uint2 read_tr(const unsigned char* p) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+    }
+    // Column tok(b, lr), rows 32 kk + 8 g + e, from column_base.
+    __device__ __forceinline__ static int column_base(int lr, int g) {
+        if constexpr (sizeof(E) == 4) {
+            const int col = tok(0, lr);
+            return at(8 * g, col >> 2) + 4 * (col & 3);
+        } else {
+            return at(8 * g + (lr >> 2), lr & 3) + 8 * (lr & 1);
+        }
+    }
+    __device__ __forceinline__ static OneT<E> transposed(const unsigned char* t, int base, int kk, int b) {
+        OneT<E> x;
+        const int off = (base ^ (kRun * (b >> 1)) ^ (4 * int(sizeof(E)) * (b & 1))) + 32 * kk * kRow;
+        if constexpr (sizeof(E) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x.a[e] = *reinterpret_cast<const float*>(t + (off ^ (32 * e)) + e * kRow);
+                x.b[e] = *reinterpret_cast<const float*>(t + (off ^ (32 * e)) + (e + 4) * kRow);
+            }
+        } else {
+            const uint2 a = read_tr(t + off), c = read_tr(t + off + 4 * kRow);
+            x.h = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, c.x, c.y));
+        }
+        return x;
+    }
+    // The same of a tile in two planes.
+    __device__ __forceinline__ static TwoT<E> transposed_two(const unsigned char* t, int base, int kk, int b) {
+        TwoT<E> x;
+        const OneT<E> o = transposed(t, base, kk, b);
+        if constexpr (sizeof(E) == 4)
+            x.a = o.a, x.b = o.b;
+        else
+            x.h = o.h, x.l = transposed(t + kBytes, base, kk, b).h;
         return x;
     }
     // Values col .. col + 3 (a multiple of 4) of a row.
-    __device__ __forceinline__ static f32x4 four(const unsigned char* t, int row, int col) {
+    __device__ __forceinline__ static int four_at(int row, int col) {
+        if constexpr (sizeof(E) == 4) return at(row, col >> 2);
+        return at(row, col >> 3) + 8 * ((col >> 2) & 1);
+    }
+    __device__ __forceinline__ static f32x4 four(const unsigned char* t, int off) {
         if constexpr (sizeof(E) == 4) {
-            return *reinterpret_cast<const f32x4*>(t + at(row, col >> 2));
+            return *reinterpret_cast<const f32x4*>(t + off);
         } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(t + at(row, col >> 3) + 8 * ((col >> 2) & 1));
+            const uint2 u = *reinterpret_cast<const uint2*>(t + off);
             return f32x4{mfma::lo_half(u.x), mfma::hi_half(u.x), mfma::lo_half(u.y), mfma::hi_half(u.y)};
         }
     }
-    __device__ __forceinline__ static void put4(unsigned char* t, int row, int col, const f32x4& x) {
+    __device__ __forceinline__ static void put4(unsigned char* t, int off, const f32x4& x) {
         if constexpr (sizeof(E) == 4)
-            *reinterpret_cast<f32x4*>(t + at(row, col >> 2)) = x;
+            *reinterpret_cast<f32x4*>(t + off) = x;
         else
-            *reinterpret_cast<uint2*>(t + at(row, col >> 3) + 8 * ((col >> 2) & 1)) =
-                make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
+            *reinterpret_cast<uint2*>(t + off) = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
     }
-    // Rows tok(b, 4 g .. 4 g + 3) of column c0 + lr, in accumulator order.
-    __device__ __forceinline__ static f32x4 block(const unsigned char* t, int b, int c0, int g, int lr) {
-        const int row = tok(b, 4 * g);
+    // Rows tok(b, 4 g .. 4 g + 3) of column c0 + lr, in accumulator order, from block_base.
+    __device__ __forceinline__ static int block_base(int c0, int lr, int g) {
+        const int row = tok(0, 4 * g);
+        if constexpr (sizeof(E) == 4) return at(row, (c0 + lr) >> 2) + 4 * (lr & 3);
+        const int col = c0 + 4 * (lr & 3);
+        return at(row + (lr >> 2), col >> 3) + 8 * ((col >> 2) & 1);
+    }
+    __device__ __forceinline__ static f32x4 block(const unsigned char* t, int base, int b) {
+        const int off = (base ^ (4 * (b & 1) * kRow)) + (b >> 1) * 32 * kRow;
         if constexpr (sizeof(E) == 4) {
-            return f32x4{value(t, row, c0 + lr), value(t, row + 1, c0 + lr), value(t, row + 2, c0 + lr), value(t, row + 3, c0 + lr)};
+            f32x4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const float*>(t + (off ^ (32 * r)) + r * kRow);
+            return x;
         } else {
-            const uint2 u = read_tr(t, row + (lr >> 2), c0 + 4 * (lr & 3));
+            const uint2 u = read_tr(t + off);
             return f32x4{mfma::lo_half(u.x), mfma::hi_half(u.x), mfma::lo_half(u.y), mfma::hi_half(u.y)};
         }
     }
@@ -216,53 +241,69 @@ struct Tile {
 template <typename E, int K>
 constexpr int kTwoBytes = sizeof(E) == 4 ? Tile<E, K>::kBytes : 2 * Tile<E, K>::kBytes;
 
-// Eight consecutive values of a row, of which the first `n` are there.
+// Eight consecutive values of a row, of which the first `n` are there, one by one.
 template <typename TIn>
 struct Eight {
     static constexpr int kVecs = int(sizeof(TIn)) / 2;
     uint4 v[kVecs];
-    __device__ __forceinline__ void load(const TIn* p, int n, bool vec) {
+    __device__ __forceinline__ void load(const TIn* p, int n) {
+        uint32_t w[4 * kVecs];
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(0, 0, 0, 0);
-        if (n <= 0) return;
-        if (vec) {
-            v[0] = reinterpret_cast<const uint4*>(p)[0];
-            if constexpr (kVecs == 2) {
-                if (n > 4) v[1] = reinterpret_cast<const uint4*>(p)[1];
-            }
-        } else {
-            uint32_t w[4 * kVecs];
+        for (int i = 0; i < 4 * kVecs; ++i) w[i] = 0;
 #pragma unroll
-            for (int i = 0; i < 4 * kVecs; ++i) w[i] = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i >= n) break;
-                if constexpr (kVecs == 2)
-                    w[i] = __float_as_uint(p[i]);
-                else
-                    w[i >> 1] |= uint32_t(p[i]) << (16 * (i & 1));
-            }
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        for (int i = 0; i < 8; ++i) {
+            if (i >= n) break;
+            if constexpr (kVecs == 2)
+                w[i] = __float_as_uint(p[i]);
+            else
+                w[i >> 1] |= uint32_t(p[i]) << (16 * (i & 1));
         }
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
 };
 
+// Byte offset of the 16-byte piece from column `col` of a row; outside every view past the row's width.
+template <typename TIn>
+__device__ __forceinline__ int piece_at(int row, int stride, int col, int width) {
+    return col < width ? (row * stride + col) * int(sizeof(TIn)) : mfma::kOutside;
+}
+
 // 64 rows of K values: each thread's 8-value pieces in registers and then in a tile.
-template <typename TIn, int K, int NT>
+// kVec: rows in 16-byte pieces, read through a view that ends with the last live
+// row; else value by value.
+template <typename TIn, int K, int NT, bool kVec>
 struct Stage {
-    static constexpr int kPer = kChunk * (K / 8) / NT;
+    static constexpr int kPer = kChunk * (K / 8) / NT, kVecs = Eight<TIn>::kVecs;
     Eight<TIn> x[kPer];
-    // Rows of p by stride, `live` of them there, `width` values each.
-    __device__ __forceinline__ void load(const TIn* p, int64_t stride, int live, int width, bool vec) {
+    int off[kVec ? kPer * kVecs : 1];
+    __device__ __forceinline__ void init(int64_t stride, int width) {
+        if constexpr (kVec) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int q = int(threadIdx.x) + i * NT, row = q / (K / 8), u = q % (K / 8);
-            x[i].load(p + row * stride + 8 * u, row < live ? width - 8 * u : 0, vec);
+            for (int i = 0; i < kPer; ++i) {
+                const int q = int(threadIdx.x) + i * NT, row = q / (K / 8), u = q % (K / 8);
+#pragma unroll
+                for (int j = 0; j < kVecs; ++j) off[i * kVecs + j] = piece_at<TIn>(row, int(stride), 8 * u + 4 * j, width);
+            }
+        }
+    }
+    // Rows of p by stride, `live` of them there, `width` values each.
+    __device__ __forceinline__ void load(const TIn* p, int64_t stride, int live, int width) {
+        if constexpr (kVec) {
+            const auto r = mfma::make_rsrc(p, ((live - 1) * stride + width) * int(sizeof(TIn)));
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+#pragma unroll
+                for (int j = 0; j < kVecs; ++j) x[i].v[j] = mfma::buf_load16<mfma::kPolicyDefault>(r, off[i * kVecs + j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int q = int(threadIdx.x) + i * NT, row = q / (K / 8), u = q % (K / 8);
+                x[i].load(p + row * stride + 8 * u, row < live ? width - 8 * u : 0);
+            }
         }
     }
     __device__ __forceinline__ void put(unsigned char* t) const {
-        constexpr int kVecs = Eight<TIn>::kVecs;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int q = int(threadIdx.x) + i * NT, row = q / (K / 8), u = q % (K / 8);
@@ -279,8 +320,9 @@ struct StageDense {
     static constexpr int kChunks = Tile<E, K>::kChunks, kPer = ROWS * kChunks / NT;
     uint4 x[kPer];
     __device__ __forceinline__ void load(const E* p) {
+        const auto r = mfma::make_rsrc(p, ROWS * K * int(sizeof(E)));
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] = reinterpret_cast<const uint4*>(p)[int(threadIdx.x) + i * NT];
+        for (int i = 0; i < kPer; ++i) x[i] = mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * (int(threadIdx.x) + i * NT));
     }
     __device__ __forceinline__ void put(unsigned char* t) const {
 #pragma unroll
@@ -312,7 +354,7 @@ struct DeltaArgs {
     Live live;
     int group, dk, dv, dvp, chunks;  // group: value streams of a key stream
     int gate_f32, form;
-    int vec_k, vec_v, vec_o, vec_o8;  // rows in 16-byte pieces (q and k, v; out and dout in 4 values, and whole)
+    int vec_k, vec_v, vec_o;  // rows of q and k, of v, of out (and dout) in 16-byte pieces
     float scale;
 };
 
@@ -356,11 +398,17 @@ __device__ __forceinline__ bool stream_and_block(int64_t N, int blocks, int64_t&
 
 inline int dk_padded(const DeltaRule& r) { return r.dk <= 64 ? 64 : 128; }
 
+// Whether a row is whole 16-byte pieces, and 64 rows of it lie within one buffer view.
 inline bool whole_pieces(const DeltaRule& r, int64_t width, std::initializer_list<int64_t> strides) {
     const int v = r.dtype == RACE_BF16 ? 8 : 4;
     if (width % v != 0) return false;
     for (int64_t s : strides)
         if (s % v != 0) return false;
+    return true;
+}
+inline bool near_rows(std::initializer_list<int64_t> token_strides) {
+    for (int64_t s : token_strides)
+        if (s > (int64_t(1) << 22)) return false;
     return true;
 }
 
@@ -373,10 +421,9 @@ inline DeltaArgs delta_args(const DeltaRule& r, const DeltaInputs& in) {
     a.group = r.Nk > 0 ? int(r.N / r.Nk) : 1;
     a.dk = r.dk, a.dv = r.dv, a.dvp = (r.dv + 15) / 16 * 16, a.chunks = int(delta_chunks(r));
     a.gate_f32 = r.gate_dtype == RACE_F32, a.form = r.form;
-    a.vec_k = whole_pieces(r, r.dk, {r.qn, r.qt, r.kn, r.kt});
-    a.vec_v = whole_pieces(r, r.dv, {r.vn, r.vt});
-    a.vec_o = r.dv % 4 == 0;
-    a.vec_o8 = whole_pieces(r, r.dv, {});
+    a.vec_k = whole_pieces(r, r.dk, {r.qn, r.qt, r.kn, r.kt}) && near_rows({r.qt, r.kt});
+    a.vec_v = whole_pieces(r, r.dv, {r.vn, r.vt}) && near_rows({r.vt});
+    a.vec_o = whole_pieces(r, r.dv, {});
     a.scale = r.scale;
     return a;
 }
