@@ -109,6 +109,18 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
         if (!active) continue;
         const float* E = reinterpret_cast<const float*>(buf + L::kVec);
         const int64_t nc = n * a.chunks + c;
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        One kf[NS][4];
+        f32x4 o[4], e[4];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) kf[i][b] = Rows::one(buf + L::kK, k_row, b, i);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            o[b] = Square::block(buf + L::kV, o_at, b);
+            e[b] = *reinterpret_cast<const f32x4*>(E + tok(b, 4 * g));
+        }
         Two s[NS];
         TIn* ds = static_cast<TIn*>(w.ds) + (nc * a.dvp + col) * DK + 8 * g;
 #pragma unroll
@@ -116,52 +128,59 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
             operand(dS[2 * i], dS[2 * i + 1], odd, s[i]);
             store_run(ds + 32 * i, delta::first(s[i]));
         }
+        stage_wall();
+        One mf[4], mg[2];
+        f32x4 zb[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            mf[b] = Square::transposed(buf + L::kM, s_col, 1, b);
+            zb[b] = *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) mg[b] = Square::transposed(buf + L::kM, s_col, 0, b);
         // dO as it is, and as E dO scale.
-        One o[2], eo[2];
+        One od[2], eo[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            f32x4 x[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[h] = Square::block(buf + L::kV, o_at, 2 * kk + h);
-            operand(x[0], x[1], odd, o[kk]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[h] *= *reinterpret_cast<const f32x4*>(E + tok(2 * kk + h, 4 * g)) * a.scale;
-            operand(x[0], x[1], odd, eo[kk]);
+            operand(o[2 * kk], o[2 * kk + 1], odd, od[kk]);
+            operand(o[2 * kk] * e[2 * kk] * a.scale, o[2 * kk + 1] * e[2 * kk + 1] * a.scale, odd, eo[kk]);
         }
         // dY = M^T dO + Z b (K dS').
         f32x4 x[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) x[b] = mac(Rows::one(buf + L::kK, k_row, b, i), s[i], x[b]);
+            for (int b = 0; b < 4; ++b) x[b] = mac(kf[i][b], s[i], i == 0 ? zero : x[b]);
+        stage_wall();
+        Two tf[4], tg[2];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] *= *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
+        for (int b = 0; b < 4; ++b) tf[b] = Square::transposed_two(buf + L::kT, s_col, 1, b);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = mac(Square::transposed(buf + L::kM, s_col, 1, b), o[1], x[b]);
+        for (int b = 0; b < 2; ++b) tg[b] = Square::transposed_two(buf + L::kT, s_col, 0, b);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) x[b] = mac(Square::transposed(buf + L::kM, s_col, 0, b), o[0], x[b]);
+        for (int b = 0; b < 4; ++b) x[b] = mac(mf[b], od[1], x[b] * zb[b]);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) x[b] = mac(mg[b], od[0], x[b]);
         Two y[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
+        stage_wall();
+        One qc[2][DK / 16];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) qc[kk][i] = Rows::transposed(buf + L::kQ, k_col, kk, i);
         // dD = T^T dY.
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-            x[b] = mac(Square::transposed_two(buf + L::kT, s_col, 1, b), y[1], f32x4{0.f, 0.f, 0.f, 0.f});
+        for (int b = 0; b < 4; ++b) x[b] = mac(tf[b], y[1], zero);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) x[b] = mac(Square::transposed_two(buf + L::kT, s_col, 0, b), y[0], x[b]);
-        Two d[2];
-        TIn* dd = static_cast<TIn*>(w.dd) + (nc * a.dvp + col) * kChunk + 8 * g;
+        for (int b = 0; b < 2; ++b) x[b] = mac(tg[b], y[0], x[b]);
+        stage_wall();
+        One kc[2][DK / 16];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            One plain;
-            operand(x[2 * kk], x[2 * kk + 1], odd, plain);
-            store_run(dd + 32 * kk, plain);
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) x[2 * kk + h] *= -*reinterpret_cast<const f32x4*>(E + tok(2 * kk + h, 4 * g));
-            operand(x[2 * kk], x[2 * kk + 1], odd, d[kk]);
-        }
+            for (int i = 0; i < DK / 16; ++i) kc[kk][i] = Rows::transposed(buf + L::kK, k_col, kk, i);
         // dS = e^{G_last} dS' + scale Q^T (E dO) - K^T (E dD).
         const float decay = E[63];
 #pragma unroll
@@ -169,10 +188,21 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-            for (int i = 0; i < DK / 16; ++i) {
-                dS[i] = mac(Rows::transposed(buf + L::kQ, k_col, kk, i), eo[kk], dS[i]);
-                dS[i] = mac(Rows::transposed(buf + L::kK, k_col, kk, i), d[kk], dS[i]);
-            }
+            for (int i = 0; i < DK / 16; ++i) dS[i] = mac(qc[kk][i], eo[kk], dS[i]);
+        Two d[2];
+        TIn* dd = static_cast<TIn*>(w.dd) + (nc * a.dvp + col) * kChunk + 8 * g;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            One plain;
+            operand(x[2 * kk], x[2 * kk + 1], odd, plain);
+            store_run(dd + 32 * kk, plain);
+            operand(x[2 * kk] * -e[2 * kk], x[2 * kk + 1] * -e[2 * kk + 1], odd, d[kk]);
+        }
+        stage_wall();
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) dS[i] = mac(kc[kk][i], d[kk], dS[i]);
     }
     if (!w.dstate || !active || col >= a.dv) return;
 #pragma unroll

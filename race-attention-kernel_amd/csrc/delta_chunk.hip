@@ -211,6 +211,7 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
     using L = ChunkLds<TIn, DK>;
     using Rows = Tile<TIn, DK>;
     using Square = Tile<TIn, 64>;
+    using One = OneT<TIn>;
     using Two = TwoT<TIn>;
     constexpr int NS = DK / 32;
     int64_t n;
@@ -272,6 +273,12 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
         if (!active) continue;
         const float* E = reinterpret_cast<const float*>(buf + L::kVec);
         const int64_t nc = n * a.chunks + c;
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        One kf[NS][4];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) kf[i][b] = Rows::one(buf + L::kK, k_row, b, i);
         Two s[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) operand(S[2 * i], S[2 * i + 1], odd, s[i]);
@@ -280,56 +287,61 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
 #pragma unroll
             for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first(s[i]));
         }
+        stage_wall();
+        Two tf[4], tg[2];
+        f32x4 e[4], v[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            e[b] = *reinterpret_cast<const f32x4*>(E + tok(b, 4 * g));
+            v[b] = Square::block(buf + L::kV, v_at, b);
+            tf[b] = Square::two(buf + L::kT, s_row, b, 0);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) tg[b] = Square::two(buf + L::kT, s_row, 2 + b, 1);
         // D = V - E K S.
         f32x4 x[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) x[b] = mac(Rows::one(buf + L::kK, k_row, b, i), s[i], x[b]);
+            for (int b = 0; b < 4; ++b) x[b] = mac(kf[i][b], s[i], i == 0 ? zero : x[b]);
+        stage_wall();
+        One kc[2][DK / 16];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const f32x4 e = *reinterpret_cast<const f32x4*>(E + tok(b, 4 * g));
-            const f32x4 v = Square::block(buf + L::kV, v_at, b);
+        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[b][r] = fmaf(-e[r], x[b][r], v[r]);
-        }
+            for (int i = 0; i < DK / 16; ++i) kc[kk][i] = Rows::transposed(buf + L::kK, k_col, kk, i);
+        f32x4 zb[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) zb[b] = *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[b][r] = fmaf(-e[b][r], x[b][r], v[b][r]);
         Two d[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, d[kk]);
         // Y = T D; T is lower triangular.
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = mac(Square::two(buf + L::kT, s_row, b, 0), d[0], f32x4{0.f, 0.f, 0.f, 0.f});
+        for (int b = 0; b < 4; ++b) x[b] = mac(tf[b], d[0], zero);
 #pragma unroll
-        for (int b = 2; b < 4; ++b) x[b] = mac(Square::two(buf + L::kT, s_row, b, 1), d[1], x[b]);
+        for (int b = 2; b < 4; ++b) x[b] = mac(tg[b - 2], d[1], x[b]);
+        stage_wall();
+        One qf[NS][4];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) qf[i][b] = Rows::one(buf + L::kQ, k_row, b, i);
         Two y[2], z[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[2 * kk + h] *= *reinterpret_cast<const f32x4*>(E + 64 + tok(2 * kk + h, 4 * g));
-            operand(x[2 * kk], x[2 * kk + 1], odd, z[kk]);
+            operand(x[2 * kk] * zb[2 * kk], x[2 * kk + 1] * zb[2 * kk + 1], odd, z[kk]);
         }
         if constexpr (kRecords) {
             TIn* yt = static_cast<TIn*>(a.yt) + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, delta::first(y[kk]));
         }
-        // O^T = scale S^T Q^T E + Y^T M^T: a token's columns in a lane.
-        f32x4 o[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) o[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) o[b] = mac(s[i], Rows::one(buf + L::kQ, k_row, b, i), o[b]);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) o[b] *= E[tok(b, lr)] * a.scale;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) o[b] = mac(y[0], Square::one(buf + L::kM, s_row, b, 0), o[b]);
-#pragma unroll
-        for (int b = 2; b < 4; ++b) o[b] = mac(y[1], Square::one(buf + L::kM, s_row, b, 1), o[b]);
         // S = e^{G_last} S + K^T (Z b Y).
         const float decay = E[63];
 #pragma unroll
@@ -337,7 +349,24 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-            for (int i = 0; i < DK / 16; ++i) S[i] = mac(Rows::transposed(buf + L::kK, k_col, kk, i), z[kk], S[i]);
+            for (int i = 0; i < DK / 16; ++i) S[i] = mac(kc[kk][i], z[kk], S[i]);
+        stage_wall();
+        One mf[4], mg[2];
+        float es[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) mf[b] = Square::one(buf + L::kM, s_row, b, 0), es[b] = E[tok(b, lr)] * a.scale;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) mg[b] = Square::one(buf + L::kM, s_row, 2 + b, 1);
+        // O^T = scale S^T Q^T E + Y^T M^T, S the state before the chunk: a token's columns in a lane.
+        f32x4 o[4];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) o[b] = mac(s[i], qf[i][b], i == 0 ? zero : o[b]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) o[b] = mac(y[0], mf[b], o[b] * es[b]);
+#pragma unroll
+        for (int b = 2; b < 4; ++b) o[b] = mac(y[1], mg[b - 2], o[b]);
         const int64_t t0 = int64_t(c) * kChunk;
         if constexpr (kVec) {
             // Rows past the last live one lie outside the view.

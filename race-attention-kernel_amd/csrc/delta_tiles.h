@@ -111,6 +111,12 @@ __device__ __forceinline__ void store_run(float* p, const OneT<float>& x) {
     *reinterpret_cast<f32x4*>(p + 4) = x.b;
 }
 
+// A wall the scheduler moves nothing across.  The walks have one wave a SIMD:
+// nothing hides a read's latency but the wave's own instructions, and left alone
+// the compiler puts each LDS read right in front of its product.  A stage's reads
+// are issued before the products of the stage before it.
+__device__ __forceinline__ void stage_wall() { __builtin_amdgcn_sched_barrier(0); }
+
 // ---- tiles ----
 
 // Offsets come in two parts: a lane's own (`..._base`, the same for every chunk)
