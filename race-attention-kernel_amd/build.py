@@ -39,6 +39,14 @@ HIP_FLAGS = [
     f"-I{INCLUDE}", f"-I{CSRC}",
 ]
 
+# Sources whose kernels run one wave a SIMD with most of its 512 registers: products
+# whose results the vector ALU reads next stay in the half it reads (their walks:
+# 198 -> 24 register copies a chunk).
+SOURCE_FLAGS = {
+    "delta_chunk": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "delta_bwd": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+}
+
 
 def hip_sources() -> list[pathlib.Path]:
     return sorted(CSRC.glob("*.hip"))
@@ -71,7 +79,7 @@ def build_hip_library(verbose: bool = False, jobs: int = 8) -> pathlib.Path:
 
     def compile_one(src_obj):
         src, obj = src_obj
-        _run([HIPCC, *HIP_FLAGS, "-c", str(src), "-o", str(obj)], verbose)
+        _run([HIPCC, *HIP_FLAGS, *SOURCE_FLAGS.get(src.stem, []), "-c", str(src), "-o", str(obj)], verbose)
 
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs)))) as ex:
         list(ex.map(compile_one, zip(srcs, objs)))
