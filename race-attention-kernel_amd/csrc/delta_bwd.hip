@@ -81,20 +81,23 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
     sk.init(a.kt, a.dk);
     sq.init(a.qt, a.dk);
     so.init(a.dv, a.dv - cb * 64);
-    auto fetch = [&](int c) {
+    auto fetch = [&](int c, int part) {  // as the forward's
         const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
-        sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
-        sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
-        stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
-        smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
-        so.load(op + t0 * a.dv, a.dv, live, a.dv - cb * 64);
-        svec = a.vec[nc * 128 + (threadIdx.x & 127)];
+        if (part == 0) sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
+        if (part == 1) sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
+        if (part == 2) stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
+        if (part == 3) {
+            smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
+            so.load(op + t0 * a.dv, a.dv, live, a.dv - cb * 64);
+            svec = a.vec[nc * 128 + (threadIdx.x & 127)];
+        }
     };
     // What a lane adds to a tile's start.
     const int k_row = Rows::row_base(lr, g), k_col = Rows::column_base(lr, g), s_col = Square::column_base(lr, g);
     const int o_at = Square::block_base(16 * wave, lr, g);
-    if (chunks > 0) fetch(chunks - 1);
+    if (chunks > 0)
+        for (int p = 0; p < 4; ++p) fetch(chunks - 1, p);
     for (int c = chunks - 1; c >= 0; --c) {
         unsigned char* buf = lds + (L::kBuffers == 2 ? (c & 1) * L::kBytes : 0);
         if (L::kBuffers == 1 && c < chunks - 1) __syncthreads();  // the chunk before is done with the buffer
@@ -104,9 +107,12 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
         smm.put(buf + L::kM);
         so.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
-        if (c > 0) fetch(c - 1);
+        const int next = c > 0 ? c - 1 : 0;  // the last chunk's loads are not used
         __syncthreads();
-        if (!active) continue;
+        if (!active) {
+            for (int p = 0; p < 4; ++p) fetch(next, p);
+            continue;
+        }
         const float* E = reinterpret_cast<const float*>(buf + L::kVec);
         const int64_t nc = n * a.chunks + c;
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -129,6 +135,7 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
             store_run(ds + 32 * i, delta::first(s[i]));
         }
         stage_wall();
+        fetch(next, 0);
         One mf[4], mg[2];
         f32x4 zb[4];
 #pragma unroll
@@ -152,6 +159,7 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 #pragma unroll
             for (int b = 0; b < 4; ++b) x[b] = mac(kf[i][b], s[i], i == 0 ? zero : x[b]);
         stage_wall();
+        fetch(next, 1);
         Two tf[4], tg[2];
 #pragma unroll
         for (int b = 0; b < 4; ++b) tf[b] = Square::transposed_two(buf + L::kT, s_col, 1, b);
@@ -165,6 +173,7 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
         stage_wall();
+        fetch(next, 2);
         One qc[2][DK / 16];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
@@ -176,6 +185,7 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 #pragma unroll
         for (int b = 0; b < 2; ++b) x[b] = mac(tg[b], y[0], x[b]);
         stage_wall();
+        fetch(next, 3);
         One kc[2][DK / 16];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)

@@ -245,20 +245,24 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
     sk.init(a.kt, a.dk);
     sq.init(a.qt, a.dk);
     sv.init(a.vt, a.dv - cb * 64);
-    auto fetch = [&](int c) {
+    // A chunk's loads, in four parts: all at once they fill the queue, and the wave waits to issue them.
+    auto fetch = [&](int c, int part) {
         const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
-        sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
-        sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
-        stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
-        smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
-        sv.load(vp + t0 * a.vt, a.vt, live, a.dv - cb * 64);
-        svec = a.vec[nc * 128 + (threadIdx.x & 127)];
+        if (part == 0) sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
+        if (part == 1) sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
+        if (part == 2) stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
+        if (part == 3) {
+            smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
+            sv.load(vp + t0 * a.vt, a.vt, live, a.dv - cb * 64);
+            svec = a.vec[nc * 128 + (threadIdx.x & 127)];
+        }
     };
     // What a lane adds to a tile's start.
     const int k_row = Rows::row_base(lr, g), k_col = Rows::column_base(lr, g), s_row = Square::row_base(lr, g);
     const int v_at = Square::block_base(16 * wave, lr, g);
-    if (chunks > 0) fetch(0);
+    if (chunks > 0)
+        for (int p = 0; p < 4; ++p) fetch(0, p);
     for (int c = 0; c < chunks; ++c) {
         unsigned char* buf = lds + (L::kBuffers == 2 ? (c & 1) * L::kBytes : 0);
         if (L::kBuffers == 1 && c > 0) __syncthreads();  // the chunk before is done with the buffer
@@ -268,9 +272,12 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
         smm.put(buf + L::kM);
         sv.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
-        if (c + 1 < chunks) fetch(c + 1);
+        const int next = c + 1 < chunks ? c + 1 : c;  // the last chunk's loads are not used
         __syncthreads();
-        if (!active) continue;
+        if (!active) {
+            for (int p = 0; p < 4; ++p) fetch(next, p);
+            continue;
+        }
         const float* E = reinterpret_cast<const float*>(buf + L::kVec);
         const int64_t nc = n * a.chunks + c;
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -288,6 +295,7 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
             for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first(s[i]));
         }
         stage_wall();
+        fetch(next, 0);
         Two tf[4], tg[2];
         f32x4 e[4], v[4];
 #pragma unroll
@@ -305,6 +313,7 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
 #pragma unroll
             for (int b = 0; b < 4; ++b) x[b] = mac(kf[i][b], s[i], i == 0 ? zero : x[b]);
         stage_wall();
+        fetch(next, 1);
         One kc[2][DK / 16];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
@@ -326,6 +335,7 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
 #pragma unroll
         for (int b = 2; b < 4; ++b) x[b] = mac(tg[b - 2], d[1], x[b]);
         stage_wall();
+        fetch(next, 2);
         One qf[NS][4];
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -351,6 +361,7 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
 #pragma unroll
             for (int i = 0; i < DK / 16; ++i) S[i] = mac(kc[kk][i], z[kk], S[i]);
         stage_wall();
+        fetch(next, 3);
         One mf[4], mg[2];
         float es[4];
 #pragma unroll
