@@ -41,6 +41,13 @@ struct DeltaBwdArgs {
 
 // ---- the walk ----
 
+__device__ __forceinline__ void store_gate(void* p, int64_t i, int f32, float x) {
+    if (f32)
+        static_cast<float*>(p)[i] = x;
+    else
+        static_cast<bf16_t*>(p)[i] = f32_to_bf16(x);
+}
+
 template <typename TIn, int DK, bool kVec>
 __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwdArgs w) {
     extern __shared__ __align__(16) unsigned char lds[];
@@ -214,6 +221,23 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 #pragma unroll
             for (int i = 0; i < DK / 16; ++i) dS[i] = mac(kc[kk][i], d[kk], dS[i]);
     }
+    // Chunks past the stream's last have no gradients; nor have those of a key stream past all of its.
+    const int64_t end = int64_t(chunks) * kChunk, i0 = threadIdx.x;
+    if (w.dv)
+        for (int64_t i = end * a.dv + i0; i < a.T * a.dv && cb == 0; i += kThreads)
+            store_val(static_cast<TIn*>(w.dv) + n * a.T * a.dv + i, 0.f);
+    for (void* p : {w.dgate, w.dbeta})
+        for (int64_t t = end + i0; p && t < a.T && cb == 0; t += kThreads) store_gate(p, n * a.T + t, a.gate_f32, 0.f);
+    if (n % a.group == 0 && cb == 0) {
+        int64_t most = 0;
+        for (int h = 0; h < a.group; ++h) {
+            const int64_t l = a.live.of(n + h, a.T);
+            most = l > most ? l : most;
+        }
+        for (void* p : {w.dq, w.dk})
+            for (int64_t i = (most + kChunk - 1) / kChunk * kChunk * a.dk + i0; p && i < a.T * a.dk; i += kThreads)
+                store_val(static_cast<TIn*>(p) + nk * a.T * a.dk + i, 0.f);
+    }
     if (!w.dstate || !active || col >= a.dv) return;
 #pragma unroll
     for (int i = 0; i < DK / 16; ++i)
@@ -226,36 +250,82 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 
 // ---- the chunks' gradients ----
 
-constexpr int kGradThreads = 512;
+// Workgroups that stay, one a CU of an MI355X, each taking every 256th chunk: the
+// next slice's rows are on their way while a slice is worked on.  (A workgroup a
+// chunk, one resident a CU for its LDS, waited for its loads two thirds of its time:
+// 8 x 16 streams of 4096 tokens 700 us.)
+constexpr int kGradWorkgroups = 256;
 
-// Columns of the state a step takes: 64 of bf16, 32 of fp32 for the LDS.
+// Columns of the state a step takes (fp32: half as many, for the LDS), and threads:
+// 16 waves of bf16 rows; fp32 fragments take twice the registers.
 template <typename TIn>
 constexpr int kSlice = sizeof(TIn) == 2 ? 64 : 32;
+template <typename TIn>
+constexpr int kGradThreads = sizeof(TIn) == 2 ? 1024 : 512;
 
 template <typename TIn, int DK>
 struct GradLds {
-    static constexpr int SL = kSlice<TIn>, kS = int(sizeof(TIn));
+    static constexpr int SL = kSlice<TIn>, kS = int(sizeof(TIn)), kSquare = Tile<TIn, 64>::kBytes;
     static constexpr int kK = 0, kQ = Tile<TIn, DK>::kBytes, kSt = 2 * kQ, kDs = kSt + SL * DK * kS;
-    static constexpr int kSquare = Tile<TIn, 64>::kBytes;
-    // L^T and X^T lie over the slices of S and dS', once those are read.
-    static constexpr int kL = kSt, kX = kSt + kSquare;
-    static constexpr int kStates = 2 * SL * DK * kS > 2 * kSquare ? 2 * SL * DK * kS : 2 * kSquare;
-    static constexpr int kYt = kSt + kStates, kDd = kYt + SL * kChunk * kS, kO = kDd + SL * kChunk * kS;
-    static constexpr int kBytes = kO + kChunk * SL * kS;
+    static constexpr int kYt = kDs + SL * DK * kS, kDd = kYt + SL * kChunk * kS, kO = kDd + SL * kChunk * kS;
+    static constexpr int kL = kO + kChunk * SL * kS, kX = kL + kSquare, kSums = kX + kSquare;
+    static constexpr int kBytes = kSums + int(sizeof(double)) * kChunk + int(sizeof(float)) * (21 * kChunk + 16);
 };
 
-// Dense rows of K values to a tile, zeros past the first `rows` of ROWS.
-template <typename E, int K, int ROWS>
-__device__ __forceinline__ void stage_rows(const E* p, int rows, unsigned char* t) {
-    constexpr int kChunks = Tile<E, K>::kChunks;
+// ROWS dense rows of K values: a thread's 16-byte pieces in registers, zeros past the
+// first `rows`, then in a tile.
+template <typename E, int K, int ROWS, int NT>
+struct Pieces {
+    static constexpr int kChunks = Tile<E, K>::kChunks, kTotal = ROWS * kChunks, kPer = (kTotal + NT - 1) / NT;
+    uint4 x[kPer];
+    __device__ __forceinline__ void load(const E* p, int rows, int tid) {
+        const auto r = mfma::make_rsrc(p, rows * K * int(sizeof(E)));
 #pragma unroll
-    for (int i = 0; i < (ROWS * kChunks + kGradThreads - 1) / kGradThreads; ++i) {
-        const int q = int(threadIdx.x) + i * kGradThreads, row = q / kChunks, u = q % kChunks;
-        if (ROWS * kChunks % kGradThreads != 0 && q >= ROWS * kChunks) break;
-        const uint4 x = row < rows ? reinterpret_cast<const uint4*>(p)[q] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(t + Tile<E, K>::at(row, u)) = x;
+        for (int i = 0; i < kPer; ++i) {
+            const int q = tid + i * NT;
+            if (kTotal % NT == 0 || q < kTotal) x[i] = mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * q);
+        }
     }
-}
+    __device__ __forceinline__ void put(unsigned char* t, int tid) const {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int q = tid + i * NT;
+            if (kTotal % NT == 0 || q < kTotal)
+                *reinterpret_cast<uint4*>(t + Tile<E, K>::at(q / kChunks, q % kChunks)) = x[i];
+        }
+    }
+};
+
+// 64 rows of `width` values by stride, of which `live` are there, in K columns.
+template <typename TIn, int K, int NT, bool kVec>
+struct RowPieces {
+    static constexpr int kVecs = Eight<TIn>::kVecs, kTotal = kChunk * (K / 8), kPer = (kTotal + NT - 1) / NT;
+    Eight<TIn> x[kPer];
+    __device__ __forceinline__ void load(const TIn* p, int64_t stride, int live, int width, int tid) {
+        const auto r = mfma::make_rsrc(p, ((live - 1) * stride + width) * int(sizeof(TIn)));
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int q = tid + i * NT, row = q / (K / 8), u = q % (K / 8);
+            if (kTotal % NT != 0 && q >= kTotal) continue;
+            if constexpr (kVec) {
+#pragma unroll
+                for (int j = 0; j < kVecs; ++j)
+                    x[i].v[j] = mfma::buf_load16<mfma::kPolicyDefault>(r, piece_at<TIn>(row, int(stride), 8 * u + 4 * j, width));
+            } else {
+                x[i].load(p + row * stride + 8 * u, row < live ? width - 8 * u : 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void put(unsigned char* t, int tid) const {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int q = tid + i * NT, row = q / (K / 8), u = q % (K / 8);
+            if (kTotal % NT != 0 && q >= kTotal) continue;
+#pragma unroll
+            for (int j = 0; j < kVecs; ++j) *reinterpret_cast<uint4*>(t + Tile<TIn, K>::at(row, kVecs * u + j)) = x[i].v[j];
+        }
+    }
+};
 
 template <typename TIn>
 __device__ __forceinline__ float dot16(const uint4& x, const uint4& y, float s) {
@@ -264,277 +334,275 @@ __device__ __forceinline__ float dot16(const uint4& x, const uint4& y, float s) 
     return s;
 }
 
-__device__ __forceinline__ void store_gate(void* p, int64_t i, int f32, float x) {
-    if (f32)
-        static_cast<float*>(p)[i] = x;
-    else
-        static_cast<bf16_t*>(p)[i] = f32_to_bf16(x);
+// What a workgroup does between two barriers: a slice of the value columns of a
+// stream in a chunk.  Only live ones are taken: the walk wrote the zeros of the rest.
+struct GradUnit {
+    int item, nk, c, h, v0, live;  // item: key stream and chunk
+};
+__device__ __forceinline__ int live_rows(const DeltaArgs& a, int nk, int c, int h) {
+    const int64_t l = a.live.of(int64_t(nk) * a.group + h, a.T) - int64_t(c) * kChunk;
+    return l < 0 ? 0 : l < kChunk ? int(l) : kChunk;
+}
+// The next live stream of the unit's chunk or, past its last, of a chunk to come.
+__device__ __forceinline__ bool next_stream(const DeltaArgs& a, int items, GradUnit& u) {
+    u.v0 = 0;
+    while (true) {
+        if (++u.h >= a.group) {
+            u.h = 0;
+            u.item += gridDim.x;
+            if (u.item >= items) return false;
+            u.nk = unsigned(u.item) / unsigned(a.chunks), u.c = u.item - u.nk * a.chunks;
+        }
+        u.live = live_rows(a, u.nk, u.c, u.h);
+        if (u.live > 0) return true;
+    }
 }
 
-// A chunk of a key stream: eight waves, wave (th, dq) of 32 tokens and a quarter of
-// the key columns; of the 64 x 64 matrices 32 rows and 16 columns.
-template <typename TIn, int DK, bool kVec>
-__global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBwdArgs w) {
+// Wave (th, dq): TB blocks of 16 tokens and a quarter of the key columns; of the 64 x
+// 64 matrices its tokens' rows and 16 columns.  kShared: key streams with several
+// value streams, whose dQ and dK are summed in registers.
+template <typename TIn, int DK, bool kVec, bool kShared>
+__global__ __launch_bounds__(kGradThreads<TIn>) void delta_grads_kernel(const DeltaBwdArgs w, int items) {
     extern __shared__ __align__(16) unsigned char lds[];
-    __shared__ double G[kChunk];
-    __shared__ float beta[kChunk];
-    __shared__ float row_sum[4][kChunk], col_sum[2][kChunk], b_sum[2][kChunk], dots[3][4][kChunk], ss[8];
     const DeltaArgs& a = w.f;
     using L = GradLds<TIn, DK>;
     using Rows = Tile<TIn, DK>;
     using Square = Tile<TIn, 64>;
     using Out = Tile<TIn, L::SL>;
     using One = OneT<TIn>;
-    constexpr int NB = DK / 64, SL = L::SL;
-    const int64_t nkc = blockIdx.x, nk = nkc / a.chunks;
-    const int c = int(nkc - nk * a.chunks), t0 = c * kChunk;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-    const int th = wave >> 2, dq = wave & 3;
-    const int here = int(a.T - t0 < kChunk ? a.T - t0 : kChunk);  // rows of the chunk, live or not
-    int most = 0;
-    for (int h = 0; h < a.group; ++h) {
-        const int64_t l = a.live.of(nk * a.group + h, a.T) - t0;
-        most = max(most, int(l < kChunk ? l : kChunk));
-    }
-    if (most > 0) {
-        Stage<TIn, DK, kGradThreads, kVec> sk, sq;
-        sk.init(a.kt, a.dk);
-        sq.init(a.qt, a.dk);
-        sk.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, most, a.dk);
-        sq.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, most, a.dk);
-        sk.put(lds + L::kK);
-        sq.put(lds + L::kQ);
-    }
-    const int k_col = Rows::column_base(lr, g), s_col = Square::column_base(lr, g), o_row = Out::row_base(lr, g);
-    const int k_row = Rows::row_base(lr, g), s_row = Square::row_base(lr, g);
-    f32x4 gq[2][NB], gk[2][NB];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) gq[i][b] = gk[i][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int NB = DK / 64, SL = L::SL, NT = kGradThreads<TIn>, NW = NT / 64, TB = 16 / NW;
+    double* G = reinterpret_cast<double*>(lds + L::kSums);
+    float* beta = reinterpret_cast<float*>(G + kChunk);
+    float* row_sum = beta + kChunk;         // [4][64]
+    float* col_sum = row_sum + 4 * kChunk;  // [4 / TB][64]
+    float* b_sum = col_sum + 4 * kChunk;    // [4 / TB][64]
+    float* dots = b_sum + 4 * kChunk;       // [2][4][64]
+    float* ss = dots + 8 * kChunk;          // [NW]
+    int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), th = wave >> 2, dq = wave & 3;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-    for (int h = 0; h < a.group; ++h) {
-        const int64_t n = nk * a.group + h, len = a.live.of(n, a.T), nc = n * a.chunks + c;
-        const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
-        TIn* dv = w.dv ? static_cast<TIn*>(w.dv) + (n * a.T + t0) * a.dv : nullptr;
-        if (live <= 0) {
-            if (dv)
-                for (int i = threadIdx.x; i < here * a.dv; i += kGradThreads) store_val(dv + i, 0.f);
-            if (int(threadIdx.x) < here) {
-                if (w.dgate) store_gate(w.dgate, n * a.T + t0 + threadIdx.x, a.gate_f32, 0.f);
-                if (w.dbeta) store_gate(w.dbeta, n * a.T + t0 + threadIdx.x, a.gate_f32, 0.f);
-            }
-            continue;
+    Pieces<TIn, DK, SL, NT> ps, pd;
+    Pieces<TIn, 64, SL, NT> py, pdd;
+    RowPieces<TIn, SL, NT, kVec> po;
+    RowPieces<TIn, DK, NT, kVec> pk, pq;
+    float pg = 0.f, pb = 0.f;
+    // The loads of a unit: its slice, with a stream's first the gates, with a chunk's first K and Q.
+    auto prefetch = [&](const GradUnit& u, bool new_item) {
+        const int lane = tid & 63;
+        const int64_t nk = u.nk, n = nk * a.group + u.h;
+        const int rows = min(SL, a.dvp - u.v0);
+        const int64_t t0 = int64_t(u.c) * kChunk, slice = (n * a.chunks + u.c) * a.dvp + u.v0;
+        if (new_item) {
+            int most = u.live;  // of the chunk's first live stream, and of those after it
+            for (int h = u.h + 1; a.live.lengths && h < a.group; ++h) most = max(most, live_rows(a, u.nk, u.c, h));
+            pk.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, most, a.dk, tid);
+            pq.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, most, a.dk, tid);
         }
-        __syncthreads();  // K and Q are there; the stream before is done with the tiles and the sums
-        if (wave == 0) {
+        if (u.v0 == 0 && wave == 0) {
             const int64_t at = n * a.T + t0 + lane;
-            double s = lane < live && a.gate ? double(log_decay(gate_value(a.gate, at, a.gate_f32), a.form)) * kLog2e : 0.0;
-            for (int d = 1; d < 64; d <<= 1) {
-                const double o = __shfl_up(s, d);
-                if (lane >= d) s += o;
-            }
-            G[lane] = s;
-            beta[lane] = lane < live ? gate_value(a.beta, at, a.gate_f32) : 0.f;
+            pg = lane < u.live && a.gate ? gate_value(a.gate, at, a.gate_f32) : 0.f;
+            pb = lane < u.live ? gate_value(a.beta, at, a.gate_f32) : 0.f;
         }
-        f32x4 P[2], H[2], qs[2][NB], fs[2][NB], zs[2][NB];
+        ps.load(static_cast<const TIn*>(a.st) + slice * DK, rows, tid);
+        pd.load(static_cast<const TIn*>(w.ds) + slice * DK, rows, tid);
+        py.load(static_cast<const TIn*>(a.yt) + slice * kChunk, rows, tid);
+        pdd.load(static_cast<const TIn*>(w.dd) + slice * kChunk, rows, tid);
+        po.load(static_cast<const TIn*>(w.dout) + (n * a.T + t0) * a.dv + u.v0, a.dv, u.live, a.dv - u.v0, tid);
+    };
+
+    GradUnit u = {int(blockIdx.x) - int(gridDim.x), 0, 0, a.group, 0, 0};
+    if (!next_stream(a, items, u)) return;
+    bool new_item = true, more = true;
+    prefetch(u, true);
+    f32x4 gq[TB][NB], gk[TB][NB];
+    f32x4 P[TB], H[TB], qs[TB][NB], fs[TB][NB], zs[TB][NB];
+    float s_ds = 0.f, gate = 0.f;
+    while (more) {
+        // A new value each time round, as far as the compiler knows: it would keep every address made of it.
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63, g = lane >> 4, lr = lane & 15;
+        const int k_col = Rows::column_base(lr, g), s_col = Square::column_base(lr, g), o_row = Out::row_base(lr, g);
+        const int k_row = Rows::row_base(lr, g), s_row = Square::row_base(lr, g);
+        const bool first = u.v0 == 0;
+        const int64_t nk = u.nk, n = nk * a.group + u.h, t0 = int64_t(u.c) * kChunk;
+        const int live = u.live, here = int(a.T - t0 < kChunk ? a.T - t0 : kChunk), v0 = u.v0;
+        __syncthreads();  // the unit before is done with the LDS
+        if (new_item) {
+            pk.put(lds + L::kK, tid);
+            pq.put(lds + L::kQ, tid);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            P[i] = H[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < TB; ++i)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) qs[i][b] = fs[i][b] = zs[i][b] = P[i];
+                for (int b = 0; b < NB; ++b) gq[i][b] = gk[i][b] = zero;
         }
-        float s_ds = 0.f;
-        for (int v0 = 0; v0 < a.dv; v0 += SL) {
-            if (v0 > 0) __syncthreads();  // the slice before is read
-            const int rows = min(SL, a.dvp - v0);
-            {
-                constexpr int kCk = Rows::kChunks;
-                const uint4* sp = reinterpret_cast<const uint4*>(static_cast<const TIn*>(a.st) + (nc * a.dvp + v0) * DK);
-                const uint4* dp = reinterpret_cast<const uint4*>(static_cast<const TIn*>(w.ds) + (nc * a.dvp + v0) * DK);
-#pragma unroll
-                for (int i = 0; i < SL * kCk / kGradThreads; ++i) {
-                    const int q = int(threadIdx.x) + i * kGradThreads, row = q / kCk, u = q % kCk;
-                    uint4 x = make_uint4(0, 0, 0, 0), y = x;
-                    if (row < rows) x = sp[q], y = dp[q];
-                    s_ds = dot16<TIn>(x, y, s_ds);
-                    *reinterpret_cast<uint4*>(lds + L::kSt + Rows::at(row, u)) = x;
-                    *reinterpret_cast<uint4*>(lds + L::kDs + Rows::at(row, u)) = y;
-                }
+        if (first) {
+            if (wave == 0) {
+                gate = pg;
+                const double s = lane < live && a.gate ? double(log_decay(pg, a.form)) * kLog2e : 0.0;
+                G[lane] = wave_scan(s);
+                beta[lane] = pb;
             }
-            stage_rows<TIn, 64, SL>(static_cast<const TIn*>(a.yt) + (nc * a.dvp + v0) * kChunk, rows, lds + L::kYt);
-            stage_rows<TIn, 64, SL>(static_cast<const TIn*>(w.dd) + (nc * a.dvp + v0) * kChunk, rows, lds + L::kDd);
-            {
-                const TIn* p = static_cast<const TIn*>(w.dout) + (n * a.T + t0) * a.dv + v0;
-                constexpr int kEights = SL / 8, kVecs = Eight<TIn>::kVecs;
-                const auto view = mfma::make_rsrc(p, ((live - 1) * int64_t(a.dv) + a.dv - v0) * int(sizeof(TIn)));
+            s_ds = 0.f;
 #pragma unroll
-                for (int i = 0; i < (kChunk * kEights + kGradThreads - 1) / kGradThreads; ++i) {
-                    const int q = int(threadIdx.x) + i * kGradThreads, row = q / kEights, u = q % kEights;
-                    if (kChunk * kEights < kGradThreads && q >= kChunk * kEights) break;
-                    Eight<TIn> x;
-                    if constexpr (kVec) {
+            for (int i = 0; i < TB; ++i) {
+                P[i] = H[i] = zero;
 #pragma unroll
-                        for (int j = 0; j < kVecs; ++j)
-                            x.v[j] = mfma::buf_load16<mfma::kPolicyDefault>(view, piece_at<TIn>(row, a.dv, 8 * u + 4 * j, a.dv - v0));
+                for (int b = 0; b < NB; ++b) qs[i][b] = fs[i][b] = zs[i][b] = zero;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < ps.kPer; ++i)
+            if (ps.kTotal % NT == 0 || tid + i * NT < ps.kTotal) s_ds = dot16<TIn>(ps.x[i], pd.x[i], s_ds);
+        ps.put(lds + L::kSt, tid);
+        pd.put(lds + L::kDs, tid);
+        py.put(lds + L::kYt, tid);
+        pdd.put(lds + L::kDd, tid);
+        po.put(lds + L::kO, tid);
+        GradUnit next = u;
+        next.v0 += SL;
+        const bool last = next.v0 >= a.dv;
+        more = !last || next_stream(a, items, next);
+        new_item = more && next.item != u.item;
+        const bool item_done = !more || new_item;
+        if (more) prefetch(next, new_item);
+        u = next;
+        __syncthreads();
+        TIn* dv = w.dv ? static_cast<TIn*>(w.dv) + (n * a.T + t0) * a.dv : nullptr;
+#pragma unroll
+        for (int kk = 0; kk < SL / 32; ++kk) {
+            const One yc = Square::transposed(lds + L::kYt, s_col, kk, dq);
+            One ya[TB], da[TB], oa[TB];
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                const int b = TB * th + i;
+                ya[i] = Square::transposed(lds + L::kYt, s_col, kk, b);
+                da[i] = Square::transposed(lds + L::kDd, s_col, kk, b);
+                oa[i] = Out::one(lds + L::kO, o_row, b, kk);
+                P[i] = mac(oa[i], yc, P[i]);
+                H[i] = mac(da[i], yc, H[i]);
+                // A token's dV: four waves hold the same rows, each writes every fourth run.
+                if (dv && ((v0 >> 5) + kk) % 4 == dq && tok(b, lr) < here) {
+                    const int cv = v0 + 32 * kk + 8 * g;
+                    TIn* o = dv + int64_t(tok(b, lr)) * a.dv + cv;
+                    if (kVec && cv + 8 <= a.dv) {
+                        store_run(o, da[i]);
                     } else {
-                        x.load(p + row * a.dv + 8 * u, row < live ? a.dv - v0 - 8 * u : 0);
-                    }
+                        const auto run = __builtin_bit_cast(Eight<TIn>, da[i]);
 #pragma unroll
-                    for (int j = 0; j < kVecs; ++j)
-                        *reinterpret_cast<uint4*>(lds + L::kO + Out::at(row, kVecs * u + j)) = x.v[j];
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < SL / 32; ++kk) {
-                const One yc = Square::transposed(lds + L::kYt, s_col, kk, dq);
-                One ya[2], da[2], oa[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int b = 2 * th + i;
-                    ya[i] = Square::transposed(lds + L::kYt, s_col, kk, b);
-                    da[i] = Square::transposed(lds + L::kDd, s_col, kk, b);
-                    oa[i] = Out::one(lds + L::kO, o_row, b, kk);
-                    P[i] = mac(oa[i], yc, P[i]);
-                    H[i] = mac(da[i], yc, H[i]);
-                    // A token's dV: these waves hold the same rows, each writes every fourth run.
-                    if (dv && ((v0 >> 5) + kk) % 4 == dq && tok(b, lr) < here) {
-                        const int cv = v0 + 32 * kk + 8 * g;
-                        TIn* o = dv + int64_t(tok(b, lr)) * a.dv + cv;
-                        if (kVec && cv + 8 <= a.dv) {
-                            store_run(o, da[i]);
-                        } else {
-                            const auto run = __builtin_bit_cast(Eight<TIn>, da[i]);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                constexpr int kPer = 16 / int(sizeof(TIn));
-                                if (cv + e < a.dv) store_val(o + e, mfma::Elem<TIn>::get(run.v[e / kPer], e % kPer));
-                            }
+                        for (int e = 0; e < 8; ++e) {
+                            constexpr int kPer = 16 / int(sizeof(TIn));
+                            if (cv + e < a.dv) store_val(o + e, mfma::Elem<TIn>::get(run.v[e / kPer], e % kPer));
                         }
                     }
                 }
+            }
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const One st = Rows::transposed(lds + L::kSt, k_col, kk, dq * NB + b);
-                    const One ds = Rows::transposed(lds + L::kDs, k_col, kk, dq * NB + b);
+            for (int b = 0; b < NB; ++b) {
+                const One st = Rows::transposed(lds + L::kSt, k_col, kk, dq * NB + b);
+                const One ds = Rows::transposed(lds + L::kDs, k_col, kk, dq * NB + b);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        qs[i][b] = mac(st, oa[i], qs[i][b]);
-                        fs[i][b] = mac(st, da[i], fs[i][b]);
-                        zs[i][b] = mac(ds, ya[i], zs[i][b]);
-                    }
+                for (int i = 0; i < TB; ++i) {
+                    qs[i][b] = mac(st, oa[i], qs[i][b]);
+                    fs[i][b] = mac(st, da[i], fs[i][b]);
+                    zs[i][b] = mac(ds, ya[i], zs[i][b]);
                 }
             }
         }
-        // Rows tok(2 th + i, 4 g + r), column tok(dq, lr) of the 64 x 64 matrices.
+        if (!last) continue;
+        // Rows tok(TB th + i, 4 g + r), column tok(dq, lr) of the 64 x 64 matrices.
         const int jc = tok(dq, lr);
-        const float bj = beta[jc];
-        const double Gj = G[jc];
-        float in_row[2][4], in_col = 0.f, in_b = 0.f;
-        f32x4 Lm[2], Xm[2];
+        {
+            const float bj = beta[jc];
+            const double Gj = G[jc];
+            float in_col = 0.f, in_b = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            f32x4 qk = {0.f, 0.f, 0.f, 0.f}, kk = qk;
+            for (int i = 0; i < TB; ++i) {
+                f32x4 qk = zero, kk = zero, Lm, Xm;
 #pragma unroll
-            for (int s = 0; s < DK / 32; ++s) {
-                const One kj = Rows::one(lds + L::kK, k_row, dq, s);
-                qk = mac(Rows::one(lds + L::kQ, k_row, 2 * th + i, s), kj, qk);
-                kk = mac(Rows::one(lds + L::kK, k_row, 2 * th + i, s), kj, kk);
+                for (int s = 0; s < DK / 32; ++s) {
+                    const One kj = Rows::one(lds + L::kK, k_row, dq, s);
+                    qk = mac(Rows::one(lds + L::kQ, k_row, TB * th + i, s), kj, qk);
+                    kk = mac(Rows::one(lds + L::kK, k_row, TB * th + i, s), kj, kk);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = tok(TB * th + i, 4 * g + r);
+                    const float e = row >= jc ? __builtin_amdgcn_exp2f(float(G[row] - Gj)) : 0.f;
+                    const float p = a.scale * e * P[i][r], hm = row > jc ? -e * H[i][r] : 0.f;
+                    Lm[r] = bj * p;
+                    Xm[r] = bj * hm;
+                    const float pair = fmaf(p, qk[r], hm * kk[r]);
+                    in_b += pair;
+                    in_col += bj * pair;
+                    const float in_row = row_scan(bj * pair);
+                    if (lr == 15) row_sum[dq * kChunk + row] = in_row;
+                }
+                const int at = Square::four_at(jc, tok(TB * th + i, 4 * g));
+                Square::put4(lds + L::kL, at, Lm);
+                Square::put4(lds + L::kX, at, Xm);
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = tok(2 * th + i, 4 * g + r);
-                const float e = row >= jc ? __builtin_amdgcn_exp2f(float(G[row] - Gj)) : 0.f;
-                const float p = a.scale * e * P[i][r], hm = row > jc ? -e * H[i][r] : 0.f;
-                Lm[i][r] = bj * p;
-                Xm[i][r] = bj * hm;
-                const float pair = fmaf(p, qk[r], hm * kk[r]);
-                in_b += pair;
-                in_row[i][r] = bj * pair;
-                in_col += bj * pair;
-            }
+            in_col += __shfl_xor(in_col, 16);
+            in_col += __shfl_xor(in_col, 32);
+            in_b += __shfl_xor(in_b, 16);
+            in_b += __shfl_xor(in_b, 32);
+            if (g == 0) col_sum[th * kChunk + jc] = in_col, b_sum[th * kChunk + jc] = in_b;
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                for (int d = 1; d < 16; d <<= 1) in_row[i][r] += __shfl_xor(in_row[i][r], d);
-                if (lr == 0) row_sum[dq][tok(2 * th + i, 4 * g + r)] = in_row[i][r];
-            }
-        in_col += __shfl_xor(in_col, 16);
-        in_col += __shfl_xor(in_col, 32);
-        in_b += __shfl_xor(in_b, 16);
-        in_b += __shfl_xor(in_b, 32);
-        if (g == 0) col_sum[th][jc] = in_col, b_sum[th][jc] = in_b;
-        for (int d = 1; d < 64; d <<= 1) s_ds += __shfl_xor(s_ds, d);
+        s_ds = wave_sum(s_ds);
         if (lane == 0) ss[wave] = s_ds;
         // What comes from the states, by rows: a token a lane, its key columns in registers.
-        const double last = G[63];
+        const double end = G[63];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = tok(2 * th + i, lr);
-            const float e = __builtin_amdgcn_exp2f(float(G[row])), z = __builtin_amdgcn_exp2f(float(last - G[row]));
-            float dot[3] = {0.f, 0.f, 0.f};
+        for (int i = 0; i < TB; ++i) {
+            const int row = tok(TB * th + i, lr);
+            const float e = __builtin_amdgcn_exp2f(float(G[row])), z = __builtin_amdgcn_exp2f(float(end - G[row]));
+            const float b_row = beta[row];
+            float from_s = 0.f, from_z = 0.f;  // of E q.(S dO) - E k.(S dD), and of Z k.(dS' Y)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const int cd = tok(dq * NB + b, 4 * g);
-                const int at = Rows::four_at(row, cd);
+                const int at = Rows::four_at(row, tok(dq * NB + b, 4 * g));
                 const f32x4 q4 = Rows::four(lds + L::kQ, at), k4 = Rows::four(lds + L::kK, at);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float qv = qs[i][b][r] * (e * a.scale), fv = fs[i][b][r] * e, zv = zs[i][b][r] * z;
-                    dot[0] = fmaf(q4[r], qv, dot[0]);
-                    dot[1] = fmaf(k4[r], fv, dot[1]);
-                    dot[2] = fmaf(k4[r], zv, dot[2]);
-                    gq[i][b][r] += qv;
-                    gk[i][b][r] += beta[row] * zv - fv;
+                    from_s = fmaf(q4[r], qv, fmaf(-k4[r], fv, from_s));
+                    from_z = fmaf(k4[r], zv, from_z);
+                    if constexpr (kShared) {
+                        gq[i][b][r] += qv;
+                        gk[i][b][r] += fmaf(b_row, zv, -fv);
+                    } else {
+                        gq[i][b][r] = qv;
+                        gk[i][b][r] = fmaf(b_row, zv, -fv);
+                    }
                 }
             }
-#pragma unroll
-            for (int x = 0; x < 3; ++x) {
-                dot[x] += __shfl_xor(dot[x], 16);
-                dot[x] += __shfl_xor(dot[x], 32);
-                if (g == 0) dots[x][dq][row] = dot[x];
-            }
-        }
-        __syncthreads();  // the slices of S and dS' are read
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int at = Square::four_at(jc, tok(2 * th + i, 4 * g));
-            Square::put4(lds + L::kL, at, Lm[i]);
-            Square::put4(lds + L::kX, at, Xm[i]);
+            from_s += __shfl_xor(from_s, 16);
+            from_s += __shfl_xor(from_s, 32);
+            from_z += __shfl_xor(from_z, 16);
+            from_z += __shfl_xor(from_z, 32);
+            if (g == 0) dots[dq * kChunk + row] = from_s, dots[(4 + dq) * kChunk + row] = from_z;
         }
         __syncthreads();
         if (wave == 0 && (w.dgate || w.dbeta)) {
-            const float z = dots[2][0][lane] + dots[2][1][lane] + dots[2][2][lane] + dots[2][3][lane];
             const int64_t at = n * a.T + t0 + lane;
-            if (w.dbeta && lane < here)
-                store_gate(w.dbeta, at, a.gate_f32, lane < live ? b_sum[0][lane] + b_sum[1][lane] + z : 0.f);
+            float z = 0.f, cols = 0.f, bs = 0.f;
+            double dg = 0.0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                z += dots[(4 + x) * kChunk + lane];
+                dg += double(row_sum[x * kChunk + lane]) + dots[x * kChunk + lane];
+            }
+#pragma unroll
+            for (int x = 0; x < 4 / TB; ++x) cols += col_sum[x * kChunk + lane], bs += b_sum[x * kChunk + lane];
+            if (w.dbeta && lane < here) store_gate(w.dbeta, at, a.gate_f32, lane < live ? bs + z : 0.f);
             if (w.dgate) {
                 const float bz = beta[lane] * z;
-                double all = bz;
-                for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
-                float s = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s += ss[i];
-                double dg = -double(bz);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) dg += double(row_sum[x][lane]) + dots[0][x][lane] - dots[1][x][lane];
-                dg -= double(col_sum[0][lane]) + col_sum[1][lane];
-                if (lane == 63) dg += all + double(__builtin_amdgcn_exp2f(float(last))) * s;
-                for (int d = 1; d < 64; d <<= 1) {
-                    const double o = __shfl_down(dg, d);
-                    if (lane + d < 64) dg += o;
-                }
-                float x = 0.f;
-                if (lane < live) {
-                    const float gv = gate_value(a.gate, at, a.gate_f32);
-                    const bool lowest = log_decay(gv, a.form) <= kLowestLog;  // constant there
-                    x = lowest ? 0.f : float(dg);
-                    if (a.form == RACE_GATE_SIGMOID) x *= 1.f / (1.f + expf(gv));
-                }
+                const float behind = wave_sum(bz) + __builtin_amdgcn_exp2f(float(end)) * wave_sum(lane < NW ? ss[lane] : 0.f);
+                dg -= double(bz) + cols;
+                dg = wave_scan(__shfl(dg, 63 - lane));
+                dg = __shfl(dg, 63 - lane) + behind;
+                float x = lane < live && log_decay(gate, a.form) > kLowestLog ? float(dg) : 0.f;  // constant below
+                if (a.form == RACE_GATE_SIGMOID) x *= 1.f / (1.f + expf(gate));
                 if (lane < here) store_gate(w.dgate, at, a.gate_f32, x);
             }
         }
@@ -542,51 +610,54 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int b = 2 * th + i;
+            for (int i = 0; i < TB; ++i) {
+                const int b = TB * th + i;
+                const bool low = kk <= (b >> 1), high = kk >= (b >> 1);
                 One l, lt, x, xt;
-                if (kk <= th) {
+                if (low) {
                     l = Square::transposed(lds + L::kL, s_col, kk, b);
                     x = Square::transposed(lds + L::kX, s_col, kk, b);
                 }
-                if (kk >= th) {
+                if (high) {
                     lt = Square::one(lds + L::kL, s_row, b, kk);
                     xt = Square::one(lds + L::kX, s_row, b, kk);
                 }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     const One kf = Rows::transposed(lds + L::kK, k_col, kk, dq * NB + nb);
-                    if (kk <= th) {
+                    if (low) {
                         gq[i][nb] = mac(kf, l, gq[i][nb]);
                         gk[i][nb] = mac(kf, x, gk[i][nb]);
                     }
-                    if (kk >= th) {
+                    if (high) {
                         gk[i][nb] = mac(kf, xt, gk[i][nb]);
                         gk[i][nb] = mac(Rows::transposed(lds + L::kQ, k_col, kk, dq * NB + nb), lt, gk[i][nb]);
                     }
                 }
             }
         }
-    }
+        if (kShared && !item_done) continue;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = tok(2 * th + i, lr);
-        if (row >= here) continue;
+        for (int i = 0; i < TB; ++i) {
+            const int row = tok(TB * th + i, lr);
+            if (row >= here) continue;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int cd = tok(dq * NB + b, 4 * g), there = a.dk - cd;
-            if (there <= 0) continue;
-            const int64_t at = (nk * a.T + t0 + row) * a.dk + cd;
-            for (int x = 0; x < 2; ++x) {
-                TIn* p = static_cast<TIn*>(x ? w.dk : w.dq);
-                if (!p) continue;
-                const f32x4 v = x ? gk[i][b] : gq[i][b];
-                if (a.dk % 4 == 0) {
-                    store4_of(p + at, v);
-                } else {
+            for (int b = 0; b < NB; ++b) {
+                const int cd = tok(dq * NB + b, 4 * g), there = a.dk - cd;
+                if (there <= 0) continue;
+                const int64_t at = (nk * a.T + t0 + row) * a.dk + cd;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (r < there) store_val(p + at + r, v[r]);
+                for (int x = 0; x < 2; ++x) {
+                    TIn* p = static_cast<TIn*>(x ? w.dk : w.dq);
+                    if (!p) continue;
+                    const f32x4 v = x ? gk[i][b] : gq[i][b];
+                    if (kVec) {
+                        store4_of(p + at, v);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (r < there) store_val(p + at + r, v[r]);
+                    }
                 }
             }
         }
@@ -597,13 +668,18 @@ template <typename TIn, int DK, bool kVec>
 hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
     using L = ChunkLds<TIn, DK>;
     constexpr int walk = L::kBuffers * L::kBytes, grads = GradLds<TIn, DK>::kBytes;
-    static_assert(walk <= kGfx950LdsBytes && grads + 8192 <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
+    static_assert(walk <= kGfx950LdsBytes && grads <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
     const int64_t blocks = (r.dv + 63) / 64;
     delta_bwd_walk_kernel<TIn, DK, kVec><<<unsigned((r.N + 7) / 8 * 8 * blocks), kThreads, walk, stream>>>(w);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (!w.dq && !w.dk && !w.dv && !w.dgate && !w.dbeta) return hipSuccess;
-    delta_grads_kernel<TIn, DK, kVec><<<unsigned(r.Nk * w.f.chunks), kGradThreads, grads, stream>>>(w);
+    const int items = int(r.Nk * w.f.chunks);
+    const unsigned grid = unsigned(items < kGradWorkgroups ? items : kGradWorkgroups);
+    if (w.f.group > 1 || !kVec)
+        delta_grads_kernel<TIn, DK, kVec, true><<<grid, kGradThreads<TIn>, grads, stream>>>(w, items);
+    else
+        delta_grads_kernel<TIn, DK, kVec, kVec ? false : true><<<grid, kGradThreads<TIn>, grads, stream>>>(w, items);
     return hipGetLastError();
 }
 

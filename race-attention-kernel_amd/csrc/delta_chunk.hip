@@ -83,10 +83,7 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
         if (wave == 0) {
             const int64_t at = n * a.T + t0 + lane;
             double s = lane < live && a.gate ? double(log_decay(gate_value(a.gate, at, a.gate_f32), a.form)) * kLog2e : 0.0;
-            for (int d = 1; d < 64; d <<= 1) {
-                const double o = __shfl_up(s, d);
-                if (lane >= d) s += o;
-            }
+            s = wave_scan(s);
             G[lane] = s;
             const float bv = lane < live ? gate_value(a.beta, at, a.gate_f32) : 0.f;
             b[lane] = bv;

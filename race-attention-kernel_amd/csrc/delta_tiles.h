@@ -117,6 +117,37 @@ __device__ __forceinline__ void store_run(float* p, const OneT<float>& x) {
 // are issued before the products of the stage before it.
 __device__ __forceinline__ void stage_wall() { __builtin_amdgcn_sched_barrier(0); }
 
+// ---- sums over lanes, by data-parallel moves within the vector ALU ----
+
+template <int kCtrl, int kRows>
+__device__ __forceinline__ float moved(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), kCtrl, kRows, 0xf, true));
+}
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double moved(double x) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), kCtrl, kRows, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), kCtrl, kRows, 0xf, true);
+    return __hiloint2double(hi, lo);
+}
+// Over the 16 lanes of a row so far: lane 15 of each has its sum.
+template <typename F>
+__device__ __forceinline__ F row_scan(F x) {
+    x += moved<0x111, 0xf>(x);  // shifts by 1, 2, 4 and 8 lanes, zeros from outside
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    return x + moved<0x118, 0xf>(x);
+}
+// Inclusive, over the 64 lanes: then the last lanes of the rows and halves before.
+template <typename F>
+__device__ __forceinline__ F wave_scan(F x) {
+    x = row_scan(x);
+    x += moved<0x142, 0xa>(x);
+    return x + moved<0x143, 0xc>(x);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wave_scan(x)), 63));
+}
+
 // ---- tiles ----
 
 // Offsets come in two parts: a lane's own (`..._base`, the same for every chunk)
