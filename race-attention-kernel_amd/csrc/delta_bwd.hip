@@ -256,12 +256,11 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 // 8 x 16 streams of 4096 tokens 700 us.)
 constexpr int kGradWorkgroups = 256;
 
-// Columns of the state a step takes (fp32: half as many, for the LDS), and threads:
-// 16 waves of bf16 rows; fp32 fragments take twice the registers.
+// Columns of the state a step takes (fp32: half as many, for the LDS), and threads
+// (1024 have 128 registers each: the rows on their way spilled, 669 us for 496).
 template <typename TIn>
 constexpr int kSlice = sizeof(TIn) == 2 ? 64 : 32;
-template <typename TIn>
-constexpr int kGradThreads = sizeof(TIn) == 2 ? 1024 : 512;
+constexpr int kGradThreads = 512;
 
 template <typename TIn, int DK>
 struct GradLds {
@@ -362,7 +361,7 @@ __device__ __forceinline__ bool next_stream(const DeltaArgs& a, int items, GradU
 // 64 matrices its tokens' rows and 16 columns.  kShared: key streams with several
 // value streams, whose dQ and dK are summed in registers.
 template <typename TIn, int DK, bool kVec, bool kShared>
-__global__ __launch_bounds__(kGradThreads<TIn>) void delta_grads_kernel(const DeltaBwdArgs w, int items) {
+__global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBwdArgs w, int items) {
     extern __shared__ __align__(16) unsigned char lds[];
     const DeltaArgs& a = w.f;
     using L = GradLds<TIn, DK>;
@@ -370,7 +369,7 @@ __global__ __launch_bounds__(kGradThreads<TIn>) void delta_grads_kernel(const De
     using Square = Tile<TIn, 64>;
     using Out = Tile<TIn, L::SL>;
     using One = OneT<TIn>;
-    constexpr int NB = DK / 64, SL = L::SL, NT = kGradThreads<TIn>, NW = NT / 64, TB = 16 / NW;
+    constexpr int NB = DK / 64, SL = L::SL, NT = kGradThreads, NW = NT / 64, TB = 16 / NW;
     double* G = reinterpret_cast<double*>(lds + L::kSums);
     float* beta = reinterpret_cast<float*>(G + kChunk);
     float* row_sum = beta + kChunk;         // [4][64]
@@ -386,7 +385,7 @@ __global__ __launch_bounds__(kGradThreads<TIn>) void delta_grads_kernel(const De
     Pieces<TIn, 64, SL, NT> py, pdd;
     RowPieces<TIn, SL, NT, kVec> po;
     RowPieces<TIn, DK, NT, kVec> pk, pq;
-    float pg = 0.f, pb = 0.f;
+    uint32_t pg = 0, pb = 0;
     // The loads of a unit: its slice, with a stream's first the gates, with a chunk's first K and Q.
     auto prefetch = [&](const GradUnit& u, bool new_item) {
         const int lane = tid & 63;
@@ -401,8 +400,11 @@ __global__ __launch_bounds__(kGradThreads<TIn>) void delta_grads_kernel(const De
         }
         if (u.v0 == 0 && wave == 0) {
             const int64_t at = n * a.T + t0 + lane;
-            pg = lane < u.live && a.gate ? gate_value(a.gate, at, a.gate_f32) : 0.f;
-            pb = lane < u.live ? gate_value(a.beta, at, a.gate_f32) : 0.f;
+            pg = pb = 0;
+            if (lane < u.live) {
+                if (a.gate) pg = gate_bits(a.gate, at, a.gate_f32);
+                pb = gate_bits(a.beta, at, a.gate_f32);
+            }
         }
         ps.load(static_cast<const TIn*>(a.st) + slice * DK, rows, tid);
         pd.load(static_cast<const TIn*>(w.ds) + slice * DK, rows, tid);
@@ -438,10 +440,10 @@ __global__ __launch_bounds__(kGradThreads<TIn>) void delta_grads_kernel(const De
         }
         if (first) {
             if (wave == 0) {
-                gate = pg;
-                const double s = lane < live && a.gate ? double(log_decay(pg, a.form)) * kLog2e : 0.0;
+                gate = gate_of(pg, a.gate_f32);
+                const double s = lane < live && a.gate ? double(log_decay(gate, a.form)) * kLog2e : 0.0;
                 G[lane] = wave_scan(s);
-                beta[lane] = pb;
+                beta[lane] = gate_of(pb, a.gate_f32);
             }
             s_ds = 0.f;
 #pragma unroll
@@ -677,9 +679,9 @@ hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_
     const int items = int(r.Nk * w.f.chunks);
     const unsigned grid = unsigned(items < kGradWorkgroups ? items : kGradWorkgroups);
     if (w.f.group > 1 || !kVec)
-        delta_grads_kernel<TIn, DK, kVec, true><<<grid, kGradThreads<TIn>, grads, stream>>>(w, items);
+        delta_grads_kernel<TIn, DK, kVec, true><<<grid, kGradThreads, grads, stream>>>(w, items);
     else
-        delta_grads_kernel<TIn, DK, kVec, kVec ? false : true><<<grid, kGradThreads<TIn>, grads, stream>>>(w, items);
+        delta_grads_kernel<TIn, DK, kVec, kVec ? false : true><<<grid, kGradThreads, grads, stream>>>(w, items);
     return hipGetLastError();
 }
 

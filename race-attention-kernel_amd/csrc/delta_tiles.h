@@ -402,6 +402,11 @@ constexpr float kLowestLog = -200.f;
 __device__ __forceinline__ float gate_value(const void* p, int64_t i, int f32) {
     return f32 ? static_cast<const float*>(p)[i] : to_f32(static_cast<const bf16_t*>(p)[i]);
 }
+// In two steps, for a load that is on its way while other things go on.
+__device__ __forceinline__ uint32_t gate_bits(const void* p, int64_t i, int f32) {
+    return f32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float gate_of(uint32_t bits, int f32) { return __uint_as_float(f32 ? bits : bits << 16); }
 __device__ __forceinline__ float log_decay(float g, int form) {
     const float l = form == RACE_GATE_LOG ? g : fminf(g, 0.f) - log1pf(expf(-fabsf(g)));
     return l < kLowestLog ? kLowestLog : l;
