@@ -682,9 +682,10 @@ typedef struct race_delta_shape {
  * launch and need no workspace. */
 #define RACE_DELTA_STEP_TOKENS 16
 
-/* Workspace of race_delta_fwd in bytes (0 with records), and the bytes of the
- * records (nullable) race_delta_bwd reads. */
-race_status race_delta_fwd_workspace_bytes(const race_delta_shape* shape, size_t* bytes, size_t* record_bytes);
+/* Workspace of race_delta_fwd in bytes, with or without records, and the bytes of
+ * the records (nullable) race_delta_bwd reads. */
+race_status race_delta_fwd_workspace_bytes(const race_delta_shape* shape, int32_t with_records, size_t* bytes,
+                                           size_t* record_bytes);
 
 /* out [value_streams][seq_len][value_dim] and, with final_state (nullable), the
  * state after the last token.  gate (nullable) and beta: [value_streams][seq_len].

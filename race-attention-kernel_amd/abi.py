@@ -283,7 +283,7 @@ def lib() -> ctypes.CDLL:
         L.race_gated_scan_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
         L.race_gated_scan_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, sc, vp, sz, vp]
         dl = ctypes.POINTER(RaceDeltaShape)
-        L.race_delta_fwd_workspace_bytes.argtypes = [dl, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        L.race_delta_fwd_workspace_bytes.argtypes = [dl, i32, ctypes.POINTER(sz), ctypes.POINTER(sz)]
         L.race_delta_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, dl, vp, sz, vp]
         L.race_delta_bwd_workspace_bytes.argtypes = [dl, ctypes.POINTER(sz)]
         L.race_delta_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, dl, vp, sz, vp]
@@ -655,10 +655,10 @@ def delta_shape(N: int, T: int, dk: int, dv: int, *, key_streams: int | None = N
                           scale, (ctypes.c_int64 * 6)(*(strides or (T * dk, dk, T * dk, dk, T * dv, dv))))
 
 
-def delta_workspace_bytes(sh: RaceDeltaShape):
+def delta_workspace_bytes(sh: RaceDeltaShape, with_records: bool = False):
     """(status, bytes, record_bytes) of race_delta_fwd."""
     b, r = ctypes.c_size_t(0), ctypes.c_size_t(0)
-    st = lib().race_delta_fwd_workspace_bytes(ctypes.byref(sh), ctypes.byref(b), ctypes.byref(r))
+    st = lib().race_delta_fwd_workspace_bytes(ctypes.byref(sh), int(with_records), ctypes.byref(b), ctypes.byref(r))
     return st, b.value, r.value
 
 

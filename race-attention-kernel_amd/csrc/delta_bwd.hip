@@ -72,13 +72,16 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
     const TIn* op = static_cast<const TIn*>(w.dout) + n * a.T * a.dv + cb * 64;
 
     f32x4 dS[DK / 16];
+    if (w.dfinal) {
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i)
+        for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = tok(i, 4 * g + r);
-            dS[i][r] = w.dfinal && active && row < a.dk && col < a.dv ? w.dfinal[(n * a.dk + row) * a.dv + col] : 0.f;
-        }
+            for (int r = 0; r < 4; ++r)
+                dS[i][r] = state_value(w.dfinal + n * a.dk * a.dv, tok(i, 4 * g + r), col, a.dk, a.dv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) dS[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 
     Stage<TIn, DK, kThreads, kVec> sk, sq;
     StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;

@@ -23,6 +23,8 @@
 // three roundings of an output.  Log decays are summed in 64 bits: differences of
 // long sums lose the digits the products keep.
 // A few tokens (decode) go token by token in 32 bits: delta_step_kernel.
+#include <algorithm>
+
 #include "delta_tiles.h"
 
 namespace race {
@@ -202,7 +204,13 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
 
 // ---- the walk over a stream's chunks ----
 
-template <typename TIn, int DK, bool kVec, bool kRecords>
+// What a walk leaves: outputs; outputs and the records of a backward; or, in place
+// of outputs, what its segment does to a state: columns of the identity (with
+// values of zero) beside those of the values (from zero, the first segment's from
+// its state).
+enum WalkMode { kOutputs, kRecording, kMaps };
+
+template <typename TIn, int DK, bool kVec, WalkMode kMode>
 __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a) {
     extern __shared__ __align__(16) unsigned char lds[];
     using L = ChunkLds<TIn, DK>;
@@ -211,28 +219,43 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
     using One = OneT<TIn>;
     using Two = TwoT<TIn>;
     constexpr int NS = DK / 32;
-    int64_t n;
+    const int value_blocks = (a.dv + 63) / 64, blocks = value_blocks + (kMode == kMaps ? (a.dk + 63) / 64 : 0);
+    const int walks = kMode == kMaps ? a.segs - 1 : a.segs;  // no state follows the last segment's
+    int64_t ns;
     int cb;
-    if (!stream_and_block(a.N, (a.dv + 63) / 64, n, cb)) return;
+    if (!stream_and_block(a.N * walks, blocks, ns, cb)) return;
+    const int64_t n = unsigned(ns) / unsigned(walks);
+    const int seg = int(ns - n * walks);
+    const bool unit = kMode == kMaps && cb >= value_blocks;
+    if (unit && seg == 0) return;  // its start is known
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
     const bool odd = g & 1;
-    const int c0 = cb * 64 + wave * 16, col = c0 + lr;
-    const bool active = c0 < a.dv;
+    const int width = unit ? a.dk : a.dv, values = unit ? 0 : a.dv - cb * 64;
+    const int c0 = (unit ? cb - value_blocks : cb) * 64 + wave * 16, col = c0 + lr;
+    const bool active = c0 < width;
     const int64_t nk = n / a.group, len = a.live.of(n, a.T);
-    const int chunks = int((len + kChunk - 1) / kChunk);
+    const int all = int((len + kChunk - 1) / kChunk);
+    const int from = min(seg * a.seg_chunks, all), chunks = min(from + a.seg_chunks, all);
     const TIn* kp = static_cast<const TIn*>(a.k) + nk * a.kn;
     const TIn* qp = static_cast<const TIn*>(a.q) + nk * a.qn;
-    const TIn* vp = static_cast<const TIn*>(a.v) + n * a.vn + cb * 64;
+    const TIn* vp = static_cast<const TIn*>(a.v) + n * a.vn + (unit ? 0 : cb * 64);
     TIn* op = static_cast<TIn*>(a.out) + n * a.T * a.dv;
+    const float* start = kMode != kMaps && a.starts ? a.starts + ns * a.dk * a.dv
+                         : a.state && seg == 0      ? a.state + n * a.dk * a.dv
+                                                    : nullptr;
 
     f32x4 S[DK / 16];
+    if (start && !unit) {
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i)
+        for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = tok(i, 4 * g + r);
-            S[i][r] = a.state && active && row < a.dk && col < a.dv ? a.state[(n * a.dk + row) * a.dv + col] : 0.f;
-        }
+            for (int r = 0; r < 4; ++r) S[i][r] = state_value(start, tok(i, 4 * g + r), col, a.dk, a.dv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[i][r] = unit && tok(i, 4 * g + r) == col ? 1.f : 0.f;
+    }
 
     Stage<TIn, DK, kThreads, kVec> sk, sq;
     StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;
@@ -241,32 +264,32 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
     float svec;
     sk.init(a.kt, a.dk);
     sq.init(a.qt, a.dk);
-    sv.init(a.vt, a.dv - cb * 64);
+    sv.init(a.vt, values);
     // A chunk's loads, in four parts: all at once they fill the queue, and the wave waits to issue them.
     auto fetch = [&](int c, int part) {
         const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
         if (part == 0) sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
-        if (part == 1) sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
+        if (part == 1 && kMode != kMaps) sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
         if (part == 2) stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
         if (part == 3) {
-            smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
-            sv.load(vp + t0 * a.vt, a.vt, live, a.dv - cb * 64);
+            if (kMode != kMaps) smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
+            sv.load(vp + t0 * a.vt, a.vt, live, values);
             svec = a.vec[nc * 128 + (threadIdx.x & 127)];
         }
     };
     // What a lane adds to a tile's start.
     const int k_row = Rows::row_base(lr, g), k_col = Rows::column_base(lr, g), s_row = Square::row_base(lr, g);
     const int v_at = Square::block_base(16 * wave, lr, g);
-    if (chunks > 0)
-        for (int p = 0; p < 4; ++p) fetch(0, p);
-    for (int c = 0; c < chunks; ++c) {
+    if (from < chunks)
+        for (int p = 0; p < 4; ++p) fetch(from, p);
+    for (int c = from; c < chunks; ++c) {
         unsigned char* buf = lds + (L::kBuffers == 2 ? (c & 1) * L::kBytes : 0);
-        if (L::kBuffers == 1 && c > 0) __syncthreads();  // the chunk before is done with the buffer
+        if (L::kBuffers == 1 && c > from) __syncthreads();  // the chunk before is done with the buffer
         sk.put(buf + L::kK);
-        sq.put(buf + L::kQ);
+        if (kMode != kMaps) sq.put(buf + L::kQ);
         stm.put(buf + L::kT);
-        smm.put(buf + L::kM);
+        if (kMode != kMaps) smm.put(buf + L::kM);
         sv.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
         const int next = c + 1 < chunks ? c + 1 : c;  // the last chunk's loads are not used
@@ -286,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
         Two s[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) operand(S[2 * i], S[2 * i + 1], odd, s[i]);
-        if constexpr (kRecords) {
+        if constexpr (kMode == kRecording) {
             TIn* st = static_cast<TIn*>(a.st) + (nc * a.dvp + col) * DK + 8 * g;
 #pragma unroll
             for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first(s[i]));
@@ -334,17 +357,19 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
         stage_wall();
         fetch(next, 2);
         One qf[NS][4];
+        if constexpr (kMode != kMaps) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+            for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int b = 0; b < 4; ++b) qf[i][b] = Rows::one(buf + L::kQ, k_row, b, i);
+                for (int b = 0; b < 4; ++b) qf[i][b] = Rows::one(buf + L::kQ, k_row, b, i);
+        }
         Two y[2], z[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
             operand(x[2 * kk] * zb[2 * kk], x[2 * kk + 1] * zb[2 * kk + 1], odd, z[kk]);
         }
-        if constexpr (kRecords) {
+        if constexpr (kMode == kRecording) {
             TIn* yt = static_cast<TIn*>(a.yt) + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, delta::first(y[kk]));
@@ -359,6 +384,7 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
             for (int i = 0; i < DK / 16; ++i) S[i] = mac(kc[kk][i], z[kk], S[i]);
         stage_wall();
         fetch(next, 3);
+        if constexpr (kMode == kMaps) continue;
         One mf[4], mg[2];
         float es[4];
 #pragma unroll
@@ -396,16 +422,102 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
             }
         }
     }
-    if (!active || col >= a.dv) return;
-    for (int64_t t = len + g; t < a.T; t += 4) store_val(op + t * a.dv + col, 0.f);
-    if (a.final_state) {
+    if (!active || col >= width) return;
+    float* to = nullptr;
+    if constexpr (kMode == kMaps) {
+        const int64_t at = n * a.segs + seg;
+        to = unit ? a.map_a + at * a.dk * a.dk : a.map_x + at * a.dk * a.dv;
+    } else {
+        // The segment's tokens past the stream's last live one.
+        const int64_t left = int64_t(seg) * a.seg_chunks * kChunk, right = left + int64_t(a.seg_chunks) * kChunk;
+        const int64_t stop = right < a.T ? right : a.T;
+        for (int64_t t = (len > left ? len : left) + g; t < stop; t += 4) store_val(op + t * a.dv + col, 0.f);
+        const bool last = all == 0 ? seg == 0 : from < all && chunks == all;
+        if (last && a.final_state) to = a.final_state + n * a.dk * a.dv;
+    }
+    if (!to) return;
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = tok(i, 4 * g + r);
+            if (row < a.dk) to[row * width + col] = S[i][r];
+        }
+}
+
+// ---- the segments' starts ----
+
+// starts[0] = the state, starts[p + 1] = map_a[p] starts[p] + map_x[p], the first
+// segment's map_x being what follows it; a wave 16 columns, products in fp32.  A
+// segment's maps are read through LDS (rows apart by 4 banks), the next one's loads
+// meanwhile in registers.
+template <int DK>
+__global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a) {
+    constexpr int kPitch = DK + 4, kPer = DK * DK / kThreads;
+    __shared__ __align__(16) float A[DK * kPitch];
+    const int64_t n = blockIdx.y;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
+    const int col = blockIdx.x * 64 + wave * 16 + lr;
+    f32x4 S[DK / 16], X[DK / 16];  // rows 16 i + 4 g + r
+    float next[kPer];
+    auto load = [&](int p) {
+        const int64_t at = n * a.segs + p;
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) X[i][r] = state_value(a.map_x + at * a.dk * a.dv, 16 * i + 4 * g + r, col, a.dk, a.dv);
+        if (p == 0) return;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int q = int(threadIdx.x) + i * kThreads;
+            next[i] = state_value(a.map_a + at * a.dk * a.dk, q / DK, q % DK, a.dk, a.dk);
+        }
+    };
+    if (a.state) {
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[i][r] = state_value(a.state + n * a.dk * a.dv, 16 * i + 4 * g + r, col, a.dk, a.dv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    load(0);
+    for (int p = 0; p < a.segs; ++p) {
+        float* to = a.starts + (n * a.segs + p) * a.dk * a.dv;
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = tok(i, 4 * g + r);
-                if (row < a.dk) a.final_state[(n * a.dk + row) * a.dv + col] = S[i][r];
+                const int row = 16 * i + 4 * g + r;
+                if (col < a.dv && row < a.dk) to[row * a.dv + col] = S[i][r];
             }
+        if (p + 1 == a.segs) return;
+        f32x4 Y[DK / 16];
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) Y[i] = X[i];
+        if (p > 0) {
+            __syncthreads();  // the segment before is done with A
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int q = int(threadIdx.x) + i * kThreads;
+                A[q / DK * kPitch + q % DK] = next[i];
+            }
+            __syncthreads();
+        }
+        if (p + 2 < a.segs) load(p + 1);
+        if (p > 0) {
+#pragma unroll
+            for (int j = 0; j < DK / 16; ++j)
+#pragma unroll
+                for (int i = 0; i < DK / 16; ++i) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(A + (16 * i + lr) * kPitch + 16 * j + 4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) Y[i] = mfma4(x[r], S[j][r], Y[i]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i) S[i] = Y[i];
     }
 }
 
@@ -422,19 +534,25 @@ __global__ __launch_bounds__(kThreads) void delta_step_kernel(const DeltaArgs a)
     const int c = (blockIdx.x * CQ + cl) * V;
     const bool in = c < a.dv;
     float S[R][V];
+    if (a.state) {
+        const float* from = a.state + n * a.dk * a.dv;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int row = i * RG + rg;
-#pragma unroll
-        for (int j = 0; j < V; ++j) S[i][j] = 0.f;
-        if (!a.state || !in || row >= a.dk) continue;
-        const float* p = a.state + (n * a.dk + row) * a.dv + c;
-        if constexpr (V == 4) {
-            const float4 s = *reinterpret_cast<const float4*>(p);
-            S[i][0] = s.x, S[i][1] = s.y, S[i][2] = s.z, S[i][3] = s.w;
-        } else {
-            S[i][0] = *p;
+        for (int i = 0; i < R; ++i) {
+            const int row = i * RG + rg;
+            if constexpr (V == 4) {
+                const float4 s = *reinterpret_cast<const float4*>(from + min(row, a.dk - 1) * a.dv + min(c, a.dv - 4));
+                const bool there = in && row < a.dk;
+                S[i][0] = there ? s.x : 0.f, S[i][1] = there ? s.y : 0.f;
+                S[i][2] = there ? s.z : 0.f, S[i][3] = there ? s.w : 0.f;
+            } else {
+                S[i][0] = state_value(from, row, c, a.dk, a.dv);
+            }
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) S[i][j] = 0.f;
     }
     TIn* op = static_cast<TIn*>(a.out) + n * a.T * a.dv + c;
 #pragma unroll 1
@@ -515,11 +633,17 @@ hipError_t launch_chunks(const DeltaRule& r, const DeltaArgs& a, hipStream_t str
     delta_solve_kernel<TIn, DK, kVec><<<unsigned(r.N * a.chunks), kThreads, solve, stream>>>(a);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    const unsigned grid = unsigned((r.N + 7) / 8 * 8 * ((r.dv + 63) / 64));
+    const unsigned blocks = (r.dv + 63) / 64;
+    auto grid = [&](int64_t streams, unsigned each) { return unsigned((streams + 7) / 8 * 8 * each); };
+    if (a.segs > 1) {
+        delta_chunk_kernel<TIn, DK, kVec, kMaps>
+            <<<grid(r.N * (a.segs - 1), blocks + (r.dk + 63) / 64), kThreads, walk, stream>>>(a);
+        delta_join_kernel<DK><<<dim3(blocks, unsigned(r.N)), kThreads, 0, stream>>>(a);
+    }
     if (a.st)
-        delta_chunk_kernel<TIn, DK, kVec, true><<<grid, kThreads, walk, stream>>>(a);
+        delta_chunk_kernel<TIn, DK, kVec, kRecording><<<grid(r.N * a.segs, blocks), kThreads, walk, stream>>>(a);
     else
-        delta_chunk_kernel<TIn, DK, kVec, false><<<grid, kThreads, walk, stream>>>(a);
+        delta_chunk_kernel<TIn, DK, kVec, kOutputs><<<grid(r.N * a.segs, blocks), kThreads, walk, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -539,6 +663,17 @@ void launch_step(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
 
 }  // namespace
 
+// Chunks of a segment.  One walk has (dv + 63) / 64 workgroups a stream; a chunk takes
+// it about 3 us however few there are.  Split, every segment is walked twice, the
+// first time with dk columns more and without outputs, so a split pays where it
+// makes at least three segments; it aims for a workgroup a CU, and leaves a segment 8
+// chunks.  (16 streams of 32768 tokens, 128 x 128: TODO.)
+int64_t delta_segment_chunks(const DeltaRule& r) {
+    const int64_t chunks = delta_chunks(r), walks = r.N * ((r.dv + 63) / 64);
+    const int64_t segs = std::min<int64_t>(walks > 0 ? 256 / walks : 1, chunks / 8);
+    return segs < 3 ? std::max<int64_t>(chunks, 1) : (chunks + segs - 1) / segs;
+}
+
 int64_t delta_chunks(const DeltaRule& r) { return (r.T + kChunk - 1) / kChunk; }
 
 DeltaLayout delta_layout(const DeltaRule& r) {
@@ -547,13 +682,18 @@ DeltaLayout delta_layout(const DeltaRule& r) {
     l.mm = round256(nc * kChunk * kChunk * 4);
     l.vec = l.mm + round256(nc * kChunk * kChunk * es);
     l.solve_bytes = l.vec + round256(nc * 512);
+    const int64_t each = delta_segment_chunks(r), segs = std::max<int64_t>((delta_chunks(r) + each - 1) / each, 1);
+    l.segs = int(segs), l.seg_chunks = int(each);
+    l.map_x = round256(r.N * segs * r.dk * r.dv * 4);
+    l.map_a = 2 * l.map_x;
+    l.map_bytes = segs > 1 ? l.map_a + round256(r.N * segs * r.dk * r.dk * 4) : 0;
     l.yt = l.solve_bytes + round256(nc * dvp * dk_padded(r) * es);
     l.record_bytes = l.yt + round256(nc * dvp * kChunk * es);
     return l;
 }
 
 hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* state, void* out, float* final_state,
-                        void* scratch, bool records, hipStream_t stream) {
+                        void* records, void* workspace, hipStream_t stream) {
     DeltaArgs a = delta_args(r, in);
     a.state = state, a.out = out, a.final_state = final_state;
     if (!records && r.T <= kDeltaStepTokens) {
@@ -565,10 +705,16 @@ hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* 
         return hipGetLastError();
     }
     const DeltaLayout l = delta_layout(r);
-    unsigned char* base = static_cast<unsigned char*>(scratch);
+    unsigned char* maps = static_cast<unsigned char*>(workspace);
+    unsigned char* base = records ? static_cast<unsigned char*>(records) : maps + l.map_bytes;
     a.tm = base, a.mm = base + l.mm;
     a.vec = reinterpret_cast<float*>(base + l.vec);
     if (records) a.st = base + l.solve_bytes, a.yt = base + l.yt;
+    a.segs = l.segs, a.seg_chunks = l.seg_chunks;
+    if (l.segs > 1) {
+        a.starts = reinterpret_cast<float*>(maps);
+        a.map_x = reinterpret_cast<float*>(maps + l.map_x), a.map_a = reinterpret_cast<float*>(maps + l.map_a);
+    }
     const bool vec = a.vec_k && a.vec_v && a.vec_o;
     if (r.dtype == RACE_BF16)
         return vec ? launch_by_width<bf16_t, true>(r, a, stream) : launch_by_width<bf16_t, false>(r, a, stream);

@@ -386,6 +386,10 @@ struct DeltaArgs {
     void *tm, *mm;  // [N][chunks] of T (two planes of bf16, or fp32) and M, [64][64]
     float* vec;     // [N][chunks][128]: E, then Z b
     void *st, *yt;  // nullable: [N][chunks][dvp] columns of S [DK] and Y [64], in the rows' type
+    // Segments of seg_chunks chunks that are walked at once, from starts [N][segs][dk][dv];
+    // a segment takes a state s to map_a s + map_x, [N][segs][dk][dk] and [dk][dv].
+    float *starts, *map_a, *map_x;
+    int segs, seg_chunks;
     int64_t N, T;
     int64_t qn, qt, kn, kt, vn, vt;
     Live live;
@@ -416,6 +420,13 @@ __device__ __forceinline__ float log_decay(float g, int form) {
 __device__ __forceinline__ void store4_of(float* p, const f32x4& x) { *reinterpret_cast<f32x4*>(p) = x; }
 __device__ __forceinline__ void store4_of(bf16_t* p, const f32x4& x) {
     *reinterpret_cast<uint2*>(p) = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
+}
+
+// Value (row, col) of a state [dk][dv] (nullable), zero outside: read from the nearest
+// place within and chosen after, so that a wave's 32 loads have no branches between them.
+__device__ __forceinline__ float state_value(const float* s, int row, int col, int dk, int dv) {
+    const float x = s[min(row, dk - 1) * dv + min(col, dv - 1)];
+    return row < dk && col < dv ? x : 0.f;
 }
 
 // A chunk's tiles in LDS (bytes from its buffer's start).

@@ -2247,19 +2247,23 @@ bool delta_shape(const race_delta_shape* sh, const int32_t* lengths, DeltaRule* 
     return true;
 }
 
-bool delta_step(const DeltaRule& r, const void* records) { return !records && r.T <= kDeltaStepTokens; }
+size_t delta_fwd_bytes(const DeltaRule& r, bool records) {
+    if (r.N == 0 || (!records && r.T <= kDeltaStepTokens)) return 0;
+    const DeltaLayout l = delta_layout(r);
+    return size_t(l.map_bytes + (records ? 0 : l.solve_bytes));
+}
 
 }  // namespace
 }  // namespace race
 
 extern "C" {
 
-race_status race_delta_fwd_workspace_bytes(const race_delta_shape* shape, size_t* bytes, size_t* record_bytes) {
+race_status race_delta_fwd_workspace_bytes(const race_delta_shape* shape, int32_t with_records, size_t* bytes,
+                                           size_t* record_bytes) {
     DeltaRule r;
     if (!delta_shape(shape, nullptr, &r) || !bytes) return RACE_ERROR_INVALID_VALUE;
-    const DeltaLayout l = delta_layout(r);
-    *bytes = delta_step(r, nullptr) ? 0 : size_t(l.solve_bytes);
-    if (record_bytes) *record_bytes = size_t(l.record_bytes);
+    *bytes = delta_fwd_bytes(r, with_records != 0);
+    if (record_bytes) *record_bytes = size_t(delta_layout(r).record_bytes);
     return RACE_SUCCESS;
 }
 
@@ -2277,11 +2281,9 @@ race_status race_delta_fwd(const void* q, const void* k, const void* v, const vo
         return copy_floats(state, final_state, floats, stream);
     }
     if (!q || !k || !v || !beta || !out || !all_aligned16({q, k, v, gate, beta, out})) return RACE_ERROR_INVALID_VALUE;
-    if (!records && !delta_step(r, records) &&
-        (!workspace || !aligned16(workspace) || workspace_bytes < size_t(delta_layout(r).solve_bytes)))
-        return RACE_ERROR_INVALID_VALUE;
-    return launch_delta(r, {q, k, v, gate, beta}, state, out, final_state, records ? records : workspace, records != nullptr,
-                        stream);
+    const size_t need = delta_fwd_bytes(r, records != nullptr);
+    if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return RACE_ERROR_INVALID_VALUE;
+    return launch_delta(r, {q, k, v, gate, beta}, state, out, final_state, records, workspace, stream);
 }
 
 race_status race_delta_bwd_workspace_bytes(const race_delta_shape* shape, size_t* bytes) {

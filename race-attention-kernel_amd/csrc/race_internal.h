@@ -505,15 +505,18 @@ constexpr int64_t kDeltaStepTokens = 16;
 int64_t delta_chunks(const DeltaRule& r);
 // Bytes from the start of the chunks' arrays: T and M of every chunk and its
 // decays (solve_bytes in all), then, in records only, the state before every
-// chunk and the errors its tokens write.
+// chunk and the errors its tokens write.  And the segments the tokens are walked in:
+// with several, their starts and maps take map_bytes.
 struct DeltaLayout {
     int64_t mm, vec, solve_bytes, yt, record_bytes;
+    int64_t map_x, map_a, map_bytes;
+    int segs, seg_chunks;
 };
 DeltaLayout delta_layout(const DeltaRule& r);
-// scratch: record_bytes with records, solve_bytes without.  state and final_state
-// may be null, and may be the same.
+// records (nullable): record_bytes.  workspace: map_bytes, and solve_bytes more
+// without records.  state and final_state may be null, and may be the same.
 hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* state, void* out, float* final_state,
-                        void* scratch, bool records, hipStream_t stream);
+                        void* records, void* workspace, hipStream_t stream);
 
 // Gradients for dout and dfinal (nullable: zero) from the forward's inputs and
 // records; any of the outputs may be null.  dq, dk [Nk][T][dk], dv [N][T][dv],

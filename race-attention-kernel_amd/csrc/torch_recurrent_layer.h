@@ -237,13 +237,10 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> delta_forward(
     const at::Tensor fin = inplace ? *state
                                    : at::empty({sh.value_streams, sh.key_dim, sh.value_dim}, v.options().dtype(at::kFloat));
     size_t bytes = 0, record_bytes = 0;
-    check_status(race_delta_fwd_workspace_bytes(&sh, &bytes, &record_bytes), "race_delta_fwd_workspace_bytes");
+    check_status(race_delta_fwd_workspace_bytes(&sh, want_records, &bytes, &record_bytes), "race_delta_fwd_workspace_bytes");
     c10::optional<at::Tensor> records;
-    at::Tensor ws;
-    if (want_records)
-        records = workspace_of(record_bytes, q), bytes = 0;
-    else if (bytes > 0)
-        ws = workspace_of(bytes, q);
+    if (want_records) records = workspace_of(record_bytes, q);
+    const at::Tensor ws = bytes > 0 ? workspace_of(bytes, q) : at::Tensor();
     if (inplace) state->unsafeGetTensorImpl()->bump_version();  // a graph that saved it must notice
     check_status(race_delta_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), data_of(gate), beta.data_ptr(), floats_of(state),
                                 lengths_of(lengths), out.data_ptr(), fin.data_ptr<float>(), ptr_of(records), &sh,
@@ -264,7 +261,7 @@ DeltaBackward delta_backward(const at::Tensor& q, const at::Tensor& k, const c10
     const char* entry = "race_delta_rule backward";
     const race_delta_shape sh = delta_shape(entry, q, k, dout, gate, beta, dfinal, lengths, form, scale);
     size_t bytes = 0, record_bytes = 0;
-    check_status(race_delta_fwd_workspace_bytes(&sh, &bytes, &record_bytes), "race_delta_fwd_workspace_bytes");
+    check_status(race_delta_fwd_workspace_bytes(&sh, 1, &bytes, &record_bytes), "race_delta_fwd_workspace_bytes");
     check_status(race_delta_bwd_workspace_bytes(&sh, &bytes), "race_delta_bwd_workspace_bytes");
     ArgCheck(entry).on_gpu("dout", dout).on_gpu("records", records)
         .require(records.scalar_type() == at::kFloat && records.device() == q.device() &&
