@@ -48,7 +48,9 @@ __device__ __forceinline__ void store_gate(void* p, int64_t i, int f32, float x)
         static_cast<bf16_t*>(p)[i] = f32_to_bf16(x);
 }
 
-template <typename TIn, int DK, bool kVec>
+// kMaps: no records, but what the segment adds to a gradient of zero behind it (the
+// last one: to dfinal), to map_x.
+template <typename TIn, int DK, bool kVec, bool kMaps>
 __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwdArgs w) {
     extern __shared__ __align__(16) unsigned char lds[];
     const DeltaArgs& a = w.f;
@@ -58,26 +60,32 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
     using One = OneT<TIn>;
     using Two = TwoT<TIn>;
     constexpr int NS = DK / 32;
-    int64_t n;
+    const int walks = kMaps ? a.segs - 1 : a.segs;  // no gradient goes on before the first segment
+    int64_t ns;
     int cb;
-    if (!stream_and_block(a.N, (a.dv + 63) / 64, n, cb)) return;
+    if (!stream_and_block(a.N * walks, (a.dv + 63) / 64, ns, cb)) return;
+    const int64_t n = unsigned(ns) / unsigned(walks);
+    const int seg = int(ns - n * walks) + (kMaps ? 1 : 0);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
     const bool odd = g & 1;
     const int c0 = cb * 64 + wave * 16, col = c0 + lr;
     const bool active = c0 < a.dv;
     const int64_t nk = n / a.group, len = a.live.of(n, a.T);
-    const int chunks = int((len + kChunk - 1) / kChunk);
+    const int all = int((len + kChunk - 1) / kChunk);
+    const int from = min(seg * a.seg_chunks, all), chunks = min(from + a.seg_chunks, all);
     const TIn* kp = static_cast<const TIn*>(a.k) + nk * a.kn;
     const TIn* qp = static_cast<const TIn*>(a.q) + nk * a.qn;
     const TIn* op = static_cast<const TIn*>(w.dout) + n * a.T * a.dv + cb * 64;
+    const float* behind = !kMaps && a.starts             ? a.starts + ns * a.dk * a.dv
+                          : w.dfinal && seg == a.segs - 1 ? w.dfinal + n * a.dk * a.dv
+                                                          : nullptr;
 
     f32x4 dS[DK / 16];
-    if (w.dfinal) {
+    if (behind) {
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                dS[i][r] = state_value(w.dfinal + n * a.dk * a.dv, tok(i, 4 * g + r), col, a.dk, a.dv);
+            for (int r = 0; r < 4; ++r) dS[i][r] = state_value(behind, tok(i, 4 * g + r), col, a.dk, a.dv);
     } else {
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i) dS[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -106,9 +114,9 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
     // What a lane adds to a tile's start.
     const int k_row = Rows::row_base(lr, g), k_col = Rows::column_base(lr, g), s_col = Square::column_base(lr, g);
     const int o_at = Square::block_base(16 * wave, lr, g);
-    if (chunks > 0)
+    if (from < chunks)
         for (int p = 0; p < 4; ++p) fetch(chunks - 1, p);
-    for (int c = chunks - 1; c >= 0; --c) {
+    for (int c = chunks - 1; c >= from; --c) {
         unsigned char* buf = lds + (L::kBuffers == 2 ? (c & 1) * L::kBytes : 0);
         if (L::kBuffers == 1 && c < chunks - 1) __syncthreads();  // the chunk before is done with the buffer
         sk.put(buf + L::kK);
@@ -117,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
         smm.put(buf + L::kM);
         so.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
-        const int next = c > 0 ? c - 1 : 0;  // the last chunk's loads are not used
+        const int next = c > from ? c - 1 : c;  // the last chunk's loads are not used
         __syncthreads();
         if (!active) {
             for (int p = 0; p < 4; ++p) fetch(next, p);
@@ -142,7 +150,7 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             operand(dS[2 * i], dS[2 * i + 1], odd, s[i]);
-            store_run(ds + 32 * i, delta::first(s[i]));
+            if constexpr (!kMaps) store_run(ds + 32 * i, delta::first(s[i]));
         }
         stage_wall();
         fetch(next, 0);
@@ -215,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
         for (int kk = 0; kk < 2; ++kk) {
             One plain;
             operand(x[2 * kk], x[2 * kk + 1], odd, plain);
-            store_run(dd + 32 * kk, plain);
+            if constexpr (!kMaps) store_run(dd + 32 * kk, plain);
             operand(x[2 * kk] * -e[2 * kk], x[2 * kk + 1] * -e[2 * kk + 1], odd, d[kk]);
         }
         stage_wall();
@@ -224,30 +232,34 @@ __global__ __launch_bounds__(kThreads) void delta_bwd_walk_kernel(const DeltaBwd
 #pragma unroll
             for (int i = 0; i < DK / 16; ++i) dS[i] = mac(kc[kk][i], d[kk], dS[i]);
     }
-    // Chunks past the stream's last have no gradients; nor have those of a key stream past all of its.
-    const int64_t end = int64_t(chunks) * kChunk, i0 = threadIdx.x;
-    if (w.dv)
-        for (int64_t i = end * a.dv + i0; i < a.T * a.dv && cb == 0; i += kThreads)
-            store_val(static_cast<TIn*>(w.dv) + n * a.T * a.dv + i, 0.f);
-    for (void* p : {w.dgate, w.dbeta})
-        for (int64_t t = end + i0; p && t < a.T && cb == 0; t += kThreads) store_gate(p, n * a.T + t, a.gate_f32, 0.f);
-    if (n % a.group == 0 && cb == 0) {
-        int64_t most = 0;
-        for (int h = 0; h < a.group; ++h) {
-            const int64_t l = a.live.of(n + h, a.T);
-            most = l > most ? l : most;
+    if (!kMaps && seg == 0 && cb == 0) {
+        // Chunks past the stream's last have no gradients; nor have those of a key stream past all of its.
+        const int64_t end = int64_t(all) * kChunk, i0 = threadIdx.x;
+        if (w.dv)
+            for (int64_t i = end * a.dv + i0; i < a.T * a.dv; i += kThreads)
+                store_val(static_cast<TIn*>(w.dv) + n * a.T * a.dv + i, 0.f);
+        for (void* p : {w.dgate, w.dbeta})
+            for (int64_t t = end + i0; p && t < a.T; t += kThreads) store_gate(p, n * a.T + t, a.gate_f32, 0.f);
+        if (n % a.group == 0) {
+            int64_t most = 0;
+            for (int h = 0; h < a.group; ++h) {
+                const int64_t l = a.live.of(n + h, a.T);
+                most = l > most ? l : most;
+            }
+            for (void* p : {w.dq, w.dk})
+                for (int64_t i = (most + kChunk - 1) / kChunk * kChunk * a.dk + i0; p && i < a.T * a.dk; i += kThreads)
+                    store_val(static_cast<TIn*>(p) + nk * a.T * a.dk + i, 0.f);
         }
-        for (void* p : {w.dq, w.dk})
-            for (int64_t i = (most + kChunk - 1) / kChunk * kChunk * a.dk + i0; p && i < a.T * a.dk; i += kThreads)
-                store_val(static_cast<TIn*>(p) + nk * a.T * a.dk + i, 0.f);
     }
-    if (!w.dstate || !active || col >= a.dv) return;
+    float* to = kMaps ? a.map_x + (n * a.segs + seg) * a.dk * a.dv : seg == 0 ? w.dstate : nullptr;
+    if (!to || !active || col >= a.dv) return;
+    if (!kMaps) to += n * a.dk * a.dv;
 #pragma unroll
     for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = tok(i, 4 * g + r);
-            if (row < a.dk) w.dstate[(n * a.dk + row) * a.dv + col] = dS[i][r];
+            if (row < a.dk) to[row * a.dv + col] = dS[i][r];
         }
 }
 
@@ -674,8 +686,14 @@ hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_
     using L = ChunkLds<TIn, DK>;
     constexpr int walk = L::kBuffers * L::kBytes, grads = GradLds<TIn, DK>::kBytes;
     static_assert(walk <= kGfx950LdsBytes && grads <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
-    const int64_t blocks = (r.dv + 63) / 64;
-    delta_bwd_walk_kernel<TIn, DK, kVec><<<unsigned((r.N + 7) / 8 * 8 * blocks), kThreads, walk, stream>>>(w);
+    auto grid_of = [&](int64_t streams) { return unsigned((streams + 7) / 8 * 8 * ((r.dv + 63) / 64)); };
+    if (w.f.segs > 1) {
+        delta_bwd_walk_kernel<TIn, DK, kVec, true><<<grid_of(r.N * (w.f.segs - 1)), kThreads, walk, stream>>>(w);
+        DeltaArgs join = w.f;
+        join.state = w.dfinal;
+        launch_join<DK, true>(r, join, stream);
+    }
+    delta_bwd_walk_kernel<TIn, DK, kVec, false><<<grid_of(r.N * w.f.segs), kThreads, walk, stream>>>(w);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (!w.dq && !w.dk && !w.dv && !w.dgate && !w.dbeta) return hipSuccess;
@@ -697,7 +715,9 @@ hipError_t launch_by_width(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_
 
 int64_t delta_bwd_bytes(const DeltaRule& r) {
     const int64_t nc = r.N * delta_chunks(r), es = r.dtype == RACE_BF16 ? 2 : 4, dvp = (r.dv + 15) / 16 * 16;
-    return round256(nc * dvp * dk_padded(r) * es) + round256(nc * dvp * kChunk * es);
+    const DeltaLayout l = delta_layout(r);
+    // With segments, their ends and what they add to a gradient.
+    return round256(nc * dvp * dk_padded(r) * es) + round256(nc * dvp * kChunk * es) + (l.map_bytes - l.starts);
 }
 
 hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const void* dout, const float* dfinal,
@@ -712,6 +732,12 @@ hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const voi
     const int64_t es = r.dtype == RACE_BF16 ? 2 : 4;
     w.ds = scratch;
     w.dd = static_cast<unsigned char*>(scratch) + round256(r.N * w.f.chunks * w.f.dvp * dk_padded(r) * es);
+    w.f.segs = l.segs, w.f.seg_chunks = l.seg_chunks;
+    if (l.segs > 1) {
+        w.f.map_a = reinterpret_cast<float*>(base + l.map_a);
+        w.f.starts = reinterpret_cast<float*>(static_cast<unsigned char*>(w.dd) + round256(r.N * w.f.chunks * w.f.dvp * kChunk * es));
+        w.f.map_x = w.f.starts + (l.map_x - l.starts) / 4;
+    }
     w.dq = g.dq, w.dk = g.dk, w.dv = g.dv, w.dgate = g.dgate, w.dbeta = g.dbeta, w.dstate = g.dstate;
     const bool vec = w.f.vec_k && w.f.vec_o;
     if (r.dtype == RACE_BF16)

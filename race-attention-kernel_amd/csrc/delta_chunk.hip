@@ -211,9 +211,9 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
 enum WalkMode { kOutputs, kRecording, kMaps };
 
 template <typename TIn, int DK, bool kVec, WalkMode kMode>
-__global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a) {
+__global__ __launch_bounds__(kThreads, kMode == kMaps && sizeof(TIn) * DK <= 256 ? 2 : 1) void delta_chunk_kernel(const DeltaArgs a) {
     extern __shared__ __align__(16) unsigned char lds[];
-    using L = ChunkLds<TIn, DK>;
+    using L = ChunkLds<TIn, DK, kMode != kMaps>;
     using Rows = Tile<TIn, DK>;
     using Square = Tile<TIn, 64>;
     using One = OneT<TIn>;
@@ -445,82 +445,6 @@ __global__ __launch_bounds__(kThreads) void delta_chunk_kernel(const DeltaArgs a
         }
 }
 
-// ---- the segments' starts ----
-
-// starts[0] = the state, starts[p + 1] = map_a[p] starts[p] + map_x[p], the first
-// segment's map_x being what follows it; a wave 16 columns, products in fp32.  A
-// segment's maps are read through LDS (rows apart by 4 banks), the next one's loads
-// meanwhile in registers.
-template <int DK>
-__global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a) {
-    constexpr int kPitch = DK + 4, kPer = DK * DK / kThreads;
-    __shared__ __align__(16) float A[DK * kPitch];
-    const int64_t n = blockIdx.y;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-    const int col = blockIdx.x * 64 + wave * 16 + lr;
-    f32x4 S[DK / 16], X[DK / 16];  // rows 16 i + 4 g + r
-    float next[kPer];
-    auto load = [&](int p) {
-        const int64_t at = n * a.segs + p;
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) X[i][r] = state_value(a.map_x + at * a.dk * a.dv, 16 * i + 4 * g + r, col, a.dk, a.dv);
-        if (p == 0) return;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int q = int(threadIdx.x) + i * kThreads;
-            next[i] = state_value(a.map_a + at * a.dk * a.dk, q / DK, q % DK, a.dk, a.dk);
-        }
-    };
-    if (a.state) {
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) S[i][r] = state_value(a.state + n * a.dk * a.dv, 16 * i + 4 * g + r, col, a.dk, a.dv);
-    } else {
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    load(0);
-    for (int p = 0; p < a.segs; ++p) {
-        float* to = a.starts + (n * a.segs + p) * a.dk * a.dv;
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                if (col < a.dv && row < a.dk) to[row * a.dv + col] = S[i][r];
-            }
-        if (p + 1 == a.segs) return;
-        f32x4 Y[DK / 16];
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) Y[i] = X[i];
-        if (p > 0) {
-            __syncthreads();  // the segment before is done with A
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int q = int(threadIdx.x) + i * kThreads;
-                A[q / DK * kPitch + q % DK] = next[i];
-            }
-            __syncthreads();
-        }
-        if (p + 2 < a.segs) load(p + 1);
-        if (p > 0) {
-#pragma unroll
-            for (int j = 0; j < DK / 16; ++j)
-#pragma unroll
-                for (int i = 0; i < DK / 16; ++i) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(A + (16 * i + lr) * kPitch + 16 * j + 4 * g);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) Y[i] = mfma4(x[r], S[j][r], Y[i]);
-                }
-        }
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) S[i] = Y[i];
-    }
-}
-
 // ---- token by token ----
 
 // V columns a thread and R rows, every eighth: a workgroup holds 32 V columns of a
@@ -637,8 +561,8 @@ hipError_t launch_chunks(const DeltaRule& r, const DeltaArgs& a, hipStream_t str
     auto grid = [&](int64_t streams, unsigned each) { return unsigned((streams + 7) / 8 * 8 * each); };
     if (a.segs > 1) {
         delta_chunk_kernel<TIn, DK, kVec, kMaps>
-            <<<grid(r.N * (a.segs - 1), blocks + (r.dk + 63) / 64), kThreads, walk, stream>>>(a);
-        delta_join_kernel<DK><<<dim3(blocks, unsigned(r.N)), kThreads, 0, stream>>>(a);
+            <<<grid(r.N * (a.segs - 1), blocks + (r.dk + 63) / 64), kThreads, ChunkLds<TIn, DK, false>::kBytes, stream>>>(a);
+        launch_join<DK, false>(r, a, stream);
     }
     if (a.st)
         delta_chunk_kernel<TIn, DK, kVec, kRecording><<<grid(r.N * a.segs, blocks), kThreads, walk, stream>>>(a);
@@ -667,7 +591,9 @@ void launch_step(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
 // it about 3 us however few there are.  Split, every segment is walked twice, the
 // first time with dk columns more and without outputs, so a split pays where it
 // makes at least three segments; it aims for a workgroup a CU, and leaves a segment 8
-// chunks.  (16 streams of 32768 tokens, 128 x 128: TODO.)
+// chunks.  16 streams of 32768 bf16 tokens, 128 x 128: one walk 1493 us; maps 246,
+// join 52 and walks 247.  24 ragged fp32 streams of at most 2000 tokens, 64 x 64, in
+// three segments: backward 153 us in one, 54 + 10 + 77 split.
 int64_t delta_segment_chunks(const DeltaRule& r) {
     const int64_t chunks = delta_chunks(r), walks = r.N * ((r.dv + 63) / 64);
     const int64_t segs = std::min<int64_t>(walks > 0 ? 256 / walks : 1, chunks / 8);
@@ -684,11 +610,12 @@ DeltaLayout delta_layout(const DeltaRule& r) {
     l.solve_bytes = l.vec + round256(nc * 512);
     const int64_t each = delta_segment_chunks(r), segs = std::max<int64_t>((delta_chunks(r) + each - 1) / each, 1);
     l.segs = int(segs), l.seg_chunks = int(each);
-    l.map_x = round256(r.N * segs * r.dk * r.dv * 4);
-    l.map_a = 2 * l.map_x;
-    l.map_bytes = segs > 1 ? l.map_a + round256(r.N * segs * r.dk * r.dk * 4) : 0;
+    l.starts = segs > 1 ? round256(r.N * segs * r.dk * r.dk * 4) : 0;
+    l.map_x = l.starts + round256(r.N * segs * r.dk * r.dv * 4);
+    l.map_bytes = segs > 1 ? l.map_x + round256(r.N * segs * r.dk * r.dv * 4) : 0;
     l.yt = l.solve_bytes + round256(nc * dvp * dk_padded(r) * es);
-    l.record_bytes = l.yt + round256(nc * dvp * kChunk * es);
+    l.map_a = l.yt + round256(nc * dvp * kChunk * es);
+    l.record_bytes = l.map_a + l.starts;
     return l;
 }
 
@@ -712,8 +639,8 @@ hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* 
     if (records) a.st = base + l.solve_bytes, a.yt = base + l.yt;
     a.segs = l.segs, a.seg_chunks = l.seg_chunks;
     if (l.segs > 1) {
-        a.starts = reinterpret_cast<float*>(maps);
-        a.map_x = reinterpret_cast<float*>(maps + l.map_x), a.map_a = reinterpret_cast<float*>(maps + l.map_a);
+        a.map_a = reinterpret_cast<float*>(records ? base + l.map_a : maps);
+        a.starts = reinterpret_cast<float*>(maps + l.starts), a.map_x = reinterpret_cast<float*>(maps + l.map_x);
     }
     const bool vec = a.vec_k && a.vec_v && a.vec_o;
     if (r.dtype == RACE_BF16)

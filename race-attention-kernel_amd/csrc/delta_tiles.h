@@ -429,13 +429,15 @@ __device__ __forceinline__ float state_value(const float* s, int row, int col, i
     return row < dk && col < dv ? x : 0.f;
 }
 
-// A chunk's tiles in LDS (bytes from its buffer's start).
-template <typename TIn, int DK>
+// A chunk's tiles in LDS (bytes from its buffer's start).  Walks without outputs have
+// no Q and M, and one buffer, so that two workgroups share a CU.
+template <typename TIn, int DK, bool kOutputs = true>
 struct ChunkLds {
-    static constexpr int kK = 0, kQ = Tile<TIn, DK>::kBytes, kT = 2 * kQ, kM = kT + kTwoBytes<TIn, 64>;
-    static constexpr int kV = kM + Tile<TIn, 64>::kBytes, kVec = kV + Tile<TIn, 64>::kBytes, kBytes = kVec + 512;
+    static constexpr int kK = 0, kT = Tile<TIn, DK>::kBytes, kV = kT + kTwoBytes<TIn, 64>, kVec = kV + Tile<TIn, 64>::kBytes;
+    static constexpr int kQ = kVec + 512, kM = kQ + Tile<TIn, DK>::kBytes;
+    static constexpr int kBytes = kOutputs ? kM + Tile<TIn, 64>::kBytes : kQ;
     // Two buffers, where they leave the workgroup its LDS: one barrier a chunk.
-    static constexpr int kBuffers = 2 * kBytes <= kGfx950LdsBytes ? 2 : 1;
+    static constexpr int kBuffers = kOutputs && 2 * kBytes <= kGfx950LdsBytes ? 2 : 1;
 };
 
 // Consecutive streams on different XCDs, a stream's column blocks on one (they
@@ -445,6 +447,88 @@ __device__ __forceinline__ bool stream_and_block(int64_t N, int blocks, int64_t&
     const int in = int(id - eight * 8 * blocks);
     n = eight * 8 + (in & 7), cb = in >> 3;
     return n < N;
+}
+
+// ---- the segments' starts ----
+
+// starts[0] = the state, starts[p + 1] = map_a[p] starts[p] + map_x[p], the first
+// segment's map_x being what follows it; backward (kBack) from the last segment on,
+// with the maps transposed.  Products are fp32.  A workgroup has 16 columns
+// and a wave a quarter of the rows, whose part of the next segment's maps it loads
+// meanwhile; the columns meet in LDS, two copies in turn.
+template <int DK, bool kBack>
+__global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a) {
+    constexpr int NI = DK / 64, NJ = DK / 16, kPitch = DK + 4;
+    __shared__ __align__(16) float cols[2][16 * kPitch];
+    const int64_t n = blockIdx.y;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
+    const int col = blockIdx.x * 16 + lr, r0 = wave * (DK / 4);
+    const bool whole = a.dk % 4 == 0;
+    f32x4 S[NI], X[NI], A[NI][NJ];  // rows r0 + 16 i + 4 g + r; rows r0 + 16 i + lr, columns 16 j + 4 g + r
+    auto rows = [&](const float* p, f32x4 (&x)[NI]) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[i][r] = state_value(p, r0 + 16 * i + 4 * g + r, col, a.dk, a.dv);
+    };
+    auto load = [&](int p) {
+        const int64_t at = n * a.segs + p;
+        rows(a.map_x + at * a.dk * a.dv, X);
+        const float* m = a.map_a + at * a.dk * a.dk;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int row = r0 + 16 * i + lr, c = 16 * j + 4 * g;
+                if constexpr (kBack) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) A[i][j][r] = state_value(m, c + r, row, a.dk, a.dk);
+                } else if (whole) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(m + min(row, a.dk - 1) * a.dk + min(c, a.dk - 4));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) A[i][j][r] = row < a.dk && c < a.dk ? x[r] : 0.f;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) A[i][j][r] = state_value(m, row, c + r, a.dk, a.dk);
+                }
+            }
+    };
+    if (a.state) {
+        rows(a.state + n * a.dk * a.dv, S);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    auto segment = [&](int step) { return kBack ? a.segs - 1 - step : step; };
+    rows(a.map_x + (n * a.segs + segment(0)) * a.dk * a.dv, X);
+    for (int step = 0; step < a.segs; ++step) {
+        float* to = a.starts + (n * a.segs + segment(step)) * a.dk * a.dv;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = r0 + 16 * i + 4 * g + r;
+                if (col < a.dv && row < a.dk) to[row * a.dv + col] = S[i][r];
+            }
+        if (step + 1 == a.segs) return;
+        if (step > 0) {
+            float* c = cols[step & 1];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) *reinterpret_cast<f32x4*>(c + lr * kPitch + r0 + 16 * i + 4 * g) = S[i];
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const f32x4 s = *reinterpret_cast<const f32x4*>(c + lr * kPitch + 16 * j + 4 * g);
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) X[i] = mfma::mfma4(A[i][j][r], s[r], X[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) S[i] = X[i];
+        if (step + 2 < a.segs) load(segment(step + 1));
+    }
 }
 
 // ---- host ----
@@ -479,6 +563,11 @@ inline DeltaArgs delta_args(const DeltaRule& r, const DeltaInputs& in) {
     a.vec_o = whole_pieces(r, r.dv, {});
     a.scale = r.scale;
     return a;
+}
+
+template <int DK, bool kBack>
+inline void launch_join(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
+    delta_join_kernel<DK, kBack><<<dim3(unsigned(r.dv + 15) / 16, unsigned(r.N)), kThreads, 0, stream>>>(a);
 }
 
 inline int64_t round256(int64_t bytes) { return (bytes + 255) / 256 * 256; }

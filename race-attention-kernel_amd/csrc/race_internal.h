@@ -505,11 +505,12 @@ constexpr int64_t kDeltaStepTokens = 16;
 int64_t delta_chunks(const DeltaRule& r);
 // Bytes from the start of the chunks' arrays: T and M of every chunk and its
 // decays (solve_bytes in all), then, in records only, the state before every
-// chunk and the errors its tokens write.  And the segments the tokens are walked in:
-// with several, their starts and maps take map_bytes.
+// chunk, the errors its tokens write and the segments' maps of a state.  And the
+// segments the tokens are walked in: with several, map_bytes hold their maps (without
+// records), starts and what they add to a state.
 struct DeltaLayout {
-    int64_t mm, vec, solve_bytes, yt, record_bytes;
-    int64_t map_x, map_a, map_bytes;
+    int64_t mm, vec, solve_bytes, yt, map_a, record_bytes;
+    int64_t starts, map_x, map_bytes;
     int segs, seg_chunks;
 };
 DeltaLayout delta_layout(const DeltaRule& r);
