@@ -210,10 +210,14 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
 // its state).
 enum WalkMode { kOutputs, kRecording, kMaps };
 
+template <typename TIn, int DK, WalkMode kMode>
+using WalkLds = ChunkLds<TIn, DK, kMode != kMaps, !two_a_cu(sizeof(TIn) * DK, kMode == kMaps)>;
+
 template <typename TIn, int DK, bool kVec, WalkMode kMode>
-__global__ __launch_bounds__(kThreads, kMode == kMaps && sizeof(TIn) * DK <= 256 ? 2 : 1) void delta_chunk_kernel(const DeltaArgs a) {
+__global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps) ? 2 : 1) void delta_chunk_kernel(const DeltaArgs a) {
     extern __shared__ __align__(16) unsigned char lds[];
-    using L = ChunkLds<TIn, DK, kMode != kMaps>;
+    using L = WalkLds<TIn, DK, kMode>;
+    constexpr bool kLate = two_a_cu(sizeof(TIn) * DK, kMode == kMaps) && kMode != kMaps;
     using Rows = Tile<TIn, DK>;
     using Square = Tile<TIn, 64>;
     using One = OneT<TIn>;
@@ -335,10 +339,13 @@ __global__ __launch_bounds__(kThreads, kMode == kMaps && sizeof(TIn) * DK <= 256
         stage_wall();
         fetch(next, 1);
         One kc[2][DK / 16];
+        auto columns = [&] {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-            for (int i = 0; i < DK / 16; ++i) kc[kk][i] = Rows::transposed(buf + L::kK, k_col, kk, i);
+                for (int i = 0; i < DK / 16; ++i) kc[kk][i] = Rows::transposed(buf + L::kK, k_col, kk, i);
+        };
+        if (!kLate) columns();
         f32x4 zb[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) zb[b] = *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
@@ -356,8 +363,9 @@ __global__ __launch_bounds__(kThreads, kMode == kMaps && sizeof(TIn) * DK <= 256
         for (int b = 2; b < 4; ++b) x[b] = mac(tg[b - 2], d[1], x[b]);
         stage_wall();
         fetch(next, 2);
+        if (kLate) columns();
         One qf[NS][4];
-        if constexpr (kMode != kMaps) {
+        if constexpr (kMode != kMaps && !kLate) {
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
@@ -387,16 +395,25 @@ __global__ __launch_bounds__(kThreads, kMode == kMaps && sizeof(TIn) * DK <= 256
         if constexpr (kMode == kMaps) continue;
         One mf[4], mg[2];
         float es[4];
+        auto scores = [&] {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) mf[b] = Square::one(buf + L::kM, s_row, b, 0), es[b] = E[tok(b, lr)] * a.scale;
+            for (int b = 0; b < 4; ++b) mf[b] = Square::one(buf + L::kM, s_row, b, 0), es[b] = E[tok(b, lr)] * a.scale;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) mg[b] = Square::one(buf + L::kM, s_row, 2 + b, 1);
+            for (int b = 0; b < 2; ++b) mg[b] = Square::one(buf + L::kM, s_row, 2 + b, 1);
+        };
+        if (!kLate) scores();
         // O^T = scale S^T Q^T E + Y^T M^T, S the state before the chunk: a token's columns in a lane.
         f32x4 o[4];
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+        for (int i = 0; i < NS; ++i) {
+            if constexpr (kLate) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) qf[i][b] = Rows::one(buf + L::kQ, k_row, b, i);
+            }
 #pragma unroll
             for (int b = 0; b < 4; ++b) o[b] = mac(s[i], qf[i][b], i == 0 ? zero : o[b]);
+        }
+        if (kLate) scores();
 #pragma unroll
         for (int b = 0; b < 4; ++b) o[b] = mac(y[0], mf[b], o[b] * es[b]);
 #pragma unroll
@@ -551,8 +568,11 @@ __global__ __launch_bounds__(kThreads) void delta_step_kernel(const DeltaArgs a)
 
 template <typename TIn, int DK, bool kVec>
 hipError_t launch_chunks(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
-    using L = ChunkLds<TIn, DK>;
-    constexpr int solve = solve_lds_bytes<TIn, DK>(), walk = L::kBuffers * L::kBytes;
+    constexpr int solve = solve_lds_bytes<TIn, DK>();
+    using L = WalkLds<TIn, DK, kOutputs>;
+    using Maps = WalkLds<TIn, DK, kMaps>;
+    constexpr int walk = L::kBuffers * L::kBytes, maps = Maps::kBuffers * Maps::kBytes;
+    static_assert(walk == WalkLds<TIn, DK, kRecording>::kBuffers * WalkLds<TIn, DK, kRecording>::kBytes);
     static_assert(solve <= kGfx950LdsBytes && walk <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
     delta_solve_kernel<TIn, DK, kVec><<<unsigned(r.N * a.chunks), kThreads, solve, stream>>>(a);
     const hipError_t err = hipGetLastError();
@@ -561,7 +581,7 @@ hipError_t launch_chunks(const DeltaRule& r, const DeltaArgs& a, hipStream_t str
     auto grid = [&](int64_t streams, unsigned each) { return unsigned((streams + 7) / 8 * 8 * each); };
     if (a.segs > 1) {
         delta_chunk_kernel<TIn, DK, kVec, kMaps>
-            <<<grid(r.N * (a.segs - 1), blocks + (r.dk + 63) / 64), kThreads, ChunkLds<TIn, DK, false>::kBytes, stream>>>(a);
+            <<<grid(r.N * (a.segs - 1), blocks + (r.dk + 63) / 64), kThreads, maps, stream>>>(a);
         launch_join<DK, false>(r, a, stream);
     }
     if (a.st)

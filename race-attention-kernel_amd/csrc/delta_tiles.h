@@ -429,15 +429,20 @@ __device__ __forceinline__ float state_value(const float* s, int row, int col, i
     return row < dk && col < dv ? x : 0.f;
 }
 
-// A chunk's tiles in LDS (bytes from its buffer's start).  Walks without outputs have
-// no Q and M, and one buffer, so that two workgroups share a CU.
-template <typename TIn, int DK, bool kOutputs = true>
+// Whether two workgroups that walk chunks share a CU, each with one buffer, as narrow
+// keys' registers and tiles allow, and the maps' (no Q and M).  192 streams of 577
+// bf16 tokens, 64 x 128: the walk 43.5 -> 35.6 us; keys of 128 would spill (outputs of
+// 512 workgroups 356 us, of half as many that walk twice as far 247).
+constexpr bool two_a_cu(int row_bytes, bool maps) { return row_bytes <= (maps ? 256 : 128); }
+
+// A chunk's tiles in LDS (bytes from its buffer's start).
+template <typename TIn, int DK, bool kOutputs = true, bool kTwoBuffers = kOutputs>
 struct ChunkLds {
     static constexpr int kK = 0, kT = Tile<TIn, DK>::kBytes, kV = kT + kTwoBytes<TIn, 64>, kVec = kV + Tile<TIn, 64>::kBytes;
     static constexpr int kQ = kVec + 512, kM = kQ + Tile<TIn, DK>::kBytes;
     static constexpr int kBytes = kOutputs ? kM + Tile<TIn, 64>::kBytes : kQ;
     // Two buffers, where they leave the workgroup its LDS: one barrier a chunk.
-    static constexpr int kBuffers = kOutputs && 2 * kBytes <= kGfx950LdsBytes ? 2 : 1;
+    static constexpr int kBuffers = kTwoBuffers && kOutputs && 2 * kBytes <= kGfx950LdsBytes ? 2 : 1;
 };
 
 // Consecutive streams on different XCDs, a stream's column blocks on one (they
