@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     const bool odd = g & 1;
     const int c0 = cb * 64 + wave * 16, col = c0 + lr;
     const bool active = c0 < a.dv;
-    const int64_t nk = n / a.group, len = a.live.of(n, a.T);
+    const int64_t nk = a.key_stream(n), len = a.len_of(n);
     const int all = int((len + kChunk - 1) / kChunk);
     const int from = min(seg * a.seg_chunks, all), chunks = min(from + a.seg_chunks, all);
     const TIn* kp = static_cast<const TIn*>(a.k) + nk * a.kn;
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         if (n % a.group == 0) {
             int64_t most = 0;
             for (int h = 0; h < a.group; ++h) {
-                const int64_t l = a.live.of(n + h, a.T);
+                const int64_t l = a.len_of(n + h);
                 most = l > most ? l : most;
             }
             for (void* p : {w.dq, w.dk})
@@ -358,7 +358,7 @@ struct GradUnit {
     int item, nk, c, h, v0, live;  // item: key stream and chunk
 };
 __device__ __forceinline__ int live_rows(const DeltaArgs& a, int nk, int c, int h) {
-    const int64_t l = a.live.of(int64_t(nk) * a.group + h, a.T) - int64_t(c) * kChunk;
+    const int64_t l = a.len_of(int64_t(nk) * a.group + h) - int64_t(c) * kChunk;
     return l < 0 ? 0 : l < kChunk ? int(l) : kChunk;
 }
 // The next live stream of the unit's chunk or, past its last, of a chunk to come.

@@ -24,6 +24,7 @@
 // long sums lose the digits the products keep.
 // A few tokens (decode) go token by token in 32 bits: delta_step_kernel.
 #include <algorithm>
+#include <utility>
 
 #include "delta_tiles.h"
 
@@ -41,7 +42,7 @@ constexpr int kSolveMatrix = kChunk * kSolvePitch * 4;
 template <typename TIn, int DK>
 constexpr int solve_lds_bytes() {
     constexpr int tiles = 2 * Tile<TIn, DK>::kBytes;
-    return (tiles > kSolveMatrix ? tiles : kSolveMatrix) + kSolveMatrix;
+    return tiles > 2 * kSolveMatrix ? tiles : 2 * kSolveMatrix;
 }
 
 // acc += X[r0 ..][c0 ..] B for 16 x 16 fp32 blocks, B in accumulator order.
@@ -59,35 +60,52 @@ __device__ __forceinline__ f32x4 block_of(const float* x, int r0, int c0, int g,
     return v;
 }
 
+// x -= n_j x_j for every row below j, whose N is zero up to its diagonal: x_j from
+// lane j of the lane's 16.
+template <int... J>
+__device__ __forceinline__ void substitute(f32x4& x, const f32x4 (&n)[4], std::integer_sequence<int, J...>) {
+    auto step = [&](auto j) {
+        constexpr int kBroadcast = 0x150 + decltype(j)::value;  // row_newbcast
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int v = __float_as_int(x[c]);
+            x[c] = fmaf(-n[decltype(j)::value / 4][decltype(j)::value % 4],
+                        __int_as_float(__builtin_amdgcn_update_dpp(v, v, kBroadcast, 0xf, 0xf, true)), x[c]);
+        }
+    };
+    (step(std::integral_constant<int, J>{}), ...);
+}
+
 template <typename TIn, int DK, bool kVec>
-__global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a) {
+__global__ __launch_bounds__(kThreads, sizeof(TIn) * DK <= 256 ? 4 : 2) void delta_solve_kernel(const DeltaArgs a) {
     extern __shared__ __align__(16) unsigned char lds[];
-    __shared__ double G[kChunk];
-    __shared__ float b[kChunk];
+    __shared__ __align__(16) double G[kChunk];
+    __shared__ __align__(16) float b[kChunk];
     using Rows = Tile<TIn, DK>;
     unsigned char *kt = lds, *qt = lds + Rows::kBytes;
-    float* T = reinterpret_cast<float*>(lds);  // over the tiles, once they are read
-    float* Nm = reinterpret_cast<float*>(lds + solve_lds_bytes<TIn, DK>() - kSolveMatrix);
-    const int64_t nc = blockIdx.x, n = nc / a.chunks;
+    // Over the tiles, once they are read.
+    float *T = reinterpret_cast<float*>(lds), *Nm = reinterpret_cast<float*>(lds + kSolveMatrix);
+    const int64_t nc = blockIdx.x, n = blockIdx.x / unsigned(a.chunks);
     const int t0 = int(nc - n * a.chunks) * kChunk;
-    const int64_t len = a.live.of(n, a.T);
+    const int64_t len = a.len_of(n);
     if (t0 >= len) return;
     const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-    const int64_t nk = n / a.group;
+    const int64_t nk = a.key_stream(n);
     auto row_of = [&](const unsigned char* t, int row, int s) { return Rows::load(t, Rows::run_at(row, 4 * s + g)); };
     {
         Stage<TIn, DK, kThreads, kVec> k, q;
         k.init(a.kt, a.dk);
         q.init(a.qt, a.dk);
+        const int64_t at = n * a.T + t0 + min(lane, live - 1);
+        const uint32_t gate = a.gate ? gate_bits(a.gate, at, a.gate_f32) : 0, beta = gate_bits(a.beta, at, a.gate_f32);
         k.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, live, a.dk);
         q.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, live, a.dk);
         if (wave == 0) {
-            const int64_t at = n * a.T + t0 + lane;
-            double s = lane < live && a.gate ? double(log_decay(gate_value(a.gate, at, a.gate_f32), a.form)) * kLog2e : 0.0;
-            s = wave_scan(s);
+            double s = double(log_decay(gate_of(gate, a.gate_f32), a.form)) * kLog2e;
+            s = wave_scan(lane < live && a.gate ? s : 0.0);
             G[lane] = s;
-            const float bv = lane < live ? gate_value(a.beta, at, a.gate_f32) : 0.f;
+            const float bv = lane < live ? gate_of(beta, a.gate_f32) : 0.f;
             b[lane] = bv;
             const double last = __shfl(s, 63);
             float* vec = a.vec + nc * 128;
@@ -98,59 +116,68 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
         q.put(qt);
     }
     __syncthreads();
+    // Row block `wave` of K K^T, `o` of Q K^T, a token's columns in a lane.  bf16 products of the blocks above the diagonal
+    // cost less than branches around them; fp32 ones are left out, five blocks a wave in all.
+    constexpr bool kAll = sizeof(TIn) == 2;
+    const int o = kAll ? wave : 3 - wave;
+    f32x4 kk[4], qk[4];
     {
-        // K K^T: row block `wave`, to N.
-        const int i = wave;
-        for (int j = 0; j <= i; ++j) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        decltype(row_of(kt, 0, 0)) kr[DK / 32], qr[DK / 32];
 #pragma unroll
-            for (int s = 0; s < DK / 32; ++s)
-                acc = mac(row_of(kt, 16 * i + lr, s), row_of(kt, 16 * j + lr, s), acc);
-            const int col = 16 * j + lr;
-            const double gc = G[col];
-            const float bc = b[col];
+        for (int s = 0; s < DK / 32; ++s) kr[s] = row_of(kt, 16 * wave + lr, s), qr[s] = row_of(qt, 16 * o + lr, s);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                const float e = __builtin_amdgcn_exp2f(float(G[row] - gc));
-                Nm[row * kSolvePitch + col] = row > col ? e * acc[r] * bc : 0.f;
+        for (int j = 0; j < 4; ++j) {
+            kk[j] = qk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < DK / 32; ++s) {
+                const auto kj = row_of(kt, 16 * j + lr, s);
+                if (kAll || j <= wave) kk[j] = mac(kj, kr[s], kk[j]);
+                if (kAll || j <= o) qk[j] = mac(kj, qr[s], qk[j]);
             }
-        }
-        // Q K^T: row block 3 - wave (five blocks a wave in all), a token's columns in a lane.
-        const int o = 3 - wave;
-        TIn* mm = static_cast<TIn*>(a.mm) + nc * (kChunk * kChunk);
-        for (int j = 0; j <= (o | 1); ++j) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            if (j <= o) {
-#pragma unroll
-                for (int s = 0; s < DK / 32; ++s)
-                    acc = mac(row_of(kt, 16 * j + lr, s), row_of(qt, 16 * o + lr, s), acc);
-            }
-            const int row = 16 * o + lr, col = 16 * j + 4 * g;
-            const double gr = G[row];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = __builtin_amdgcn_exp2f(float(gr - G[col + r]));
-                acc[r] = row >= col + r ? a.scale * e * acc[r] * b[col + r] : 0.f;
-            }
-            store4_of(mm + row * kChunk + col, acc);
         }
     }
+    // Gam b of a row of block `block` and four columns: kept for N where both are of the same rows.
+    auto weights = [&](int block, int j) {
+        const int col = 16 * j + 4 * g;
+        const double gr = G[16 * block + lr];
+        const double2 g0 = *reinterpret_cast<const double2*>(G + col), g1 = *reinterpret_cast<const double2*>(G + col + 2);
+        const f32x4 e = {float(gr - g0.x), float(gr - g0.y), float(gr - g1.x), float(gr - g1.y)};
+        f32x4 x = *reinterpret_cast<const f32x4*>(b + col);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] *= __builtin_amdgcn_exp2f(e[r]);
+        return x;
+    };
+    auto below = [&](int block, int j, f32x4 x, int first) {  // zero past the row's token, or from it on
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = 16 * block + lr >= 16 * j + 4 * g + r + first ? x[r] : 0.f;
+        return x;
+    };
+    f32x4 gb[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        gb[j] = weights(o, j);
+        if (j <= (o | 1))  // the others are not read
+            store4_of(static_cast<TIn*>(a.mm) + nc * (kChunk * kChunk) + (16 * o + lr) * kChunk + 16 * j + 4 * g,
+                      below(o, j, gb[j] * qk[j] * a.scale, 0));
+        if (!kAll) gb[j] = weights(wave, j);
+    }
     __syncthreads();
-    // (I + N)^-1: the diagonal blocks by substitution, a column a lane, ...
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(Nm + (16 * wave + lr) * kSolvePitch + 16 * j + 4 * g) = below(wave, j, gb[j] * kk[j], 1);
+    __syncthreads();
+    // (I + N)^-1: the diagonal blocks by substitution, rows in the lanes of a row of
+    // 16 and four columns in each, ...
     {
         const int r0 = 16 * wave;
-        float x[16];
+        f32x4 n[4], x;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float s = i == lr ? 1.f : 0.f;
+        for (int j = 0; j < 4; ++j)
+            n[j] = *reinterpret_cast<const f32x4*>(Nm + (r0 + lr) * kSolvePitch + r0 + 4 * j);
 #pragma unroll
-            for (int j = 0; j < i; ++j) s = fmaf(-Nm[(r0 + i) * kSolvePitch + r0 + j], x[j], s);
-            x[i] = s;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if ((i & 3) == g) T[(r0 + i) * kSolvePitch + r0 + lr] = x[i];
+        for (int c = 0; c < 4; ++c) x[c] = lr == 4 * g + c ? 1.f : 0.f;
+        substitute(x, n, std::make_integer_sequence<int, 15>{});
+        *reinterpret_cast<f32x4*>(T + (r0 + lr) * kSolvePitch + r0 + 4 * g) = x;
     }
     __syncthreads();
     // ... then [A 0; C B]^-1 = [A' 0; -B' C A'  B'], of 16 and of 32 rows.
@@ -184,7 +211,11 @@ __global__ __launch_bounds__(kThreads) void delta_solve_kernel(const DeltaArgs a
     const int row = threadIdx.x >> 2, c0 = (threadIdx.x & 3) * 16;
     float x[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = c0 + e <= row ? T[row * kSolvePitch + c0 + e] : 0.f;
+    for (int e = 0; e < 16; e += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(T + row * kSolvePitch + c0 + e);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[e + r] = c0 + e + r <= row ? v[r] : 0.f;
+    }
     TIn* tm = static_cast<TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk) + row * kChunk + c0;
     if constexpr (sizeof(TIn) == 4) {
 #pragma unroll
@@ -237,7 +268,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
     const int width = unit ? a.dk : a.dv, values = unit ? 0 : a.dv - cb * 64;
     const int c0 = (unit ? cb - value_blocks : cb) * 64 + wave * 16, col = c0 + lr;
     const bool active = c0 < width;
-    const int64_t nk = n / a.group, len = a.live.of(n, a.T);
+    const int64_t nk = a.key_stream(n), len = a.len_of(n);
     const int all = int((len + kChunk - 1) / kChunk);
     const int from = min(seg * a.seg_chunks, all), chunks = min(from + a.seg_chunks, all);
     const TIn* kp = static_cast<const TIn*>(a.k) + nk * a.kn;
@@ -470,7 +501,7 @@ template <typename TIn, int V, int R>
 __global__ __launch_bounds__(kThreads) void delta_step_kernel(const DeltaArgs a) {
     constexpr int CQ = 32, RG = kThreads / CQ;
     __shared__ float ks[R * RG], qs[R * RG], sums[4][CQ][2 * V + 1];
-    const int64_t n = blockIdx.y, nk = n / a.group, len = a.live.of(n, a.T);
+    const int64_t n = blockIdx.y, nk = a.key_stream(n), len = a.len_of(n);
     const int cl = threadIdx.x % CQ, rg = threadIdx.x / CQ, wave = threadIdx.x >> 6;
     const int c = (blockIdx.x * CQ + cl) * V;
     const bool in = c < a.dv;

@@ -397,6 +397,15 @@ struct DeltaArgs {
     int gate_f32, form;
     int vec_k, vec_v, vec_o;  // rows of q and k, of v, of out (and dout) in 16-byte pieces
     float scale;
+
+    // Streams and their chunks have 32 bits: divisions of 64 take hundreds of instructions
+    // before a workgroup's first load.
+    __device__ __forceinline__ int64_t key_stream(int64_t n) const { return unsigned(n) / unsigned(group); }
+    __device__ __forceinline__ int64_t len_of(int64_t n) const {
+        if (!live.lengths) return T;
+        const int64_t len = live.lengths[unsigned(n) / unsigned(live.group)];
+        return len < 0 ? 0 : len < T ? len : T;
+    }
 };
 
 // Log decays below this are taken as this: e^-200 is zero in 32 bits, and a sum
