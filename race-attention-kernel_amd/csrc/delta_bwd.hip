@@ -86,10 +86,11 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
 
     f32x4 dS[DK / 16];
     if (behind) {
+        const StateView from(behind, a.dk, a.dv);
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) dS[i][r] = state_value(behind, tok(i, 4 * g + r), col, a.dk, a.dv);
+            for (int r = 0; r < 4; ++r) dS[i][r] = from.one(tok(i, 4 * g + r), col);
     } else {
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i) dS[i] = f32x4{0.f, 0.f, 0.f, 0.f};

@@ -281,10 +281,11 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
 
     f32x4 S[DK / 16];
     if (start && !unit) {
+        const StateView from(start, a.dk, a.dv);
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[i][r] = state_value(start, tok(i, 4 * g + r), col, a.dk, a.dv);
+            for (int r = 0; r < 4; ++r) S[i][r] = from.one(tok(i, 4 * g + r), col);
     } else {
 #pragma unroll
         for (int i = 0; i < DK / 16; ++i)
@@ -507,17 +508,16 @@ __global__ __launch_bounds__(kThreads) void delta_step_kernel(const DeltaArgs a)
     const bool in = c < a.dv;
     float S[R][V];
     if (a.state) {
-        const float* from = a.state + n * a.dk * a.dv;
+        const StateView from(a.state + n * a.dk * a.dv, a.dk, a.dv);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int row = i * RG + rg;
             if constexpr (V == 4) {
-                const float4 s = *reinterpret_cast<const float4*>(from + min(row, a.dk - 1) * a.dv + min(c, a.dv - 4));
-                const bool there = in && row < a.dk;
-                S[i][0] = there ? s.x : 0.f, S[i][1] = there ? s.y : 0.f;
-                S[i][2] = there ? s.z : 0.f, S[i][3] = there ? s.w : 0.f;
+                const f32x4 s = from.four(row, c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) S[i][j] = s[j];
             } else {
-                S[i][0] = state_value(from, row, c, a.dk, a.dv);
+                S[i][0] = from.one(row, c);
             }
         }
     } else {

@@ -431,12 +431,23 @@ __device__ __forceinline__ void store4_of(bf16_t* p, const f32x4& x) {
     *reinterpret_cast<uint2*>(p) = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
 }
 
-// Value (row, col) of a state [dk][dv] (nullable), zero outside: read from the nearest
-// place within and chosen after, so that a wave's 32 loads have no branches between them.
-__device__ __forceinline__ float state_value(const float* s, int row, int col, int dk, int dv) {
-    const float x = s[min(row, dk - 1) * dv + min(col, dv - 1)];
-    return row < dk && col < dv ? x : 0.f;
-}
+// Values (row, col) of a state [dk][dv], zero outside, through a buffer that ends with
+// it: a value chosen after its load would get a branch around the load and a wait
+// behind it, 32 of them at the start of a walk.
+struct StateView {
+    __amdgpu_buffer_rsrc_t r;
+    int dk, dv;
+    __device__ __forceinline__ StateView(const float* s, int dk, int dv)
+        : r(mfma::make_rsrc(s, int64_t(dk) * dv * 4)), dk(dk), dv(dv) {}
+    __device__ __forceinline__ float one(int row, int col) const {
+        const int off = row < dk && col < dv ? (row * dv + col) * 4 : mfma::kOutside;
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    }
+    __device__ __forceinline__ f32x4 four(int row, int col) const {  // dv a multiple of 4
+        const int off = row < dk && col < dv ? (row * dv + col) * 4 : mfma::kOutside;
+        return __builtin_bit_cast(f32x4, mfma::buf_load16<mfma::kPolicyDefault>(r, off));
+    }
+};
 
 // Whether two workgroups that walk chunks share a CU, each with one buffer, as narrow
 // keys' registers and tiles allow, and the maps' (no Q and M).  192 streams of 577
@@ -468,8 +479,7 @@ __device__ __forceinline__ bool stream_and_block(int64_t N, int blocks, int64_t&
 // starts[0] = the state, starts[p + 1] = map_a[p] starts[p] + map_x[p], the first
 // segment's map_x being what follows it; backward (kBack) from the last segment on,
 // with the maps transposed.  Products are fp32.  A workgroup has 16 columns
-// and a wave a quarter of the rows, whose part of the next segment's maps it loads
-// meanwhile; the columns meet in LDS, two copies in turn.
+// and a wave a quarter of the rows, whose part of the maps it loads two segments ahead; the columns meet in LDS, two copies in turn.
 template <int DK, bool kBack>
 __global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a) {
     constexpr int NI = DK / 64, NJ = DK / 16, kPitch = DK + 4;
@@ -478,17 +488,21 @@ __global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a)
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
     const int col = blockIdx.x * 16 + lr, r0 = wave * (DK / 4);
     const bool whole = a.dk % 4 == 0;
-    f32x4 S[NI], X[NI], A[NI][NJ];  // rows r0 + 16 i + 4 g + r; rows r0 + 16 i + lr, columns 16 j + 4 g + r
+    struct Maps {
+        f32x4 X[NI], A[NI][NJ];  // rows r0 + 16 i + 4 g + r; rows r0 + 16 i + lr, columns 16 j + 4 g + r
+    } even, odd;
+    f32x4 S[NI];
     auto rows = [&](const float* p, f32x4 (&x)[NI]) {
+        const StateView s(p, a.dk, a.dv);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[i][r] = state_value(p, r0 + 16 * i + 4 * g + r, col, a.dk, a.dv);
+            for (int r = 0; r < 4; ++r) x[i][r] = s.one(r0 + 16 * i + 4 * g + r, col);
     };
-    auto load = [&](int p) {
+    auto load = [&](Maps& m, int p) {
         const int64_t at = n * a.segs + p;
-        rows(a.map_x + at * a.dk * a.dv, X);
-        const float* m = a.map_a + at * a.dk * a.dk;
+        rows(a.map_x + at * a.dk * a.dv, m.X);
+        const StateView from(a.map_a + at * a.dk * a.dk, a.dk, a.dk);
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -496,14 +510,12 @@ __global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a)
                 const int row = r0 + 16 * i + lr, c = 16 * j + 4 * g;
                 if constexpr (kBack) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) A[i][j][r] = state_value(m, c + r, row, a.dk, a.dk);
+                    for (int r = 0; r < 4; ++r) m.A[i][j][r] = from.one(c + r, row);
                 } else if (whole) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(m + min(row, a.dk - 1) * a.dk + min(c, a.dk - 4));
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) A[i][j][r] = row < a.dk && c < a.dk ? x[r] : 0.f;
+                    m.A[i][j] = from.four(row, c);
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) A[i][j][r] = state_value(m, row, c + r, a.dk, a.dk);
+                    for (int r = 0; r < 4; ++r) m.A[i][j][r] = from.one(row, c + r);
                 }
             }
     };
@@ -514,9 +526,8 @@ __global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a)
         for (int i = 0; i < NI; ++i) S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     auto segment = [&](int step) { return kBack ? a.segs - 1 - step : step; };
-    rows(a.map_x + (n * a.segs + segment(0)) * a.dk * a.dv, X);
-    for (int step = 0; step < a.segs; ++step) {
-        float* to = a.starts + (n * a.segs + segment(step)) * a.dk * a.dv;
+    auto step = [&](int p, Maps& m) {
+        float* to = a.starts + (n * a.segs + segment(p)) * a.dk * a.dv;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -524,9 +535,9 @@ __global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a)
                 const int row = r0 + 16 * i + 4 * g + r;
                 if (col < a.dv && row < a.dk) to[row * a.dv + col] = S[i][r];
             }
-        if (step + 1 == a.segs) return;
-        if (step > 0) {
-            float* c = cols[step & 1];
+        if (p + 1 == a.segs) return;
+        if (p > 0) {
+            float* c = cols[p & 1];
 #pragma unroll
             for (int i = 0; i < NI; ++i) *reinterpret_cast<f32x4*>(c + lr * kPitch + r0 + 16 * i + 4 * g) = S[i];
             __syncthreads();
@@ -536,12 +547,18 @@ __global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a)
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) X[i] = mfma::mfma4(A[i][j][r], s[r], X[i]);
+                    for (int r = 0; r < 4; ++r) m.X[i] = mfma::mfma4(m.A[i][j][r], s[r], m.X[i]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < NI; ++i) S[i] = X[i];
-        if (step + 2 < a.segs) load(segment(step + 1));
+        for (int i = 0; i < NI; ++i) S[i] = m.X[i];
+        if (p + 3 < a.segs) load(m, segment(p + 2));
+    };
+    rows(a.map_x + (n * a.segs + segment(0)) * a.dk * a.dv, even.X);
+    if (a.segs > 2) load(odd, segment(1));
+    for (int p = 0; p < a.segs; p += 2) {
+        step(p, even);
+        if (p + 1 < a.segs) step(p + 1, odd);
     }
 }
 
