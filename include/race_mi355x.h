@@ -674,7 +674,7 @@ typedef struct race_delta_shape {
     int32_t gate_form;      /* race_gate; log gates are at most 0, those below -200 count as -200 */
     int32_t lengths_group;  /* value streams that share one entry of `lengths`, >= 1 */
     float scale;
-    /* Strides in elements, the values of a row next to each other; token strides up to 2^30. */
+    /* Strides in elements, the values of a row next to each other; token strides up to 2^22. */
     int64_t q_stream_stride, q_token_stride, k_stream_stride, k_token_stride, v_stream_stride, v_token_stride;
 } race_delta_shape;
 

@@ -107,12 +107,12 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     auto fetch = [&](int c, int part) {  // as the forward's
         const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
-        if (part == 0) sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
-        if (part == 1) sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
+        if (part == 0) sk.load(kp + t0 * a.kt, live);
+        if (part == 1) sq.load(qp + t0 * a.qt, live);
         if (part == 2) stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
         if (part == 3) {
             smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
-            so.load(op + t0 * a.dv, a.dv, live, a.dv - cb * 64);
+            so.load(op + t0 * a.dv, live);
             svec = a.vec[nc * 128 + (threadIdx.x & 127)];
         }
     };
@@ -319,9 +319,15 @@ struct Pieces {
 template <typename TIn, int K, int NT, bool kVec>
 struct RowPieces {
     static constexpr int kVecs = Eight<TIn>::kVecs, kTotal = kChunk * (K / 8), kPer = (kTotal + NT - 1) / NT;
-    Eight<TIn> x[kPer];
+    std::conditional_t<kVec, Eight<TIn>, Ragged<TIn>> x[kPer];
+    int stride_, width_, at_;  // of the rows loaded
     __device__ __forceinline__ void load(const TIn* p, int64_t stride, int live, int width, int tid) {
-        const auto r = mfma::make_rsrc(p, ((live - 1) * stride + width) * int(sizeof(TIn)));
+        stride_ = int(stride), width_ = width, at_ = 0;
+        __amdgpu_buffer_rsrc_t r;
+        if constexpr (kVec)
+            r = mfma::make_rsrc(p, ((live - 1) * stride + width) * int(sizeof(TIn)));
+        else
+            r = ragged_view(p, stride, live, width, at_);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int q = tid + i * NT, row = q / (K / 8), u = q % (K / 8);
@@ -329,9 +335,9 @@ struct RowPieces {
             if constexpr (kVec) {
 #pragma unroll
                 for (int j = 0; j < kVecs; ++j)
-                    x[i].v[j] = mfma::buf_load16<mfma::kPolicyDefault>(r, piece_at<TIn>(row, int(stride), 8 * u + 4 * j, width));
+                    x[i].v[j] = mfma::buf_load16<mfma::kPolicyDefault>(r, piece_at<TIn>(row, stride_, 8 * u + 4 * j, width));
             } else {
-                x[i].load(p + row * stride + 8 * u, row < live ? width - 8 * u : 0);
+                x[i].load(r, at_ + row * stride_, 8 * u, width, row < live);
             }
         }
     }
@@ -340,8 +346,13 @@ struct RowPieces {
         for (int i = 0; i < kPer; ++i) {
             const int q = tid + i * NT, row = q / (K / 8), u = q % (K / 8);
             if (kTotal % NT != 0 && q >= kTotal) continue;
+            Eight<TIn> e;
+            if constexpr (kVec)
+                e = x[i];
+            else
+                e = x[i].get(at_ + row * stride_, 8 * u, width_);
 #pragma unroll
-            for (int j = 0; j < kVecs; ++j) *reinterpret_cast<uint4*>(t + Tile<TIn, K>::at(row, kVecs * u + j)) = x[i].v[j];
+            for (int j = 0; j < kVecs; ++j) *reinterpret_cast<uint4*>(t + Tile<TIn, K>::at(row, kVecs * u + j)) = e.v[j];
         }
     }
 };

@@ -99,8 +99,8 @@ __global__ __launch_bounds__(kThreads, sizeof(TIn) * DK <= 256 ? 4 : 2) void del
         q.init(a.qt, a.dk);
         const int64_t at = n * a.T + t0 + min(lane, live - 1);
         const uint32_t gate = a.gate ? gate_bits(a.gate, at, a.gate_f32) : 0, beta = gate_bits(a.beta, at, a.gate_f32);
-        k.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, a.kt, live, a.dk);
-        q.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, a.qt, live, a.dk);
+        k.load(static_cast<const TIn*>(a.k) + nk * a.kn + t0 * a.kt, live);
+        q.load(static_cast<const TIn*>(a.q) + nk * a.qn + t0 * a.qt, live);
         if (wave == 0) {
             double s = double(log_decay(gate_of(gate, a.gate_f32), a.form)) * kLog2e;
             s = wave_scan(lane < live && a.gate ? s : 0.0);
@@ -305,12 +305,12 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
     auto fetch = [&](int c, int part) {
         const int64_t nc = n * a.chunks + c, t0 = int64_t(c) * kChunk;
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
-        if (part == 0) sk.load(kp + t0 * a.kt, a.kt, live, a.dk);
-        if (part == 1 && kMode != kMaps) sq.load(qp + t0 * a.qt, a.qt, live, a.dk);
+        if (part == 0) sk.load(kp + t0 * a.kt, live);
+        if (part == 1 && kMode != kMaps) sq.load(qp + t0 * a.qt, live);
         if (part == 2) stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
         if (part == 3) {
             if (kMode != kMaps) smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
-            sv.load(vp + t0 * a.vt, a.vt, live, values);
+            sv.load(vp + t0 * a.vt, live);
             svec = a.vec[nc * 128 + (threadIdx.x & 127)];
         }
     };
@@ -451,23 +451,23 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
 #pragma unroll
         for (int b = 2; b < 4; ++b) o[b] = mac(y[1], mg[b - 2], o[b]);
         const int64_t t0 = int64_t(c) * kChunk;
-        if constexpr (kVec) {
-            // Rows past the last live one lie outside the view.
-            const int rows = int(len - t0 < kChunk ? len - t0 : kChunk);
-            const auto out = mfma::make_rsrc(op + t0 * a.dv, int64_t(rows) * a.dv * int(sizeof(TIn)));
-            const bool there = c0 + 4 * g < a.dv;
+        // Rows past the last live one lie outside the view.
+        const int rows = int(len - t0 < kChunk ? len - t0 : kChunk), bytes = int(sizeof(TIn));
+        const auto out = mfma::make_rsrc(op + t0 * a.dv, int64_t(rows) * a.dv * bytes);
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-                mfma::store4<TIn, mfma::kPolicyDefault>(
-                    out, there ? (tok(b, lr) * a.dv + c0 + 4 * g) * int(sizeof(TIn)) : mfma::kOutside, o[b]);
-        } else {
+        for (int b = 0; b < 4; ++b) {
+            const int at = (tok(b, lr) * a.dv + c0 + 4 * g) * bytes, there = a.dv - c0 - 4 * g;
+            if constexpr (kVec) {
+                mfma::store4<TIn, mfma::kPolicyDefault>(out, there > 0 ? at : mfma::kOutside, o[b]);
+            } else {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int64_t t = t0 + tok(b, lr);
-                if (t >= len) continue;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (c0 + 4 * g + r < a.dv) store_val(op + t * a.dv + c0 + 4 * g + r, o[b][r]);
+                for (int r = 0; r < 4; ++r) {
+                    const int off = r < there ? at + r * bytes : mfma::kOutside;
+                    if constexpr (sizeof(TIn) == 4)
+                        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[b][r]), out, off, 0, 0);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b16(f32_to_bf16(o[b][r]), out, off, 0, 0);
+                }
             }
         }
     }

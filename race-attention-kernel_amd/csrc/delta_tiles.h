@@ -278,27 +278,85 @@ struct Tile {
 template <typename E, int K>
 constexpr int kTwoBytes = sizeof(E) == 4 ? Tile<E, K>::kBytes : 2 * Tile<E, K>::kBytes;
 
-// Eight consecutive values of a row, of which the first `n` are there, one by one.
+// Eight consecutive values of a row.
 template <typename TIn>
 struct Eight {
     static constexpr int kVecs = int(sizeof(TIn)) / 2;
     uint4 v[kVecs];
-    __device__ __forceinline__ void load(const TIn* p, int n) {
-        uint32_t w[4 * kVecs];
+};
+
+// Eight values of a row, from column c on, wherever the row starts: zeros from its
+// `width` on, and a row that is not there is one of zeros.  It is at element `at` of a
+// view.  Offsets past the view's end stand for what is not there (a branch
+// would wait for every load), and what has come is put in place when it is wanted.
+template <typename TIn>
+struct Ragged;
+
+// In pieces of four; the row's last is read as the four values that end it.
+template <>
+struct Ragged<float> {
+    f32x4 x[2];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int at, int c, int width, bool there) {
 #pragma unroll
-        for (int i = 0; i < 4 * kVecs; ++i) w[i] = 0;
+        for (int i = 0; i < 2; ++i, c += 4) {
+            if (width >= 4) {
+                const int off = there && c < width ? (at + min(c, width - 4)) * 4 : mfma::kOutside;
+                x[i] = __builtin_bit_cast(f32x4, mfma::buf_load16<mfma::kPolicyDefault>(r, off));
+            } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (i >= n) break;
-            if constexpr (kVecs == 2)
-                w[i] = __float_as_uint(p[i]);
-            else
-                w[i >> 1] |= uint32_t(p[i]) << (16 * (i & 1));
+                for (int e = 0; e < 4; ++e) {
+                    const int off = there && c + e < width ? (at + c + e) * 4 : mfma::kOutside;
+                    x[i][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+                }
+            }
         }
+    }
+    __device__ __forceinline__ Eight<float> get(int, int c, int width) const {
+        Eight<float> out;
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        for (int i = 0; i < 2; ++i, c += 4) {
+            f32x4 v = x[i];
+            const int by = width >= 4 && c < width ? max(c + 4 - width, 0) : 0;
+            if (by & 1) v = f32x4{v[1], v[2], v[3], 0.f};
+            if (by & 2) v = f32x4{v[2], v[3], 0.f, 0.f};
+            out.v[i] = __builtin_bit_cast(uint4, v);
+        }
+        return out;
     }
 };
+
+// Through the words they lie in.
+template <>
+struct Ragged<bf16_t> {
+    uint32_t w[5];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int at, int c, int width, bool there) {
+        const int odd = at & 1, n = there && width > c ? width - c : -5;
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, 2 * i - odd < n ? (at + c - odd + 2 * i) * 2 : mfma::kOutside, 0, 0);
+    }
+    __device__ __forceinline__ Eight<bf16_t> get(int at, int c, int width) const {
+        Eight<bf16_t> out;
+        uint32_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = width - c - 2 * i;
+            x[i] = __builtin_amdgcn_alignbit(w[i + 1], w[i], 16 * (at & 1));
+            x[i] = n > 1 ? x[i] : n > 0 ? x[i] & 0xffffu : 0u;
+        }
+        out.v[0] = make_uint4(x[0], x[1], x[2], x[3]);
+        return out;
+    }
+};
+
+// A view of `live` rows from p on for them, and the element of it that p is: from the
+// word that p lies in to the end of the last one (arrays start 16-byte aligned).
+template <typename TIn>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t ragged_view(const TIn* p, int64_t stride, int live, int width, int& at) {
+    at = int(reinterpret_cast<uintptr_t>(p) & 3) / int(sizeof(TIn));
+    const int64_t bytes = ((live - 1) * stride + width + at) * int(sizeof(TIn));
+    return mfma::make_rsrc(p - at, (bytes + 3) & ~int64_t(3));
+}
 
 // Byte offset of the 16-byte piece from column `col` of a row; outside every view past the row's width.
 template <typename TIn>
@@ -307,14 +365,20 @@ __device__ __forceinline__ int piece_at(int row, int stride, int col, int width)
 }
 
 // 64 rows of K values: each thread's 8-value pieces in registers and then in a tile.
-// kVec: rows in 16-byte pieces, read through a view that ends with the last live
-// row; else value by value.
+// Through a view that ends with the last live row: in 16-byte pieces (kVec), or
+// value by value.
 template <typename TIn, int K, int NT, bool kVec>
 struct Stage {
     static constexpr int kPer = kChunk * (K / 8) / NT, kVecs = Eight<TIn>::kVecs;
-    Eight<TIn> x[kPer];
+    std::conditional_t<kVec, Eight<TIn>, Ragged<TIn>> x[kPer];
     int off[kVec ? kPer * kVecs : 1];
+    int stride_, width_, at_;  // of the rows loaded
+    // Wide rows compute the offsets of their values each time: kept, they take the registers that
+    // the products need (32 streams of 3000 fp32 tokens, 100 x 127: the walk 269 -> 185 us; 96
+    // of 1500 bf16 ones, 33 x 50: kept 97, again 112).
+    static constexpr bool kAgain = K * sizeof(TIn) > 128;
     __device__ __forceinline__ void init(int64_t stride, int width) {
+        stride_ = int(stride), width_ = width;
         if constexpr (kVec) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
@@ -324,29 +388,38 @@ struct Stage {
             }
         }
     }
-    // Rows of p by stride, `live` of them there, `width` values each.
-    __device__ __forceinline__ void load(const TIn* p, int64_t stride, int live, int width) {
+    // Rows of p, `live` of them there.
+    __device__ __forceinline__ void load(const TIn* p, int live) {
         if constexpr (kVec) {
-            const auto r = mfma::make_rsrc(p, ((live - 1) * stride + width) * int(sizeof(TIn)));
+            const auto r = mfma::make_rsrc(p, ((live - 1) * int64_t(stride_) + width_) * int(sizeof(TIn)));
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
 #pragma unroll
                 for (int j = 0; j < kVecs; ++j) x[i].v[j] = mfma::buf_load16<mfma::kPolicyDefault>(r, off[i * kVecs + j]);
         } else {
+            const auto r = ragged_view(p, stride_, live, width_, at_);
+            int tid = threadIdx.x;
+            if constexpr (kAgain) asm volatile("" : "+v"(tid));
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int q = int(threadIdx.x) + i * NT, row = q / (K / 8), u = q % (K / 8);
-                x[i].load(p + row * stride + 8 * u, row < live ? width - 8 * u : 0);
+                const int q = tid + i * NT, row = q / (K / 8), u = q % (K / 8);
+                x[i].load(r, at_ + row * stride_, 8 * u, width_, row < live);
             }
         }
     }
     __device__ __forceinline__ void put(unsigned char* t) const {
+        int tid = threadIdx.x;
+        if constexpr (!kVec && kAgain) asm volatile("" : "+v"(tid));
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int q = int(threadIdx.x) + i * NT, row = q / (K / 8), u = q % (K / 8);
+            const int q = tid + i * NT, row = q / (K / 8), u = q % (K / 8);
+            Eight<TIn> e;
+            if constexpr (kVec)
+                e = x[i];
+            else
+                e = x[i].get(at_ + row * stride_, 8 * u, width_);
 #pragma unroll
-            for (int j = 0; j < kVecs; ++j)
-                *reinterpret_cast<uint4*>(t + Tile<TIn, K>::at(row, kVecs * u + j)) = x[i].v[j];
+            for (int j = 0; j < kVecs; ++j) *reinterpret_cast<uint4*>(t + Tile<TIn, K>::at(row, kVecs * u + j)) = e.v[j];
         }
     }
 };
@@ -574,11 +647,6 @@ inline bool whole_pieces(const DeltaRule& r, int64_t width, std::initializer_lis
         if (s % v != 0) return false;
     return true;
 }
-inline bool near_rows(std::initializer_list<int64_t> token_strides) {
-    for (int64_t s : token_strides)
-        if (s > (int64_t(1) << 22)) return false;
-    return true;
-}
 
 inline DeltaArgs delta_args(const DeltaRule& r, const DeltaInputs& in) {
     DeltaArgs a = {};
@@ -589,8 +657,8 @@ inline DeltaArgs delta_args(const DeltaRule& r, const DeltaInputs& in) {
     a.group = r.Nk > 0 ? int(r.N / r.Nk) : 1;
     a.dk = r.dk, a.dv = r.dv, a.dvp = (r.dv + 15) / 16 * 16, a.chunks = int(delta_chunks(r));
     a.gate_f32 = r.gate_dtype == RACE_F32, a.form = r.form;
-    a.vec_k = whole_pieces(r, r.dk, {r.qn, r.qt, r.kn, r.kt}) && near_rows({r.qt, r.kt});
-    a.vec_v = whole_pieces(r, r.dv, {r.vn, r.vt}) && near_rows({r.vt});
+    a.vec_k = whole_pieces(r, r.dk, {r.qn, r.qt, r.kn, r.kt});
+    a.vec_v = whole_pieces(r, r.dv, {r.vn, r.vt});
     a.vec_o = whole_pieces(r, r.dv, {});
     a.scale = r.scale;
     return a;

@@ -2239,7 +2239,7 @@ bool delta_shape(const race_delta_shape* sh, const int32_t* lengths, DeltaRule* 
     for (int64_t s : {sh->q_stream_stride, sh->k_stream_stride, sh->v_stream_stride})
         if (s < 0 || s > (int64_t(1) << 40)) return false;
     for (int64_t s : {sh->q_token_stride, sh->k_token_stride, sh->v_token_stride})
-        if (s < 0 || s > (int64_t(1) << 30)) return false;
+        if (s < 0 || s > (int64_t(1) << 22)) return false;  // 64 rows within a 32-bit offset
     *r = DeltaRule{sh->value_streams,   sh->key_streams,    sh->seq_len,         sh->key_dim,        sh->value_dim,
                    sh->q_stream_stride, sh->q_token_stride, sh->k_stream_stride, sh->k_token_stride, sh->v_stream_stride,
                    sh->v_token_stride,  sh->dtype,          sh->gate_dtype,      sh->gate_form,      sh->scale,

@@ -208,7 +208,7 @@ race_delta_shape delta_shape(const char* entry, const at::Tensor& q, const at::T
     return sh;
 }
 
-constexpr int64_t kDeltaFar = int64_t(1) << 30;  // the largest token stride
+constexpr int64_t kDeltaFar = int64_t(1) << 22;  // the largest token stride; a copy past it
 
 // q or k as rows [N, T, dk]: bucket probabilities [N, T, L, R] are rows of L R.
 at::Tensor as_key_rows(const at::Tensor& t) { return as_rows(t.dim() == 4 ? t.flatten(2) : t, kDeltaFar); }

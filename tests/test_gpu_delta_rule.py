@@ -629,3 +629,21 @@ def test_offsets_past_32_bits(race, cuda):
         # Chunks start at other tokens: both sides are rounded, independently.
         assert (a - b).norm() <= 2 ** 0.5 * 2.0 ** -7 * b.norm(), name
     assert (final - final2).norm() <= 2 ** 0.5 * 2.0 ** -15 * final2.norm()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("stride", [1 << 22, (1 << 22) - 1, (1 << 22) + 1])
+@pytest.mark.parametrize("T", [5, 70])
+def test_the_longest_token_stride(race, cuda, T, stride, dtype):
+    # Rows up to 2^22 values apart are read in place, those further apart from a copy.
+    *args, _, _ = make(2, 2, T, 33, 48, dtype, seed=22)
+    want = race.race_delta_rule_carry(*args)
+    wide = torch.full((T * stride + 64,), math.nan, dtype=dtype, device=cuda)
+    view = lambda t: torch.as_strided(wide, t.shape, (96, stride, 1))
+    for i in range(3):
+        moved = list(args)
+        moved[i] = view(args[i])
+        moved[i].copy_(args[i])
+        got = race.race_delta_rule_carry(*moved)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+        wide.fill_(math.nan)
