@@ -34,7 +34,7 @@ __device__ __forceinline__ void load_weight_run(float (&x)[V], const void* w, in
     for (int i = 0; i < V; ++i) x[i] = in ? 1.f : 0.f;
     if (!w || !in) return;
     if (w_f32) {
-        constexpr int kPer = V >= 4 ? 4 : 1;
+        constexpr int kPer = V >= 4 ? 4 : V;
 #pragma unroll
         for (int i = 0; i < V; i += kPer) {
             Run<float, kPer> r;
@@ -147,6 +147,8 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&y)[V], floa
             *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
         else
             *reinterpret_cast<uint32_t*>(p) = w[0];
+    } else if constexpr (V == 2) {
+        *reinterpret_cast<uint16_t*>(p) = uint16_t(__builtin_amdgcn_cvt_pk_fp8_f32(y[0] * f, y[1] * f, 0, false));
     } else {
         *p = uint8_t(__builtin_amdgcn_cvt_pk_fp8_f32(y[0] * f, 0.f, 0, false) & 0xff);
     }
@@ -335,10 +337,12 @@ hipError_t launch_column_sums(const float* partial, int rows, int d, void* out, 
 // Whether the rows' pieces of `v` values lie at multiples of their size.
 bool add_norm_whole(const AddNorm& n, int v) { return n.D % v == 0 && n.xs % v == 0 && n.rs % v == 0; }
 int add_norm_vector(const AddNorm& n) {
-    if (n.dtype == RACE_BF16) return add_norm_whole(n, 8) ? 8 : 1;
-    return add_norm_whole(n, 4) ? 4 : 1;
+    const int wide = n.dtype == RACE_BF16 ? 8 : 4;
+    return add_norm_whole(n, wide) ? wide : add_norm_whole(n, 2) ? 2 : 1;
 }
 
+// Pieces of 16 bytes where the rows lie so, else of two values or one: 16384 bf16 rows of
+// 1000 / 1002 / 1001 values, forward and backward, 47 / 58 / 111 us.
 // f(V, NP, NT) as compile-time values for rows of D values in pieces of v: a wave
 // a row while it holds the row in 4 pieces a lane, then a workgroup.
 template <int V, typename F>
@@ -354,9 +358,16 @@ hipError_t by_row(int D, F f) {
     if (pieces <= 256) return call(integral_constant<int, 4>{}, wave);
     if (pieces <= 512) return call(integral_constant<int, 2>{}, four);
     if (pieces <= 1024) return call(integral_constant<int, 4>{}, four);
-    if (pieces <= 2048) return call(integral_constant<int, 2>{}, all);
-    if (V > 1 || pieces <= 4096) return call(integral_constant<int, 4>{}, all);
-    return call(integral_constant<int, 16>{}, all);
+    if constexpr (V == 1) {
+        if (pieces > 8192) return call(integral_constant<int, 16>{}, all);
+    }
+    if constexpr (V <= 2) {
+        if (pieces > 4096) return call(integral_constant<int, 8>{}, all);
+    }
+    if constexpr (V <= 4) {
+        if (pieces > 2048) return call(integral_constant<int, 4>{}, all);
+    }
+    return call(integral_constant<int, 2>{}, all);
 }
 
 // Rows of a workgroup of by_row's shape.
@@ -365,6 +376,9 @@ int rows_of_workgroup(const AddNorm& n) {
     return (n.D + v - 1) / v <= 256 ? 4 : 1;
 }
 
+// Workgroups that walk over the rows.  Backward, half as many: 9235 rows of 1001 fp32 values
+// 34 us against 27; twice as many: 29.  Forward, 1024 .. 4096 are alike (32768 x 2048 bf16: 89 .. 92 us,
+// 537 MB; backward 116 us).
 constexpr int kAddNormFwdWorkgroups = 2048, kAddNormBwdWorkgroups = 1024;
 
 unsigned add_norm_grid(const AddNorm& n, int most) {
@@ -385,7 +399,8 @@ AddNormArgs add_norm_args(const AddNorm& n, const void* x, const void* w) {
 template <typename TIn, typename F>
 hipError_t by_piece(const AddNorm& n, F f) {
     constexpr int kWide = sizeof(TIn) == 2 ? 8 : 4;
-    return add_norm_vector(n) > 1 ? by_row<kWide>(n.D, f) : by_row<1>(n.D, f);
+    const int v = add_norm_vector(n);
+    return v == kWide ? by_row<kWide>(n.D, f) : v == 2 ? by_row<2>(n.D, f) : by_row<1>(n.D, f);
 }
 
 template <typename TIn>
@@ -453,8 +468,16 @@ __global__ __launch_bounds__(kThreads) void gate_norm_kernel(const GateNormArgs 
     for (int64_t first = int64_t(blockIdx.x) * per; first < a.rows; first += int64_t(gridDim.x) * per) {
         const int64_t row = first + r0;
         const bool there = row < a.rows;
-        const int64_t bt = row / a.H, b = bt / a.T;
-        const int h = int(row - bt * a.H), t = int(bt - b * a.T);
+        int64_t b;
+        int t, h;
+        if (a.rows < (int64_t(1) << 31)) {  // divisions of 64 bits would cost more than the rest of a short row
+            const unsigned bt = unsigned(row) / unsigned(a.H), b32 = bt / unsigned(a.T);
+            h = int(unsigned(row) - bt * a.H), t = int(bt - b32 * a.T), b = b32;
+        } else {
+            const int64_t bt = row / a.H;
+            b = bt / a.T;
+            h = int(row - bt * a.H), t = int(bt - b * a.T);
+        }
         const TIn* xp = static_cast<const TIn*>(a.x) + (b * a.H + h) * a.xn + t * a.xt;
         const TIn* zp = static_cast<const TIn*>(a.z) + b * a.zb + t * a.zt + h * a.zh;
         X x[NS], z[NS], up[NS];
@@ -528,18 +551,24 @@ int gate_norm_vector(const GateNorm& n) {
             if (s % v != 0) return false;
         return true;
     };
-    if (n.dtype == RACE_BF16) return whole(8) ? 8 : 1;
-    return whole(4) ? 4 : 1;
+    const int wide = n.dtype == RACE_BF16 ? 8 : 4;
+    return whole(wide) ? wide : whole(2) ? 2 : 1;
 }
 
+// Lanes of a row: one for each wide piece, or for four narrow ones, so that short rows
+// leave a workgroup more of them (262144 rows of 33 bf16 values, forward and backward:
+// a piece a lane 75 + 137 us, four 35 + 57).
+constexpr int kNarrowPieces = 4;
 int lane_shift_of(const GateNorm& n) {
-    const int v = gate_norm_vector(n), pieces = (n.d + v - 1) / v;
+    const int v = gate_norm_vector(n), each = v >= 4 ? 1 : kNarrowPieces, pieces = (n.d + v * each - 1) / (v * each);
     int k = 0;
     while (k < 6 && (1 << k) < pieces) ++k;
     return k;
 }
 
-constexpr int kGateNormFwdWorkgroups = 2048, kGateNormBwdWorkgroups = 1024;
+// As add_norm's.  [16 * 12, 577, 96] fp32: forward with 1024 35 us, with 2048 or 4096 28; backward
+// with 512, 1024 and 2048 65, 46 and 38.  [8 * 16, 4096, 128] bf16: 92 and 137 us.
+constexpr int kGateNormFwdWorkgroups = 2048, kGateNormBwdWorkgroups = 2048;
 
 template <bool kBack>
 hipError_t launch_gate_norm_any(const GateNorm& n, GateNormArgs a, int most, unsigned* workgroups, hipStream_t stream) {
@@ -551,18 +580,20 @@ hipError_t launch_gate_norm_any(const GateNorm& n, GateNormArgs a, int most, uns
     const unsigned grid = unsigned(std::min<int64_t>((a.rows + per - 1) / per, most));
     *workgroups = grid;
     const size_t lds = kBack && a.partial ? size_t(per) * n.d * sizeof(float) : 0;
-    const bool wide = gate_norm_vector(n) > 1;
-    if (n.dtype == RACE_BF16) {
-        if (wide)
-            gate_norm_kernel<bf16_t, 8, 1, kBack><<<grid, kThreads, lds, stream>>>(a);
-        else
-            gate_norm_kernel<bf16_t, 1, 4, kBack><<<grid, kThreads, lds, stream>>>(a);
-    } else if (wide) {
-        gate_norm_kernel<float, 4, 1, kBack><<<grid, kThreads, lds, stream>>>(a);
-    } else {
-        gate_norm_kernel<float, 1, 4, kBack><<<grid, kThreads, lds, stream>>>(a);
-    }
-    return hipGetLastError();
+    const int v = gate_norm_vector(n);
+    auto launch = [&](auto type, auto pieces, auto per_lane) {
+        gate_norm_kernel<decltype(type), decltype(pieces)::value, decltype(per_lane)::value, kBack>
+            <<<grid, kThreads, lds, stream>>>(a);
+        return hipGetLastError();
+    };
+    using std::integral_constant;
+    auto by_type = [&](auto type) {
+        constexpr int kWide = sizeof(type) == 2 ? 8 : 4;
+        if (v == kWide) return launch(type, integral_constant<int, kWide>{}, integral_constant<int, 1>{});
+        if (v == 2) return launch(type, integral_constant<int, 2>{}, integral_constant<int, kNarrowPieces>{});
+        return launch(type, integral_constant<int, 1>{}, integral_constant<int, kNarrowPieces>{});
+    };
+    return n.dtype == RACE_BF16 ? by_type(bf16_t{}) : by_type(float{});
 }
 
 }  // namespace

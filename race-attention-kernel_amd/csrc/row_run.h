@@ -18,6 +18,8 @@ struct Run {
         } else if constexpr (V * sizeof(TIn) == 8) {
             const uint2 v = *reinterpret_cast<const uint2*>(p);
             w[0] = v.x, w[1] = v.y;
+        } else if constexpr (V * sizeof(TIn) == 4 && V == 2) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (sizeof(TIn) == 4) {
             w[0] = __float_as_uint(*p);
         } else {
@@ -38,8 +40,12 @@ struct Run {
         else if constexpr (V * sizeof(TIn) == 16)
             *reinterpret_cast<uint4*>(p) = make_uint4(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]),
                                                       mfma::pack2(x[4], x[5]), mfma::pack2(x[6], x[7]));
+        else if constexpr (V * sizeof(TIn) == 8 && sizeof(TIn) == 4)
+            *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
         else if constexpr (V * sizeof(TIn) == 8)
             *reinterpret_cast<uint2*>(p) = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
+        else if constexpr (V == 2)
+            *reinterpret_cast<uint32_t*>(p) = mfma::pack2(x[0], x[1]);
         else
             store_val(p, x[0]);
     }
