@@ -20,7 +20,10 @@
 // gradient is the sum of the dG from it on.  Pairs of tokens that a decay does not
 // lie between cancel in it exactly, R and C holding the same numbers.
 //
-// Bound by memory: the walk's and the forward's kept states.  Key streams that
+// 128 streams of 4096 bf16 tokens, 128 x 128: the walk 255 us (707 MB past the caches),
+// bound as the forward's; the gradients 485 us (1010 MB), whose workgroups stay and
+// load the next slice's rows meanwhile: a chunk's kept states come in slices of 64 value
+// columns, and its 64 x 64 matrices and sums between two barriers take half of the time.  Key streams that
 // several value streams share sum their gradients in the registers of one
 // workgroup, in order: results are bitwise reproducible.
 #include "delta_tiles.h"

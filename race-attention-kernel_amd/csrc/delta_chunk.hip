@@ -22,7 +22,14 @@
 // once, as the output is: relative errors of at most 8e-6 of a state and of two to
 // three roundings of an output.  Log decays are summed in 64 bits: differences of
 // long sums lose the digits the products keep.
-// A few tokens (decode) go token by token in 32 bits: delta_step_kernel.
+// A few tokens (decode) go token by token in 32 bits: delta_step_kernel, bound by the
+// states' bytes (1024 streams, 128 x 128: 134 MB, 23 us).
+// The walk is bound by its chain of products: a chunk's K S, T D, K^T Z follow one
+// another, 3 us with a wave a SIMD, its matrix cores busy for a quarter of it; so
+// its waves hold no more than they need, loads for the next chunk go out between the
+// stages, and few streams are walked in segments (delta_segment_chunks).  128 streams
+// of 4096 bf16 tokens, 128 x 128, with records: solve 95 us (324 MB past the caches),
+// walk 306 us (849 MB).
 #include <algorithm>
 #include <utility>
 

