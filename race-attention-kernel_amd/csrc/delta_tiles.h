@@ -350,7 +350,8 @@ struct Ragged<bf16_t> {
 };
 
 // A view of `live` rows from p on for them, and the element of it that p is: from the
-// word that p lies in to the end of the last one (arrays start 16-byte aligned).
+// word that p lies in (arrays start 16-byte aligned) to the end of the last one, whose
+// other half, where it lies behind the array, shares its allocation and is cut off.
 template <typename TIn>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t ragged_view(const TIn* p, int64_t stride, int live, int width, int& at) {
     at = int(reinterpret_cast<uintptr_t>(p) & 3) / int(sizeof(TIn));

@@ -647,3 +647,70 @@ def test_the_longest_token_stride(race, cuda, T, stride, dtype):
         got = race.race_delta_rule_carry(*moved)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
         wide.fill_(math.nan)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_streams_without_tokens_among_those_in_segments(race, cuda, dtype):
+    T = 1600
+    *args, dout, dfinal = make(3, 1, T, 64, 48, dtype, seed=23)
+    lengths = torch.tensor([0, T - 5, 1], dtype=torch.int32, device=cuda)
+    outs, grads = check(race, args, dout, dfinal, dtype, "segments", scale=0.125, lengths=lengths)
+    assert (outs[0][0] == 0).all() and torch.equal(outs[1][0], args[5][0]) and torch.equal(grads[5][0], dfinal[0])
+    for d in grads[2:5]:
+        assert (d[0] == 0).all() and (d[2, 1:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("d", [64, 33])
+def test_one_row_for_all_tokens(race, cuda, d, dtype):
+    # Token strides of zero, and rows that overlap, with padding behind them.
+    N, T = 4, 100
+    *args, dout, dfinal = make(N, N, T, d, d, dtype, seed=24)
+    lengths = torch.tensor([100, 64, 70, 3], dtype=torch.int32, device=cuda)
+    same = [t[:, :1].expand(N, T, d) for t in args[:3]]
+    slide = args[2].reshape(-1)[:3 * 2048 + T * 8 + d].as_strided((N, T, d), (2048, 8, 1))
+    for q, k, v in ((same[0], same[1], same[2]), (args[0], args[1], slide)):
+        dense = [t.contiguous() for t in (q, k, v)]
+        got = race.race_delta_rule_carry(q, k, v, *args[3:], scale=0.125, lengths=lengths)
+        want = race.race_delta_rule_carry(*dense, *args[3:], scale=0.125, lengths=lengths)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        grads = []
+        for rows in ((q, k, v), dense):
+            leaves = [t.detach().requires_grad_(True) for t in rows]
+            grads.append(torch.autograd.grad(race.race_delta_rule(*leaves, *args[3:], scale=0.125, lengths=lengths), leaves, (dout, dfinal)))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_most_streams(race, cuda, dtype):
+    N, T, d = 65535, 3, 8
+    *args, dout, dfinal = make(N, N // 3, T, d, d, dtype, seed=25)
+    leaves = [t.detach().requires_grad_(True) for t in args]
+    outs = race.race_delta_rule(*leaves, scale=0.5)
+    grads = torch.autograd.grad(outs, leaves, (dout, dfinal))
+    stepped = race.race_delta_rule_carry(*args, scale=0.5)
+    for part in (slice(0, 300), slice(N - 300, N)):
+        keys = slice(part.start // 3, part.stop // 3)
+        some = [t[keys] if i < 2 else t[part] for i, t in enumerate(args)]
+        want = reference(*some, scale=0.5, dout=dout[part], dfinal=dfinal[part])
+        for name, got in (("out", outs[0]), ("state", outs[1]), ("out", stepped[0]), ("state", stepped[1])):
+            close(name, got.detach()[part], want[name], dtype)
+        for i, name in enumerate(NAMES):
+            close("d" + name, grads[i][keys if i < 2 else part], want["d" + name], dtype)
+
+
+def test_one_long_stream(race, cuda):
+    # A million tokens in 256 segments, against two calls that split them elsewhere; both keep the tolerance.
+    T, cut = 1 << 20, 600_011
+    *args, dout, dfinal = make(1, 1, T, 64, 64, F32, seed=26)
+    args[3] = args[3] * 0.01  # decays of hundreds of tokens
+    leaves = [t.detach().requires_grad_(True) for t in args]
+    out, state = race.race_delta_rule(*leaves, scale=0.125)
+    grads = torch.autograd.grad((out, state), leaves, (dout, dfinal))
+    o1, mid = race.race_delta_rule(*(t[:, :cut] for t in leaves[:5]), leaves[5], scale=0.125)
+    o2, last = race.race_delta_rule(*(t[:, cut:] for t in leaves[:5]), mid, scale=0.125)
+    split = torch.autograd.grad((torch.cat([o1, o2], 1), last), leaves, (dout, dfinal))
+    for name, a, b in zip(("out", "state", *("d" + n for n in NAMES)), (out, state, *grads), (torch.cat([o1, o2], 1), last, *split)):
+        err = (a.detach().double() - b.detach().double()).norm() / b.detach().double().norm()
+        say(name, f"{float(err):.1e}")
+        assert err <= 2 * tolerance(name, F32), name

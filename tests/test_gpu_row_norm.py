@@ -294,3 +294,23 @@ def test_gradients_of_gradients_and_tangents_are_refused(race, cuda):
 def test_refusals(race, cuda, call):
     with pytest.raises(RuntimeError, match="race_(add|gate)_norm"):
         call(race, lambda *s: torch.zeros(*s, device=cuda))
+
+
+# Rows in pieces of two values and of one, through every number of pieces a thread holds.
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [2, 126, 130, 514, 1026, 2050, 4098, 5001, 8190, 8194, 8195, 10002, 12287, 16382])
+def test_add_norm_of_narrow_pieces(race, cuda, D, dtype):
+    test_add_norm_and_gradients(race, cuda, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [2, 130, 1002, 5001, 5002, 8195, 10002, 16382])
+def test_e4m3_rows_of_narrow_pieces(race, cuda, D, dtype):
+    test_e4m3_rows(race, cuda, D, 0, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B, T, H, d", [(2, 5, 3, 2), (1, 9, 2, 6), (2, 7, 3, 50), (3, 5, 2, 66), (1, 11, 4, 130), (2, 3, 2, 254), (2, 5, 3, 17),
+                                        (2, 70, 3, 65), (1, 4, 5, 129), (1, 2000, 3, 33)])
+def test_gate_norm_of_narrow_pieces(race, cuda, B, T, H, d, dtype):
+    test_gate_norm_and_gradients(race, cuda, B, T, H, d, dtype)
