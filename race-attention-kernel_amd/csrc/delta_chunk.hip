@@ -648,13 +648,15 @@ void launch_step(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
 // Chunks of a segment.  One walk has (dv + 63) / 64 workgroups a stream; a chunk takes
 // it about 3 us however few there are.  Split, every segment is walked twice, the
 // first time with dk columns more and without outputs, so a split pays where it
-// makes at least three segments; it aims for a workgroup a CU, and leaves a segment 8
-// chunks.  16 streams of 32768 bf16 tokens, 128 x 128: one walk 1493 us; maps 246,
-// join 52 and walks 247.  24 ragged fp32 streams of at most 2000 tokens, 64 x 64, in
-// three segments: backward 153 us in one, 54 + 10 + 77 split.
+// makes at least three segments (16 bf16 streams, 128 x 128, of 9 chunks in one 31 us, in
+// three 34; of 12 in one 40, in three 39); it aims for a workgroup a CU.
+// 16 streams of 32768 tokens, 128 x 128: one walk 1493 us; maps 246, join 25 and walks 247.
+// A segment has 4 chunks at least: the join takes a step a segment.  24 ragged fp32
+// streams of at most 24 chunks, 64 x 64, forward and backward, segments of 8 94 + 129
+// us, of 4 59 + 84, of 3 60 + 75; 16 bf16 ones of 24, 128 x 128, 58, 54, 57.
 int64_t delta_segment_chunks(const DeltaRule& r) {
     const int64_t chunks = delta_chunks(r), walks = r.N * ((r.dv + 63) / 64);
-    const int64_t segs = std::min<int64_t>(walks > 0 ? 256 / walks : 1, chunks / 8);
+    const int64_t segs = std::min<int64_t>(walks > 0 ? 256 / walks : 1, chunks / 4);
     return segs < 3 ? std::max<int64_t>(chunks, 1) : (chunks + segs - 1) / segs;
 }
 

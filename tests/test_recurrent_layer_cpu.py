@@ -102,8 +102,8 @@ def test_delta_rule_refuses_on_the_host(race):
     assert abi.delta_fwd(0, 0, 0, None, 0, 16, None, 0, 16, None, abi.delta_shape(4, 0, 64, 48), None, 0, 0) == 0
     # A few tokens need no memory, and long sequences of few streams more than the sum of their chunks.
     assert abi.delta_workspace_bytes(abi.delta_shape(4, 16, 64, 48))[1] == 0
-    one, two = (abi.delta_workspace_bytes(abi.delta_shape(1, T, 64, 48))[1] for T in (1024, 2048))
-    assert two > 2 * one > 0
+    one, two = (abi.delta_workspace_bytes(abi.delta_shape(1, T, 64, 48))[1] for T in (512, 2048))
+    assert two > 4 * one > 0
 
 
 def test_delta_rule_refuses_tensors_of_the_host(race):
