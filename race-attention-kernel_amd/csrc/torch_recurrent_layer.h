@@ -156,8 +156,6 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>, c10::optional<a
 
 // ---- the gated delta rule ----
 
-int64_t token_width(const at::Tensor& t) { return t.dim() == 4 ? t.size(2) * t.size(3) : t.size(2); }
-
 race_delta_shape delta_shape(const char* entry, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                              const c10::optional<at::Tensor>& gate, const at::Tensor& beta,
                              const c10::optional<at::Tensor>& state, const c10::optional<at::Tensor>& lengths, int64_t form,
