@@ -57,7 +57,7 @@ using BwdWalkLds = ChunkLds<TIn, DK, true, !two_a_cu(sizeof(TIn) * DK, false)>;
 
 // kMaps: no records, but what the segment adds to a gradient of zero behind it (the
 // last one: to dfinal), to map_x.
-template <typename TIn, int DK, bool kVec, bool kMaps>
+template <typename TIn, int DK, bool kVec, bool kVecV, bool kMaps>
 __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1) void delta_bwd_walk_kernel(const DeltaBwdArgs w) {
     extern __shared__ __align__(16) unsigned char lds[];
     const DeltaArgs& a = w.f;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     Stage<TIn, DK, kThreads, kVec> sk, sq;
     StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;
     StageDense<TIn, 64, kChunk, kThreads> smm;
-    Stage<TIn, 64, kThreads, kVec> so;
+    Stage<TIn, 64, kThreads, kVecV> so;
     float svec;
     sk.init(a.kt, a.dk);
     sq.init(a.qt, a.dk);
@@ -394,7 +394,7 @@ __device__ __forceinline__ bool next_stream(const DeltaArgs& a, int items, GradU
 // Wave (th, dq): TB blocks of 16 tokens and a quarter of the key columns; of the 64 x
 // 64 matrices its tokens' rows and 16 columns.  kShared: key streams with several
 // value streams, whose dQ and dK are summed in registers.
-template <typename TIn, int DK, bool kVec, bool kShared>
+template <typename TIn, int DK, bool kVec, bool kVecV, bool kShared>
 __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBwdArgs w, int items) {
     extern __shared__ __align__(16) unsigned char lds[];
     const DeltaArgs& a = w.f;
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
 
     Pieces<TIn, DK, SL, NT> ps, pd;
     Pieces<TIn, 64, SL, NT> py, pdd;
-    RowPieces<TIn, SL, NT, kVec> po;
+    RowPieces<TIn, SL, NT, kVecV> po;
     RowPieces<TIn, DK, NT, kVec> pk, pq;
     uint32_t pg = 0, pb = 0;
     // The loads of a unit: its slice, with a stream's first the gates, with a chunk's first K and Q.
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
                 if (dv && ((v0 >> 5) + kk) % 4 == dq && tok(b, lr) < here) {
                     const int cv = v0 + 32 * kk + 8 * g;
                     TIn* o = dv + int64_t(tok(b, lr)) * a.dv + cv;
-                    if (kVec && cv + 8 <= a.dv) {
+                    if (kVecV && cv + 8 <= a.dv) {
                         store_run(o, da[i]);
                     } else {
                         const auto run = __builtin_bit_cast(Eight<TIn>, da[i]);
@@ -700,34 +700,40 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
     }
 }
 
-template <typename TIn, int DK, bool kVec>
+template <typename TIn, int DK, bool kVec, bool kVecV>
 hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
     using L = BwdWalkLds<TIn, DK>;
     constexpr int walk = L::kBuffers * L::kBytes, grads = GradLds<TIn, DK>::kBytes;
     static_assert(walk <= kGfx950LdsBytes && grads <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
     auto grid_of = [&](int64_t streams) { return unsigned((streams + 7) / 8 * 8 * ((r.dv + 63) / 64)); };
     if (w.f.segs > 1) {
-        delta_bwd_walk_kernel<TIn, DK, kVec, true><<<grid_of(r.N * (w.f.segs - 1)), kThreads, walk, stream>>>(w);
+        delta_bwd_walk_kernel<TIn, DK, kVec, kVecV, true><<<grid_of(r.N * (w.f.segs - 1)), kThreads, walk, stream>>>(w);
         DeltaArgs join = w.f;
         join.state = w.dfinal;
         launch_join<DK, true>(r, join, stream);
     }
-    delta_bwd_walk_kernel<TIn, DK, kVec, false><<<grid_of(r.N * w.f.segs), kThreads, walk, stream>>>(w);
+    delta_bwd_walk_kernel<TIn, DK, kVec, kVecV, false><<<grid_of(r.N * w.f.segs), kThreads, walk, stream>>>(w);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (!w.dq && !w.dk && !w.dv && !w.dgate && !w.dbeta) return hipSuccess;
     const int items = int(r.Nk * w.f.chunks);
     const unsigned grid = unsigned(items < kGradWorkgroups ? items : kGradWorkgroups);
-    if (w.f.group > 1 || !kVec)
-        delta_grads_kernel<TIn, DK, kVec, true><<<grid, kGradThreads, grads, stream>>>(w, items);
+    constexpr bool kAll = kVec && kVecV;  // others have one form
+    if (w.f.group > 1 || !kAll)
+        delta_grads_kernel<TIn, DK, kVec, kVecV, true><<<grid, kGradThreads, grads, stream>>>(w, items);
     else
-        delta_grads_kernel<TIn, DK, kVec, kVec ? false : true><<<grid, kGradThreads, grads, stream>>>(w, items);
+        delta_grads_kernel<TIn, DK, kVec, kVecV, !kAll><<<grid, kGradThreads, grads, stream>>>(w, items);
     return hipGetLastError();
 }
 
-template <typename TIn, bool kVec>
+template <typename TIn, bool kVec, bool kVecV>
 hipError_t launch_by_width(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
-    return r.dk <= 64 ? launch_backward<TIn, 64, kVec>(r, w, stream) : launch_backward<TIn, 128, kVec>(r, w, stream);
+    return r.dk <= 64 ? launch_backward<TIn, 64, kVec, kVecV>(r, w, stream) : launch_backward<TIn, 128, kVec, kVecV>(r, w, stream);
+}
+template <typename TIn>
+hipError_t launch_by_pieces(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
+    if (!w.f.vec_k) return launch_by_width<TIn, false, false>(r, w, stream);
+    return w.f.vec_o ? launch_by_width<TIn, true, true>(r, w, stream) : launch_by_width<TIn, true, false>(r, w, stream);
 }
 
 }  // namespace
@@ -758,10 +764,7 @@ hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const voi
         w.f.map_x = w.f.starts + (l.map_x - l.starts) / 4;
     }
     w.dq = g.dq, w.dk = g.dk, w.dv = g.dv, w.dgate = g.dgate, w.dbeta = g.dbeta, w.dstate = g.dstate;
-    const bool vec = w.f.vec_k && w.f.vec_o;
-    if (r.dtype == RACE_BF16)
-        return vec ? launch_by_width<bf16_t, true>(r, w, stream) : launch_by_width<bf16_t, false>(r, w, stream);
-    return vec ? launch_by_width<float, true>(r, w, stream) : launch_by_width<float, false>(r, w, stream);
+    return r.dtype == RACE_BF16 ? launch_by_pieces<bf16_t>(r, w, stream) : launch_by_pieces<float>(r, w, stream);
 }
 
 }  // namespace race
