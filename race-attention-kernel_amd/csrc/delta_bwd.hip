@@ -53,7 +53,7 @@ __device__ __forceinline__ void store_gate(void* p, int64_t i, int f32, float x)
 
 // dO in the place of V.  192 streams of 577 tokens, 64 x 128: two workgroups a CU 53.2 -> 43.2 us.
 template <typename TIn, int DK>
-using BwdWalkLds = ChunkLds<TIn, DK, true, !two_a_cu(sizeof(TIn) * DK, false)>;
+using BwdWalkLds = ChunkLds<TIn, DK, 1, true, !two_a_cu(sizeof(TIn) * DK, false)>;
 
 // kMaps: no records, but what the segment adds to a gradient of zero behind it (the
 // last one: to dfinal), to map_x.
@@ -66,6 +66,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     using Square = Tile<TIn, 64>;
     using One = OneT<TIn>;
     using Two = TwoT<TIn>;
+    using Three = ThreeT<TIn>;
     constexpr int NS = DK / 32;
     const int walks = kMaps ? a.segs - 1 : a.segs;  // no gradient goes on before the first segment
     int64_t ns;
@@ -100,8 +101,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     }
 
     Stage<TIn, DK, kThreads, kVec> sk, sq;
-    StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;
-    StageDense<TIn, 64, kChunk, kThreads> smm;
+    StageDense<TIn, 64, kChunk, kThreads, 3> stm;
+    StageDense<TIn, 64, kChunk, kThreads, 1> smm;
     Stage<TIn, 64, kThreads, kVecV> so;
     float svec;
     sk.init(a.kt, a.dk);
@@ -112,9 +113,9 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
         if (part == 0) sk.load(kp + t0 * a.kt, live);
         if (part == 1) sq.load(qp + t0 * a.qt, live);
-        if (part == 2) stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
+        if (part == 2) stm.load(a.tm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
         if (part == 3) {
-            smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
+            smm.load(a.mm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
             so.load(op + t0 * a.dv, live);
             svec = a.vec[nc * 128 + (threadIdx.x & 127)];
         }
@@ -129,8 +130,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         if (L::kBuffers == 1 && c < chunks - 1) __syncthreads();  // the chunk before is done with the buffer
         sk.put(buf + L::kK);
         sq.put(buf + L::kQ);
-        stm.put(buf + L::kT);
-        smm.put(buf + L::kM);
+        stm.put(buf + L::kT, threadIdx.x);
+        smm.put(buf + L::kM, threadIdx.x);
         so.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
         const int next = c > from ? c - 1 : c;  // the last chunk's loads are not used
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             operand(dS[2 * i], dS[2 * i + 1], odd, s[i]);
-            if constexpr (!kMaps) store_run(ds + 32 * i, delta::first(s[i]));
+            if constexpr (!kMaps) store_run(ds + 32 * i, delta::first<1>(s[i]));
         }
         stage_wall();
         fetch(next, 0);
@@ -186,11 +187,11 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
             for (int b = 0; b < 4; ++b) x[b] = mac(kf[i][b], s[i], i == 0 ? zero : x[b]);
         stage_wall();
         fetch(next, 1);
-        Two tf[4], tg[2];
+        Three tf[4], tg[2];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) tf[b] = Square::transposed_two(buf + L::kT, s_col, 1, b);
+        for (int b = 0; b < 4; ++b) tf[b] = Square::template transposed_parts<3>(buf + L::kT, s_col, 1, b);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) tg[b] = Square::transposed_two(buf + L::kT, s_col, 0, b);
+        for (int b = 0; b < 2; ++b) tg[b] = Square::template transposed_parts<3>(buf + L::kT, s_col, 0, b);
 #pragma unroll
         for (int b = 0; b < 4; ++b) x[b] = mac(mf[b], od[1], x[b] * zb[b]);
 #pragma unroll
@@ -751,7 +752,7 @@ hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const voi
     w.f = delta_args(r, in);
     const DeltaLayout l = delta_layout(r);
     unsigned char* base = const_cast<unsigned char*>(static_cast<const unsigned char*>(records));
-    w.f.tm = base, w.f.mm = base + l.mm, w.f.vec = reinterpret_cast<float*>(base + l.vec);
+    w.f.tm = reinterpret_cast<float*>(base), w.f.mm = reinterpret_cast<float*>(base + l.mm), w.f.vec = reinterpret_cast<float*>(base + l.vec);
     w.f.st = base + l.solve_bytes, w.f.yt = base + l.yt;
     w.dout = dout, w.dfinal = dfinal;
     const int64_t es = r.dtype == RACE_BF16 ? 2 : 4;

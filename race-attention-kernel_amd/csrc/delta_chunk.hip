@@ -16,20 +16,22 @@
 // S, D, Y and O do not mix, so its waves share the K, Q and T tiles in LDS and
 // nothing else, and every product takes its right operand from the accumulators
 // before it (delta_tiles.h).
-// Precision.  Sums are fp32.  fp32 rows run in fp32 products.  With bf16 rows the
-// state's own path (T, D, Y, the state's update) takes what is computed as bf16
-// hi + lo pairs, 16 bits, and the output's path takes M, S and Y rounded to bf16
-// once, as the output is: relative errors of at most 8e-6 of a state and of two to
-// three roundings of an output.  Log decays are summed in 64 bits: differences of
-// long sums lose the digits the products keep.
+// Precision.  Sums are fp32, and so are the factors of a product that are computed: with
+// fp32 rows in fp32 products, with bf16 rows in three parts of bf16 (delta_tiles.h), so
+// that a call of bf16 rows gives what one of the same rows in fp32 does, its outputs
+// rounded once.  Errors are relative to the terms of a sum: where a chunk overwrites
+// what a state held, a rounding of that, 2^-24, is left until the next chunk.  The
+// output's own products, whose result is rounded to bf16 right away, take S, Y and M
+// in two parts.  Log decays are summed in 64 bits: differences of long sums lose the
+// digits the products keep.
 // A few tokens (decode) go token by token in 32 bits: delta_step_kernel, bound by the
 // states' bytes (1024 streams, 128 x 128: 134 MB, 23 us).
 // The walk is bound by its chain of products: a chunk's K S, T D, K^T Z follow one
-// another, 3 us with a wave a SIMD, its matrix cores busy for a quarter of it; so
+// another, 4 us with a wave a SIMD, its matrix cores busy for less than a third of it; so
 // its waves hold no more than they need, loads for the next chunk go out between the
 // stages, and few streams are walked in segments (delta_segment_chunks).  128 streams
-// of 4096 bf16 tokens, 128 x 128, with records: solve 95 us (324 MB past the caches),
-// walk 306 us (849 MB).
+// of 4096 bf16 tokens, 128 x 128, with records: solve 105 us, walk 385 us (with every
+// factor in two parts and M in one 306 us, its outputs off by half a rounding more).
 #include <algorithm>
 #include <utility>
 
@@ -164,8 +166,7 @@ __global__ __launch_bounds__(kThreads, sizeof(TIn) * DK <= 256 ? 4 : 2) void del
     for (int j = 0; j < 4; ++j) {
         gb[j] = weights(o, j);
         if (j <= (o | 1))  // the others are not read
-            store4_of(static_cast<TIn*>(a.mm) + nc * (kChunk * kChunk) + (16 * o + lr) * kChunk + 16 * j + 4 * g,
-                      below(o, j, gb[j] * qk[j] * a.scale, 0));
+            store4_of(a.mm + nc * (kChunk * kChunk) + (16 * o + lr) * kChunk + 16 * j + 4 * g, below(o, j, gb[j] * qk[j] * a.scale, 0));
         if (!kAll) gb[j] = weights(wave, j);
     }
     __syncthreads();
@@ -216,27 +217,13 @@ __global__ __launch_bounds__(kThreads, sizeof(TIn) * DK <= 256 ? 4 : 2) void del
     }
     __syncthreads();
     const int row = threadIdx.x >> 2, c0 = (threadIdx.x & 3) * 16;
-    float x[16];
+    float* tm = a.tm + nc * (kChunk * kChunk) + row * kChunk + c0;
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(T + row * kSolvePitch + c0 + e);
+        f32x4 x = *reinterpret_cast<const f32x4*>(T + row * kSolvePitch + c0 + e);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[e + r] = c0 + e + r <= row ? v[r] : 0.f;
-    }
-    TIn* tm = static_cast<TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk) + row * kChunk + c0;
-    if constexpr (sizeof(TIn) == 4) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) store4_of(tm + e, f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e += 8) {
-            uint2 hi[2], lo[2];
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-                mfma::split4<true>(x[e + 4 * p], x[e + 4 * p + 1], x[e + 4 * p + 2], x[e + 4 * p + 3], hi[p], lo[p]);
-            *reinterpret_cast<uint4*>(tm + e) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
-            *reinterpret_cast<uint4*>(tm + kChunk * kChunk + e) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
-        }
+        for (int r = 0; r < 4; ++r) x[r] = c0 + e + r <= row ? x[r] : 0.f;
+        store4_of(tm + e, x);
     }
 }
 
@@ -249,7 +236,7 @@ __global__ __launch_bounds__(kThreads, sizeof(TIn) * DK <= 256 ? 4 : 2) void del
 enum WalkMode { kOutputs, kRecording, kMaps };
 
 template <typename TIn, int DK, WalkMode kMode>
-using WalkLds = ChunkLds<TIn, DK, kMode != kMaps, !two_a_cu(sizeof(TIn) * DK, kMode == kMaps)>;
+using WalkLds = ChunkLds<TIn, DK, 2, kMode != kMaps, !two_a_cu(sizeof(TIn) * DK, kMode == kMaps)>;
 
 // kVec, kVecV: rows of keys, and of values and outputs, in 16-byte pieces.
 template <typename TIn, int DK, bool kVec, bool kVecV, WalkMode kMode>
@@ -261,6 +248,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
     using Square = Tile<TIn, 64>;
     using One = OneT<TIn>;
     using Two = TwoT<TIn>;
+    using Three = ThreeT<TIn>;
     constexpr int NS = DK / 32;
     const int value_blocks = (a.dv + 63) / 64, blocks = value_blocks + (kMode == kMaps ? (a.dk + 63) / 64 : 0);
     const int walks = kMode == kMaps ? a.segs - 1 : a.segs;  // no state follows the last segment's
@@ -302,8 +290,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
     }
 
     Stage<TIn, DK, kThreads, kVec> sk, sq;
-    StageDense<TIn, 64, kTwoRows<TIn>, kThreads> stm;
-    StageDense<TIn, 64, kChunk, kThreads> smm;
+    StageDense<TIn, 64, kChunk, kThreads, 3> stm;
+    StageDense<TIn, 64, kChunk, kThreads, 2> smm;
     Stage<TIn, 64, kThreads, kVecV> sv;
     float svec;
     sk.init(a.kt, a.dk);
@@ -315,9 +303,9 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
         if (part == 0) sk.load(kp + t0 * a.kt, live);
         if (part == 1 && kMode != kMaps) sq.load(qp + t0 * a.qt, live);
-        if (part == 2) stm.load(static_cast<const TIn*>(a.tm) + nc * (kTwoRows<TIn> * kChunk));
+        if (part == 2) stm.load(a.tm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
         if (part == 3) {
-            if (kMode != kMaps) smm.load(static_cast<const TIn*>(a.mm) + nc * (kChunk * kChunk));
+            if (kMode != kMaps) smm.load(a.mm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
             sv.load(vp + t0 * a.vt, live);
             svec = a.vec[nc * 128 + (threadIdx.x & 127)];
         }
@@ -332,8 +320,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         if (L::kBuffers == 1 && c > from) __syncthreads();  // the chunk before is done with the buffer
         sk.put(buf + L::kK);
         if (kMode != kMaps) sq.put(buf + L::kQ);
-        stm.put(buf + L::kT);
-        if (kMode != kMaps) smm.put(buf + L::kM);
+        stm.put(buf + L::kT, threadIdx.x);
+        if (kMode != kMaps) smm.put(buf + L::kM, threadIdx.x);
         sv.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
         const int next = c + 1 < chunks ? c + 1 : c;  // the last chunk's loads are not used
@@ -350,26 +338,26 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         for (int i = 0; i < NS; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) kf[i][b] = Rows::one(buf + L::kK, k_row, b, i);
-        Two s[NS];
+        Three s[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) operand(S[2 * i], S[2 * i + 1], odd, s[i]);
         if constexpr (kMode == kRecording) {
             TIn* st = static_cast<TIn*>(a.st) + (nc * a.dvp + col) * DK + 8 * g;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first(s[i]));
+            for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first<1>(s[i]));
         }
         stage_wall();
         fetch(next, 0);
-        Two tf[4], tg[2];
+        Three tf[4], tg[2];
         f32x4 e[4], v[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             e[b] = *reinterpret_cast<const f32x4*>(E + tok(b, 4 * g));
             v[b] = Square::block(buf + L::kV, v_at, b);
-            tf[b] = Square::two(buf + L::kT, s_row, b, 0);
+            tf[b] = Square::template parts<3>(buf + L::kT, s_row, b, 0);
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) tg[b] = Square::two(buf + L::kT, s_row, 2 + b, 1);
+        for (int b = 0; b < 2; ++b) tg[b] = Square::template parts<3>(buf + L::kT, s_row, 2 + b, 1);
         // D = V - E K S.
         f32x4 x[4];
 #pragma unroll
@@ -393,7 +381,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[b][r] = fmaf(-e[b][r], x[b][r], v[b][r]);
-        Two d[2];
+        Three d[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, d[kk]);
         // Y = T D; T is lower triangular.
@@ -411,7 +399,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
 #pragma unroll
                 for (int b = 0; b < 4; ++b) qf[i][b] = Rows::one(buf + L::kQ, k_row, b, i);
         }
-        Two y[2], z[2];
+        Two y[2];  // for the output
+        Three z[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
@@ -420,7 +409,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         if constexpr (kMode == kRecording) {
             TIn* yt = static_cast<TIn*>(a.yt) + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, delta::first(y[kk]));
+            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, delta::first<1>(y[kk]));
         }
         // S = e^{G_last} S + K^T (Z b Y).
         const float decay = E[63];
@@ -433,13 +422,13 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         stage_wall();
         fetch(next, 3);
         if constexpr (kMode == kMaps) continue;
-        One mf[4], mg[2];
+        Two mf[4], mg[2];
         float es[4];
         auto scores = [&] {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) mf[b] = Square::one(buf + L::kM, s_row, b, 0), es[b] = E[tok(b, lr)] * a.scale;
+            for (int b = 0; b < 4; ++b) mf[b] = Square::template parts<2>(buf + L::kM, s_row, b, 0), es[b] = E[tok(b, lr)] * a.scale;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) mg[b] = Square::one(buf + L::kM, s_row, 2 + b, 1);
+            for (int b = 0; b < 2; ++b) mg[b] = Square::template parts<2>(buf + L::kM, s_row, 2 + b, 1);
         };
         if (!kLate) scores();
         // O^T = scale S^T Q^T E + Y^T M^T, S the state before the chunk: a token's columns in a lane.
@@ -451,7 +440,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
                 for (int b = 0; b < 4; ++b) qf[i][b] = Rows::one(buf + L::kQ, k_row, b, i);
             }
 #pragma unroll
-            for (int b = 0; b < 4; ++b) o[b] = mac(s[i], qf[i][b], i == 0 ? zero : o[b]);
+            for (int b = 0; b < 4; ++b) o[b] = mac(delta::first<2>(s[i]), qf[i][b], i == 0 ? zero : o[b]);
         }
         if (kLate) scores();
 #pragma unroll
@@ -675,7 +664,7 @@ DeltaLayout delta_layout(const DeltaRule& r) {
     const int64_t nc = r.N * delta_chunks(r), es = r.dtype == RACE_BF16 ? 2 : 4, dvp = (r.dv + 15) / 16 * 16;
     DeltaLayout l;
     l.mm = round256(nc * kChunk * kChunk * 4);
-    l.vec = l.mm + round256(nc * kChunk * kChunk * es);
+    l.vec = l.mm + round256(nc * kChunk * kChunk * 4);
     l.solve_bytes = l.vec + round256(nc * 512);
     const int64_t each = delta_segment_chunks(r), segs = std::max<int64_t>((delta_chunks(r) + each - 1) / each, 1);
     l.segs = int(segs), l.seg_chunks = int(each);
@@ -703,7 +692,7 @@ hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* 
     const DeltaLayout l = delta_layout(r);
     unsigned char* maps = static_cast<unsigned char*>(workspace);
     unsigned char* base = records ? static_cast<unsigned char*>(records) : maps + l.map_bytes;
-    a.tm = base, a.mm = base + l.mm;
+    a.tm = reinterpret_cast<float*>(base), a.mm = reinterpret_cast<float*>(base + l.mm);
     a.vec = reinterpret_cast<float*>(base + l.vec);
     if (records) a.st = base + l.solve_bytes, a.yt = base + l.yt;
     a.segs = l.segs, a.seg_chunks = l.seg_chunks;

@@ -2,10 +2,12 @@
 // (delta_chunk.hip, delta_bwd.hip): 64-token tiles in LDS and the order of
 // matrix-core operands.  Not part of the ABI.
 //
-// Operands.  bf16 rows run on v_mfma_f32_16x16x32_bf16; what is computed from
-// them enters a product rounded to bf16 (One) or as a bf16 hi + lo pair (Two:
-// 16 bits, lo * lo left out).  fp32 rows run on v_mfma_f32_16x16x4_f32 as they
-// are, eight steps for the same 32 values.
+// Operands.  bf16 rows run on v_mfma_f32_16x16x32_bf16 as they are (One); what is
+// computed from them in 32 bits enters a product as three bf16 parts whose sum it is
+// (Three: 24 bits; the products of parts below 2^-24 are left out), or as the first
+// two (Two: 16 bits) where the result is rounded to bf16 right away.  fp32 rows run
+// on v_mfma_f32_16x16x4_f32 as they are, eight steps for the same 32 values: sixteen
+// times the matrix time of one bf16 product, 2.7 times that of the six of Three by Three.
 //
 // Order.  A lane of a wave has group g = lane / 16 and index lr = lane % 16.  A
 // fragment holds 8 consecutive values of the contraction index, 32 kk + 8 g + e,
@@ -40,38 +42,37 @@ __device__ __forceinline__ constexpr int tok(int b, int m) {
 
 // ---- operands ----
 
-template <typename TIn>
-struct OneT;
-template <typename TIn>
-struct TwoT;
-template <>
-struct OneT<bf16_t> {
-    bf16x8 h;
+// P bf16 parts of fp32 values, each the rounding of what the parts before leave.
+template <typename TIn, int P>
+struct PartsT;
+template <int P>
+struct PartsT<bf16_t, P> {
+    bf16x8 p[P];
 };
-template <>
-struct TwoT<bf16_t> {
-    bf16x8 h, l;
-};
-template <>
-struct OneT<float> {
+template <int P>
+struct PartsT<float, P> {
     f32x4 a, b;
 };
-template <>
-struct TwoT<float> : OneT<float> {};
+template <typename TIn>
+using OneT = PartsT<TIn, 1>;
+template <typename TIn>
+using TwoT = PartsT<TIn, 2>;
+template <typename TIn>
+using ThreeT = PartsT<TIn, 3>;
 
-__device__ __forceinline__ f32x4 mac(const OneT<bf16_t>& x, const OneT<bf16_t>& y, f32x4 acc) {
-    return mfma::mfma16(x.h, y.h, acc);
+// Small products first.
+template <int PX, int PY>
+__device__ __forceinline__ f32x4 mac(const PartsT<bf16_t, PX>& x, const PartsT<bf16_t, PY>& y, f32x4 acc) {
+    constexpr int kMost = PX > PY ? PX : PY;
+#pragma unroll
+    for (int s = kMost - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i < PX; ++i)
+            if (s - i >= 0 && s - i < PY) acc = mfma::mfma16(x.p[i], y.p[s - i], acc);
+    return acc;
 }
-__device__ __forceinline__ f32x4 mac(const OneT<bf16_t>& x, const TwoT<bf16_t>& y, f32x4 acc) {
-    return mfma::mfma16(x.h, y.h, mfma::mfma16(x.h, y.l, acc));
-}
-__device__ __forceinline__ f32x4 mac(const TwoT<bf16_t>& x, const OneT<bf16_t>& y, f32x4 acc) {
-    return mfma::mfma16(x.h, y.h, mfma::mfma16(x.l, y.h, acc));
-}
-__device__ __forceinline__ f32x4 mac(const TwoT<bf16_t>& x, const TwoT<bf16_t>& y, f32x4 acc) {
-    return mfma::mfma16(x.h, y.h, mfma::mfma16(x.h, y.l, mfma::mfma16(x.l, y.h, acc)));
-}
-__device__ __forceinline__ f32x4 mac(const OneT<float>& x, const OneT<float>& y, f32x4 acc) {
+template <int PX, int PY>
+__device__ __forceinline__ f32x4 mac(const PartsT<float, PX>& x, const PartsT<float, PY>& y, f32x4 acc) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc = mfma::mfma4(x.a[e], y.a[e], acc);
 #pragma unroll
@@ -79,33 +80,54 @@ __device__ __forceinline__ f32x4 mac(const OneT<float>& x, const OneT<float>& y,
     return acc;
 }
 
-__device__ __forceinline__ OneT<bf16_t> first(const TwoT<bf16_t>& x) { return {x.h}; }
-__device__ __forceinline__ OneT<float> first(const TwoT<float>& x) { return x; }
+// The first Q parts.
+template <int Q, int P>
+__device__ __forceinline__ PartsT<bf16_t, Q> first(const PartsT<bf16_t, P>& x) {
+    PartsT<bf16_t, Q> y;
+#pragma unroll
+    for (int i = 0; i < Q; ++i) y.p[i] = x.p[i];
+    return y;
+}
+template <int Q, int P>
+__device__ __forceinline__ PartsT<float, Q> first(const PartsT<float, P>& x) {
+    return {x.a, x.b};
+}
+
+// The next part of four values, which keep what it leaves.
+__device__ __forceinline__ uint2 take_part(f32x4& x) {
+    const uint2 h = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
+    x -= f32x4{mfma::lo_half(h.x), mfma::hi_half(h.x), mfma::lo_half(h.y), mfma::hi_half(h.y)};
+    return h;
+}
 
 // A block pair's accumulators as operands.
 __device__ __forceinline__ bf16x8 swapped(uint2 x0, uint2 x1, bool odd) {
     return __builtin_bit_cast(bf16x8, make_uint4(odd ? x1.x : x0.x, odd ? x1.y : x0.y, odd ? x0.x : x1.x, odd ? x0.y : x1.y));
 }
-__device__ __forceinline__ void operand(const f32x4& x0, const f32x4& x1, bool odd, OneT<bf16_t>& out) {
-    uint2 h0, h1, none;
-    mfma::split4<false>(x0[0], x0[1], x0[2], x0[3], h0, none);
-    mfma::split4<false>(x1[0], x1[1], x1[2], x1[3], h1, none);
-    out.h = swapped(h0, h1, odd);
+template <int P>
+__device__ __forceinline__ void operand(const f32x4& x0, const f32x4& x1, bool odd, PartsT<bf16_t, P>& out) {
+    if constexpr (P < 2) {
+        f32x4 y0 = x0, y1 = x1;
+        out.p[0] = swapped(take_part(y0), take_part(y1), odd);
+    } else {  // fewer moves than swapping every part
+        f32x4 y0, y1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y0[e] = odd ? x1[e] : x0[e], y1[e] = odd ? x0[e] : x1[e];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const uint2 h0 = take_part(y0), h1 = take_part(y1);
+            out.p[i] = __builtin_bit_cast(bf16x8, make_uint4(h0.x, h0.y, h1.x, h1.y));
+        }
+    }
 }
-__device__ __forceinline__ void operand(const f32x4& x0, const f32x4& x1, bool odd, TwoT<bf16_t>& out) {
-    uint2 h0, h1, l0, l1;
-    mfma::split4<true>(x0[0], x0[1], x0[2], x0[3], h0, l0);
-    mfma::split4<true>(x1[0], x1[1], x1[2], x1[3], h1, l1);
-    out.h = swapped(h0, h1, odd);
-    out.l = swapped(l0, l1, odd);
-}
-__device__ __forceinline__ void operand(const f32x4& x0, const f32x4& x1, bool odd, OneT<float>& out) {
+template <int P>
+__device__ __forceinline__ void operand(const f32x4& x0, const f32x4& x1, bool odd, PartsT<float, P>& out) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) out.a[e] = odd ? x1[e] : x0[e], out.b[e] = odd ? x0[e] : x1[e];
 }
 
 // A fragment to memory: 8 consecutive values.
-__device__ __forceinline__ void store_run(bf16_t* p, const OneT<bf16_t>& x) { *reinterpret_cast<bf16x8*>(p) = x.h; }
+__device__ __forceinline__ void store_run(bf16_t* p, const OneT<bf16_t>& x) { *reinterpret_cast<bf16x8*>(p) = x.p[0]; }
 __device__ __forceinline__ void store_run(float* p, const OneT<float>& x) {
     *reinterpret_cast<f32x4*>(p) = x.a;
     *reinterpret_cast<f32x4*>(p + 4) = x.b;
@@ -174,7 +196,7 @@ struct Tile {
         if constexpr (sizeof(E) == 4)
             return {*reinterpret_cast<const f32x4*>(t + off), *reinterpret_cast<const f32x4*>(t + (off ^ 16))};
         else
-            return {*reinterpret_cast<const bf16x8*>(t + off)};
+            return {{*reinterpret_cast<const bf16x8*>(t + off)}};
     }
     // Row lr of block b (rows tok(b, .)), values 32 i + 8 g .., from row_base.
     __device__ __forceinline__ static int row_base(int lr, int g) { return run_at(tok(0, lr), g); }
@@ -184,14 +206,17 @@ struct Tile {
     __device__ __forceinline__ static OneT<E> one(const unsigned char* t, int base, int b, int i) {
         return load(t, row_off(base, b, i));
     }
-    // The same of a tile in two planes (bf16), or of fp32 values.
-    __device__ __forceinline__ static TwoT<E> two(const unsigned char* t, int base, int b, int i) {
-        TwoT<E> x;
-        const OneT<E> o = one(t, base, b, i);
-        if constexpr (sizeof(E) == 4)
+    // The same of a tile in P planes of parts, PLANE bytes apart (bf16), or of fp32 values.
+    template <int P, int PLANE = kBytes>
+    __device__ __forceinline__ static PartsT<E, P> parts(const unsigned char* t, int base, int b, int i) {
+        PartsT<E, P> x;
+        if constexpr (sizeof(E) == 4) {
+            const OneT<E> o = one(t, base, b, i);
             x.a = o.a, x.b = o.b;
-        else
-            x.h = o.h, x.l = one(t + kBytes, base, b, i).h;
+        } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p) x.p[p] = one(t + p * PLANE, base, b, i).p[0];
+        }
         return x;
     }
     // Four rows of one column: of the 16 lanes of a group, lane 4 r + q names four
@@ -221,18 +246,21 @@ struct Tile {
             }
         } else {
             const uint2 a = read_tr(t + off), c = read_tr(t + off + 4 * kRow);
-            x.h = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, c.x, c.y));
+            x.p[0] = __builtin_bit_cast(bf16x8, make_uint4(a.x, a.y, c.x, c.y));
         }
         return x;
     }
-    // The same of a tile in two planes.
-    __device__ __forceinline__ static TwoT<E> transposed_two(const unsigned char* t, int base, int kk, int b) {
-        TwoT<E> x;
-        const OneT<E> o = transposed(t, base, kk, b);
-        if constexpr (sizeof(E) == 4)
+    // The same of a tile in P planes.
+    template <int P, int PLANE = kBytes>
+    __device__ __forceinline__ static PartsT<E, P> transposed_parts(const unsigned char* t, int base, int kk, int b) {
+        PartsT<E, P> x;
+        if constexpr (sizeof(E) == 4) {
+            const OneT<E> o = transposed(t, base, kk, b);
             x.a = o.a, x.b = o.b;
-        else
-            x.h = o.h, x.l = transposed(t + kBytes, base, kk, b).h;
+        } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p) x.p[p] = transposed(t + p * PLANE, base, kk, b).p[0];
+        }
         return x;
     }
     // Values col .. col + 3 (a multiple of 4) of a row.
@@ -254,6 +282,16 @@ struct Tile {
         else
             *reinterpret_cast<uint2*>(t + off) = make_uint2(mfma::pack2(x[0], x[1]), mfma::pack2(x[2], x[3]));
     }
+    // Four fp32 values in P planes of parts (bf16), or as they are.
+    template <int P, int PLANE = kBytes>
+    __device__ __forceinline__ static void put4_parts(unsigned char* t, int off, f32x4 x) {
+        if constexpr (sizeof(E) == 4) {
+            *reinterpret_cast<f32x4*>(t + off) = x;
+        } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p) *reinterpret_cast<uint2*>(t + p * PLANE + off) = take_part(x);
+        }
+    }
     // Rows tok(b, 4 g .. 4 g + 3) of column c0 + lr, in accumulator order, from block_base.
     __device__ __forceinline__ static int block_base(int c0, int lr, int g) {
         const int row = tok(0, 4 * g);
@@ -274,9 +312,9 @@ struct Tile {
         }
     }
 };
-// Bytes of a tile that two() reads.
-template <typename E, int K>
-constexpr int kTwoBytes = sizeof(E) == 4 ? Tile<E, K>::kBytes : 2 * Tile<E, K>::kBytes;
+// Bytes of a tile in P planes.
+template <typename E, int K, int P>
+constexpr int kPartsBytes = (sizeof(E) == 4 ? 1 : P) * Tile<E, K>::kBytes;
 
 // Eight consecutive values of a row.
 template <typename TIn>
@@ -425,28 +463,28 @@ struct Stage {
     }
 };
 
-// Dense rows of K values in memory, ROWS of them, to tiles of 64 rows one after another.
-template <typename E, int K, int ROWS, int NT>
+// Dense rows of K fp32 values in memory, ROWS of them, to a tile in P planes, PLANE bytes apart.
+template <typename E, int K, int ROWS, int NT, int P, int PLANE = Tile<E, K>::kBytes>
 struct StageDense {
-    static constexpr int kChunks = Tile<E, K>::kChunks, kPer = ROWS * kChunks / NT;
-    uint4 x[kPer];
-    __device__ __forceinline__ void load(const E* p) {
-        const auto r = mfma::make_rsrc(p, ROWS * K * int(sizeof(E)));
+    static constexpr int kTotal = ROWS * K / 4, kPer = (kTotal + NT - 1) / NT;
+    f32x4 x[kPer];
+    // `rows` of them, zeros behind.
+    __device__ __forceinline__ void load(const float* p, int rows, int tid) {
+        const auto r = mfma::make_rsrc(p, rows * K * 4);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) x[i] = mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * (int(threadIdx.x) + i * NT));
+        for (int i = 0; i < kPer; ++i)
+            if (kTotal % NT == 0 || tid + i * NT < kTotal)
+                x[i] = __builtin_bit_cast(f32x4, mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * (tid + i * NT)));
     }
-    __device__ __forceinline__ void put(unsigned char* t) const {
+    __device__ __forceinline__ void put(unsigned char* t, int tid) const {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int q = int(threadIdx.x) + i * NT;
-            *reinterpret_cast<uint4*>(t + Tile<E, K>::at(q / kChunks, q % kChunks)) = x[i];
+            const int q = tid + i * NT;
+            if (kTotal % NT == 0 || q < kTotal)
+                Tile<E, K>::template put4_parts<P, PLANE>(t, Tile<E, K>::four_at(q / (K / 4), 4 * (q % (K / 4))), x[i]);
         }
     }
 };
-
-// Rows of two planes (bf16), or of fp32 values, in memory and as a tile that two() reads.
-template <typename E>
-constexpr int kTwoRows = sizeof(E) == 4 ? kChunk : 2 * kChunk;
 
 // ---- what the kernels share ----
 
@@ -457,7 +495,7 @@ struct DeltaArgs {
     const float* state;
     void* out;
     float* final_state;
-    void *tm, *mm;  // [N][chunks] of T (two planes of bf16, or fp32) and M, [64][64]
+    float *tm, *mm;  // [N][chunks] of T and M, [64][64]
     float* vec;     // [N][chunks][128]: E, then Z b
     void *st, *yt;  // nullable: [N][chunks][dvp] columns of S [DK] and Y [64], in the rows' type
     // Segments of seg_chunks chunks that are walked at once, from starts [N][segs][dk][dv];
@@ -529,12 +567,12 @@ struct StateView {
 // 512 workgroups 356 us, of half as many that walk twice as far 247).
 constexpr bool two_a_cu(int row_bytes, bool maps) { return row_bytes <= (maps ? 256 : 128); }
 
-// A chunk's tiles in LDS (bytes from its buffer's start).
-template <typename TIn, int DK, bool kOutputs = true, bool kTwoBuffers = kOutputs>
+// A chunk's tiles in LDS (bytes from its buffer's start); T in three parts, M in MP.
+template <typename TIn, int DK, int MP, bool kOutputs = true, bool kTwoBuffers = kOutputs>
 struct ChunkLds {
-    static constexpr int kK = 0, kT = Tile<TIn, DK>::kBytes, kV = kT + kTwoBytes<TIn, 64>, kVec = kV + Tile<TIn, 64>::kBytes;
+    static constexpr int kK = 0, kT = Tile<TIn, DK>::kBytes, kV = kT + kPartsBytes<TIn, 64, 3>, kVec = kV + Tile<TIn, 64>::kBytes;
     static constexpr int kQ = kVec + 512, kM = kQ + Tile<TIn, DK>::kBytes;
-    static constexpr int kBytes = kOutputs ? kM + Tile<TIn, 64>::kBytes : kQ;
+    static constexpr int kBytes = kOutputs ? kM + kPartsBytes<TIn, 64, MP> : kQ;
     // Two buffers, where they leave the workgroup its LDS: one barrier a chunk.
     static constexpr int kBuffers = kTwoBuffers && kOutputs && 2 * kBytes <= kGfx950LdsBytes ? 2 : 1;
 };
