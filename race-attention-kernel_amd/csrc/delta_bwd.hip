@@ -20,11 +20,16 @@
 // gradient is the sum of the dG from it on.  Pairs of tokens that a decay does not
 // lie between cancel in it exactly, R and C holding the same numbers.
 //
-// 128 streams of 4096 bf16 tokens, 128 x 128: the walk 255 us (707 MB past the caches),
-// bound as the forward's; the gradients 485 us (1010 MB), whose workgroups stay and
-// load the next slice's rows meanwhile: a chunk's kept states come in slices of 64 value
-// columns, and its 64 x 64 matrices and sums between two barriers take half of the time.  Key streams that
-// several value streams share sum their gradients in the registers of one
+// Precision as the forward's: sums are fp32, S, Y, dS' and dD are kept in fp32, and bf16 rows'
+// products take what is computed in three parts; where every gradient of the second
+// launch is rounded to bf16 right away, in two.  (With S, Y, dS', dD, L and X rounded to
+// bf16 once each, the gradients were off by twice what their own rounding costs.)
+//
+// 128 streams of 4096 bf16 tokens, 128 x 128: the walk 382 us, bound as the forward's;
+// the gradients 705 us (three parts 845; rounded once 485), whose workgroups stay and load
+// the next slice's rows meanwhile: a chunk's kept states come in slices of 32 value
+// columns, and its 64 x 64 matrices and sums between two barriers take half of the time.
+// Key streams that several value streams share sum their gradients in the registers of one
 // workgroup, in order: results are bitwise reproducible.
 #include "delta_tiles.h"
 
@@ -37,7 +42,7 @@ struct DeltaBwdArgs {
     DeltaArgs f;
     const void* dout;
     const float* dfinal;
-    void *ds, *dd;  // [N][chunks][dvp] columns of dS' [DK] and dD [64]
+    float *ds, *dd;  // [N][chunks][dvp] columns of dS' [DK] and dD [64]
     void *dq, *dk, *dv, *dgate, *dbeta;
     float* dstate;
 };
@@ -51,9 +56,9 @@ __device__ __forceinline__ void store_gate(void* p, int64_t i, int f32, float x)
         static_cast<bf16_t*>(p)[i] = f32_to_bf16(x);
 }
 
-// dO in the place of V.  192 streams of 577 tokens, 64 x 128: two workgroups a CU 53.2 -> 43.2 us.
+// dO in the place of V.  192 streams of 577 tokens, 64 x 128: two workgroups a CU 73 us, one 86.
 template <typename TIn, int DK>
-using BwdWalkLds = ChunkLds<TIn, DK, 1, true, !two_a_cu(sizeof(TIn) * DK, false)>;
+using BwdWalkLds = ChunkLds<TIn, DK, 3, true, !two_a_cu(sizeof(TIn) * DK, false)>;
 
 // kMaps: no records, but what the segment adds to a gradient of zero behind it (the
 // last one: to dfinal), to map_x.
@@ -65,9 +70,9 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     using Rows = Tile<TIn, DK>;
     using Square = Tile<TIn, 64>;
     using One = OneT<TIn>;
-    using Two = TwoT<TIn>;
     using Three = ThreeT<TIn>;
     constexpr int NS = DK / 32;
+    constexpr bool kLate = two_a_cu(sizeof(TIn) * DK, false);  // the reads of M, T and Q behind a product, for its registers: 78 -> 73 us of that
     const int walks = kMaps ? a.segs - 1 : a.segs;  // no gradient goes on before the first segment
     int64_t ns;
     int cb;
@@ -101,8 +106,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     }
 
     Stage<TIn, DK, kThreads, kVec> sk, sq;
-    StageDense<TIn, 64, kChunk, kThreads, 3> stm;
-    StageDense<TIn, 64, kChunk, kThreads, 1> smm;
+    StageSquare<TIn, 3> stm, smm;
     Stage<TIn, 64, kThreads, kVecV> so;
     float svec;
     sk.init(a.kt, a.dk);
@@ -113,9 +117,9 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
         if (part == 0) sk.load(kp + t0 * a.kt, live);
         if (part == 1) sq.load(qp + t0 * a.qt, live);
-        if (part == 2) stm.load(a.tm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
+        if (part == 2) stm.load(a.tm + nc * SquareOf<TIn>::kBytes);
         if (part == 3) {
-            smm.load(a.mm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
+            smm.load(a.mm + nc * SquareOf<TIn>::kBytes);
             so.load(op + t0 * a.dv, live);
             svec = a.vec[nc * 128 + (threadIdx.x & 127)];
         }
@@ -130,8 +134,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         if (L::kBuffers == 1 && c < chunks - 1) __syncthreads();  // the chunk before is done with the buffer
         sk.put(buf + L::kK);
         sq.put(buf + L::kQ);
-        stm.put(buf + L::kT, threadIdx.x);
-        smm.put(buf + L::kM, threadIdx.x);
+        stm.put(buf + L::kT);
+        smm.put(buf + L::kM);
         so.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
         const int next = c > from ? c - 1 : c;  // the last chunk's loads are not used
@@ -154,26 +158,29 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
             o[b] = Square::block(buf + L::kV, o_at, b);
             e[b] = *reinterpret_cast<const f32x4*>(E + tok(b, 4 * g));
         }
-        Two s[NS];
-        TIn* ds = static_cast<TIn*>(w.ds) + (nc * a.dvp + col) * DK + 8 * g;
+        Three s[NS];
+        float* ds = w.ds + (nc * a.dvp + col) * DK + 8 * g;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             operand(dS[2 * i], dS[2 * i + 1], odd, s[i]);
-            if constexpr (!kMaps) store_run(ds + 32 * i, delta::first<1>(s[i]));
+            if constexpr (!kMaps) store_run(ds + 32 * i, dS[2 * i], dS[2 * i + 1], odd);
         }
         stage_wall();
         fetch(next, 0);
-        One mf[4], mg[2];
+        Three mf[4], mg[2];
         f32x4 zb[4];
+        auto scores = [&] {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            mf[b] = Square::transposed(buf + L::kM, s_col, 1, b);
-            zb[b] = *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
-        }
+            for (int b = 0; b < 4; ++b) mf[b] = Square::template transposed_parts<3>(buf + L::kM, s_col, 1, b);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) mg[b] = Square::transposed(buf + L::kM, s_col, 0, b);
+            for (int b = 0; b < 2; ++b) mg[b] = Square::template transposed_parts<3>(buf + L::kM, s_col, 0, b);
+        };
+        if (!kLate) scores();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) zb[b] = *reinterpret_cast<const f32x4*>(E + 64 + tok(b, 4 * g));
         // dO as it is, and as E dO scale.
-        One od[2], eo[2];
+        One od[2];
+        Three eo[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             operand(o[2 * kk], o[2 * kk + 1], odd, od[kk]);
@@ -185,32 +192,41 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         for (int i = 0; i < NS; ++i)
 #pragma unroll
             for (int b = 0; b < 4; ++b) x[b] = mac(kf[i][b], s[i], i == 0 ? zero : x[b]);
+        if (kLate) scores();
         stage_wall();
         fetch(next, 1);
         Three tf[4], tg[2];
+        auto inverse = [&] {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) tf[b] = Square::template transposed_parts<3>(buf + L::kT, s_col, 1, b);
+            for (int b = 0; b < 4; ++b) tf[b] = Square::template transposed_parts<3>(buf + L::kT, s_col, 1, b);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) tg[b] = Square::template transposed_parts<3>(buf + L::kT, s_col, 0, b);
+            for (int b = 0; b < 2; ++b) tg[b] = Square::template transposed_parts<3>(buf + L::kT, s_col, 0, b);
+        };
+        if (!kLate) inverse();
 #pragma unroll
         for (int b = 0; b < 4; ++b) x[b] = mac(mf[b], od[1], x[b] * zb[b]);
 #pragma unroll
         for (int b = 0; b < 2; ++b) x[b] = mac(mg[b], od[0], x[b]);
-        Two y[2];
+        if (kLate) inverse();
+        Three y[2];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) operand(x[2 * kk], x[2 * kk + 1], odd, y[kk]);
         stage_wall();
         fetch(next, 2);
         One qc[2][DK / 16];
+        auto queries = [&] {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+            for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-            for (int i = 0; i < DK / 16; ++i) qc[kk][i] = Rows::transposed(buf + L::kQ, k_col, kk, i);
+                for (int i = 0; i < DK / 16; ++i) qc[kk][i] = Rows::transposed(buf + L::kQ, k_col, kk, i);
+        };
+        if (!kLate) queries();
         // dD = T^T dY.
 #pragma unroll
         for (int b = 0; b < 4; ++b) x[b] = mac(tf[b], y[1], zero);
 #pragma unroll
         for (int b = 0; b < 2; ++b) x[b] = mac(tg[b], y[0], x[b]);
+        if (kLate) queries();
         stage_wall();
         fetch(next, 3);
         One kc[2][DK / 16];
@@ -226,13 +242,11 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int i = 0; i < DK / 16; ++i) dS[i] = mac(qc[kk][i], eo[kk], dS[i]);
-        Two d[2];
-        TIn* dd = static_cast<TIn*>(w.dd) + (nc * a.dvp + col) * kChunk + 8 * g;
+        Three d[2];
+        float* dd = w.dd + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            One plain;
-            operand(x[2 * kk], x[2 * kk + 1], odd, plain);
-            if constexpr (!kMaps) store_run(dd + 32 * kk, plain);
+            if constexpr (!kMaps) store_run(dd + 32 * kk, x[2 * kk], x[2 * kk + 1], odd);
             operand(x[2 * kk] * -e[2 * kk], x[2 * kk + 1] * -e[2 * kk + 1], odd, d[kk]);
         }
         stage_wall();
@@ -276,51 +290,56 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
 
 // Workgroups that stay, one a CU of an MI355X, each taking every 256th chunk: the
 // next slice's rows are on their way while a slice is worked on.  (A workgroup a
-// chunk, one resident a CU for its LDS, waited for its loads two thirds of its time:
-// 8 x 16 streams of 4096 tokens 700 us.)
+// chunk, one resident a CU for its LDS, waited for its loads two thirds of its time: with
+// rows kept in bf16, 8 x 16 streams of 4096 tokens 700 us for 669.)
 constexpr int kGradWorkgroups = 256;
 
-// Columns of the state a step takes (fp32: half as many, for the LDS), and threads
-// (1024 have 128 registers each: the rows on their way spilled, 669 us for 496).
-template <typename TIn>
-constexpr int kSlice = sizeof(TIn) == 2 ? 64 : 32;
+// Columns of the state a step takes, for the LDS, and threads (1024 have 128 registers
+// each: the rows on their way spill).
+constexpr int kSlice = 32;
 constexpr int kGradThreads = 512;
 
-template <typename TIn, int DK>
+// P: parts of computed values.
+template <typename TIn, int DK, int P>
 struct GradLds {
-    static constexpr int SL = kSlice<TIn>, kS = int(sizeof(TIn)), kSquare = Tile<TIn, 64>::kBytes;
-    static constexpr int kK = 0, kQ = Tile<TIn, DK>::kBytes, kSt = 2 * kQ, kDs = kSt + SL * DK * kS;
-    static constexpr int kYt = kDs + SL * DK * kS, kDd = kYt + SL * kChunk * kS, kO = kDd + SL * kChunk * kS;
-    static constexpr int kL = kO + kChunk * SL * kS, kX = kL + kSquare, kSums = kX + kSquare;
-    static constexpr int kBytes = kSums + int(sizeof(double)) * kChunk + int(sizeof(float)) * (21 * kChunk + 16);
+    static constexpr int SL = kSlice, kS = int(sizeof(TIn)), kP = sizeof(TIn) == 2 ? P : 1;  // planes
+    using Out = Tile<TIn, sizeof(TIn) == 2 ? 64 : SL>;  // rows of a slice of dO
+    static constexpr int kStPlane = SL * DK * kS, kYtPlane = SL * kChunk * kS, kSquare = kPartsBytes<TIn, 64, P>;
+    static constexpr int kK = 0, kQ = Tile<TIn, DK>::kBytes, kSt = 2 * kQ, kDs = kSt + kP * kStPlane;
+    static constexpr int kYt = kDs + kP * kStPlane, kDd = kYt + kP * kYtPlane, kO = kDd + kP * kYtPlane, kEnd = kO + Out::kBytes;
+    static constexpr int kSumBytes = int(sizeof(double)) * kChunk + int(sizeof(float)) * (21 * kChunk + 16);
+    // L and X, over the slices' tiles where there is no more LDS: a barrier more.
+    static constexpr bool kOver = kEnd + 2 * kSquare + kSumBytes > kGfx950LdsBytes;
+    static constexpr int kL = kOver ? kSt : kEnd, kX = kL + kSquare, kSums = kOver ? kEnd : kX + kSquare;
+    static constexpr int kBytes = kSums + kSumBytes;
+    static_assert(!kOver || kX + kSquare <= kO);
 };
 
-// ROWS dense rows of K values: a thread's 16-byte pieces in registers, zeros past the
-// first `rows`, then in a tile.
-template <typename E, int K, int ROWS, int NT>
-struct Pieces {
-    static constexpr int kChunks = Tile<E, K>::kChunks, kTotal = ROWS * kChunks, kPer = (kTotal + NT - 1) / NT;
-    uint4 x[kPer];
-    __device__ __forceinline__ void load(const E* p, int rows, int tid) {
-        const auto r = mfma::make_rsrc(p, rows * K * int(sizeof(E)));
+// Dense rows of K fp32 values in memory, ROWS of them, to a tile in P planes, PLANE bytes apart.
+template <typename E, int K, int ROWS, int NT, int P, int PLANE = Tile<E, K>::kBytes>
+struct StageDense {
+    static constexpr int kTotal = ROWS * K / 4, kPer = (kTotal + NT - 1) / NT;
+    f32x4 x[kPer];
+    // `rows` of them, zeros behind.
+    __device__ __forceinline__ void load(const float* p, int rows, int tid) {
+        const auto r = mfma::make_rsrc(p, rows * K * 4);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int q = tid + i * NT;
-            if (kTotal % NT == 0 || q < kTotal) x[i] = mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * q);
-        }
+        for (int i = 0; i < kPer; ++i)
+            if (kTotal % NT == 0 || tid + i * NT < kTotal)
+                x[i] = __builtin_bit_cast(f32x4, mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * (tid + i * NT)));
     }
     __device__ __forceinline__ void put(unsigned char* t, int tid) const {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int q = tid + i * NT;
             if (kTotal % NT == 0 || q < kTotal)
-                *reinterpret_cast<uint4*>(t + Tile<E, K>::at(q / kChunks, q % kChunks)) = x[i];
+                Tile<E, K>::template put4_parts<P, PLANE>(t, Tile<E, K>::four_at(q / (K / 4), 4 * (q % (K / 4))), x[i]);
         }
     }
 };
 
-// 64 rows of `width` values by stride, of which `live` are there, in K columns.
-template <typename TIn, int K, int NT, bool kVec>
+// 64 rows of `width` values by stride, of which `live` are there, in K columns; to a tile T.
+template <typename TIn, int K, int NT, bool kVec, typename T = Tile<TIn, K>>
 struct RowPieces {
     static constexpr int kVecs = Eight<TIn>::kVecs, kTotal = kChunk * (K / 8), kPer = (kTotal + NT - 1) / NT;
     std::conditional_t<kVec, Eight<TIn>, Ragged<TIn>> x[kPer];
@@ -356,17 +375,10 @@ struct RowPieces {
             else
                 e = x[i].get(at_ + row * stride_, 8 * u, width_);
 #pragma unroll
-            for (int j = 0; j < kVecs; ++j) *reinterpret_cast<uint4*>(t + Tile<TIn, K>::at(row, kVecs * u + j)) = e.v[j];
+            for (int j = 0; j < kVecs; ++j) *reinterpret_cast<uint4*>(t + T::at(row, kVecs * u + j)) = e.v[j];
         }
     }
 };
-
-template <typename TIn>
-__device__ __forceinline__ float dot16(const uint4& x, const uint4& y, float s) {
-#pragma unroll
-    for (int i = 0; i < 16 / int(sizeof(TIn)); ++i) s = fmaf(mfma::Elem<TIn>::get(x, i), mfma::Elem<TIn>::get(y, i), s);
-    return s;
-}
 
 // What a workgroup does between two barriers: a slice of the value columns of a
 // stream in a chunk.  Only live ones are taken: the walk wrote the zeros of the rest.
@@ -395,15 +407,16 @@ __device__ __forceinline__ bool next_stream(const DeltaArgs& a, int items, GradU
 // Wave (th, dq): TB blocks of 16 tokens and a quarter of the key columns; of the 64 x
 // 64 matrices its tokens' rows and 16 columns.  kShared: key streams with several
 // value streams, whose dQ and dK are summed in registers.
-template <typename TIn, int DK, bool kVec, bool kVecV, bool kShared>
+template <typename TIn, int DK, int kParts, bool kVec, bool kVecV, bool kShared>
 __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBwdArgs w, int items) {
     extern __shared__ __align__(16) unsigned char lds[];
     const DeltaArgs& a = w.f;
-    using L = GradLds<TIn, DK>;
+    using L = GradLds<TIn, DK, kParts>;
     using Rows = Tile<TIn, DK>;
     using Square = Tile<TIn, 64>;
-    using Out = Tile<TIn, L::SL>;
+    using Out = typename L::Out;
     using One = OneT<TIn>;
+    using Many = PartsT<TIn, kParts>;
     constexpr int NB = DK / 64, SL = L::SL, NT = kGradThreads, NW = NT / 64, TB = 16 / NW;
     double* G = reinterpret_cast<double*>(lds + L::kSums);
     float* beta = reinterpret_cast<float*>(G + kChunk);
@@ -416,9 +429,9 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), th = wave >> 2, dq = wave & 3;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-    Pieces<TIn, DK, SL, NT> ps, pd;
-    Pieces<TIn, 64, SL, NT> py, pdd;
-    RowPieces<TIn, SL, NT, kVecV> po;
+    StageDense<TIn, DK, SL, NT, kParts, L::kStPlane> ps, pd;
+    StageDense<TIn, 64, SL, NT, kParts, L::kYtPlane> py, pdd;
+    RowPieces<TIn, SL, NT, kVecV, Out> po;
     RowPieces<TIn, DK, NT, kVec> pk, pq;
     uint32_t pg = 0, pb = 0;
     // The loads of a unit: its slice, with a stream's first the gates, with a chunk's first K and Q.
@@ -441,10 +454,10 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
                 pb = gate_bits(a.beta, at, a.gate_f32);
             }
         }
-        ps.load(static_cast<const TIn*>(a.st) + slice * DK, rows, tid);
-        pd.load(static_cast<const TIn*>(w.ds) + slice * DK, rows, tid);
-        py.load(static_cast<const TIn*>(a.yt) + slice * kChunk, rows, tid);
-        pdd.load(static_cast<const TIn*>(w.dd) + slice * kChunk, rows, tid);
+        ps.load(a.st + slice * DK, rows, tid);
+        pd.load(w.ds + slice * DK, rows, tid);
+        py.load(a.yt + slice * kChunk, rows, tid);
+        pdd.load(w.dd + slice * kChunk, rows, tid);
         po.load(static_cast<const TIn*>(w.dout) + (n * a.T + t0) * a.dv + u.v0, a.dv, u.live, a.dv - u.v0, tid);
     };
 
@@ -490,7 +503,9 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
         }
 #pragma unroll
         for (int i = 0; i < ps.kPer; ++i)
-            if (ps.kTotal % NT == 0 || tid + i * NT < ps.kTotal) s_ds = dot16<TIn>(ps.x[i], pd.x[i], s_ds);
+            if (ps.kTotal % NT == 0 || tid + i * NT < ps.kTotal)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s_ds = fmaf(ps.x[i][r], pd.x[i][r], s_ds);
         ps.put(lds + L::kSt, tid);
         pd.put(lds + L::kDs, tid);
         py.put(lds + L::kYt, tid);
@@ -508,13 +523,14 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
         TIn* dv = w.dv ? static_cast<TIn*>(w.dv) + (n * a.T + t0) * a.dv : nullptr;
 #pragma unroll
         for (int kk = 0; kk < SL / 32; ++kk) {
-            const One yc = Square::transposed(lds + L::kYt, s_col, kk, dq);
-            One ya[TB], da[TB], oa[TB];
+            const Many yc = Square::template transposed_parts<kParts, L::kYtPlane>(lds + L::kYt, s_col, kk, dq);
+            Many ya[TB], da[TB];
+            One oa[TB];
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const int b = TB * th + i;
-                ya[i] = Square::transposed(lds + L::kYt, s_col, kk, b);
-                da[i] = Square::transposed(lds + L::kDd, s_col, kk, b);
+                ya[i] = Square::template transposed_parts<kParts, L::kYtPlane>(lds + L::kYt, s_col, kk, b);
+                da[i] = Square::template transposed_parts<kParts, L::kYtPlane>(lds + L::kDd, s_col, kk, b);
                 oa[i] = Out::one(lds + L::kO, o_row, b, kk);
                 P[i] = mac(oa[i], yc, P[i]);
                 H[i] = mac(da[i], yc, H[i]);
@@ -523,9 +539,9 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
                     const int cv = v0 + 32 * kk + 8 * g;
                     TIn* o = dv + int64_t(tok(b, lr)) * a.dv + cv;
                     if (kVecV && cv + 8 <= a.dv) {
-                        store_run(o, da[i]);
+                        store_run(o, delta::first<1>(da[i]));
                     } else {
-                        const auto run = __builtin_bit_cast(Eight<TIn>, da[i]);
+                        const auto run = __builtin_bit_cast(Eight<TIn>, delta::first<1>(da[i]));
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             constexpr int kPer = 16 / int(sizeof(TIn));
@@ -536,8 +552,8 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const One st = Rows::transposed(lds + L::kSt, k_col, kk, dq * NB + b);
-                const One ds = Rows::transposed(lds + L::kDs, k_col, kk, dq * NB + b);
+                const Many st = Rows::template transposed_parts<kParts, L::kStPlane>(lds + L::kSt, k_col, kk, dq * NB + b);
+                const Many ds = Rows::template transposed_parts<kParts, L::kStPlane>(lds + L::kDs, k_col, kk, dq * NB + b);
 #pragma unroll
                 for (int i = 0; i < TB; ++i) {
                     qs[i][b] = mac(st, oa[i], qs[i][b]);
@@ -547,6 +563,7 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
             }
         }
         if (!last) continue;
+        if constexpr (L::kOver) __syncthreads();  // the slice's products are done with its tiles
         // Rows tok(TB th + i, 4 g + r), column tok(dq, lr) of the 64 x 64 matrices.
         const int jc = tok(dq, lr);
         {
@@ -576,8 +593,8 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
                     if (lr == 15) row_sum[dq * kChunk + row] = in_row;
                 }
                 const int at = Square::four_at(jc, tok(TB * th + i, 4 * g));
-                Square::put4(lds + L::kL, at, Lm);
-                Square::put4(lds + L::kX, at, Xm);
+                Square::template put4_parts<kParts>(lds + L::kL, at, Lm);
+                Square::template put4_parts<kParts>(lds + L::kX, at, Xm);
             }
             in_col += __shfl_xor(in_col, 16);
             in_col += __shfl_xor(in_col, 32);
@@ -650,14 +667,14 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
             for (int i = 0; i < TB; ++i) {
                 const int b = TB * th + i;
                 const bool low = kk <= (b >> 1), high = kk >= (b >> 1);
-                One l, lt, x, xt;
+                Many l, lt, x, xt;
                 if (low) {
-                    l = Square::transposed(lds + L::kL, s_col, kk, b);
-                    x = Square::transposed(lds + L::kX, s_col, kk, b);
+                    l = Square::template transposed_parts<kParts>(lds + L::kL, s_col, kk, b);
+                    x = Square::template transposed_parts<kParts>(lds + L::kX, s_col, kk, b);
                 }
                 if (high) {
-                    lt = Square::one(lds + L::kL, s_row, b, kk);
-                    xt = Square::one(lds + L::kX, s_row, b, kk);
+                    lt = Square::template parts<kParts>(lds + L::kL, s_row, b, kk);
+                    xt = Square::template parts<kParts>(lds + L::kX, s_row, b, kk);
                 }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
@@ -701,11 +718,25 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
     }
 }
 
+template <typename TIn, int DK, int P, bool kVec, bool kVecV>
+hipError_t launch_grads(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
+    constexpr int grads = GradLds<TIn, DK, P>::kBytes;
+    static_assert(grads <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
+    const int items = int(r.Nk * w.f.chunks);
+    const unsigned grid = unsigned(items < kGradWorkgroups ? items : kGradWorkgroups);
+    constexpr bool kAll = kVec && kVecV;  // others have one form
+    if (w.f.group > 1 || !kAll)
+        delta_grads_kernel<TIn, DK, P, kVec, kVecV, true><<<grid, kGradThreads, grads, stream>>>(w, items);
+    else
+        delta_grads_kernel<TIn, DK, P, kVec, kVecV, !kAll><<<grid, kGradThreads, grads, stream>>>(w, items);
+    return hipGetLastError();
+}
+
 template <typename TIn, int DK, bool kVec, bool kVecV>
 hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_t stream) {
     using L = BwdWalkLds<TIn, DK>;
-    constexpr int walk = L::kBuffers * L::kBytes, grads = GradLds<TIn, DK>::kBytes;
-    static_assert(walk <= kGfx950LdsBytes && grads <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
+    constexpr int walk = L::kBuffers * L::kBytes;
+    static_assert(walk <= kGfx950LdsBytes, "gfx950 gives a workgroup at most 160 KB of LDS");
     auto grid_of = [&](int64_t streams) { return unsigned((streams + 7) / 8 * 8 * ((r.dv + 63) / 64)); };
     if (w.f.segs > 1) {
         delta_bwd_walk_kernel<TIn, DK, kVec, kVecV, true><<<grid_of(r.N * (w.f.segs - 1)), kThreads, walk, stream>>>(w);
@@ -717,14 +748,9 @@ hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     if (!w.dq && !w.dk && !w.dv && !w.dgate && !w.dbeta) return hipSuccess;
-    const int items = int(r.Nk * w.f.chunks);
-    const unsigned grid = unsigned(items < kGradWorkgroups ? items : kGradWorkgroups);
-    constexpr bool kAll = kVec && kVecV;  // others have one form
-    if (w.f.group > 1 || !kAll)
-        delta_grads_kernel<TIn, DK, kVec, kVecV, true><<<grid, kGradThreads, grads, stream>>>(w, items);
-    else
-        delta_grads_kernel<TIn, DK, kVec, kVecV, !kAll><<<grid, kGradThreads, grads, stream>>>(w, items);
-    return hipGetLastError();
+    // Gradients that are all rounded to bf16 right away take two parts, those of fp32 gates three.
+    if (sizeof(TIn) == 2 && w.f.gate_f32) return launch_grads<TIn, DK, 3, kVec, kVecV>(r, w, stream);
+    return launch_grads<TIn, DK, 2, kVec, kVecV>(r, w, stream);
 }
 
 template <typename TIn, bool kVec, bool kVecV>
@@ -740,10 +766,10 @@ hipError_t launch_by_pieces(const DeltaRule& r, const DeltaBwdArgs& w, hipStream
 }  // namespace
 
 int64_t delta_bwd_bytes(const DeltaRule& r) {
-    const int64_t nc = r.N * delta_chunks(r), es = r.dtype == RACE_BF16 ? 2 : 4, dvp = (r.dv + 15) / 16 * 16;
+    const int64_t nc = r.N * delta_chunks(r), dvp = (r.dv + 15) / 16 * 16;
     const DeltaLayout l = delta_layout(r);
     // With segments, their ends and what they add to a gradient.
-    return round256(nc * dvp * dk_padded(r) * es) + round256(nc * dvp * kChunk * es) + (l.map_bytes - l.starts);
+    return round256(nc * dvp * dk_padded(r) * 4) + round256(nc * dvp * kChunk * 4) + (l.map_bytes - l.starts);
 }
 
 hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const void* dout, const float* dfinal,
@@ -752,16 +778,16 @@ hipError_t launch_delta_bwd(const DeltaRule& r, const DeltaInputs& in, const voi
     w.f = delta_args(r, in);
     const DeltaLayout l = delta_layout(r);
     unsigned char* base = const_cast<unsigned char*>(static_cast<const unsigned char*>(records));
-    w.f.tm = reinterpret_cast<float*>(base), w.f.mm = reinterpret_cast<float*>(base + l.mm), w.f.vec = reinterpret_cast<float*>(base + l.vec);
-    w.f.st = base + l.solve_bytes, w.f.yt = base + l.yt;
+    w.f.tm = base, w.f.mm = base + l.mm, w.f.vec = reinterpret_cast<float*>(base + l.vec);
+    w.f.st = reinterpret_cast<float*>(base + l.solve_bytes), w.f.yt = reinterpret_cast<float*>(base + l.yt);
     w.dout = dout, w.dfinal = dfinal;
-    const int64_t es = r.dtype == RACE_BF16 ? 2 : 4;
-    w.ds = scratch;
-    w.dd = static_cast<unsigned char*>(scratch) + round256(r.N * w.f.chunks * w.f.dvp * dk_padded(r) * es);
+    const int64_t nc = r.N * w.f.chunks;
+    w.ds = static_cast<float*>(scratch);
+    w.dd = w.ds + round256(nc * w.f.dvp * dk_padded(r) * 4) / 4;
     w.f.segs = l.segs, w.f.seg_chunks = l.seg_chunks;
     if (l.segs > 1) {
         w.f.map_a = reinterpret_cast<float*>(base + l.map_a);
-        w.f.starts = reinterpret_cast<float*>(static_cast<unsigned char*>(w.dd) + round256(r.N * w.f.chunks * w.f.dvp * kChunk * es));
+        w.f.starts = w.dd + round256(nc * w.f.dvp * kChunk * 4) / 4;
         w.f.map_x = w.f.starts + (l.map_x - l.starts) / 4;
     }
     w.dq = g.dq, w.dk = g.dk, w.dv = g.dv, w.dgate = g.dgate, w.dbeta = g.dbeta, w.dstate = g.dstate;

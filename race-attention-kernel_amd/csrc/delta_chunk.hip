@@ -30,8 +30,7 @@
 // another, 4 us with a wave a SIMD, its matrix cores busy for less than a third of it; so
 // its waves hold no more than they need, loads for the next chunk go out between the
 // stages, and few streams are walked in segments (delta_segment_chunks).  128 streams
-// of 4096 bf16 tokens, 128 x 128, with records: solve 105 us, walk 385 us (with every
-// factor in two parts and M in one 306 us, its outputs off by half a rounding more).
+// of 4096 bf16 tokens, 128 x 128, with records: solve 116 us, walk 406 us.
 #include <algorithm>
 #include <utility>
 
@@ -166,7 +165,8 @@ __global__ __launch_bounds__(kThreads, sizeof(TIn) * DK <= 256 ? 4 : 2) void del
     for (int j = 0; j < 4; ++j) {
         gb[j] = weights(o, j);
         if (j <= (o | 1))  // the others are not read
-            store4_of(a.mm + nc * (kChunk * kChunk) + (16 * o + lr) * kChunk + 16 * j + 4 * g, below(o, j, gb[j] * qk[j] * a.scale, 0));
+            SquareOf<TIn>::put4(a.mm + nc * SquareOf<TIn>::kBytes, 16 * o + lr, 16 * j + 4 * g, below(o, j, gb[j] * qk[j] * a.scale, 0),
+                                a.st ? 3 : 2);  // the third part is the backward's
         if (!kAll) gb[j] = weights(wave, j);
     }
     __syncthreads();
@@ -217,13 +217,17 @@ __global__ __launch_bounds__(kThreads, sizeof(TIn) * DK <= 256 ? 4 : 2) void del
     }
     __syncthreads();
     const int row = threadIdx.x >> 2, c0 = (threadIdx.x & 3) * 16;
-    float* tm = a.tm + nc * (kChunk * kChunk) + row * kChunk + c0;
+    unsigned char* tm = a.tm + nc * SquareOf<TIn>::kBytes;
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-        f32x4 x = *reinterpret_cast<const f32x4*>(T + row * kSolvePitch + c0 + e);
+    for (int e = 0; e < 16; e += 8) {
+        f32x4 x[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = c0 + e + r <= row ? x[r] : 0.f;
-        store4_of(tm + e, x);
+        for (int h = 0; h < 2; ++h) {
+            x[h] = *reinterpret_cast<const f32x4*>(T + row * kSolvePitch + c0 + e + 4 * h);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[h][r] = c0 + e + 4 * h + r <= row ? x[h][r] : 0.f;
+        }
+        SquareOf<TIn>::put8(tm, row, c0 + e, x[0], x[1]);
     }
 }
 
@@ -290,8 +294,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
     }
 
     Stage<TIn, DK, kThreads, kVec> sk, sq;
-    StageDense<TIn, 64, kChunk, kThreads, 3> stm;
-    StageDense<TIn, 64, kChunk, kThreads, 2> smm;
+    StageSquare<TIn, 3> stm;
+    StageSquare<TIn, 2> smm;
     Stage<TIn, 64, kThreads, kVecV> sv;
     float svec;
     sk.init(a.kt, a.dk);
@@ -303,9 +307,9 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         const int live = int(len - t0 < kChunk ? len - t0 : kChunk);
         if (part == 0) sk.load(kp + t0 * a.kt, live);
         if (part == 1 && kMode != kMaps) sq.load(qp + t0 * a.qt, live);
-        if (part == 2) stm.load(a.tm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
+        if (part == 2) stm.load(a.tm + nc * SquareOf<TIn>::kBytes);
         if (part == 3) {
-            if (kMode != kMaps) smm.load(a.mm + nc * (kChunk * kChunk), kChunk, threadIdx.x);
+            if (kMode != kMaps) smm.load(a.mm + nc * SquareOf<TIn>::kBytes);
             sv.load(vp + t0 * a.vt, live);
             svec = a.vec[nc * 128 + (threadIdx.x & 127)];
         }
@@ -320,8 +324,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         if (L::kBuffers == 1 && c > from) __syncthreads();  // the chunk before is done with the buffer
         sk.put(buf + L::kK);
         if (kMode != kMaps) sq.put(buf + L::kQ);
-        stm.put(buf + L::kT, threadIdx.x);
-        if (kMode != kMaps) smm.put(buf + L::kM, threadIdx.x);
+        stm.put(buf + L::kT);
+        if (kMode != kMaps) smm.put(buf + L::kM);
         sv.put(buf + L::kV);
         reinterpret_cast<float*>(buf + L::kVec)[threadIdx.x & 127] = svec;
         const int next = c + 1 < chunks ? c + 1 : c;  // the last chunk's loads are not used
@@ -342,9 +346,9 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
 #pragma unroll
         for (int i = 0; i < NS; ++i) operand(S[2 * i], S[2 * i + 1], odd, s[i]);
         if constexpr (kMode == kRecording) {
-            TIn* st = static_cast<TIn*>(a.st) + (nc * a.dvp + col) * DK + 8 * g;
+            float* st = a.st + (nc * a.dvp + col) * DK + 8 * g;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) store_run(st + 32 * i, delta::first<1>(s[i]));
+            for (int i = 0; i < NS; ++i) store_run(st + 32 * i, S[2 * i], S[2 * i + 1], odd);
         }
         stage_wall();
         fetch(next, 0);
@@ -407,9 +411,9 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
             operand(x[2 * kk] * zb[2 * kk], x[2 * kk + 1] * zb[2 * kk + 1], odd, z[kk]);
         }
         if constexpr (kMode == kRecording) {
-            TIn* yt = static_cast<TIn*>(a.yt) + (nc * a.dvp + col) * kChunk + 8 * g;
+            float* yt = a.yt + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, delta::first<1>(y[kk]));
+            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, x[2 * kk], x[2 * kk + 1], odd);
         }
         // S = e^{G_last} S + K^T (Z b Y).
         const float decay = E[63];
@@ -661,18 +665,19 @@ int64_t delta_segment_chunks(const DeltaRule& r) {
 int64_t delta_chunks(const DeltaRule& r) { return (r.T + kChunk - 1) / kChunk; }
 
 DeltaLayout delta_layout(const DeltaRule& r) {
-    const int64_t nc = r.N * delta_chunks(r), es = r.dtype == RACE_BF16 ? 2 : 4, dvp = (r.dv + 15) / 16 * 16;
+    const int64_t nc = r.N * delta_chunks(r), dvp = (r.dv + 15) / 16 * 16;
     DeltaLayout l;
-    l.mm = round256(nc * kChunk * kChunk * 4);
-    l.vec = l.mm + round256(nc * kChunk * kChunk * 4);
+    const int64_t square = r.dtype == RACE_BF16 ? SquareOf<bf16_t>::kBytes : SquareOf<float>::kBytes;
+    l.mm = round256(nc * square);
+    l.vec = l.mm + round256(nc * square);
     l.solve_bytes = l.vec + round256(nc * 512);
     const int64_t each = delta_segment_chunks(r), segs = std::max<int64_t>((delta_chunks(r) + each - 1) / each, 1);
     l.segs = int(segs), l.seg_chunks = int(each);
     l.starts = segs > 1 ? round256(r.N * segs * r.dk * r.dk * 4) : 0;
     l.map_x = l.starts + round256(r.N * segs * r.dk * r.dv * 4);
     l.map_bytes = segs > 1 ? l.map_x + round256(r.N * segs * r.dk * r.dv * 4) : 0;
-    l.yt = l.solve_bytes + round256(nc * dvp * dk_padded(r) * es);
-    l.map_a = l.yt + round256(nc * dvp * kChunk * es);
+    l.yt = l.solve_bytes + round256(nc * dvp * dk_padded(r) * 4);
+    l.map_a = l.yt + round256(nc * dvp * kChunk * 4);
     l.record_bytes = l.map_a + l.starts;
     return l;
 }
@@ -692,9 +697,9 @@ hipError_t launch_delta(const DeltaRule& r, const DeltaInputs& in, const float* 
     const DeltaLayout l = delta_layout(r);
     unsigned char* maps = static_cast<unsigned char*>(workspace);
     unsigned char* base = records ? static_cast<unsigned char*>(records) : maps + l.map_bytes;
-    a.tm = reinterpret_cast<float*>(base), a.mm = reinterpret_cast<float*>(base + l.mm);
+    a.tm = base, a.mm = base + l.mm;
     a.vec = reinterpret_cast<float*>(base + l.vec);
-    if (records) a.st = base + l.solve_bytes, a.yt = base + l.yt;
+    if (records) a.st = reinterpret_cast<float*>(base + l.solve_bytes), a.yt = reinterpret_cast<float*>(base + l.yt);
     a.segs = l.segs, a.seg_chunks = l.seg_chunks;
     if (l.segs > 1) {
         a.map_a = reinterpret_cast<float*>(records ? base + l.map_a : maps);

@@ -132,6 +132,12 @@ __device__ __forceinline__ void store_run(float* p, const OneT<float>& x) {
     *reinterpret_cast<f32x4*>(p) = x.a;
     *reinterpret_cast<f32x4*>(p + 4) = x.b;
 }
+// A block pair's accumulators, as such a run.
+__device__ __forceinline__ void store_run(float* p, const f32x4& x0, const f32x4& x1, bool odd) {
+    OneT<float> x;
+    operand(x0, x1, odd, x);
+    store_run(p, x);
+}
 
 // A wall the scheduler moves nothing across.  The walks have one wave a SIMD:
 // nothing hides a read's latency but the wave's own instructions, and left alone
@@ -463,26 +469,88 @@ struct Stage {
     }
 };
 
-// Dense rows of K fp32 values in memory, ROWS of them, to a tile in P planes, PLANE bytes apart.
-template <typename E, int K, int ROWS, int NT, int P, int PLANE = Tile<E, K>::kBytes>
-struct StageDense {
-    static constexpr int kTotal = ROWS * K / 4, kPer = (kTotal + NT - 1) / NT;
-    f32x4 x[kPer];
-    // `rows` of them, zeros behind.
-    __device__ __forceinline__ void load(const float* p, int rows, int tid) {
-        const auto r = mfma::make_rsrc(p, rows * K * 4);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (kTotal % NT == 0 || tid + i * NT < kTotal)
-                x[i] = __builtin_bit_cast(f32x4, mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * (tid + i * NT)));
+// T or M of a chunk in memory: a lower triangle [64][64], as fp32 values or as three
+// parts of bf16.  A part is rows 32 .. 63, then the first half of rows 0 .. 31: what
+// is right of it is not read anywhere.  (Split where they are made, not in the walks,
+// whose chains would wait for it: 128 streams of 4096 bf16 tokens, 128 x 128, solve and
+// walks 104 + 437 + 405 -> 116 + 406 + 382 us.)
+template <typename E>
+struct SquareOf {
+    static constexpr int64_t kBytes = kChunk * kChunk * 4;
+    // Four (eight) values from column `col` of a row, their first `parts` parts.
+    __device__ __forceinline__ static void put4(unsigned char* p, int row, int col, const f32x4& x, int) {
+        *reinterpret_cast<f32x4*>(p + (row * kChunk + col) * 4) = x;
     }
-    __device__ __forceinline__ void put(unsigned char* t, int tid) const {
+    __device__ __forceinline__ static void put8(unsigned char* p, int row, int col, const f32x4& x, const f32x4& y) {
+        put4(p, row, col, x, 1), put4(p, row, col + 4, y, 1);
+    }
+};
+template <>
+struct SquareOf<bf16_t> {
+    static constexpr int kHalf = 32 * kChunk * 2, kPart = kHalf + kHalf / 2;
+    static constexpr int64_t kBytes = 3 * kPart;
+    __device__ __forceinline__ static int at(int row, int col) {
+        return row < 32 ? kHalf + (row * 32 + col) * 2 : ((row - 32) * kChunk + col) * 2;
+    }
+    __device__ __forceinline__ static void put4(unsigned char* p, int row, int col, f32x4 x, int parts) {
+        if (row < 32 && col >= 32) return;
+        p += at(row, col);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int q = tid + i * NT;
-            if (kTotal % NT == 0 || q < kTotal)
-                Tile<E, K>::template put4_parts<P, PLANE>(t, Tile<E, K>::four_at(q / (K / 4), 4 * (q % (K / 4))), x[i]);
+        for (int i = 0; i < 3; ++i)
+            if (i < 2 || parts > 2) *reinterpret_cast<uint2*>(p + i * kPart) = take_part(x);
+    }
+    __device__ __forceinline__ static void put8(unsigned char* p, int row, int col, f32x4 x, f32x4 y) {
+        if (row < 32 && col >= 32) return;
+        p += at(row, col);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const uint2 a = take_part(x), b = take_part(y);
+            *reinterpret_cast<uint4*>(p + i * kPart) = make_uint4(a.x, a.y, b.x, b.y);
         }
+    }
+};
+
+// Its first P parts (or its values) to a tile in as many planes, by a walk's threads.
+template <typename E, int P>
+struct StageSquare {
+    f32x4 x[4];
+    __device__ __forceinline__ void load(const unsigned char* p) {
+        const auto r = mfma::make_rsrc(p, SquareOf<E>::kBytes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            x[i] = __builtin_bit_cast(f32x4, mfma::buf_load16<mfma::kPolicyDefault>(r, 16 * (int(threadIdx.x) + i * kThreads)));
+    }
+    __device__ __forceinline__ void put(unsigned char* t) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = int(threadIdx.x) + i * kThreads;
+            *reinterpret_cast<f32x4*>(t + Tile<E, 64>::at(q / 16, q % 16)) = x[i];
+        }
+    }
+};
+template <int P>
+struct StageSquare<bf16_t, P> {
+    static_assert(kThreads == 256);
+    using S = SquareOf<bf16_t>;
+    using T = Tile<bf16_t, 64>;
+    uint4 low[P], high[(P + 1) / 2];  // rows 32 .. 63, a part each; rows 0 .. 31, two parts each
+    __device__ __forceinline__ void load(const unsigned char* p) {
+        const int tid = threadIdx.x;
+        const auto r = mfma::make_rsrc(p, P * S::kPart);
+#pragma unroll
+        for (int i = 0; i < P; ++i) low[i] = mfma::buf_load16<mfma::kPolicyDefault>(r, i * S::kPart + 16 * tid);
+#pragma unroll
+        for (int i = 0; i < (P + 1) / 2; ++i)  // past the last part, outside the view
+            high[i] = mfma::buf_load16<mfma::kPolicyDefault>(r, (2 * i + (tid >> 7)) * S::kPart + S::kHalf + 16 * (tid & 127));
+    }
+    __device__ __forceinline__ void put(unsigned char* t) const {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < P; ++i) *reinterpret_cast<uint4*>(t + i * T::kBytes + T::at(32 + (tid >> 3), tid & 7)) = low[i];
+#pragma unroll
+        for (int i = 0; i < (P + 1) / 2; ++i)
+            if (2 * i + 1 < P || tid < 128)
+                *reinterpret_cast<uint4*>(t + (2 * i + (tid >> 7)) * T::kBytes + T::at((tid & 127) >> 2, tid & 3)) = high[i];
     }
 };
 
@@ -495,9 +563,9 @@ struct DeltaArgs {
     const float* state;
     void* out;
     float* final_state;
-    float *tm, *mm;  // [N][chunks] of T and M, [64][64]
+    unsigned char *tm, *mm;  // [N][chunks] of T and M, as SquareOf has them
     float* vec;     // [N][chunks][128]: E, then Z b
-    void *st, *yt;  // nullable: [N][chunks][dvp] columns of S [DK] and Y [64], in the rows' type
+    float *st, *yt;  // nullable: [N][chunks][dvp] columns of S [DK] and Y [64]
     // Segments of seg_chunks chunks that are walked at once, from starts [N][segs][dk][dv];
     // a segment takes a state s to map_a s + map_x, [N][segs][dk][dk] and [dk][dv].
     float *starts, *map_a, *map_x;

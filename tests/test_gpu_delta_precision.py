@@ -3,10 +3,11 @@
 Tolerances.  bf16 values are fp32 values, so the recurrence of bf16 rows owes what
 fp32 rows owe: 384 * 2^-24 of the terms (test_gpu_delta_rule).  Results in 32 bits are
 held to that as they are.  Results in bf16 are off by the rounding of a value, at most
-half of its step, and by no more than that tolerance beyond it, with 2 * 2^-16 added
-for outputs, whose product of two factors takes each in two parts of bf16: what lies
-beyond a value's half step counts, in 2-norm over a stream and over its rows (8 times,
-as there)."""
+half of its step, and by no more than that tolerance beyond it: what lies beyond a value's
+half step counts, in 2-norm over a stream and over its rows (8 times, as there).  Where
+only bf16 comes of a product, its computed factors are taken in two parts of bf16, each
+within 2^-16: two of them in outputs, four in the gradients of calls with bf16 gates (the
+pairs of tokens take two rows' and then their own matrix's)."""
 from __future__ import annotations
 
 import pytest
@@ -67,3 +68,19 @@ def test_small_values_overwrite_a_large_state(race, cuda, T):
         err = float((final[:, 0] - v[:, -1].float()).abs().max())
         say(T, f"{err:.1e} of {8 * 2.0 ** -24 * largest:.1e}")
         assert err <= 8 * 2.0 ** -24 * largest
+
+
+@pytest.mark.parametrize("gate_dtype", [F32, BF16])
+@pytest.mark.parametrize("N, Nk, T, dk, dv", SHAPES)
+def test_gradients(race, cuda, N, Nk, T, dk, dv, gate_dtype):
+    *args, dout, dfinal = make(N, Nk, T, dk, dv, BF16, seed=33, gate_dtype=gate_dtype)
+    leaves = [t.clone().requires_grad_(True) for t in args]
+    outs = race.race_delta_rule(*leaves, scale=dk ** -0.5)
+    grads = torch.autograd.grad(outs, leaves, (dout, dfinal))
+    want = reference(*(t.float() for t in args), scale=dk ** -0.5, dout=dout, dfinal=dfinal)
+    for name, t, d in zip(NAMES, args, grads):
+        assert d.dtype == t.dtype
+        if t.dtype == BF16:
+            rounded_once("d" + name, d, want["d" + name], f"T={T}", pairs=0 if gate_dtype == F32 else 4)
+        else:
+            close("d" + name, d, want["d" + name], F32, f"T={T}")
