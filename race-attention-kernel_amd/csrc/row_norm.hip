@@ -131,7 +131,11 @@ __device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(
 
 // The factor to 8 bits for a largest magnitude, and the scale it leaves.  Finite
 // where the magnitude is subnormal; zero for rows of zeros, whose scale is zero.
-__device__ __forceinline__ float to_e4m3_factor(float most) { return most > 0.f ? fminf(448.f / most, FLT_MAX) : 0.f; }
+// Products of bf16 values often lie half way between two values of 8 bits, and the
+// factors' rounding decides: y is (s r) w, r rounded once from a mean that is the sum
+// times 1 / D, and the factor 448 times the reciprocal, as elementwise passes over rows have
+// them, so that both take the same one wherever the sum of squares is the same.
+__device__ __forceinline__ float to_e4m3_factor(float most) { return most > 0.f ? fminf(448.f * (1.f / most), FLT_MAX) : 0.f; }
 
 template <int V>
 __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&y)[V], float f) {
@@ -155,6 +159,14 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&y)[V], floa
     }
 }
 
+// The mean rounded before eps is added, and the root once (rsqrtf is a step off now and then).
+__device__ __forceinline__ float mean_and_eps(float sum, float inv_d, float eps) {
+#pragma clang fp contract(off)
+    const float mean = sum * inv_d;
+    return mean + eps;
+}
+__device__ __forceinline__ float rounded_rsqrt(float x) { return float(rsqrt(double(x))); }
+
 // NP pieces of V values per thread, piece j at column (j NT + thread) V.
 template <typename TIn, int V, int NP, int NT, bool kE4m3>
 __global__ __launch_bounds__(kRowThreads<NT>) void add_norm_kernel(const AddNormArgs a) {
@@ -171,6 +183,7 @@ __global__ __launch_bounds__(kRowThreads<NT>) void add_norm_kernel(const AddNorm
         c[j] = (j * NT + l) * V, in[j] = c[j] < a.D;
         load_weight_run<V>(w[j], a.w, a.w_f32, c[j], in[j]);
     }
+    const float inv_d = 1.f / float(a.D);
     for (int64_t row = int64_t(blockIdx.x) * kRows + threadIdx.x / NT; row < a.rows; row += int64_t(gridDim.x) * kRows) {
         const TIn* xp = static_cast<const TIn*>(a.x) + row * a.xs;
         const TIn* rp = static_cast<const TIn*>(a.residual) + row * a.rs;
@@ -195,13 +208,13 @@ __global__ __launch_bounds__(kRowThreads<NT>) void add_norm_kernel(const AddNorm
             }
             if (a.residual && in[j]) X::store(static_cast<TIn*>(a.sum) + row * a.D + c[j], s[j]);
         }
-        const float r = rsqrtf(reduce.sum(ss) / float(a.D) + a.eps);
+        const float r = rounded_rsqrt(mean_and_eps(reduce.sum(ss), inv_d, a.eps));
         uint32_t most = 0;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                s[j][i] *= r * w[j][i];
+                s[j][i] = s[j][i] * r * w[j][i];
                 if constexpr (kE4m3) most = max(most, in[j] ? magnitude(s[j][i]) : 0u);
             }
             if constexpr (!kE4m3) {
