@@ -586,7 +586,8 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
                     const float p = a.scale * e * P[i][r], hm = row > jc ? -e * H[i][r] : 0.f;
                     Lm[r] = bj * p;
                     Xm[r] = bj * hm;
-                    const float pair = fmaf(p, qk[r], hm * kk[r]);
+                    // A key stream may go on past this value stream, with any values.
+                    const float pair = row >= jc && row < live ? fmaf(p, qk[r], hm * kk[r]) : 0.f;
                     in_b += pair;
                     in_col += bj * pair;
                     const float in_row = row_scan(bj * pair);
@@ -648,6 +649,7 @@ __global__ __launch_bounds__(kGradThreads) void delta_grads_kernel(const DeltaBw
             }
 #pragma unroll
             for (int x = 0; x < 4 / TB; ++x) cols += col_sum[x * kChunk + lane], bs += b_sum[x * kChunk + lane];
+            if (lane >= live) z = 0.f, dg = 0.0;
             if (w.dbeta && lane < here) store_gate(w.dbeta, at, a.gate_f32, lane < live ? bs + z : 0.f);
             if (w.dgate) {
                 const float bz = beta[lane] * z;
