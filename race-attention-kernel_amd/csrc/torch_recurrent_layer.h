@@ -356,6 +356,20 @@ struct AddNormNode : torch::autograd::Function<AddNormNode> {
     }
 };
 
+// The residual stream's gradient; the rows in 8 bits and their scales have none.
+struct AddNormE4m3Node : torch::autograd::Function<AddNormE4m3Node> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual,
+                                 const c10::optional<at::Tensor>& weight, double eps, int64_t group) {
+        const auto [y, sum, scales] = add_norm_forward("race_add_norm_e4m3", x, residual, weight, eps, true, group);
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({y, *scales});
+        return {y, *scales, *sum};
+    }
+    static variable_list backward(AutogradContext*, variable_list up) {
+        return {up[2], up[2], at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
 struct GateNormNode : torch::autograd::Function<GateNormNode> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate,
                                  const c10::optional<at::Tensor>& weight, double eps) {
@@ -376,6 +390,12 @@ struct GateNormNode : torch::autograd::Function<GateNormNode> {
         return differentiated_once("race_gate_norm", up, {or_undefined(a), or_undefined(b), or_undefined(c), at::Tensor()});
     }
 };
+
+// For calls without derivatives.
+void refuse_tangents(const char* entry, std::initializer_list<c10::optional<at::Tensor>> inputs) {
+    for (const auto& t : inputs)
+        TORCH_CHECK(!t || !t->_fw_grad(0).defined(), entry, ": an input has a forward-mode tangent; the call has no jvp");
+}
 
 // Rows of any leading dimensions as [rows, D]: a view where one row stride
 // reaches them all, else a copy.
@@ -410,11 +430,14 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> add_norm(const at::Tensor& x_i
     return {y.view(x_in.sizes()), sum};
 }
 
-// (y in e4m3, scales, sum or None); no gradients.
+// (y in e4m3, scales, sum or None); gradients through sum alone.
 std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> add_norm_e4m3(
     const at::Tensor& x_in, const c10::optional<at::Tensor>& residual_in, const c10::optional<at::Tensor>& weight, double eps,
     int64_t group) {
     const char* entry = "race_add_norm_e4m3";
+    refuse_tangents(entry, {x_in, residual_in, weight});
+    const bool node = residual_in && wants_grad({x_in, residual_in});
+    if (node) check_capture(entry, {x_in, residual_in});
     if (residual_in)
         ArgCheck(entry).require(residual_in->sizes() == x_in.sizes(), "residual",
                                 [&] { return "has shape " + dims(*residual_in) + ", x " + dims(x_in); }).raise();
@@ -425,7 +448,14 @@ std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> add_norm_e4m3(
     const at::Tensor x = rows("x", x_in);
     c10::optional<at::Tensor> residual;
     if (residual_in) residual = rows("residual", *residual_in);
-    auto [y, sum, scales] = add_norm_forward(entry, x, residual, weight, eps, true, group);
+    at::Tensor y;
+    c10::optional<at::Tensor> sum, scales;
+    if (node) {
+        const variable_list outs = AddNormE4m3Node::apply(x, *residual, weight, eps, group);
+        y = outs[0], scales = outs[1], sum = outs[2];
+    } else {
+        std::tie(y, sum, scales) = add_norm_forward(entry, x, residual, weight, eps, true, group);
+    }
     if (x_in.dim() == 2) return {y, *scales, sum};
     std::vector<int64_t> per(x_in.sizes().begin(), x_in.sizes().end());
     per.back() = scales->size(1);
@@ -465,6 +495,7 @@ std::tuple<at::Tensor, at::Tensor> delta_rule_carry(const at::Tensor& q, const a
                                                     const c10::optional<at::Tensor>& gate, const at::Tensor& beta,
                                                     const at::Tensor& state, const c10::optional<at::Tensor>& lengths,
                                                     int64_t form, double scale, bool inplace) {
+    refuse_tangents("race_delta_rule_carry", {q, k, v, gate, beta, state});
     const auto r = delta_forward("race_delta_rule_carry", as_key_rows(q), as_key_rows(k), as_rows(v, kDeltaFar),
                                  as_per_token(gate), as_per_token(beta), state, as_lengths(lengths), form, scale, false, inplace);
     return {std::get<0>(r), std::get<1>(r)};

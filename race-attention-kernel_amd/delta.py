@@ -50,6 +50,6 @@ def race_delta_rule_carry(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gat
                           state: torch.Tensor, *, gate_form: str = "log", scale: float = 1.0,
                           lengths: torch.Tensor | None = None, inplace: bool = False):
     """(out, new_state): race_delta_rule continued from a carried state, without
-    autograd; with inplace=True the state tensor itself is advanced and returned.
+    autograd (its outputs require no gradients, whatever its inputs do); with inplace=True the state tensor itself is advanced and returned.
     Calls of at most 16 tokens (decode) run one small launch."""
     return _lib.ext().delta_rule_carry(q, k, v, gate, beta, state, lengths, _form_id(gate_form), scale, inplace)

@@ -35,8 +35,9 @@ def race_add_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight:
 
 def race_add_norm_e4m3(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, *,
                        eps: float = 1e-6, group: int = 0):
-    """(y8, scales, sum): race_add_norm with y in 8 bits, for an 8-bit projection;
-    no autograd.
+    """(y8, scales, sum): race_add_norm with y in 8 bits, for an 8-bit projection.
+    Gradients pass through sum, the residual stream, alone: y8 and scales have none,
+    so the weight and what lies behind them get none.
 
     y8 is float8_e4m3fn and y8 * scale stands for y: one float32 scale for each
     row (group 0, scales [..., 1]) or for each `group` of 32, 64 or 128 columns
