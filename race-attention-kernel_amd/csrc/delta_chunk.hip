@@ -629,7 +629,7 @@ hipError_t launch_by_width(const DeltaRule& r, const DeltaArgs& a, hipStream_t s
 }
 
 // Keys by pieces where only the values cannot be: 128 streams of 2048 bf16 tokens, 64 x 50,
-// forward and backward 471 -> 378 us, of fp32 ones, 128 x 17, 1460 -> 1304.
+// forward and backward 620 -> 526 us, of fp32 ones, 128 x 17, 1488 -> 1327.
 template <typename TIn>
 hipError_t launch_by_pieces(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
     if (!a.vec_k) return launch_by_width<TIn, false, false>(r, a, stream);
@@ -648,14 +648,14 @@ void launch_step(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
 }  // namespace
 
 // Chunks of a segment.  One walk has (dv + 63) / 64 workgroups a stream; a chunk takes
-// it about 3 us however few there are.  Split, every segment is walked twice, the
+// it about 4 us however few there are.  Split, every segment is walked twice, the
 // first time with dk columns more and without outputs, so a split pays where it
-// makes at least three segments (16 bf16 streams, 128 x 128, of 9 chunks in one 31 us, in
-// three 34; of 12 in one 40, in three 39); it aims for a workgroup a CU.
-// 16 streams of 32768 tokens, 128 x 128: one walk 1493 us; maps 246, join 25 and walks 247.
+// makes at least three segments (16 bf16 streams, 128 x 128, of 9 chunks in one 36 us, in
+// three 38; of 12 in one 47, in three 46); it aims for a workgroup a CU.
+// 16 streams of 32768 tokens, 128 x 128: one walk 1749 us; maps 329, join 28 and walks 298.
 // A segment has 4 chunks at least: the join takes a step a segment.  24 ragged fp32
 // streams of at most 24 chunks, 64 x 64, forward and backward, segments of 8 94 + 129
-// us, of 4 59 + 84, of 3 60 + 75; 16 bf16 ones of 24, 128 x 128, 58, 54, 57.
+// us, of 4 59 + 85, of 3 61 + 77; 16 bf16 ones of 24, 128 x 128, 68, 62, 63.
 int64_t delta_segment_chunks(const DeltaRule& r) {
     const int64_t chunks = delta_chunks(r), walks = r.N * ((r.dv + 63) / 64);
     const int64_t segs = std::min<int64_t>(walks > 0 ? 256 / walks : 1, chunks / 4);

@@ -419,8 +419,8 @@ struct Stage {
     int off[kVec ? kPer * kVecs : 1];
     int stride_, width_, at_;  // of the rows loaded
     // Wide rows compute the offsets of their values each time: kept, they take the registers that
-    // the products need (32 streams of 3000 fp32 tokens, 100 x 127: the walk 269 -> 185 us; 96
-    // of 1500 bf16 ones, 33 x 50: kept 97, again 112).
+    // the products need (32 streams of 3000 fp32 tokens, 100 x 127: the walk 213 -> 186 us; 96
+    // of 1500 bf16 ones, 33 x 50: kept 120, again 132).
     static constexpr bool kAgain = K * sizeof(TIn) > 128;
     __device__ __forceinline__ void init(int64_t stride, int width) {
         stride_ = int(stride), width_ = width;
@@ -631,8 +631,8 @@ struct StateView {
 
 // Whether two workgroups that walk chunks share a CU, each with one buffer, as narrow
 // keys' registers and tiles allow, and the maps' (no Q and M).  192 streams of 577
-// bf16 tokens, 64 x 128: the walk 43.5 -> 35.6 us; keys of 128 would spill (outputs of
-// 512 workgroups 356 us, of half as many that walk twice as far 247).
+// bf16 tokens, 64 x 128: the walk 52 -> 44 us; beside outputs, keys of 128 leave no LDS
+// for a second.
 constexpr bool two_a_cu(int row_bytes, bool maps) { return row_bytes <= (maps ? 256 : 128); }
 
 // A chunk's tiles in LDS (bytes from its buffer's start); T in three parts, M in MP.
@@ -746,7 +746,8 @@ __global__ __launch_bounds__(kThreads) void delta_join_kernel(const DeltaArgs a)
 
 inline int dk_padded(const DeltaRule& r) { return r.dk <= 64 ? 64 : 128; }
 
-// Whether a row is whole 16-byte pieces, and 64 rows of it lie within one buffer view.
+// Whether rows of this width and these strides are whole 16-byte pieces.  (That 64 of them
+// lie within a view's 32-bit offsets is the API's limit on token strides, 2^22.)
 inline bool whole_pieces(const DeltaRule& r, int64_t width, std::initializer_list<int64_t> strides) {
     const int v = r.dtype == RACE_BF16 ? 8 : 4;
     if (width % v != 0) return false;
