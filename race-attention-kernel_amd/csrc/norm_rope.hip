@@ -384,27 +384,8 @@ struct RopeSums {
     int d, w_f32;
 };
 __global__ __launch_bounds__(1024) void rope_weight_sums_kernel(const RopeSums a) {
-    __shared__ float sums[32][33];
     const int z = blockIdx.y;
-    void* dw = z ? a.dw[1] : a.dw[0];
-    const int cl = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-    const int rows = z ? a.rows[1] : a.rows[0], per = (rows + 31) / 32, from = run * per, to = min(rows, from + per);
-    const float* p = a.partial + int64_t(z ? a.rows[0] : 0) * a.d + c;
-    float s = 0.f;
-    if (c < a.d && dw) {
-#pragma unroll 8
-        for (int r = from; r < to; ++r) s += p[int64_t(r) * a.d];
-    }
-    sums[run][cl] = s;
-    __syncthreads();
-    if (run != 0 || c >= a.d || !dw) return;
-    float total = 0.f;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) total += sums[r][cl];
-    if (a.w_f32)
-        static_cast<float*>(dw)[c] = total;
-    else
-        static_cast<bf16_t*>(dw)[c] = f32_to_bf16(total);
+    column_sums(a.partial + int64_t(z ? a.rows[0] : 0) * a.d, z ? a.rows[1] : a.rows[0], a.d, z ? a.dw[1] : a.dw[0], a.w_f32);
 }
 
 int log2_up(int64_t x) {

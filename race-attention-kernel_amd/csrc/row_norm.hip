@@ -321,26 +321,8 @@ __global__ __launch_bounds__(kRowThreads<NT>) void add_norm_bwd_kernel(const Add
     }
 }
 
-// out[c] = the sum of partial[rows][d], 32 columns and 32 runs of rows a workgroup.
 __global__ __launch_bounds__(1024) void column_sums_kernel(const float* partial, int rows, int d, void* out, int f32) {
-    __shared__ float sums[32][33];
-    const int cl = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
-    const int per = (rows + 31) / 32, from = run * per, to = min(rows, from + per);
-    float s = 0.f;
-    if (c < d) {
-#pragma unroll 8
-        for (int r = from; r < to; ++r) s += partial[int64_t(r) * d + c];
-    }
-    sums[run][cl] = s;
-    __syncthreads();
-    if (run != 0 || c >= d) return;
-    float total = 0.f;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) total += sums[r][cl];
-    if (f32)
-        static_cast<float*>(out)[c] = total;
-    else
-        static_cast<bf16_t*>(out)[c] = f32_to_bf16(total);
+    column_sums(partial, rows, d, out, f32);
 }
 
 hipError_t launch_column_sums(const float* partial, int rows, int d, void* out, int f32, hipStream_t stream) {

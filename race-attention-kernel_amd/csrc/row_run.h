@@ -1,5 +1,5 @@
 // row_run.h -- runs of consecutive values of a row, loaded and stored as one
-// piece of up to 16 bytes.  Not part of the ABI.
+// piece of up to 16 bytes, and sums over rows.  Not part of the ABI.
 #pragma once
 
 #include "mfma_common.h"
@@ -50,5 +50,28 @@ struct Run {
             store_val(p, x[0]);
     }
 };
+
+// out[c] (nullable) = the sum of partial[rows][d] over its rows, in fp32 or bf16: a workgroup
+// of 1024 threads takes 32 columns in 32 runs of rows, in a fixed order.
+__device__ __forceinline__ void column_sums(const float* partial, int rows, int d, void* out, int f32) {
+    __shared__ float sums[32][33];
+    const int cl = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
+    const int per = (rows + 31) / 32, from = run * per, to = min(rows, from + per);
+    float s = 0.f;
+    if (c < d && out) {
+#pragma unroll 8
+        for (int r = from; r < to; ++r) s += partial[int64_t(r) * d + c];
+    }
+    sums[run][cl] = s;
+    __syncthreads();
+    if (run != 0 || c >= d || !out) return;
+    float total = 0.f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) total += sums[r][cl];
+    if (f32)
+        static_cast<float*>(out)[c] = total;
+    else
+        static_cast<bf16_t*>(out)[c] = f32_to_bf16(total);
+}
 
 }  // namespace race
