@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             operand(dS[2 * i], dS[2 * i + 1], odd, s[i]);
-            if constexpr (!kMaps) store_run(ds + 32 * i, dS[2 * i], dS[2 * i + 1], odd);
+            if constexpr (!kMaps) store_run(ds + 32 * i, dS[2 * i], dS[2 * i + 1], odd, s[i]);
         }
         stage_wall();
         fetch(next, 0);
@@ -246,7 +246,11 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
         float* dd = w.dd + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            if constexpr (!kMaps) store_run(dd + 32 * kk, x[2 * kk], x[2 * kk + 1], odd);
+            if constexpr (!kMaps) {
+                OneT<float> run;
+                operand(x[2 * kk], x[2 * kk + 1], odd, run);
+                store_run(dd + 32 * kk, run);
+            }
             operand(x[2 * kk] * -e[2 * kk], x[2 * kk + 1] * -e[2 * kk + 1], odd, d[kk]);
         }
         stage_wall();
@@ -751,7 +755,9 @@ hipError_t launch_backward(const DeltaRule& r, const DeltaBwdArgs& w, hipStream_
     if (err != hipSuccess) return err;
     if (!w.dq && !w.dk && !w.dv && !w.dgate && !w.dbeta) return hipSuccess;
     // Gradients that are all rounded to bf16 right away take two parts, those of fp32 gates three.
-    if (sizeof(TIn) == 2 && w.f.gate_f32) return launch_grads<TIn, DK, 3, kVec, kVecV>(r, w, stream);
+    if constexpr (sizeof(TIn) == 2) {
+        if (w.f.gate_f32) return launch_grads<TIn, DK, 3, kVec, kVecV>(r, w, stream);
+    }
     return launch_grads<TIn, DK, 2, kVec, kVecV>(r, w, stream);
 }
 

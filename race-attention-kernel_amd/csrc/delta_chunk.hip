@@ -348,7 +348,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         if constexpr (kMode == kRecording) {
             float* st = a.st + (nc * a.dvp + col) * DK + 8 * g;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) store_run(st + 32 * i, S[2 * i], S[2 * i + 1], odd);
+            for (int i = 0; i < NS; ++i) store_run(st + 32 * i, S[2 * i], S[2 * i + 1], odd, s[i]);
         }
         stage_wall();
         fetch(next, 0);
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, kMode == kMaps
         if constexpr (kMode == kRecording) {
             float* yt = a.yt + (nc * a.dvp + col) * kChunk + 8 * g;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, x[2 * kk], x[2 * kk + 1], odd);
+            for (int kk = 0; kk < 2; ++kk) store_run(yt + 32 * kk, x[2 * kk], x[2 * kk + 1], odd, y[kk]);
         }
         // S = e^{G_last} S + K^T (Z b Y).
         const float decay = E[63];
@@ -629,7 +629,7 @@ hipError_t launch_by_width(const DeltaRule& r, const DeltaArgs& a, hipStream_t s
 }
 
 // Keys by pieces where only the values cannot be: 128 streams of 2048 bf16 tokens, 64 x 50,
-// forward and backward 620 -> 526 us, of fp32 ones, 128 x 17, 1488 -> 1327.
+// forward and backward 620 -> 525 us, of fp32 ones, 128 x 17, 1480 -> 1307.
 template <typename TIn>
 hipError_t launch_by_pieces(const DeltaRule& r, const DeltaArgs& a, hipStream_t stream) {
     if (!a.vec_k) return launch_by_width<TIn, false, false>(r, a, stream);

@@ -132,11 +132,16 @@ __device__ __forceinline__ void store_run(float* p, const OneT<float>& x) {
     *reinterpret_cast<f32x4*>(p) = x.a;
     *reinterpret_cast<f32x4*>(p + 4) = x.b;
 }
-// A block pair's accumulators, as such a run.
-__device__ __forceinline__ void store_run(float* p, const f32x4& x0, const f32x4& x1, bool odd) {
-    OneT<float> x;
-    operand(x0, x1, odd, x);
-    store_run(p, x);
+// A block pair's accumulators as such a run; `x` is their operand (fp32: that run).
+template <int P>
+__device__ __forceinline__ void store_run(float* p, const f32x4& x0, const f32x4& x1, bool odd, const PartsT<bf16_t, P>&) {
+    OneT<float> run;
+    operand(x0, x1, odd, run);
+    store_run(p, run);
+}
+template <int P>
+__device__ __forceinline__ void store_run(float* p, const f32x4&, const f32x4&, bool, const PartsT<float, P>& x) {
+    store_run(p, first<1>(x));
 }
 
 // A wall the scheduler moves nothing across.  The walks have one wave a SIMD:
@@ -419,7 +424,7 @@ struct Stage {
     int off[kVec ? kPer * kVecs : 1];
     int stride_, width_, at_;  // of the rows loaded
     // Wide rows compute the offsets of their values each time: kept, they take the registers that
-    // the products need (32 streams of 3000 fp32 tokens, 100 x 127: the walk 213 -> 186 us; 96
+    // the products need (32 streams of 3000 fp32 tokens, 100 x 127: the walk 216 -> 173 us; 96
     // of 1500 bf16 ones, 33 x 50: kept 120, again 132).
     static constexpr bool kAgain = K * sizeof(TIn) > 128;
     __device__ __forceinline__ void init(int64_t stride, int width) {
