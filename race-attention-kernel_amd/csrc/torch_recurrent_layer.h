@@ -401,7 +401,7 @@ void refuse_tangents(const char* entry, std::initializer_list<c10::optional<at::
 // reaches them all, else a copy.
 at::Tensor as_matrix(const char* entry, const char* name, const at::Tensor& t) {
     ArgCheck(entry).require(t.dim() >= 1, name, "is a scalar; rows [..., D] are taken").raise();
-    return as_rows(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}));
+    return as_rows(t.dim() == 2 ? t : t.dim() == 1 ? t.unsqueeze(0) : t.flatten(0, -2));
 }
 
 // (y, sum or None); rows [..., D].
