@@ -25,8 +25,8 @@
 // launch is rounded to bf16 right away, in two.  (With S, Y, dS', dD, L and X rounded to
 // bf16 once each, the gradients were off by twice what their own rounding costs.)
 //
-// 128 streams of 4096 bf16 tokens, 128 x 128: the walk 382 us, bound as the forward's;
-// the gradients 705 us (three parts 845; rounded once 485), whose workgroups stay and load
+// 128 streams of 4096 bf16 tokens, 128 x 128: the walk 395 us, bound as the forward's;
+// the gradients 710 us (three parts 845; rounded once 485), whose workgroups stay and load
 // the next slice's rows meanwhile: a chunk's kept states come in slices of 32 value
 // columns, and its 64 x 64 matrices and sums between two barriers take half of the time.
 // Key streams that several value streams share sum their gradients in the registers of one
@@ -72,7 +72,8 @@ __global__ __launch_bounds__(kThreads, two_a_cu(sizeof(TIn) * DK, false) ? 2 : 1
     using One = OneT<TIn>;
     using Three = ThreeT<TIn>;
     constexpr int NS = DK / 32;
-    constexpr bool kLate = two_a_cu(sizeof(TIn) * DK, false);  // the reads of M, T and Q behind a product, for its registers: 78 -> 73 us of that
+    // M, T and Q are read behind a product, for its registers: 78 -> 73 us in the case above.
+    constexpr bool kLate = two_a_cu(sizeof(TIn) * DK, false);
     const int walks = kMaps ? a.segs - 1 : a.segs;  // no gradient goes on before the first segment
     int64_t ns;
     int cb;
